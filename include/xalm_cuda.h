@@ -280,6 +280,60 @@ int xalm_cuda_latent_window(float* out, const float* q, const float* cache, cons
 int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, const float* h, const float* w_router, const float* bias, const float* w_gate,
                          const float* w_up, const float* w_down, const float* base, int base_gated, int T, int K, int E, int top, int ff, int w_bf16);
 
+/* ---- batched serving over a paged cache: several sequences at once, DEVICE arrays in and out ---------------------------------------------------
+ * Keys and values of all sequences lie in one pool of pages; a table names each sequence's pages in their order.  Pools, tables and rows are the caller's
+ * device memory; the calls only enqueue kernels on the given stream (NULL: the legacy default stream) of the cache's device, whichever device is current, and
+ * keep nothing: calls on different streams, captured graphs among them, do not meet unless they are given the same workspace or write the same pages.
+ * Lengths and tables are read when the kernels run, so a captured graph serves every step of a batch whose arrays are rewritten in place.
+ *
+ * xalm_paged_cache: `type` is XALM_F32, XALM_F16 or XALM_BF16, of keys, values, mean keys and of the queries and results of the attending calls.  page_size 16, 32, 64,
+ *   128 or 256 slots; dim, vdim multiples of 8, at most 256.  Strides in ELEMENTS, entries of a head are neighbours: slots within heads or heads within slots, each stride a multiple
+ *   of 16 bytes; pools at 16-byte boundaries.  means (pages, kv_heads, dim), dense, or NULL: the mean of a page's keys, kept for every page whose last
+ *   slot was appended.  status: one int or NULL; kernels set bit 0 where a table named a page outside the pool (such a page reads as zeros and is not written) and bit 1
+ *   where starts, lens and the table do not fit one another (lengths are cut to the table); nothing else reports what is only known on the device.
+ * xalm_paged_batch: rows starts[s] .. starts[s + 1] - 1 are the new tokens of sequence s, lens[s] its tokens, the new ones included: row starts[s] + i is at position
+ *   lens[s] - n + i.  starts has seqs + 1 entries; rows outside [starts[0], starts[seqs]) of `rows` are left alone.  table (seqs, max_pages), rows table_row apart.
+ *   Sequences group_bounds[i] .. group_bounds[i + 1] - 1 (ascending) have the same pages for their first group_shared[i] tokens: those are read once for all of
+ *   them; what a call computes does not depend on it.  At most 4096 sequences and groups.
+ * Rows of arrays are `*_row` elements apart and begin at 16-byte boundaries; heads within a row are dense.
+ *
+ * paged_append: k (rows, kv_heads dim), v (rows, kv_heads vdim), q (rows, heads dim) of in_type; the first 2 rot_half entries of every head of k and q are turned by
+ *   position * freq[i] (entry i with i + rot_half, or with `neighbours` 2 i with 2 i + 1; cos and sin times rot_mag); keys and values go to their pages, queries to q_out
+ *   in the cache's type, rounded once.  q NULL: keys and values only.  Then the mean keys of the pages that are full now.
+ * paged_attend: out[row, h] = sum_j softmax_j(scale q . k_j) v_j over the positions j up to the row's own; rows that see nothing give zeros.  lse (rows, heads): the logarithm of the
+ *   softmax's denominator (-infinity where a row sees nothing), or NULL.
+ * paged_select: for every row and kv head `top` pages by their place in the sequence, ascending, -1 behind them: the row's own page, the `recent` before it, the `first`
+ *   of the sequence, and of the others those with the largest score = (sum of the kv head's queries) . mean key, equal scores from the lowest place on; NaN and -infinity count as the lowest
+ *   finite number, +infinity as the largest.  out (rows, kv_heads, top).
+ * paged_attend_selected: paged_attend over the listed pages only (rows, kv_heads, n_lists <= 1024), in any order; entries outside 0 .. the row's own page are passed
+ *   over, a page counts once.
+ * paged_workspace: bytes of workspace (at a 256-byte boundary) that paged_attend (n_lists 0) and paged_attend_selected need for these sizes; its contents need no preparation. */
+typedef struct xalm_paged_cache {
+	int type, device;
+	int pages, page_size, kv_heads, dim, vdim;
+	void *k, *v;
+	long long k_page, k_slot, k_head;
+	long long v_page, v_slot, v_head;
+	void* means;
+	int* status;
+} xalm_paged_cache;
+typedef struct xalm_paged_batch {
+	int rows, seqs, max_pages, groups;
+	const int *starts, *lens, *table;
+	long long table_row;
+	const int *group_bounds, *group_shared;
+} xalm_paged_batch;
+int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch* batch, const void* k, long long k_row, const void* v, long long v_row, const void* q,
+                           long long q_row, int heads, int in_type, void* q_out, long long q_out_row, const float* freq, int rot_half, float rot_mag, int neighbours,
+                           void* cuda_stream);
+int xalm_cuda_paged_attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, float scale, void* out,
+                           long long out_row, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream);
+int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, int top, int first, int recent,
+                           int* out, void* cuda_stream);
+int xalm_cuda_paged_attend_selected(const xalm_paged_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, const int* lists,
+                                    int n_lists, float scale, void* out, long long out_row, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream);
+int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_batch* batch, int heads, int n_lists, size_t* bytes);
+
 /* Tensor parallel plumbing (no reference analogue).  Rank 0 makes an id, the host side ships it to
  * the other ranks (torch.distributed / MPI / a file), every rank calls comm_init before finalize. */
 #define XALM_COMM_ID_BYTES 128

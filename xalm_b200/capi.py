@@ -120,6 +120,11 @@ SYMBOLS = {
     "xalm_cuda_latent_window": (_i, [_vp] * 4 + [_i] * 6 + [_vp, _vp, C.c_float, _i, _i, _i, _i]),
     "xalm_cuda_moe_chosen": (_i, [_vp] * 11 + [_i] * 7),
     "xalm_cuda_rows_add": (_i, [_vp] * 4 + [_i] * 3),
+    "xalm_cuda_paged_append": (_i, [_vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong, _i, _i, _vp, C.c_longlong, _vp, _i, C.c_float, _i, _vp]),
+    "xalm_cuda_paged_attend": (_i, [_vp, _vp, _vp, C.c_longlong, _i, C.c_float, _vp, C.c_longlong, _vp, _vp, _sz, _vp]),
+    "xalm_cuda_paged_select": (_i, [_vp, _vp, _vp, C.c_longlong, _i, _i, _i, _i, _vp, _vp]),
+    "xalm_cuda_paged_attend_selected": (_i, [_vp, _vp, _vp, C.c_longlong, _i, _vp, _i, C.c_float, _vp, C.c_longlong, _vp, _vp, _sz, _vp]),
+    "xalm_cuda_paged_workspace": (_i, [_vp, _vp, _i, _i, C.POINTER(_sz)]),
 }
 PRECISION_BF16, PRECISION_F32 = 0, 1            # enum xalm_precision
 

@@ -1,0 +1,438 @@
+// paged.cuh — what the kernels of the paged cache (xalm_cuda_paged_*) share: the cache and the batch as they see them, and the plan by which attention's
+// CTAs divide their work.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace xalm {
+namespace paged {
+
+constexpr int KT = 64;              // keys of a tile, the unit in which attention counts its work
+constexpr int MAX_SEGMENTS = 4096;  // sequences and groups of one call: the plan lies in shared memory
+constexpr int MAX_LIST = 1024;      // pages that a list of attend_selected names
+constexpr int ERR_PAGE = 1, ERR_BATCH = 2; // bits of the cache's status word
+
+struct Cache {
+	uint8_t *k, *v, *means;
+	long long k_page, k_slot, k_head, v_page, v_slot, v_head; // elements
+	int pages, shift, G, d, dv;                               // page size 1 << shift
+	int* status;
+};
+struct BatchView {
+	int N, B, max_pages, n_groups;
+	const int *starts, *lens, *table;
+	long long table_row;
+	const int *bounds, *shared;
+};
+
+__device__ __forceinline__ void report(const Cache& c, int bit) {
+	if (c.status) atomicOr(c.status, bit);
+}
+
+// A sequence's rows [a, a + n) and its length.  Whatever the arrays hold, rows lie in [0, N) and positions in the table.
+struct Seq {
+	int a, n, len;
+};
+__device__ __forceinline__ int capacity(const Cache& c, const BatchView& b) { return (int) min((long long) b.max_pages << c.shift, 0x7fffffffll); }
+__device__ __forceinline__ Seq seq_of(const Cache& c, const BatchView& b, int s) {
+	Seq q;
+	q.a = min(max(b.starts[s], 0), b.N);
+	q.n = min(max(b.starts[s + 1], q.a), b.N) - q.a;
+	q.len = min(max(b.lens[s], 0), capacity(c, b));
+	return q;
+}
+__device__ __forceinline__ bool seq_ok(const Cache& c, const BatchView& b, int s) {
+	const int a = b.starts[s], e = b.starts[s + 1], l = b.lens[s];
+	return a >= 0 && e >= a && e <= b.N && l >= e - a && l <= capacity(c, b);
+}
+// The sequence of a row: the last s with starts[s] <= row.  A whole warp asks, with 32 probes a round.
+__device__ __forceinline__ int seq_of_row(const BatchView& b, int row) {
+	const int lane = threadIdx.x & 31;
+	int lo = 0, n = b.B; // the answer lies in [lo, lo + n)
+	while (n > 1) {
+		const int step = (n + 31) / 32, at = lane * step;
+		const unsigned m = __ballot_sync(0xffffffffu, at < n && b.starts[lo + at] <= row);
+		const int k = m ? 31 - __clz(m) : 0;
+		lo += k * step;
+		n = min(step, n - k * step);
+	}
+	return lo;
+}
+// Page of the pool that holds page j of a sequence; -1 when the table names none there
+__device__ __forceinline__ int page_of(const Cache& c, const BatchView& b, int s, int j) {
+	const int p = b.table[(long long) s * b.table_row + j];
+	return p >= 0 && p < c.pages ? p : -1;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+// eight neighbouring elements at a 16-byte boundary
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+	if constexpr (sizeof(T) == 4) {
+		const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+		x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+	} else {
+		const uint4 u = *reinterpret_cast<const uint4*>(p);
+		const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+		for (int i = 0; i < 8; i++) x[i] = to_f(t[i]);
+	}
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+	if constexpr (sizeof(T) == 4) {
+		reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+		reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+	} else {
+		uint4 u;
+		T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+		for (int i = 0; i < 8; i++) t[i] = from_f<T>(x[i]);
+		*reinterpret_cast<uint4*>(p) = u;
+	}
+}
+
+// ---- attention's work --------------------------------------------------------------------------------------------------------------------
+// A segment is a run of keys that the same rows read: a group's shared pages (segment i < n_groups: the rows of all its sequences, every row sees every
+// key) or a sequence's pages behind them (segment n_groups + s: its own rows, causal).  Rows are (token, query head of the kv head) pairs, `rep` to a token.
+// A segment's unit is one kv head and M of its rows; a unit's work is its tiles of KT keys.  The tiles of all units, laid end to end, are cut into as many equal
+// parts as there are CTAs, whatever the sequences' lengths: a CTA walks its part, and writes, for each unit that it meets, a partial result into slot
+// (unit + CTA) — both numbers only grow along the walk, so no two pieces share a slot.  A unit that one CTA holds whole, and whose rows read no other
+// segment, goes straight to the output; paged_join_kernel joins the rest.
+struct Part {
+	float* o;            // (slots, M, dv): sums of exp(s - m) v
+	float2* ml;          // (slots, M): m (in units of log2), sum of exp
+	int slots, M, grid;
+	int small_rows;      // own segments of at most this many rows belong to this part when `small`, the others when `big`
+	int small, big, prefix;
+	long long* cum_w;    // the plan, left by CTA 0 for the join: tiles and units before each segment, keys shared by each sequence
+	int *cum_u, *shs;
+};
+struct Attn {
+	Cache c;
+	BatchView b;
+	const uint8_t* q;
+	uint8_t* out;
+	long long q_row, out_row; // elements
+	float* lse;
+	int H, rep;
+	float scale;
+	const int* lists;         // (N, G, S): pages by their place in the sequence; NULL: all
+	int S;
+	int n_parts;
+	Part part[2];
+};
+struct Plan {
+	long long* cum_w; // segments + 1
+	int *cum_u, *shs;
+	int segs;
+	long long total;
+};
+__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (B + n_groups + 1) * 12 + (size_t) B * 4 + 32 * 12 + 16; }
+
+// rows of a segment and the tiles of its unit t
+__device__ __forceinline__ int seg_rows(const Attn& a, int seg, int& row0, int& s_first) {
+	if (seg < a.b.n_groups) {
+		const int s0 = min(max(a.b.bounds[seg], 0), a.b.B), s1 = min(max(a.b.bounds[seg + 1], s0), a.b.B);
+		s_first = s0;
+		if (s0 == s1) { row0 = 0; return 0; }
+		row0 = seq_of(a.c, a.b, s0).a;
+		const Seq l = seq_of(a.c, a.b, s1 - 1);
+		return max(l.a + l.n - row0, 0) * a.rep;
+	}
+	s_first = seg - a.b.n_groups;
+	const Seq q = seq_of(a.c, a.b, s_first);
+	row0 = q.a;
+	return q.n * a.rep;
+}
+// keys of an own segment that the rows up to `last` of it see
+__device__ __forceinline__ int own_keys(const Seq& q, int shared, int rep, int last) { return max(q.len - q.n + last / rep + 1 - shared, 0); }
+
+__device__ __forceinline__ bool in_part(const Part& p, bool prefix, int rows) { return prefix ? p.prefix : rows <= p.small_rows ? p.small : p.big; }
+
+// tiles of unit t of a segment
+__device__ __forceinline__ int unit_tiles(const Attn& a, const Part& part, int seg, int rows, const Seq& q, int shared, int t) {
+	if (seg < a.b.n_groups) return (shared + KT - 1) / KT;
+	return (own_keys(q, shared, a.rep, min((t + 1) * part.M, rows) - 1) + KT - 1) / KT;
+}
+
+// All threads of the CTA.  Shared keys of each group (whole pages, and no more than every row of its sequences sees; a group of one sequence has none),
+// then a running sum over the segments.
+template <int NT>
+__device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& p) {
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.B, n = a.b.n_groups;
+	p.segs = n + B;
+	p.cum_w = reinterpret_cast<long long*>(smem);
+	long long* sum_w = p.cum_w + p.segs + 1;
+	p.cum_u = reinterpret_cast<int*>(sum_w + 32);
+	int* sum_u = p.cum_u + p.segs + 1;
+	p.shs = sum_u + 32;
+	for (int s = tid; s < B; s += NT) p.shs[s] = 0;
+	__syncthreads();
+	for (int i = warp; i < n; i += NT / 32) {
+		const int s0 = min(max(a.b.bounds[i], 0), B), s1 = min(max(a.b.bounds[i + 1], s0), B);
+		if (s1 - s0 < 2) continue;
+		int m = max(a.b.shared[i], 0);
+		for (int s = s0 + lane; s < s1; s += 32) {
+			const Seq q = seq_of(a.c, a.b, s);
+			m = min(m, max(q.len - q.n, 0));
+		}
+		m = __reduce_min_sync(0xffffffffu, m) >> a.c.shift << a.c.shift;
+		for (int s = s0 + lane; s < s1; s += 32) p.shs[s] = m;
+	}
+	__syncthreads();
+	long long carry_w = 0;
+	int carry_u = 0;
+	if (tid == 0) { p.cum_w[0] = 0; p.cum_u[0] = 0; }
+	for (int base = 0; base < p.segs; base += NT) {
+		const int seg = base + tid;
+		long long w = 0;
+		int u = 0, in_seg = 0;
+		bool wide = false; // own rows of many tiles: their sum is the whole warp's
+		if (seg < p.segs) {
+			int row0, s;
+			const int rows = seg_rows(a, seg, row0, s), tiles = (rows + part.M - 1) / part.M;
+			if (in_part(part, seg < n, rows) && rows) {
+				if (seg < n) w = (long long) tiles * ((p.shs[s] + KT - 1) / KT);
+				else {
+					const Seq q = seq_of(a.c, a.b, s);
+					if (tiles <= 4) {
+						for (int t = 0; t < tiles; t++) w += unit_tiles(a, part, seg, rows, q, p.shs[s], t);
+					} else wide = true;
+					if (part.cum_w && blockIdx.x == 0 && !seq_ok(a.c, a.b, s)) report(a.c, ERR_BATCH);
+				}
+				in_seg = tiles;
+			}
+		}
+		for (unsigned m = __ballot_sync(0xffffffffu, wide); m; m &= m - 1) {
+			const int from = __ffs(m) - 1, wseg = base + (tid & ~31) + from, n_tiles = __shfl_sync(0xffffffffu, in_seg, from);
+			const Seq q = seq_of(a.c, a.b, wseg - n);
+			long long sum = 0;
+			for (int t = lane; t < n_tiles; t += 32) sum += unit_tiles(a, part, wseg, q.n * a.rep, q, p.shs[wseg - n], t);
+#pragma unroll
+			for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+			if (lane == from) w = sum;
+		}
+		w *= a.c.G;
+		u = w ? in_seg * a.c.G : 0;
+#pragma unroll
+		for (int o = 1; o < 32; o <<= 1) {
+			const long long x = __shfl_up_sync(0xffffffffu, w, o);
+			const int y = __shfl_up_sync(0xffffffffu, u, o);
+			if (lane >= o) { w += x; u += y; }
+		}
+		if (lane == 31) { sum_w[warp] = w; sum_u[warp] = u; }
+		__syncthreads();
+		long long bw = carry_w;
+		int bu = carry_u;
+		for (int i = 0; i < warp; i++) { bw += sum_w[i]; bu += sum_u[i]; }
+		if (seg < p.segs) { p.cum_w[seg + 1] = bw + w; p.cum_u[seg + 1] = bu + u; }
+		for (int i = 0; i < NT / 32; i++) { carry_w += sum_w[i]; carry_u += sum_u[i]; }
+		__syncthreads();
+	}
+	p.total = p.cum_w[p.segs];
+	if (part.cum_w && blockIdx.x == 0) {
+		for (int i = tid; i <= p.segs; i += NT) { part.cum_w[i] = p.cum_w[i]; part.cum_u[i] = p.cum_u[i]; }
+		for (int i = tid; i < B; i += NT) part.shs[i] = p.shs[i];
+	}
+}
+
+// First tile of a CTA's share.  Fewer tiles than CTAs: one to each of the first CTAs, so that no share between two others is empty.
+__device__ __forceinline__ int shares(long long total, int grid) { return (int) min(total, (long long) grid); }
+__device__ __forceinline__ long long part_begin(long long total, int grid, int cta) {
+	const int n = shares(total, grid);
+	return cta >= n ? total : total * cta / n;
+}
+
+// One unit of a CTA's walk, with what both its producer and its consumers need to know of it
+struct Piece {
+	int seg, g, t, u;    // segment, kv head, rows [M t, M (t + 1)) of the segment, number among all units
+	int j0, j1;          // tiles of the unit that are this CTA's
+	int w;               // all tiles of the unit
+	int row0, rows;      // first token row of the segment, (token, head) rows of the segment
+	int s;               // whose table row holds the pages (SELECTED: the sequence)
+	int key0;            // position of the segment's first key
+	Seq q;
+};
+// The walk over a CTA's part of the tiles
+struct Walk {
+	long long at, end;   // tiles
+	Piece x;
+	int tiles;           // row tiles of the segment
+};
+__device__ __forceinline__ void walk_segment(const Attn& a, const Part& part, const Plan& p, Walk& k) {
+	k.x.rows = seg_rows(a, k.x.seg, k.x.row0, k.x.s);
+	k.tiles = (k.x.rows + part.M - 1) / part.M;
+	k.x.q = seq_of(a.c, a.b, k.x.s);
+	k.x.key0 = k.x.seg < a.b.n_groups ? 0 : p.shs[k.x.s];
+}
+__device__ __forceinline__ int walk_tiles(const Attn& a, const Part& part, const Plan& p, const Walk& k) {
+	return unit_tiles(a, part, k.x.seg, k.x.rows, k.x.q, p.shs[k.x.s], k.x.t);
+}
+// false: nothing for this CTA
+__device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, const Plan& p, Walk& k) {
+	k.at = part_begin(p.total, part.grid, blockIdx.x);
+	k.end = part_begin(p.total, part.grid, blockIdx.x + 1);
+	if (k.at >= k.end) return false;
+	int lo = 0, hi = p.segs - 1; // the last segment that begins at or before k.at and is not empty
+	while (lo < hi) {
+		const int mid = (lo + hi + 1) >> 1;
+		if (p.cum_w[mid] <= k.at) lo = mid;
+		else hi = mid - 1;
+	}
+	k.x.seg = lo;
+	walk_segment(a, part, p, k);
+	long long rem = k.at - p.cum_w[lo];
+	const long long per = (p.cum_w[lo + 1] - p.cum_w[lo]) / a.c.G;
+	k.x.g = (int) (rem / per);
+	rem -= per * k.x.g;
+	const int lane = threadIdx.x & 31;
+	for (int t0 = 0;; t0 += 32) { // whole warps walk: 32 units' tiles at a time
+		const int w = t0 + lane < k.tiles ? unit_tiles(a, part, lo, k.x.rows, k.x.q, p.shs[k.x.s], t0 + lane) : 0;
+		long long sum = w;
+#pragma unroll
+		for (int o = 1; o < 32; o <<= 1) {
+			const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+			if (lane >= o) sum += x;
+		}
+		const unsigned m = __ballot_sync(0xffffffffu, sum > rem);
+		if (m || t0 + 32 >= k.tiles) {
+			const int at = m ? __ffs(m) - 1 : 0;
+			k.x.t = t0 + at;
+			k.x.w = __shfl_sync(0xffffffffu, w, at);
+			rem -= __shfl_sync(0xffffffffu, sum, at) - k.x.w;
+			break;
+		}
+		rem -= __shfl_sync(0xffffffffu, sum, 31);
+	}
+	k.x.j0 = (int) rem;
+	k.x.j1 = (int) min((long long) k.x.w, rem + (k.end - k.at));
+	k.x.u = p.cum_u[lo] + k.x.g * k.tiles + k.x.t;
+	return true;
+}
+__device__ __forceinline__ bool walk_next(const Attn& a, const Part& part, const Plan& p, Walk& k) {
+	k.at += k.x.j1 - k.x.j0;
+	if (k.at >= k.end) return false;
+	do {
+		if (++k.x.t == k.tiles) {
+			k.x.t = 0;
+			if (++k.x.g == a.c.G) {
+				k.x.g = 0;
+				do k.x.seg++;
+				while (p.cum_w[k.x.seg + 1] == p.cum_w[k.x.seg]); // ends: k.at < k.end <= total
+				walk_segment(a, part, p, k);
+			}
+		}
+		k.x.w = walk_tiles(a, part, p, k);
+	} while (k.x.w == 0);
+	k.x.j0 = 0;
+	k.x.j1 = (int) min((long long) k.x.w, k.end - k.at);
+	k.x.u = p.cum_u[k.x.seg] + k.x.g * k.tiles + k.x.t;
+	return true;
+}
+// SELECTED: units are (row, kv head, M of its query heads), every one of `w` tiles
+__device__ __forceinline__ int list_tiles(const Attn& a) { return (int) ((((long long) a.S << a.c.shift) + KT - 1) / KT); }
+__device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk& k, long long unit) {
+	const int tiles = (a.rep + part.M - 1) / part.M;
+	k.x.u = (int) unit;
+	k.x.t = (int) (unit % tiles);
+	k.x.g = (int) (unit / tiles % a.c.G);
+	k.x.row0 = (int) (unit / tiles / a.c.G);
+	k.x.rows = a.rep;
+	k.x.seg = 0;
+	k.x.key0 = 0;
+	k.x.w = list_tiles(a);
+	k.x.s = seq_of_row(a.b, k.x.row0); // whole warps walk
+	k.x.q = seq_of(a.c, a.b, k.x.s);
+}
+__device__ __forceinline__ long long list_total(const Attn& a, const Part& part) {
+	return (long long) a.b.N * a.c.G * ((a.rep + part.M - 1) / part.M) * list_tiles(a);
+}
+__device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk& k) {
+	const long long total = list_total(a, part);
+	k.at = part_begin(total, part.grid, blockIdx.x);
+	k.end = part_begin(total, part.grid, blockIdx.x + 1);
+	if (k.at >= k.end) return false;
+	const int w = list_tiles(a);
+	list_unit(a, part, k, k.at / w);
+	k.x.j0 = (int) (k.at % w);
+	k.x.j1 = (int) min((long long) w, k.x.j0 + (k.end - k.at));
+	return true;
+}
+__device__ __forceinline__ bool list_next(const Attn& a, const Part& part, Walk& k) {
+	k.at += k.x.j1 - k.x.j0;
+	if (k.at >= k.end) return false;
+	list_unit(a, part, k, k.x.u + 1);
+	k.x.j0 = 0;
+	k.x.j1 = (int) min((long long) k.x.w, k.end - k.at);
+	return true;
+}
+__device__ __forceinline__ bool row_in_seq(const Seq& q, int row) { return row >= q.a && row < q.a + q.n; }
+
+// The list of (row, kv head), by a whole warp: pages that the row sees, each once, in ascending order, into `pages` (NULL: counted only).  Lists that come
+// so, with -1 behind, cost one pass; any other order, and pages named twice, cost a pass over the list for every page.  *own: whether the row's own page is among them.
+__device__ __forceinline__ int list_pages(const Attn& a, int row, int g, int own_page, int* pages, bool* own) {
+	const int lane = threadIdx.x & 31;
+	const int* l = a.lists + ((long long) row * a.c.G + g) * a.S;
+	const int most = min(own_page, a.b.max_pages - 1);
+	int n = 0, before = -1;
+	bool tidy = true, gap = false;
+	*own = false;
+	for (int i = 0; i < a.S; i += 32) {
+		const int e = i + lane < a.S ? l[i + lane] : -1;
+		const bool ok = e >= 0 && e <= most;
+		const unsigned m = __ballot_sync(0xffffffffu, ok);
+		int prev = __shfl_up_sync(0xffffffffu, e, 1);
+		if (lane == 0) prev = before;
+		tidy = tidy && (m & (m + 1)) == 0 && !(gap && m) && __all_sync(0xffffffffu, !ok || e > prev);
+		gap = gap || m != 0xffffffffu;
+		before = __shfl_sync(0xffffffffu, e, 31);
+		if (pages && ok) pages[n + __popc(m & ((1u << lane) - 1))] = e;
+		n += __popc(m);
+		*own = *own || __any_sync(0xffffffffu, ok && e == own_page);
+	}
+	if (tidy) {
+		__syncwarp();
+		return n;
+	}
+	n = 0;
+	for (int last = -1;;) { // the next larger entry, until there is none
+		int m = 0x7fffffff;
+		for (int i = lane; i < a.S; i += 32) {
+			const int e = l[i];
+			if (e > last && e <= most) m = min(m, e);
+		}
+		m = __reduce_min_sync(0xffffffffu, m);
+		if (m == 0x7fffffff) break;
+		if (pages && lane == 0) pages[n] = m;
+		n++;
+		last = m;
+	}
+	__syncwarp();
+	return n;
+}
+
+int launch_join(const Attn& a, int type, cudaStream_t s);
+int launch_attn_rows(const Attn& a, int type, cudaStream_t s);
+
+} // namespace paged
+} // namespace xalm

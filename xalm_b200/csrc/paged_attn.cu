@@ -1,0 +1,351 @@
+// paged_attn.cu — attention over the paged cache: rows of fp32 caches by fp32 FMAs, and the join of what several CTAs have of the same rows.
+#include "paged.cuh"
+
+namespace xalm {
+namespace paged {
+
+// =========================================================================================================================================
+// Attention by fp32 FMAs: 16 (token, head) rows of one kv head at a time, 32 keys at a time in shared memory as fp32, one running maximum and
+// sum per row.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s = scale q.k; kept in log2 units: exp2((q.k - m') scale log2 e).
+// =========================================================================================================================================
+constexpr int RM = 16, RK = 32, RT = 128;
+
+template <typename T, int NC, bool LIST> // NC columns of V per thread
+__global__ void __launch_bounds__(RT) paged_rows_kernel(const Attn a) {
+	extern __shared__ __align__(16) uint8_t smem[];
+	const Part& part = a.part[0];
+	const int d = a.c.d, dv = a.c.dv, kp = d + 4, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	float* sq = reinterpret_cast<float*>(smem);  // [RM][d]
+	float* sk = sq + RM * d;                      // [RK][d + 4]
+	float* sv = sk + RK * kp;                     // [RK][dv]
+	float* sp = sv + RK * dv;                     // [RM][RK]
+	float* s_corr = sp + RM * RK;                 // [RM] factor of what a row has so far, then its sum
+	int* s_lim = reinterpret_cast<int*>(s_corr + 2 * RM); // [RM] keys that a row sees
+	int* s_page = s_lim + RM;                     // [RK]
+	int* s_list = s_page + RK;                    // [S]
+	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list + ((LIST ? a.S : 0) + 1) / 2 * 2);
+	Plan plan;
+	pdl_wait();
+	pdl_launch_dependents();
+	if (!LIST) make_plan<RT>(a, part, s_plan, plan);
+	Walk k;
+	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
+	const long long total = LIST ? list_total(a, part) : plan.total;
+	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
+		const Piece& x = k.x;
+		__syncthreads();
+		int pos = 0, listed = 0;
+		if (LIST) {
+			if (!row_in_seq(x.q, x.row0)) continue; // the same for every thread
+			pos = x.q.len - x.q.n + x.row0 - x.q.a;
+			bool own;
+			const int n = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, warp == 0 ? s_list : nullptr, &own);
+			listed = own ? ((n - 1) << a.c.shift) + (pos & ((1 << a.c.shift) - 1)) + 1 : n << a.c.shift;
+		}
+		const int shared = LIST ? 0 : plan.shs[x.s];
+		const bool prefix = !LIST && x.seg < a.b.n_groups;
+		const int rows = min(RM, x.rows - x.t * RM);
+		const int h0 = x.g * a.rep;
+		for (int i = tid; i < RM * (d / 8); i += RT) {
+			const int r = i / (d / 8), c = i % (d / 8) * 8;
+			float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+			if (r < rows) {
+				const int w = x.t * RM + r;
+				load8(reinterpret_cast<const T*>(a.q) + (long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * d + c, v);
+			}
+#pragma unroll
+			for (int e = 0; e < 8; e++) sq[r * d + c + e] = v[e];
+		}
+		if (tid < RM) s_lim[tid] = tid >= rows ? 0 : LIST ? listed : prefix ? shared : own_keys(x.q, shared, a.rep, x.t * RM + tid);
+		__syncthreads();
+		const int first = x.j0 * KT, last = min(x.j1 * KT, s_lim[rows - 1]); // the last row sees the most
+		float m[4], l[4], acc[RM][NC];
+#pragma unroll
+		for (int r = 0; r < 4; r++) { m[r] = -INFINITY; l[r] = 0.f; }
+#pragma unroll
+		for (int r = 0; r < RM; r++)
+#pragma unroll
+			for (int c = 0; c < NC; c++) acc[r][c] = 0.f;
+		const float c1 = a.scale * 1.4426950408889634f;
+		for (int kb = first; kb < last; kb += RK) {
+			const int n_keys = min(RK, last - kb);
+			if (tid < RK) {
+				const int key = x.key0 + kb + tid;
+				int pg = -1;
+				if (tid < n_keys) {
+					pg = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
+					if (pg < 0) report(a.c, ERR_PAGE);
+				}
+				s_page[tid] = pg;
+			}
+			__syncthreads();
+			for (int i = tid; i < RK * (d / 8); i += RT) {
+				const int r = i / (d / 8), c = i % (d / 8) * 8, pg = s_page[r];
+				float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+				if (pg >= 0)
+					load8(reinterpret_cast<const T*>(a.c.k) + pg * a.c.k_page + ((x.key0 + kb + r) & ((1 << a.c.shift) - 1)) * a.c.k_slot + x.g * a.c.k_head + c, v);
+				reinterpret_cast<float4*>(sk + r * kp + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+				reinterpret_cast<float4*>(sk + r * kp + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+			}
+			for (int i = tid; i < RK * (dv / 8); i += RT) {
+				const int r = i / (dv / 8), c = i % (dv / 8) * 8, pg = s_page[r];
+				float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+				if (pg >= 0)
+					load8(reinterpret_cast<const T*>(a.c.v) + pg * a.c.v_page + ((x.key0 + kb + r) & ((1 << a.c.shift) - 1)) * a.c.v_slot + x.g * a.c.v_head + c, v);
+				reinterpret_cast<float4*>(sv + r * dv + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+				reinterpret_cast<float4*>(sv + r * dv + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+			}
+			__syncthreads();
+			float s[4] = {0.f, 0.f, 0.f, 0.f};
+			for (int c = 0; c < d; c += 4) { // lane = key, four rows to a warp
+				const float4 kk = *reinterpret_cast<const float4*>(sk + lane * kp + c);
+#pragma unroll
+				for (int r = 0; r < 4; r++) {
+					const float4 qq = *reinterpret_cast<const float4*>(sq + (warp * 4 + r) * d + c);
+					s[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[r]))));
+				}
+			}
+#pragma unroll
+			for (int r = 0; r < 4; r++) {
+				const float sc = kb + lane < s_lim[warp * 4 + r] ? s[r] * c1 : -INFINITY;
+				const float mt = fmaxf(m[r], warp_max(sc)), base = mt == -INFINITY ? 0.f : mt;
+				const float p = exp2f(sc - base), corr = exp2f(m[r] - base);
+				l[r] = l[r] * corr + warp_sum(p);
+				m[r] = mt;
+				sp[(warp * 4 + r) * RK + lane] = p;
+				if (lane == 0) s_corr[warp * 4 + r] = corr;
+			}
+			__syncthreads();
+			const bool all = kb + n_keys <= s_lim[0]; // every row sees every key of this tile (rows that are not there see none, and are not written)
+#pragma unroll
+			for (int c = 0; c < NC; c++) {
+				const int col = tid + c * RT;
+				if (col >= dv) break;
+#pragma unroll
+				for (int r = 0; r < RM; r++) acc[r][c] *= s_corr[r];
+				if (all) {
+					for (int j = 0; j < n_keys; j++) {
+						const float v = sv[j * dv + col];
+#pragma unroll
+						for (int r = 0; r < RM; r++) acc[r][c] = fmaf(sp[r * RK + j], v, acc[r][c]);
+					}
+				} else { // what a row does not see may be anything, an infinity or a NaN too
+					for (int j = 0; j < n_keys; j++) {
+						const float v = sv[j * dv + col];
+#pragma unroll
+						for (int r = 0; r < RM; r++)
+							if (kb + j < s_lim[r]) acc[r][c] = fmaf(sp[r * RK + j], v, acc[r][c]);
+					}
+				}
+			}
+			__syncthreads();
+		}
+		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
+		const long long slot = (long long) x.u + blockIdx.x;
+#pragma unroll
+		for (int r = 0; r < 4; r++)
+			if (lane == 0) {
+				const int row = warp * 4 + r;
+				s_corr[row] = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
+				if (row < rows) {
+					if (!direct) {
+						if (slot < part.slots) part.ml[slot * RM + row] = make_float2(m[r], l[r]);
+					} else if (a.lse) {
+						const int w = x.t * RM + row;
+						a.lse[(long long) (x.row0 + w / a.rep) * a.H + h0 + w % a.rep] = l[r] > 0.f || l[r] != l[r] ? (m[r] + log2f(l[r])) * 0.6931471805599453f : -INFINITY;
+					}
+				}
+			}
+		__syncthreads();
+#pragma unroll
+		for (int c = 0; c < NC; c++) {
+			const int col = tid + c * RT;
+			if (col >= dv) break;
+#pragma unroll
+			for (int r = 0; r < RM; r++)
+				if (r < rows) {
+					if (direct) {
+						const int w = x.t * RM + r;
+						reinterpret_cast<T*>(a.out)[(long long) (x.row0 + w / a.rep) * a.out_row + (h0 + w % a.rep) * dv + col] = from_f<T>(s_corr[r] == 0.f ? 0.f : acc[r][c] * s_corr[r]);
+					} else if (slot < part.slots) part.o[(slot * RM + r) * dv + col] = acc[r][c];
+				}
+		}
+	}
+	(void) total;
+}
+
+// =========================================================================================================================================
+// The join: a warp per (row, query head).  Its unit in each part lies in the slots (unit + CTA) of the CTAs whose share of the tiles meets the unit's.
+// =========================================================================================================================================
+template <typename T, bool LIST>
+__global__ void __launch_bounds__(256) paged_join_kernel(const Attn a) {
+	pdl_wait();
+	const long long id = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
+	const int lane = threadIdx.x & 31, dv = a.c.dv;
+	if (id >= (long long) a.b.N * a.H) return;
+	const int row = (int) (id / a.H), h = (int) (id % a.H), g = h / a.rep, r = h % a.rep;
+	const int s = seq_of_row(a.b, row);
+	const Seq q = seq_of(a.c, a.b, s);
+	if (!row_in_seq(q, row)) return;
+	// pieces: (part, unit, row of the unit, first CTA, CTAs)
+	int which[2], unit[2], at[2], c0[2], n[2], found = 0;
+	bool direct = false;
+	for (int i = 0; i < a.n_parts; i++) {
+		const Part& p = a.part[i];
+		const long long total = LIST ? list_total(a, p) : p.cum_w[a.b.n_groups + a.b.B];
+		if (!total) continue;
+		const int shared = LIST ? 0 : p.shs[s];
+		for (int own = 0; own < (LIST ? 1 : 2); own++) {
+			int seg = 0, rows, row0, s_first, u, w;
+			long long w0;
+			int idx; // row of the segment
+			if (LIST) {
+				const int tiles = (a.rep + p.M - 1) / p.M;
+				idx = r;
+				u = (int) (((long long) row * a.c.G + g) * tiles + r / p.M);
+				w = list_tiles(a);
+				w0 = (long long) u * w;
+			} else {
+				if (own) seg = a.b.n_groups + s;
+				else {
+					if (!shared) continue;
+					int lo = 0, hi = a.b.n_groups - 1; // the group of s
+					while (lo < hi) {
+						const int mid = (lo + hi + 1) >> 1;
+						if (a.b.bounds[mid] <= s) lo = mid;
+						else hi = mid - 1;
+					}
+					seg = lo;
+				}
+				rows = seg_rows(a, seg, row0, s_first);
+				if (!in_part(p, !own, rows)) continue;
+				const long long seg_w = p.cum_w[seg + 1] - p.cum_w[seg];
+				if (!seg_w) continue;
+				const int tiles = (rows + p.M - 1) / p.M;
+				idx = (row - row0) * a.rep + r;
+				if (idx < 0 || idx >= rows) continue;
+				const int t = idx / p.M;
+				const Seq fq = seq_of(a.c, a.b, s_first);
+				const int sh = p.shs[s_first];
+				w = unit_tiles(a, p, seg, rows, fq, sh, t);
+				if (!w) continue;
+				long long before = 0;
+				if (!own) before = (long long) t * w;
+				else {
+					for (int i2 = lane; i2 < t; i2 += 32) before += unit_tiles(a, p, seg, rows, fq, sh, i2);
+#pragma unroll
+					for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+				}
+				u = p.cum_u[seg] + g * tiles + t;
+				w0 = p.cum_w[seg] + seg_w / a.c.G * g + before;
+			}
+			const int n_shares = shares(total, p.grid);
+			int first = (int) (w0 * n_shares / total), last = (int) ((w0 + w - 1) * n_shares / total); // a share begins at floor(total cta / shares)
+			while (first + 1 < n_shares && part_begin(total, p.grid, first + 1) <= w0) first++;
+			while (last + 1 < n_shares && part_begin(total, p.grid, last + 1) <= w0 + w - 1) last++;
+			if (first == last && !shared) direct = true;
+			if (found < 2) {
+				which[found] = i; unit[found] = u; at[found] = idx % p.M; c0[found] = first; n[found] = last - first + 1;
+				found++;
+			}
+		}
+	}
+	if (direct) return; // the CTA that had all of the row has written it
+	float m = -INFINITY;
+	for (int f = 0; f < found; f++) {
+		const Part& p = a.part[which[f]];
+		for (int i = lane; i < n[f]; i += 32) {
+			const long long slot = (long long) unit[f] + c0[f] + i;
+			if (slot < p.slots) {
+				const float2 ml = p.ml[slot * p.M + at[f]];
+				m = ml.x != ml.x || m != m ? NAN : fmaxf(m, ml.x);
+			}
+		}
+	}
+	const bool nan = __any_sync(0xffffffffu, m != m);
+	m = warp_max(m);
+	const float base = nan ? NAN : m == -INFINITY ? 0.f : m;
+	float l = 0.f, acc[8];
+#pragma unroll
+	for (int i = 0; i < 8; i++) acc[i] = 0.f;
+	for (int f = 0; f < found; f++) {
+		const Part& p = a.part[which[f]];
+		for (int i = 0; i < n[f]; i++) {
+			const long long slot = (long long) unit[f] + c0[f] + i;
+			if (slot >= p.slots) continue;
+			const float2 ml = p.ml[slot * p.M + at[f]];
+			if (ml.x == -INFINITY) continue; // nothing that the row sees
+			const float w = exp2f(ml.x - base);
+			l = fmaf(ml.y, w, l);
+			const float* o = p.o + (slot * p.M + at[f]) * dv;
+#pragma unroll
+			for (int c = 0; c < 2; c++)
+				if (c * 128 + lane * 4 < dv) {
+					const float4 v = *reinterpret_cast<const float4*>(o + c * 128 + lane * 4);
+					acc[4 * c] = fmaf(v.x, w, acc[4 * c]);
+					acc[4 * c + 1] = fmaf(v.y, w, acc[4 * c + 1]);
+					acc[4 * c + 2] = fmaf(v.z, w, acc[4 * c + 2]);
+					acc[4 * c + 3] = fmaf(v.w, w, acc[4 * c + 3]);
+				}
+		}
+	}
+	const bool any = l > 0.f || l != l;
+	const float inv = any ? 1.f / l : 0.f;
+	T* out = reinterpret_cast<T*>(a.out) + (long long) row * a.out_row + h * dv;
+#pragma unroll
+	for (int c = 0; c < 2; c++)
+		if (c * 128 + lane * 4 < dv) {
+			T v[4];
+#pragma unroll
+			for (int e = 0; e < 4; e++) v[e] = from_f<T>(any ? acc[4 * c + e] * inv : 0.f);
+			if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out + c * 128 + lane * 4) = *reinterpret_cast<const uint4*>(v);
+			else *reinterpret_cast<uint2*>(out + c * 128 + lane * 4) = *reinterpret_cast<const uint2*>(v);
+		}
+	if (a.lse && lane == 0) a.lse[(long long) row * a.H + h] = any ? (base + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename K, typename... A>
+static cudaError_t launch(K kernel, int grid, int block, size_t smem, cudaStream_t s, bool after, const A&... args) {
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = dim3((unsigned) grid);
+	cfg.blockDim = dim3((unsigned) block);
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = s;
+	cudaLaunchAttribute at[1];
+	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at[0].val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = at;
+	cfg.numAttrs = after ? 1 : 0;
+	return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T>
+static int join_typed(const Attn& a, cudaStream_t s) {
+	const long long warps = (long long) a.b.N * a.H;
+	const int grid = (int) ((warps + 7) / 8);
+	XALM_CUDA_CHECK(a.lists ? launch(paged_join_kernel<T, true>, grid, 256, 0, s, true, a) : launch(paged_join_kernel<T, false>, grid, 256, 0, s, true, a));
+	return XALM_OK;
+}
+int launch_join(const Attn& a, int type, cudaStream_t s) {
+	return type == XALM_F32 ? join_typed<float>(a, s) : type == XALM_F16 ? join_typed<__half>(a, s) : join_typed<__nv_bfloat16>(a, s);
+}
+
+template <typename T, int NC, bool LIST>
+static int rows_typed(const Attn& a, cudaStream_t s) {
+	const size_t smem = (size_t) (RM * a.c.d + RK * (a.c.d + 4) + RK * a.c.dv + RM * RK + 2 * RM) * 4 + (RM + RK + (LIST ? a.S : 0) + 2) * 4 + 16 +
+	                    (LIST ? 0 : plan_bytes(a.b.B, a.b.n_groups));
+	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_rows_kernel<T, NC, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	XALM_CUDA_CHECK(launch(paged_rows_kernel<T, NC, LIST>, a.part[0].grid, RT, smem, s, false, a));
+	return XALM_OK;
+}
+template <typename T>
+static int rows_cols(const Attn& a, cudaStream_t s) {
+	if (a.lists) return a.c.dv > RT ? rows_typed<T, 2, true>(a, s) : rows_typed<T, 1, true>(a, s);
+	return a.c.dv > RT ? rows_typed<T, 2, false>(a, s) : rows_typed<T, 1, false>(a, s);
+}
+int launch_attn_rows(const Attn& a, int type, cudaStream_t s) {
+	return type == XALM_F32 ? rows_cols<float>(a, s) : type == XALM_F16 ? rows_cols<__half>(a, s) : rows_cols<__nv_bfloat16>(a, s);
+}
+
+} // namespace paged
+} // namespace xalm
