@@ -378,7 +378,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 	for (int i = 0; i < a.n_parts; i++) {
 		Part& p = a.part[i];
 		p.M = 16;
-		p.grid = sms * 2;
+		p.grid = sms * (cache->type == XALM_F32 ? 2 : mma_ctas_per_sm(c, b, n_lists));
 		p.small_rows = 0x7fffffff;
 		p.small = p.big = p.prefix = 1;
 		const long long rows = (long long) b.N * a.rep;
@@ -440,7 +440,7 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 	a.scale = scale;
 	a.lists = lists;
 	cudaStream_t s = (cudaStream_t) stream;
-	XALM_TRY(launch_attn_rows(a, cache->type, s));
+	XALM_TRY(cache->type == XALM_F32 ? launch_attn_rows(a, s) : launch_attn_mma(a, cache->type, s));
 	return launch_join(a, cache->type, s);
 }
 

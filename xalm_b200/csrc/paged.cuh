@@ -14,7 +14,7 @@ namespace paged {
 constexpr int KT = 64;              // keys of a tile, the unit in which attention counts its work
 constexpr int MAX_SEGMENTS = 4096;  // sequences and groups of one call: the plan lies in shared memory
 constexpr int MAX_LIST = 1024;      // pages that a list of attend_selected names
-constexpr int ERR_PAGE = 1, ERR_BATCH = 2; // bits of the cache's status word
+constexpr int ERR_PAGE = 1, ERR_BATCH = 2, ERR_WAIT = 4; // bits of the cache's status word
 
 struct Cache {
 	uint8_t *k, *v, *means;
@@ -351,18 +351,22 @@ __device__ __forceinline__ bool walk_next(const Attn& a, const Part& part, const
 }
 // SELECTED: units are (row, kv head, M of its query heads), every one of `w` tiles
 __device__ __forceinline__ int list_tiles(const Attn& a) { return (int) ((((long long) a.S << a.c.shift) + KT - 1) / KT); }
-__device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk& k, long long unit) {
+__device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk& k, long long unit, bool walking) {
 	const int tiles = (a.rep + part.M - 1) / part.M;
 	k.x.u = (int) unit;
 	k.x.t = (int) (unit % tiles);
 	k.x.g = (int) (unit / tiles % a.c.G);
-	k.x.row0 = (int) (unit / tiles / a.c.G);
+	const int row = (int) (unit / tiles / a.c.G);
+	const bool same_row = walking && row == k.x.row0;
+	k.x.row0 = row;
 	k.x.rows = a.rep;
 	k.x.seg = 0;
 	k.x.key0 = 0;
 	k.x.w = list_tiles(a);
-	k.x.s = seq_of_row(a.b, k.x.row0); // whole warps walk
-	k.x.q = seq_of(a.c, a.b, k.x.s);
+	if (!same_row) {
+		k.x.s = seq_of_row(a.b, k.x.row0); // whole warps walk
+		k.x.q = seq_of(a.c, a.b, k.x.s);
+	}
 }
 __device__ __forceinline__ long long list_total(const Attn& a, const Part& part) {
 	return (long long) a.b.N * a.c.G * ((a.rep + part.M - 1) / part.M) * list_tiles(a);
@@ -373,7 +377,7 @@ __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk
 	k.end = part_begin(total, part.grid, blockIdx.x + 1);
 	if (k.at >= k.end) return false;
 	const int w = list_tiles(a);
-	list_unit(a, part, k, k.at / w);
+	list_unit(a, part, k, k.at / w, false);
 	k.x.j0 = (int) (k.at % w);
 	k.x.j1 = (int) min((long long) w, k.x.j0 + (k.end - k.at));
 	return true;
@@ -381,7 +385,7 @@ __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk
 __device__ __forceinline__ bool list_next(const Attn& a, const Part& part, Walk& k) {
 	k.at += k.x.j1 - k.x.j0;
 	if (k.at >= k.end) return false;
-	list_unit(a, part, k, k.x.u + 1);
+	list_unit(a, part, k, k.x.u + 1, true);
 	k.x.j0 = 0;
 	k.x.j1 = (int) min((long long) k.x.w, k.end - k.at);
 	return true;
@@ -431,8 +435,26 @@ __device__ __forceinline__ int list_pages(const Attn& a, int row, int g, int own
 	return n;
 }
 
+// Launches; `after`: may start while the kernel before it on the stream still runs (it waits for it itself).
+template <typename K, typename... A>
+inline cudaError_t launch(K kernel, dim3 grid, int block, size_t smem, cudaStream_t s, bool after, const A&... args) {
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = grid;
+	cfg.blockDim = dim3((unsigned) block);
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = s;
+	cudaLaunchAttribute at[1];
+	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at[0].val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = at;
+	cfg.numAttrs = after ? 1 : 0;
+	return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 int launch_join(const Attn& a, int type, cudaStream_t s);
-int launch_attn_rows(const Attn& a, int type, cudaStream_t s);
+int launch_attn_rows(const Attn& a, cudaStream_t s); // fp32 caches
+// 16-bit caches: CTAs per SM that the kernel's shared memory leaves room for
+int mma_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists);
+int launch_attn_mma(const Attn& a, int type, cudaStream_t s);
 
 } // namespace paged
 } // namespace xalm

@@ -10,9 +10,10 @@ namespace paged {
 // =========================================================================================================================================
 constexpr int RM = 16, RK = 32, RT = 128;
 
-template <typename T, int NC, bool LIST> // NC columns of V per thread
-__global__ void __launch_bounds__(RT) paged_rows_kernel(const Attn a) {
+template <int NC, bool LIST> // NC columns of V per thread
+__global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ Attn a) {
 	extern __shared__ __align__(16) uint8_t smem[];
+	using T = float;
 	const Part& part = a.part[0];
 	const int d = a.c.d, dv = a.c.dv, kp = d + 4, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	float* sq = reinterpret_cast<float*>(smem);  // [RM][d]
@@ -30,7 +31,6 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const Attn a) {
 	if (!LIST) make_plan<RT>(a, part, s_plan, plan);
 	Walk k;
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
-	const long long total = LIST ? list_total(a, part) : plan.total;
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		__syncthreads();
@@ -171,14 +171,13 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const Attn a) {
 				}
 		}
 	}
-	(void) total;
 }
 
 // =========================================================================================================================================
 // The join: a warp per (row, query head).  Its unit in each part lies in the slots (unit + CTA) of the CTAs whose share of the tiles meets the unit's.
 // =========================================================================================================================================
 template <typename T, bool LIST>
-__global__ void __launch_bounds__(256) paged_join_kernel(const Attn a) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn a) {
 	pdl_wait();
 	const long long id = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
 	const int lane = threadIdx.x & 31, dv = a.c.dv;
@@ -274,8 +273,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Attn a) {
 			const long long slot = (long long) unit[f] + c0[f] + i;
 			if (slot >= p.slots) continue;
 			const float2 ml = p.ml[slot * p.M + at[f]];
-			if (ml.x == -INFINITY) continue; // nothing that the row sees
-			const float w = exp2f(ml.x - base);
+			if (ml.x == -INFINITY && ml.y == 0.f) continue; // nothing that the row sees
+			const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - base); // a sum that is NaN stays one
 			l = fmaf(ml.y, w, l);
 			const float* o = p.o + (slot * p.M + at[f]) * dv;
 #pragma unroll
@@ -304,21 +303,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Attn a) {
 	if (a.lse && lane == 0) a.lse[(long long) row * a.H + h] = any ? (base + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
-template <typename K, typename... A>
-static cudaError_t launch(K kernel, int grid, int block, size_t smem, cudaStream_t s, bool after, const A&... args) {
-	cudaLaunchConfig_t cfg = {};
-	cfg.gridDim = dim3((unsigned) grid);
-	cfg.blockDim = dim3((unsigned) block);
-	cfg.dynamicSmemBytes = smem;
-	cfg.stream = s;
-	cudaLaunchAttribute at[1];
-	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-	at[0].val.programmaticStreamSerializationAllowed = 1;
-	cfg.attrs = at;
-	cfg.numAttrs = after ? 1 : 0;
-	return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename T>
 static int join_typed(const Attn& a, cudaStream_t s) {
 	const long long warps = (long long) a.b.N * a.H;
@@ -330,21 +314,17 @@ int launch_join(const Attn& a, int type, cudaStream_t s) {
 	return type == XALM_F32 ? join_typed<float>(a, s) : type == XALM_F16 ? join_typed<__half>(a, s) : join_typed<__nv_bfloat16>(a, s);
 }
 
-template <typename T, int NC, bool LIST>
-static int rows_typed(const Attn& a, cudaStream_t s) {
+template <int NC, bool LIST>
+static int rows_cols(const Attn& a, cudaStream_t s) {
 	const size_t smem = (size_t) (RM * a.c.d + RK * (a.c.d + 4) + RK * a.c.dv + RM * RK + 2 * RM) * 4 + (RM + RK + (LIST ? a.S : 0) + 2) * 4 + 16 +
 	                    (LIST ? 0 : plan_bytes(a.b.B, a.b.n_groups));
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_rows_kernel<T, NC, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-	XALM_CUDA_CHECK(launch(paged_rows_kernel<T, NC, LIST>, a.part[0].grid, RT, smem, s, false, a));
+	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_rows_kernel<NC, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	XALM_CUDA_CHECK(launch(paged_rows_kernel<NC, LIST>, a.part[0].grid, RT, smem, s, false, a));
 	return XALM_OK;
 }
-template <typename T>
-static int rows_cols(const Attn& a, cudaStream_t s) {
-	if (a.lists) return a.c.dv > RT ? rows_typed<T, 2, true>(a, s) : rows_typed<T, 1, true>(a, s);
-	return a.c.dv > RT ? rows_typed<T, 2, false>(a, s) : rows_typed<T, 1, false>(a, s);
-}
-int launch_attn_rows(const Attn& a, int type, cudaStream_t s) {
-	return type == XALM_F32 ? rows_cols<float>(a, s) : type == XALM_F16 ? rows_cols<__half>(a, s) : rows_cols<__nv_bfloat16>(a, s);
+int launch_attn_rows(const Attn& a, cudaStream_t s) {
+	if (a.lists) return a.c.dv > RT ? rows_cols<2, true>(a, s) : rows_cols<1, true>(a, s);
+	return a.c.dv > RT ? rows_cols<2, false>(a, s) : rows_cols<1, false>(a, s);
 }
 
 } // namespace paged

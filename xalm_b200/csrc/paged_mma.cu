@@ -1,0 +1,398 @@
+// paged_mma.cu — attention over paged caches of 16-bit elements, for few rows: a token, or the few (token, head) rows that fit one 16-row matrix tile.
+#include <cuda.h>
+
+#include "paged.cuh"
+#include "paged_tma.cuh"
+
+namespace xalm {
+namespace paged {
+
+// =========================================================================================================================================
+// out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j, in one pass over the pages.  A step of single tokens reads every key and value once
+// for a handful of rows: HBM bounds it, and what the kernel has to do is to keep enough bytes on their way.  A warp brings tiles of 64 keys and values
+// by TMA (boxes of a page's slots, 64 entries wide, swizzled) into a ring; four warps take a tile each, so that none waits for another: scores and sums by
+// mma.sync m16n8k16 with the 16 rows as A, running maximum and sum in registers.  At the end of a piece the four join through shared memory.  (tcgen05 would want 64
+// rows or more: a step of four heads to a kv head has four.)
+// Probabilities enter the second product in the cache's type, a rounding of 2^-9 (bf16) or 2^-12 (fp16) of each, of either sign; scores, maxima and sums stay in fp32.
+// =========================================================================================================================================
+constexpr int MM = 16, CW = 4, MT = (CW + 1) * 32;
+
+struct MmaConfig {
+	int stages, per_sm;
+	size_t smem;
+};
+template <int D>
+struct Sizes {
+	static constexpr int TILE = KT * D * 2;         // bytes of a key or value tile
+	static constexpr int STAGE = 2 * TILE;
+	static constexpr int Q = MM * D * 2;
+	static constexpr int OS = D + 8;                // floats between rows of the join's buffer
+	static constexpr int JOIN = CW * 8 * OS * 4;
+};
+// Two CTAs of three or more stages on an SM, or one with what there is: bytes on their way count, not how many CTAs ask for them
+template <int D>
+static MmaConfig mma_config(size_t plan, int n_lists) {
+	using Z = Sizes<D>;
+	const size_t fixed = 1024 + Z::Q + Z::JOIN + CW * MM * 8 + 256 + (size_t) n_lists * 4 + 16 + plan;
+	for (int per_sm = 2; per_sm >= 1; per_sm--) {
+		const size_t room = per_sm == 2 ? 113 * 1024 : 226 * 1024;
+		const int n = room > fixed ? (int) ((room - fixed) / Z::STAGE) : 0;
+		if (n >= 3 || per_sm == 1) {
+			const int stages = n > 8 ? 8 : n;
+			return MmaConfig{stages, per_sm, fixed + (size_t) stages * Z::STAGE};
+		}
+	}
+	return MmaConfig{};
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+	if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+		asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+		             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+		             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+	else
+		asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+		             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+		             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+// 16-byte chunk c of row r in a tile of 64-entry columns with `rows` rows each, as the copy engine's 128-byte swizzle lays it
+__device__ __forceinline__ uint32_t chunk_at(uint32_t base, int rows, int r, int c) { return base + (uint32_t) ((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+	if constexpr (std::is_same<T, __half>::value) {
+		const __half2 h = __floats2half2_rn(lo, hi);
+		return *reinterpret_cast<const uint32_t*>(&h);
+	} else {
+		const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+		return *reinterpret_cast<const uint32_t*>(&h);
+	}
+}
+__device__ __forceinline__ float ex2(float x) {
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+
+template <typename T, int D, bool LIST>
+__global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const __grid_constant__ CUtensorMap kmap,
+                                                                         const __grid_constant__ CUtensorMap vmap, const int stages) {
+	using Z = Sizes<D>;
+	extern __shared__ uint8_t raw[];
+	uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+	uint8_t* ring = smem;
+	uint8_t* s_q = ring + (size_t) stages * Z::STAGE;
+	float* s_o = reinterpret_cast<float*>(s_q + Z::Q);                    // [CW][8][OS]
+	float2* s_ml = reinterpret_cast<float2*>((uint8_t*) s_o + Z::JOIN);   // [CW][MM]
+	uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + CW * MM);         // [8]
+	uint64_t* empty = full + 8;                                           // [8]
+	int* s_dead = reinterpret_cast<int*>(empty + 8);
+	int* s_list = reinterpret_cast<int*>((uint8_t*) full + 256);          // [S]
+	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list) + ((LIST ? a.S * 4 : 0) + 15) / 16 * 16;
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	if (tid == 0) {
+		for (int i = 0; i < stages; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+		*s_dead = 0;
+		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+	}
+	pdl_wait();
+	pdl_launch_dependents();
+	Plan plan;
+	if (!LIST) make_plan<MT>(a, part, s_plan, plan);
+	__syncthreads();
+	const int dc = (a.c.d + 63) / 64, vc = (a.c.dv + 63) / 64;
+	const int P = 1 << a.c.shift, W = min(P, KT), per = KT / W; // slots of a box, boxes of a tile's column
+	Walk k;
+	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
+	int n = 0; // tiles that this CTA's pieces have had so far: tile n lies in stage n % stages and is warp n % CW's
+
+	if (warp == CW) { // ---- the copies ----
+		const int boxes = per * (dc + vc);
+		for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
+			const Piece& x = k.x;
+			int pages = 0, vis = 0x7fffffff;
+			if (LIST) {
+				if (!row_in_seq(x.q, x.row0)) continue;
+				const int pos = x.q.len - x.q.n + x.row0 - x.q.a;
+				bool own;
+				pages = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, s_list, &own);
+				vis = pages << a.c.shift;
+				if (own) vis += (pos & (P - 1)) + 1 - P;
+			} else if (x.seg < a.b.n_groups) vis = plan.shs[x.s];
+			else vis = own_keys(x.q, x.key0, a.rep, min((x.t + 1) * MM, x.rows) - 1);
+			const int j1 = min(x.j1, (vis + KT - 1) / KT);
+			int id = -1;
+			for (int j = x.j0, e = 0; j < j1; j++, e += per, n++) { // entry e: the e-th box's worth of slots from the piece's first on
+				if ((e & 31) == 0) { // the pages of the next 32
+					const int at = x.j0 * KT + (e + lane) * W;
+					id = -1;
+					if (at < vis) {
+						const int key = x.key0 + at;
+						id = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
+						if (id < 0) report(a.c, ERR_PAGE);
+					}
+				}
+				const int st = n % stages;
+				if (!wait_for(&empty[st], ((n / stages) & 1) ^ 1, s_dead, a.c)) break;
+				if (lane == 0) mbar_expect_tx(&full[st], (uint32_t) (boxes * W * 128));
+				__syncwarp();
+				const int which = lane / per, part_of = lane % per; // column block (keys, then values), box of the tile
+				const int pg = __shfl_sync(0xffffffffu, id, (e + part_of) & 31);
+				if (lane < boxes) {
+					const int slot = (x.key0 + j * KT + part_of * W) & (P - 1), block = which < dc ? which : which - dc;
+					uint8_t* dst = ring + (size_t) st * Z::STAGE + (which < dc ? 0 : Z::TILE) + block * KT * 128 + part_of * W * 128;
+					copy_box(dst, which < dc ? &kmap : &vmap, block * 64, slot, x.g, pg < 0 ? a.c.pages : pg, &full[st]); // behind the last page: zeros
+				}
+				__syncwarp();
+			}
+			if (*(volatile int*) s_dead) break;
+		}
+		if (*(volatile int*) s_dead) // gave up: copies still on their way end first
+			for (int i = max(0, n - stages); i < n; i++) wait_some(&full[i % stages], (i / stages) & 1);
+		return;
+	}
+
+	// ---- the products ----
+	const uint32_t q_at = smem_u32(s_q);
+	const int kd = (a.c.d + 15) / 16, nd = (a.c.dv + 15) / 16;
+	const float c1 = a.scale * 1.4426950408889634f;
+	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
+		const Piece& x = k.x;
+		const bool prefix = !LIST && x.seg < a.b.n_groups;
+		const int rows = min(MM, x.rows - x.t * MM), h0 = x.g * a.rep;
+		int lim0, lim1, least, most; // keys that this lane's two rows see; that the first and the last row see
+		if (LIST) {
+			if (!row_in_seq(x.q, x.row0)) continue;
+			const int pos = x.q.len - x.q.n + x.row0 - x.q.a;
+			bool own;
+			const int pages = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, nullptr, &own);
+			least = most = lim0 = lim1 = (pages << a.c.shift) + (own ? (pos & (P - 1)) + 1 - P : 0);
+		} else if (prefix) least = most = lim0 = lim1 = plan.shs[x.s];
+		else {
+			least = own_keys(x.q, x.key0, a.rep, x.t * MM);
+			most = own_keys(x.q, x.key0, a.rep, x.t * MM + rows - 1);
+			lim0 = own_keys(x.q, x.key0, a.rep, min(x.t * MM + lane / 4, x.rows - 1));
+			lim1 = own_keys(x.q, x.key0, a.rep, min(x.t * MM + lane / 4 + 8, x.rows - 1));
+		}
+		for (int i = tid; i < MM * dc * 8; i += CW * 32) {
+			const int r = i / (dc * 8), c = i % (dc * 8);
+			uint4 v = make_uint4(0, 0, 0, 0);
+			if (r < rows && c * 8 < a.c.d) {
+				const int w = x.t * MM + r;
+				v = *reinterpret_cast<const uint4*>(a.q + ((long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d + c * 8) * 2);
+			}
+			*reinterpret_cast<uint4*>(s_q + (chunk_at(q_at, MM, r, c) - q_at)) = v;
+		}
+		bar_sync(1, CW * 32);
+		float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+		for (int i = 0; i < D / 8; i++)
+#pragma unroll
+			for (int e = 0; e < 4; e++) o[i][e] = 0.f;
+		const int j1 = min(x.j1, (most + KT - 1) / KT);
+		const bool high = rows > 8;
+		for (int j = x.j0; j < j1; j++, n++) {
+			if (n % CW != warp) continue;
+			const int st = n % stages;
+			if (!wait_for(&full[st], (n / stages) & 1, s_dead, a.c)) continue;
+			const uint32_t kt = smem_u32(ring + (size_t) st * Z::STAGE), vt = kt + Z::TILE;
+			const int base = j * KT;
+			if (base + KT > most) { // slots that no row sees may hold anything: as zeros they add nothing
+				for (int i = lane; i < (base + KT - most) * vc * 8; i += 32) {
+					const int r = most - base + i / (vc * 8), c = i % (vc * 8);
+					asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at(vt, KT, r, c)), "r"(0) : "memory");
+				}
+				__syncwarp();
+			}
+			float s[8][4];
+#pragma unroll
+			for (int i = 0; i < 8; i++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) s[i][e] = 0.f;
+#pragma unroll
+			for (int kk = 0; kk < D / 16; kk++)
+				if (kk < kd) {
+					uint32_t qa[4];
+					ldsm4(qa, chunk_at(q_at, MM, (lane & 7) + ((lane >> 3) & 1) * 8, kk * 2 + (lane >> 4)));
+#pragma unroll
+					for (int i = 0; i < 4; i++) { // 16 keys
+						uint32_t b[4];
+						ldsm4(b, chunk_at(kt, KT, i * 16 + (lane & 7) + (lane >> 4) * 8, kk * 2 + ((lane >> 3) & 1)));
+						mma16<T>(s[2 * i], qa, b[0], b[1]);
+						mma16<T>(s[2 * i + 1], qa, b[2], b[3]);
+					}
+				}
+			const bool cut = base + KT > least;
+			float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+			for (int i = 0; i < 8; i++) {
+#pragma unroll
+				for (int e = 0; e < 4; e++) {
+					s[i][e] *= c1;
+					if (cut && base + i * 8 + (lane & 3) * 2 + (e & 1) >= (e < 2 ? lim0 : lim1)) s[i][e] = -INFINITY;
+				}
+				t0 = fmaxf(t0, fmaxf(s[i][0], s[i][1]));
+				t1 = fmaxf(t1, fmaxf(s[i][2], s[i][3]));
+			}
+#pragma unroll
+			for (int w = 1; w < 4; w <<= 1) {
+				t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
+				t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
+			}
+			const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+			if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+				const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+				l0 *= f0;
+				l1 *= f1;
+#pragma unroll
+				for (int i = 0; i < D / 8; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
+				m0 = n0;
+				m1 = n1;
+			}
+			const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+			uint32_t p[8][2];
+#pragma unroll
+			for (int i = 0; i < 8; i++) {
+				const float x0 = ex2(s[i][0] - b0), x1 = ex2(s[i][1] - b0);
+				l0 += x0 + x1;
+				p[i][0] = pack16<T>(x0, x1);
+				p[i][1] = 0;
+				if (high) {
+					const float x2 = ex2(s[i][2] - b1), x3 = ex2(s[i][3] - b1);
+					l1 += x2 + x3;
+					p[i][1] = pack16<T>(x2, x3);
+				}
+			}
+#pragma unroll
+			for (int i = 0; i < 4; i++) { // 16 keys
+				const uint32_t pa[4] = {p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1]};
+#pragma unroll
+				for (int c = 0; c < D / 16; c++)
+					if (c < nd) {
+						uint32_t b[4];
+						ldsm4_t(b, chunk_at(vt, KT, i * 16 + (lane & 15), c * 2 + (lane >> 4)));
+						mma16<T>(o[2 * c], pa, b[0], b[1]);
+						mma16<T>(o[2 * c + 1], pa, b[2], b[3]);
+					}
+			}
+			if (base + KT > most) asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the zeros, before the next copy
+			__syncwarp();
+			if (lane == 0) mbar_arrive(&empty[st]);
+		}
+		// ---- the four warps' sums ----
+#pragma unroll
+		for (int w = 1; w < 4; w <<= 1) {
+			l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+			l1 += __shfl_xor_sync(0xffffffffu, l1, w);
+		}
+		if ((lane & 3) == 0) {
+			s_ml[warp * MM + lane / 4] = make_float2(m0, l0);
+			s_ml[warp * MM + lane / 4 + 8] = make_float2(m1, l1);
+		}
+		bar_sync(1, CW * 32);
+		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && x.key0 == 0;
+		const long long slot = (long long) x.u + blockIdx.x;
+		const bool mixed = !LIST && !prefix && least < most && x.j1 * KT > least; // some row of the tile must not see what another does
+#pragma unroll
+		for (int half = 0; half < 2; half++) {
+			if (half && !high) break;
+			float f;
+			{
+				const int r = lane / 4 + half * 8;
+				float mx = -INFINITY;
+#pragma unroll
+				for (int w = 0; w < CW; w++) mx = fmaxf(mx, s_ml[w * MM + r].x);
+				const float mine = half ? m1 : m0;
+				f = mine == -INFINITY ? 0.f : ex2(mine - mx);
+			}
+#pragma unroll
+			for (int i = 0; i < D / 8; i++)
+				if (i * 8 < a.c.dv)
+					*reinterpret_cast<float2*>(s_o + (warp * 8 + lane / 4) * Z::OS + i * 8 + (lane & 3) * 2) = make_float2(o[i][half * 2] * f, o[i][half * 2 + 1] * f);
+			bar_sync(1, CW * 32);
+			const int rh = min(8, rows - half * 8), cols = a.c.dv / 4;
+			for (int i = tid; i < rh * cols; i += CW * 32) {
+				const int r = i / cols, c = i % cols * 4, row = half * 8 + r;
+				float mx = -INFINITY, l = 0.f;
+#pragma unroll
+				for (int w = 0; w < CW; w++) mx = fmaxf(mx, s_ml[w * MM + row].x);
+#pragma unroll
+				for (int w = 0; w < CW; w++) {
+					const float2 ml = s_ml[w * MM + row];
+					l += ml.y * (ml.x == -INFINITY ? 0.f : ex2(ml.x - mx)); // a NaN stays one
+				}
+				float4 v = *reinterpret_cast<const float4*>(s_o + r * Z::OS + c);
+#pragma unroll
+				for (int w = 1; w < CW; w++) {
+					const float4 u = *reinterpret_cast<const float4*>(s_o + (w * 8 + r) * Z::OS + c);
+					v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+				}
+				put_row<T>(a, part, x, MM, row, c, v, mx, l, direct, slot);
+			}
+			bar_sync(1, CW * 32);
+		}
+		if (mixed) {
+			// A value that is not finite and that only later rows see has met probabilities of zero in the product: rows that did not come out finite
+			// are done again, key by key.
+			bool again = false;
+#pragma unroll
+			for (int i = 0; i < D / 8; i++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) again = again || !(fabsf(o[i][e]) <= 3.0e38f);
+			if (tid == 0) s_ml[0].x = 0.f;
+			bar_sync(1, CW * 32);
+			if (again) s_ml[0].x = 1.f;
+			bar_sync(1, CW * 32);
+			const bool redo = s_ml[0].x != 0.f;
+			bar_sync(1, CW * 32);
+			if (redo)
+				for (int r = 0; r < rows; r++) slow_row<T>(a, part, x, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, CW * 32);
+		}
+		bar_sync(1, CW * 32);
+	}
+}
+
+template <int D>
+static MmaConfig config_of(const Cache&, const BatchView& b, int n_lists) { return mma_config<D>(n_lists ? 0 : plan_bytes(b.B, b.n_groups), n_lists); }
+static int padded(const Cache& c) {
+	const int d = c.d > c.dv ? c.d : c.dv;
+	return d <= 64 ? 64 : d <= 128 ? 128 : 256;
+}
+int mma_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists) {
+	const int D = padded(c);
+	return (D == 64 ? config_of<64>(c, b, n_lists) : D == 128 ? config_of<128>(c, b, n_lists) : config_of<256>(c, b, n_lists)).per_sm;
+}
+
+template <typename T, int D, bool LIST>
+static int launch_typed(const Attn& a, int type, cudaStream_t s) {
+	const MmaConfig cfg = config_of<D>(a.c, a.b, LIST ? a.S : 0);
+	if (cfg.stages < 1) return set_error(XALM_ERR_INVALID, "paged attention: no shared memory left for pages beside %d sequences", a.b.B);
+	CUtensorMap kmap, vmap;
+	XALM_TRY(pool_map(a.c, type, true, &kmap));
+	XALM_TRY(pool_map(a.c, type, false, &vmap));
+	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_mma_kernel<T, D, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) cfg.smem));
+	XALM_CUDA_CHECK(launch(paged_mma_kernel<T, D, LIST>, a.part[0].grid, MT, cfg.smem, s, false, a, a.part[0], kmap, vmap, cfg.stages));
+	return XALM_OK;
+}
+template <typename T, int D>
+static int launch_lists(const Attn& a, int type, cudaStream_t s) {
+	return a.lists ? launch_typed<T, D, true>(a, type, s) : launch_typed<T, D, false>(a, type, s);
+}
+template <typename T>
+static int launch_size(const Attn& a, int type, cudaStream_t s) {
+	switch (padded(a.c)) {
+		case 64: return launch_lists<T, 64>(a, type, s);
+		case 128: return launch_lists<T, 128>(a, type, s);
+		default: return launch_lists<T, 256>(a, type, s);
+	}
+}
+int launch_attn_mma(const Attn& a, int type, cudaStream_t s) { return type == XALM_F16 ? launch_size<__half>(a, type, s) : launch_size<__nv_bfloat16>(a, type, s); }
+
+} // namespace paged
+} // namespace xalm

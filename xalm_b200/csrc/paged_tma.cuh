@@ -1,0 +1,144 @@
+// paged_tma.cuh — pages through the copy engine, waits that end, and what the tensor-core kernels over paged caches share at the end of a piece.
+#pragma once
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace xalm {
+namespace paged {
+
+// A pool as the copy engine sees it: (entries, slots, heads, pages), boxes of 64 entries and min(page, 64) slots of one head.  Entries behind the head's
+// last and pages behind the pool's last read as zeros.
+static inline int pool_map(const Cache& c, int type, bool keys, CUtensorMap* map) {
+	typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+	                           CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+	static const Encode encode = [] {
+		void* f = nullptr;
+		cudaDriverEntryPointQueryResult q;
+		if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+			cudaGetLastError();
+			return (Encode) nullptr;
+		}
+		return (Encode) f;
+	}();
+	if (!encode) return set_error(XALM_ERR_CUDA, "paged attention: this driver has no cuTensorMapEncodeTiled");
+	const int P = 1 << c.shift;
+	const cuuint64_t dims[4] = {(cuuint64_t) (keys ? c.d : c.dv), (cuuint64_t) P, (cuuint64_t) c.G, (cuuint64_t) c.pages};
+	const cuuint64_t strides[3] = {(cuuint64_t) (keys ? c.k_slot : c.v_slot) * 2, (cuuint64_t) (keys ? c.k_head : c.v_head) * 2, (cuuint64_t) (keys ? c.k_page : c.v_page) * 2};
+	const cuuint32_t box[4] = {64, (cuuint32_t) (P < KT ? P : KT), 1, 1}, steps[4] = {1, 1, 1, 1};
+	const CUresult r = encode(map, type == XALM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, keys ? c.k : c.v, dims, strides, box, steps,
+	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+	if (r != CUDA_SUCCESS) return set_error(XALM_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled failed (%d)", (int) r);
+	return XALM_OK;
+}
+__device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int x, int slot, int head, int page, uint64_t* bar) {
+	asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)), "l"(map), "r"(x),
+	             "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+	             : "memory");
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+	uint32_t ok;
+	asm volatile(
+	    "{\n"
+	    ".reg .pred p;\n"
+	    "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+	    "selp.u32 %0, 1, 0, p;\n"
+	    "}\n"
+	    : "=r"(ok)
+	    : "r"(smem_u32(bar)), "r"(parity)
+	    : "memory");
+	return ok != 0;
+}
+constexpr int WAIT_TRIES = 1 << 22; // seconds: far beyond what a copy takes
+__device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity) {
+	for (int i = 0; i < WAIT_TRIES; i++)
+		if (try_wait(bar, parity)) return true;
+	return false;
+}
+// A wait of a whole warp that ends: when it gives up, or another of the CTA has, the status word says so and nobody waits any more
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* dead, const Cache& c) {
+	bool ok = false;
+	for (int i = 0; i < WAIT_TRIES && !(ok = try_wait(bar, parity)); i++)
+		if (*(volatile int*) dead) break;
+	ok = __all_sync(0xffffffffu, ok);
+	if (!ok && !*(volatile int*) dead) {
+		*(volatile int*) dead = 1;
+		report(c, ERR_WAIT);
+	}
+	return ok;
+}
+
+// Four neighbouring sums of one row of a piece, with the row's maximum (log2 units) and sum: to the output, or to the slot that the join reads
+template <typename T>
+__device__ __forceinline__ void put_row(const Attn& a, const Part& part, const Piece& x, int M, int row, int c, float4 v, float m, float l, bool direct, long long slot) {
+	if (direct) {
+		const int w = x.t * M + row, h = x.g * a.rep + w % a.rep;
+		const long long token = x.row0 + w / a.rep;
+		const bool any = l > 0.f || l != l;
+		const float inv = any ? 1.f / l : 0.f;
+		T t[4] = {from_f<T>(any ? v.x * inv : 0.f), from_f<T>(any ? v.y * inv : 0.f), from_f<T>(any ? v.z * inv : 0.f), from_f<T>(any ? v.w * inv : 0.f)};
+		*reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + token * a.out_row + h * a.c.dv + c) = *reinterpret_cast<const uint2*>(t);
+		if (a.lse && c == 0) a.lse[token * a.H + h] = any ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+	} else if (slot < part.slots) {
+		*reinterpret_cast<float4*>(part.o + (slot * M + row) * a.c.dv + c) = v;
+		if (c == 0) part.ml[slot * M + row] = make_float2(m, l);
+	}
+}
+
+// One row of a piece by fp32 FMAs, with only the keys that it sees: for rows that a value which is not finite has spoilt.  `threads` (128) threads of barrier 1;
+// `buf`: 2 x 128 floats and more.
+template <typename T>
+__device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Piece& x, int M, int row, int lim, float* buf, bool direct, long long slot, int threads) {
+	const int tid = threadIdx.x % 128, lane = tid & 31, warp = tid >> 5, w = x.t * M + row, P = 1 << a.c.shift;
+	const T* q = reinterpret_cast<const T*>(a.q) + (long long) (x.row0 + w / a.rep) * a.q_row + (x.g * a.rep + w % a.rep) * a.c.d;
+	const int first = x.j0 * KT, last = min(x.j1 * KT, lim);
+	float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
+	for (int kb = first; kb < last; kb += 128) {
+		float s = -INFINITY;
+		if (kb + tid < last) {
+			const int key = x.key0 + kb + tid, pg = page_of(a.c, a.b, x.s, key >> a.c.shift);
+			s = 0.f;
+			if (pg >= 0) {
+				const T* kk = reinterpret_cast<const T*>(a.c.k) + pg * a.c.k_page + (key & (P - 1)) * a.c.k_slot + x.g * a.c.k_head;
+				for (int i = 0; i < a.c.d; i++) s = fmaf(to_f(q[i]), to_f(kk[i]), s);
+			}
+			s *= a.scale * 1.4426950408889634f;
+		}
+		float mx = warp_max(s);
+		if (__any_sync(0xffffffffu, s != s)) mx = NAN;
+		bar_sync(1, threads);
+		if (lane == 0) buf[128 + warp] = mx;
+		bar_sync(1, threads);
+		float top = m;
+		for (int i = 0; i < 4; i++) top = top != top || buf[128 + i] != buf[128 + i] ? NAN : fmaxf(top, buf[128 + i]);
+		const float base = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : exp2f(m - base);
+		buf[tid] = exp2f(s - base);
+		bar_sync(1, threads);
+		m = top;
+		l *= f;
+		acc[0] *= f;
+		acc[1] *= f;
+		for (int i = 0; i < min(128, last - kb); i++) {
+			const int key = x.key0 + kb + i, pg = page_of(a.c, a.b, x.s, key >> a.c.shift);
+			l += buf[i];
+			if (pg < 0) continue;
+			const T* v = reinterpret_cast<const T*>(a.c.v) + pg * a.c.v_page + (key & (P - 1)) * a.c.v_slot + x.g * a.c.v_head;
+			for (int c = 0; c < 2; c++)
+				if (c * 128 + tid < a.c.dv) acc[c] = fmaf(buf[i], to_f(v[c * 128 + tid]), acc[c]);
+		}
+		bar_sync(1, threads);
+	}
+	bar_sync(1, threads);
+	for (int c = 0; c < 2; c++)
+		if (c * 128 + tid < a.c.dv) buf[c * 128 + tid] = acc[c];
+	bar_sync(1, threads);
+	for (int c = tid * 4; c < a.c.dv; c += 512) put_row<T>(a, part, x, M, row, c, *reinterpret_cast<const float4*>(buf + c), m, l, direct, slot);
+	bar_sync(1, threads);
+}
+
+} // namespace paged
+} // namespace xalm
