@@ -46,7 +46,7 @@ def _sources(d, exts):
 _ENGINE_TUS = ["mix_ops.cu", "swa_one.cu", "swa_mma.cu", "rec_chunk.cu", "delta_chunk.cu", "prefill.cu"]  # what the config.json families share
 FAMILY_TUS = {"Llama": ["xalm_cuda.cu", "attn_cluster.cu", "prefill.cu", "decode_mega.cu"],
               **{f: [f.lower() + ".cu", *_ENGINE_TUS] for f in ("Nabalix", "Bolovik", "Duletar", "Kubolorn", "Mizerax", "Pavitar")}}
-CUDA_TUS = ["abi.cu", "xalm_cuda.cu", "attn_cluster.cu", "prefill.cu", "decode_mega.cu", "nabalix.cu", "bolovik.cu", "duletar.cu", "kubolorn.cu", "mizerax.cu", "pavitar.cu", "mix_ops.cu", "swa_one.cu", "swa_mma.cu", "rec_chunk.cu", "delta_chunk.cu", "paged.cu", "paged_attn.cu", "paged_mma.cu"]
+CUDA_TUS = ["abi.cu", "xalm_cuda.cu", "attn_cluster.cu", "prefill.cu", "decode_mega.cu", "nabalix.cu", "bolovik.cu", "duletar.cu", "kubolorn.cu", "mizerax.cu", "pavitar.cu", "mix_ops.cu", "swa_one.cu", "swa_mma.cu", "rec_chunk.cu", "delta_chunk.cu", "paged.cu", "paged_attn.cu", "paged_mma.cu", "paged_tc.cu"]
 
 
 def _tus(families):

@@ -360,6 +360,8 @@ static int sm_count(int device, int* n) {
 	return XALM_OK;
 }
 
+constexpr int SMALL_ROWS = 16;
+
 // ---- attention: parts, workspace --------------------------------------------------------------------------------------------------------------
 static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchView& b, int heads, int n_lists, Attn& a, size_t* bytes) {
 	if (heads <= 0 || heads % c.G) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
@@ -372,22 +374,26 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 	a.H = heads;
 	a.rep = heads / c.G;
 	a.S = n_lists;
-	a.n_parts = 1;
+	// Two kernels divide the segments by their rows: up to 16 fill one 16-row tile, more go to tcgen05.  The second is launched only where some segment may have more.
+	const bool f32 = cache->type == XALM_F32;
+	const bool tc = !f32 && !n_lists && tc_fits(c, b) && (b.n_groups || b.N > b.B) && (long long) b.N * a.rep > SMALL_ROWS;
+	a.n_parts = tc ? 2 : 1;
 	size_t at = 0;
 	auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
 	for (int i = 0; i < a.n_parts; i++) {
 		Part& p = a.part[i];
-		p.M = 16;
-		p.grid = sms * (cache->type == XALM_F32 ? 2 : mma_ctas_per_sm(c, b, n_lists));
-		p.small_rows = 0x7fffffff;
-		p.small = p.big = p.prefix = 1;
+		const bool big = tc && i == 0;
+		p.M = big ? TC_ROWS : 16;
+		p.grid = sms * (big ? 1 : f32 ? 2 : mma_ctas_per_sm(c, b, n_lists));
+		p.least_rows = big ? SMALL_ROWS + 1 : 1;
+		p.most_rows = tc && !big ? SMALL_ROWS : 0x7fffffff;
 		const long long rows = (long long) b.N * a.rep;
-		long long units = n_lists ? (long long) b.N * ((a.rep + p.M - 1) / p.M) : rows / p.M + b.B + (b.n_groups ? rows / p.M + b.n_groups : 0);
-		units = units * c.G + p.grid;
-		if (units > 0x7fffffff / p.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
-		p.slots = (int) units;
-		p.o = (float*) take((size_t) units * p.M * c.dv * 4);
-		p.ml = (float2*) take((size_t) units * p.M * 8);
+		// a segment of `rows` rows has at most rows / M + 1 tiles, a part that takes short ones only has one
+		const long long tiles = n_lists ? (long long) b.N * ((a.rep + p.M - 1) / p.M) : (tc && !big ? 0 : rows / p.M) + b.B + (b.n_groups ? (tc && !big ? 0 : rows / p.M) + b.n_groups : 0);
+		if (tiles * c.G + p.grid > 0x7fffffff / p.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
+		p.slots = n_lists || !b.n_groups ? 2 * p.grid : (int) (tiles * c.G) + p.grid;
+		p.o = (float*) take((size_t) p.slots * p.M * c.dv * 4);
+		p.ml = (float2*) take((size_t) p.slots * p.M * 8);
 		if (!n_lists) {
 			p.cum_w = (long long*) take((size_t) (b.B + b.n_groups + 1) * 8);
 			p.cum_u = (int*) take((size_t) (b.B + b.n_groups + 1) * 4);
@@ -440,7 +446,11 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 	a.scale = scale;
 	a.lists = lists;
 	cudaStream_t s = (cudaStream_t) stream;
-	XALM_TRY(cache->type == XALM_F32 ? launch_attn_rows(a, s) : launch_attn_mma(a, cache->type, s));
+	if (cache->type == XALM_F32) XALM_TRY(launch_attn_rows(a, s));
+	else {
+		if (a.n_parts == 2) XALM_TRY(launch_attn_tc(a, 0, cache->type, s));
+		XALM_TRY(launch_attn_mma(a, a.n_parts - 1, cache->type, s));
+	}
 	return launch_join(a, cache->type, s);
 }
 

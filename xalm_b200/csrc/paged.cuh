@@ -122,8 +122,7 @@ struct Part {
 	float* o;            // (slots, M, dv): sums of exp(s - m) v
 	float2* ml;          // (slots, M): m (in units of log2), sum of exp
 	int slots, M, grid;
-	int small_rows;      // own segments of at most this many rows belong to this part when `small`, the others when `big`
-	int small, big, prefix;
+	int least_rows, most_rows; // segments of so many rows are this part's
 	long long* cum_w;    // the plan, left by CTA 0 for the join: tiles and units before each segment, keys shared by each sequence
 	int *cum_u, *shs;
 };
@@ -167,7 +166,7 @@ __device__ __forceinline__ int seg_rows(const Attn& a, int seg, int& row0, int& 
 // keys of an own segment that the rows up to `last` of it see
 __device__ __forceinline__ int own_keys(const Seq& q, int shared, int rep, int last) { return max(q.len - q.n + last / rep + 1 - shared, 0); }
 
-__device__ __forceinline__ bool in_part(const Part& p, bool prefix, int rows) { return prefix ? p.prefix : rows <= p.small_rows ? p.small : p.big; }
+__device__ __forceinline__ bool in_part(const Part& p, int rows) { return rows >= p.least_rows && rows <= p.most_rows; }
 
 // tiles of unit t of a segment
 __device__ __forceinline__ int unit_tiles(const Attn& a, const Part& part, int seg, int rows, const Seq& q, int shared, int t) {
@@ -211,7 +210,7 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 		if (seg < p.segs) {
 			int row0, s;
 			const int rows = seg_rows(a, seg, row0, s), tiles = (rows + part.M - 1) / part.M;
-			if (in_part(part, seg < n, rows) && rows) {
+			if (in_part(part, rows)) {
 				if (seg < n) w = (long long) tiles * ((p.shs[s] + KT - 1) / KT);
 				else {
 					const Seq q = seq_of(a.c, a.b, s);
@@ -272,7 +271,9 @@ struct Piece {
 	int s;               // whose table row holds the pages (SELECTED: the sequence)
 	int key0;            // position of the segment's first key
 	Seq q;
+	bool first;          // of this CTA's pieces
 };
+__device__ __forceinline__ long long piece_slot(const Attn& a, int unit, int cta, bool first) { return a.b.n_groups && !a.lists ? (long long) unit + cta : 2ll * cta + !first; }
 // The walk over a CTA's part of the tiles
 struct Walk {
 	long long at, end;   // tiles
@@ -293,6 +294,7 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, cons
 	k.at = part_begin(p.total, part.grid, blockIdx.x);
 	k.end = part_begin(p.total, part.grid, blockIdx.x + 1);
 	if (k.at >= k.end) return false;
+	k.x.first = true;
 	int lo = 0, hi = p.segs - 1; // the last segment that begins at or before k.at and is not empty
 	while (lo < hi) {
 		const int mid = (lo + hi + 1) >> 1;
@@ -332,6 +334,7 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, cons
 __device__ __forceinline__ bool walk_next(const Attn& a, const Part& part, const Plan& p, Walk& k) {
 	k.at += k.x.j1 - k.x.j0;
 	if (k.at >= k.end) return false;
+	k.x.first = false;
 	do {
 		if (++k.x.t == k.tiles) {
 			k.x.t = 0;
@@ -376,6 +379,7 @@ __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk
 	k.at = part_begin(total, part.grid, blockIdx.x);
 	k.end = part_begin(total, part.grid, blockIdx.x + 1);
 	if (k.at >= k.end) return false;
+	k.x.first = true;
 	const int w = list_tiles(a);
 	list_unit(a, part, k, k.at / w, false);
 	k.x.j0 = (int) (k.at % w);
@@ -385,6 +389,7 @@ __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk
 __device__ __forceinline__ bool list_next(const Attn& a, const Part& part, Walk& k) {
 	k.at += k.x.j1 - k.x.j0;
 	if (k.at >= k.end) return false;
+	k.x.first = false;
 	list_unit(a, part, k, k.x.u + 1, true);
 	k.x.j0 = 0;
 	k.x.j1 = (int) min((long long) k.x.w, k.end - k.at);
@@ -454,7 +459,10 @@ int launch_join(const Attn& a, int type, cudaStream_t s);
 int launch_attn_rows(const Attn& a, cudaStream_t s); // fp32 caches
 // 16-bit caches: CTAs per SM that the kernel's shared memory leaves room for
 int mma_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists);
-int launch_attn_mma(const Attn& a, int type, cudaStream_t s);
+int launch_attn_mma(const Attn& a, int part, int type, cudaStream_t s);
+constexpr int TC_ROWS = 256; // rows of a unit on tcgen05
+bool tc_fits(const Cache& c, const BatchView& b);
+int launch_attn_tc(const Attn& a, int part, int type, cudaStream_t s);
 
 } // namespace paged
 } // namespace xalm

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 			__syncthreads();
 		}
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
-		const long long slot = (long long) x.u + blockIdx.x;
+		const long long slot = piece_slot(a, x.u, blockIdx.x, x.first);
 #pragma unroll
 		for (int r = 0; r < 4; r++)
 			if (lane == 0) {
@@ -186,8 +186,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 	const int s = seq_of_row(a.b, row);
 	const Seq q = seq_of(a.c, a.b, s);
 	if (!row_in_seq(q, row)) return;
-	// pieces: (part, unit, row of the unit, first CTA, CTAs)
+	// pieces: (part, unit, row of the unit, first CTA, CTAs, whether the unit begins behind the start of its first CTA's share)
 	int which[2], unit[2], at[2], c0[2], n[2], found = 0;
+	bool starts_in[2];
 	bool direct = false;
 	for (int i = 0; i < a.n_parts; i++) {
 		const Part& p = a.part[i];
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 					seg = lo;
 				}
 				rows = seg_rows(a, seg, row0, s_first);
-				if (!in_part(p, !own, rows)) continue;
+				if (!in_part(p, rows)) continue;
 				const long long seg_w = p.cum_w[seg + 1] - p.cum_w[seg];
 				if (!seg_w) continue;
 				const int tiles = (rows + p.M - 1) / p.M;
@@ -245,6 +246,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 			if (first == last && !shared) direct = true;
 			if (found < 2) {
 				which[found] = i; unit[found] = u; at[found] = idx % p.M; c0[found] = first; n[found] = last - first + 1;
+				starts_in[found] = part_begin(total, p.grid, first) < w0; // the unit is not its first CTA's first piece
 				found++;
 			}
 		}
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 	for (int f = 0; f < found; f++) {
 		const Part& p = a.part[which[f]];
 		for (int i = lane; i < n[f]; i += 32) {
-			const long long slot = (long long) unit[f] + c0[f] + i;
+			const long long slot = piece_slot(a, unit[f], c0[f] + i, i > 0 || !starts_in[f]);
 			if (slot < p.slots) {
 				const float2 ml = p.ml[slot * p.M + at[f]];
 				m = ml.x != ml.x || m != m ? NAN : fmaxf(m, ml.x);
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 	for (int f = 0; f < found; f++) {
 		const Part& p = a.part[which[f]];
 		for (int i = 0; i < n[f]; i++) {
-			const long long slot = (long long) unit[f] + c0[f] + i;
+			const long long slot = piece_slot(a, unit[f], c0[f] + i, i > 0 || !starts_in[f]);
 			if (slot >= p.slots) continue;
 			const float2 ml = p.ml[slot * p.M + at[f]];
 			if (ml.x == -INFINITY && ml.y == 0.f) continue; // nothing that the row sees

@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		*s_dead = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 	}
-	pdl_wait();
 	pdl_launch_dependents();
 	Plan plan;
 	if (!LIST) make_plan<MT>(a, part, s_plan, plan);
@@ -155,6 +154,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		}
 		if (*(volatile int*) s_dead) // gave up: copies still on their way end first
 			for (int i = max(0, n - stages); i < n; i++) wait_some(&full[i % stages], (i / stages) & 1);
+		pdl_wait(); // beside the kernel of many rows, whose inputs were complete before it began, but not ahead of it to the join
 		return;
 	}
 
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		}
 		bar_sync(1, CW * 32);
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && x.key0 == 0;
-		const long long slot = (long long) x.u + blockIdx.x;
+		const long long slot = piece_slot(a, x.u, blockIdx.x, x.first);
 		const bool mixed = !LIST && !prefix && least < most && x.j1 * KT > least; // some row of the tile must not see what another does
 #pragma unroll
 		for (int half = 0; half < 2; half++) {
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			const bool redo = s_ml[0].x != 0.f;
 			bar_sync(1, CW * 32);
 			if (redo)
-				for (int r = 0; r < rows; r++) slow_row<T>(a, part, x, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, CW * 32);
+				for (int r = 0; r < rows; r++) slow_row<T>(a, part, x, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, tid, 1);
 		}
 		bar_sync(1, CW * 32);
 	}
@@ -370,29 +370,31 @@ int mma_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists) {
 }
 
 template <typename T, int D, bool LIST>
-static int launch_typed(const Attn& a, int type, cudaStream_t s) {
+static int launch_typed(const Attn& a, int part, int type, cudaStream_t s) {
 	const MmaConfig cfg = config_of<D>(a.c, a.b, LIST ? a.S : 0);
 	if (cfg.stages < 1) return set_error(XALM_ERR_INVALID, "paged attention: no shared memory left for pages beside %d sequences", a.b.B);
 	CUtensorMap kmap, vmap;
 	XALM_TRY(pool_map(a.c, type, true, &kmap));
 	XALM_TRY(pool_map(a.c, type, false, &vmap));
 	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_mma_kernel<T, D, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) cfg.smem));
-	XALM_CUDA_CHECK(launch(paged_mma_kernel<T, D, LIST>, a.part[0].grid, MT, cfg.smem, s, false, a, a.part[0], kmap, vmap, cfg.stages));
+	XALM_CUDA_CHECK(launch(paged_mma_kernel<T, D, LIST>, a.part[part].grid, MT, cfg.smem, s, part > 0, a, a.part[part], kmap, vmap, cfg.stages));
 	return XALM_OK;
 }
 template <typename T, int D>
-static int launch_lists(const Attn& a, int type, cudaStream_t s) {
-	return a.lists ? launch_typed<T, D, true>(a, type, s) : launch_typed<T, D, false>(a, type, s);
+static int launch_lists(const Attn& a, int part, int type, cudaStream_t s) {
+	return a.lists ? launch_typed<T, D, true>(a, part, type, s) : launch_typed<T, D, false>(a, part, type, s);
 }
 template <typename T>
-static int launch_size(const Attn& a, int type, cudaStream_t s) {
+static int launch_size(const Attn& a, int part, int type, cudaStream_t s) {
 	switch (padded(a.c)) {
-		case 64: return launch_lists<T, 64>(a, type, s);
-		case 128: return launch_lists<T, 128>(a, type, s);
-		default: return launch_lists<T, 256>(a, type, s);
+		case 64: return launch_lists<T, 64>(a, part, type, s);
+		case 128: return launch_lists<T, 128>(a, part, type, s);
+		default: return launch_lists<T, 256>(a, part, type, s);
 	}
 }
-int launch_attn_mma(const Attn& a, int type, cudaStream_t s) { return type == XALM_F16 ? launch_size<__half>(a, type, s) : launch_size<__nv_bfloat16>(a, type, s); }
+int launch_attn_mma(const Attn& a, int part, int type, cudaStream_t s) {
+	return type == XALM_F16 ? launch_size<__half>(a, part, type, s) : launch_size<__nv_bfloat16>(a, part, type, s);
+}
 
 } // namespace paged
 } // namespace xalm

@@ -1,0 +1,415 @@
+// paged_tc.cu — attention over paged caches of 16-bit elements, for many rows: what a group of sequences has in common, prompts and their continuations.
+#include "paged.cuh"
+#include "paged_tma.cuh"
+
+namespace xalm {
+namespace paged {
+
+// =========================================================================================================================================
+// The same sums as paged_mma_kernel for 256 (token, head) rows at a time, two halves of 128: S = Q K^T and O += P V by tcgen05 with S, P and O in tensor memory.
+// One warp brings tiles of 64 keys and of 64 values by TMA, each read once for both halves; one issues the products; four warps to a half turn S into P, a row to a
+// thread.  At 128 channels a tile of a half takes the tensor pipe 256 cycles and the exponential unit 512 / 2 — neither waits for the other as long as the halves take turns, and one
+// load of keys and values for 256 rows asks L2 for 32 bytes a cycle where 128 rows would ask for 64.
+// P lies in tensor memory where S lay (its first 32 columns), two S buffers to a half: the scores of the next tile are under way while this one's are worked on.
+// O accumulates unscaled and is rescaled only when a row's maximum has grown by more than 2^11.5 over the one its probabilities are taken against (fp16 holds those).
+// V comes with its entries as the fast dimension, which the second product reads as it is (B transposed).
+// Tensor memory: S of half h, buffer b at columns 128 h + 64 b; O of half h at 256 + 128 h: the whole 512 of an SM, so heads of more than 128 entries stay on mma.sync.
+// =========================================================================================================================================
+constexpr int TT = 320;            // copies, products, 2 x 4 warps of softmax
+constexpr int HALF_ROWS = 128;
+constexpr int QB = HALF_ROWS * 128; // bytes of 64 entries of a half's queries
+constexpr int KB = KT * 128;        // bytes of 64 entries of a key or value tile
+constexpr int RING = 4;
+
+__device__ __forceinline__ bool elect() {
+	uint32_t pred;
+	asm volatile(
+	    "{\n"
+	    ".reg .pred p;\n"
+	    "elect.sync _|p, 0xffffffff;\n"
+	    "selp.u32 %0, 1, 0, p;\n"
+	    "}\n"
+	    : "=r"(pred));
+	return pred != 0;
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// D (+)= A B^T with A from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+	asm volatile(
+	    "{\n"
+	    ".reg .pred p;\n"
+	    "setp.ne.b32 p, %4, 0;\n"
+	    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+	    "}\n" ::"r"(d),
+	    "l"(a), "l"(b), "r"(idesc), "r"(add)
+	    : "memory");
+}
+// with A from tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+	asm volatile(
+	    "{\n"
+	    ".reg .pred p;\n"
+	    "setp.ne.b32 p, %4, 0;\n"
+	    "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+	    "}\n" ::"r"(d),
+	    "r"(a), "l"(b), "r"(idesc), "r"(add)
+	    : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+	asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// 128-byte swizzle.  Fast dimension = the summed one: 8-row groups 1024 bytes apart.  Fast dimension = the output's columns: groups of 8 summed rows 1024 bytes apart,
+// blocks of 64 columns `block` bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t at) { return (uint64_t) ((at & 0x3FFFFu) >> 4) | ((uint64_t) (1024 >> 4) << 32) | (1ull << 46) | (2ull << 61); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t at, uint32_t block) { return desc_k(at) | ((uint64_t) (block >> 4) << 16); }
+template <typename T>
+__device__ __forceinline__ uint32_t instr(int n, bool b_transposed) {
+	const uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
+	return (1u << 4) | (f << 7) | (f << 10) | ((b_transposed ? 1u : 0u) << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (HALF_ROWS >> 4) << 24);
+}
+#define XALM_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+__device__ __forceinline__ void ld32(uint32_t at, uint32_t* r) {
+	asm volatile(
+	    "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+	    "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+	    : XALM_R8(r, 0), XALM_R8(r, 8), XALM_R8(r, 16), XALM_R8(r, 24)
+	    : "r"(at));
+}
+#undef XALM_R8
+// The loads issued so far have landed in these registers: none of them is used ahead of the wait
+#define XALM_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void wait_ld(uint32_t* r) {
+	asm volatile("tcgen05.wait::ld.sync.aligned;" : XALM_RW8(r, 0), XALM_RW8(r, 8), XALM_RW8(r, 16), XALM_RW8(r, 24)::"memory");
+}
+#undef XALM_RW8
+#define XALM_R8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void st32(uint32_t at, const uint32_t* r) {
+	asm volatile(
+	    "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+	    "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n" ::XALM_R8(r, 0),
+	    XALM_R8(r, 8), XALM_R8(r, 16), XALM_R8(r, 24), "r"(at)
+	    : "memory");
+}
+#undef XALM_R8
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair16(float lo, float hi) {
+	if constexpr (std::is_same<T, __half>::value) {
+		const __half2 h = __floats2half2_rn(lo, hi);
+		return *reinterpret_cast<const uint32_t*>(&h);
+	} else {
+		const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+		return *reinterpret_cast<const uint32_t*>(&h);
+	}
+}
+
+// A piece as the three kinds of warps see it
+struct TcPiece {
+	bool prefix;
+	int rows, most, j1; // rows of the unit, keys that its last row sees, last tile of the piece that any row sees
+};
+__device__ __forceinline__ TcPiece tc_piece(const Attn& a, const Plan& plan, const Piece& x) {
+	TcPiece p;
+	p.prefix = x.seg < a.b.n_groups;
+	p.rows = min(TC_ROWS, x.rows - x.t * TC_ROWS);
+	p.most = p.prefix ? plan.shs[x.s] : own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + p.rows - 1);
+	p.j1 = min(x.j1, (p.most + KT - 1) / KT);
+	return p;
+}
+
+struct TcShared {
+	uint64_t k_full[RING], k_empty[RING], v_full[RING], v_empty[RING];
+	uint64_t q_full[2], s_full[2][2], p_full[2], o_full[2];
+	uint32_t tmem;
+	int dead, flag[2];
+	float buf[2][256];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const __grid_constant__ CUtensorMap kmap,
+                                                         const __grid_constant__ CUtensorMap vmap) {
+	extern __shared__ uint8_t raw[];
+	uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+	uint8_t* s_q = smem;                       // [half][2 blocks][128 rows][128 bytes]
+	uint8_t* s_k = s_q + 4 * QB;               // [RING][2 blocks][64 keys][128 bytes]
+	uint8_t* s_v = s_k + RING * 2 * KB;
+	TcShared& sh = *reinterpret_cast<TcShared*>(s_v + RING * 2 * KB);
+	uint8_t* s_plan = reinterpret_cast<uint8_t*>(&sh + 1);
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	if (tid == 0) {
+		for (int i = 0; i < RING; i++) { mbar_init(&sh.k_full[i], 1); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1); }
+		for (int h = 0; h < 2; h++) {
+			mbar_init(&sh.q_full[h], 4); mbar_init(&sh.p_full[h], 4); mbar_init(&sh.o_full[h], 1);
+			mbar_init(&sh.s_full[h][0], 1); mbar_init(&sh.s_full[h][1], 1);
+		}
+		sh.dead = 0;
+		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+	}
+	if (warp == 1) {
+		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
+		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+	}
+	pdl_launch_dependents();
+	Plan plan;
+	make_plan<TT>(a, part, s_plan, plan);
+	fence_before();
+	__syncthreads();
+	fence_after();
+	const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+	const int dc = (a.c.d + 63) / 64, vc = (a.c.dv + 63) / 64, P = 1 << a.c.shift, W = min(P, KT), per = KT / W;
+	Walk k;
+	bool more = walk_begin(a, part, plan, k);
+	int n = 0; // tiles so far
+
+	if (warp == 0) { // ---- copies ----
+		for (; more; more = walk_next(a, part, plan, k)) {
+			const Piece& x = k.x;
+			const TcPiece p = tc_piece(a, plan, x);
+			int id = -1;
+			for (int j = x.j0, e = 0; j < p.j1; j++, e += per, n++) {
+				if ((e & 31) == 0) {
+					const int at = x.j0 * KT + (e + lane) * W;
+					id = -1;
+					if (at < p.most) {
+						id = page_of(a.c, a.b, x.s, (x.key0 + at) >> a.c.shift);
+						if (id < 0) report(a.c, ERR_PAGE);
+					}
+				}
+				const int st = n % RING, part_of = lane % per, block = lane / per;
+				const int pg = __shfl_sync(0xffffffffu, id, (e + part_of) & 31), page = pg < 0 ? a.c.pages : pg;
+				const int slot = (x.key0 + j * KT + part_of * W) & (P - 1);
+				if (!wait_for(&sh.k_empty[st], ((n / RING) & 1) ^ 1, &sh.dead, a.c)) break;
+				if (lane == 0) mbar_expect_tx(&sh.k_full[st], (uint32_t) (dc * KB));
+				__syncwarp();
+				if (block < dc) copy_box(s_k + (st * 2 + block) * KB + part_of * W * 128, &kmap, block * 64, slot, x.g, page, &sh.k_full[st]);
+				__syncwarp();
+				if (!wait_for(&sh.v_empty[st], ((n / RING) & 1) ^ 1, &sh.dead, a.c)) { n++; break; }
+				if (lane == 0) mbar_expect_tx(&sh.v_full[st], (uint32_t) (vc * KB));
+				__syncwarp();
+				if (block < vc) copy_box(s_v + (st * 2 + block) * KB + part_of * W * 128, &vmap, block * 64, slot, x.g, page, &sh.v_full[st]);
+				__syncwarp();
+			}
+			if (*(volatile int*) &sh.dead) break;
+		}
+		if (*(volatile int*) &sh.dead) // gave up: copies still on their way end first
+			for (int i = max(0, n - RING); i < n; i++) {
+				wait_some(&sh.k_full[i % RING], (i / RING) & 1);
+				wait_some(&sh.v_full[i % RING], (i / RING) & 1);
+			}
+	} else if (warp == 1) { // ---- products ----
+		const int kd = (a.c.d + 15) / 16, nv = (a.c.dv + 15) / 16 * 16;
+		const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>(nv, true);
+		const uint32_t q_at = smem_u32(s_q), k_at = smem_u32(s_k), v_at = smem_u32(s_v);
+		int pieces = 0, count[2] = {0, 0}; // pieces with tiles, tiles of each half
+		bool ok = true;
+		for (; more && ok; more = walk_next(a, part, plan, k)) {
+			const Piece& x = k.x;
+			const TcPiece p = tc_piece(a, plan, x);
+			if (p.j1 <= x.j0) continue;
+			const int halves = p.rows > HALF_ROWS ? 2 : 1;
+			auto scores = [&](int m, int h, int buffer) { // tile m's, of half h
+				if (elect()) {
+					for (int s = 0; s < kd; s++)
+						mma_ss(tmem + 128 * h + 64 * buffer, desc_k(q_at + (h * 2 + (s >> 2)) * QB) + 2 * (s & 3), desc_k(k_at + ((m % RING) * 2 + (s >> 2)) * KB) + 2 * (s & 3), id_s, s != 0);
+					commit(&sh.s_full[h][buffer]);
+					if (h == halves - 1) commit(&sh.k_empty[m % RING]);
+				}
+				__syncwarp();
+			};
+			ok = ok && wait_for(&sh.q_full[0], pieces & 1, &sh.dead, a.c) && wait_for(&sh.q_full[1], pieces & 1, &sh.dead, a.c) &&
+			     wait_for(&sh.k_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
+			if (!ok) break;
+			pieces++;
+			fence_after();
+			for (int h = 0; h < halves; h++) scores(n, h, count[h] & 1);
+			for (int j = x.j0; j < p.j1 && ok; j++, n++) {
+				if (j + 1 < p.j1) ok = ok && wait_for(&sh.k_full[(n + 1) % RING], ((n + 1) / RING) & 1, &sh.dead, a.c);
+				ok = ok && wait_for(&sh.v_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
+				for (int h = 0; h < halves && ok; h++) {
+					fence_after();
+					if (j + 1 < p.j1) scores(n + 1, h, (count[h] + 1) & 1); // its buffer's P went into a product issued before
+					ok = wait_for(&sh.p_full[h], count[h] & 1, &sh.dead, a.c);
+					if (!ok) break;
+					fence_after();
+					if (elect()) {
+						for (int s = 0; s < KT / 16; s++)
+							mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 64 * (count[h] & 1) + 8 * s, desc_mn(v_at + (n % RING) * 2 * KB + s * 2048, KB), id_o, j != x.j0 || s != 0);
+						commit(&sh.o_full[h]);
+						if (h == halves - 1) commit(&sh.v_empty[n % RING]);
+					}
+					__syncwarp();
+					count[h]++;
+				}
+			}
+		}
+	} else { // ---- softmax ----
+		const int h = warp < 6 ? 0 : 1, quad = warp & 3, r = quad * 32 + lane, wt = (warp - 2 - 4 * h) * 32 + lane; // row of the half: the tensor memory lanes that this warp may read
+		const uint32_t lanes = (uint32_t) (quad * 32) << 16, t_o = tmem + 256 + 128 * h + lanes;
+		const bool negative = a.scale < 0.f;
+		const float c1 = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f; // a negative scale turns the queries' signs
+		int done = 0, tiles = 0; // tiles of this half, of the CTA
+		for (; more; more = walk_next(a, part, plan, k)) {
+			const Piece& x = k.x;
+			const TcPiece p = tc_piece(a, plan, x);
+			const bool direct = x.j0 == 0 && x.j1 == x.w && !p.prefix && x.key0 == 0, here = h * HALF_ROWS < p.rows;
+			const long long slot = piece_slot(a, x.u, blockIdx.x, x.first);
+			const int row = h * HALF_ROWS + r, w = x.t * TC_ROWS + row;
+			const bool mine = row < p.rows;
+			const long long token = x.row0 + w / a.rep;
+			const int head = x.g * a.rep + w % a.rep;
+			float m = -INFINITY, l = 0.f;
+			int lim = 0, least = 0;
+			if (p.j1 > x.j0) {
+				for (int c = 0; c < dc * 8; c++) {
+					uint4 v = make_uint4(0, 0, 0, 0);
+					if (mine && c * 8 < a.c.d) v = *reinterpret_cast<const uint4*>(a.q + (token * a.q_row + head * a.c.d + c * 8) * 2);
+					if (negative) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
+					*reinterpret_cast<uint4*>(s_q + (h * 2 + (c >> 3)) * QB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+				}
+				asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+				__syncwarp();
+				if (lane == 0) mbar_arrive(&sh.q_full[h]);
+				if (p.prefix) lim = least = p.most;
+				else {
+					least = own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + min(h * HALF_ROWS, p.rows - 1));
+					lim = own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + min(row, p.rows - 1));
+				}
+			}
+			for (int j = x.j0; j < p.j1; j++, tiles++) {
+				if (!here) continue;
+				const int b = done & 1, base = j * KT;
+				const uint32_t t_s = tmem + 128 * h + 64 * b + lanes;
+				if (!wait_for(&sh.s_full[h][b], (done >> 1) & 1, &sh.dead, a.c)) break;
+				fence_after();
+				uint32_t s[KT];
+				ld32(t_s, s);
+				ld32(t_s + 32, s + 32);
+				if (base + KT > p.most) { // slots that no row sees may hold anything: as zeros they add nothing
+					if (!wait_for(&sh.v_full[tiles % RING], (tiles / RING) & 1, &sh.dead, a.c)) break;
+					for (int i = wt; i < (base + KT - p.most) * vc * 8; i += 128) {
+						const int rr = p.most - base + i / (vc * 8), c = i % (vc * 8);
+						*reinterpret_cast<uint4*>(s_v + ((tiles % RING) * 2 + (c >> 3)) * KB + rr * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+					}
+					asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+				}
+				__syncwarp();
+				wait_ld(s);
+				wait_ld(s + 32);
+				float mx = -INFINITY;
+				if (base + KT > least) {
+#pragma unroll
+					for (int i = 0; i < KT; i++)
+						if (base + i >= lim) s[i] = 0xff800000u;
+				}
+#pragma unroll
+				for (int i = 0; i < KT; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
+				mx *= c1;
+				const bool grow = mx > m + 11.5f;
+				if (j == x.j0) m = mx;
+				else if (__any_sync(0xffffffffu, grow)) { // rare: the sums so far are complete before they are rescaled
+					if (!wait_for(&sh.o_full[h], (done - 1) & 1, &sh.dead, a.c)) break;
+					fence_after();
+					const float to = grow ? mx : m, f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
+#pragma unroll
+					for (int c = 0; c < 4; c++)
+						if (c * 32 < a.c.dv) {
+							uint32_t o[32];
+							ld32(t_o + 32 * c, o);
+							wait_ld(o);
+#pragma unroll
+							for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+							st32(t_o + 32 * c, o);
+						}
+					wait_st();
+					l *= f;
+					m = to;
+				}
+				const float nm = m == -INFINITY ? 0.f : -m;
+				float sum = 0.f;
+				uint32_t q[KT / 2];
+#pragma unroll
+				for (int i = 0; i < KT / 2; i++) {
+					const float p0 = exp2_approx(fmaf(__uint_as_float(s[2 * i]), c1, nm)), p1 = exp2_approx(fmaf(__uint_as_float(s[2 * i + 1]), c1, nm));
+					sum += p0 + p1;
+					q[i] = pair16<T>(p0, p1);
+				}
+				l += sum;
+				st32(t_s, q);
+				wait_st();
+				fence_before();
+				__syncwarp();
+				if (lane == 0) mbar_arrive(&sh.p_full[h]);
+				done++;
+			}
+			if (p.j1 > x.j0 && here) wait_for(&sh.o_full[h], (done - 1) & 1, &sh.dead, a.c);
+			fence_after();
+			bool again = false;
+			if (here) {
+#pragma unroll
+				for (int c = 0; c < 4; c++)
+					if (c * 32 < a.c.dv) {
+						uint32_t o[32];
+#pragma unroll
+						for (int i = 0; i < 32; i++) o[i] = 0;
+						__syncwarp();
+						if (p.j1 > x.j0) {
+							ld32(t_o + 32 * c, o);
+							wait_ld(o);
+						}
+#pragma unroll
+						for (int i = 0; i < 32; i += 4)
+							if (mine && c * 32 + i < a.c.dv) {
+								const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+								put_row<T>(a, part, x, TC_ROWS, row, c * 32 + i, v, m, l, direct, slot);
+								again = again || !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f);
+							}
+					}
+				fence_before();
+				if (!p.prefix && p.j1 > x.j0 && x.j1 * KT > least && least < p.most) {
+					// A value that is not finite and that only later rows see has met probabilities of zero: those rows are done again, key by key
+					if (wt == 0) sh.flag[h] = 0;
+					bar_sync(2 + h, 128);
+					if (again) sh.flag[h] = 1;
+					bar_sync(2 + h, 128);
+					const bool redo = *(volatile int*) &sh.flag[h] != 0;
+					bar_sync(2 + h, 128);
+					if (redo)
+						for (int i = h * HALF_ROWS; i < min(p.rows, (h + 1) * HALF_ROWS); i++)
+							slow_row<T>(a, part, x, TC_ROWS, i, own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + i), sh.buf[h], direct, slot, wt, 2 + h);
+				}
+			}
+		}
+	}
+	fence_before();
+	__syncthreads();
+	if (warp == 1) {
+		fence_after();
+		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+	}
+}
+
+static size_t tc_smem(const BatchView& b) { return 1024 + 4 * QB + 4 * RING * KB + sizeof(TcShared) + plan_bytes(b.B, b.n_groups); }
+bool tc_fits(const Cache& c, const BatchView& b) { return c.d <= 128 && c.dv <= 128 && tc_smem(b) <= 226 * 1024; }
+
+template <typename T>
+static int launch_typed(const Attn& a, int part, int type, cudaStream_t s) {
+	CUtensorMap kmap, vmap;
+	XALM_TRY(pool_map(a.c, type, true, &kmap));
+	XALM_TRY(pool_map(a.c, type, false, &vmap));
+	const size_t smem = tc_smem(a.b);
+	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	XALM_CUDA_CHECK(launch(paged_tc_kernel<T>, a.part[part].grid, TT, smem, s, false, a, a.part[part], kmap, vmap));
+	return XALM_OK;
+}
+int launch_attn_tc(const Attn& a, int part, int type, cudaStream_t s) {
+	return type == XALM_F16 ? launch_typed<__half>(a, part, type, s) : launch_typed<__nv_bfloat16>(a, part, type, s);
+}
+
+} // namespace paged
+} // namespace xalm

@@ -89,11 +89,11 @@ __device__ __forceinline__ void put_row(const Attn& a, const Part& part, const P
 	}
 }
 
-// One row of a piece by fp32 FMAs, with only the keys that it sees: for rows that a value which is not finite has spoilt.  `threads` (128) threads of barrier 1;
-// `buf`: 2 x 128 floats and more.
+// One row of a piece by fp32 FMAs, with only the keys that it sees: for rows that a value which is not finite has spoilt.  128 threads, which share
+// barrier `bar`; `buf`: 256 floats.
 template <typename T>
-__device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Piece& x, int M, int row, int lim, float* buf, bool direct, long long slot, int threads) {
-	const int tid = threadIdx.x % 128, lane = tid & 31, warp = tid >> 5, w = x.t * M + row, P = 1 << a.c.shift;
+__device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Piece& x, int M, int row, int lim, float* buf, bool direct, long long slot, int tid, int bar) {
+	const int lane = tid & 31, warp = tid >> 5, w = x.t * M + row, P = 1 << a.c.shift;
 	const T* q = reinterpret_cast<const T*>(a.q) + (long long) (x.row0 + w / a.rep) * a.q_row + (x.g * a.rep + w % a.rep) * a.c.d;
 	const int first = x.j0 * KT, last = min(x.j1 * KT, lim);
 	float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
@@ -110,14 +110,14 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 		}
 		float mx = warp_max(s);
 		if (__any_sync(0xffffffffu, s != s)) mx = NAN;
-		bar_sync(1, threads);
+		bar_sync(bar, 128);
 		if (lane == 0) buf[128 + warp] = mx;
-		bar_sync(1, threads);
+		bar_sync(bar, 128);
 		float top = m;
 		for (int i = 0; i < 4; i++) top = top != top || buf[128 + i] != buf[128 + i] ? NAN : fmaxf(top, buf[128 + i]);
 		const float base = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : exp2f(m - base);
 		buf[tid] = exp2f(s - base);
-		bar_sync(1, threads);
+		bar_sync(bar, 128);
 		m = top;
 		l *= f;
 		acc[0] *= f;
@@ -130,14 +130,14 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 			for (int c = 0; c < 2; c++)
 				if (c * 128 + tid < a.c.dv) acc[c] = fmaf(buf[i], to_f(v[c * 128 + tid]), acc[c]);
 		}
-		bar_sync(1, threads);
+		bar_sync(bar, 128);
 	}
-	bar_sync(1, threads);
+	bar_sync(bar, 128);
 	for (int c = 0; c < 2; c++)
 		if (c * 128 + tid < a.c.dv) buf[c * 128 + tid] = acc[c];
-	bar_sync(1, threads);
+	bar_sync(bar, 128);
 	for (int c = tid * 4; c < a.c.dv; c += 512) put_row<T>(a, part, x, M, row, c, *reinterpret_cast<const float4*>(buf + c), m, l, direct, slot);
-	bar_sync(1, threads);
+	bar_sync(bar, 128);
 }
 
 } // namespace paged
