@@ -563,6 +563,40 @@ def test_calls_repeat_themselves_bit_for_bit():
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_many_rows_many_times(type):
+    """Groups of all sizes around the tensor-core units' halves, long enough for several pieces to a CTA; every repetition the same, and no wait that gave up."""
+    g = torch.Generator().manual_seed(44)
+    sizes = [64, 33, 5, 31, 70]
+    bounds = [0]
+    for n in sizes:
+        bounds.append(bounds[-1] + n)
+    shared = [64 * n for n in (90, 31, 200, 64, 17)]
+    lens = [shared[i] + int(torch.randint(1, 400, (1,), generator=g)) for i, n in enumerate(sizes) for _ in range(n)]
+    B, G, d, page = bounds[-1], 4, 128, 64
+    width, pages = max(-(-n // page) for n in lens), 2000
+    gg = torch.Generator(device="cuda").manual_seed(45)
+    k, v = (torch.randn(pages, page, G, d, generator=gg, device="cuda").to(TYPES[type]) for _ in range(2))
+    table = torch.randint(0, pages, (B, width), generator=gg, device="cuda", dtype=torch.int32)
+    for i in range(len(sizes)):
+        table[bounds[i]:bounds[i + 1], :shared[i] // page] = table[bounds[i], :shared[i] // page]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cache = paged.PagedCache(k, v)
+    q = torch.randn(B, 4 * G, d, generator=gg, device="cuda").to(TYPES[type])
+    alone = paged.Batch(i32(range(B + 1)), i32(lens), table)
+    together = paged.Batch(i32(range(B + 1)), i32(lens), table, groups=i32(bounds), shared=i32(shared))
+    want, want_lse = paged.attend(cache, alone, q, d ** -0.5, want_lse=True)
+    first, first_lse = paged.attend(cache, together, q, d ** -0.5, want_lse=True)
+    cache.check()
+    # two ways of the same sums: each rounds every probability once and the result once
+    spread = 2 * HALF[type] * float(v.abs().max())
+    assert float((first.float() - want.float()).abs().max()) < spread and float((first_lse - want_lse).abs().max()) < 1e-4
+    for _ in range(300):
+        out, lse = paged.attend(cache, together, q, d ** -0.5, want_lse=True)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)
+    cache.check()
+
+
 def test_a_workspace_too_small_is_refused():
     import ctypes as C
     p = Problem("bf16", [1], [100], d=64, page=16, seed=43)

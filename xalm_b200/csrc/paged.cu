@@ -361,6 +361,7 @@ static int sm_count(int device, int* n) {
 }
 
 constexpr int SMALL_ROWS = 16;
+constexpr int LEAD = 2, LEAD_TC = 4;
 
 // ---- attention: parts, workspace --------------------------------------------------------------------------------------------------------------
 static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchView& b, int heads, int n_lists, Attn& a, size_t* bytes) {
@@ -385,6 +386,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		const bool big = tc && i == 0;
 		p.M = big ? TC_ROWS : 16;
 		p.grid = sms * (big ? 1 : f32 ? 2 : mma_ctas_per_sm(c, b, n_lists));
+		p.lead = big ? LEAD_TC : LEAD;
 		p.least_rows = big ? SMALL_ROWS + 1 : 1;
 		p.most_rows = tc && !big ? SMALL_ROWS : 0x7fffffff;
 		const long long rows = (long long) b.N * a.rep;

@@ -14,6 +14,8 @@ namespace paged {
 constexpr int KT = 64;              // keys of a tile, the unit in which attention counts its work
 constexpr int MAX_SEGMENTS = 4096;  // sequences and groups of one call: the plan lies in shared memory
 constexpr int MAX_LIST = 1024;      // pages that a list of attend_selected names
+// Sequences of more rows than this on average fill units of their own: reading the shared pages once for each of them costs less than joining two results of every row
+constexpr int ALONE_ROWS = 128;
 constexpr int ERR_PAGE = 1, ERR_BATCH = 2, ERR_WAIT = 4; // bits of the cache's status word
 
 struct Cache {
@@ -121,7 +123,7 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 struct Part {
 	float* o;            // (slots, M, dv): sums of exp(s - m) v
 	float2* ml;          // (slots, M): m (in units of log2), sum of exp
-	int slots, M, grid;
+	int slots, M, grid, lead;
 	int least_rows, most_rows; // segments of so many rows are this part's
 	long long* cum_w;    // the plan, left by CTA 0 for the join: tiles and units before each segment, keys shared by each sequence
 	int *cum_u, *shs;
@@ -144,11 +146,13 @@ struct Plan {
 	long long* cum_w; // segments + 1
 	int *cum_u, *shs;
 	int segs;
-	long long total;
+	long long total, share;
 };
 __host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (B + n_groups + 1) * 12 + (size_t) B * 4 + 32 * 12 + 16; }
 
-// rows of a segment and the tiles of its unit t
+__host__ __device__ __forceinline__ long long share_of(long long total, int grid) { return (total + grid - 1) / grid; }
+
+// rows of a segment, its first row and sequence
 __device__ __forceinline__ int seg_rows(const Attn& a, int seg, int& row0, int& s_first) {
 	if (seg < a.b.n_groups) {
 		const int s0 = min(max(a.b.bounds[seg], 0), a.b.B), s1 = min(max(a.b.bounds[seg + 1], s0), a.b.B);
@@ -174,7 +178,13 @@ __device__ __forceinline__ int unit_tiles(const Attn& a, const Part& part, int s
 	return (own_keys(q, shared, a.rep, min((t + 1) * part.M, rows) - 1) + KT - 1) / KT;
 }
 
-// All threads of the CTA.  Shared keys of each group (whole pages, and no more than every row of its sequences sees; a group of one sequence has none),
+// its work: nothing, or its tiles behind `lead`
+__device__ __forceinline__ int unit_work(const Attn& a, const Part& part, int seg, int rows, const Seq& q, int shared, int t) {
+	const int w = unit_tiles(a, part, seg, rows, q, shared, t);
+	return w ? w + part.lead : 0;
+}
+
+// All threads of the CTA.  Shared keys of each group (whole pages, and no more than every row of its sequences sees; a group of one sequence, or of sequences with many rows each, has none),
 // then a running sum over the segments.
 template <int NT>
 __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& p) {
@@ -190,6 +200,8 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 	for (int i = warp; i < n; i += NT / 32) {
 		const int s0 = min(max(a.b.bounds[i], 0), B), s1 = min(max(a.b.bounds[i + 1], s0), B);
 		if (s1 - s0 < 2) continue;
+		const Seq last = seq_of(a.c, a.b, s1 - 1);
+		if ((long long) (last.a + last.n - seq_of(a.c, a.b, s0).a) * a.rep > (long long) (s1 - s0) * ALONE_ROWS) continue;
 		int m = max(a.b.shared[i], 0);
 		for (int s = s0 + lane; s < s1; s += 32) {
 			const Seq q = seq_of(a.c, a.b, s);
@@ -211,11 +223,11 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 			int row0, s;
 			const int rows = seg_rows(a, seg, row0, s), tiles = (rows + part.M - 1) / part.M;
 			if (in_part(part, rows)) {
-				if (seg < n) w = (long long) tiles * ((p.shs[s] + KT - 1) / KT);
+				if (seg < n) w = (long long) tiles * unit_work(a, part, seg, rows, Seq(), p.shs[s], 0);
 				else {
 					const Seq q = seq_of(a.c, a.b, s);
 					if (tiles <= 4) {
-						for (int t = 0; t < tiles; t++) w += unit_tiles(a, part, seg, rows, q, p.shs[s], t);
+						for (int t = 0; t < tiles; t++) w += unit_work(a, part, seg, rows, q, p.shs[s], t);
 					} else wide = true;
 					if (part.cum_w && blockIdx.x == 0 && !seq_ok(a.c, a.b, s)) report(a.c, ERR_BATCH);
 				}
@@ -226,7 +238,7 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 			const int from = __ffs(m) - 1, wseg = base + (tid & ~31) + from, n_tiles = __shfl_sync(0xffffffffu, in_seg, from);
 			const Seq q = seq_of(a.c, a.b, wseg - n);
 			long long sum = 0;
-			for (int t = lane; t < n_tiles; t += 32) sum += unit_tiles(a, part, wseg, q.n * a.rep, q, p.shs[wseg - n], t);
+			for (int t = lane; t < n_tiles; t += 32) sum += unit_work(a, part, wseg, q.n * a.rep, q, p.shs[wseg - n], t);
 #pragma unroll
 			for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 			if (lane == from) w = sum;
@@ -249,17 +261,11 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 		__syncthreads();
 	}
 	p.total = p.cum_w[p.segs];
+	p.share = share_of(p.total, part.grid);
 	if (part.cum_w && blockIdx.x == 0) {
 		for (int i = tid; i <= p.segs; i += NT) { part.cum_w[i] = p.cum_w[i]; part.cum_u[i] = p.cum_u[i]; }
 		for (int i = tid; i < B; i += NT) part.shs[i] = p.shs[i];
 	}
-}
-
-// First tile of a CTA's share.  Fewer tiles than CTAs: one to each of the first CTAs, so that no share between two others is empty.
-__device__ __forceinline__ int shares(long long total, int grid) { return (int) min(total, (long long) grid); }
-__device__ __forceinline__ long long part_begin(long long total, int grid, int cta) {
-	const int n = shares(total, grid);
-	return cta >= n ? total : total * cta / n;
 }
 
 // One unit of a CTA's walk, with what both its producer and its consumers need to know of it
@@ -271,12 +277,11 @@ struct Piece {
 	int s;               // whose table row holds the pages (SELECTED: the sequence)
 	int key0;            // position of the segment's first key
 	Seq q;
-	bool first;          // of this CTA's pieces
 };
-__device__ __forceinline__ long long piece_slot(const Attn& a, int unit, int cta, bool first) { return a.b.n_groups && !a.lists ? (long long) unit + cta : 2ll * cta + !first; }
-// The walk over a CTA's part of the tiles
+__device__ __forceinline__ long long piece_slot(const Attn& a, int unit, int cta, bool begins) { return a.b.n_groups && !a.lists ? (long long) unit + cta : 2ll * cta + begins; }
+// The walk over a CTA's share of the work
 struct Walk {
-	long long at, end;   // tiles
+	long long at, end;
 	Piece x;
 	int tiles;           // row tiles of the segment
 };
@@ -286,16 +291,19 @@ __device__ __forceinline__ void walk_segment(const Attn& a, const Part& part, co
 	k.x.q = seq_of(a.c, a.b, k.x.s);
 	k.x.key0 = k.x.seg < a.b.n_groups ? 0 : p.shs[k.x.s];
 }
-__device__ __forceinline__ int walk_tiles(const Attn& a, const Part& part, const Plan& p, const Walk& k) {
-	return unit_tiles(a, part, k.x.seg, k.x.rows, k.x.q, p.shs[k.x.s], k.x.t);
+// The piece of the unit at k.at, `in` of whose work lies behind the share's start; the walk's place moves behind it
+__device__ __forceinline__ void walk_piece(const Part& part, Walk& k, long long in) {
+	const long long left = k.x.w + part.lead - in, take = min(left, k.end - k.at); // tiles lie behind the lead
+	k.x.j0 = (int) max(in - part.lead, 0ll);
+	k.x.j1 = (int) max(in + take - part.lead, 0ll);
+	k.at += take;
 }
 // false: nothing for this CTA
 __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, const Plan& p, Walk& k) {
-	k.at = part_begin(p.total, part.grid, blockIdx.x);
-	k.end = part_begin(p.total, part.grid, blockIdx.x + 1);
+	k.at = min(p.share * blockIdx.x, p.total);
+	k.end = min(k.at + p.share, p.total);
 	if (k.at >= k.end) return false;
-	k.x.first = true;
-	int lo = 0, hi = p.segs - 1; // the last segment that begins at or before k.at and is not empty
+	int lo = 0, hi = p.segs - 1; // the last segment that begins at or before k.at
 	while (lo < hi) {
 		const int mid = (lo + hi + 1) >> 1;
 		if (p.cum_w[mid] <= k.at) lo = mid;
@@ -308,8 +316,8 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, cons
 	k.x.g = (int) (rem / per);
 	rem -= per * k.x.g;
 	const int lane = threadIdx.x & 31;
-	for (int t0 = 0;; t0 += 32) { // whole warps walk: 32 units' tiles at a time
-		const int w = t0 + lane < k.tiles ? unit_tiles(a, part, lo, k.x.rows, k.x.q, p.shs[k.x.s], t0 + lane) : 0;
+	for (int t0 = 0;; t0 += 32) { // whole warps walk: 32 units at a time
+		const int w = t0 + lane < k.tiles ? unit_work(a, part, lo, k.x.rows, k.x.q, p.shs[k.x.s], t0 + lane) : 0;
 		long long sum = w;
 #pragma unroll
 		for (int o = 1; o < 32; o <<= 1) {
@@ -318,23 +326,20 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, cons
 		}
 		const unsigned m = __ballot_sync(0xffffffffu, sum > rem);
 		if (m || t0 + 32 >= k.tiles) {
-			const int at = m ? __ffs(m) - 1 : 0;
+			const int at = m ? __ffs(m) - 1 : 0, found = __shfl_sync(0xffffffffu, w, at);
 			k.x.t = t0 + at;
-			k.x.w = __shfl_sync(0xffffffffu, w, at);
-			rem -= __shfl_sync(0xffffffffu, sum, at) - k.x.w;
+			k.x.w = max(found - part.lead, 0);
+			rem -= __shfl_sync(0xffffffffu, sum, at) - found;
 			break;
 		}
 		rem -= __shfl_sync(0xffffffffu, sum, 31);
 	}
-	k.x.j0 = (int) rem;
-	k.x.j1 = (int) min((long long) k.x.w, rem + (k.end - k.at));
 	k.x.u = p.cum_u[lo] + k.x.g * k.tiles + k.x.t;
+	walk_piece(part, k, rem);
 	return true;
 }
 __device__ __forceinline__ bool walk_next(const Attn& a, const Part& part, const Plan& p, Walk& k) {
-	k.at += k.x.j1 - k.x.j0;
 	if (k.at >= k.end) return false;
-	k.x.first = false;
 	do {
 		if (++k.x.t == k.tiles) {
 			k.x.t = 0;
@@ -345,15 +350,16 @@ __device__ __forceinline__ bool walk_next(const Attn& a, const Part& part, const
 				walk_segment(a, part, p, k);
 			}
 		}
-		k.x.w = walk_tiles(a, part, p, k);
+		k.x.w = unit_tiles(a, part, k.x.seg, k.x.rows, k.x.q, p.shs[k.x.s], k.x.t);
 	} while (k.x.w == 0);
-	k.x.j0 = 0;
-	k.x.j1 = (int) min((long long) k.x.w, k.end - k.at);
 	k.x.u = p.cum_u[k.x.seg] + k.x.g * k.tiles + k.x.t;
+	walk_piece(part, k, 0);
 	return true;
 }
-// SELECTED: units are (row, kv head, M of its query heads), every one of `w` tiles
+// With lists: units are (row, kv head, M of its query heads), all of the same work
 __device__ __forceinline__ int list_tiles(const Attn& a) { return (int) ((((long long) a.S << a.c.shift) + KT - 1) / KT); }
+__device__ __forceinline__ long long list_units(const Attn& a, const Part& part) { return (long long) a.b.N * a.c.G * ((a.rep + part.M - 1) / part.M); }
+__device__ __forceinline__ long long list_total(const Attn& a, const Part& part) { return list_units(a, part) * (list_tiles(a) + part.lead); }
 __device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk& k, long long unit, bool walking) {
 	const int tiles = (a.rep + part.M - 1) / part.M;
 	k.x.u = (int) unit;
@@ -371,28 +377,20 @@ __device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk&
 		k.x.q = seq_of(a.c, a.b, k.x.s);
 	}
 }
-__device__ __forceinline__ long long list_total(const Attn& a, const Part& part) {
-	return (long long) a.b.N * a.c.G * ((a.rep + part.M - 1) / part.M) * list_tiles(a);
-}
 __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk& k) {
-	const long long total = list_total(a, part);
-	k.at = part_begin(total, part.grid, blockIdx.x);
-	k.end = part_begin(total, part.grid, blockIdx.x + 1);
+	const long long total = list_total(a, part), share = share_of(total, part.grid);
+	k.at = min(share * blockIdx.x, total);
+	k.end = min(k.at + share, total);
 	if (k.at >= k.end) return false;
-	k.x.first = true;
-	const int w = list_tiles(a);
+	const int w = list_tiles(a) + part.lead;
 	list_unit(a, part, k, k.at / w, false);
-	k.x.j0 = (int) (k.at % w);
-	k.x.j1 = (int) min((long long) w, k.x.j0 + (k.end - k.at));
+	walk_piece(part, k, k.at % w);
 	return true;
 }
 __device__ __forceinline__ bool list_next(const Attn& a, const Part& part, Walk& k) {
-	k.at += k.x.j1 - k.x.j0;
 	if (k.at >= k.end) return false;
-	k.x.first = false;
 	list_unit(a, part, k, k.x.u + 1, true);
-	k.x.j0 = 0;
-	k.x.j1 = (int) min((long long) k.x.w, k.end - k.at);
+	walk_piece(part, k, 0);
 	return true;
 }
 __device__ __forceinline__ bool row_in_seq(const Seq& q, int row) { return row >= q.a && row < q.a + q.n; }

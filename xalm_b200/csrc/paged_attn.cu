@@ -33,10 +33,11 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
+		if (x.j0 == x.j1) continue; // the same for every thread
 		__syncthreads();
 		int pos = 0, listed = 0;
 		if (LIST) {
-			if (!row_in_seq(x.q, x.row0)) continue; // the same for every thread
+			if (!row_in_seq(x.q, x.row0)) continue;
 			pos = x.q.len - x.q.n + x.row0 - x.q.a;
 			bool own;
 			const int n = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, warp == 0 ? s_list : nullptr, &own);
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 			__syncthreads();
 		}
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
-		const long long slot = piece_slot(a, x.u, blockIdx.x, x.first);
+		const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
 #pragma unroll
 		for (int r = 0; r < 4; r++)
 			if (lane == 0) {
@@ -174,122 +175,160 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 }
 
 // =========================================================================================================================================
-// The join: a warp per (row, query head).  Its unit in each part lies in the slots (unit + CTA) of the CTAs whose share of the tiles meets the unit's.
+// The join: a warp per (row, query head).  Its unit in each part lies in the slots of the CTAs whose shares meet the unit's tiles.  A lane takes a piece's maximum and sum;
+// then the pieces' rows are added with their weights, four on their way at a time: bound by the latency of the three loads that depend on one another.
 // =========================================================================================================================================
+struct JoinUnit {
+	int part, unit, at, cta, n; // which part, unit, row of the unit, first CTA, CTAs
+};
+template <bool LIST>
+__device__ __forceinline__ bool join_unit(const Attn& a, int i, int seg, int s_first, int row, int r, int g, JoinUnit& o) {
+	const Part& p = a.part[i];
+	long long total, w0;
+	int w, idx;
+	if (LIST) {
+		const int tiles = (a.rep + p.M - 1) / p.M;
+		idx = r;
+		total = list_total(a, p);
+		o.unit = (int) (((long long) row * a.c.G + g) * tiles + r / p.M);
+		w = list_tiles(a);
+		w0 = (long long) o.unit * (w + p.lead);
+	} else {
+		int row0, s;
+		const int rows = seg_rows(a, seg, row0, s);
+		total = p.cum_w[a.b.n_groups + a.b.B];
+		const long long seg_at = p.cum_w[seg], seg_w = p.cum_w[seg + 1] - seg_at;
+		const int sh = p.shs[s_first], u0 = p.cum_u[seg];
+		if (!in_part(p, rows) || !seg_w) return false;
+		const int tiles = (rows + p.M - 1) / p.M;
+		idx = (row - row0) * a.rep + r;
+		if (idx < 0 || idx >= rows) return false;
+		const int t = idx / p.M, lane = threadIdx.x & 31;
+		const Seq q = seq_of(a.c, a.b, s_first);
+		w = unit_tiles(a, p, seg, rows, q, sh, t);
+		if (!w) return false;
+		long long before = 0;
+		if (t) {
+			for (int j = lane; j < t; j += 32) before += unit_work(a, p, seg, rows, q, sh, j);
+#pragma unroll
+			for (int e = 16; e; e >>= 1) before += __shfl_xor_sync(0xffffffffu, before, e);
+		}
+		o.unit = u0 + g * tiles + t;
+		w0 = seg_at + seg_w / a.c.G * g + before;
+	}
+	const long long share = share_of(total, p.grid);
+	w0 += p.lead;
+	if (total < 0x80000000ll) { // short divisions where they do
+		o.cta = (int) ((unsigned) w0 / (unsigned) share);
+		o.n = (int) ((unsigned) (w0 + w - 1) / (unsigned) share) - o.cta + 1;
+	} else {
+		o.cta = (int) (w0 / share);
+		o.n = (int) ((w0 + w - 1) / share) - o.cta + 1;
+	}
+	o.part = i;
+	o.at = idx % p.M;
+	return true;
+}
+
 template <typename T, bool LIST>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn a) {
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ Attn a) {
 	pdl_wait();
-	const long long id = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
+	const long long id = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
 	const int lane = threadIdx.x & 31, dv = a.c.dv;
 	if (id >= (long long) a.b.N * a.H) return;
-	const int row = (int) (id / a.H), h = (int) (id % a.H), g = h / a.rep, r = h % a.rep;
+	const int row = (int) (id / a.H), h = (int) (id - (long long) row * a.H), g = h / a.rep, r = h - g * a.rep;
 	const int s = seq_of_row(a.b, row);
-	const Seq q = seq_of(a.c, a.b, s);
-	if (!row_in_seq(q, row)) return;
-	// pieces: (part, unit, row of the unit, first CTA, CTAs, whether the unit begins behind the start of its first CTA's share)
-	int which[2], unit[2], at[2], c0[2], n[2], found = 0;
-	bool starts_in[2];
-	bool direct = false;
-	for (int i = 0; i < a.n_parts; i++) {
-		const Part& p = a.part[i];
-		const long long total = LIST ? list_total(a, p) : p.cum_w[a.b.n_groups + a.b.B];
-		if (!total) continue;
-		const int shared = LIST ? 0 : p.shs[s];
-		for (int own = 0; own < (LIST ? 1 : 2); own++) {
-			int seg = 0, rows, row0, s_first, u, w;
-			long long w0;
-			int idx; // row of the segment
-			if (LIST) {
-				const int tiles = (a.rep + p.M - 1) / p.M;
-				idx = r;
-				u = (int) (((long long) row * a.c.G + g) * tiles + r / p.M);
-				w = list_tiles(a);
-				w0 = (long long) u * w;
-			} else {
-				if (own) seg = a.b.n_groups + s;
-				else {
-					if (!shared) continue;
-					int lo = 0, hi = a.b.n_groups - 1; // the group of s
-					while (lo < hi) {
-						const int mid = (lo + hi + 1) >> 1;
-						if (a.b.bounds[mid] <= s) lo = mid;
-						else hi = mid - 1;
-					}
-					seg = lo;
-				}
-				rows = seg_rows(a, seg, row0, s_first);
-				if (!in_part(p, rows)) continue;
-				const long long seg_w = p.cum_w[seg + 1] - p.cum_w[seg];
-				if (!seg_w) continue;
-				const int tiles = (rows + p.M - 1) / p.M;
-				idx = (row - row0) * a.rep + r;
-				if (idx < 0 || idx >= rows) continue;
-				const int t = idx / p.M;
-				const Seq fq = seq_of(a.c, a.b, s_first);
-				const int sh = p.shs[s_first];
-				w = unit_tiles(a, p, seg, rows, fq, sh, t);
-				if (!w) continue;
-				long long before = 0;
-				if (!own) before = (long long) t * w;
-				else {
-					for (int i2 = lane; i2 < t; i2 += 32) before += unit_tiles(a, p, seg, rows, fq, sh, i2);
-#pragma unroll
-					for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-				}
-				u = p.cum_u[seg] + g * tiles + t;
-				w0 = p.cum_w[seg] + seg_w / a.c.G * g + before;
+	if (!row_in_seq(seq_of(a.c, a.b, s), row)) return;
+	JoinUnit u[2];
+	int found = 0;
+	if (LIST) found = join_unit<LIST>(a, 0, 0, 0, row, r, g, u[0]);
+	else {
+		const int shared = a.part[0].shs[s];
+		if (shared) { // the group of s
+			int lo = 0, hi = a.b.n_groups - 1;
+			while (lo < hi) {
+				const int mid = (lo + hi + 1) >> 1;
+				if (a.b.bounds[mid] <= s) lo = mid;
+				else hi = mid - 1;
 			}
-			const int n_shares = shares(total, p.grid);
-			int first = (int) (w0 * n_shares / total), last = (int) ((w0 + w - 1) * n_shares / total); // a share begins at floor(total cta / shares)
-			while (first + 1 < n_shares && part_begin(total, p.grid, first + 1) <= w0) first++;
-			while (last + 1 < n_shares && part_begin(total, p.grid, last + 1) <= w0 + w - 1) last++;
-			if (first == last && !shared) direct = true;
-			if (found < 2) {
-				which[found] = i; unit[found] = u; at[found] = idx % p.M; c0[found] = first; n[found] = last - first + 1;
-				starts_in[found] = part_begin(total, p.grid, first) < w0; // the unit is not its first CTA's first piece
+			const int first = min(max(a.b.bounds[lo], 0), a.b.B - 1);
+			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit<LIST>(a, i, lo, first, row, r, g, u[0]);
+		}
+		JoinUnit own;
+		for (int i = 0; i < a.n_parts; i++)
+			if (join_unit<LIST>(a, i, a.b.n_groups + s, s, row, r, g, own)) {
+				if (own.n == 1 && !shared) return; // the CTA that had all of the row has written it
+				if (found) u[1] = own;
+				else u[0] = own;
 				found++;
+				break;
 			}
-		}
 	}
-	if (direct) return; // the CTA that had all of the row has written it
+	if (LIST && u[0].n == 1) return;
+	const int n0 = found ? u[0].n : 0, n = n0 + (found > 1 ? u[1].n : 0); // pieces
 	float m = -INFINITY;
-	for (int f = 0; f < found; f++) {
-		const Part& p = a.part[which[f]];
-		for (int i = lane; i < n[f]; i += 32) {
-			const long long slot = piece_slot(a, unit[f], c0[f] + i, i > 0 || !starts_in[f]);
-			if (slot < p.slots) {
-				const float2 ml = p.ml[slot * p.M + at[f]];
-				m = ml.x != ml.x || m != m ? NAN : fmaxf(m, ml.x);
-			}
+	bool nan = false;
+	auto piece = [&](int i, const float*& o) { // the i-th piece's maximum and sum, and where its row lies
+		const JoinUnit& x = i < n0 ? u[0] : u[1];
+		const Part& p = a.part[x.part];
+		const int c = i < n0 ? i : i - n0;
+		const long long slot = piece_slot(a, x.unit, x.cta + c, c == 0);
+		float2 ml = make_float2(-INFINITY, 0.f);
+		if (slot < p.slots) {
+			ml = p.ml[slot * p.M + x.at];
+			o = p.o + (slot * p.M + x.at) * dv;
 		}
+		return ml;
+	};
+	const float* o = a.part[0].o;
+	for (int i = lane; i < n; i += 32) {
+		const float2 ml = piece(i, o);
+		nan = nan || ml.x != ml.x;
+		m = fmaxf(m, ml.x);
 	}
-	const bool nan = __any_sync(0xffffffffu, m != m);
 	m = warp_max(m);
+	nan = __any_sync(0xffffffffu, nan);
 	const float base = nan ? NAN : m == -INFINITY ? 0.f : m;
 	float l = 0.f, acc[8];
 #pragma unroll
 	for (int i = 0; i < 8; i++) acc[i] = 0.f;
-	for (int f = 0; f < found; f++) {
-		const Part& p = a.part[which[f]];
-		for (int i = 0; i < n[f]; i++) {
-			const long long slot = piece_slot(a, unit[f], c0[f] + i, i > 0 || !starts_in[f]);
-			if (slot >= p.slots) continue;
-			const float2 ml = p.ml[slot * p.M + at[f]];
-			if (ml.x == -INFINITY && ml.y == 0.f) continue; // nothing that the row sees
-			const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - base); // a sum that is NaN stays one
-			l = fmaf(ml.y, w, l);
-			const float* o = p.o + (slot * p.M + at[f]) * dv;
+	for (int i0 = 0; i0 < n; i0 += 32) {
+		float wgt = 0.f;
+		bool some = false;
+		const float* row_at = a.part[0].o;
+		if (i0 + lane < n) {
+			const float2 ml = piece(i0 + lane, row_at);
+			some = ml.x != -INFINITY || ml.y != 0.f; // else nothing that the row sees
+			wgt = !some || ml.x == -INFINITY ? 0.f : exp2f(ml.x - base);
+			if (some) l += ml.y * wgt; // a sum that is NaN stays one
+		}
+		for (unsigned left = __ballot_sync(0xffffffffu, some); left;) {
+			float4 v[4][2];
+			float f[4];
 #pragma unroll
-			for (int c = 0; c < 2; c++)
-				if (c * 128 + lane * 4 < dv) {
-					const float4 v = *reinterpret_cast<const float4*>(o + c * 128 + lane * 4);
-					acc[4 * c] = fmaf(v.x, w, acc[4 * c]);
-					acc[4 * c + 1] = fmaf(v.y, w, acc[4 * c + 1]);
-					acc[4 * c + 2] = fmaf(v.z, w, acc[4 * c + 2]);
-					acc[4 * c + 3] = fmaf(v.w, w, acc[4 * c + 3]);
+			for (int j = 0; j < 4; j++) {
+				const bool one = left != 0;
+				const int from = one ? __ffs(left) - 1 : 0;
+				left &= left - 1;
+				f[j] = __shfl_sync(0xffffffffu, wgt, from);
+				const float* at = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_at), from));
+				if (!one) f[j] = 0.f;
+#pragma unroll
+				for (int c = 0; c < 2; c++)
+					v[j][c] = one && c * 128 + lane * 4 < dv ? *reinterpret_cast<const float4*>(at + c * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+			}
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+#pragma unroll
+				for (int c = 0; c < 2; c++) {
+					acc[4 * c] = fmaf(v[j][c].x, f[j], acc[4 * c]);
+					acc[4 * c + 1] = fmaf(v[j][c].y, f[j], acc[4 * c + 1]);
+					acc[4 * c + 2] = fmaf(v[j][c].z, f[j], acc[4 * c + 2]);
+					acc[4 * c + 3] = fmaf(v[j][c].w, f[j], acc[4 * c + 3]);
 				}
 		}
 	}
+	l = warp_sum(l);
 	const bool any = l > 0.f || l != l;
 	const float inv = any ? 1.f / l : 0.f;
 	T* out = reinterpret_cast<T*>(a.out) + (long long) row * a.out_row + h * dv;
@@ -308,8 +347,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 template <typename T>
 static int join_typed(const Attn& a, cudaStream_t s) {
 	const long long warps = (long long) a.b.N * a.H;
-	const int grid = (int) ((warps + 7) / 8);
-	XALM_CUDA_CHECK(a.lists ? launch(paged_join_kernel<T, true>, grid, 256, 0, s, true, a) : launch(paged_join_kernel<T, false>, grid, 256, 0, s, true, a));
+	const int grid = (int) ((warps + 3) / 4);
+	XALM_CUDA_CHECK(a.lists ? launch(paged_join_kernel<T, true>, grid, 128, 0, s, true, a) : launch(paged_join_kernel<T, false>, grid, 128, 0, s, true, a));
 	return XALM_OK;
 }
 int launch_join(const Attn& a, int type, cudaStream_t s) {

@@ -10,9 +10,9 @@ namespace paged {
 // =========================================================================================================================================
 // out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j, in one pass over the pages.  A step of single tokens reads every key and value once
 // for a handful of rows: HBM bounds it, and what the kernel has to do is to keep enough bytes on their way.  A warp brings tiles of 64 keys and values
-// by TMA (boxes of a page's slots, 64 entries wide, swizzled) into a ring; four warps take a tile each, so that none waits for another: scores and sums by
-// mma.sync m16n8k16 with the 16 rows as A, running maximum and sum in registers.  At the end of a piece the four join through shared memory.  (tcgen05 would want 64
-// rows or more: a step of four heads to a kv head has four.)
+// by TMA (boxes of a page's slots, 64 entries wide, swizzled) into a ring; four warps take 16 keys of a tile each, with maximum, sum and output of their own, so that
+// none waits for another and a stage is free again after a quarter of a tile's work: scores and sums by mma.sync m16n8k16 with the 16 rows as A, queries and sums in registers.
+// At the end of a piece the four join through shared memory.  (tcgen05 would want 64 rows or more: a step of four heads to a kv head has four.)
 // Probabilities enter the second product in the cache's type, a rounding of 2^-9 (bf16) or 2^-12 (fp16) of each, of either sign; scores, maxima and sums stay in fp32.
 // =========================================================================================================================================
 constexpr int MM = 16, CW = 4, MT = (CW + 1) * 32;
@@ -25,15 +25,14 @@ template <int D>
 struct Sizes {
 	static constexpr int TILE = KT * D * 2;         // bytes of a key or value tile
 	static constexpr int STAGE = 2 * TILE;
-	static constexpr int Q = MM * D * 2;
 	static constexpr int OS = D + 8;                // floats between rows of the join's buffer
-	static constexpr int JOIN = CW * 8 * OS * 4;
+	static constexpr int JOIN = CW * 4 * OS * 4;    // four rows of every warp
 };
 // Two CTAs of three or more stages on an SM, or one with what there is: bytes on their way count, not how many CTAs ask for them
 template <int D>
 static MmaConfig mma_config(size_t plan, int n_lists) {
 	using Z = Sizes<D>;
-	const size_t fixed = 1024 + Z::Q + Z::JOIN + CW * MM * 8 + 256 + (size_t) n_lists * 4 + 16 + plan;
+	const size_t fixed = 1024 + Z::JOIN + CW * MM * 8 + 256 + (size_t) n_lists * 4 + 16 + plan;
 	for (int per_sm = 2; per_sm >= 1; per_sm--) {
 		const size_t room = per_sm == 2 ? 113 * 1024 : 226 * 1024;
 		const int n = room > fixed ? (int) ((room - fixed) / Z::STAGE) : 0;
@@ -87,8 +86,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	extern __shared__ uint8_t raw[];
 	uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
 	uint8_t* ring = smem;
-	uint8_t* s_q = ring + (size_t) stages * Z::STAGE;
-	float* s_o = reinterpret_cast<float*>(s_q + Z::Q);                    // [CW][8][OS]
+	float* s_o = reinterpret_cast<float*>(ring + (size_t) stages * Z::STAGE); // [CW][4][OS]
 	float2* s_ml = reinterpret_cast<float2*>((uint8_t*) s_o + Z::JOIN);   // [CW][MM]
 	uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + CW * MM);         // [8]
 	uint64_t* empty = full + 8;                                           // [8]
@@ -97,7 +95,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list) + ((LIST ? a.S * 4 : 0) + 15) / 16 * 16;
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	if (tid == 0) {
-		for (int i = 0; i < stages; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+		for (int i = 0; i < stages; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], CW); }
 		*s_dead = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 	}
@@ -109,12 +107,13 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	const int P = 1 << a.c.shift, W = min(P, KT), per = KT / W; // slots of a box, boxes of a tile's column
 	Walk k;
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
-	int n = 0; // tiles that this CTA's pieces have had so far: tile n lies in stage n % stages and is warp n % CW's
+	int n = 0; // tiles that this CTA's pieces have had so far: tile n lies in stage n % stages
 
 	if (warp == CW) { // ---- the copies ----
 		const int boxes = per * (dc + vc);
 		for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 			const Piece& x = k.x;
+			if (x.j0 == x.j1) continue;
 			int pages = 0, vis = 0x7fffffff;
 			if (LIST) {
 				if (!row_in_seq(x.q, x.row0)) continue;
@@ -159,16 +158,28 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	}
 
 	// ---- the products ----
-	const uint32_t q_at = smem_u32(s_q);
 	const int kd = (a.c.d + 15) / 16, nd = (a.c.dv + 15) / 16;
 	const float c1 = a.scale * 1.4426950408889634f;
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
+		if (x.j0 == x.j1) continue;
 		const bool prefix = !LIST && x.seg < a.b.n_groups;
 		const int rows = min(MM, x.rows - x.t * MM), h0 = x.g * a.rep;
 		int lim0, lim1, least, most; // keys that this lane's two rows see; that the first and the last row see
+		if (LIST && !row_in_seq(x.q, x.row0)) continue;
+		// queries as A: rows lane / 4 and lane / 4 + 8, entries 2 (lane % 4) and 8 more of every 16
+		uint32_t qa[D / 16][4];
+#pragma unroll
+		for (int half = 0; half < 2; half++) {
+			const int r = lane / 4 + half * 8, w = x.t * MM + r;
+			const uint8_t* at = a.q + ((long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d + (lane & 3) * 2) * 2;
+#pragma unroll
+			for (int kk = 0; kk < D / 16; kk++) {
+				qa[kk][half] = r < rows && kk * 16 < a.c.d ? *reinterpret_cast<const uint32_t*>(at + kk * 32) : 0;
+				qa[kk][half + 2] = r < rows && kk * 16 + 8 < a.c.d ? *reinterpret_cast<const uint32_t*>(at + kk * 32 + 16) : 0;
+			}
+		}
 		if (LIST) {
-			if (!row_in_seq(x.q, x.row0)) continue;
 			const int pos = x.q.len - x.q.n + x.row0 - x.q.a;
 			bool own;
 			const int pages = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, nullptr, &own);
@@ -180,16 +191,6 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			lim0 = own_keys(x.q, x.key0, a.rep, min(x.t * MM + lane / 4, x.rows - 1));
 			lim1 = own_keys(x.q, x.key0, a.rep, min(x.t * MM + lane / 4 + 8, x.rows - 1));
 		}
-		for (int i = tid; i < MM * dc * 8; i += CW * 32) {
-			const int r = i / (dc * 8), c = i % (dc * 8);
-			uint4 v = make_uint4(0, 0, 0, 0);
-			if (r < rows && c * 8 < a.c.d) {
-				const int w = x.t * MM + r;
-				v = *reinterpret_cast<const uint4*>(a.q + ((long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d + c * 8) * 2);
-			}
-			*reinterpret_cast<uint4*>(s_q + (chunk_at(q_at, MM, r, c) - q_at)) = v;
-		}
-		bar_sync(1, CW * 32);
 		float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
 		for (int i = 0; i < D / 8; i++)
@@ -198,44 +199,39 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		const int j1 = min(x.j1, (most + KT - 1) / KT);
 		const bool high = rows > 8;
 		for (int j = x.j0; j < j1; j++, n++) {
-			if (n % CW != warp) continue;
 			const int st = n % stages;
 			if (!wait_for(&full[st], (n / stages) & 1, s_dead, a.c)) continue;
-			const uint32_t kt = smem_u32(ring + (size_t) st * Z::STAGE), vt = kt + Z::TILE;
-			const int base = j * KT;
-			if (base + KT > most) { // slots that no row sees may hold anything: as zeros they add nothing
-				for (int i = lane; i < (base + KT - most) * vc * 8; i += 32) {
-					const int r = most - base + i / (vc * 8), c = i % (vc * 8);
+			const uint32_t kt = smem_u32(ring + (size_t) st * Z::STAGE) + warp * 16 * 128, vt = kt + Z::TILE; // this warp's 16 keys
+			const int base = j * KT + warp * 16;
+			const bool tail = base + 16 > most;
+			if (tail) { // slots that no row sees may hold anything: as zeros they add nothing
+				const int from = max(most - base, 0);
+				for (int i = lane; i < (16 - from) * vc * 8; i += 32) {
+					const int r = from + i / (vc * 8), c = i % (vc * 8);
 					asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at(vt, KT, r, c)), "r"(0) : "memory");
 				}
 				__syncwarp();
 			}
-			float s[8][4];
+			float s[2][4];
 #pragma unroll
-			for (int i = 0; i < 8; i++)
+			for (int i = 0; i < 2; i++)
 #pragma unroll
 				for (int e = 0; e < 4; e++) s[i][e] = 0.f;
 #pragma unroll
 			for (int kk = 0; kk < D / 16; kk++)
 				if (kk < kd) {
-					uint32_t qa[4];
-					ldsm4(qa, chunk_at(q_at, MM, (lane & 7) + ((lane >> 3) & 1) * 8, kk * 2 + (lane >> 4)));
-#pragma unroll
-					for (int i = 0; i < 4; i++) { // 16 keys
-						uint32_t b[4];
-						ldsm4(b, chunk_at(kt, KT, i * 16 + (lane & 7) + (lane >> 4) * 8, kk * 2 + ((lane >> 3) & 1)));
-						mma16<T>(s[2 * i], qa, b[0], b[1]);
-						mma16<T>(s[2 * i + 1], qa, b[2], b[3]);
-					}
+					uint32_t b[4];
+					ldsm4(b, chunk_at(kt, KT, (lane & 7) + (lane >> 4) * 8, kk * 2 + ((lane >> 3) & 1)));
+					mma16<T>(s[0], qa[kk], b[0], b[1]);
+					mma16<T>(s[1], qa[kk], b[2], b[3]);
 				}
-			const bool cut = base + KT > least;
 			float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-			for (int i = 0; i < 8; i++) {
+			for (int i = 0; i < 2; i++) {
 #pragma unroll
 				for (int e = 0; e < 4; e++) {
 					s[i][e] *= c1;
-					if (cut && base + i * 8 + (lane & 3) * 2 + (e & 1) >= (e < 2 ? lim0 : lim1)) s[i][e] = -INFINITY;
+					if (base + 16 > least && base + i * 8 + (lane & 3) * 2 + (e & 1) >= (e < 2 ? lim0 : lim1)) s[i][e] = -INFINITY;
 				}
 				t0 = fmaxf(t0, fmaxf(s[i][0], s[i][1]));
 				t1 = fmaxf(t1, fmaxf(s[i][2], s[i][3]));
@@ -256,32 +252,28 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				m1 = n1;
 			}
 			const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-			uint32_t p[8][2];
+			uint32_t pa[4];
 #pragma unroll
-			for (int i = 0; i < 8; i++) {
+			for (int i = 0; i < 2; i++) {
 				const float x0 = ex2(s[i][0] - b0), x1 = ex2(s[i][1] - b0);
 				l0 += x0 + x1;
-				p[i][0] = pack16<T>(x0, x1);
-				p[i][1] = 0;
+				pa[2 * i] = pack16<T>(x0, x1);
+				pa[2 * i + 1] = 0;
 				if (high) {
 					const float x2 = ex2(s[i][2] - b1), x3 = ex2(s[i][3] - b1);
 					l1 += x2 + x3;
-					p[i][1] = pack16<T>(x2, x3);
+					pa[2 * i + 1] = pack16<T>(x2, x3);
 				}
 			}
 #pragma unroll
-			for (int i = 0; i < 4; i++) { // 16 keys
-				const uint32_t pa[4] = {p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1]};
-#pragma unroll
-				for (int c = 0; c < D / 16; c++)
-					if (c < nd) {
-						uint32_t b[4];
-						ldsm4_t(b, chunk_at(vt, KT, i * 16 + (lane & 15), c * 2 + (lane >> 4)));
-						mma16<T>(o[2 * c], pa, b[0], b[1]);
-						mma16<T>(o[2 * c + 1], pa, b[2], b[3]);
-					}
-			}
-			if (base + KT > most) asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the zeros, before the next copy
+			for (int c = 0; c < D / 16; c++)
+				if (c < nd) {
+					uint32_t b[4];
+					ldsm4_t(b, chunk_at(vt, KT, lane & 15, c * 2 + (lane >> 4)));
+					mma16<T>(o[2 * c], pa, b[0], b[1]);
+					mma16<T>(o[2 * c + 1], pa, b[2], b[3]);
+				}
+			if (tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the zeros, before the next copy
 			__syncwarp();
 			if (lane == 0) mbar_arrive(&empty[st]);
 		}
@@ -297,28 +289,30 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		}
 		bar_sync(1, CW * 32);
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && x.key0 == 0;
-		const long long slot = piece_slot(a, x.u, blockIdx.x, x.first);
+		const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
 		const bool mixed = !LIST && !prefix && least < most && x.j1 * KT > least; // some row of the tile must not see what another does
+		float f[2];
 #pragma unroll
 		for (int half = 0; half < 2; half++) {
-			if (half && !high) break;
-			float f;
-			{
-				const int r = lane / 4 + half * 8;
-				float mx = -INFINITY;
+			float mx = -INFINITY;
 #pragma unroll
-				for (int w = 0; w < CW; w++) mx = fmaxf(mx, s_ml[w * MM + r].x);
-				const float mine = half ? m1 : m0;
-				f = mine == -INFINITY ? 0.f : ex2(mine - mx);
+			for (int w = 0; w < CW; w++) mx = fmaxf(mx, s_ml[w * MM + lane / 4 + half * 8].x);
+			const float mine = half ? m1 : m0;
+			f[half] = mine == -INFINITY ? 0.f : ex2(mine - mx);
+		}
+#pragma unroll
+		for (int four = 0; four < 4; four++) { // four rows at a time
+			if (four * 4 >= rows) break;
+			if ((lane >> 4) == (four & 1)) {
+#pragma unroll
+				for (int i = 0; i < D / 8; i++)
+					if (i * 8 < a.c.dv)
+						*reinterpret_cast<float2*>(s_o + (warp * 4 + (lane / 4) % 4) * Z::OS + i * 8 + (lane & 3) * 2) = make_float2(o[i][four & 2] * f[four >> 1], o[i][(four & 2) + 1] * f[four >> 1]);
 			}
-#pragma unroll
-			for (int i = 0; i < D / 8; i++)
-				if (i * 8 < a.c.dv)
-					*reinterpret_cast<float2*>(s_o + (warp * 8 + lane / 4) * Z::OS + i * 8 + (lane & 3) * 2) = make_float2(o[i][half * 2] * f, o[i][half * 2 + 1] * f);
 			bar_sync(1, CW * 32);
-			const int rh = min(8, rows - half * 8), cols = a.c.dv / 4;
+			const int rh = min(4, rows - four * 4), cols = a.c.dv / 4;
 			for (int i = tid; i < rh * cols; i += CW * 32) {
-				const int r = i / cols, c = i % cols * 4, row = half * 8 + r;
+				const int r = i / cols, c = i % cols * 4, row = four * 4 + r;
 				float mx = -INFINITY, l = 0.f;
 #pragma unroll
 				for (int w = 0; w < CW; w++) mx = fmaxf(mx, s_ml[w * MM + row].x);
@@ -330,7 +324,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				float4 v = *reinterpret_cast<const float4*>(s_o + r * Z::OS + c);
 #pragma unroll
 				for (int w = 1; w < CW; w++) {
-					const float4 u = *reinterpret_cast<const float4*>(s_o + (w * 8 + r) * Z::OS + c);
+					const float4 u = *reinterpret_cast<const float4*>(s_o + (w * 4 + r) * Z::OS + c);
 					v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
 				}
 				put_row<T>(a, part, x, MM, row, c, v, mx, l, direct, slot);
@@ -354,7 +348,6 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			if (redo)
 				for (int r = 0; r < rows; r++) slow_row<T>(a, part, x, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, tid, 1);
 		}
-		bar_sync(1, CW * 32);
 	}
 }
 

@@ -125,7 +125,7 @@ __device__ __forceinline__ TcPiece tc_piece(const Attn& a, const Plan& plan, con
 
 struct TcShared {
 	uint64_t k_full[RING], k_empty[RING], v_full[RING], v_empty[RING];
-	uint64_t q_full[2], s_full[2][2], p_full[2], o_full[2];
+	uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2]; // by half and by the tile's parity, so that nobody is ever two phases ahead of a wait
 	uint32_t tmem;
 	int dead, flag[2];
 	float buf[2][256];
@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	if (tid == 0) {
 		for (int i = 0; i < RING; i++) { mbar_init(&sh.k_full[i], 1); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1); }
 		for (int h = 0; h < 2; h++) {
-			mbar_init(&sh.q_full[h], 4); mbar_init(&sh.p_full[h], 4); mbar_init(&sh.o_full[h], 1);
-			mbar_init(&sh.s_full[h][0], 1); mbar_init(&sh.s_full[h][1], 1);
+			mbar_init(&sh.q_full[h], 4);
+			for (int b = 0; b < 2; b++) { mbar_init(&sh.s_full[h][b], 1); mbar_init(&sh.p_full[h][b], 4); mbar_init(&sh.o_full[h][b], 1); }
 		}
 		sh.dead = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	if (warp == 0) { // ---- copies ----
 		for (; more; more = walk_next(a, part, plan, k)) {
 			const Piece& x = k.x;
+			if (x.j0 == x.j1) continue;
 			const TcPiece p = tc_piece(a, plan, x);
 			int id = -1;
 			for (int j = x.j0, e = 0; j < p.j1; j++, e += per, n++) {
@@ -206,10 +207,11 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 		const int kd = (a.c.d + 15) / 16, nv = (a.c.dv + 15) / 16 * 16;
 		const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>(nv, true);
 		const uint32_t q_at = smem_u32(s_q), k_at = smem_u32(s_k), v_at = smem_u32(s_v);
-		int pieces = 0, count[2] = {0, 0}; // pieces with tiles, tiles of each half
+		int pieces[2] = {0, 0}, count[2] = {0, 0}; // of each half: pieces with tiles, tiles
 		bool ok = true;
 		for (; more && ok; more = walk_next(a, part, plan, k)) {
 			const Piece& x = k.x;
+			if (x.j0 == x.j1) continue;
 			const TcPiece p = tc_piece(a, plan, x);
 			if (p.j1 <= x.j0) continue;
 			const int halves = p.rows > HALF_ROWS ? 2 : 1;
@@ -222,10 +224,9 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				}
 				__syncwarp();
 			};
-			ok = ok && wait_for(&sh.q_full[0], pieces & 1, &sh.dead, a.c) && wait_for(&sh.q_full[1], pieces & 1, &sh.dead, a.c) &&
-			     wait_for(&sh.k_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
+			for (int h = 0; h < halves; h++) ok = ok && wait_for(&sh.q_full[h], pieces[h]++ & 1, &sh.dead, a.c);
+			ok = ok && wait_for(&sh.k_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
 			if (!ok) break;
-			pieces++;
 			fence_after();
 			for (int h = 0; h < halves; h++) scores(n, h, count[h] & 1);
 			for (int j = x.j0; j < p.j1 && ok; j++, n++) {
@@ -233,14 +234,19 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				ok = ok && wait_for(&sh.v_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
 				for (int h = 0; h < halves && ok; h++) {
 					fence_after();
-					if (j + 1 < p.j1) scores(n + 1, h, (count[h] + 1) & 1); // its buffer's P went into a product issued before
-					ok = wait_for(&sh.p_full[h], count[h] & 1, &sh.dead, a.c);
+					if (j + 1 < p.j1) {
+						// Its buffer holds the P of the product before: only products into one accumulator are sure to follow one another, so its end is waited for
+						if (j > x.j0 && !(ok = wait_for(&sh.o_full[h][(count[h] - 1) & 1], ((count[h] - 1) >> 1) & 1, &sh.dead, a.c))) break;
+						fence_after();
+						scores(n + 1, h, (count[h] + 1) & 1);
+					}
+					ok = wait_for(&sh.p_full[h][count[h] & 1], (count[h] >> 1) & 1, &sh.dead, a.c);
 					if (!ok) break;
 					fence_after();
 					if (elect()) {
 						for (int s = 0; s < KT / 16; s++)
 							mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 64 * (count[h] & 1) + 8 * s, desc_mn(v_at + (n % RING) * 2 * KB + s * 2048, KB), id_o, j != x.j0 || s != 0);
-						commit(&sh.o_full[h]);
+						commit(&sh.o_full[h][count[h] & 1]);
 						if (h == halves - 1) commit(&sh.v_empty[n % RING]);
 					}
 					__syncwarp();
@@ -256,16 +262,17 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 		int done = 0, tiles = 0; // tiles of this half, of the CTA
 		for (; more; more = walk_next(a, part, plan, k)) {
 			const Piece& x = k.x;
+			if (x.j0 == x.j1) continue;
 			const TcPiece p = tc_piece(a, plan, x);
 			const bool direct = x.j0 == 0 && x.j1 == x.w && !p.prefix && x.key0 == 0, here = h * HALF_ROWS < p.rows;
-			const long long slot = piece_slot(a, x.u, blockIdx.x, x.first);
+			const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
 			const int row = h * HALF_ROWS + r, w = x.t * TC_ROWS + row;
 			const bool mine = row < p.rows;
 			const long long token = x.row0 + w / a.rep;
 			const int head = x.g * a.rep + w % a.rep;
 			float m = -INFINITY, l = 0.f;
 			int lim = 0, least = 0;
-			if (p.j1 > x.j0) {
+			if (p.j1 > x.j0 && here) {
 				for (int c = 0; c < dc * 8; c++) {
 					uint4 v = make_uint4(0, 0, 0, 0);
 					if (mine && c * 8 < a.c.d) v = *reinterpret_cast<const uint4*>(a.q + (token * a.q_row + head * a.c.d + c * 8) * 2);
@@ -313,7 +320,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool grow = mx > m + 11.5f;
 				if (j == x.j0) m = mx;
 				else if (__any_sync(0xffffffffu, grow)) { // rare: the sums so far are complete before they are rescaled
-					if (!wait_for(&sh.o_full[h], (done - 1) & 1, &sh.dead, a.c)) break;
+					if (!wait_for(&sh.o_full[h][(done - 1) & 1], ((done - 1) >> 1) & 1, &sh.dead, a.c)) break;
 					fence_after();
 					const float to = grow ? mx : m, f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
 #pragma unroll
@@ -344,10 +351,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				wait_st();
 				fence_before();
 				__syncwarp();
-				if (lane == 0) mbar_arrive(&sh.p_full[h]);
+				if (lane == 0) mbar_arrive(&sh.p_full[h][b]);
 				done++;
 			}
-			if (p.j1 > x.j0 && here) wait_for(&sh.o_full[h], (done - 1) & 1, &sh.dead, a.c);
+			if (p.j1 > x.j0 && here) wait_for(&sh.o_full[h][(done - 1) & 1], ((done - 1) >> 1) & 1, &sh.dead, a.c);
 			fence_after();
 			bool again = false;
 			if (here) {

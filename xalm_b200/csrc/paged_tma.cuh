@@ -53,7 +53,7 @@ __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
 	    : "memory");
 	return ok != 0;
 }
-constexpr int WAIT_TRIES = 1 << 22; // seconds: far beyond what a copy takes
+constexpr int WAIT_TRIES = 1 << 18; // about two seconds of suspended tries: far beyond what a copy or a product takes
 __device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity) {
 	for (int i = 0; i < WAIT_TRIES; i++)
 		if (try_wait(bar, parity)) return true;
