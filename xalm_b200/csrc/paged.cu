@@ -40,9 +40,10 @@ __global__ void __launch_bounds__(AT) paged_append_kernel(const AppendArgs a) {
 	pdl_launch_dependents();
 	const int row = blockIdx.x, tid = threadIdx.x, d = a.c.d, dv = a.c.dv, G = a.c.G;
 	const int s = seq_of_row(a.b, row);
-	const Seq q = seq_of(a.c, a.b, s);
+	const View view = view_of(a.c, a.b);
+	const Seq q = seq_of(view, s);
 	const bool in = row >= q.a && row < q.a + q.n;
-	if (tid == 0 && row == q.a && !seq_ok(a.c, a.b, s)) report(a.c, ERR_BATCH);
+	if (tid == 0 && row == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
 	if (!in) return; // behind the last sequence
 	const int pos = q.len - q.n + row - q.a;
 	if (pos < 0) return;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(128) paged_means_kernel(const Cache c, const B
 		lo += k * step;
 		n = min(step, n - k * step);
 	}
-	const Seq q = seq_of(c, b, lo);
+	const Seq q = seq_of(view_of(c, b), lo);
 	const int first = max(q.len - q.n, 0) >> c.shift; // page of the first new token
 	const int j = first + item - ((q.a >> c.shift) + lo);
 	if (q.n == 0 || j < first || (long long) (j + 1) << c.shift > q.len) return; // not filled
@@ -179,10 +180,11 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(const SelectArgs a) {
 	pdl_launch_dependents();
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, g = blockIdx.y, d = a.c.d;
 	const int s = seq_of_row(a.b, row);
-	const Seq q = seq_of(a.c, a.b, s);
+	const View view = view_of(a.c, a.b);
+	const Seq q = seq_of(view, s);
 	if (!row_in_seq(q, row)) return;
 	const int pos = q.len - q.n + row - q.a, last = pos < 0 ? -1 : pos >> a.c.shift;
-	if (tid == 0 && row == q.a && !seq_ok(a.c, a.b, s)) report(a.c, ERR_BATCH);
+	if (tid == 0 && row == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
 	int* out = a.out + ((long long) row * a.c.G + g) * a.top;
 	const int lo = min(a.first, last + 1), hi = max(last - a.recent, lo); // pages [lo, hi) are chosen by score, those before and from hi to last are always
 	const int fixed = lo + last + 1 - hi, want = min(a.top - fixed, hi - lo);

@@ -35,21 +35,33 @@ __device__ __forceinline__ void report(const Cache& c, int bit) {
 	if (c.status) atomicOr(c.status, bit);
 }
 
+// What says which rows and lengths the sequences have: in device memory, or a copy of it in shared memory
+struct View {
+	int N, B, n_groups, cap; // cap: positions that a table row has room for
+	const int *starts, *lens, *bounds;
+};
+__device__ __forceinline__ View view_of(const Cache& c, const BatchView& b) {
+	return View{b.N, b.B, b.n_groups, (int) min((long long) b.max_pages << c.shift, 0x7fffffffll), b.starts, b.lens, b.bounds};
+}
 // A sequence's rows [a, a + n) and its length.  Whatever the arrays hold, rows lie in [0, N) and positions in the table.
 struct Seq {
 	int a, n, len;
 };
-__device__ __forceinline__ int capacity(const Cache& c, const BatchView& b) { return (int) min((long long) b.max_pages << c.shift, 0x7fffffffll); }
-__device__ __forceinline__ Seq seq_of(const Cache& c, const BatchView& b, int s) {
+__device__ __forceinline__ Seq seq_of(const View& v, int s) {
 	Seq q;
-	q.a = min(max(b.starts[s], 0), b.N);
-	q.n = min(max(b.starts[s + 1], q.a), b.N) - q.a;
-	q.len = min(max(b.lens[s], 0), capacity(c, b));
+	q.a = min(max(v.starts[s], 0), v.N);
+	q.n = min(max(v.starts[s + 1], q.a), v.N) - q.a;
+	q.len = min(max(v.lens[s], 0), v.cap);
 	return q;
 }
-__device__ __forceinline__ bool seq_ok(const Cache& c, const BatchView& b, int s) {
-	const int a = b.starts[s], e = b.starts[s + 1], l = b.lens[s];
-	return a >= 0 && e >= a && e <= b.N && l >= e - a && l <= capacity(c, b);
+__device__ __forceinline__ bool seq_ok(const View& v, int s) {
+	const int a = v.starts[s], e = v.starts[s + 1], l = v.lens[s];
+	return a >= 0 && e >= a && e <= v.N && l >= e - a && l <= v.cap;
+}
+// The sequences of a group
+__device__ __forceinline__ int2 group_of(const View& v, int i) {
+	const int s0 = min(max(v.bounds[i], 0), v.B);
+	return make_int2(s0, min(max(v.bounds[i + 1], s0), v.B));
 }
 // The sequence of a row: the last s with starts[s] <= row.  A whole warp asks, with 32 probes a round.
 __device__ __forceinline__ int seq_of_row(const BatchView& b, int row) {
@@ -147,25 +159,27 @@ struct Plan {
 	int *cum_u, *shs;
 	int segs;
 	long long total, share;
+	View v; // in shared memory
 };
-__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (B + n_groups + 1) * 12 + (size_t) B * 4 + 32 * 12 + 16; }
+__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (B + n_groups + 1) * 12 + (size_t) (3 * B + n_groups + 3) * 4 + 32 * 12; }
 
 __host__ __device__ __forceinline__ long long share_of(long long total, int grid) { return (total + grid - 1) / grid; }
 
 // rows of a segment, its first row and sequence
-__device__ __forceinline__ int seg_rows(const Attn& a, int seg, int& row0, int& s_first) {
-	if (seg < a.b.n_groups) {
-		const int s0 = min(max(a.b.bounds[seg], 0), a.b.B), s1 = min(max(a.b.bounds[seg + 1], s0), a.b.B);
-		s_first = s0;
-		if (s0 == s1) { row0 = 0; return 0; }
-		row0 = seq_of(a.c, a.b, s0).a;
-		const Seq l = seq_of(a.c, a.b, s1 - 1);
-		return max(l.a + l.n - row0, 0) * a.rep;
+__device__ __forceinline__ int seg_rows(const View& v, int rep, int seg, int& row0, int& s_first) {
+	if (seg < v.n_groups) {
+		const int2 g = group_of(v, seg);
+		s_first = min(g.x, v.B - 1);
+		row0 = 0;
+		if (g.x == g.y) return 0;
+		row0 = seq_of(v, g.x).a;
+		const Seq l = seq_of(v, g.y - 1);
+		return max(l.a + l.n - row0, 0) * rep;
 	}
-	s_first = seg - a.b.n_groups;
-	const Seq q = seq_of(a.c, a.b, s_first);
+	s_first = seg - v.n_groups;
+	const Seq q = seq_of(v, s_first);
 	row0 = q.a;
-	return q.n * a.rep;
+	return q.n * rep;
 }
 // keys of an own segment that the rows up to `last` of it see
 __device__ __forceinline__ int own_keys(const Seq& q, int shared, int rep, int last) { return max(q.len - q.n + last / rep + 1 - shared, 0); }
@@ -195,22 +209,33 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 	p.cum_u = reinterpret_cast<int*>(sum_w + 32);
 	int* sum_u = p.cum_u + p.segs + 1;
 	p.shs = sum_u + 32;
-	for (int s = tid; s < B; s += NT) p.shs[s] = 0;
+	int *starts = p.shs + B, *lens = starts + B + 1, *bounds = lens + B;
+	// the arrays come in at once: what follows asks for them in turn, and every asking of memory is most of a microsecond
+	for (int i = tid; i <= B; i += NT) {
+		starts[i] = a.b.starts[i];
+		if (i < B) { lens[i] = a.b.lens[i]; p.shs[i] = 0; }
+	}
+	if (n)
+		for (int i = tid; i <= n; i += NT) bounds[i] = a.b.bounds[i];
+	p.v = view_of(a.c, a.b);
+	p.v.starts = starts;
+	p.v.lens = lens;
+	p.v.bounds = bounds;
 	__syncthreads();
 	for (int i = warp; i < n; i += NT / 32) {
-		const int s0 = min(max(a.b.bounds[i], 0), B), s1 = min(max(a.b.bounds[i + 1], s0), B);
-		if (s1 - s0 < 2) continue;
-		const Seq last = seq_of(a.c, a.b, s1 - 1);
-		if ((long long) (last.a + last.n - seq_of(a.c, a.b, s0).a) * a.rep > (long long) (s1 - s0) * ALONE_ROWS) continue;
 		int m = max(a.b.shared[i], 0);
-		for (int s = s0 + lane; s < s1; s += 32) {
-			const Seq q = seq_of(a.c, a.b, s);
+		const int2 g = group_of(p.v, i);
+		if (g.y - g.x < 2) continue;
+		const Seq last = seq_of(p.v, g.y - 1);
+		if ((long long) (last.a + last.n - seq_of(p.v, g.x).a) * a.rep > (long long) (g.y - g.x) * ALONE_ROWS) continue;
+		for (int s = g.x + lane; s < g.y; s += 32) {
+			const Seq q = seq_of(p.v, s);
 			m = min(m, max(q.len - q.n, 0));
 		}
 		m = __reduce_min_sync(0xffffffffu, m) >> a.c.shift << a.c.shift;
-		for (int s = s0 + lane; s < s1; s += 32) p.shs[s] = m;
+		for (int s = g.x + lane; s < g.y; s += 32) p.shs[s] = m;
 	}
-	__syncthreads();
+	if (n) __syncthreads();
 	long long carry_w = 0;
 	int carry_u = 0;
 	if (tid == 0) { p.cum_w[0] = 0; p.cum_u[0] = 0; }
@@ -221,22 +246,22 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 		bool wide = false; // own rows of many tiles: their sum is the whole warp's
 		if (seg < p.segs) {
 			int row0, s;
-			const int rows = seg_rows(a, seg, row0, s), tiles = (rows + part.M - 1) / part.M;
+			const int rows = seg_rows(p.v, a.rep, seg, row0, s), tiles = (rows + part.M - 1) / part.M;
 			if (in_part(part, rows)) {
 				if (seg < n) w = (long long) tiles * unit_work(a, part, seg, rows, Seq(), p.shs[s], 0);
 				else {
-					const Seq q = seq_of(a.c, a.b, s);
+					const Seq q = seq_of(p.v, s);
 					if (tiles <= 4) {
 						for (int t = 0; t < tiles; t++) w += unit_work(a, part, seg, rows, q, p.shs[s], t);
 					} else wide = true;
-					if (part.cum_w && blockIdx.x == 0 && !seq_ok(a.c, a.b, s)) report(a.c, ERR_BATCH);
+					if (part.cum_w && blockIdx.x == 0 && !seq_ok(p.v, s)) report(a.c, ERR_BATCH);
 				}
 				in_seg = tiles;
 			}
 		}
 		for (unsigned m = __ballot_sync(0xffffffffu, wide); m; m &= m - 1) {
 			const int from = __ffs(m) - 1, wseg = base + (tid & ~31) + from, n_tiles = __shfl_sync(0xffffffffu, in_seg, from);
-			const Seq q = seq_of(a.c, a.b, wseg - n);
+			const Seq q = seq_of(p.v, wseg - n);
 			long long sum = 0;
 			for (int t = lane; t < n_tiles; t += 32) sum += unit_work(a, part, wseg, q.n * a.rep, q, p.shs[wseg - n], t);
 #pragma unroll
@@ -286,9 +311,9 @@ struct Walk {
 	int tiles;           // row tiles of the segment
 };
 __device__ __forceinline__ void walk_segment(const Attn& a, const Part& part, const Plan& p, Walk& k) {
-	k.x.rows = seg_rows(a, k.x.seg, k.x.row0, k.x.s);
+	k.x.rows = seg_rows(p.v, a.rep, k.x.seg, k.x.row0, k.x.s);
 	k.tiles = (k.x.rows + part.M - 1) / part.M;
-	k.x.q = seq_of(a.c, a.b, k.x.s);
+	k.x.q = seq_of(p.v, k.x.s);
 	k.x.key0 = k.x.seg < a.b.n_groups ? 0 : p.shs[k.x.s];
 }
 // The piece of the unit at k.at, `in` of whose work lies behind the share's start; the walk's place moves behind it
@@ -374,7 +399,7 @@ __device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk&
 	k.x.w = list_tiles(a);
 	if (!same_row) {
 		k.x.s = seq_of_row(a.b, k.x.row0); // whole warps walk
-		k.x.q = seq_of(a.c, a.b, k.x.s);
+		k.x.q = seq_of(view_of(a.c, a.b), k.x.s);
 	}
 }
 __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk& k) {

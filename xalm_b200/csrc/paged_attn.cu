@@ -182,7 +182,7 @@ struct JoinUnit {
 	int part, unit, at, cta, n; // which part, unit, row of the unit, first CTA, CTAs
 };
 template <bool LIST>
-__device__ __forceinline__ bool join_unit(const Attn& a, int i, int seg, int s_first, int row, int r, int g, JoinUnit& o) {
+__device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, int seg, int s_first, int row, int r, int g, JoinUnit& o) {
 	const Part& p = a.part[i];
 	long long total, w0;
 	int w, idx;
@@ -195,7 +195,7 @@ __device__ __forceinline__ bool join_unit(const Attn& a, int i, int seg, int s_f
 		w0 = (long long) o.unit * (w + p.lead);
 	} else {
 		int row0, s;
-		const int rows = seg_rows(a, seg, row0, s);
+		const int rows = seg_rows(v, a.rep, seg, row0, s);
 		total = p.cum_w[a.b.n_groups + a.b.B];
 		const long long seg_at = p.cum_w[seg], seg_w = p.cum_w[seg + 1] - seg_at;
 		const int sh = p.shs[s_first], u0 = p.cum_u[seg];
@@ -204,7 +204,7 @@ __device__ __forceinline__ bool join_unit(const Attn& a, int i, int seg, int s_f
 		idx = (row - row0) * a.rep + r;
 		if (idx < 0 || idx >= rows) return false;
 		const int t = idx / p.M, lane = threadIdx.x & 31;
-		const Seq q = seq_of(a.c, a.b, s_first);
+		const Seq q = seq_of(v, s_first);
 		w = unit_tiles(a, p, seg, rows, q, sh, t);
 		if (!w) return false;
 		long long before = 0;
@@ -238,10 +238,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 	if (id >= (long long) a.b.N * a.H) return;
 	const int row = (int) (id / a.H), h = (int) (id - (long long) row * a.H), g = h / a.rep, r = h - g * a.rep;
 	const int s = seq_of_row(a.b, row);
-	if (!row_in_seq(seq_of(a.c, a.b, s), row)) return;
+	const View v = view_of(a.c, a.b);
+	if (!row_in_seq(seq_of(v, s), row)) return;
 	JoinUnit u[2];
 	int found = 0;
-	if (LIST) found = join_unit<LIST>(a, 0, 0, 0, row, r, g, u[0]);
+	if (LIST) found = join_unit<LIST>(a, v, 0, 0, 0, row, r, g, u[0]);
 	else {
 		const int shared = a.part[0].shs[s];
 		if (shared) { // the group of s
@@ -252,11 +253,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 				else hi = mid - 1;
 			}
 			const int first = min(max(a.b.bounds[lo], 0), a.b.B - 1);
-			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit<LIST>(a, i, lo, first, row, r, g, u[0]);
+			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit<LIST>(a, v, i, lo, first, row, r, g, u[0]);
 		}
 		JoinUnit own;
 		for (int i = 0; i < a.n_parts; i++)
-			if (join_unit<LIST>(a, i, a.b.n_groups + s, s, row, r, g, own)) {
+			if (join_unit<LIST>(a, v, i, a.b.n_groups + s, s, row, r, g, own)) {
 				if (own.n == 1 && !shared) return; // the CTA that had all of the row has written it
 				if (found) u[1] = own;
 				else u[0] = own;
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 			if (some) l += ml.y * wgt; // a sum that is NaN stays one
 		}
 		for (unsigned left = __ballot_sync(0xffffffffu, some); left;) {
-			float4 v[4][2];
+			float4 x[4][2];
 			float f[4];
 #pragma unroll
 			for (int j = 0; j < 4; j++) {
@@ -315,16 +316,16 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 				if (!one) f[j] = 0.f;
 #pragma unroll
 				for (int c = 0; c < 2; c++)
-					v[j][c] = one && c * 128 + lane * 4 < dv ? *reinterpret_cast<const float4*>(at + c * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+					x[j][c] = one && c * 128 + lane * 4 < dv ? *reinterpret_cast<const float4*>(at + c * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 			}
 #pragma unroll
 			for (int j = 0; j < 4; j++)
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
-					acc[4 * c] = fmaf(v[j][c].x, f[j], acc[4 * c]);
-					acc[4 * c + 1] = fmaf(v[j][c].y, f[j], acc[4 * c + 1]);
-					acc[4 * c + 2] = fmaf(v[j][c].z, f[j], acc[4 * c + 2]);
-					acc[4 * c + 3] = fmaf(v[j][c].w, f[j], acc[4 * c + 3]);
+					acc[4 * c] = fmaf(x[j][c].x, f[j], acc[4 * c]);
+					acc[4 * c + 1] = fmaf(x[j][c].y, f[j], acc[4 * c + 1]);
+					acc[4 * c + 2] = fmaf(x[j][c].z, f[j], acc[4 * c + 2]);
+					acc[4 * c + 3] = fmaf(x[j][c].w, f[j], acc[4 * c + 3]);
 				}
 		}
 	}

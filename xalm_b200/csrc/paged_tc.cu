@@ -203,10 +203,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				wait_some(&sh.k_full[i % RING], (i / RING) & 1);
 				wait_some(&sh.v_full[i % RING], (i / RING) & 1);
 			}
-	} else if (warp == 1) { // ---- products ----
+	} else if (warp == 1) { // ---- products: one thread issues them, with nothing to compute but two additions to a descriptor ----
 		const int kd = (a.c.d + 15) / 16, nv = (a.c.dv + 15) / 16 * 16;
 		const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>(nv, true);
-		const uint32_t q_at = smem_u32(s_q), k_at = smem_u32(s_k), v_at = smem_u32(s_v);
+		const uint64_t q_at = desc_k(smem_u32(s_q)), k_at = desc_k(smem_u32(s_k)), v_at = desc_mn(smem_u32(s_v), KB);
 		int pieces[2] = {0, 0}, count[2] = {0, 0}; // of each half: pieces with tiles, tiles
 		bool ok = true;
 		for (; more && ok; more = walk_next(a, part, plan, k)) {
@@ -214,45 +214,49 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			if (x.j0 == x.j1) continue;
 			const TcPiece p = tc_piece(a, plan, x);
 			if (p.j1 <= x.j0) continue;
-			const int halves = p.rows > HALF_ROWS ? 2 : 1;
-			auto scores = [&](int m, int h, int buffer) { // tile m's, of half h
-				if (elect()) {
-					for (int s = 0; s < kd; s++)
-						mma_ss(tmem + 128 * h + 64 * buffer, desc_k(q_at + (h * 2 + (s >> 2)) * QB) + 2 * (s & 3), desc_k(k_at + ((m % RING) * 2 + (s >> 2)) * KB) + 2 * (s & 3), id_s, s != 0);
+			const int halves = p.rows > HALF_ROWS ? 2 : 1, tiles = p.j1 - x.j0;
+			__syncwarp();
+			if (elect()) { // not `lane == 0`: in a branch that the compiler cannot tell to be one thread's, it does not keep the operands of unrolled products apart
+				auto scores = [&](int m, int h, int buffer) { // tile m's, of half h
+					const uint64_t q = q_at + h * (2 * QB >> 4), kk = k_at + (m % RING) * (2 * KB >> 4);
+					const uint32_t d = tmem + 128 * h + 64 * buffer;
+#pragma unroll
+					for (int s = 0; s < 8; s++)
+						if (s < kd) mma_ss(d, q + (s >> 2) * (QB >> 4) + 2 * (s & 3), kk + (s >> 2) * (KB >> 4) + 2 * (s & 3), id_s, s != 0);
 					commit(&sh.s_full[h][buffer]);
 					if (h == halves - 1) commit(&sh.k_empty[m % RING]);
-				}
-				__syncwarp();
-			};
-			for (int h = 0; h < halves; h++) ok = ok && wait_for(&sh.q_full[h], pieces[h]++ & 1, &sh.dead, a.c);
-			ok = ok && wait_for(&sh.k_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
-			if (!ok) break;
-			fence_after();
-			for (int h = 0; h < halves; h++) scores(n, h, count[h] & 1);
-			for (int j = x.j0; j < p.j1 && ok; j++, n++) {
-				if (j + 1 < p.j1) ok = ok && wait_for(&sh.k_full[(n + 1) % RING], ((n + 1) / RING) & 1, &sh.dead, a.c);
-				ok = ok && wait_for(&sh.v_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
-				for (int h = 0; h < halves && ok; h++) {
-					fence_after();
-					if (j + 1 < p.j1) {
-						// Its buffer holds the P of the product before: only products into one accumulator are sure to follow one another, so its end is waited for
-						if (j > x.j0 && !(ok = wait_for(&sh.o_full[h][(count[h] - 1) & 1], ((count[h] - 1) >> 1) & 1, &sh.dead, a.c))) break;
+				};
+				for (int h = 0; h < halves; h++) ok = ok && wait_alone(&sh.q_full[h], pieces[h] & 1, &sh.dead, a.c);
+				ok = ok && wait_alone(&sh.k_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
+				fence_after();
+				if (ok)
+					for (int h = 0; h < halves; h++) scores(n, h, count[h] & 1);
+				for (int j = 0; j < tiles && ok; j++) {
+					const int m = n + j;
+					const bool next = j + 1 < tiles;
+					ok = (!next || wait_alone(&sh.k_full[(m + 1) % RING], ((m + 1) / RING) & 1, &sh.dead, a.c)) && wait_alone(&sh.v_full[m % RING], (m / RING) & 1, &sh.dead, a.c);
+					for (int h = 0; h < halves && ok; h++) {
+						const int c = count[h] + j;
+						if (next) {
+							// Its buffer holds the P of the product before: only products into one accumulator are sure to follow one another, so its end is waited for
+							if (j && !(ok = wait_alone(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c))) break;
+							fence_after();
+							scores(m + 1, h, (c + 1) & 1);
+						}
+						if (!(ok = wait_alone(&sh.p_full[h][c & 1], (c >> 1) & 1, &sh.dead, a.c))) break;
 						fence_after();
-						scores(n + 1, h, (count[h] + 1) & 1);
+						const uint64_t v = v_at + (m % RING) * (2 * KB >> 4);
+						const uint32_t prob = tmem + 128 * h + 64 * (c & 1);
+#pragma unroll
+						for (int s = 0; s < KT / 16; s++) mma_ts(tmem + 256 + 128 * h, prob + 8 * s, v + s * (2048 >> 4), id_o, j != 0 || s != 0);
+						commit(&sh.o_full[h][c & 1]);
+						if (h == halves - 1) commit(&sh.v_empty[m % RING]);
 					}
-					ok = wait_for(&sh.p_full[h][count[h] & 1], (count[h] >> 1) & 1, &sh.dead, a.c);
-					if (!ok) break;
-					fence_after();
-					if (elect()) {
-						for (int s = 0; s < KT / 16; s++)
-							mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 64 * (count[h] & 1) + 8 * s, desc_mn(v_at + (n % RING) * 2 * KB + s * 2048, KB), id_o, j != x.j0 || s != 0);
-						commit(&sh.o_full[h][count[h] & 1]);
-						if (h == halves - 1) commit(&sh.v_empty[n % RING]);
-					}
-					__syncwarp();
-					count[h]++;
 				}
 			}
+			ok = __all_sync(0xffffffffu, ok);
+			for (int h = 0; h < halves; h++) { pieces[h]++; count[h] += tiles; }
+			n += tiles;
 		}
 	} else { // ---- softmax ----
 		const int h = warp < 6 ? 0 : 1, quad = warp & 3, r = quad * 32 + lane, wt = (warp - 2 - 4 * h) * 32 + lane; // row of the half: the tensor memory lanes that this warp may read
@@ -273,11 +277,20 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			float m = -INFINITY, l = 0.f;
 			int lim = 0, least = 0;
 			if (p.j1 > x.j0 && here) {
-				for (int c = 0; c < dc * 8; c++) {
-					uint4 v = make_uint4(0, 0, 0, 0);
-					if (mine && c * 8 < a.c.d) v = *reinterpret_cast<const uint4*>(a.q + (token * a.q_row + head * a.c.d + c * 8) * 2);
-					if (negative) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-					*reinterpret_cast<uint4*>(s_q + (h * 2 + (c >> 3)) * QB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+				// this warp's 32 rows, two at a time, all of them on their way together
+				uint4 v[16];
+				const int c = lane & 15;
+#pragma unroll
+				for (int i = 0; i < 16; i++) {
+					const int rr = h * HALF_ROWS + quad * 32 + i * 2 + (lane >> 4), ww = x.t * TC_ROWS + rr;
+					v[i] = make_uint4(0, 0, 0, 0);
+					if (rr < p.rows && c * 8 < a.c.d) v[i] = *reinterpret_cast<const uint4*>(a.q + ((long long) (x.row0 + ww / a.rep) * a.q_row + (x.g * a.rep + ww % a.rep) * a.c.d + c * 8) * 2);
+				}
+#pragma unroll
+				for (int i = 0; i < 16; i++) {
+					const int rr = quad * 32 + i * 2 + (lane >> 4);
+					if (negative) { v[i].x ^= 0x80008000u; v[i].y ^= 0x80008000u; v[i].z ^= 0x80008000u; v[i].w ^= 0x80008000u; }
+					if (c < dc * 8) *reinterpret_cast<uint4*>(s_q + (h * 2 + (c >> 3)) * QB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
 				}
 				asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 				__syncwarp();
@@ -358,24 +371,53 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			fence_after();
 			bool again = false;
 			if (here) {
+				// 64 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side
+				uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // two blocks of 32 rows of 128 bytes, QB apart
+				const bool any = l > 0.f || l != l;
+				const float inv = direct ? (any ? 1.f / l : 0.f) : 1.f;
+				if (mine) {
+					if (!direct) {
+						if (slot < part.slots) part.ml[slot * TC_ROWS + row] = make_float2(m, l);
+					} else if (a.lse) a.lse[token * a.H + head] = any ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+				}
 #pragma unroll
-				for (int c = 0; c < 4; c++)
-					if (c * 32 < a.c.dv) {
-						uint32_t o[32];
+				for (int c = 0; c < 2; c++)
+					if (c * 64 < a.c.dv) {
+						uint32_t o[64];
 #pragma unroll
-						for (int i = 0; i < 32; i++) o[i] = 0;
-						__syncwarp();
+						for (int i = 0; i < 64; i++) o[i] = 0;
 						if (p.j1 > x.j0) {
-							ld32(t_o + 32 * c, o);
+							ld32(t_o + 64 * c, o);
+							ld32(t_o + 64 * c + 32, o + 32);
 							wait_ld(o);
+							wait_ld(o + 32);
 						}
+						__syncwarp();
 #pragma unroll
-						for (int i = 0; i < 32; i += 4)
-							if (mine && c * 32 + i < a.c.dv) {
-								const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-								put_row<T>(a, part, x, TC_ROWS, row, c * 32 + i, v, m, l, direct, slot);
-								again = again || !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f);
+						for (int i = 0; i < 16; i++) {
+							float4 v = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+							if (mine && c * 64 + i * 4 < a.c.dv) again = again || !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f);
+							if (direct) {
+								v.x = any ? v.x * inv : 0.f;
+								v.y = any ? v.y * inv : 0.f;
+								v.z = any ? v.z * inv : 0.f;
+								v.w = any ? v.w * inv : 0.f;
 							}
+							*reinterpret_cast<float4*>(stage + (i >> 3) * QB + lane * 128 + (((i & 7) ^ (lane & 7)) << 4)) = v;
+						}
+						__syncwarp();
+						const int col = c * 64 + (lane & 15) * 4;
+						for (int i = 0; i < 16; i++) {
+							const int rr = i * 2 + (lane >> 4), at = h * HALF_ROWS + quad * 32 + rr;
+							if (at >= p.rows || col >= a.c.dv) continue;
+							const float4 v = *reinterpret_cast<const float4*>(stage + ((lane & 15) >> 3) * QB + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+							if (direct) {
+								const int ww = x.t * TC_ROWS + at;
+								const uint2 t = make_uint2(pair16<T>(v.x, v.y), pair16<T>(v.z, v.w));
+								*reinterpret_cast<uint2*>(a.out + ((long long) (x.row0 + ww / a.rep) * a.out_row + (x.g * a.rep + ww % a.rep) * a.c.dv + col) * 2) = t;
+							} else if (slot < part.slots) *reinterpret_cast<float4*>(part.o + (slot * TC_ROWS + at) * a.c.dv + col) = v;
+						}
+						__syncwarp();
 					}
 				fence_before();
 				if (!p.prefix && p.j1 > x.j0 && x.j1 * KT > least && least < p.most) {

@@ -72,6 +72,17 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* de
 	return ok;
 }
 
+// The same for one thread
+__device__ __forceinline__ bool wait_alone(uint64_t* bar, uint32_t parity, int* dead, const Cache& c) {
+	for (int i = 0; i < WAIT_TRIES; i++) {
+		if (try_wait(bar, parity)) return true;
+		if (*(volatile int*) dead) return false;
+	}
+	*(volatile int*) dead = 1;
+	report(c, ERR_WAIT);
+	return false;
+}
+
 // Four neighbouring sums of one row of a piece, with the row's maximum (log2 units) and sum: to the output, or to the slot that the join reads
 template <typename T>
 __device__ __forceinline__ void put_row(const Attn& a, const Part& part, const Piece& x, int M, int row, int c, float4 v, float m, float l, bool direct, long long slot) {
