@@ -7,15 +7,17 @@ namespace paged {
 
 // =========================================================================================================================================
 // The same sums as paged_mma_kernel for 256 (token, head) rows at a time, two halves of 128: S = Q K^T and O += P V by tcgen05 with S, P and O in tensor memory.
-// One warp brings tiles of 64 keys and of 64 values by TMA, each read once for both halves; one issues the products; four warps to a half turn S into P, a row to a
-// thread.  At 128 channels a tile of a half takes the tensor pipe 256 cycles and the exponential unit 512 / 2 — neither waits for the other as long as the halves take turns, and one
-// load of keys and values for 256 rows asks L2 for 32 bytes a cycle where 128 rows would ask for 64.
+// One warp brings tiles of 64 keys and of 64 values by TMA, each read once for both halves; a warp to a half issues its products; four warps to a half turn S into P, a row to a
+// thread.  At 128 channels a tile of a half takes the tensor pipe 622 cycles (431 of them the scores, which shared memory bounds) and the exponential unit 512, which the halves share by
+// turns; one load of keys and values for 256 rows asks L2 for half of what 128 rows would.  One warp that issued both halves' products was what everything waited for:
+// a product takes 30 cycles to issue and a wait that is over 150 (2800 cycles a tile).
 // P lies in tensor memory where S lay (its first 32 columns), two S buffers to a half: the scores of the next tile are under way while this one's are worked on.
 // O accumulates unscaled and is rescaled only when a row's maximum has grown by more than 2^11.5 over the one its probabilities are taken against (fp16 holds those).
 // V comes with its entries as the fast dimension, which the second product reads as it is (B transposed).
 // Tensor memory: S of half h, buffer b at columns 128 h + 64 b; O of half h at 256 + 128 h: the whole 512 of an SM, so heads of more than 128 entries stay on mma.sync.
+// What runs once to a piece is kept short and in loops: code that comes from memory for the first time costs more than it takes to run.
 // =========================================================================================================================================
-constexpr int TT = 320;            // copies, products, 2 x 4 warps of softmax
+constexpr int TT = 384;            // copies, products of either half, none, 2 x 4 warps of softmax
 constexpr int HALF_ROWS = 128;
 constexpr int QB = HALF_ROWS * 128; // bytes of 64 entries of a half's queries
 constexpr int KB = KT * 128;        // bytes of 64 entries of a key or value tile
@@ -124,7 +126,7 @@ __device__ __forceinline__ TcPiece tc_piece(const Attn& a, const Plan& plan, con
 }
 
 struct TcShared {
-	uint64_t k_full[RING], k_empty[RING], v_full[RING], v_empty[RING];
+	uint64_t full[RING], empty[RING];
 	uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2]; // by half and by the tile's parity, so that nobody is ever two phases ahead of a wait
 	uint32_t tmem;
 	int dead, flag[2];
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(&sh + 1);
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	if (tid == 0) {
-		for (int i = 0; i < RING; i++) { mbar_init(&sh.k_full[i], 1); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1); }
+		for (int i = 0; i < RING; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 2); }
 		for (int h = 0; h < 2; h++) {
 			mbar_init(&sh.q_full[h], 4);
 			for (int b = 0; b < 2; b++) { mbar_init(&sh.s_full[h][b], 1); mbar_init(&sh.p_full[h][b], 4); mbar_init(&sh.o_full[h][b], 1); }
@@ -163,17 +165,24 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	fence_after();
 	const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
 	const int dc = (a.c.d + 63) / 64, vc = (a.c.dv + 63) / 64, P = 1 << a.c.shift, W = min(P, KT), per = KT / W;
+	const int h = warp < 4 ? warp - 1 : (warp - 4) >> 2; // the half of a warp that has one
+	const int quad = warp & 3;                           // which lanes of tensor memory a softmax warp may read
+	const uint32_t lanes = (uint32_t) (quad * 32) << 16, t_o = tmem + 256 + 128 * h;
+	const bool negative = a.scale < 0.f;
+	const float c1 = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f; // a negative scale turns the queries' signs
 	Walk k;
-	bool more = walk_begin(a, part, plan, k);
-	int n = 0; // tiles so far
-
-	if (warp == 0) { // ---- copies ----
-		for (; more; more = walk_next(a, part, plan, k)) {
-			const Piece& x = k.x;
-			if (x.j0 == x.j1) continue;
-			const TcPiece p = tc_piece(a, plan, x);
+	// tiles of the CTA, tiles and pieces of this warp's half so far
+	int n = 0, done = 0, pieces = 0;
+	bool ok = true;
+	for (bool more = walk_begin(a, part, plan, k); more && ok; more = walk_next(a, part, plan, k)) {
+		const Piece& x = k.x;
+		if (x.j0 == x.j1) continue;
+		const TcPiece p = tc_piece(a, plan, x);
+		const int tiles = max(p.j1 - x.j0, 0);
+		const bool here = h >= 0 && h * HALF_ROWS < p.rows;
+		if (warp == 0) { // ---- copies ----
 			int id = -1;
-			for (int j = x.j0, e = 0; j < p.j1; j++, e += per, n++) {
+			for (int j = 0, e = 0; j < tiles && ok; j++, e += per) {
 				if ((e & 31) == 0) {
 					const int at = x.j0 * KT + (e + lane) * W;
 					id = -1;
@@ -182,139 +191,96 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 						if (id < 0) report(a.c, ERR_PAGE);
 					}
 				}
-				const int st = n % RING, part_of = lane % per, block = lane / per;
+				const int st = (n + j) % RING, part_of = lane % per, block = lane / per;
 				const int pg = __shfl_sync(0xffffffffu, id, (e + part_of) & 31), page = pg < 0 ? a.c.pages : pg;
-				const int slot = (x.key0 + j * KT + part_of * W) & (P - 1);
-				if (!wait_for(&sh.k_empty[st], ((n / RING) & 1) ^ 1, &sh.dead, a.c)) break;
-				if (lane == 0) mbar_expect_tx(&sh.k_full[st], (uint32_t) (dc * KB));
+				const int slot = (x.key0 + (x.j0 + j) * KT + part_of * W) & (P - 1);
+				if (!(ok = wait_for(&sh.empty[st], (((n + j) / RING) & 1) ^ 1, &sh.dead, a.c))) break;
+				if (lane == 0) mbar_expect_tx(&sh.full[st], (uint32_t) ((dc + vc) * KB));
 				__syncwarp();
-				if (block < dc) copy_box(s_k + (st * 2 + block) * KB + part_of * W * 128, &kmap, block * 64, slot, x.g, page, &sh.k_full[st]);
-				__syncwarp();
-				if (!wait_for(&sh.v_empty[st], ((n / RING) & 1) ^ 1, &sh.dead, a.c)) { n++; break; }
-				if (lane == 0) mbar_expect_tx(&sh.v_full[st], (uint32_t) (vc * KB));
-				__syncwarp();
-				if (block < vc) copy_box(s_v + (st * 2 + block) * KB + part_of * W * 128, &vmap, block * 64, slot, x.g, page, &sh.v_full[st]);
+				if (block < dc) copy_box(s_k + (st * 2 + block) * KB + part_of * W * 128, &kmap, block * 64, slot, x.g, page, &sh.full[st]);
+				else if (block < dc + vc) copy_box(s_v + (st * 2 + block - dc) * KB + part_of * W * 128, &vmap, (block - dc) * 64, slot, x.g, page, &sh.full[st]);
 				__syncwarp();
 			}
-			if (*(volatile int*) &sh.dead) break;
-		}
-		if (*(volatile int*) &sh.dead) // gave up: copies still on their way end first
-			for (int i = max(0, n - RING); i < n; i++) {
-				wait_some(&sh.k_full[i % RING], (i / RING) & 1);
-				wait_some(&sh.v_full[i % RING], (i / RING) & 1);
-			}
-	} else if (warp == 1) { // ---- products: one thread issues them, with nothing to compute but two additions to a descriptor ----
-		const int kd = (a.c.d + 15) / 16, nv = (a.c.dv + 15) / 16 * 16;
-		const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>(nv, true);
-		const uint64_t q_at = desc_k(smem_u32(s_q)), k_at = desc_k(smem_u32(s_k)), v_at = desc_mn(smem_u32(s_v), KB);
-		int pieces[2] = {0, 0}, count[2] = {0, 0}; // of each half: pieces with tiles, tiles
-		bool ok = true;
-		for (; more && ok; more = walk_next(a, part, plan, k)) {
-			const Piece& x = k.x;
-			if (x.j0 == x.j1) continue;
-			const TcPiece p = tc_piece(a, plan, x);
-			if (p.j1 <= x.j0) continue;
-			const int halves = p.rows > HALF_ROWS ? 2 : 1, tiles = p.j1 - x.j0;
-			__syncwarp();
-			if (elect()) { // not `lane == 0`: in a branch that the compiler cannot tell to be one thread's, it does not keep the operands of unrolled products apart
-				auto scores = [&](int m, int h, int buffer) { // tile m's, of half h
-					const uint64_t q = q_at + h * (2 * QB >> 4), kk = k_at + (m % RING) * (2 * KB >> 4);
-					const uint32_t d = tmem + 128 * h + 64 * buffer;
-#pragma unroll
-					for (int s = 0; s < 8; s++)
-						if (s < kd) mma_ss(d, q + (s >> 2) * (QB >> 4) + 2 * (s & 3), kk + (s >> 2) * (KB >> 4) + 2 * (s & 3), id_s, s != 0);
-					commit(&sh.s_full[h][buffer]);
-					if (h == halves - 1) commit(&sh.k_empty[m % RING]);
-				};
-				for (int h = 0; h < halves; h++) ok = ok && wait_alone(&sh.q_full[h], pieces[h] & 1, &sh.dead, a.c);
-				ok = ok && wait_alone(&sh.k_full[n % RING], (n / RING) & 1, &sh.dead, a.c);
-				fence_after();
-				if (ok)
-					for (int h = 0; h < halves; h++) scores(n, h, count[h] & 1);
-				for (int j = 0; j < tiles && ok; j++) {
-					const int m = n + j;
-					const bool next = j + 1 < tiles;
-					ok = (!next || wait_alone(&sh.k_full[(m + 1) % RING], ((m + 1) / RING) & 1, &sh.dead, a.c)) && wait_alone(&sh.v_full[m % RING], (m / RING) & 1, &sh.dead, a.c);
-					for (int h = 0; h < halves && ok; h++) {
-						const int c = count[h] + j;
-						if (next) {
-							// Its buffer holds the P of the product before: only products into one accumulator are sure to follow one another, so its end is waited for
-							if (j && !(ok = wait_alone(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c))) break;
+			if (!ok) // gave up: copies still on their way end first
+				for (int i = max(0, n - RING); i < n + tiles; i++) wait_some(&sh.full[i % RING], (i / RING) & 1);
+		} else if (warp <= 2) { // ---- products: one thread issues them, with nothing to compute but two additions to a descriptor ----
+			if (here && tiles) {
+				__syncwarp();
+				if (elect()) { // not `lane == 0`: in a branch that the compiler cannot tell to be one thread's, it does not keep the operands of unrolled products apart
+					const int kd = (a.c.d + 15) / 16;
+					const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>((a.c.dv + 15) / 16 * 16, true), t_s = tmem + 128 * h;
+					const uint64_t q = desc_k(smem_u32(s_q)) + h * (2 * QB >> 4), k_at = desc_k(smem_u32(s_k)), v_at = desc_mn(smem_u32(s_v), KB);
+					ok = wait_alone(&sh.q_full[h], pieces & 1, &sh.dead, a.c);
+					for (int j = -1; j < tiles && ok; j++) { // the scores of tile j + 1, then the second product of tile j
+						const int m = n + j, c = done + j;
+						if (j + 1 < tiles) {
+							if (!(ok = wait_alone(&sh.full[(m + 1) % RING], ((m + 1) / RING) & 1, &sh.dead, a.c))) break;
+							// Their buffer holds the P of the product before: only products into one accumulator are sure to follow one another, so its end is waited for
+							if (j > 0 && !(ok = wait_alone(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c))) break;
 							fence_after();
-							scores(m + 1, h, (c + 1) & 1);
+							const uint64_t kk = k_at + ((m + 1) % RING) * (2 * KB >> 4);
+							const uint32_t d = t_s + 64 * ((c + 1) & 1);
+#pragma unroll
+							for (int s = 0; s < 8; s++)
+								if (s < kd) mma_ss(d, q + (s >> 2) * (QB >> 4) + 2 * (s & 3), kk + (s >> 2) * (KB >> 4) + 2 * (s & 3), id_s, s != 0);
+							commit(&sh.s_full[h][(c + 1) & 1]);
 						}
+						if (j < 0) continue;
 						if (!(ok = wait_alone(&sh.p_full[h][c & 1], (c >> 1) & 1, &sh.dead, a.c))) break;
 						fence_after();
 						const uint64_t v = v_at + (m % RING) * (2 * KB >> 4);
-						const uint32_t prob = tmem + 128 * h + 64 * (c & 1);
+						const uint32_t prob = t_s + 64 * (c & 1);
 #pragma unroll
-						for (int s = 0; s < KT / 16; s++) mma_ts(tmem + 256 + 128 * h, prob + 8 * s, v + s * (2048 >> 4), id_o, j != 0 || s != 0);
+						for (int s = 0; s < KT / 16; s++) mma_ts(t_o, prob + 8 * s, v + s * (2048 >> 4), id_o, j != 0 || s != 0);
 						commit(&sh.o_full[h][c & 1]);
-						if (h == halves - 1) commit(&sh.v_empty[m % RING]);
+						commit(&sh.empty[m % RING]);
 					}
 				}
-			}
+			} else if (lane == 0) // no rows in this half: the tiles are let go one by one all the same, so that this warp does not get ahead of their barriers' phases
+				for (int j = n; j < n + tiles && ok; j++)
+					if ((ok = wait_alone(&sh.full[j % RING], (j / RING) & 1, &sh.dead, a.c))) mbar_arrive(&sh.empty[j % RING]);
 			ok = __all_sync(0xffffffffu, ok);
-			for (int h = 0; h < halves; h++) { pieces[h]++; count[h] += tiles; }
-			n += tiles;
-		}
-	} else { // ---- softmax ----
-		const int h = warp < 6 ? 0 : 1, quad = warp & 3, r = quad * 32 + lane, wt = (warp - 2 - 4 * h) * 32 + lane; // row of the half: the tensor memory lanes that this warp may read
-		const uint32_t lanes = (uint32_t) (quad * 32) << 16, t_o = tmem + 256 + 128 * h + lanes;
-		const bool negative = a.scale < 0.f;
-		const float c1 = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f; // a negative scale turns the queries' signs
-		int done = 0, tiles = 0; // tiles of this half, of the CTA
-		for (; more; more = walk_next(a, part, plan, k)) {
-			const Piece& x = k.x;
-			if (x.j0 == x.j1) continue;
-			const TcPiece p = tc_piece(a, plan, x);
-			const bool direct = x.j0 == 0 && x.j1 == x.w && !p.prefix && x.key0 == 0, here = h * HALF_ROWS < p.rows;
+		} else if (warp >= 4 && here) { // ---- softmax ----
+			const int r = quad * 32 + lane, wt = tid & 127, row = h * HALF_ROWS + r, first = x.t * TC_ROWS + h * HALF_ROWS; // row of the half, of the unit; the half's first row of the segment
+			const bool direct = x.j0 == 0 && x.j1 == x.w && !p.prefix && x.key0 == 0, mine = row < p.rows;
 			const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
-			const int row = h * HALF_ROWS + r, w = x.t * TC_ROWS + row;
-			const bool mine = row < p.rows;
-			const long long token = x.row0 + w / a.rep;
-			const int head = x.g * a.rep + w % a.rep;
+			// rows two at a time, 16 bytes to a lane: token and head of row first + quad * 32 + (lane >> 4) + 2 i
+			const int at0 = first + quad * 32 + (lane >> 4), tok0 = at0 / a.rep, sub0 = at0 - tok0 * a.rep, ch = lane & 15;
 			float m = -INFINITY, l = 0.f;
-			int lim = 0, least = 0;
-			if (p.j1 > x.j0 && here) {
-				// this warp's 32 rows, two at a time, all of them on their way together
-				uint4 v[16];
-				const int c = lane & 15;
-#pragma unroll
-				for (int i = 0; i < 16; i++) {
-					const int rr = h * HALF_ROWS + quad * 32 + i * 2 + (lane >> 4), ww = x.t * TC_ROWS + rr;
-					v[i] = make_uint4(0, 0, 0, 0);
-					if (rr < p.rows && c * 8 < a.c.d) v[i] = *reinterpret_cast<const uint4*>(a.q + ((long long) (x.row0 + ww / a.rep) * a.q_row + (x.g * a.rep + ww % a.rep) * a.c.d + c * 8) * 2);
-				}
-#pragma unroll
+			int lim = p.most, least = p.most;
+			if (!p.prefix) {
+				least = own_keys(x.q, x.key0, a.rep, first);
+				lim = own_keys(x.q, x.key0, a.rep, min(first + r, x.t * TC_ROWS + p.rows - 1));
+			}
+			if (tiles) {
+				int tok = tok0, sub = sub0;
+#pragma unroll 8
 				for (int i = 0; i < 16; i++) {
 					const int rr = quad * 32 + i * 2 + (lane >> 4);
-					if (negative) { v[i].x ^= 0x80008000u; v[i].y ^= 0x80008000u; v[i].z ^= 0x80008000u; v[i].w ^= 0x80008000u; }
-					if (c < dc * 8) *reinterpret_cast<uint4*>(s_q + (h * 2 + (c >> 3)) * QB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+					uint4 v = make_uint4(0, 0, 0, 0);
+					if (h * HALF_ROWS + rr < p.rows && ch * 8 < a.c.d) v = *reinterpret_cast<const uint4*>(a.q + ((long long) (x.row0 + tok) * a.q_row + (x.g * a.rep + sub) * a.c.d + ch * 8) * 2);
+					if (negative) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
+					if (ch < dc * 8) *reinterpret_cast<uint4*>(s_q + (h * 2 + (ch >> 3)) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v;
+					for (sub += 2; sub >= a.rep; sub -= a.rep) tok++;
 				}
 				asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 				__syncwarp();
 				if (lane == 0) mbar_arrive(&sh.q_full[h]);
-				if (p.prefix) lim = least = p.most;
-				else {
-					least = own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + min(h * HALF_ROWS, p.rows - 1));
-					lim = own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + min(row, p.rows - 1));
-				}
 			}
-			for (int j = x.j0; j < p.j1; j++, tiles++) {
-				if (!here) continue;
-				const int b = done & 1, base = j * KT;
+			for (int j = 0; j < tiles; j++) {
+				const int c = done + j, b = c & 1, base = (x.j0 + j) * KT;
 				const uint32_t t_s = tmem + 128 * h + 64 * b + lanes;
-				if (!wait_for(&sh.s_full[h][b], (done >> 1) & 1, &sh.dead, a.c)) break;
+				if (!(ok = wait_for(&sh.s_full[h][b], (c >> 1) & 1, &sh.dead, a.c))) break;
 				fence_after();
 				uint32_t s[KT];
 				ld32(t_s, s);
 				ld32(t_s + 32, s + 32);
 				if (base + KT > p.most) { // slots that no row sees may hold anything: as zeros they add nothing
-					if (!wait_for(&sh.v_full[tiles % RING], (tiles / RING) & 1, &sh.dead, a.c)) break;
+					const int st = (n + j) % RING;
+					if (!(ok = wait_for(&sh.full[st], ((n + j) / RING) & 1, &sh.dead, a.c))) break;
 					for (int i = wt; i < (base + KT - p.most) * vc * 8; i += 128) {
-						const int rr = p.most - base + i / (vc * 8), c = i % (vc * 8);
-						*reinterpret_cast<uint4*>(s_v + ((tiles % RING) * 2 + (c >> 3)) * KB + rr * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+						const int rr = p.most - base + i / (vc * 8), cc = i % (vc * 8);
+						*reinterpret_cast<uint4*>(s_v + (st * 2 + (cc >> 3)) * KB + rr * 128 + ((cc & 7) << 4)) = make_uint4(0, 0, 0, 0);
 					}
 					asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 				}
@@ -331,22 +297,21 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				for (int i = 0; i < KT; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
 				mx *= c1;
 				const bool grow = mx > m + 11.5f;
-				if (j == x.j0) m = mx;
+				if (j == 0) m = mx;
 				else if (__any_sync(0xffffffffu, grow)) { // rare: the sums so far are complete before they are rescaled
-					if (!wait_for(&sh.o_full[h][(done - 1) & 1], ((done - 1) >> 1) & 1, &sh.dead, a.c)) break;
+					if (!(ok = wait_for(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c))) break;
 					fence_after();
 					const float to = grow ? mx : m, f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
+#pragma unroll 1
+					for (int i0 = 0; i0 < a.c.dv; i0 += 32) {
+						uint32_t o[32];
+						ld32(t_o + lanes + i0, o);
+						wait_ld(o);
 #pragma unroll
-					for (int c = 0; c < 4; c++)
-						if (c * 32 < a.c.dv) {
-							uint32_t o[32];
-							ld32(t_o + 32 * c, o);
-							wait_ld(o);
-#pragma unroll
-							for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-							st32(t_o + 32 * c, o);
-						}
-					wait_st();
+						for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+						st32(t_o + lanes + i0, o);
+						wait_st();
+					}
 					l *= f;
 					m = to;
 				}
@@ -365,75 +330,74 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				fence_before();
 				__syncwarp();
 				if (lane == 0) mbar_arrive(&sh.p_full[h][b]);
-				done++;
 			}
-			if (p.j1 > x.j0 && here) wait_for(&sh.o_full[h][(done - 1) & 1], ((done - 1) >> 1) & 1, &sh.dead, a.c);
+			// ---- the piece's sums: 64 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side ----
+			if (tiles && ok) ok = wait_for(&sh.o_full[h][(done + tiles - 1) & 1], ((done + tiles - 1) >> 1) & 1, &sh.dead, a.c);
 			fence_after();
 			bool again = false;
-			if (here) {
-				// 64 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side
-				uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // two blocks of 32 rows of 128 bytes, QB apart
-				const bool any = l > 0.f || l != l;
-				const float inv = direct ? (any ? 1.f / l : 0.f) : 1.f;
-				if (mine) {
-					if (!direct) {
-						if (slot < part.slots) part.ml[slot * TC_ROWS + row] = make_float2(m, l);
-					} else if (a.lse) a.lse[token * a.H + head] = any ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-				}
-#pragma unroll
-				for (int c = 0; c < 2; c++)
-					if (c * 64 < a.c.dv) {
-						uint32_t o[64];
-#pragma unroll
-						for (int i = 0; i < 64; i++) o[i] = 0;
-						if (p.j1 > x.j0) {
-							ld32(t_o + 64 * c, o);
-							ld32(t_o + 64 * c + 32, o + 32);
-							wait_ld(o);
-							wait_ld(o + 32);
-						}
-						__syncwarp();
-#pragma unroll
-						for (int i = 0; i < 16; i++) {
-							float4 v = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-							if (mine && c * 64 + i * 4 < a.c.dv) again = again || !(fabsf(v.x) <= 3.0e38f && fabsf(v.y) <= 3.0e38f && fabsf(v.z) <= 3.0e38f && fabsf(v.w) <= 3.0e38f);
-							if (direct) {
-								v.x = any ? v.x * inv : 0.f;
-								v.y = any ? v.y * inv : 0.f;
-								v.z = any ? v.z * inv : 0.f;
-								v.w = any ? v.w * inv : 0.f;
-							}
-							*reinterpret_cast<float4*>(stage + (i >> 3) * QB + lane * 128 + (((i & 7) ^ (lane & 7)) << 4)) = v;
-						}
-						__syncwarp();
-						const int col = c * 64 + (lane & 15) * 4;
-						for (int i = 0; i < 16; i++) {
-							const int rr = i * 2 + (lane >> 4), at = h * HALF_ROWS + quad * 32 + rr;
-							if (at >= p.rows || col >= a.c.dv) continue;
-							const float4 v = *reinterpret_cast<const float4*>(stage + ((lane & 15) >> 3) * QB + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-							if (direct) {
-								const int ww = x.t * TC_ROWS + at;
-								const uint2 t = make_uint2(pair16<T>(v.x, v.y), pair16<T>(v.z, v.w));
-								*reinterpret_cast<uint2*>(a.out + ((long long) (x.row0 + ww / a.rep) * a.out_row + (x.g * a.rep + ww % a.rep) * a.c.dv + col) * 2) = t;
-							} else if (slot < part.slots) *reinterpret_cast<float4*>(part.o + (slot * TC_ROWS + at) * a.c.dv + col) = v;
-						}
-						__syncwarp();
-					}
-				fence_before();
-				if (!p.prefix && p.j1 > x.j0 && x.j1 * KT > least && least < p.most) {
-					// A value that is not finite and that only later rows see has met probabilities of zero: those rows are done again, key by key
-					if (wt == 0) sh.flag[h] = 0;
-					bar_sync(2 + h, 128);
-					if (again) sh.flag[h] = 1;
-					bar_sync(2 + h, 128);
-					const bool redo = *(volatile int*) &sh.flag[h] != 0;
-					bar_sync(2 + h, 128);
-					if (redo)
-						for (int i = h * HALF_ROWS; i < min(p.rows, (h + 1) * HALF_ROWS); i++)
-							slow_row<T>(a, part, x, TC_ROWS, i, own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + i), sh.buf[h], direct, slot, wt, 2 + h);
+			uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // two blocks of 32 rows of 128 bytes, QB apart
+			const bool any = l > 0.f || l != l;
+			const float inv = direct ? (any ? 1.f / l : 0.f) : 1.f;
+			if (mine) {
+				if (!direct) {
+					if (slot < part.slots) part.ml[slot * TC_ROWS + row] = make_float2(m, l);
+				} else if (a.lse) {
+					const int w = first + r;
+					a.lse[(long long) (x.row0 + w / a.rep) * a.H + x.g * a.rep + w % a.rep] = any ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 				}
 			}
+#pragma unroll 1
+			for (int c0 = 0; c0 < a.c.dv; c0 += 64) {
+				uint32_t o[64];
+#pragma unroll
+				for (int i = 0; i < 64; i++) o[i] = 0;
+				if (tiles) {
+					ld32(t_o + lanes + c0, o);
+					ld32(t_o + lanes + c0 + 32, o + 32);
+					wait_ld(o);
+					wait_ld(o + 32);
+				}
+#pragma unroll
+				for (int i = 0; i < 16; i++) {
+					float4 v = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+					const float worst = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), sum = v.x + v.y + v.z + v.w;
+					again = again || (c0 + i * 4 < a.c.dv && (worst > 3.0e38f || sum != sum));
+					if (direct) { v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv; }
+					*reinterpret_cast<float4*>(stage + (i >> 3) * QB + lane * 128 + (((i & 7) ^ (lane & 7)) << 4)) = v;
+				}
+				__syncwarp();
+				const int col = c0 + ch * 4;
+				int tok = tok0, sub = sub0;
+#pragma unroll 4
+				for (int i = 0; i < 16; i++) {
+					const int rr = i * 2 + (lane >> 4), at = h * HALF_ROWS + quad * 32 + rr;
+					if (at < p.rows && col < a.c.dv) {
+						const float4 v = *reinterpret_cast<const float4*>(stage + (ch >> 3) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
+						if (direct)
+							*reinterpret_cast<uint2*>(a.out + ((long long) (x.row0 + tok) * a.out_row + (x.g * a.rep + sub) * a.c.dv + col) * 2) = make_uint2(pair16<T>(v.x, v.y), pair16<T>(v.z, v.w));
+						else if (slot < part.slots) *reinterpret_cast<float4*>(part.o + (slot * TC_ROWS + at) * a.c.dv + col) = v;
+					}
+					for (sub += 2; sub >= a.rep; sub -= a.rep) tok++;
+				}
+				__syncwarp();
+			}
+			fence_before();
+			if (!p.prefix && tiles && x.j1 * KT > least && least < p.most) {
+				// A value that is not finite and that only later rows see has met probabilities of zero: those rows are done again, key by key
+				if (wt == 0) sh.flag[h] = 0;
+				bar_sync(2 + h, 128);
+				if (again && mine) sh.flag[h] = 1;
+				bar_sync(2 + h, 128);
+				const bool redo = *(volatile int*) &sh.flag[h] != 0;
+				bar_sync(2 + h, 128);
+				if (redo)
+					for (int i = h * HALF_ROWS; i < min(p.rows, (h + 1) * HALF_ROWS); i++)
+						slow_row<T>(a, part, x, TC_ROWS, i, own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + i), sh.buf[h], direct, slot, wt, 2 + h);
+			}
 		}
+		n += tiles;
+		if (here) done += tiles;
+		pieces += here && tiles;
 	}
 	fence_before();
 	__syncthreads();
