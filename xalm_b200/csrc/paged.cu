@@ -398,6 +398,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		p.slots = n_lists || !b.n_groups ? 2 * p.grid : (int) (tiles * c.G) + p.grid;
 		p.o = (float*) take((size_t) p.slots * p.M * c.dv * 4);
 		p.ml = (float2*) take((size_t) p.slots * p.M * 8);
+		p.head = (Head*) take((size_t) p.grid * sizeof(Head));
 		if (!n_lists) {
 			p.cum_w = (long long*) take((size_t) (b.B + b.n_groups + 1) * 8);
 			p.cum_u = (int*) take((size_t) (b.B + b.n_groups + 1) * 4);
@@ -436,6 +437,7 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 		Part& p = a.part[i];
 		p.o = (float*) (base + (size_t) p.o);
 		p.ml = (float2*) (base + (size_t) p.ml);
+		p.head = (Head*) (base + (size_t) p.head);
 		if (!n_lists) {
 			p.cum_w = (long long*) (base + (size_t) p.cum_w);
 			p.cum_u = (int*) (base + (size_t) p.cum_u);

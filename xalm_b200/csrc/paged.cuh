@@ -132,6 +132,9 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // parts as there are CTAs, whatever the sequences' lengths: a CTA walks its part, and writes, for each unit that it meets, a partial result into slot
 // (unit + CTA) — both numbers only grow along the walk, so no two pieces share a slot.  A unit that one CTA holds whole, and whose rows read no other
 // segment, goes straight to the output; paged_join_kernel joins the rest.
+struct Head { // the unit inside which a CTA's share begins, and no other segment's business: what the join needs to know of it
+	int u, j0, w, share, row0, first, rows, g; // number; tiles before the share (0: no such unit), all; tiles to a CTA; first token row; first and number of its (token, head) rows
+};
 struct Part {
 	float* o;            // (slots, M, dv): sums of exp(s - m) v
 	float2* ml;          // (slots, M): m (in units of log2), sum of exp
@@ -139,6 +142,7 @@ struct Part {
 	int least_rows, most_rows; // segments of so many rows are this part's
 	long long* cum_w;    // the plan, left by CTA 0 for the join: tiles and units before each segment, keys shared by each sequence
 	int *cum_u, *shs;
+	Head* head;          // (grid)
 };
 struct Attn {
 	Cache c;
@@ -189,7 +193,7 @@ __device__ __forceinline__ bool in_part(const Part& p, int rows) { return rows >
 // tiles of unit t of a segment
 __device__ __forceinline__ int unit_tiles(const Attn& a, const Part& part, int seg, int rows, const Seq& q, int shared, int t) {
 	if (seg < a.b.n_groups) return (shared + KT - 1) / KT;
-	return (own_keys(q, shared, a.rep, min((t + 1) * part.M, rows) - 1) + KT - 1) / KT;
+	return max((own_keys(q, shared, a.rep, min((t + 1) * part.M, rows) - 1) + KT - 1) / KT, 1); // rows that see nothing have to be written as well
 }
 
 // its work: nothing, or its tiles behind `lead`
@@ -417,6 +421,12 @@ __device__ __forceinline__ bool list_next(const Attn& a, const Part& part, Walk&
 	list_unit(a, part, k, k.x.u + 1, true);
 	walk_piece(part, k, 0);
 	return true;
+}
+// by one thread of a CTA, before its first walk_next / list_next
+__device__ __forceinline__ void write_head(const Attn& a, const Part& part, const Walk& k, bool any, bool alone, long long share) {
+	Head h = {};
+	if (any && alone) h = Head{k.x.u, k.x.j0, k.x.w, (int) share, k.x.row0, k.x.t * part.M, min(part.M, k.x.rows - k.x.t * part.M), k.x.g};
+	part.head[blockIdx.x] = h;
 }
 __device__ __forceinline__ bool row_in_seq(const Seq& q, int row) { return row >= q.a && row < q.a + q.n; }
 

@@ -31,6 +31,8 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 	if (!LIST) make_plan<RT>(a, part, s_plan, plan);
 	Walk k;
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
+	if (tid == 0)
+		write_head(a, part, k, more, LIST ? more && row_in_seq(k.x.q, k.x.row0) : more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, LIST ? share_of(list_total(a, part), part.grid) : plan.share);
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue; // the same for every thread
@@ -175,49 +177,36 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 }
 
 // =========================================================================================================================================
-// The join: a warp per (row, query head).  Its unit in each part lies in the slots of the CTAs whose shares meet the unit's tiles.  A lane takes a piece's maximum and sum;
-// then the pieces' rows are added with their weights, four on their way at a time: bound by the latency of the three loads that depend on one another.
+// The join of what several CTAs have of the same rows, a warp to a row.  A lane takes a piece's maximum and sum, then the pieces' rows are added with their weights, four
+// loads on their way at a time.  Two kinds of blocks: with groups, for a kv head of a sequence whose rows read shared pages; and for 16 rows
+// of the units that a CTA's share begins inside.  Bound by the latency of three or four loads that depend on one another.
 // =========================================================================================================================================
+constexpr int JT = 128, JR = 16;
+
 struct JoinUnit {
 	int part, unit, at, cta, n; // which part, unit, row of the unit, first CTA, CTAs
 };
-template <bool LIST>
-__device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, int seg, int s_first, int row, int r, int g, JoinUnit& o) {
+// The unit of row `idx` of a segment: where its pieces lie
+__device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, int seg, int s_first, int idx, int g, JoinUnit& o) {
 	const Part& p = a.part[i];
-	long long total, w0;
-	int w, idx;
-	if (LIST) {
-		const int tiles = (a.rep + p.M - 1) / p.M;
-		idx = r;
-		total = list_total(a, p);
-		o.unit = (int) (((long long) row * a.c.G + g) * tiles + r / p.M);
-		w = list_tiles(a);
-		w0 = (long long) o.unit * (w + p.lead);
-	} else {
-		int row0, s;
-		const int rows = seg_rows(v, a.rep, seg, row0, s);
-		total = p.cum_w[a.b.n_groups + a.b.B];
-		const long long seg_at = p.cum_w[seg], seg_w = p.cum_w[seg + 1] - seg_at;
-		const int sh = p.shs[s_first], u0 = p.cum_u[seg];
-		if (!in_part(p, rows) || !seg_w) return false;
-		const int tiles = (rows + p.M - 1) / p.M;
-		idx = (row - row0) * a.rep + r;
-		if (idx < 0 || idx >= rows) return false;
-		const int t = idx / p.M, lane = threadIdx.x & 31;
-		const Seq q = seq_of(v, s_first);
-		w = unit_tiles(a, p, seg, rows, q, sh, t);
-		if (!w) return false;
-		long long before = 0;
-		if (t) {
-			for (int j = lane; j < t; j += 32) before += unit_work(a, p, seg, rows, q, sh, j);
+	int row0, s;
+	const int rows = seg_rows(v, a.rep, seg, row0, s);
+	const long long total = p.cum_w[a.b.n_groups + a.b.B], seg_at = p.cum_w[seg], seg_w = p.cum_w[seg + 1] - seg_at;
+	const int sh = p.shs[s_first], u0 = p.cum_u[seg];
+	if (!in_part(p, rows) || !seg_w) return false;
+	const int tiles = (rows + p.M - 1) / p.M, t = idx / p.M, lane = threadIdx.x & 31;
+	if (idx < 0 || idx >= rows) return false;
+	const Seq q = seq_of(v, s_first);
+	const int w = unit_tiles(a, p, seg, rows, q, sh, t);
+	if (!w) return false;
+	long long before = 0;
+	if (t) {
+		for (int j = lane; j < t; j += 32) before += unit_work(a, p, seg, rows, q, sh, j);
 #pragma unroll
-			for (int e = 16; e; e >>= 1) before += __shfl_xor_sync(0xffffffffu, before, e);
-		}
-		o.unit = u0 + g * tiles + t;
-		w0 = seg_at + seg_w / a.c.G * g + before;
+		for (int e = 16; e; e >>= 1) before += __shfl_xor_sync(0xffffffffu, before, e);
 	}
-	const long long share = share_of(total, p.grid);
-	w0 += p.lead;
+	const long long share = share_of(total, p.grid), w0 = seg_at + seg_w / a.c.G * g + before + p.lead;
+	o.unit = u0 + g * tiles + t;
 	if (total < 0x80000000ll) { // short divisions where they do
 		o.cta = (int) ((unsigned) w0 / (unsigned) share);
 		o.n = (int) ((unsigned) (w0 + w - 1) / (unsigned) share) - o.cta + 1;
@@ -226,46 +215,13 @@ __device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, i
 		o.n = (int) ((w0 + w - 1) / share) - o.cta + 1;
 	}
 	o.part = i;
-	o.at = idx % p.M;
+	o.at = idx - t * p.M;
 	return true;
 }
 
-template <typename T, bool LIST>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ Attn a) {
-	pdl_wait();
-	const long long id = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
+template <typename T>
+__device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], int found, int row, int h) {
 	const int lane = threadIdx.x & 31, dv = a.c.dv;
-	if (id >= (long long) a.b.N * a.H) return;
-	const int row = (int) (id / a.H), h = (int) (id - (long long) row * a.H), g = h / a.rep, r = h - g * a.rep;
-	const int s = seq_of_row(a.b, row);
-	const View v = view_of(a.c, a.b);
-	if (!row_in_seq(seq_of(v, s), row)) return;
-	JoinUnit u[2];
-	int found = 0;
-	if (LIST) found = join_unit<LIST>(a, v, 0, 0, 0, row, r, g, u[0]);
-	else {
-		const int shared = a.part[0].shs[s];
-		if (shared) { // the group of s
-			int lo = 0, hi = a.b.n_groups - 1;
-			while (lo < hi) {
-				const int mid = (lo + hi + 1) >> 1;
-				if (a.b.bounds[mid] <= s) lo = mid;
-				else hi = mid - 1;
-			}
-			const int first = min(max(a.b.bounds[lo], 0), a.b.B - 1);
-			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit<LIST>(a, v, i, lo, first, row, r, g, u[0]);
-		}
-		JoinUnit own;
-		for (int i = 0; i < a.n_parts; i++)
-			if (join_unit<LIST>(a, v, i, a.b.n_groups + s, s, row, r, g, own)) {
-				if (own.n == 1 && !shared) return; // the CTA that had all of the row has written it
-				if (found) u[1] = own;
-				else u[0] = own;
-				found++;
-				break;
-			}
-	}
-	if (LIST && u[0].n == 1) return;
 	const int n0 = found ? u[0].n : 0, n = n0 + (found > 1 ? u[1].n : 0); // pieces
 	float m = -INFINITY;
 	bool nan = false;
@@ -345,15 +301,70 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 	if (a.lse && lane == 0) a.lse[(long long) row * a.H + h] = any ? (base + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
+// blocks of a part's boundaries: one to 16 rows of each
+__host__ __device__ __forceinline__ int boundary_blocks(const Part& p) { return p.grid * (p.M > JR ? p.M / JR : 1); }
+
 template <typename T>
-static int join_typed(const Attn& a, cudaStream_t s) {
-	const long long warps = (long long) a.b.N * a.H;
-	const int grid = (int) ((warps + 3) / 4);
-	XALM_CUDA_CHECK(a.lists ? launch(paged_join_kernel<T, true>, grid, 128, 0, s, true, a) : launch(paged_join_kernel<T, false>, grid, 128, 0, s, true, a));
-	return XALM_OK;
+__global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ Attn a) {
+	pdl_wait();
+	const int warp = threadIdx.x >> 5, n_seq = a.b.n_groups && !a.lists ? a.b.B * a.c.G : 0;
+	int id = blockIdx.x;
+	if (id < n_seq) {
+		const int s = id / a.c.G, g = id - s * a.c.G; // a sequence's rows of one kv head
+		const int shared = a.part[0].shs[s];
+		if (!shared) return;
+		const View v = view_of(a.c, a.b);
+		const Seq q = seq_of(v, s);
+		int lo = 0, hi = a.b.n_groups - 1; // its group
+		while (lo < hi) {
+			const int mid = (lo + hi + 1) >> 1;
+			if (a.b.bounds[mid] <= s) lo = mid;
+			else hi = mid - 1;
+		}
+		const int first = min(group_of(v, lo).x, a.b.B - 1), row0 = seq_of(v, first).a;
+		for (int r = warp; r < q.n * a.rep; r += JT / 32) {
+			JoinUnit u[2];
+			int found = 0;
+			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit(a, v, i, lo, first, (q.a - row0) * a.rep + r, g, u[0]);
+			const int had = found;
+			for (int i = 0; i < a.n_parts && found == had; i++) found += join_unit(a, v, i, a.b.n_groups + s, s, r, g, had ? u[1] : u[0]);
+			join_row<T>(a, u, found, q.a + r / a.rep, g * a.rep + r % a.rep);
+		}
+		return;
+	}
+	id -= n_seq;
+	for (int i = 0; i < a.n_parts; i++) {
+		const Part& p = a.part[i];
+		const int blocks = boundary_blocks(p), chunks = blocks / p.grid;
+		if (id >= blocks) {
+			id -= blocks;
+			continue;
+		}
+		const int cta = id / chunks;
+		const Head x = p.head[cta];
+		if (!x.j0 || x.j0 > x.share) return; // of the shares that begin inside a unit, the first joins it
+		JoinUnit u[2];
+		u[0].part = i;
+		u[0].unit = x.u;
+		u[0].cta = cta - 1;
+		u[0].n = (x.share - x.j0 + x.w - 1) / x.share + 1;
+		for (int r = (id - cta * chunks) * JR + warp; r < min(x.rows, (id - cta * chunks) * JR + JR); r += JT / 32) {
+			const int w = x.first + r, tok = w / a.rep;
+			u[0].at = r;
+			join_row<T>(a, u, 1, x.row0 + tok, x.g * a.rep + w - tok * a.rep);
+		}
+		return;
+	}
 }
+
 int launch_join(const Attn& a, int type, cudaStream_t s) {
-	return type == XALM_F32 ? join_typed<float>(a, s) : type == XALM_F16 ? join_typed<__half>(a, s) : join_typed<__nv_bfloat16>(a, s);
+	int grid = 0;
+	for (int i = 0; i < a.n_parts; i++) grid += boundary_blocks(a.part[i]);
+	if (a.b.n_groups && !a.lists) grid += a.b.B * a.c.G;
+	XALM_CUDA_CHECK(type == XALM_F32   ? launch(paged_join_kernel<float>, grid, JT, 0, s, true, a)
+	                : type == XALM_F16 ? launch(paged_join_kernel<__half>, grid, JT, 0, s, true, a)
+	                                   : launch(paged_join_kernel<__nv_bfloat16>, grid, JT, 0, s, true, a));
+	return XALM_OK;
 }
 
 template <int NC, bool LIST>

@@ -107,6 +107,8 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	const int P = 1 << a.c.shift, W = min(P, KT), per = KT / W; // slots of a box, boxes of a tile's column
 	Walk k;
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
+	if (tid == 0)
+		write_head(a, part, k, more, LIST ? more && row_in_seq(k.x.q, k.x.row0) : more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, LIST ? share_of(list_total(a, part), part.grid) : plan.share);
 	int n = 0; // tiles that this CTA's pieces have had so far: tile n lies in stage n % stages
 
 	if (warp == CW) { // ---- the copies ----
@@ -345,8 +347,9 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			bar_sync(1, CW * 32);
 			const bool redo = s_ml[0].x != 0.f;
 			bar_sync(1, CW * 32);
+			const Piece y = x; // in memory only here
 			if (redo)
-				for (int r = 0; r < rows; r++) slow_row<T>(a, part, x, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, tid, 1);
+				for (int r = 0; r < rows; r++) slow_row<T>(a, part, y, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, tid, 1);
 		}
 	}
 }

@@ -174,7 +174,9 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	// tiles of the CTA, tiles and pieces of this warp's half so far
 	int n = 0, done = 0, pieces = 0;
 	bool ok = true;
-	for (bool more = walk_begin(a, part, plan, k); more && ok; more = walk_next(a, part, plan, k)) {
+	bool more = walk_begin(a, part, plan, k);
+	if (tid == 96) write_head(a, part, k, more, more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, plan.share); // a warp with nothing else to do
+	for (; more && ok; more = walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue;
 		const TcPiece p = tc_piece(a, plan, x);
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			const bool direct = x.j0 == 0 && x.j1 == x.w && !p.prefix && x.key0 == 0, mine = row < p.rows;
 			const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
 			// rows two at a time, 16 bytes to a lane: token and head of row first + quad * 32 + (lane >> 4) + 2 i
-			const int at0 = first + quad * 32 + (lane >> 4), tok0 = at0 / a.rep, sub0 = at0 - tok0 * a.rep, ch = lane & 15;
+			const int row0 = x.row0, head0 = x.g * a.rep, at0 = first + quad * 32 + (lane >> 4), tok0 = at0 / a.rep, sub0 = at0 - tok0 * a.rep, ch = lane & 15;
 			float m = -INFINITY, l = 0.f;
 			int lim = p.most, least = p.most;
 			if (!p.prefix) {
@@ -254,14 +256,24 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			}
 			if (tiles) {
 				int tok = tok0, sub = sub0;
-#pragma unroll 8
-				for (int i = 0; i < 16; i++) {
-					const int rr = quad * 32 + i * 2 + (lane >> 4);
-					uint4 v = make_uint4(0, 0, 0, 0);
-					if (h * HALF_ROWS + rr < p.rows && ch * 8 < a.c.d) v = *reinterpret_cast<const uint4*>(a.q + ((long long) (x.row0 + tok) * a.q_row + (x.g * a.rep + sub) * a.c.d + ch * 8) * 2);
-					if (negative) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-					if (ch < dc * 8) *reinterpret_cast<uint4*>(s_q + (h * 2 + (ch >> 3)) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v;
-					for (sub += 2; sub >= a.rep; sub -= a.rep) tok++;
+				const int left = p.rows - h * HALF_ROWS - quad * 32 - (lane >> 4); // row 2 i is one of the unit's while 2 i < left
+#pragma unroll 1
+				for (int i0 = 0; i0 < 32; i0 += 16) { // eight loads on their way together
+					uint4 v[8];
+#pragma unroll
+					for (int i = 0; i < 8; i++) {
+						const bool some = i0 + 2 * i < left && ch * 8 < a.c.d;
+						v[i] = *reinterpret_cast<const uint4*>(a.q + (some ? ((long long) (row0 + tok) * a.q_row + (head0 + sub) * a.c.d + ch * 8) * 2 : 0));
+						if (!some) v[i] = make_uint4(0, 0, 0, 0);
+						sub += 2;
+						while (sub >= a.rep) { sub -= a.rep; tok++; }
+					}
+#pragma unroll
+					for (int i = 0; i < 8; i++) {
+						const int rr = quad * 32 + i0 + i * 2 + (lane >> 4);
+						if (negative) { v[i].x ^= 0x80008000u; v[i].y ^= 0x80008000u; v[i].z ^= 0x80008000u; v[i].w ^= 0x80008000u; }
+						if (ch < dc * 8) *reinterpret_cast<uint4*>(s_q + (h * 2 + (ch >> 3)) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v[i];
+					}
 				}
 				asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 				__syncwarp();
@@ -287,14 +299,17 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				__syncwarp();
 				wait_ld(s);
 				wait_ld(s + 32);
-				float mx = -INFINITY;
 				if (base + KT > least) {
 #pragma unroll
 					for (int i = 0; i < KT; i++)
 						if (base + i >= lim) s[i] = 0xff800000u;
 				}
+				float m8[8]; // eight chains: one of 64 would be waited for link by link
 #pragma unroll
-				for (int i = 0; i < KT; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
+				for (int i = 0; i < 8; i++) m8[i] = __uint_as_float(s[i]);
+#pragma unroll
+				for (int i = 8; i < KT; i++) m8[i & 7] = fmaxf(m8[i & 7], __uint_as_float(s[i]));
+				float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
 				mx *= c1;
 				const bool grow = mx > m + 11.5f;
 				if (j == 0) m = mx;
@@ -316,15 +331,23 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 					m = to;
 				}
 				const float nm = m == -INFINITY ? 0.f : -m;
-				float sum = 0.f;
+				const f32x2 c2 = pack2(c1, c1), n2 = pack2(nm, nm);
+				f32x2 sum[4] = {pack2(0.f, 0.f), pack2(0.f, 0.f), pack2(0.f, 0.f), pack2(0.f, 0.f)};
 				uint32_t q[KT / 2];
 #pragma unroll
-				for (int i = 0; i < KT / 2; i++) {
-					const float p0 = exp2_approx(fmaf(__uint_as_float(s[2 * i]), c1, nm)), p1 = exp2_approx(fmaf(__uint_as_float(s[2 * i + 1]), c1, nm));
-					sum += p0 + p1;
+				for (int i = 0; i < KT / 2; i++) { // two at a time where there is an instruction for two
+					float p0, p1;
+					unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, n2), p0, p1);
+					p0 = exp2_approx(p0);
+					p1 = exp2_approx(p1);
+					sum[i & 3] = add2(sum[i & 3], pack2(p0, p1));
 					q[i] = pair16<T>(p0, p1);
 				}
-				l += sum;
+				{
+					float e, o;
+					unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), e, o);
+					l += e + o;
+				}
 				st32(t_s, q);
 				wait_st();
 				fence_before();
@@ -366,18 +389,27 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 					*reinterpret_cast<float4*>(stage + (i >> 3) * QB + lane * 128 + (((i & 7) ^ (lane & 7)) << 4)) = v;
 				}
 				__syncwarp();
-				const int col = c0 + ch * 4;
+				const int col = c0 + ch * 4, left = col < a.c.dv && (direct || slot < part.slots) ? p.rows - h * HALF_ROWS - quad * 32 - (lane >> 4) : 0;
 				int tok = tok0, sub = sub0;
-#pragma unroll 4
-				for (int i = 0; i < 16; i++) {
-					const int rr = i * 2 + (lane >> 4), at = h * HALF_ROWS + quad * 32 + rr;
-					if (at < p.rows && col < a.c.dv) {
-						const float4 v = *reinterpret_cast<const float4*>(stage + (ch >> 3) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
-						if (direct)
-							*reinterpret_cast<uint2*>(a.out + ((long long) (x.row0 + tok) * a.out_row + (x.g * a.rep + sub) * a.c.dv + col) * 2) = make_uint2(pair16<T>(v.x, v.y), pair16<T>(v.z, v.w));
-						else if (slot < part.slots) *reinterpret_cast<float4*>(part.o + (slot * TC_ROWS + at) * a.c.dv + col) = v;
+				float* po = part.o + (slot * TC_ROWS + h * HALF_ROWS + quad * 32 + (lane >> 4)) * a.c.dv + col;
+#pragma unroll 1
+				for (int i0 = 0; i0 < 16; i0 += 4) {
+					float4 v[4];
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						const int rr = (i0 + i) * 2 + (lane >> 4);
+						v[i] = *reinterpret_cast<const float4*>(stage + (ch >> 3) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
 					}
-					for (sub += 2; sub >= a.rep; sub -= a.rep) tok++;
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						if (2 * (i0 + i) < left) {
+							if (direct)
+								*reinterpret_cast<uint2*>(a.out + ((long long) (row0 + tok) * a.out_row + (head0 + sub) * a.c.dv + col) * 2) = make_uint2(pair16<T>(v[i].x, v[i].y), pair16<T>(v[i].z, v[i].w));
+							else *reinterpret_cast<float4*>(po + (i0 + i) * 2 * a.c.dv) = v[i];
+						}
+						sub += 2;
+						while (sub >= a.rep) { sub -= a.rep; tok++; }
+					}
 				}
 				__syncwarp();
 			}
@@ -390,9 +422,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				bar_sync(2 + h, 128);
 				const bool redo = *(volatile int*) &sh.flag[h] != 0;
 				bar_sync(2 + h, 128);
+				const Piece y = x; // in memory only here
 				if (redo)
 					for (int i = h * HALF_ROWS; i < min(p.rows, (h + 1) * HALF_ROWS); i++)
-						slow_row<T>(a, part, x, TC_ROWS, i, own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + i), sh.buf[h], direct, slot, wt, 2 + h);
+						slow_row<T>(a, part, y, TC_ROWS, i, own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + i), sh.buf[h], direct, slot, wt, 2 + h);
 			}
 		}
 		n += tiles;

@@ -21,6 +21,7 @@ from . import types as T
 
 _TYPES = {torch.float32: T.F32.id, torch.float16: T.F16.id, torch.bfloat16: T.BF16.id}
 _INVALID, _UNSUPPORTED = 1, 2
+_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(device).cuda_stream says, in a twentieth of its 2 us
 
 
 class _Cache(C.Structure):
@@ -54,7 +55,8 @@ class PagedCache:
             _refuse("paged cache: the entries of a head are neighbours")
         if means is not None and (means.shape != (k.shape[0], k.shape[2], k.shape[3]) or means.dtype != k.dtype or means.device != k.device or not means.is_contiguous()):
             _refuse(f"paged cache: mean keys {tuple(means.shape)} {means.dtype}")
-        self.k, self.v, self.means, self.device = k, v, means, k.device
+        self.k, self.v, self.means, self.device, self.index, self.dtype = k, v, means, k.device, k.device.index, k.dtype
+        self.needs = {}  # bytes of workspace by the sizes of a call
         self.kv_heads, self.dim, self.vdim = k.shape[2], k.shape[3], v.shape[3]
         if k.device.type != "cuda":
             _refuse("paged cache: the pools lie on no GPU")
@@ -99,60 +101,80 @@ class Batch:
 
 def _rows(t, what, n, heads, dim, dtype, device):
     """Row stride of (n, heads, dim) rows whose heads are dense."""
-    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        _refuse(f"paged cache: {what} {tuple(t.shape)}, not ({n}, {heads if heads is not None else 'heads'}, {dim})")
-    if (dtype is not None and t.dtype != dtype) or t.device != device:
+    if t.shape != (n, heads, dim):
+        _refuse(f"paged cache: {what} {tuple(t.shape)}, not ({n}, {heads}, {dim})")
+    if t.dtype is not dtype or t.device != device:
         _refuse(f"paged cache: {what} is {t.dtype} on {t.device}")
-    s = t.stride()
-    if s[2] != 1 or (s[1] != dim and t.shape[1] > 1):
+    row, head, entry = t.stride()
+    if entry != 1 or (head != dim and heads > 1):
         _refuse(f"paged cache: the heads of {what} are dense")
-    return s[0] if n > 1 else (t.shape[1] * dim + 7) // 8 * 8
+    return row if n > 1 else heads * dim
 
 
 def _start(cache, batch, rows):
     if batch.device != cache.device:
         _refuse(f"paged cache: a batch on {batch.device}, a cache on {cache.device}")
     batch.c.rows = rows
-    return torch.cuda.current_stream(cache.device).cuda_stream
+    return _stream(cache.index)
+
+
+def _heads(q):
+    if q.dim() != 3:
+        _refuse(f"paged cache: q {tuple(q.shape)}, not (rows, heads, dim)")
+    return q.shape[1]
 
 
 def append(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_out=None):
     """k (rows, kv_heads, dim) and v (rows, kv_heads, vdim) into the pages of their sequences; returns the turned queries in the cache's type (None without q).  freq
     (n): the first 2 n entries of every head are turned."""
-    n, dev = k.shape[0], cache.device
+    n, dev, dt = k.shape[0], cache.device, k.dtype
     stream = _start(cache, batch, n)
-    kr, vr = _rows(k, "k", n, cache.kv_heads, cache.dim, None, dev), _rows(v, "v", n, cache.kv_heads, cache.vdim, k.dtype, dev)
-    qr = qor = heads = qp = qop = 0
+    kr, vr = _rows(k, "k", n, cache.kv_heads, cache.dim, dt, dev), _rows(v, "v", n, cache.kv_heads, cache.vdim, dt, dev)
+    qr = qor = heads = qp = qop = fp = rot = 0
     if q is not None:
-        qr, heads = _rows(q, "q", n, None, cache.dim, k.dtype, dev), q.shape[1]
+        heads = _heads(q)
+        qr = _rows(q, "q", n, heads, cache.dim, dt, dev)
         if q_out is None:
-            q_out = torch.empty((n, heads, cache.dim), dtype=cache.k.dtype, device=dev)
-        qor, qp, qop = _rows(q_out, "q_out", n, heads, cache.dim, cache.k.dtype, dev), q.data_ptr(), q_out.data_ptr()
+            q_out = torch.empty((n, heads, cache.dim), dtype=cache.dtype, device=dev)
+            qor = heads * cache.dim
+        else:
+            qor = _rows(q_out, "q_out", n, heads, cache.dim, cache.dtype, dev)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         _refuse("paged append: q_out without q")
-    if freq is not None and (freq.dtype != torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev):
-        _refuse(f"paged append: freq {tuple(freq.shape)} {freq.dtype} on {freq.device}")
-    capi.check(capi.lib().xalm_cuda_paged_append(cache.p, batch.p, k.data_ptr(), kr, v.data_ptr(), vr, qp, qr, heads, _type(k), qop, qor,
-                                                 0 if freq is None else freq.data_ptr(), 0 if freq is None else freq.numel(), mag, int(neighbours), stream))
+    if freq is not None:
+        if freq.dtype is not torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev:
+            _refuse(f"paged append: freq {tuple(freq.shape)} {freq.dtype} on {freq.device}")
+        fp, rot = freq.data_ptr(), freq.shape[0]
+    capi.check(capi.lib().xalm_cuda_paged_append(cache.p, batch.p, k.data_ptr(), kr, v.data_ptr(), vr, qp, qr, heads, _type(k), qop, qor, fp, rot, mag, neighbours, stream))
     return q_out
 
 
 def _attend(cache, batch, q, lists, scale, out, want_lse):
-    n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    n, heads, dev = q.shape[0], _heads(q), cache.device
     stream = _start(cache, batch, n)
-    qr = _rows(q, "q", n, None, cache.dim, cache.k.dtype, cache.device)
+    qr = _rows(q, "q", n, heads, cache.dim, cache.dtype, dev)
     if out is None:
-        out = torch.empty((n, heads, cache.vdim), dtype=cache.k.dtype, device=cache.device)
-    outr = _rows(out, "out", n, heads, cache.vdim, cache.k.dtype, cache.device)
-    lse = torch.empty((n, heads), dtype=torch.float32, device=cache.device) if want_lse else None
-    s, L, need = 0 if lists is None else lists.shape[2], capi.lib(), C.c_size_t(0)
-    capi.check(L.xalm_cuda_paged_workspace(cache.p, batch.p, heads, s, C.byref(need)))
-    work = torch.empty(need.value, dtype=torch.uint8, device=cache.device)  # the current stream's, or the graph's that is being captured
-    args = (scale, out.data_ptr(), outr, 0 if lse is None else lse.data_ptr(), work.data_ptr(), need.value, stream)
-    if lists is None:
-        capi.check(L.xalm_cuda_paged_attend(cache.p, batch.p, q.data_ptr(), qr, heads, *args))
+        out = torch.empty((n, heads, cache.vdim), dtype=cache.dtype, device=dev)
+        outr = heads * cache.vdim
     else:
-        capi.check(L.xalm_cuda_paged_attend_selected(cache.p, batch.p, q.data_ptr(), qr, heads, lists.data_ptr(), s, *args))
+        outr = _rows(out, "out", n, heads, cache.vdim, cache.dtype, dev)
+    lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if want_lse else None
+    s, L = 0 if lists is None else lists.shape[2], capi.lib()
+    sizes = n, heads, s, batch.c.seqs, batch.c.groups
+    need = cache.needs.get(sizes)
+    if need is None:
+        b = C.c_size_t(0)
+        capi.check(L.xalm_cuda_paged_workspace(cache.p, batch.p, heads, s, C.byref(b)))
+        if len(cache.needs) > 1000:
+            cache.needs.clear()
+        need = cache.needs[sizes] = b.value
+    work = torch.empty(need, dtype=torch.uint8, device=dev)  # the current stream's, or the graph's that is being captured
+    lp = None if lse is None else lse.data_ptr()
+    if lists is None:
+        capi.check(L.xalm_cuda_paged_attend(cache.p, batch.p, q.data_ptr(), qr, heads, scale, out.data_ptr(), outr, lp, work.data_ptr(), need, stream))
+    else:
+        capi.check(L.xalm_cuda_paged_attend_selected(cache.p, batch.p, q.data_ptr(), qr, heads, lists.data_ptr(), s, scale, out.data_ptr(), outr, lp, work.data_ptr(), need, stream))
     return (out, lse) if want_lse else out
 
 
@@ -163,15 +185,15 @@ def attend(cache, batch, q, scale, out=None, want_lse=False):
 
 
 def select(cache, batch, q, top, first=1, recent=1, out=None):
-    """The `top` pages that each row and kv head reads: (rows, kv_heads, top) int32, places in the sequence, ascending, -1 behind."""
-    n = q.shape[0]
+    """The `top` pages that each row and kv head reads: (rows, kv_heads, top) int32, places in the sequence, ascending, -1 behind; rows outside every sequence are left as they were."""
+    n, heads, dev = q.shape[0], _heads(q), cache.device
     stream = _start(cache, batch, n)
-    qr = _rows(q, "q", n, None, cache.dim, cache.k.dtype, cache.device)
+    qr = _rows(q, "q", n, heads, cache.dim, cache.dtype, dev)
     if out is None:
-        out = torch.full((n, cache.kv_heads, max(top, 0)), -1, dtype=torch.int32, device=cache.device)
-    if out.shape != (n, cache.kv_heads, top) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != cache.device:
+        out = torch.empty((n, cache.kv_heads, max(top, 0)), dtype=torch.int32, device=dev)
+    elif out.shape != (n, cache.kv_heads, top) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != dev:
         _refuse(f"paged select: out {tuple(out.shape)} {out.dtype}")
-    capi.check(capi.lib().xalm_cuda_paged_select(cache.p, batch.p, q.data_ptr(), qr, q.shape[1], top, first, recent, out.data_ptr(), stream))
+    capi.check(capi.lib().xalm_cuda_paged_select(cache.p, batch.p, q.data_ptr(), qr, heads, top, first, recent, out.data_ptr(), stream))
     return out
 
 
