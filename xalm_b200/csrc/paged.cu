@@ -149,8 +149,12 @@ __global__ void __launch_bounds__(128) paged_means_kernel(const Cache c, const B
 }
 
 // =========================================================================================================================================
-// select: a CTA per (row, kv head).  score_j = (sum over the head's queries) . mean_j, summed in 64 bits: which page is the last to be taken must not hang on the
-// order of a sum.  The pages are taken by their scores as ordered integers, equal ones from the lowest index on; a NaN counts as the lowest finite number.
+// select: score_j = (sum over the kv head's queries) . mean_j, and of the pages between the first and the recent ones those with the largest scores, equal ones from the lowest
+// place on.  Which page is the last to be taken must not hang on how a sum was rounded, and sums in 64 bits cost a conversion per mean and row (279 us for 1341
+// tokens of 8 heads over 110 to 235 pages).  So scores are taken in fp32, each off by at most E = (d + rep + 4) 2^-24 sum_i (sum_r |q_ri|) max |mean|; of the want-th largest, t, the true
+// one is off by no more than E, so pages above t + 2 E are taken, those below t - 2 E are not, and only where those between are more than are wanted are they summed in 64 bits.
+// Steps of single tokens: a CTA to (row, kv head), 8 lanes to a page.  Longer ones: R rows of a sequence to a CTA, so that a page's mean is read and converted once for
+// all of them: 64 pages at a time in shared memory, a thread taking one page and R / 4 rows; then a warp to a row.  The want-th largest is found bit by bit from above, up to 512 keys in a warp's registers.
 // =========================================================================================================================================
 struct SelectArgs {
 	Cache c;
@@ -160,132 +164,384 @@ struct SelectArgs {
 	int H, rep, top, first, recent;
 	int* out;
 };
-constexpr int ST = 256;
+constexpr int ST = 256, SP = 64;
+typedef unsigned long long u64;
 
-__device__ __forceinline__ unsigned long long ordered(double x) {
+__device__ __forceinline__ u64 ordered(double x) { // the order of numbers as integers, from 1 to 2^64 - 2; NaN and -infinity as the lowest finite, +infinity as the largest
 	const double big = 1.7976931348623157e308;
 	x = x != x ? -big : fmin(fmax(x, -big), big) + 0.0;
 	const long long b = __double_as_longlong(x);
-	return b < 0 ? ~(unsigned long long) b : (unsigned long long) b | (1ull << 63);
+	return b < 0 ? ~(u64) b : (u64) b | (1ull << 63);
+}
+__device__ __forceinline__ unsigned ordered32(float x) {
+	const int b = __float_as_int(x + 0.f);
+	return b < 0 ? ~(unsigned) b : (unsigned) b | (1u << 31);
+}
+__device__ __forceinline__ float unordered32(unsigned k) { return __int_as_float(k >> 31 ? (int) (k & 0x7fffffffu) : (int) ~k); }
+
+// The threads that have a row: a warp, or the CTA
+template <int TEAM>
+__device__ __forceinline__ int team_sum(int x, int* buf) {
+	x = __reduce_add_sync(0xffffffffu, x);
+	if constexpr (TEAM > 32) {
+		__syncthreads();
+		if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
+		__syncthreads();
+		x = 0;
+#pragma unroll
+		for (int w = 0; w < TEAM / 32; w++) x += buf[w];
+	}
+	return x;
+}
+template <int TEAM>
+__device__ __forceinline__ void team_sync() {
+	if constexpr (TEAM > 32) __syncthreads();
+	else __syncwarp();
+}
+// A number that exactly `want` keys of [lo, hi) reach, or where equal keys forbid that, the want-th largest key: bit by bit from above until it divides
+template <int TEAM, typename K>
+__device__ __forceinline__ K divide_keys(const u64* key, int lo, int hi, int want, int tid, int* buf) {
+	K prefix = 0;
+	for (int bit = sizeof(K) * 8 - 1; bit >= 0; bit--) {
+		const K c = prefix | (K) 1 << bit;
+		int n = 0;
+		for (int j = lo + tid; j < hi; j += TEAM) n += (K) key[j] >= c;
+		n = team_sum<TEAM>(n, buf);
+		if (n >= want) prefix = c;
+		if (n == want) break;
+	}
+	return prefix;
+}
+constexpr int IN_REGS = 16; // keys that a lane holds
+// The same by one warp, keys in registers (zeros behind the last)
+__device__ __forceinline__ unsigned divide_regs(const unsigned (&k)[IN_REGS], int want) {
+	unsigned prefix = 0;
+	for (int bit = 31; bit >= 0; bit--) {
+		const unsigned c = prefix | 1u << bit;
+		int n = 0;
+#pragma unroll
+		for (int i = 0; i < IN_REGS; i++) n += k[i] >= c;
+		n = __reduce_add_sync(0xffffffffu, n);
+		if (n >= want) prefix = c;
+		if (n == want) break;
+	}
+	return prefix;
+}
+// (sum of the row's queries) . mean of page j, in 64 bits, by a warp
+template <typename T>
+__device__ __forceinline__ double exact_score(const SelectArgs& a, int s, int row, int g, int j) {
+	const int lane = threadIdx.x & 31, page = page_of(a.c, a.b, s, j);
+	double x = 0;
+	if (page >= 0)
+		for (int i = lane; i < a.c.d; i += 32) {
+			double qs = 0;
+			for (int r = 0; r < a.rep; r++) qs += (double) to_f(reinterpret_cast<const T*>(a.q)[(long long) row * a.q_row + (g * a.rep + r) * a.c.d + i]);
+			x = fma((double) to_f(reinterpret_cast<const T*>(a.c.means)[((long long) page * a.c.G + g) * a.c.d + i]), qs, x);
+		}
+#pragma unroll
+	for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+	return x;
+}
+
+// A row's list.  key[j] holds ordered32 of the fp32 scores of pages [lo, hi).
+template <typename T, int TEAM>
+__device__ void pick_pages(const SelectArgs& a, const Seq& q, int s, int row, int g, float err, u64* key, int tid, int* buf) {
+	const int lane = tid & 31;
+	const int pos = q.len - q.n + row - q.a, last = pos < 0 ? -1 : pos >> a.c.shift;
+	const int lo = min(a.first, last + 1), hi = max(last - a.recent, lo); // pages [lo, hi) are chosen by score, those before and from hi to last are always
+	const int fixed = lo + last + 1 - hi, want = min(a.top - fixed, hi - lo);
+	int* out = a.out + ((long long) row * a.c.G + g) * a.top;
+	const bool by_score = want > 0 && want < hi - lo;
+	u64 least = 0; // taken: keys above it, and the first `ties` of those equal to it
+	int ties = 0;
+	if (by_score) {
+		unsigned least32 = ~0u; // the want-th largest: the least of those that reach the dividing number
+		if (TEAM == 32 && hi - lo <= 32 * IN_REGS) {
+			unsigned k[IN_REGS];
+#pragma unroll
+			for (int i = 0; i < IN_REGS; i++) k[i] = lo + lane + 32 * i < hi ? (unsigned) key[lo + lane + 32 * i] : 0u;
+			const unsigned cut = divide_regs(k, want);
+#pragma unroll
+			for (int i = 0; i < IN_REGS; i++)
+				if (k[i] >= cut) least32 = min(least32, k[i]);
+		} else {
+			const unsigned cut = divide_keys<TEAM, unsigned>(key, lo, hi, want, tid, buf);
+			for (int j = lo + tid; j < hi; j += TEAM)
+				if ((unsigned) key[j] >= cut) least32 = min(least32, (unsigned) key[j]);
+		}
+		least32 = __reduce_min_sync(0xffffffffu, least32);
+		if constexpr (TEAM > 32) {
+			__syncthreads();
+			if (lane == 0) buf[tid >> 5] = (int) least32;
+			__syncthreads();
+			for (int w = 0; w < TEAM / 32; w++) least32 = min(least32, (unsigned) buf[w]);
+		}
+		const float t = unordered32(least32), up = t + 2.f * err, down = t - 2.f * err;
+		int sure = 0, near = 0;
+		for (int j = lo + tid; j < hi; j += TEAM) {
+			const float x = unordered32((unsigned) key[j]);
+			const bool above = x > up, below = x < down; // both false where something is not finite
+			sure += above;
+			near += !above && !below;
+			key[j] = above ? ~0ull : below ? 0ull : 1ull;
+		}
+		sure = team_sum<TEAM>(sure, buf);
+		near = team_sum<TEAM>(near, buf);
+		if (sure + near > want) { // the order of those between, in 64 bits
+			team_sync<TEAM>();
+			if (near <= 32) { // a lane holds one of them; what stands before it says whether it is taken
+				if (tid < 32) {
+					int n = 0, page = -1;
+					double x = 0;
+					for (int j0 = lo; j0 < hi; j0 += 32)
+						for (unsigned m = __ballot_sync(0xffffffffu, j0 + lane < hi && key[min(j0 + lane, hi - 1)] == 1); m; m &= m - 1, n++) {
+							const int j = j0 + __ffs(m) - 1;
+							const double e = exact_score<T>(a, s, row, g, j);
+							if (lane == n) { x = e; page = j; }
+						}
+					const u64 mine = page >= 0 ? ordered(x) : 0;
+					int rank = 0;
+					for (int i = 0; i < n; i++) {
+						const u64 o = __shfl_sync(0xffffffffu, mine, i);
+						rank += o > mine || (o == mine && i < lane);
+					}
+					__syncwarp();
+					if (page >= 0) key[page] = rank < want - sure ? 1ull : 0ull;
+				}
+			} else {
+				for (int j0 = lo + tid / 32; j0 < hi; j0 += TEAM / 32)
+					if (key[j0] == 1) {
+						const double x = exact_score<T>(a, s, row, g, j0);
+						__syncwarp();
+						if (lane == 0) key[j0] = ordered(x);
+						__syncwarp();
+					}
+				team_sync<TEAM>();
+				least = divide_keys<TEAM, u64>(key, lo, hi, want, tid, buf);
+				int above = 0, equal = 0;
+				for (int j = lo + tid; j < hi; j += TEAM) { above += key[j] > least; equal += key[j] == least; }
+				above = team_sum<TEAM>(above, buf);
+				equal = team_sum<TEAM>(equal, buf);
+				ties = want - above;
+			}
+		}
+	}
+	team_sync<TEAM>();
+	// in ascending order, a team's worth of pages at a time
+	int written = 0, tied = 0;
+	for (int base = 0; base <= last; base += TEAM) {
+		const int j = base + tid;
+		const bool mid = j >= lo && j < hi, tie = by_score && least && mid && key[j] == least;
+		int rank = 0; // among the ties before it
+		if (least) {
+			const unsigned tm = __ballot_sync(0xffffffffu, tie);
+			rank = tied + __popc(tm & ((1u << lane) - 1));
+			if constexpr (TEAM > 32) {
+				__syncthreads();
+				if (lane == 0) buf[tid >> 5] = __popc(tm);
+				__syncthreads();
+				for (int w = 0; w < TEAM / 32; w++) {
+					if (w < tid >> 5) rank += buf[w];
+					tied += buf[w];
+				}
+			} else tied += __popc(tm);
+		}
+		const bool take = j <= last && (mid ? (by_score ? key[j] > least || (tie && rank < ties) : want > 0) : true);
+		const unsigned om = __ballot_sync(0xffffffffu, take);
+		int at = written + __popc(om & ((1u << lane) - 1));
+		if constexpr (TEAM > 32) {
+			__syncthreads();
+			if (lane == 0) buf[tid >> 5] = __popc(om);
+			__syncthreads();
+			for (int w = 0; w < TEAM / 32; w++) {
+				if (w < tid >> 5) at += buf[w];
+				written += buf[w];
+			}
+		} else written += __popc(om);
+		if (take && at < a.top) out[at] = j;
+	}
+	for (int i = written + tid; i < a.top; i += TEAM) out[i] = -1;
+}
+
+// max |mean| as the bound takes it: infinite when something is not finite
+__device__ __forceinline__ float grow_bound(float m, const float (&v)[8]) {
+#pragma unroll
+	for (int e = 0; e < 8; e++) m = fabsf(v[e]) <= 3.4e38f ? fmaxf(m, fabsf(v[e])) : INFINITY;
+	return m;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(ST) paged_select_kernel(const SelectArgs a) {
-	extern __shared__ __align__(16) unsigned long long keys[]; // one per page
-	__shared__ double s_q[256];
-	__shared__ int s_hist[256], s_warp[ST / 32];
-	__shared__ unsigned long long s_prefix;
-	__shared__ int s_need;
-	pdl_wait();
+__global__ void __launch_bounds__(ST) paged_select_step_kernel(const __grid_constant__ SelectArgs a) {
+	extern __shared__ __align__(16) u64 keys[]; // one per page
+	__shared__ __align__(16) float s_q[256];
+	__shared__ float s_max[ST / 32], s_abs[ST / 32];
+	__shared__ int buf[ST / 32];
 	pdl_launch_dependents();
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, g = blockIdx.y, d = a.c.d;
 	const int s = seq_of_row(a.b, row);
 	const View view = view_of(a.c, a.b);
 	const Seq q = seq_of(view, s);
 	if (!row_in_seq(q, row)) return;
-	const int pos = q.len - q.n + row - q.a, last = pos < 0 ? -1 : pos >> a.c.shift;
-	if (tid == 0 && row == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
-	int* out = a.out + ((long long) row * a.c.G + g) * a.top;
-	const int lo = min(a.first, last + 1), hi = max(last - a.recent, lo); // pages [lo, hi) are chosen by score, those before and from hi to last are always
-	const int fixed = lo + last + 1 - hi, want = min(a.top - fixed, hi - lo);
-	unsigned long long least = 0; // keys above it are taken, of those equal to it the first `ties`
-	int ties = 0;
-	if (want > 0 && want < hi - lo) {
+	if (tid == 0 && g == 0 && row == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
+	const int pos = q.len - q.n + row - q.a, last = pos < 0 ? -1 : pos >> a.c.shift, lo = min(a.first, last + 1), hi = max(last - a.recent, lo);
+	float err = 0.f;
+	if (hi - lo > a.top - (lo + last + 1 - hi)) {
+		float abs_q = 0.f;
 		for (int i = tid; i < d; i += ST) {
-			double x = 0;
-			for (int r = 0; r < a.rep; r++) x += (double) to_f(reinterpret_cast<const T*>(a.q)[(long long) row * a.q_row + (g * a.rep + r) * d + i]);
+			float x = 0.f;
+			for (int r = 0; r < a.rep; r++) {
+				const float e = to_f(reinterpret_cast<const T*>(a.q)[(long long) row * a.q_row + (g * a.rep + r) * d + i]);
+				x += e;
+				abs_q += fabsf(e);
+			}
 			s_q[i] = x;
 		}
 		__syncthreads();
-		const int sub = lane & 7; // eight lanes to a page
-		for (int j0 = lo + warp * 4; j0 < hi; j0 += ST / 8) {
-			const int j = j0 + (lane >> 3);
-			const int page = j < hi ? page_of(a.c, a.b, s, j) : -1;
-			double x = 0;
-			if (page >= 0) {
-				const T* m = reinterpret_cast<const T*>(a.c.means) + ((long long) page * a.c.G + g) * d;
-				for (int c = sub * 8; c < d; c += 64) {
-					float v[8];
-					load8(m + c, v);
-#pragma unroll
-					for (int e = 0; e < 8; e++) x = fma((double) v[e], s_q[c + e], x);
-				}
-			} else if (j < hi && sub == 0) report(a.c, ERR_PAGE);
-#pragma unroll
-			for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-			if (sub == 0 && j < hi) keys[j] = ordered(x);
+		for (int j = lo + tid; j < hi; j += ST) { // which pages, all at once: a mean's address hangs on it
+			const int page = page_of(a.c, a.b, s, j);
+			if (page < 0) report(a.c, ERR_PAGE);
+			keys[j] = (u64) (unsigned) page;
 		}
-		if (tid == 0) { s_prefix = 0; s_need = want; }
-		// the want-th largest key, eight bits at a time
-		for (int shift = 56; shift >= 0; shift -= 8) {
-			s_hist[tid] = 0;
-			__syncthreads();
-			const unsigned long long prefix = s_prefix;
-			for (int j = lo + tid; j < hi; j += ST)
-				if (shift == 56 || keys[j] >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[(int) (keys[j] >> shift) & 255], 1);
-			__syncthreads();
-			if (warp == 0) { // from the top bin down: lane l holds bins 255 - 8 l .. 248 - 8 l
-				int n[8], sum = 0;
+		__syncthreads();
+		const int sub = lane & 7;
+		float most = 0.f;
+		for (int j0 = lo + warp * 4 + (lane >> 3); j0 < hi; j0 += 4 * (ST / 8)) { // four pages of each eight lanes on their way together
+			int page[4];
+			float x[4];
 #pragma unroll
-				for (int e = 0; e < 8; e++) { n[e] = s_hist[255 - lane * 8 - e]; sum += n[e]; }
-				int before = sum;
-#pragma unroll
-				for (int o = 1; o < 32; o <<= 1) {
-					const int x = __shfl_up_sync(0xffffffffu, before, o);
-					if (lane >= o) before += x;
-				}
-				before -= sum;
-				const int need = s_need;
-				__syncwarp();
-				if (before < need && before + sum >= need) {
-					int acc = before;
-#pragma unroll
-					for (int e = 0; e < 8; e++) {
-						if (acc < need && acc + n[e] >= need) {
-							s_prefix = prefix | (unsigned long long) (255 - lane * 8 - e) << shift;
-							s_need = need - acc;
-						}
-						acc += n[e];
-					}
-				}
+			for (int u = 0; u < 4; u++) {
+				const int j = j0 + u * (ST / 8);
+				page[u] = j < hi ? (int) keys[j] : -1;
+				x[u] = 0.f;
 			}
-			__syncthreads();
+			for (int c = sub * 8; c < d; c += 64) {
+				float v[4][8];
+#pragma unroll
+				for (int u = 0; u < 4; u++) load8(reinterpret_cast<const T*>(a.c.means) + ((long long) max(page[u], 0) * a.c.G + g) * d + c, v[u]);
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					if (page[u] >= 0) {
+						most = grow_bound(most, v[u]);
+#pragma unroll
+						for (int e = 0; e < 8; e++) x[u] = fmaf(v[u][e], s_q[c + e], x[u]);
+					}
+			}
+#pragma unroll
+			for (int u = 0; u < 4; u++) {
+				const unsigned mask = 0xffu << (lane & 24);
+#pragma unroll
+				for (int o = 4; o; o >>= 1) x[u] += __shfl_xor_sync(mask, x[u], o); // all eight have read their page
+				if (sub == 0 && j0 + u * (ST / 8) < hi) keys[j0 + u * (ST / 8)] = ordered32(x[u]);
+			}
 		}
-		least = s_prefix;
-		ties = s_need;
-	} else if (want > 0) {
-		least = 0; // all of them
+		most = warp_max(most);
+		abs_q = warp_sum(abs_q);
+		if (lane == 0) { s_max[warp] = most; s_abs[warp] = abs_q; }
+		__syncthreads();
+		most = abs_q = 0.f;
+		for (int w = 0; w < ST / 32; w++) { most = fmaxf(most, s_max[w]); abs_q += s_abs[w]; }
+		err = 1.1f * (float) (d + a.rep + 4) * 5.9604645e-8f * abs_q * most;
 	}
-	const bool by_score = want > 0 && want < hi - lo;
-	// in ascending order, a block's worth of pages at a time
-	int written = 0, tied = 0;
-	for (int base = 0; base <= last; base += ST) {
-		const int j = base + tid;
-		const bool mid = j >= lo && j < hi;
-		const bool tie = by_score && mid && keys[j] == least;
-		// place among the ties before it
-		const unsigned tm = __ballot_sync(0xffffffffu, tie);
-		__syncthreads();
-		if (lane == 0) s_warp[warp] = __popc(tm);
-		__syncthreads();
-		int rank = tied + __popc(tm & ((1u << lane) - 1));
-		for (int w = 0; w < ST / 32; w++) {
-			if (w < warp) rank += s_warp[w];
-			tied += s_warp[w];
-		}
-		const bool take = j <= last && (mid ? (by_score ? keys[j] > least || (tie && rank < ties) : want > 0) : true);
-		const unsigned om = __ballot_sync(0xffffffffu, take);
-		__syncthreads();
-		if (lane == 0) s_warp[warp] = __popc(om);
-		__syncthreads();
-		int at = written + __popc(om & ((1u << lane) - 1));
-		for (int w = 0; w < ST / 32; w++) {
-			if (w < warp) at += s_warp[w];
-			written += s_warp[w];
-		}
-		if (take && at < a.top) out[at] = j;
+	if (hi - lo <= 32 * IN_REGS) {
+		if (warp == 0) pick_pages<T, 32>(a, q, s, row, g, err, keys, lane, nullptr);
+	} else pick_pages<T, ST>(a, q, s, row, g, err, keys, tid, buf);
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_constant__ SelectArgs a) {
+	extern __shared__ __align__(16) uint8_t smem[];
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y, d = a.c.d, dp = d + 4;
+	u64* keys = reinterpret_cast<u64*>(smem);                              // [R][max_pages]
+	float* s_q = reinterpret_cast<float*>(keys + (size_t) R * a.b.max_pages); // [R][d]
+	float* s_m = s_q + R * d;                                              // [SP][d + 4]
+	float* s_abs = s_m + SP * dp;                                          // [R]
+	float* s_max = s_abs + R;                                              // [8]
+	pdl_launch_dependents();
+	// sequence s has room for floor(starts[s + 1] / R) - floor(starts[s] / R) + 1 blocks of rows, from number floor(starts[s] / R) + s on
+	int s = 0;
+	for (int n = a.b.B; n > 1;) {
+		const int step = (n + 31) / 32, at = lane * step;
+		const unsigned m = __ballot_sync(0xffffffffu, at < n && max(a.b.starts[s + at], 0) / R + s + at <= (int) blockIdx.x);
+		const int k = m ? 31 - __clz(m) : 0;
+		s += k * step;
+		n = min(step, n - k * step);
 	}
-	for (int i = written + tid; i < a.top; i += ST) out[i] = -1;
+	const View view = view_of(a.c, a.b);
+	const Seq q = seq_of(view, s);
+	const long long first = q.a + (long long) ((int) blockIdx.x - (q.a / R + s)) * R;
+	if (first < q.a || first >= q.a + q.n) return;
+	const int row0 = (int) first, rows = min(R, q.a + q.n - row0);
+	if (tid == 0 && g == 0 && row0 == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
+	for (int r = warp; r < R; r += ST / 32) {
+		float abs_q = 0.f;
+		for (int i = lane; i < d; i += 32) {
+			float x = 0.f;
+			if (r < rows)
+				for (int h = 0; h < a.rep; h++) {
+					const float e = to_f(reinterpret_cast<const T*>(a.q)[(long long) (row0 + r) * a.q_row + (g * a.rep + h) * d + i]);
+					x += e;
+					abs_q += fabsf(e);
+				}
+			s_q[r * d + i] = x;
+		}
+		abs_q = warp_sum(abs_q);
+		if (lane == 0) s_abs[r] = abs_q;
+	}
+	const int last = (q.len - q.n + row0 + rows - 1 - q.a) >> a.c.shift; // of the last row; negative where it sees nothing
+	const int lo = min(a.first, max(last + 1, 0)), hi = max(last - a.recent, lo);
+	float most = 0.f;
+	const int dc = d / 8;
+	for (int p0 = lo; p0 < hi; p0 += SP) {
+		__syncthreads();
+		for (int i = tid; i < SP * dc; i += ST) {
+			const int j = i / dc, c = (i - j * dc) * 8;
+			float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+			if (p0 + j < hi) {
+				const int page = page_of(a.c, a.b, s, p0 + j);
+				if (page >= 0) load8(reinterpret_cast<const T*>(a.c.means) + ((long long) page * a.c.G + g) * d + c, v);
+				else if (c == 0) report(a.c, ERR_PAGE);
+			}
+			most = grow_bound(most, v);
+			*reinterpret_cast<float4*>(s_m + j * dp + c) = make_float4(v[0], v[1], v[2], v[3]);
+			*reinterpret_cast<float4*>(s_m + j * dp + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+		}
+		__syncthreads();
+		const int j = tid & (SP - 1), r0 = tid / SP * (R / 4);
+		float x[R / 4];
+#pragma unroll
+		for (int r = 0; r < R / 4; r++) x[r] = 0.f;
+		for (int c = 0; c < d; c += 4) {
+			const float4 m = *reinterpret_cast<const float4*>(s_m + j * dp + c);
+#pragma unroll
+			for (int r = 0; r < R / 4; r++) {
+				const float4 e = *reinterpret_cast<const float4*>(s_q + (r0 + r) * d + c);
+				x[r] = fmaf(m.x, e.x, fmaf(m.y, e.y, fmaf(m.z, e.z, fmaf(m.w, e.w, x[r]))));
+			}
+		}
+		if (p0 + j < hi)
+#pragma unroll
+			for (int r = 0; r < R / 4; r++) keys[(size_t) (r0 + r) * a.b.max_pages + p0 + j] = ordered32(x[r]);
+	}
+	most = warp_max(most);
+	if (lane == 0) s_max[warp] = most;
+	__syncthreads();
+	most = 0.f;
+	for (int w = 0; w < ST / 32; w++) most = fmaxf(most, s_max[w]);
+	for (int r = warp; r < rows; r += ST / 32)
+		pick_pages<T, 32>(a, q, s, row0 + r, g, 1.1f * (float) (d + a.rep + 4) * 5.9604645e-8f * s_abs[r] * most, keys + (size_t) r * a.b.max_pages, lane, nullptr);
+}
+
+template <typename T>
+static int select_typed(const SelectArgs& a, cudaStream_t s) {
+	// 16 rows to a CTA where their scores fit beside one another (R rows of p pages: 8 R p bytes), 8 up to twice as many pages, else and for single tokens one
+	const int R = a.b.N <= a.b.B ? 1 : a.b.max_pages <= 1024 ? 16 : a.b.max_pages <= 2048 ? 8 : 1;
+	const size_t smem = (size_t) R * a.b.max_pages * 8 + (R > 1 ? (size_t) (R * a.c.d + SP * (a.c.d + 4) + R + ST / 32) * 4 : 0);
+	const dim3 grid((unsigned) (R > 1 ? a.b.N / R + a.b.B : a.b.N), (unsigned) a.c.G);
+	void (*kernel)(SelectArgs) = R == 16 ? paged_select_rows_kernel<T, 16> : R == 8 ? paged_select_rows_kernel<T, 8> : paged_select_step_kernel<T>;
+	if (smem > 48 * 1024) XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	kernel<<<grid, ST, smem, s>>>(a);
+	XALM_CUDA_CHECK(cudaGetLastError());
+	return XALM_OK;
 }
 
 // ---- checks and launches -----------------------------------------------------------------------------------------------------------------------
@@ -560,8 +816,7 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
 	if (heads <= 0 || heads % a.c.G || heads > 65535) return set_error(XALM_ERR_INVALID, "paged select: %d query heads over %d", heads, a.c.G);
 	if (top <= 0 || top > MAX_LIST || first < 0 || recent < 0 || first > top || recent > top || first + recent + 1 > top)
 		return set_error(XALM_ERR_INVALID, "paged select: %d pages, of them the first %d, %d recent ones and the token's own (at most %d)", top, first, recent, MAX_LIST);
-	const size_t smem = (size_t) a.b.max_pages * 8;
-	if (smem > 192 * 1024) return set_error(XALM_ERR_INVALID, "paged select: sequences of %d pages (at most %d)", a.b.max_pages, 192 * 1024 / 8);
+	if (a.b.max_pages > 24576) return set_error(XALM_ERR_INVALID, "paged select: sequences of %d pages (at most 24576)", a.b.max_pages);
 	if (a.b.N) {
 		XALM_TRY(check_rows("q", q, q_row, heads * a.c.d, element_bytes(cache->type)));
 		if (!out) return set_error(XALM_ERR_INVALID, "paged select: out is NULL");
@@ -577,11 +832,8 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
 	a.first = first;
 	a.recent = recent;
 	a.out = out;
-	void (*kernel)(SelectArgs) = cache->type == XALM_F32 ? paged_select_kernel<float> : cache->type == XALM_F16 ? paged_select_kernel<__half> : paged_select_kernel<__nv_bfloat16>;
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-	kernel<<<dim3((unsigned) a.b.N, (unsigned) a.c.G), ST, smem, (cudaStream_t) stream>>>(a);
-	XALM_CUDA_CHECK(cudaGetLastError());
-	return XALM_OK;
+	cudaStream_t s = (cudaStream_t) stream;
+	return cache->type == XALM_F32 ? select_typed<float>(a, s) : cache->type == XALM_F16 ? select_typed<__half>(a, s) : select_typed<__nv_bfloat16>(a, s);
 }
 
 } // extern "C"

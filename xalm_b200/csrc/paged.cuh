@@ -66,6 +66,7 @@ __device__ __forceinline__ int2 group_of(const View& v, int i) {
 // The sequence of a row: the last s with starts[s] <= row.  A whole warp asks, with 32 probes a round.
 __device__ __forceinline__ int seq_of_row(const BatchView& b, int row) {
 	const int lane = threadIdx.x & 31;
+	if (row < b.B && b.starts[row] <= row && b.starts[row + 1] > row) return row; // steps of single tokens: one asking of memory
 	int lo = 0, n = b.B; // the answer lies in [lo, lo + n)
 	while (n > 1) {
 		const int step = (n + 31) / 32, at = lane * step;
