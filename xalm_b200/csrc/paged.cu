@@ -14,9 +14,9 @@ namespace xalm {
 namespace paged {
 
 // =========================================================================================================================================
-// append: a CTA per new token; row's position p = len - n + i, page table[p / P], slot p % P.  Bound by HBM (every element in and out once): a thread takes
-// eight neighbouring elements of a head, and its partners of the rotation from the same 16 or 32 bytes or from the chunk half a rotation away (the second
-// reading of a line hits L1).  The angle p * freq is taken in 64 bits and brought into [-pi, pi] there: in 32 bits position 100000 is 0.004 rad off.
+// append: a row's position is p = len - n + i, its page table[p / P], its slot p % P.  Bound by HBM (every element in and out once), so a thread takes 16 or 32 bytes of a head
+// with those half a rotation away that they are turned with, of R rows at once: R = 4 keeps enough bytes on their way in prompts; steps of few tokens
+// have a CTA to a row.  The angle p * freq is taken in 64 bits and brought into [-pi, pi] there: in 32 bits position 100000 is 0.004 rad off.
 // =========================================================================================================================================
 struct AppendArgs {
 	Cache c;
@@ -29,77 +29,122 @@ struct AppendArgs {
 	int rot;
 	float mag;
 	int neighbours;
+	int paired;                 // halves whose chunks of eight pair up: a thread takes both
+	int per_head, per_value;    // work items of a head of q or k, of v
+	unsigned by_head, by_value; // 2^32 / those, rounded up (0 for one)
 };
 
 constexpr int AT = 256;
 
-template <typename I, typename T>
-__global__ void __launch_bounds__(AT) paged_append_kernel(const AppendArgs a) {
-	__shared__ float s_cos[128], s_sin[128];
-	pdl_wait();
-	pdl_launch_dependents();
-	const int row = blockIdx.x, tid = threadIdx.x, d = a.c.d, dv = a.c.dv, G = a.c.G;
-	const int s = seq_of_row(a.b, row);
-	const View view = view_of(a.c, a.b);
-	const Seq q = seq_of(view, s);
-	const bool in = row >= q.a && row < q.a + q.n;
-	if (tid == 0 && row == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
-	if (!in) return; // behind the last sequence
-	const int pos = q.len - q.n + row - q.a;
-	if (pos < 0) return;
-	const int page = page_of(a.c, a.b, s, pos >> a.c.shift), slot = pos & ((1 << a.c.shift) - 1);
-	if (page < 0 && tid == 0) report(a.c, ERR_PAGE);
-	for (int i = tid; i < a.rot; i += AT) {
-		const double x = (double) pos * (double) a.freq[i], turns = rint(x * 0.15915494309189535);
-		float sn, cs;
-		sincosf((float) fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x)), &sn, &cs); // 2 pi as the sum of two doubles
-		s_cos[i] = cs * a.mag;
-		s_sin[i] = sn * a.mag;
+template <typename I>
+struct Chunk { // eight elements as they came
+	uint4 u[sizeof(I) / 2];
+	__device__ __forceinline__ void load(const I* p) {
+#pragma unroll
+		for (int i = 0; i < (int) sizeof(I) / 2; i++) u[i] = reinterpret_cast<const uint4*>(p)[i];
 	}
-	__syncthreads();
-	const int dc = d / 8, vc = dv / 8, n_q = a.q ? a.H * dc : 0, n_k = n_q + G * dc, n_all = n_k + (page < 0 ? 0 : G * vc);
-	for (int i = tid; i < n_all; i += AT) {
-		float x[8];
-		if (i >= n_k) { // a value
-			const int h = (i - n_k) / vc, c = (i - n_k) % vc * 8;
-			load8(reinterpret_cast<const I*>(a.v) + (long long) row * a.v_row + h * dv + c, x);
-			store8(reinterpret_cast<T*>(a.c.v) + page * a.c.v_page + slot * a.c.v_slot + h * a.c.v_head + c, x);
-			continue;
-		}
-		const bool key = i >= n_q;
-		if (key && page < 0) break;
-		const int h = (key ? i - n_q : i) / dc, c = (key ? i - n_q : i) % dc * 8;
-		const I* in_head = key ? reinterpret_cast<const I*>(a.k) + (long long) row * a.k_row + h * d : reinterpret_cast<const I*>(a.q) + (long long) row * a.q_row + h * d;
-		load8(in_head + c, x);
-		float y[8];
+	__device__ __forceinline__ void floats(float (&x)[8]) const {
+		const I* t = reinterpret_cast<const I*>(u);
 #pragma unroll
-		for (int e = 0; e < 8; e++) y[e] = x[e];
-		if (c < 2 * a.rot) {
-			if (a.neighbours) {
-#pragma unroll
-				for (int e = 0; e < 8; e += 2) {
-					const int f = (c + e) / 2;
-					if (f < a.rot) {
-						y[e] = x[e] * s_cos[f] - x[e + 1] * s_sin[f];
-						y[e + 1] = x[e + 1] * s_cos[f] + x[e] * s_sin[f];
-					}
-				}
-			} else {
-				const bool low = c < a.rot;
-				float p[8];
-				if (a.rot % 8 == 0) load8(in_head + (low ? c + a.rot : c - a.rot), p); // a chunk lies in one half
-#pragma unroll
-				for (int e = 0; e < 8; e++) {
-					const int at = c + e;
-					if (at >= 2 * a.rot) continue;
-					const int f = at < a.rot ? at : at - a.rot;
-					const float o = a.rot % 8 == 0 ? p[e] : to_f(in_head[at < a.rot ? at + a.rot : at - a.rot]);
-					y[e] = at < a.rot ? x[e] * s_cos[f] - o * s_sin[f] : x[e] * s_cos[f] + o * s_sin[f];
+		for (int i = 0; i < 8; i++) x[i] = to_f(t[i]);
+	}
+};
+
+template <typename I, typename T, int R>
+__global__ void __launch_bounds__(AT) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+	__shared__ float s_cos[R][128], s_sin[R][128];
+	__shared__ int s_pos[R], s_page[R]; // position (-1: not a row of any sequence, or before its first token), page of the pool (-1: none)
+	pdl_launch_dependents();
+	const int row0 = blockIdx.x * R, tid = threadIdx.x, warp = tid >> 5, d = a.c.d, dv = a.c.dv, G = a.c.G;
+	if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, AT);
+	if (warp < R) {
+		const int row = row0 + warp;
+		int pos = -1, page = -1;
+		if (row < a.b.N) {
+			const int s = seq_of_row(a.b, row);
+			const View view = view_of(a.c, a.b);
+			const Seq q = seq_of(view, s);
+			if (row_in_seq(q, row)) {
+				pos = q.len - q.n + row - q.a;
+				if (pos >= 0) {
+					page = page_of(a.c, a.b, s, pos >> a.c.shift);
+					if (page < 0 && (tid & 31) == 0) report(a.c, ERR_PAGE);
 				}
 			}
 		}
-		if (key) store8(reinterpret_cast<T*>(a.c.k) + page * a.c.k_page + slot * a.c.k_slot + h * a.c.k_head + c, y);
-		else store8(reinterpret_cast<T*>(a.q_out) + (long long) row * a.q_out_row + h * d + c, y);
+		if ((tid & 31) == 0) { s_pos[warp] = pos; s_page[warp] = page; }
+	}
+	__syncthreads();
+	for (int i = tid; i < R * a.rot; i += AT) {
+		const int r = i / a.rot, f = i - r * a.rot;
+		if (s_pos[r] < 0) continue;
+		const double x = (double) s_pos[r] * (double) a.freq[f], turns = rint(x * 0.15915494309189535);
+		float sn, cs;
+		sincosf((float) fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x)), &sn, &cs); // 2 pi as the sum of two doubles
+		s_cos[r][f] = cs * a.mag;
+		s_sin[r][f] = sn * a.mag;
+	}
+	__syncthreads();
+	const int n_q = a.q ? a.H * a.per_head : 0, n_k = n_q + G * a.per_head, n_all = n_k + G * a.per_value, slot_mask = (1 << a.c.shift) - 1;
+	for (int i = tid; i < n_all; i += AT) {
+		const bool value = i >= n_k, key = !value && i >= n_q;
+		const int j = value ? i - n_k : key ? i - n_q : i, per = value ? a.per_value : a.per_head;
+		const int h = per == 1 ? j : (int) __umulhi((unsigned) j, value ? a.by_value : a.by_head), u = j - h * per;
+		const int c = value || !a.paired || u * 8 < a.rot ? u * 8 : u * 8 + a.rot; // the item's first element; behind the pairs come the chunks that are not turned
+		const bool pair = !value && a.paired && u * 8 < a.rot;
+		const I* in = value ? reinterpret_cast<const I*>(a.v) + h * dv + c : key ? reinterpret_cast<const I*>(a.k) + h * d + c : reinterpret_cast<const I*>(a.q) + h * d + c;
+		const long long step = value ? a.v_row : key ? a.k_row : a.q_row;
+		Chunk<I> x[R], y[R];
+		bool go[R];
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			go[r] = s_pos[r] >= 0 && !((value || key) && s_page[r] < 0);
+			if (!go[r]) continue;
+			x[r].load(in + (row0 + r) * step);
+			if (pair) y[r].load(in + (row0 + r) * step + a.rot);
+		}
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			if (!go[r]) continue;
+			float lo[8], hi[8];
+			x[r].floats(lo);
+			T* out = value ? reinterpret_cast<T*>(a.c.v) + s_page[r] * a.c.v_page + (s_pos[r] & slot_mask) * a.c.v_slot + h * a.c.v_head + c
+			         : key ? reinterpret_cast<T*>(a.c.k) + s_page[r] * a.c.k_page + (s_pos[r] & slot_mask) * a.c.k_slot + h * a.c.k_head + c
+			               : reinterpret_cast<T*>(a.q_out) + (row0 + r) * a.q_out_row + h * d + c;
+			if (pair) {
+				y[r].floats(hi);
+#pragma unroll
+				for (int e = 0; e < 8; e++) {
+					const float cs = s_cos[r][c + e], sn = s_sin[r][c + e], l = lo[e];
+					lo[e] = l * cs - hi[e] * sn;
+					hi[e] = hi[e] * cs + l * sn;
+				}
+				store8(out + a.rot, hi);
+			} else if (!value && !a.paired && c < 2 * a.rot) {
+				if (a.neighbours) {
+#pragma unroll
+					for (int e = 0; e < 8; e += 2) {
+						const int f = (c + e) / 2;
+						if (f < a.rot) {
+							const float l = lo[e];
+							lo[e] = l * s_cos[r][f] - lo[e + 1] * s_sin[r][f];
+							lo[e + 1] = lo[e + 1] * s_cos[r][f] + l * s_sin[r][f];
+						}
+					}
+				} else { // halves that end inside a chunk
+					const I* head = in - c + (row0 + r) * step;
+#pragma unroll
+					for (int e = 0; e < 8; e++) {
+						const int at = c + e;
+						if (at >= 2 * a.rot) continue;
+						const int f = at < a.rot ? at : at - a.rot;
+						const float o = to_f(head[at < a.rot ? at + a.rot : f]);
+						lo[e] = at < a.rot ? lo[e] * s_cos[r][f] - o * s_sin[r][f] : lo[e] * s_cos[r][f] + o * s_sin[r][f];
+					}
+				}
+			}
+			store8(out, lo);
+		}
 	}
 }
 
@@ -378,17 +423,17 @@ __global__ void __launch_bounds__(ST) paged_select_step_kernel(const __grid_cons
 	__shared__ int buf[ST / 32];
 	pdl_launch_dependents();
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, g = blockIdx.y, d = a.c.d;
+	if (row == 0 && g == 0) check_seqs(a.c, a.b, tid, ST);
 	const int s = seq_of_row(a.b, row);
-	const View view = view_of(a.c, a.b);
-	const Seq q = seq_of(view, s);
+	const Seq q = seq_of(view_of(a.c, a.b), s);
 	if (!row_in_seq(q, row)) return;
-	if (tid == 0 && g == 0 && row == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
 	const int pos = q.len - q.n + row - q.a, last = pos < 0 ? -1 : pos >> a.c.shift, lo = min(a.first, last + 1), hi = max(last - a.recent, lo);
 	float err = 0.f;
 	if (hi - lo > a.top - (lo + last + 1 - hi)) {
 		float abs_q = 0.f;
 		for (int i = tid; i < d; i += ST) {
 			float x = 0.f;
+#pragma unroll 4
 			for (int r = 0; r < a.rep; r++) {
 				const float e = to_f(reinterpret_cast<const T*>(a.q)[(long long) row * a.q_row + (g * a.rep + r) * d + i]);
 				x += e;
@@ -454,9 +499,11 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 	u64* keys = reinterpret_cast<u64*>(smem);                              // [R][max_pages]
 	float* s_q = reinterpret_cast<float*>(keys + (size_t) R * a.b.max_pages); // [R][d]
 	float* s_m = s_q + R * d;                                              // [SP][d + 4]
-	float* s_abs = s_m + SP * dp;                                          // [R]
-	float* s_max = s_abs + R;                                              // [8]
+	float* s_abs = s_m + SP * dp;                                          // [R][d / 8]
+	float* s_max = s_abs + R * (d / 8);                                    // [8]
+	int* s_page = reinterpret_cast<int*>(s_max + ST / 32);                 // [max_pages]
 	pdl_launch_dependents();
+	if (blockIdx.x == 0 && g == 0) check_seqs(a.c, a.b, tid, ST);
 	// sequence s has room for floor(starts[s + 1] / R) - floor(starts[s] / R) + 1 blocks of rows, from number floor(starts[s] / R) + s on
 	int s = 0;
 	for (int n = a.b.B; n > 1;) {
@@ -466,44 +513,55 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 		s += k * step;
 		n = min(step, n - k * step);
 	}
-	const View view = view_of(a.c, a.b);
-	const Seq q = seq_of(view, s);
+	const Seq q = seq_of(view_of(a.c, a.b), s);
 	const long long first = q.a + (long long) ((int) blockIdx.x - (q.a / R + s)) * R;
 	if (first < q.a || first >= q.a + q.n) return;
 	const int row0 = (int) first, rows = min(R, q.a + q.n - row0);
-	if (tid == 0 && g == 0 && row0 == q.a && !seq_ok(view, s)) report(a.c, ERR_BATCH);
-	for (int r = warp; r < R; r += ST / 32) {
-		float abs_q = 0.f;
-		for (int i = lane; i < d; i += 32) {
-			float x = 0.f;
-			if (r < rows)
-				for (int h = 0; h < a.rep; h++) {
-					const float e = to_f(reinterpret_cast<const T*>(a.q)[(long long) (row0 + r) * a.q_row + (g * a.rep + h) * d + i]);
-					x += e;
-					abs_q += fabsf(e);
-				}
-			s_q[r * d + i] = x;
+	const int dc = d / 8;
+	for (int i = tid; i < R * dc; i += ST) { // eight entries of a row's sum
+		const int r = i / dc, c = (i - r * dc) * 8;
+		float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, abs_q = 0.f;
+		if (r < rows) {
+			const T* at = reinterpret_cast<const T*>(a.q) + (long long) (row0 + r) * a.q_row + g * a.rep * d + c;
+#pragma unroll 4
+			for (int h = 0; h < a.rep; h++) {
+				float v[8];
+				load8(at + h * d, v);
+#pragma unroll
+				for (int e = 0; e < 8; e++) { sum[e] += v[e]; abs_q += fabsf(v[e]); }
+			}
 		}
-		abs_q = warp_sum(abs_q);
-		if (lane == 0) s_abs[r] = abs_q;
+#pragma unroll
+		for (int e = 0; e < 8; e++) s_q[r * d + c + e] = sum[e];
+		s_abs[i] = abs_q;
 	}
 	const int last = (q.len - q.n + row0 + rows - 1 - q.a) >> a.c.shift; // of the last row; negative where it sees nothing
 	const int lo = min(a.first, max(last + 1, 0)), hi = max(last - a.recent, lo);
+	for (int j = lo + tid; j < hi; j += ST) { // which pages, all at once: a mean's address hangs on it
+		s_page[j] = page_of(a.c, a.b, s, j);
+		if (s_page[j] < 0) report(a.c, ERR_PAGE);
+	}
 	float most = 0.f;
-	const int dc = d / 8;
 	for (int p0 = lo; p0 < hi; p0 += SP) {
 		__syncthreads();
-		for (int i = tid; i < SP * dc; i += ST) {
-			const int j = i / dc, c = (i - j * dc) * 8;
-			float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-			if (p0 + j < hi) {
-				const int page = page_of(a.c, a.b, s, p0 + j);
-				if (page >= 0) load8(reinterpret_cast<const T*>(a.c.means) + ((long long) page * a.c.G + g) * d + c, v);
-				else if (c == 0) report(a.c, ERR_PAGE);
+		for (int i0 = tid; i0 < SP * dc; i0 += 4 * ST) {
+			float v[4][8];
+#pragma unroll
+			for (int u = 0; u < 4; u++) {
+				const int i = i0 + u * ST, j = i / dc, page = i < SP * dc && p0 + j < hi ? s_page[p0 + j] : -1;
+				load8(reinterpret_cast<const T*>(a.c.means) + ((long long) max(page, 0) * a.c.G + g) * d + (i - j * dc) * 8, v[u]);
+				if (page < 0)
+#pragma unroll
+					for (int e = 0; e < 8; e++) v[u][e] = 0.f;
 			}
-			most = grow_bound(most, v);
-			*reinterpret_cast<float4*>(s_m + j * dp + c) = make_float4(v[0], v[1], v[2], v[3]);
-			*reinterpret_cast<float4*>(s_m + j * dp + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+			for (int u = 0; u < 4; u++) {
+				const int i = i0 + u * ST, j = i / dc, c = (i - j * dc) * 8;
+				if (i >= SP * dc) break;
+				most = grow_bound(most, v[u]);
+				*reinterpret_cast<float4*>(s_m + j * dp + c) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+				*reinterpret_cast<float4*>(s_m + j * dp + c + 4) = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
+			}
 		}
 		__syncthreads();
 		const int j = tid & (SP - 1), r0 = tid / SP * (R / 4);
@@ -527,15 +585,17 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 	__syncthreads();
 	most = 0.f;
 	for (int w = 0; w < ST / 32; w++) most = fmaxf(most, s_max[w]);
-	for (int r = warp; r < rows; r += ST / 32)
-		pick_pages<T, 32>(a, q, s, row0 + r, g, 1.1f * (float) (d + a.rep + 4) * 5.9604645e-8f * s_abs[r] * most, keys + (size_t) r * a.b.max_pages, lane, nullptr);
+	for (int r = warp; r < rows; r += ST / 32) {
+		const float abs_q = warp_sum(lane < dc ? s_abs[r * dc + lane] : 0.f);
+		pick_pages<T, 32>(a, q, s, row0 + r, g, 1.1f * (float) (d + a.rep + 4) * 5.9604645e-8f * abs_q * most, keys + (size_t) r * a.b.max_pages, lane, nullptr);
+	}
 }
 
 template <typename T>
 static int select_typed(const SelectArgs& a, cudaStream_t s) {
 	// 16 rows to a CTA where their scores fit beside one another (R rows of p pages: 8 R p bytes), 8 up to twice as many pages, else and for single tokens one
 	const int R = a.b.N <= a.b.B ? 1 : a.b.max_pages <= 1024 ? 16 : a.b.max_pages <= 2048 ? 8 : 1;
-	const size_t smem = (size_t) R * a.b.max_pages * 8 + (R > 1 ? (size_t) (R * a.c.d + SP * (a.c.d + 4) + R + ST / 32) * 4 : 0);
+	const size_t smem = (size_t) R * a.b.max_pages * 8 + (R > 1 ? (size_t) (R * a.c.d + SP * (a.c.d + 4) + R * a.c.d / 8 + ST / 32 + a.b.max_pages) * 4 : 0);
 	const dim3 grid((unsigned) (R > 1 ? a.b.N / R + a.b.B : a.b.N), (unsigned) a.c.G);
 	void (*kernel)(SelectArgs) = R == 16 ? paged_select_rows_kernel<T, 16> : R == 8 ? paged_select_rows_kernel<T, 8> : paged_select_step_kernel<T>;
 	if (smem > 48 * 1024) XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
@@ -751,9 +811,17 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 	a.H = heads;
 	a.freq = freq; a.rot = rot_half; a.mag = rot_mag; a.neighbours = neighbours;
 	cudaStream_t s = (cudaStream_t) stream;
+	a.paired = !neighbours && rot_half % 8 == 0;
+	a.per_head = (a.c.d - (a.paired ? rot_half : 0)) / 8;
+	a.per_value = a.c.dv / 8;
+	a.by_head = (unsigned) ((0x100000000ull + a.per_head - 1) / a.per_head);
+	a.by_value = (unsigned) ((0x100000000ull + a.per_value - 1) / a.per_value);
+	int sms = 0;
+	XALM_TRY(sm_count(cache->device, &sms));
+	const bool many = a.b.N >= sms * 4; // four rows to a CTA once that still gives every SM one
 	void (*kernel)(AppendArgs) = nullptr;
 	switch (in_type * 16 + cache->type) {
-#define XALM_PAGED_APPEND(I, IT, C, CT) case IT * 16 + CT: kernel = paged_append_kernel<I, C>; break;
+#define XALM_PAGED_APPEND(I, IT, C, CT) case IT * 16 + CT: kernel = many ? paged_append_kernel<I, C, 4> : paged_append_kernel<I, C, 1>; break;
 		XALM_PAGED_APPEND(float, XALM_F32, float, XALM_F32)
 		XALM_PAGED_APPEND(float, XALM_F32, __half, XALM_F16)
 		XALM_PAGED_APPEND(float, XALM_F32, __nv_bfloat16, XALM_BF16)
@@ -765,7 +833,7 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 		XALM_PAGED_APPEND(__nv_bfloat16, XALM_BF16, __nv_bfloat16, XALM_BF16)
 #undef XALM_PAGED_APPEND
 	}
-	kernel<<<a.b.N, AT, 0, s>>>(a);
+	kernel<<<many ? (a.b.N + 3) / 4 : a.b.N, AT, 0, s>>>(a);
 	XALM_CUDA_CHECK(cudaGetLastError());
 	if (a.c.means) {
 		const dim3 grid((unsigned) ((a.b.N >> a.c.shift) + a.b.B), (unsigned) a.c.G);

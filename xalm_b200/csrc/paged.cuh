@@ -58,6 +58,12 @@ __device__ __forceinline__ bool seq_ok(const View& v, int s) {
 	const int a = v.starts[s], e = v.starts[s + 1], l = v.lens[s];
 	return a >= 0 && e >= a && e <= v.N && l >= e - a && l <= v.cap;
 }
+// One CTA of a call looks all sequences over
+__device__ __forceinline__ void check_seqs(const Cache& c, const BatchView& b, int tid, int threads) {
+	const View v = view_of(c, b);
+	for (int s = tid; s < b.B; s += threads)
+		if (!seq_ok(v, s)) report(c, ERR_BATCH);
+}
 // The sequences of a group
 __device__ __forceinline__ int2 group_of(const View& v, int i) {
 	const int s0 = min(max(v.bounds[i], 0), v.B);
@@ -240,6 +246,9 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 		m = __reduce_min_sync(0xffffffffu, m) >> a.c.shift << a.c.shift;
 		for (int s = g.x + lane; s < g.y; s += 32) p.shs[s] = m;
 	}
+	if (blockIdx.x == 0)
+		for (int s = tid; s < B; s += NT)
+			if (!seq_ok(p.v, s)) report(a.c, ERR_BATCH);
 	if (n) __syncthreads();
 	long long carry_w = 0;
 	int carry_u = 0;
@@ -259,7 +268,6 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 					if (tiles <= 4) {
 						for (int t = 0; t < tiles; t++) w += unit_work(a, part, seg, rows, q, p.shs[s], t);
 					} else wide = true;
-					if (part.cum_w && blockIdx.x == 0 && !seq_ok(p.v, s)) report(a.c, ERR_BATCH);
 				}
 				in_seg = tiles;
 			}

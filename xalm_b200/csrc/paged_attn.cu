@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 	pdl_wait();
 	pdl_launch_dependents();
 	if (!LIST) make_plan<RT>(a, part, s_plan, plan);
+	else if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, RT);
 	Walk k;
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
 	if (tid == 0)

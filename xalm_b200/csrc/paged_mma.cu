@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	pdl_launch_dependents();
 	Plan plan;
 	if (!LIST) make_plan<MT>(a, part, s_plan, plan);
+	else if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, MT);
 	__syncthreads();
 	const int dc = (a.c.d + 63) / 64, vc = (a.c.dv + 63) / 64;
 	const int P = 1 << a.c.shift, W = min(P, KT), per = KT / W; // slots of a box, boxes of a tile's column
