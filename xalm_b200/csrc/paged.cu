@@ -257,20 +257,47 @@ __device__ __forceinline__ K divide_keys(const u64* key, int lo, int hi, int wan
 	}
 	return prefix;
 }
-constexpr int IN_REGS = 16; // keys that a lane holds
-// The same by one warp, keys in registers (zeros behind the last)
-__device__ __forceinline__ unsigned divide_regs(const unsigned (&k)[IN_REGS], int want) {
-	unsigned prefix = 0;
-	for (int bit = 31; bit >= 0; bit--) {
-		const unsigned c = prefix | 1u << bit;
+constexpr int IN_REGS = 16; // keys that a lane holds at most
+// The want-th largest of keys [lo, hi) by one warp, N to a lane in registers.  Halving the scores' range divides them in six or seven counts where they are spread evenly, bits
+// need fourteen; bits where that fails (equal scores, some far from all others, some not finite).
+template <int N>
+__device__ __forceinline__ unsigned nth_in_regs(const u64* key, int lo, int hi, int want) {
+	const int lane = threadIdx.x & 31;
+	unsigned k[N], top = 0, low = ~0u;
+#pragma unroll
+	for (int i = 0; i < N; i++) {
+		const int j = lo + lane + 32 * i;
+		k[i] = j < hi ? (unsigned) key[j] : 0u;
+		top = max(top, k[i]);
+		if (j < hi) low = min(low, k[i]);
+	}
+	float up = unordered32(__reduce_max_sync(0xffffffffu, top)), down = unordered32(__reduce_min_sync(0xffffffffu, low));
+	unsigned cut = 0;
+	for (int step = 0; step < 20; step++) {
+		const float mid = 0.5f * up + 0.5f * down;
+		const unsigned c = ordered32(mid);
 		int n = 0;
 #pragma unroll
-		for (int i = 0; i < IN_REGS; i++) n += k[i] >= c;
+		for (int i = 0; i < N; i++) n += k[i] >= c;
 		n = __reduce_add_sync(0xffffffffu, n);
-		if (n >= want) prefix = c;
-		if (n == want) break;
+		if (n == want) { cut = c; break; }
+		(n > want ? down : up) = mid;
 	}
-	return prefix;
+	if (!cut)
+		for (int bit = 31; bit >= 0; bit--) {
+			const unsigned c = cut | 1u << bit;
+			int n = 0;
+#pragma unroll
+			for (int i = 0; i < N; i++) n += k[i] >= c;
+			n = __reduce_add_sync(0xffffffffu, n);
+			if (n >= want) cut = c;
+			if (n == want) break;
+		}
+	unsigned least = ~0u;
+#pragma unroll
+	for (int i = 0; i < N; i++)
+		if (k[i] >= cut) least = min(least, k[i]);
+	return least;
 }
 // (sum of the row's queries) . mean of page j, in 64 bits, by a warp
 template <typename T>
@@ -301,15 +328,9 @@ __device__ void pick_pages(const SelectArgs& a, const Seq& q, int s, int row, in
 	int ties = 0;
 	if (by_score) {
 		unsigned least32 = ~0u; // the want-th largest: the least of those that reach the dividing number
-		if (TEAM == 32 && hi - lo <= 32 * IN_REGS) {
-			unsigned k[IN_REGS];
-#pragma unroll
-			for (int i = 0; i < IN_REGS; i++) k[i] = lo + lane + 32 * i < hi ? (unsigned) key[lo + lane + 32 * i] : 0u;
-			const unsigned cut = divide_regs(k, want);
-#pragma unroll
-			for (int i = 0; i < IN_REGS; i++)
-				if (k[i] >= cut) least32 = min(least32, k[i]);
-		} else {
+		if (TEAM == 32 && hi - lo <= 256) least32 = nth_in_regs<8>(key, lo, hi, want);
+		else if (TEAM == 32 && hi - lo <= 32 * IN_REGS) least32 = nth_in_regs<IN_REGS>(key, lo, hi, want);
+		else {
 			const unsigned cut = divide_keys<TEAM, unsigned>(key, lo, hi, want, tid, buf);
 			for (int j = lo + tid; j < hi; j += TEAM)
 				if ((unsigned) key[j] >= cut) least32 = min(least32, (unsigned) key[j]);
@@ -408,18 +429,22 @@ __device__ void pick_pages(const SelectArgs& a, const Seq& q, int s, int row, in
 	for (int i = written + tid; i < a.top; i += TEAM) out[i] = -1;
 }
 
-// max |mean| as the bound takes it: infinite when something is not finite
-__device__ __forceinline__ float grow_bound(float m, const float (&v)[8]) {
+// max |mean|, as the bits of a number: of two without signs the larger one's are larger, and those of what is not finite larger than all others'
+__device__ __forceinline__ unsigned grow_bound(unsigned m, const float (&v)[8]) {
 #pragma unroll
-	for (int e = 0; e < 8; e++) m = fabsf(v[e]) <= 3.4e38f ? fmaxf(m, fabsf(v[e])) : INFINITY;
+	for (int e = 0; e < 8; e++) m = max(m, (unsigned) __float_as_int(v[e]) & 0x7fffffffu);
 	return m;
+}
+__device__ __forceinline__ float score_error(int d, int rep, float abs_q, unsigned most) {
+	return most >= 0x7f800000u ? INFINITY : 1.1f * (float) (d + rep + 4) * 5.9604645e-8f * abs_q * __int_as_float((int) most);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(ST) paged_select_step_kernel(const __grid_constant__ SelectArgs a) {
 	extern __shared__ __align__(16) u64 keys[]; // one per page
 	__shared__ __align__(16) float s_q[256];
-	__shared__ float s_max[ST / 32], s_abs[ST / 32];
+	__shared__ float s_abs[ST / 32];
+	__shared__ unsigned s_max[ST / 32];
 	__shared__ int buf[ST / 32];
 	pdl_launch_dependents();
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x, g = blockIdx.y, d = a.c.d;
@@ -449,7 +474,7 @@ __global__ void __launch_bounds__(ST) paged_select_step_kernel(const __grid_cons
 		}
 		__syncthreads();
 		const int sub = lane & 7;
-		float most = 0.f;
+		unsigned most = 0;
 		for (int j0 = lo + warp * 4 + (lane >> 3); j0 < hi; j0 += 4 * (ST / 8)) { // four pages of each eight lanes on their way together
 			int page[4];
 			float x[4];
@@ -479,13 +504,13 @@ __global__ void __launch_bounds__(ST) paged_select_step_kernel(const __grid_cons
 				if (sub == 0 && j0 + u * (ST / 8) < hi) keys[j0 + u * (ST / 8)] = ordered32(x[u]);
 			}
 		}
-		most = warp_max(most);
+		most = __reduce_max_sync(0xffffffffu, most);
 		abs_q = warp_sum(abs_q);
 		if (lane == 0) { s_max[warp] = most; s_abs[warp] = abs_q; }
 		__syncthreads();
-		most = abs_q = 0.f;
-		for (int w = 0; w < ST / 32; w++) { most = fmaxf(most, s_max[w]); abs_q += s_abs[w]; }
-		err = 1.1f * (float) (d + a.rep + 4) * 5.9604645e-8f * abs_q * most;
+		abs_q = 0.f;
+		for (int w = 0; w < ST / 32; w++) { most = max(most, s_max[w]); abs_q += s_abs[w]; }
+		err = score_error(d, a.rep, abs_q, most);
 	}
 	if (hi - lo <= 32 * IN_REGS) {
 		if (warp == 0) pick_pages<T, 32>(a, q, s, row, g, err, keys, lane, nullptr);
@@ -500,7 +525,7 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 	float* s_q = reinterpret_cast<float*>(keys + (size_t) R * a.b.max_pages); // [R][d]
 	float* s_m = s_q + R * d;                                              // [SP][d + 4]
 	float* s_abs = s_m + SP * dp;                                          // [R][d / 8]
-	float* s_max = s_abs + R * (d / 8);                                    // [8]
+	unsigned* s_max = reinterpret_cast<unsigned*>(s_abs + R * (d / 8));    // [8]
 	int* s_page = reinterpret_cast<int*>(s_max + ST / 32);                 // [max_pages]
 	pdl_launch_dependents();
 	if (blockIdx.x == 0 && g == 0) check_seqs(a.c, a.b, tid, ST);
@@ -541,7 +566,7 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 		s_page[j] = page_of(a.c, a.b, s, j);
 		if (s_page[j] < 0) report(a.c, ERR_PAGE);
 	}
-	float most = 0.f;
+	unsigned most = 0;
 	for (int p0 = lo; p0 < hi; p0 += SP) {
 		__syncthreads();
 		for (int i0 = tid; i0 < SP * dc; i0 += 4 * ST) {
@@ -580,14 +605,13 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 #pragma unroll
 			for (int r = 0; r < R / 4; r++) keys[(size_t) (r0 + r) * a.b.max_pages + p0 + j] = ordered32(x[r]);
 	}
-	most = warp_max(most);
+	most = __reduce_max_sync(0xffffffffu, most);
 	if (lane == 0) s_max[warp] = most;
 	__syncthreads();
-	most = 0.f;
-	for (int w = 0; w < ST / 32; w++) most = fmaxf(most, s_max[w]);
+	for (int w = 0; w < ST / 32; w++) most = max(most, s_max[w]);
 	for (int r = warp; r < rows; r += ST / 32) {
 		const float abs_q = warp_sum(lane < dc ? s_abs[r * dc + lane] : 0.f);
-		pick_pages<T, 32>(a, q, s, row0 + r, g, 1.1f * (float) (d + a.rep + 4) * 5.9604645e-8f * abs_q * most, keys + (size_t) r * a.b.max_pages, lane, nullptr);
+		pick_pages<T, 32>(a, q, s, row0 + r, g, score_error(d, a.rep, abs_q, most), keys + (size_t) r * a.b.max_pages, lane, nullptr);
 	}
 }
 
