@@ -10,7 +10,7 @@ namespace paged {
 // =========================================================================================================================================
 // out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j, in one pass over the pages.  A step of single tokens reads every key and value once
 // for a handful of rows: HBM bounds it, and what the kernel has to do is to keep enough bytes on their way.  A warp brings tiles of 64 keys and values
-// by TMA (boxes of a page's slots, 64 entries wide, swizzled) into a ring; four warps take 16 keys of a tile each, with maximum, sum and output of their own, so that
+// by TMA (a page's slots, 64 entries wide, swizzled) into a ring; four warps take 16 keys of a tile each, with maximum, sum and output of their own, so that
 // none waits for another and a stage is free again after a quarter of a tile's work: scores and sums by mma.sync m16n8k16 with the 16 rows as A, queries and sums in registers.
 // At the end of a piece the four join through shared memory.  (tcgen05 would want 64 rows or more: a step of four heads to a kv head has four.)
 // Probabilities enter the second product in the cache's type, a rounding of 2^-9 (bf16) or 2^-12 (fp16) of each, of either sign; scores, maxima and sums stay in fp32.
@@ -32,7 +32,7 @@ struct Sizes {
 template <int D>
 static MmaConfig mma_config(size_t plan, int n_lists) {
 	using Z = Sizes<D>;
-	const size_t fixed = 1024 + Z::JOIN + CW * MM * 8 + 256 + (size_t) n_lists * 4 + 16 + plan;
+	const size_t fixed = 1024 + Z::JOIN + CW * MM * 8 + 512 + (size_t) n_lists * 4 + 16 + plan;
 	for (int per_sm = 2; per_sm >= 1; per_sm--) {
 		const size_t room = per_sm == 2 ? 113 * 1024 : 226 * 1024;
 		const int n = room > fixed ? (int) ((room - fixed) / Z::STAGE) : 0;
@@ -44,14 +44,15 @@ static MmaConfig mma_config(size_t plan, int n_lists) {
 	return MmaConfig{};
 }
 
+// Not volatile: products may move behind the loads of others, which are kept in their order
 template <typename T>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
 	if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-		asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+		asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
 		             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 		             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 	else
-		asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+		asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
 		             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 		             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -91,7 +92,8 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + CW * MM);         // [8]
 	uint64_t* empty = full + 8;                                           // [8]
 	int* s_dead = reinterpret_cast<int*>(empty + 8);
-	int* s_list = reinterpret_cast<int*>((uint8_t*) full + 256);          // [S]
+	int* s_ids = s_dead + 1;                                              // [32]
+	int* s_list = reinterpret_cast<int*>((uint8_t*) full + 512);          // [S]
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list) + ((LIST ? a.S * 4 : 0) + 15) / 16 * 16;
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	if (tid == 0) {
@@ -100,69 +102,85 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 	}
 	pdl_launch_dependents();
+	const int dc = (a.c.d + 63) / 64, vc = (a.c.dv + 63) / 64;
+	// Products run over all D entries, without a question between them (asking eight times took as long as the products).  Blocks that no copy fills are zeros.
+	if (dc < D / 64 || vc < D / 64)
+		for (int i = tid; i < stages * 2 * (D / 64) * (KT * 8); i += MT) {
+			const int block = i / (KT * 8), of_tile = block % (D / 64);
+			if (of_tile >= (block / (D / 64) % 2 ? vc : dc)) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+		}
 	Plan plan;
 	if (!LIST) make_plan<MT>(a, part, s_plan, plan);
 	else if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, MT);
 	__syncthreads();
-	const int dc = (a.c.d + 63) / 64, vc = (a.c.dv + 63) / 64;
 	const int P = 1 << a.c.shift, W = min(P, KT), per = KT / W; // slots of a box, boxes of a tile's column
 	Walk k;
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
 	if (tid == 0)
 		write_head(a, part, k, more, LIST ? more && row_in_seq(k.x.q, k.x.row0) : more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, LIST ? share_of(list_total(a, part), part.grid) : plan.share);
-	int n = 0; // tiles that this CTA's pieces have had so far: tile n lies in stage n % stages
+	int st = 0;         // the tile's stage, and how often the ring has come round
+	uint32_t round = 0;
+	auto advance = [&] {
+		if (++st == stages) { st = 0; round ^= 1; }
+	};
 
-	if (warp == CW) { // ---- the copies ----
-		const int boxes = per * (dc + vc);
+	if (warp == CW) { // ---- the copies: 32 boxes' pages in one asking, then one thread sends them ----
+		int sent = 0; // tiles
 		for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 			const Piece& x = k.x;
 			if (x.j0 == x.j1) continue;
-			int pages = 0, vis = 0x7fffffff;
+			int vis;
 			if (LIST) {
 				if (!row_in_seq(x.q, x.row0)) continue;
 				const int pos = x.q.len - x.q.n + x.row0 - x.q.a;
 				bool own;
-				pages = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, s_list, &own);
-				vis = pages << a.c.shift;
+				vis = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, s_list, &own) << a.c.shift;
 				if (own) vis += (pos & (P - 1)) + 1 - P;
 			} else if (x.seg < a.b.n_groups) vis = plan.shs[x.s];
 			else vis = own_keys(x.q, x.key0, a.rep, min((x.t + 1) * MM, x.rows) - 1);
-			const int j1 = min(x.j1, (vis + KT - 1) / KT);
-			int id = -1;
-			for (int j = x.j0, e = 0; j < j1; j++, e += per, n++) { // entry e: the e-th box's worth of slots from the piece's first on
-				if ((e & 31) == 0) { // the pages of the next 32
-					const int at = x.j0 * KT + (e + lane) * W;
-					id = -1;
-					if (at < vis) {
-						const int key = x.key0 + at;
-						id = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
-						if (id < 0) report(a.c, ERR_PAGE);
+			const int j1 = min(x.j1, (vis + KT - 1) / KT), batch = 32 / per, key0 = x.key0, g = x.g;
+			bool ok = true;
+			for (int j = x.j0; j < j1 && ok; j += batch) {
+				const int at = j * KT + lane * W, key = key0 + at;
+				int id = -1;
+				if (at < vis) {
+					id = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
+					if (id < 0) report(a.c, ERR_PAGE);
+				}
+				s_ids[lane] = id;
+				__syncwarp();
+				const int count = min(batch, j1 - j);
+				if (elect())
+					for (int i = 0, st1 = st, round1 = round; i < count; i++) {
+						if (!(ok = wait_alone(&empty[st1], round1 ^ 1, s_dead, a.c))) break;
+						mbar_expect_tx(&full[st1], (uint32_t) ((dc + vc) * KT * 128));
+						const uint32_t dst = smem_u32(ring) + (uint32_t) st1 * Z::STAGE;
+						const int slot = (key0 + (j + i) * KT) & (P - 1);
+						copy_tile(dst, &kmap, a.c.d, g, slot, per, W, s_ids + i * per, a.c.pages, &full[st1]);
+						copy_tile(dst + Z::TILE, &vmap, a.c.dv, g, slot, per, W, s_ids + i * per, a.c.pages, &full[st1]);
+						if (++st1 == stages) { st1 = 0; round1 ^= 1; }
 					}
-				}
-				const int st = n % stages;
-				if (!wait_for(&empty[st], ((n / stages) & 1) ^ 1, s_dead, a.c)) break;
-				if (lane == 0) mbar_expect_tx(&full[st], (uint32_t) (boxes * W * 128));
-				__syncwarp();
-				const int which = lane / per, part_of = lane % per; // column block (keys, then values), box of the tile
-				const int pg = __shfl_sync(0xffffffffu, id, (e + part_of) & 31);
-				if (lane < boxes) {
-					const int slot = (x.key0 + j * KT + part_of * W) & (P - 1), block = which < dc ? which : which - dc;
-					uint8_t* dst = ring + (size_t) st * Z::STAGE + (which < dc ? 0 : Z::TILE) + block * KT * 128 + part_of * W * 128;
-					copy_box(dst, which < dc ? &kmap : &vmap, block * 64, slot, x.g, pg < 0 ? a.c.pages : pg, &full[st]); // behind the last page: zeros
-				}
-				__syncwarp();
+				ok = __all_sync(0xffffffffu, ok);
+				for (int i = 0; i < count; i++) advance();
+				sent += count;
 			}
-			if (*(volatile int*) s_dead) break;
+			if (!ok) break;
 		}
 		if (*(volatile int*) s_dead) // gave up: copies still on their way end first
-			for (int i = max(0, n - stages); i < n; i++) wait_some(&full[i % stages], (i / stages) & 1);
+			for (int i = max(0, sent - stages); i < sent; i++) wait_some(&full[i % stages], (i / stages) & 1);
 		pdl_wait(); // beside the kernel of many rows, whose inputs were complete before it began, but not ahead of it to the join
 		return;
 	}
 
 	// ---- the products ----
-	const int kd = (a.c.d + 15) / 16, nd = (a.c.dv + 15) / 16;
-	const float c1 = a.scale * 1.4426950408889634f;
+	const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;            // a negative scale turns the queries' signs
+	const float c1 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f); // not 0: 0 times an infinity is no number
+	const float slack = 11.5f / c1;
+	// where this lane's rows of ldmatrix lie in a tile: keys (lane & 7) + 8 (lane / 16) of this warp's 16, chunk (lane / 8) & 1; values lane & 15, chunk lane / 16.  Every two chunks
+	// further on are two bits of the address turned over, every eight a block of columns.
+	const int kr = (lane & 7) + (lane >> 4) * 8, vr = lane & 15;
+	const uint32_t k_lane = (uint32_t) ((warp * 16 + kr) * 128 + ((((lane >> 3) & 1) ^ (kr & 7)) << 4));
+	const uint32_t v_lane = (uint32_t) (Z::TILE + (warp * 16 + vr) * 128 + (((lane >> 4) ^ (vr & 7)) << 4));
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue;
@@ -178,8 +196,8 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			const uint8_t* at = a.q + ((long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d + (lane & 3) * 2) * 2;
 #pragma unroll
 			for (int kk = 0; kk < D / 16; kk++) {
-				qa[kk][half] = r < rows && kk * 16 < a.c.d ? *reinterpret_cast<const uint32_t*>(at + kk * 32) : 0;
-				qa[kk][half + 2] = r < rows && kk * 16 + 8 < a.c.d ? *reinterpret_cast<const uint32_t*>(at + kk * 32 + 16) : 0;
+				qa[kk][half] = r < rows && kk * 16 < a.c.d ? *reinterpret_cast<const uint32_t*>(at + kk * 32) ^ flip : 0;
+				qa[kk][half + 2] = r < rows && kk * 16 + 8 < a.c.d ? *reinterpret_cast<const uint32_t*>(at + kk * 32 + 16) ^ flip : 0;
 			}
 		}
 		if (LIST) {
@@ -194,92 +212,100 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			lim0 = own_keys(x.q, x.key0, a.rep, min(x.t * MM + lane / 4, x.rows - 1));
 			lim1 = own_keys(x.q, x.key0, a.rep, min(x.t * MM + lane / 4 + 8, x.rows - 1));
 		}
-		float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+		float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, b0 = 0.f, b1 = 0.f; // maxima of the raw scores, and what is added to a score times c1
 #pragma unroll
 		for (int i = 0; i < D / 8; i++)
 #pragma unroll
 			for (int e = 0; e < 4; e++) o[i][e] = 0.f;
 		const int j1 = min(x.j1, (most + KT - 1) / KT);
 		const bool high = rows > 8;
-		for (int j = x.j0; j < j1; j++, n++) {
-			const int st = n % stages;
-			if (!wait_for(&full[st], (n / stages) & 1, s_dead, a.c)) continue;
-			const uint32_t kt = smem_u32(ring + (size_t) st * Z::STAGE) + warp * 16 * 128, vt = kt + Z::TILE; // this warp's 16 keys
-			const int base = j * KT + warp * 16;
+		bool there = false; // the next tile
+		for (int j = x.j0; j < j1; j++, advance()) {
+			if (!there && !wait_for(&full[st], round, s_dead, a.c)) continue;
+			const uint32_t tile = smem_u32(ring) + (uint32_t) st * Z::STAGE;
+			const int base = j * KT + warp * 16; // this warp's 16 keys
 			const bool tail = base + 16 > most;
 			if (tail) { // slots that no row sees may hold anything: as zeros they add nothing
 				const int from = max(most - base, 0);
 				for (int i = lane; i < (16 - from) * vc * 8; i += 32) {
 					const int r = from + i / (vc * 8), c = i % (vc * 8);
-					asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at(vt, KT, r, c)), "r"(0) : "memory");
+					asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at(tile + Z::TILE + warp * 16 * 128, KT, r, c)), "r"(0) : "memory");
 				}
 				__syncwarp();
 			}
-			float s[2][4];
+			float s[2][4], s2[2][4]; // even and odd steps apart: a product waits for the one before into the same sum
 #pragma unroll
 			for (int i = 0; i < 2; i++)
 #pragma unroll
-				for (int e = 0; e < 4; e++) s[i][e] = 0.f;
+				for (int e = 0; e < 4; e++) s[i][e] = s2[i][e] = 0.f;
 #pragma unroll
 			for (int kk = 0; kk < D / 16; kk++)
-				if (kk < kd) {
-					uint32_t b[4];
-					ldsm4(b, chunk_at(kt, KT, (lane & 7) + (lane >> 4) * 8, kk * 2 + ((lane >> 3) & 1)));
-					mma16<T>(s[0], qa[kk], b[0], b[1]);
-					mma16<T>(s[1], qa[kk], b[2], b[3]);
-				}
-			float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-			for (int i = 0; i < 2; i++) {
-#pragma unroll
-				for (int e = 0; e < 4; e++) {
-					s[i][e] *= c1;
-					if (base + 16 > least && base + i * 8 + (lane & 3) * 2 + (e & 1) >= (e < 2 ? lim0 : lim1)) s[i][e] = -INFINITY;
-				}
-				t0 = fmaxf(t0, fmaxf(s[i][0], s[i][1]));
-				t1 = fmaxf(t1, fmaxf(s[i][2], s[i][3]));
+			{
+				uint32_t b[4];
+				ldsm4(b, ((tile + k_lane) ^ ((kk * 2 & 7) << 4)) + (kk >> 2) * KT * 128);
+				mma16<T>(kk & 1 ? s2[0] : s[0], qa[kk], b[0], b[1]);
+				mma16<T>(kk & 1 ? s2[1] : s[1], qa[kk], b[2], b[3]);
 			}
 #pragma unroll
-			for (int w = 1; w < 4; w <<= 1) {
-				t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
-				t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
+			for (int i = 0; i < 2; i++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) s[i][e] += s2[i][e];
+			if (base + 16 > least) {
+#pragma unroll
+				for (int i = 0; i < 2; i++)
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						if (base + i * 8 + (lane & 3) * 2 + (e & 1) >= (e < 2 ? lim0 : lim1)) s[i][e] = -INFINITY;
 			}
-			const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-			if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-				const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+			// The maximum that probabilities are taken against may lag behind by 2^11.5, which fp16 holds: then no lane has to ask its neighbours, and sums stay as they are
+			float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+			if (__any_sync(0xffffffffu, t0 > m0 + slack || t1 > m1 + slack)) {
+#pragma unroll
+				for (int w = 1; w < 4; w <<= 1) {
+					t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, w));
+					t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, w));
+				}
+				const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1), f0 = m0 == -INFINITY ? 0.f : ex2((m0 - n0) * c1), f1 = m1 == -INFINITY ? 0.f : ex2((m1 - n1) * c1);
 				l0 *= f0;
 				l1 *= f1;
 #pragma unroll
 				for (int i = 0; i < D / 8; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
 				m0 = n0;
 				m1 = n1;
+				b0 = m0 == -INFINITY ? 0.f : -m0 * c1;
+				b1 = m1 == -INFINITY ? 0.f : -m1 * c1;
 			}
-			const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+			// asked for here, known when this tile is done
+			there = j + 1 < j1 && try_wait_once(&full[st + 1 == stages ? 0 : st + 1], round ^ (st + 1 == stages));
 			uint32_t pa[4];
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
-				const float x0 = ex2(s[i][0] - b0), x1 = ex2(s[i][1] - b0);
+				const float x0 = ex2(fmaf(s[i][0], c1, b0)), x1 = ex2(fmaf(s[i][1], c1, b0));
 				l0 += x0 + x1;
 				pa[2 * i] = pack16<T>(x0, x1);
 				pa[2 * i + 1] = 0;
-				if (high) {
-					const float x2 = ex2(s[i][2] - b1), x3 = ex2(s[i][3] - b1);
+			}
+			if (high)
+#pragma unroll
+				for (int i = 0; i < 2; i++) {
+					const float x2 = ex2(fmaf(s[i][2], c1, b1)), x3 = ex2(fmaf(s[i][3], c1, b1));
 					l1 += x2 + x3;
 					pa[2 * i + 1] = pack16<T>(x2, x3);
 				}
-			}
 #pragma unroll
 			for (int c = 0; c < D / 16; c++)
-				if (c < nd) {
-					uint32_t b[4];
-					ldsm4_t(b, chunk_at(vt, KT, lane & 15, c * 2 + (lane >> 4)));
-					mma16<T>(o[2 * c], pa, b[0], b[1]);
-					mma16<T>(o[2 * c + 1], pa, b[2], b[3]);
-				}
+			{
+				uint32_t b[4];
+				ldsm4_t(b, ((tile + v_lane) ^ ((c * 2 & 7) << 4)) + (c >> 2) * KT * 128);
+				mma16<T>(o[2 * c], pa, b[0], b[1]);
+				mma16<T>(o[2 * c + 1], pa, b[2], b[3]);
+			}
 			if (tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the zeros, before the next copy
 			__syncwarp();
 			if (lane == 0) mbar_arrive(&empty[st]);
 		}
+		m0 *= c1; // in units of log2 from here on
+		m1 *= c1;
 		// ---- the four warps' sums ----
 #pragma unroll
 		for (int w = 1; w < 4; w <<= 1) {

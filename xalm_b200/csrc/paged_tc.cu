@@ -23,17 +23,6 @@ constexpr int QB = HALF_ROWS * 128; // bytes of 64 entries of a half's queries
 constexpr int KB = KT * 128;        // bytes of 64 entries of a key or value tile
 constexpr int RING = 4;
 
-__device__ __forceinline__ bool elect() {
-	uint32_t pred;
-	asm volatile(
-	    "{\n"
-	    ".reg .pred p;\n"
-	    "elect.sync _|p, 0xffffffff;\n"
-	    "selp.u32 %0, 1, 0, p;\n"
-	    "}\n"
-	    : "=r"(pred));
-	return pred != 0;
-}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // D (+)= A B^T with A from shared memory
@@ -129,7 +118,7 @@ struct TcShared {
 	uint64_t full[RING], empty[RING];
 	uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2]; // by half and by the tile's parity, so that nobody is ever two phases ahead of a wait
 	uint32_t tmem;
-	int dead, flag[2];
+	int dead, flag[2], ids[32];
 	float buf[2][256];
 };
 
@@ -182,26 +171,26 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 		const TcPiece p = tc_piece(a, plan, x);
 		const int tiles = max(p.j1 - x.j0, 0);
 		const bool here = h >= 0 && h * HALF_ROWS < p.rows;
-		if (warp == 0) { // ---- copies ----
-			int id = -1;
-			for (int j = 0, e = 0; j < tiles && ok; j++, e += per) {
-				if ((e & 31) == 0) {
-					const int at = x.j0 * KT + (e + lane) * W;
-					id = -1;
-					if (at < p.most) {
-						id = page_of(a.c, a.b, x.s, (x.key0 + at) >> a.c.shift);
-						if (id < 0) report(a.c, ERR_PAGE);
-					}
+		if (warp == 0) { // ---- copies: 32 boxes' pages in one asking, then one thread sends them ----
+			const int batch = 32 / per, key0 = x.key0, g = x.g;
+			for (int j = 0; j < tiles && ok; j += batch) {
+				const int at = (x.j0 + j) * KT + lane * W;
+				int id = -1;
+				if (at < p.most) {
+					id = page_of(a.c, a.b, x.s, (key0 + at) >> a.c.shift);
+					if (id < 0) report(a.c, ERR_PAGE);
 				}
-				const int st = (n + j) % RING, part_of = lane % per, block = lane / per;
-				const int pg = __shfl_sync(0xffffffffu, id, (e + part_of) & 31), page = pg < 0 ? a.c.pages : pg;
-				const int slot = (x.key0 + (x.j0 + j) * KT + part_of * W) & (P - 1);
-				if (!(ok = wait_for(&sh.empty[st], (((n + j) / RING) & 1) ^ 1, &sh.dead, a.c))) break;
-				if (lane == 0) mbar_expect_tx(&sh.full[st], (uint32_t) ((dc + vc) * KB));
+				sh.ids[lane] = id;
 				__syncwarp();
-				if (block < dc) copy_box(s_k + (st * 2 + block) * KB + part_of * W * 128, &kmap, block * 64, slot, x.g, page, &sh.full[st]);
-				else if (block < dc + vc) copy_box(s_v + (st * 2 + block - dc) * KB + part_of * W * 128, &vmap, (block - dc) * 64, slot, x.g, page, &sh.full[st]);
-				__syncwarp();
+				if (elect())
+					for (int i = 0; i < min(batch, tiles - j); i++) {
+						const int m = n + j + i, st = m % RING, slot = (key0 + (x.j0 + j + i) * KT) & (P - 1);
+						if (!(ok = wait_alone(&sh.empty[st], ((m / RING) & 1) ^ 1, &sh.dead, a.c))) break;
+						mbar_expect_tx(&sh.full[st], (uint32_t) ((dc + vc) * KB));
+						copy_tile(smem_u32(s_k) + st * 2 * KB, &kmap, a.c.d, g, slot, per, W, sh.ids + i * per, a.c.pages, &sh.full[st]);
+						copy_tile(smem_u32(s_v) + st * 2 * KB, &vmap, a.c.dv, g, slot, per, W, sh.ids + i * per, a.c.pages, &sh.full[st]);
+					}
+				ok = __all_sync(0xffffffffu, ok);
 			}
 			if (!ok) // gave up: copies still on their way end first
 				for (int i = max(0, n - RING); i < n + tiles; i++) wait_some(&sh.full[i % RING], (i / RING) & 1);
@@ -209,7 +198,6 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			if (here && tiles) {
 				__syncwarp();
 				if (elect()) { // not `lane == 0`: in a branch that the compiler cannot tell to be one thread's, it does not keep the operands of unrolled products apart
-					const int kd = (a.c.d + 15) / 16;
 					const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>((a.c.dv + 15) / 16 * 16, true), t_s = tmem + 128 * h;
 					const uint64_t q = desc_k(smem_u32(s_q)) + h * (2 * QB >> 4), k_at = desc_k(smem_u32(s_k)), v_at = desc_mn(smem_u32(s_v), KB);
 					ok = wait_alone(&sh.q_full[h], pieces & 1, &sh.dead, a.c);
@@ -223,8 +211,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 							const uint64_t kk = k_at + ((m + 1) % RING) * (2 * KB >> 4);
 							const uint32_t d = t_s + 64 * ((c + 1) & 1);
 #pragma unroll
-							for (int s = 0; s < 8; s++)
-								if (s < kd) mma_ss(d, q + (s >> 2) * (QB >> 4) + 2 * (s & 3), kk + (s >> 2) * (KB >> 4) + 2 * (s & 3), id_s, s != 0);
+							for (int s = 0; s < 4; s++) mma_ss(d, q + 2 * s, kk + 2 * s, id_s, s != 0); // queries are zeros behind the head's last entry, and so are keys
+							if (dc > 1)
+#pragma unroll
+								for (int s = 0; s < 4; s++) mma_ss(d, q + (QB >> 4) + 2 * s, kk + (KB >> 4) + 2 * s, id_s, 1);
 							commit(&sh.s_full[h][(c + 1) & 1]);
 						}
 						if (j < 0) continue;

@@ -9,8 +9,9 @@
 namespace xalm {
 namespace paged {
 
-// A pool as the copy engine sees it: (entries, slots, heads, pages), boxes of 64 entries and min(page, 64) slots of one head.  Entries behind the head's
-// last and pages behind the pool's last read as zeros.
+// A pool as the copy engine sees it: (64 entries, slots, blocks of 64 entries, heads, pages), boxes of min(page, 64) slots of one head with all their blocks, one behind the other.  Heads whose
+// last block is not full are (entries, slots, 1, heads, pages) and come block by block: entries behind the last read as zeros, as pages behind the pool's last do.
+__host__ __device__ __forceinline__ bool whole_heads(int dim) { return dim % 64 == 0; }
 static inline int pool_map(const Cache& c, int type, bool keys, CUtensorMap* map) {
 	typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
 	                           CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -25,21 +26,40 @@ static inline int pool_map(const Cache& c, int type, bool keys, CUtensorMap* map
 	}();
 	if (!encode) return set_error(XALM_ERR_CUDA, "paged attention: this driver has no cuTensorMapEncodeTiled");
 	const int P = 1 << c.shift;
-	const cuuint64_t dims[4] = {(cuuint64_t) (keys ? c.d : c.dv), (cuuint64_t) P, (cuuint64_t) c.G, (cuuint64_t) c.pages};
-	const cuuint64_t strides[3] = {(cuuint64_t) (keys ? c.k_slot : c.v_slot) * 2, (cuuint64_t) (keys ? c.k_head : c.v_head) * 2, (cuuint64_t) (keys ? c.k_page : c.v_page) * 2};
-	const cuuint32_t box[4] = {64, (cuuint32_t) (P < KT ? P : KT), 1, 1}, steps[4] = {1, 1, 1, 1};
-	const CUresult r = encode(map, type == XALM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, keys ? c.k : c.v, dims, strides, box, steps,
+	const int dim = keys ? c.d : c.dv, blocks = P >= KT && whole_heads(dim) ? dim / 64 : 1;
+	const cuuint64_t dims[5] = {(cuuint64_t) (dim / blocks), (cuuint64_t) P, (cuuint64_t) blocks, (cuuint64_t) c.G, (cuuint64_t) c.pages};
+	const cuuint64_t strides[4] = {(cuuint64_t) (keys ? c.k_slot : c.v_slot) * 2, 128, (cuuint64_t) (keys ? c.k_head : c.v_head) * 2, (cuuint64_t) (keys ? c.k_page : c.v_page) * 2};
+	const cuuint32_t box[5] = {64, (cuuint32_t) (P < KT ? P : KT), (cuuint32_t) blocks, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
+	const CUresult r = encode(map, type == XALM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, keys ? c.k : c.v, dims, strides, box, steps,
 	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 	if (r != CUDA_SUCCESS) return set_error(XALM_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled failed (%d)", (int) r);
 	return XALM_OK;
 }
-__device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int x, int slot, int head, int page, uint64_t* bar) {
-	asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)), "l"(map), "r"(x),
-	             "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, uint64_t* bar) {
+	asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(map), "r"(x), "r"(slot),
+	             "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
 	             : "memory");
+}
+// One thread: keys or values of a tile, `per` runs of W slots whose pages are id[0 .. per) (-1: none), into [block][64 slots][128 bytes] at dst
+__device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, int dim, int head, int slot, int per, int W, const int* id, int none, uint64_t* bar) {
+	if (per == 1 && whole_heads(dim)) copy_box(dst, map, 0, slot, head, id[0] < 0 ? none : id[0], bar);
+	else
+		for (int i = 0; i < per; i++)
+			for (int x = 0; x < dim; x += 64) copy_box(dst + (x / 64 * KT + i * W) * 128, map, x, slot, head, id[i] < 0 ? none : id[i], bar);
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+__device__ __forceinline__ bool elect() { // one thread of a converged warp, in a way that the compiler knows for one
+	uint32_t pred;
+	asm volatile(
+	    "{\n"
+	    ".reg .pred p;\n"
+	    "elect.sync _|p, 0xffffffff;\n"
+	    "selp.u32 %0, 1, 0, p;\n"
+	    "}\n"
+	    : "=r"(pred));
+	return pred != 0;
+}
 __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
 	uint32_t ok;
 	asm volatile(
@@ -52,6 +72,20 @@ __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
 	    : "r"(smem_u32(bar)), "r"(parity)
 	    : "memory");
 	return ok != 0;
+}
+// The same, without waiting; a whole warp agrees
+__device__ __forceinline__ bool try_wait_once(uint64_t* bar, uint32_t parity) {
+	uint32_t ok;
+	asm volatile(
+	    "{\n"
+	    ".reg .pred p;\n"
+	    "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+	    "selp.u32 %0, 1, 0, p;\n"
+	    "}\n"
+	    : "=r"(ok)
+	    : "r"(smem_u32(bar)), "r"(parity)
+	    : "memory");
+	return __all_sync(0xffffffffu, ok != 0);
 }
 constexpr int WAIT_TRIES = 1 << 18; // about two seconds of suspended tries: far beyond what a copy or a product takes
 __device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity) {
