@@ -703,7 +703,7 @@ static int sm_count(int device, int* n) {
 }
 
 constexpr int SMALL_ROWS = 16;
-constexpr int LEAD = 2, LEAD_TC = 4;
+constexpr int LEAD = 6, LEAD_TC = 8;
 
 // ---- attention: parts, workspace --------------------------------------------------------------------------------------------------------------
 static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchView& b, int heads, int n_lists, Attn& a, size_t* bytes) {
@@ -735,12 +735,14 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		// a segment of `rows` rows has at most rows / M + 1 tiles, a part that takes short ones only has one
 		const long long tiles = n_lists ? (long long) b.N * ((a.rep + p.M - 1) / p.M) : (tc && !big ? 0 : rows / p.M) + b.B + (b.n_groups ? (tc && !big ? 0 : rows / p.M) + b.n_groups : 0);
 		if (tiles * c.G + p.grid > 0x7fffffff / p.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
+		const long long keys = std::min((long long) b.max_pages << c.shift, 0x7fffffffll), work = n_lists ? (((long long) n_lists << c.shift) + KT - 1) / KT : keys / KT + 1;
+		if (tiles * c.G > 0x7fffffffll / (work + p.lead)) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads over up to %lld keys are too many for one call", b.N, heads, work * KT);
 		p.slots = n_lists || !b.n_groups ? 2 * p.grid : (int) (tiles * c.G) + p.grid;
 		p.o = (float*) take((size_t) p.slots * p.M * c.dv * 4);
 		p.ml = (float2*) take((size_t) p.slots * p.M * 8);
 		p.head = (Head*) take((size_t) p.grid * sizeof(Head));
 		if (!n_lists) {
-			p.cum_w = (long long*) take((size_t) (b.B + b.n_groups + 1) * 8);
+			p.cum_w = (int*) take((size_t) (b.B + b.n_groups + 1) * 4);
 			p.cum_u = (int*) take((size_t) (b.B + b.n_groups + 1) * 4);
 			p.shs = (int*) take((size_t) b.B * 4);
 		}
@@ -779,7 +781,7 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 		p.ml = (float2*) (base + (size_t) p.ml);
 		p.head = (Head*) (base + (size_t) p.head);
 		if (!n_lists) {
-			p.cum_w = (long long*) (base + (size_t) p.cum_w);
+			p.cum_w = (int*) (base + (size_t) p.cum_w);
 			p.cum_u = (int*) (base + (size_t) p.cum_u);
 			p.shs = (int*) (base + (size_t) p.shs);
 		}

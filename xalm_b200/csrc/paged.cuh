@@ -147,8 +147,7 @@ struct Part {
 	float2* ml;          // (slots, M): m (in units of log2), sum of exp
 	int slots, M, grid, lead;
 	int least_rows, most_rows; // segments of so many rows are this part's
-	long long* cum_w;    // the plan, left by CTA 0 for the join: tiles and units before each segment, keys shared by each sequence
-	int *cum_u, *shs;
+	int *cum_w, *cum_u, *shs; // the plan, left by CTA 0 for the join: work and units before each segment, keys shared by each sequence
 	Head* head;          // (grid)
 };
 struct Attn {
@@ -166,15 +165,14 @@ struct Attn {
 	Part part[2];
 };
 struct Plan {
-	long long* cum_w; // segments + 1
-	int *cum_u, *shs;
+	int *cum_w, *cum_u, *shs; // segments + 1, the same, sequences
 	int segs;
-	long long total, share;
+	int total, share;
 	View v; // in shared memory
 };
-__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (B + n_groups + 1) * 12 + (size_t) (3 * B + n_groups + 3) * 4 + 32 * 12; }
+__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (5 * B + 3 * n_groups + 5 + 64) * 4; }
 
-__host__ __device__ __forceinline__ long long share_of(long long total, int grid) { return (total + grid - 1) / grid; }
+__host__ __device__ __forceinline__ int share_of(int total, int grid) { return (int) (((unsigned) total + grid - 1) / grid); }
 
 // rows of a segment, its first row and sequence
 __device__ __forceinline__ int seg_rows(const View& v, int rep, int seg, int& row0, int& s_first) {
@@ -215,12 +213,10 @@ template <int NT>
 __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& p) {
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.B, n = a.b.n_groups;
 	p.segs = n + B;
-	p.cum_w = reinterpret_cast<long long*>(smem);
-	long long* sum_w = p.cum_w + p.segs + 1;
-	p.cum_u = reinterpret_cast<int*>(sum_w + 32);
-	int* sum_u = p.cum_u + p.segs + 1;
-	p.shs = sum_u + 32;
-	int *starts = p.shs + B, *lens = starts + B + 1, *bounds = lens + B;
+	p.cum_w = reinterpret_cast<int*>(smem);
+	p.cum_u = p.cum_w + p.segs + 1;
+	p.shs = p.cum_u + p.segs + 1;
+	int *starts = p.shs + B, *lens = starts + B + 1, *bounds = lens + B, *sum_w = bounds + n + 1, *sum_u = sum_w + 32;
 	// the arrays come in at once: what follows asks for them in turn, and every asking of memory is most of a microsecond
 	for (int i = tid; i <= B; i += NT) {
 		starts[i] = a.b.starts[i];
@@ -233,72 +229,76 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 	p.v.lens = lens;
 	p.v.bounds = bounds;
 	__syncthreads();
-	for (int i = warp; i < n; i += NT / 32) {
-		int m = max(a.b.shared[i], 0);
-		const int2 g = group_of(p.v, i);
-		if (g.y - g.x < 2) continue;
-		const Seq last = seq_of(p.v, g.y - 1);
-		if ((long long) (last.a + last.n - seq_of(p.v, g.x).a) * a.rep > (long long) (g.y - g.x) * ALONE_ROWS) continue;
-		for (int s = g.x + lane; s < g.y; s += 32) {
-			const Seq q = seq_of(p.v, s);
-			m = min(m, max(q.len - q.n, 0));
+	// rows that two sequences claim, or sequences that two groups do, would be work without bounds: then there is none
+	bool bad = false;
+	for (int i = tid; i < p.segs; i += NT) {
+		if (i < n) bad = bad || bounds[i] > bounds[i + 1];
+		else {
+			const int s = i - n;
+			bad = bad || starts[s] > starts[s + 1];
+			if (blockIdx.x == 0 && !seq_ok(p.v, s)) report(a.c, ERR_BATCH);
 		}
-		m = __reduce_min_sync(0xffffffffu, m) >> a.c.shift << a.c.shift;
-		for (int s = g.x + lane; s < g.y; s += 32) p.shs[s] = m;
 	}
-	if (blockIdx.x == 0)
-		for (int s = tid; s < B; s += NT)
-			if (!seq_ok(p.v, s)) report(a.c, ERR_BATCH);
-	if (n) __syncthreads();
-	long long carry_w = 0;
-	int carry_u = 0;
+	bad = __syncthreads_or(bad);
+	if (bad && blockIdx.x == 0 && tid == 0) report(a.c, ERR_BATCH);
+	if (n && !bad) {
+		for (int i = warp; i < n; i += NT / 32) {
+			int m = max(a.b.shared[i], 0);
+			const int2 g = group_of(p.v, i);
+			if (g.y - g.x < 2) continue;
+			const Seq last = seq_of(p.v, g.y - 1);
+			if ((float) (last.a + last.n - seq_of(p.v, g.x).a) * a.rep > (float) (g.y - g.x) * ALONE_ROWS) continue;
+			for (int s = g.x + lane; s < g.y; s += 32) {
+				const Seq q = seq_of(p.v, s);
+				m = min(m, max(q.len - q.n, 0));
+			}
+			m = __reduce_min_sync(0xffffffffu, m) >> a.c.shift << a.c.shift;
+			for (int s = g.x + lane; s < g.y; s += 32) p.shs[s] = m;
+		}
+		__syncthreads();
+	}
+	int carry_w = 0, carry_u = 0;
 	if (tid == 0) { p.cum_w[0] = 0; p.cum_u[0] = 0; }
 	for (int base = 0; base < p.segs; base += NT) {
 		const int seg = base + tid;
-		long long w = 0;
-		int u = 0, in_seg = 0;
+		int w = 0, u = 0, in_seg = 0;
 		bool wide = false; // own rows of many tiles: their sum is the whole warp's
-		if (seg < p.segs) {
+		if (seg < p.segs && !bad) {
 			int row0, s;
-			const int rows = seg_rows(p.v, a.rep, seg, row0, s), tiles = (rows + part.M - 1) / part.M;
+			const int rows = seg_rows(p.v, a.rep, seg, row0, s);
 			if (in_part(part, rows)) {
-				if (seg < n) w = (long long) tiles * unit_work(a, part, seg, rows, Seq(), p.shs[s], 0);
-				else {
-					const Seq q = seq_of(p.v, s);
-					if (tiles <= 4) {
-						for (int t = 0; t < tiles; t++) w += unit_work(a, part, seg, rows, q, p.shs[s], t);
-					} else wide = true;
-				}
-				in_seg = tiles;
+				in_seg = (rows + part.M - 1) / part.M;
+				if (seg < n) w = in_seg * unit_work(a, part, seg, rows, Seq(), p.shs[s], 0);
+				else if (in_seg == 1) w = unit_work(a, part, seg, rows, seq_of(p.v, s), p.shs[s], 0);
+				else wide = true;
 			}
 		}
 		for (unsigned m = __ballot_sync(0xffffffffu, wide); m; m &= m - 1) {
 			const int from = __ffs(m) - 1, wseg = base + (tid & ~31) + from, n_tiles = __shfl_sync(0xffffffffu, in_seg, from);
 			const Seq q = seq_of(p.v, wseg - n);
-			long long sum = 0;
+			int sum = 0;
 			for (int t = lane; t < n_tiles; t += 32) sum += unit_work(a, part, wseg, q.n * a.rep, q, p.shs[wseg - n], t);
-#pragma unroll
-			for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+			sum = __reduce_add_sync(0xffffffffu, sum);
 			if (lane == from) w = sum;
 		}
 		w *= a.c.G;
 		u = w ? in_seg * a.c.G : 0;
 #pragma unroll
 		for (int o = 1; o < 32; o <<= 1) {
-			const long long x = __shfl_up_sync(0xffffffffu, w, o);
-			const int y = __shfl_up_sync(0xffffffffu, u, o);
+			const int x = __shfl_up_sync(0xffffffffu, w, o), y = __shfl_up_sync(0xffffffffu, u, o);
 			if (lane >= o) { w += x; u += y; }
 		}
 		if (lane == 31) { sum_w[warp] = w; sum_u[warp] = u; }
 		__syncthreads();
-		long long bw = carry_w;
-		int bu = carry_u;
-		for (int i = 0; i < warp; i++) { bw += sum_w[i]; bu += sum_u[i]; }
-		if (seg < p.segs) { p.cum_w[seg + 1] = bw + w; p.cum_u[seg + 1] = bu + u; }
-		for (int i = 0; i < NT / 32; i++) { carry_w += sum_w[i]; carry_u += sum_u[i]; }
+		for (int i = 0; i < NT / 32; i++) {
+			if (i == warp) { w += carry_w; u += carry_u; }
+			carry_w += sum_w[i];
+			carry_u += sum_u[i];
+		}
+		if (seg < p.segs) { p.cum_w[seg + 1] = w; p.cum_u[seg + 1] = u; }
 		__syncthreads();
 	}
-	p.total = p.cum_w[p.segs];
+	p.total = carry_w;
 	p.share = share_of(p.total, part.grid);
 	if (part.cum_w && blockIdx.x == 0) {
 		for (int i = tid; i <= p.segs; i += NT) { part.cum_w[i] = p.cum_w[i]; part.cum_u[i] = p.cum_u[i]; }
@@ -319,7 +319,7 @@ struct Piece {
 __device__ __forceinline__ long long piece_slot(const Attn& a, int unit, int cta, bool begins) { return a.b.n_groups && !a.lists ? (long long) unit + cta : 2ll * cta + begins; }
 // The walk over a CTA's share of the work
 struct Walk {
-	long long at, end;
+	int at, end;
 	Piece x;
 	int tiles;           // row tiles of the segment
 };
@@ -329,17 +329,20 @@ __device__ __forceinline__ void walk_segment(const Attn& a, const Part& part, co
 	k.x.q = seq_of(p.v, k.x.s);
 	k.x.key0 = k.x.seg < a.b.n_groups ? 0 : p.shs[k.x.s];
 }
+__device__ __forceinline__ void share_begin(int total, int share, Walk& k) {
+	k.at = (int) min((unsigned long long) share * blockIdx.x, (unsigned long long) total);
+	k.end = k.at + min(share, total - k.at);
+}
 // The piece of the unit at k.at, `in` of whose work lies behind the share's start; the walk's place moves behind it
-__device__ __forceinline__ void walk_piece(const Part& part, Walk& k, long long in) {
-	const long long left = k.x.w + part.lead - in, take = min(left, k.end - k.at); // tiles lie behind the lead
-	k.x.j0 = (int) max(in - part.lead, 0ll);
-	k.x.j1 = (int) max(in + take - part.lead, 0ll);
+__device__ __forceinline__ void walk_piece(const Part& part, Walk& k, int in) {
+	const int left = k.x.w + part.lead - in, take = min(left, k.end - k.at); // tiles lie behind the lead
+	k.x.j0 = max(in - part.lead, 0);
+	k.x.j1 = max(in + take - part.lead, 0);
 	k.at += take;
 }
 // false: nothing for this CTA
 __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, const Plan& p, Walk& k) {
-	k.at = min(p.share * blockIdx.x, p.total);
-	k.end = min(k.at + p.share, p.total);
+	share_begin(p.total, p.share, k);
 	if (k.at >= k.end) return false;
 	int lo = 0, hi = p.segs - 1; // the last segment that begins at or before k.at
 	while (lo < hi) {
@@ -349,17 +352,21 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, cons
 	}
 	k.x.seg = lo;
 	walk_segment(a, part, p, k);
-	long long rem = k.at - p.cum_w[lo];
-	const long long per = (p.cum_w[lo + 1] - p.cum_w[lo]) / a.c.G;
-	k.x.g = (int) (rem / per);
+	int rem = k.at - p.cum_w[lo];
+	const int per = (p.cum_w[lo + 1] - p.cum_w[lo]) / a.c.G;
+	k.x.g = rem / per;
 	rem -= per * k.x.g;
 	const int lane = threadIdx.x & 31;
+	if (k.tiles == 1) { // the only one of its kv head
+		k.x.t = 0;
+		k.x.w = per - part.lead;
+	} else
 	for (int t0 = 0;; t0 += 32) { // whole warps walk: 32 units at a time
 		const int w = t0 + lane < k.tiles ? unit_work(a, part, lo, k.x.rows, k.x.q, p.shs[k.x.s], t0 + lane) : 0;
-		long long sum = w;
+		int sum = w;
 #pragma unroll
 		for (int o = 1; o < 32; o <<= 1) {
-			const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+			const int x = __shfl_up_sync(0xffffffffu, sum, o);
 			if (lane >= o) sum += x;
 		}
 		const unsigned m = __ballot_sync(0xffffffffu, sum > rem);
@@ -396,14 +403,13 @@ __device__ __forceinline__ bool walk_next(const Attn& a, const Part& part, const
 }
 // With lists: units are (row, kv head, M of its query heads), all of the same work
 __device__ __forceinline__ int list_tiles(const Attn& a) { return (int) ((((long long) a.S << a.c.shift) + KT - 1) / KT); }
-__device__ __forceinline__ long long list_units(const Attn& a, const Part& part) { return (long long) a.b.N * a.c.G * ((a.rep + part.M - 1) / part.M); }
-__device__ __forceinline__ long long list_total(const Attn& a, const Part& part) { return list_units(a, part) * (list_tiles(a) + part.lead); }
-__device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk& k, long long unit, bool walking) {
+__device__ __forceinline__ int list_total(const Attn& a, const Part& part) { return a.b.N * a.c.G * ((a.rep + part.M - 1) / part.M) * (list_tiles(a) + part.lead); }
+__device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk& k, int unit, bool walking) {
 	const int tiles = (a.rep + part.M - 1) / part.M;
-	k.x.u = (int) unit;
-	k.x.t = (int) (unit % tiles);
-	k.x.g = (int) (unit / tiles % a.c.G);
-	const int row = (int) (unit / tiles / a.c.G);
+	const int of = unit / tiles, row = of / a.c.G;
+	k.x.u = unit;
+	k.x.t = unit - of * tiles;
+	k.x.g = of - row * a.c.G;
 	const bool same_row = walking && row == k.x.row0;
 	k.x.row0 = row;
 	k.x.rows = a.rep;
@@ -416,9 +422,8 @@ __device__ __forceinline__ void list_unit(const Attn& a, const Part& part, Walk&
 	}
 }
 __device__ __forceinline__ bool list_begin(const Attn& a, const Part& part, Walk& k) {
-	const long long total = list_total(a, part), share = share_of(total, part.grid);
-	k.at = min(share * blockIdx.x, total);
-	k.end = min(k.at + share, total);
+	const int total = list_total(a, part);
+	share_begin(total, share_of(total, part.grid), k);
 	if (k.at >= k.end) return false;
 	const int w = list_tiles(a) + part.lead;
 	list_unit(a, part, k, k.at / w, false);
@@ -432,9 +437,9 @@ __device__ __forceinline__ bool list_next(const Attn& a, const Part& part, Walk&
 	return true;
 }
 // by one thread of a CTA, before its first walk_next / list_next
-__device__ __forceinline__ void write_head(const Attn& a, const Part& part, const Walk& k, bool any, bool alone, long long share) {
+__device__ __forceinline__ void write_head(const Attn& a, const Part& part, const Walk& k, bool any, bool alone, int share) {
 	Head h = {};
-	if (any && alone) h = Head{k.x.u, k.x.j0, k.x.w, (int) share, k.x.row0, k.x.t * part.M, min(part.M, k.x.rows - k.x.t * part.M), k.x.g};
+	if (any && alone) h = Head{k.x.u, k.x.j0, k.x.w, share, k.x.row0, k.x.t * part.M, min(part.M, k.x.rows - k.x.t * part.M), k.x.g};
 	part.head[blockIdx.x] = h;
 }
 __device__ __forceinline__ bool row_in_seq(const Seq& q, int row) { return row >= q.a && row < q.a + q.n; }

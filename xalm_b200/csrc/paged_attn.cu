@@ -192,7 +192,7 @@ __device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, i
 	const Part& p = a.part[i];
 	int row0, s;
 	const int rows = seg_rows(v, a.rep, seg, row0, s);
-	const long long total = p.cum_w[a.b.n_groups + a.b.B], seg_at = p.cum_w[seg], seg_w = p.cum_w[seg + 1] - seg_at;
+	const int total = p.cum_w[a.b.n_groups + a.b.B], seg_at = p.cum_w[seg], seg_w = p.cum_w[seg + 1] - seg_at;
 	const int sh = p.shs[s_first], u0 = p.cum_u[seg];
 	if (!in_part(p, rows) || !seg_w) return false;
 	const int tiles = (rows + p.M - 1) / p.M, t = idx / p.M, lane = threadIdx.x & 31;
@@ -200,21 +200,15 @@ __device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, i
 	const Seq q = seq_of(v, s_first);
 	const int w = unit_tiles(a, p, seg, rows, q, sh, t);
 	if (!w) return false;
-	long long before = 0;
+	int before = 0;
 	if (t) {
 		for (int j = lane; j < t; j += 32) before += unit_work(a, p, seg, rows, q, sh, j);
-#pragma unroll
-		for (int e = 16; e; e >>= 1) before += __shfl_xor_sync(0xffffffffu, before, e);
+		before = __reduce_add_sync(0xffffffffu, before);
 	}
-	const long long share = share_of(total, p.grid), w0 = seg_at + seg_w / a.c.G * g + before + p.lead;
+	const int share = share_of(total, p.grid), w0 = seg_at + seg_w / a.c.G * g + before + p.lead;
 	o.unit = u0 + g * tiles + t;
-	if (total < 0x80000000ll) { // short divisions where they do
-		o.cta = (int) ((unsigned) w0 / (unsigned) share);
-		o.n = (int) ((unsigned) (w0 + w - 1) / (unsigned) share) - o.cta + 1;
-	} else {
-		o.cta = (int) (w0 / share);
-		o.n = (int) ((w0 + w - 1) / share) - o.cta + 1;
-	}
+	o.cta = w0 / share;
+	o.n = (w0 + w - 1) / share - o.cta + 1;
 	o.part = i;
 	o.at = idx - t * p.M;
 	return true;

@@ -233,23 +233,19 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				}
 				__syncwarp();
 			}
-			float s[2][4], s2[2][4]; // even and odd steps apart: a product waits for the one before into the same sum
+			float s[2][4];
 #pragma unroll
 			for (int i = 0; i < 2; i++)
 #pragma unroll
-				for (int e = 0; e < 4; e++) s[i][e] = s2[i][e] = 0.f;
+				for (int e = 0; e < 4; e++) s[i][e] = 0.f;
 #pragma unroll
 			for (int kk = 0; kk < D / 16; kk++)
 			{
 				uint32_t b[4];
 				ldsm4(b, ((tile + k_lane) ^ ((kk * 2 & 7) << 4)) + (kk >> 2) * KT * 128);
-				mma16<T>(kk & 1 ? s2[0] : s[0], qa[kk], b[0], b[1]);
-				mma16<T>(kk & 1 ? s2[1] : s[1], qa[kk], b[2], b[3]);
+				mma16<T>(s[0], qa[kk], b[0], b[1]);
+				mma16<T>(s[1], qa[kk], b[2], b[3]);
 			}
-#pragma unroll
-			for (int i = 0; i < 2; i++)
-#pragma unroll
-				for (int e = 0; e < 4; e++) s[i][e] += s2[i][e];
 			if (base + 16 > least) {
 #pragma unroll
 				for (int i = 0; i < 2; i++)

@@ -124,7 +124,7 @@ struct TcShared {
 
 template <typename T>
 __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const __grid_constant__ CUtensorMap kmap,
-                                                         const __grid_constant__ CUtensorMap vmap) {
+                                                         const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
 	extern __shared__ uint8_t raw[];
 	uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
 	uint8_t* s_q = smem;                       // [half][2 blocks][128 rows][128 bytes]
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	if (tid == 0) {
 		for (int i = 0; i < RING; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 2); }
 		for (int h = 0; h < 2; h++) {
-			mbar_init(&sh.q_full[h], 4);
+			mbar_init(&sh.q_full[h], 1);
 			for (int b = 0; b < 2; b++) { mbar_init(&sh.s_full[h][b], 1); mbar_init(&sh.p_full[h][b], 4); mbar_init(&sh.o_full[h][b], 1); }
 		}
 		sh.dead = 0;
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	const int quad = warp & 3;                           // which lanes of tensor memory a softmax warp may read
 	const uint32_t lanes = (uint32_t) (quad * 32) << 16, t_o = tmem + 256 + 128 * h;
 	const bool negative = a.scale < 0.f;
-	const float c1 = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f; // a negative scale turns the queries' signs
+	const float c1 = a.scale == 0.f ? 1e-30f : fabsf(a.scale) * 1.4426950408889634f; // a negative scale turns the scores' signs
 	Walk k;
 	// tiles of the CTA, tiles and pieces of this warp's half so far
 	int n = 0, done = 0, pieces = 0;
@@ -236,8 +236,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			const int r = quad * 32 + lane, wt = tid & 127, row = h * HALF_ROWS + r, first = x.t * TC_ROWS + h * HALF_ROWS; // row of the half, of the unit; the half's first row of the segment
 			const bool direct = x.j0 == 0 && x.j1 == x.w && !p.prefix && x.key0 == 0, mine = row < p.rows;
 			const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
-			// rows two at a time, 16 bytes to a lane: token and head of row first + quad * 32 + (lane >> 4) + 2 i
-			const int row0 = x.row0, head0 = x.g * a.rep, at0 = first + quad * 32 + (lane >> 4), tok0 = at0 / a.rep, sub0 = at0 - tok0 * a.rep, ch = lane & 15;
+			const int row0 = x.row0, head0 = x.g * a.rep;
 			float m = -INFINITY, l = 0.f;
 			int lim = p.most, least = p.most;
 			if (!p.prefix) {
@@ -245,29 +244,28 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				lim = own_keys(x.q, x.key0, a.rep, min(first + r, x.t * TC_ROWS + p.rows - 1));
 			}
 			if (tiles) {
-				int tok = tok0, sub = sub0;
-				const int left = p.rows - h * HALF_ROWS - quad * 32 - (lane >> 4); // row 2 i is one of the unit's while 2 i < left
+				if (HALF_ROWS % a.rep == 0) { // whole tokens: the copy engine brings them, those of other sequences behind the last too (rows that nobody asks for)
+					asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // what the piece before has laid there on its way out
+					bar_sync(2 + h, 128);
+					if (wt < 32 && elect()) {
+						mbar_expect_tx(&sh.q_full[h], (uint32_t) (dc * QB));
+						for (int i = 0; i < dc; i++)
+							asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(s_q + (h * 2 + i) * QB)),
+							             "l"(&qmap), "r"(i * 64), "r"(0), "r"(row0 + first / a.rep), "r"(x.g), "r"(smem_u32(&sh.q_full[h]))
+							             : "memory");
+					}
+				} else {
 #pragma unroll 1
-				for (int i0 = 0; i0 < 32; i0 += 16) { // eight loads on their way together
-					uint4 v[8];
-#pragma unroll
-					for (int i = 0; i < 8; i++) {
-						const bool some = i0 + 2 * i < left && ch * 8 < a.c.d;
-						v[i] = *reinterpret_cast<const uint4*>(a.q + (some ? ((long long) (row0 + tok) * a.q_row + (head0 + sub) * a.c.d + ch * 8) * 2 : 0));
-						if (!some) v[i] = make_uint4(0, 0, 0, 0);
-						sub += 2;
-						while (sub >= a.rep) { sub -= a.rep; tok++; }
+					for (int i = lane; i < 32 * dc * 8; i += 32) { // 16 bytes of one of this warp's rows
+						const int rr = quad * 32 + i / (dc * 8), ch = i % (dc * 8), w = first + rr, tok = w / a.rep;
+						uint4 v = make_uint4(0, 0, 0, 0);
+						if (h * HALF_ROWS + rr < p.rows && ch * 8 < a.c.d) v = *reinterpret_cast<const uint4*>(a.q + ((long long) (row0 + tok) * a.q_row + (head0 + w - tok * a.rep) * a.c.d + ch * 8) * 2);
+						*reinterpret_cast<uint4*>(s_q + (h * 2 + (ch >> 3)) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v;
 					}
-#pragma unroll
-					for (int i = 0; i < 8; i++) {
-						const int rr = quad * 32 + i0 + i * 2 + (lane >> 4);
-						if (negative) { v[i].x ^= 0x80008000u; v[i].y ^= 0x80008000u; v[i].z ^= 0x80008000u; v[i].w ^= 0x80008000u; }
-						if (ch < dc * 8) *reinterpret_cast<uint4*>(s_q + (h * 2 + (ch >> 3)) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v[i];
-					}
+					asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+					bar_sync(2 + h, 128);
+					if (wt == 0) mbar_arrive(&sh.q_full[h]);
 				}
-				asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-				__syncwarp();
-				if (lane == 0) mbar_arrive(&sh.q_full[h]);
 			}
 			for (int j = 0; j < tiles; j++) {
 				const int c = done + j, b = c & 1, base = (x.j0 + j) * KT;
@@ -289,6 +287,10 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				__syncwarp();
 				wait_ld(s);
 				wait_ld(s + 32);
+				if (negative) {
+#pragma unroll
+					for (int i = 0; i < KT; i++) s[i] ^= 0x80000000u;
+				}
 				if (base + KT > least) {
 #pragma unroll
 					for (int i = 0; i < KT; i++)
@@ -344,61 +346,57 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				__syncwarp();
 				if (lane == 0) mbar_arrive(&sh.p_full[h][b]);
 			}
-			// ---- the piece's sums: 64 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side ----
+			// ---- the piece's sums: 32 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side ----
 			if (tiles && ok) ok = wait_for(&sh.o_full[h][(done + tiles - 1) & 1], ((done + tiles - 1) >> 1) & 1, &sh.dead, a.c);
 			fence_after();
 			bool again = false;
-			uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // two blocks of 32 rows of 128 bytes, QB apart
+			uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // 32 rows of 128 bytes
 			const bool any = l > 0.f || l != l;
 			const float inv = direct ? (any ? 1.f / l : 0.f) : 1.f;
 			if (mine) {
 				if (!direct) {
 					if (slot < part.slots) part.ml[slot * TC_ROWS + row] = make_float2(m, l);
 				} else if (a.lse) {
-					const int w = first + r;
-					a.lse[(long long) (x.row0 + w / a.rep) * a.H + x.g * a.rep + w % a.rep] = any ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+					const int w = first + r, tok = w / a.rep;
+					a.lse[(long long) (row0 + tok) * a.H + head0 + w - tok * a.rep] = any ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 				}
 			}
+			// where the rows go that this lane writes: four rows at a time, eight lanes to a row
+			const int left = p.rows - h * HALF_ROWS - quad * 32 - (lane >> 3), ch = lane & 7;
 #pragma unroll 1
-			for (int c0 = 0; c0 < a.c.dv; c0 += 64) {
-				uint32_t o[64];
+			for (int c0 = 0; c0 < a.c.dv; c0 += 32) {
+				uint32_t o[32];
 #pragma unroll
-				for (int i = 0; i < 64; i++) o[i] = 0;
+				for (int i = 0; i < 32; i++) o[i] = 0;
 				if (tiles) {
 					ld32(t_o + lanes + c0, o);
-					ld32(t_o + lanes + c0 + 32, o + 32);
 					wait_ld(o);
-					wait_ld(o + 32);
 				}
 #pragma unroll
-				for (int i = 0; i < 16; i++) {
+				for (int i = 0; i < 8; i++) {
 					float4 v = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-					const float worst = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), sum = v.x + v.y + v.z + v.w;
-					again = again || (c0 + i * 4 < a.c.dv && (worst > 3.0e38f || sum != sum));
+					const float sum = fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w);
+					again = again || (c0 + i * 4 < a.c.dv && !(sum <= 3.0e38f));
 					if (direct) { v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv; }
-					*reinterpret_cast<float4*>(stage + (i >> 3) * QB + lane * 128 + (((i & 7) ^ (lane & 7)) << 4)) = v;
+					*reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = v;
 				}
 				__syncwarp();
-				const int col = c0 + ch * 4, left = col < a.c.dv && (direct || slot < part.slots) ? p.rows - h * HALF_ROWS - quad * 32 - (lane >> 4) : 0;
-				int tok = tok0, sub = sub0;
-				float* po = part.o + (slot * TC_ROWS + h * HALF_ROWS + quad * 32 + (lane >> 4)) * a.c.dv + col;
+				const int col = c0 + ch * 4;
+				if (direct) {
 #pragma unroll 1
-				for (int i0 = 0; i0 < 16; i0 += 4) {
-					float4 v[4];
-#pragma unroll
-					for (int i = 0; i < 4; i++) {
-						const int rr = (i0 + i) * 2 + (lane >> 4);
-						v[i] = *reinterpret_cast<const float4*>(stage + (ch >> 3) * QB + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
+					for (int i = 0; i < 8; i++) {
+						const int rr = i * 4 + (lane >> 3), w = first + quad * 32 + rr, tok = w / a.rep;
+						const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((ch ^ (rr & 7)) << 4));
+						if (4 * i < left && col < a.c.dv)
+							*reinterpret_cast<uint2*>(a.out + ((long long) (row0 + tok) * a.out_row + (head0 + w - tok * a.rep) * a.c.dv + col) * 2) = make_uint2(pair16<T>(v.x, v.y), pair16<T>(v.z, v.w));
 					}
-#pragma unroll
-					for (int i = 0; i < 4; i++) {
-						if (2 * (i0 + i) < left) {
-							if (direct)
-								*reinterpret_cast<uint2*>(a.out + ((long long) (row0 + tok) * a.out_row + (head0 + sub) * a.c.dv + col) * 2) = make_uint2(pair16<T>(v[i].x, v[i].y), pair16<T>(v[i].z, v[i].w));
-							else *reinterpret_cast<float4*>(po + (i0 + i) * 2 * a.c.dv) = v[i];
-						}
-						sub += 2;
-						while (sub >= a.rep) { sub -= a.rep; tok++; }
+				} else if (slot < part.slots) {
+					float* po = part.o + (slot * TC_ROWS + h * HALF_ROWS + quad * 32 + (lane >> 3)) * a.c.dv + col;
+#pragma unroll 2
+					for (int i = 0; i < 8; i++) {
+						const int rr = i * 4 + (lane >> 3);
+						const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((ch ^ (rr & 7)) << 4));
+						if (4 * i < left && col < a.c.dv) *reinterpret_cast<float4*>(po + i * 4 * a.c.dv) = v;
 					}
 				}
 				__syncwarp();
@@ -435,12 +433,19 @@ bool tc_fits(const Cache& c, const BatchView& b) { return c.d <= 128 && c.dv <= 
 
 template <typename T>
 static int launch_typed(const Attn& a, int part, int type, cudaStream_t s) {
-	CUtensorMap kmap, vmap;
+	CUtensorMap kmap, vmap, qmap;
 	XALM_TRY(pool_map(a.c, type, true, &kmap));
 	XALM_TRY(pool_map(a.c, type, false, &vmap));
+	{ // (entries, heads of a kv head, tokens, kv heads): 64 entries of 128 rows
+		const int tokens = HALF_ROWS % a.rep == 0 ? HALF_ROWS / a.rep : 1;
+		const cuuint64_t dims[4] = {(cuuint64_t) a.c.d, (cuuint64_t) a.rep, (cuuint64_t) a.b.N, (cuuint64_t) a.c.G};
+		const cuuint64_t strides[3] = {(cuuint64_t) a.c.d * 2, (cuuint64_t) a.q_row * 2, (cuuint64_t) a.rep * a.c.d * 2};
+		const cuuint32_t box[4] = {64, (cuuint32_t) (tokens > 1 || a.rep == HALF_ROWS ? a.rep : 1), (cuuint32_t) tokens, 1};
+		XALM_TRY(encode_map(&qmap, type, 4, const_cast<uint8_t*>(a.q), dims, strides, box));
+	}
 	const size_t smem = tc_smem(a.b);
 	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-	XALM_CUDA_CHECK(launch(paged_tc_kernel<T>, a.part[part].grid, TT, smem, s, false, a, a.part[part], kmap, vmap));
+	XALM_CUDA_CHECK(launch(paged_tc_kernel<T>, a.part[part].grid, TT, smem, s, false, a, a.part[part], kmap, vmap, qmap));
 	return XALM_OK;
 }
 int launch_attn_tc(const Attn& a, int part, int type, cudaStream_t s) {

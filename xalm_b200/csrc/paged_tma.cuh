@@ -12,7 +12,7 @@ namespace paged {
 // A pool as the copy engine sees it: (64 entries, slots, blocks of 64 entries, heads, pages), boxes of min(page, 64) slots of one head with all their blocks, one behind the other.  Heads whose
 // last block is not full are (entries, slots, 1, heads, pages) and come block by block: entries behind the last read as zeros, as pages behind the pool's last do.
 __host__ __device__ __forceinline__ bool whole_heads(int dim) { return dim % 64 == 0; }
-static inline int pool_map(const Cache& c, int type, bool keys, CUtensorMap* map) {
+static inline int encode_map(CUtensorMap* map, int type, int n, void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
 	typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
 	                           CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 	static const Encode encode = [] {
@@ -25,15 +25,18 @@ static inline int pool_map(const Cache& c, int type, bool keys, CUtensorMap* map
 		return (Encode) f;
 	}();
 	if (!encode) return set_error(XALM_ERR_CUDA, "paged attention: this driver has no cuTensorMapEncodeTiled");
-	const int P = 1 << c.shift;
-	const int dim = keys ? c.d : c.dv, blocks = P >= KT && whole_heads(dim) ? dim / 64 : 1;
-	const cuuint64_t dims[5] = {(cuuint64_t) (dim / blocks), (cuuint64_t) P, (cuuint64_t) blocks, (cuuint64_t) c.G, (cuuint64_t) c.pages};
-	const cuuint64_t strides[4] = {(cuuint64_t) (keys ? c.k_slot : c.v_slot) * 2, 128, (cuuint64_t) (keys ? c.k_head : c.v_head) * 2, (cuuint64_t) (keys ? c.k_page : c.v_page) * 2};
-	const cuuint32_t box[5] = {64, (cuuint32_t) (P < KT ? P : KT), (cuuint32_t) blocks, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
-	const CUresult r = encode(map, type == XALM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, keys ? c.k : c.v, dims, strides, box, steps,
+	const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+	const CUresult r = encode(map, type == XALM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t) n, base, dims, strides, box, steps,
 	                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 	if (r != CUDA_SUCCESS) return set_error(XALM_ERR_CUDA, "paged attention: cuTensorMapEncodeTiled failed (%d)", (int) r);
 	return XALM_OK;
+}
+static inline int pool_map(const Cache& c, int type, bool keys, CUtensorMap* map) {
+	const int P = 1 << c.shift, dim = keys ? c.d : c.dv, blocks = P >= KT && whole_heads(dim) ? dim / 64 : 1;
+	const cuuint64_t dims[5] = {(cuuint64_t) (dim / blocks), (cuuint64_t) P, (cuuint64_t) blocks, (cuuint64_t) c.G, (cuuint64_t) c.pages};
+	const cuuint64_t strides[4] = {(cuuint64_t) (keys ? c.k_slot : c.v_slot) * 2, 128, (cuuint64_t) (keys ? c.k_head : c.v_head) * 2, (cuuint64_t) (keys ? c.k_page : c.v_page) * 2};
+	const cuuint32_t box[5] = {64, (cuuint32_t) (P < KT ? P : KT), (cuuint32_t) blocks, 1, 1};
+	return encode_map(map, type, 5, keys ? c.k : c.v, dims, strides, box);
 }
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, uint64_t* bar) {
 	asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(map), "r"(x), "r"(slot),
