@@ -703,7 +703,7 @@ static int sm_count(int device, int* n) {
 }
 
 constexpr int SMALL_ROWS = 16;
-constexpr int LEAD = 6, LEAD_TC = 8;
+constexpr int LEAD = 6, LEAD_TC = 12;
 
 // ---- attention: parts, workspace --------------------------------------------------------------------------------------------------------------
 static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchView& b, int heads, int n_lists, Attn& a, size_t* bytes) {

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 }
 
 // =========================================================================================================================================
-// The join of what several CTAs have of the same rows, a warp to a row.  A lane takes a piece's maximum and sum, then the pieces' rows are added with their weights, four
+// The join of what several CTAs have of the same rows, a warp to a row.  A lane takes a piece's maximum and sum, then the pieces' rows are added with their weights, eight
 // loads on their way at a time.  Two kinds of blocks: with groups, for a kv head of a sequence whose rows read shared pages; and for 16 rows
 // of the units that a CTA's share begins inside.  Bound by the latency of three or four loads that depend on one another.
 // =========================================================================================================================================
@@ -214,7 +214,7 @@ __device__ __forceinline__ bool join_unit(const Attn& a, const View& v, int i, i
 	return true;
 }
 
-template <typename T>
+template <typename T, int NC> // NC x 128 columns
 __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], int found, int row, int h) {
 	const int lane = threadIdx.x & 31, dv = a.c.dv;
 	const int n0 = found ? u[0].n : 0, n = n0 + (found > 1 ? u[1].n : 0); // pieces
@@ -241,9 +241,9 @@ __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], 
 	m = warp_max(m);
 	nan = __any_sync(0xffffffffu, nan);
 	const float base = nan ? NAN : m == -INFINITY ? 0.f : m;
-	float l = 0.f, acc[8];
+	float l = 0.f, acc[4 * NC];
 #pragma unroll
-	for (int i = 0; i < 8; i++) acc[i] = 0.f;
+	for (int i = 0; i < 4 * NC; i++) acc[i] = 0.f;
 	for (int i0 = 0; i0 < n; i0 += 32) {
 		float wgt = 0.f;
 		bool some = false;
@@ -255,10 +255,11 @@ __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], 
 			if (some) l += ml.y * wgt; // a sum that is NaN stays one
 		}
 		for (unsigned left = __ballot_sync(0xffffffffu, some); left;) {
-			float4 x[4][2];
-			float f[4];
+			constexpr int NB = 8 / NC;
+			float4 x[NB][NC];
+			float f[NB];
 #pragma unroll
-			for (int j = 0; j < 4; j++) {
+			for (int j = 0; j < NB; j++) {
 				const bool one = left != 0;
 				const int from = one ? __ffs(left) - 1 : 0;
 				left &= left - 1;
@@ -266,13 +267,13 @@ __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], 
 				const float* at = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_at), from));
 				if (!one) f[j] = 0.f;
 #pragma unroll
-				for (int c = 0; c < 2; c++)
+				for (int c = 0; c < NC; c++)
 					x[j][c] = one && c * 128 + lane * 4 < dv ? *reinterpret_cast<const float4*>(at + c * 128 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 			}
 #pragma unroll
-			for (int j = 0; j < 4; j++)
+			for (int j = 0; j < NB; j++)
 #pragma unroll
-				for (int c = 0; c < 2; c++) {
+				for (int c = 0; c < NC; c++) {
 					acc[4 * c] = fmaf(x[j][c].x, f[j], acc[4 * c]);
 					acc[4 * c + 1] = fmaf(x[j][c].y, f[j], acc[4 * c + 1]);
 					acc[4 * c + 2] = fmaf(x[j][c].z, f[j], acc[4 * c + 2]);
@@ -285,7 +286,7 @@ __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], 
 	const float inv = any ? 1.f / l : 0.f;
 	T* out = reinterpret_cast<T*>(a.out) + (long long) row * a.out_row + h * dv;
 #pragma unroll
-	for (int c = 0; c < 2; c++)
+	for (int c = 0; c < NC; c++)
 		if (c * 128 + lane * 4 < dv) {
 			T v[4];
 #pragma unroll
@@ -299,17 +300,14 @@ __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], 
 // blocks of a part's boundaries: one to 16 rows of each
 __host__ __device__ __forceinline__ int boundary_blocks(const Part& p) { return p.grid * (p.M > JR ? p.M / JR : 1); }
 
-template <typename T>
+template <typename T, int NC>
 __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ Attn a) {
-	pdl_wait();
 	const int warp = threadIdx.x >> 5, n_seq = a.b.n_groups && !a.lists ? a.b.B * a.c.G : 0;
 	int id = blockIdx.x;
 	if (id < n_seq) {
 		const int s = id / a.c.G, g = id - s * a.c.G; // a sequence's rows of one kv head
-		const int shared = a.part[0].shs[s];
-		if (!shared) return;
 		const View v = view_of(a.c, a.b);
-		const Seq q = seq_of(v, s);
+		const Seq q = seq_of(v, s); // the caller's arrays are there already, the other kernels' are not
 		int lo = 0, hi = a.b.n_groups - 1; // its group
 		while (lo < hi) {
 			const int mid = (lo + hi + 1) >> 1;
@@ -317,17 +315,20 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ 
 			else hi = mid - 1;
 		}
 		const int first = min(group_of(v, lo).x, a.b.B - 1), row0 = seq_of(v, first).a;
+		pdl_wait();
+		if (!a.part[0].shs[s]) return;
 		for (int r = warp; r < q.n * a.rep; r += JT / 32) {
 			JoinUnit u[2];
 			int found = 0;
 			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit(a, v, i, lo, first, (q.a - row0) * a.rep + r, g, u[0]);
 			const int had = found;
 			for (int i = 0; i < a.n_parts && found == had; i++) found += join_unit(a, v, i, a.b.n_groups + s, s, r, g, had ? u[1] : u[0]);
-			join_row<T>(a, u, found, q.a + r / a.rep, g * a.rep + r % a.rep);
+			join_row<T, NC>(a, u, found, q.a + r / a.rep, g * a.rep + r % a.rep);
 		}
 		return;
 	}
 	id -= n_seq;
+	pdl_wait();
 	for (int i = 0; i < a.n_parts; i++) {
 		const Part& p = a.part[i];
 		const int blocks = boundary_blocks(p), chunks = blocks / p.grid;
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ 
 		for (int r = (id - cta * chunks) * JR + warp; r < min(x.rows, (id - cta * chunks) * JR + JR); r += JT / 32) {
 			const int w = x.first + r, tok = w / a.rep;
 			u[0].at = r;
-			join_row<T>(a, u, 1, x.row0 + tok, x.g * a.rep + w - tok * a.rep);
+			join_row<T, NC>(a, u, 1, x.row0 + tok, x.g * a.rep + w - tok * a.rep);
 		}
 		return;
 	}
@@ -356,9 +357,10 @@ int launch_join(const Attn& a, int type, cudaStream_t s) {
 	int grid = 0;
 	for (int i = 0; i < a.n_parts; i++) grid += boundary_blocks(a.part[i]);
 	if (a.b.n_groups && !a.lists) grid += a.b.B * a.c.G;
-	XALM_CUDA_CHECK(type == XALM_F32   ? launch(paged_join_kernel<float>, grid, JT, 0, s, true, a)
-	                : type == XALM_F16 ? launch(paged_join_kernel<__half>, grid, JT, 0, s, true, a)
-	                                   : launch(paged_join_kernel<__nv_bfloat16>, grid, JT, 0, s, true, a));
+	const bool wide = a.c.dv > 128;
+	XALM_CUDA_CHECK(type == XALM_F32   ? (wide ? launch(paged_join_kernel<float, 2>, grid, JT, 0, s, true, a) : launch(paged_join_kernel<float, 1>, grid, JT, 0, s, true, a))
+	                : type == XALM_F16 ? (wide ? launch(paged_join_kernel<__half, 2>, grid, JT, 0, s, true, a) : launch(paged_join_kernel<__half, 1>, grid, JT, 0, s, true, a))
+	                                   : (wide ? launch(paged_join_kernel<__nv_bfloat16, 2>, grid, JT, 0, s, true, a) : launch(paged_join_kernel<__nv_bfloat16, 1>, grid, JT, 0, s, true, a)));
 	return XALM_OK;
 }
 
