@@ -116,7 +116,7 @@ __device__ __forceinline__ TcPiece tc_piece(const Attn& a, const Plan& plan, con
 
 struct TcShared {
 	uint64_t full[RING], empty[RING];
-	uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2][2]; // by half and by the tile's parity, so that nobody is ever two phases ahead of a wait
+	uint64_t drained[2], q_full[2], s_full[2][2], p_full[2][2], o_full[2][2]; // by half and by the tile's parity, so that nobody is ever two phases ahead of a wait
 	uint32_t tmem;
 	int dead, flag[2], ids[32];
 	float buf[2][256];
@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	if (tid == 0) {
 		for (int i = 0; i < RING; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 2); }
 		for (int h = 0; h < 2; h++) {
+			mbar_init(&sh.drained[h], 1);
 			mbar_init(&sh.q_full[h], 1);
 			for (int b = 0; b < 2; b++) { mbar_init(&sh.s_full[h][b], 1); mbar_init(&sh.p_full[h][b], 4); mbar_init(&sh.o_full[h][b], 1); }
 		}
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	bool ok = true;
 	bool more = walk_begin(a, part, plan, k);
 	if (tid == 96) write_head(a, part, k, more, more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, plan.share); // a warp with nothing else to do
-	for (; more && ok; more = walk_next(a, part, plan, k)) {
+	for (; more && (ok || warp >= 4); more = walk_next(a, part, plan, k)) { // softmax warps meet at barriers: they go on to the end whatever happens, and wait for nothing once a wait has given up
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue;
 		const TcPiece p = tc_piece(a, plan, x);
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				if (HALF_ROWS % a.rep == 0) { // whole tokens: the copy engine brings them, those of other sequences behind the last too (rows that nobody asks for)
 					asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // what the piece before has laid there on its way out
 					bar_sync(2 + h, 128);
-					if (wt < 32 && elect()) {
+					if (wt < 32 && elect() && !*(volatile int*) &sh.dead) {
 						mbar_expect_tx(&sh.q_full[h], (uint32_t) (dc * QB));
 						for (int i = 0; i < dc; i++)
 							asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(s_q + (h * 2 + i) * QB)),
@@ -270,14 +271,14 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			for (int j = 0; j < tiles; j++) {
 				const int c = done + j, b = c & 1, base = (x.j0 + j) * KT;
 				const uint32_t t_s = tmem + 128 * h + 64 * b + lanes;
-				if (!(ok = wait_for(&sh.s_full[h][b], (c >> 1) & 1, &sh.dead, a.c))) break;
+				ok = wait_for(&sh.s_full[h][b], (c >> 1) & 1, &sh.dead, a.c) && ok;
 				fence_after();
 				uint32_t s[KT];
 				ld32(t_s, s);
 				ld32(t_s + 32, s + 32);
 				if (base + KT > p.most) { // slots that no row sees may hold anything: as zeros they add nothing
 					const int st = (n + j) % RING;
-					if (!(ok = wait_for(&sh.full[st], ((n + j) / RING) & 1, &sh.dead, a.c))) break;
+					ok = wait_for(&sh.full[st], ((n + j) / RING) & 1, &sh.dead, a.c) && ok;
 					for (int i = wt; i < (base + KT - p.most) * vc * 8; i += 128) {
 						const int rr = p.most - base + i / (vc * 8), cc = i % (vc * 8);
 						*reinterpret_cast<uint4*>(s_v + (st * 2 + (cc >> 3)) * KB + rr * 128 + ((cc & 7) << 4)) = make_uint4(0, 0, 0, 0);
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool grow = mx > m + 11.5f;
 				if (j == 0) m = mx;
 				else if (__any_sync(0xffffffffu, grow)) { // rare: the sums so far are complete before they are rescaled
-					if (!(ok = wait_for(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c))) break;
+					ok = wait_for(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c) && ok;
 					fence_after();
 					const float to = grow ? mx : m, f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
 #pragma unroll 1
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				if (lane == 0) mbar_arrive(&sh.p_full[h][b]);
 			}
 			// ---- the piece's sums: 32 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side ----
-			if (tiles && ok) ok = wait_for(&sh.o_full[h][(done + tiles - 1) & 1], ((done + tiles - 1) >> 1) & 1, &sh.dead, a.c);
+			if (tiles) ok = wait_for(&sh.o_full[h][(done + tiles - 1) & 1], ((done + tiles - 1) >> 1) & 1, &sh.dead, a.c) && ok;
 			fence_after();
 			bool again = false;
 			uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // 32 rows of 128 bytes
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				// A value that is not finite and that only later rows see has met probabilities of zero: those rows are done again, key by key
 				if (wt == 0) sh.flag[h] = 0;
 				bar_sync(2 + h, 128);
-				if (again && mine) sh.flag[h] = 1;
+				if (again && mine && ok) sh.flag[h] = 1;
 				bar_sync(2 + h, 128);
 				const bool redo = *(volatile int*) &sh.flag[h] != 0;
 				bar_sync(2 + h, 128);
@@ -422,6 +423,17 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	}
 	fence_before();
 	__syncthreads();
+	if (*(volatile int*) &sh.dead) { // a wait gave up: what is still on its way into shared or tensor memory ends first
+		if (warp == 1 || warp == 2) {
+			if (elect()) {
+				commit(&sh.drained[h]);
+				wait_some(&sh.drained[h], 0);
+				if (pieces) wait_some(&sh.q_full[h], (pieces - 1) & 1);
+			}
+			__syncwarp();
+		}
+		__syncthreads();
+	}
 	if (warp == 1) {
 		fence_after();
 		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
