@@ -75,7 +75,7 @@ class PagedCache:
         bits = int(self.status.item())
         self.status.zero_()
         if bits:
-            _refuse("paged cache: " + " and ".join(t for b, t in ((1, "a table names a page outside the pool"), (2, "starts, lens and table do not fit")) if bits & b))
+            _refuse("paged cache: " + " and ".join(t for b, t in ((1, "a table names a page outside the pool"), (2, "starts, lens and table do not fit"), (4, "a kernel gave up a wait for its copies or products")) if bits & b))
 
 
 class Batch:
@@ -97,6 +97,17 @@ class Batch:
         self.c = _Batch(0, table.shape[0], table.shape[1], 0 if groups is None else shared.shape[0], starts.data_ptr(), lens.data_ptr(), table.data_ptr(), row,
                         0 if groups is None else groups.data_ptr(), 0 if groups is None else shared.data_ptr())
         self.p = C.addressof(self.c)
+        self.sized = {}  # the same with a call's number of rows, which calls in other threads do not change
+
+    def of(self, rows):
+        c = self.sized.get(rows)
+        if c is None:
+            if len(self.sized) > 1000:
+                self.sized.clear()
+            c = _Batch.from_buffer_copy(self.c)
+            c.rows = rows
+            c = self.sized[rows] = (C.addressof(c), c)
+        return c
 
 
 def _rows(t, what, n, heads, dim, dtype, device):
@@ -114,8 +125,7 @@ def _rows(t, what, n, heads, dim, dtype, device):
 def _start(cache, batch, rows):
     if batch.device != cache.device:
         _refuse(f"paged cache: a batch on {batch.device}, a cache on {cache.device}")
-    batch.c.rows = rows
-    return _stream(cache.index)
+    return batch.of(rows), _stream(cache.index)
 
 
 def _heads(q):
@@ -128,14 +138,14 @@ def append(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_o
     """k (rows, kv_heads, dim) and v (rows, kv_heads, vdim) into the pages of their sequences; returns the turned queries in the cache's type (None without q).  freq
     (n): the first 2 n entries of every head are turned."""
     n, dev, dt = k.shape[0], cache.device, k.dtype
-    stream = _start(cache, batch, n)
+    (bp, held), stream = _start(cache, batch, n)
     kr, vr = _rows(k, "k", n, cache.kv_heads, cache.dim, dt, dev), _rows(v, "v", n, cache.kv_heads, cache.vdim, dt, dev)
     qr = qor = heads = qp = qop = fp = rot = 0
     if q is not None:
         heads = _heads(q)
         qr = _rows(q, "q", n, heads, cache.dim, dt, dev)
         if q_out is None:
-            q_out = torch.empty((n, heads, cache.dim), dtype=cache.dtype, device=dev)
+            q_out = q.new_empty((n, heads, cache.dim), dtype=cache.dtype)
             qor = heads * cache.dim
         else:
             qor = _rows(q_out, "q_out", n, heads, cache.dim, cache.dtype, dev)
@@ -146,35 +156,35 @@ def append(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_o
         if freq.dtype is not torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev:
             _refuse(f"paged append: freq {tuple(freq.shape)} {freq.dtype} on {freq.device}")
         fp, rot = freq.data_ptr(), freq.shape[0]
-    capi.check(capi.lib().xalm_cuda_paged_append(cache.p, batch.p, k.data_ptr(), kr, v.data_ptr(), vr, qp, qr, heads, _type(k), qop, qor, fp, rot, mag, neighbours, stream))
+    capi.check(capi.lib().xalm_cuda_paged_append(cache.p, bp, k.data_ptr(), kr, v.data_ptr(), vr, qp, qr, heads, _type(k), qop, qor, fp, rot, mag, neighbours, stream))
     return q_out
 
 
 def _attend(cache, batch, q, lists, scale, out, want_lse):
-    n, heads, dev = q.shape[0], _heads(q), cache.device
-    stream = _start(cache, batch, n)
+    heads, n, dev = _heads(q), q.shape[0], cache.device
+    (bp, held), stream = _start(cache, batch, n)
     qr = _rows(q, "q", n, heads, cache.dim, cache.dtype, dev)
     if out is None:
-        out = torch.empty((n, heads, cache.vdim), dtype=cache.dtype, device=dev)
+        out = q.new_empty((n, heads, cache.vdim))  # torch.empty takes a microsecond longer
         outr = heads * cache.vdim
     else:
         outr = _rows(out, "out", n, heads, cache.vdim, cache.dtype, dev)
-    lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if want_lse else None
+    lse = q.new_empty((n, heads), dtype=torch.float32) if want_lse else None
     s, L = 0 if lists is None else lists.shape[2], capi.lib()
     sizes = n, heads, s, batch.c.seqs, batch.c.groups
     need = cache.needs.get(sizes)
     if need is None:
         b = C.c_size_t(0)
-        capi.check(L.xalm_cuda_paged_workspace(cache.p, batch.p, heads, s, C.byref(b)))
+        capi.check(L.xalm_cuda_paged_workspace(cache.p, bp, heads, s, C.byref(b)))
         if len(cache.needs) > 1000:
             cache.needs.clear()
         need = cache.needs[sizes] = b.value
-    work = torch.empty(need, dtype=torch.uint8, device=dev)  # the current stream's, or the graph's that is being captured
+    work = q.new_empty(need, dtype=torch.uint8)  # the current stream's, or the graph's that is being captured
     lp = None if lse is None else lse.data_ptr()
     if lists is None:
-        capi.check(L.xalm_cuda_paged_attend(cache.p, batch.p, q.data_ptr(), qr, heads, scale, out.data_ptr(), outr, lp, work.data_ptr(), need, stream))
+        capi.check(L.xalm_cuda_paged_attend(cache.p, bp, q.data_ptr(), qr, heads, scale, out.data_ptr(), outr, lp, work.data_ptr(), need, stream))
     else:
-        capi.check(L.xalm_cuda_paged_attend_selected(cache.p, batch.p, q.data_ptr(), qr, heads, lists.data_ptr(), s, scale, out.data_ptr(), outr, lp, work.data_ptr(), need, stream))
+        capi.check(L.xalm_cuda_paged_attend_selected(cache.p, bp, q.data_ptr(), qr, heads, lists.data_ptr(), s, scale, out.data_ptr(), outr, lp, work.data_ptr(), need, stream))
     return (out, lse) if want_lse else out
 
 
@@ -186,14 +196,14 @@ def attend(cache, batch, q, scale, out=None, want_lse=False):
 
 def select(cache, batch, q, top, first=1, recent=1, out=None):
     """The `top` pages that each row and kv head reads: (rows, kv_heads, top) int32, places in the sequence, ascending, -1 behind; rows outside every sequence are left as they were."""
-    n, heads, dev = q.shape[0], _heads(q), cache.device
-    stream = _start(cache, batch, n)
+    heads, n, dev = _heads(q), q.shape[0], cache.device
+    (bp, held), stream = _start(cache, batch, n)
     qr = _rows(q, "q", n, heads, cache.dim, cache.dtype, dev)
     if out is None:
-        out = torch.empty((n, cache.kv_heads, max(top, 0)), dtype=torch.int32, device=dev)
+        out = q.new_empty((n, cache.kv_heads, max(top, 0)), dtype=torch.int32)
     elif out.shape != (n, cache.kv_heads, top) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != dev:
         _refuse(f"paged select: out {tuple(out.shape)} {out.dtype}")
-    capi.check(capi.lib().xalm_cuda_paged_select(cache.p, batch.p, q.data_ptr(), qr, heads, top, first, recent, out.data_ptr(), stream))
+    capi.check(capi.lib().xalm_cuda_paged_select(cache.p, bp, q.data_ptr(), qr, heads, top, first, recent, out.data_ptr(), stream))
     return out
 
 
