@@ -659,11 +659,12 @@ static int check_cache(const xalm_paged_cache* c, Cache& o) {
 	          c->pages, shift, c->kv_heads, c->dim, c->vdim, c->status};
 	return XALM_OK;
 }
-static int check_batch(const xalm_paged_batch* b, BatchView& o) {
+static int check_batch(const xalm_paged_batch* b, const Cache& c, BatchView& o) {
 	if (!b) return set_error(XALM_ERR_INVALID, "paged cache: batch is NULL");
 	if (b->rows < 0 || b->seqs < 0 || b->max_pages < 0 || b->groups < 0 || b->table_row < b->max_pages)
 		return set_error(XALM_ERR_INVALID, "paged cache: %d rows, %d sequences of %d pages (rows %lld apart), %d groups", b->rows, b->seqs, b->max_pages, b->table_row, b->groups);
 	if ((long long) b->seqs + b->groups > MAX_SEGMENTS) return set_error(XALM_ERR_INVALID, "paged cache: %d sequences and %d groups are more than %d", b->seqs, b->groups, MAX_SEGMENTS);
+	if ((long long) b->max_pages << c.shift > 1ll << 30) return set_error(XALM_ERR_INVALID, "paged cache: tables of %d pages of %d tokens (at most 2^30 tokens)", b->max_pages, 1 << c.shift);
 	if (b->seqs && (!b->starts || !b->lens || (b->max_pages && !b->table))) return set_error(XALM_ERR_INVALID, "paged cache: starts/lens/table is NULL");
 	if (b->groups && (!b->group_bounds || !b->group_shared)) return set_error(XALM_ERR_INVALID, "paged cache: group_bounds/group_shared is NULL");
 	o = BatchView{b->rows, b->seqs, b->max_pages, b->groups, b->starts, b->lens, b->table, b->table_row, b->group_bounds, b->group_shared};
@@ -727,7 +728,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		Part& p = a.part[i];
 		const bool big = tc && i == 0;
 		p.M = big ? TC_ROWS : 16;
-		p.grid = sms * (big ? 1 : f32 ? 2 : mma_ctas_per_sm(c, b, n_lists));
+		p.grid = sms * (big ? 1 : f32 ? rows_ctas_per_sm(c, b, n_lists) : mma_ctas_per_sm(c, b, n_lists));
 		p.lead = big ? LEAD_TC : LEAD;
 		p.least_rows = big ? SMALL_ROWS + 1 : 1;
 		p.most_rows = tc && !big ? SMALL_ROWS : 0x7fffffff;
@@ -735,7 +736,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		// a segment of `rows` rows has at most rows / M + 1 tiles, a part that takes short ones only has one
 		const long long tiles = n_lists ? (long long) b.N * ((a.rep + p.M - 1) / p.M) : (tc && !big ? 0 : rows / p.M) + b.B + (b.n_groups ? (tc && !big ? 0 : rows / p.M) + b.n_groups : 0);
 		if (tiles * c.G + p.grid > 0x7fffffff / p.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
-		const long long keys = std::min((long long) b.max_pages << c.shift, 0x7fffffffll), work = n_lists ? (((long long) n_lists << c.shift) + KT - 1) / KT : keys / KT + 1;
+		const long long keys = (long long) b.max_pages << c.shift, work = n_lists ? (((long long) n_lists << c.shift) + KT - 1) / KT : keys / KT + 1;
 		if (tiles * c.G > 0x7fffffffll / (work + p.lead)) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads over up to %lld keys are too many for one call", b.N, heads, work * KT);
 		p.slots = n_lists || !b.n_groups ? 2 * p.grid : (int) (tiles * c.G) + p.grid;
 		p.o = (float*) take((size_t) p.slots * p.M * c.dv * 4);
@@ -758,7 +759,7 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 	Attn a;
 	size_t need = 0;
 	XALM_TRY(check_cache(cache, c));
-	XALM_TRY(check_batch(batch, b));
+	XALM_TRY(check_batch(batch, c, b));
 	if (heads <= 0 || heads > 65535) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
 	const int e = element_bytes(cache->type);
 	if (b.N) {
@@ -815,7 +816,7 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
                            void* stream) {
 	AppendArgs a = {};
 	XALM_TRY(check_cache(cache, a.c));
-	XALM_TRY(check_batch(batch, a.b));
+	XALM_TRY(check_batch(batch, a.c, a.b));
 	if (!is_type(in_type)) return set_error(XALM_ERR_UNSUPPORTED, "paged append: rows of type %d (F32, F16 and BF16)", in_type);
 	if (rot_half < 0 || 2 * rot_half > a.c.d || (rot_half && !freq)) return set_error(XALM_ERR_INVALID, "paged append: rotation of %d pairs in heads of %d", rot_half, a.c.d);
 	if (q && (heads <= 0 || heads > 65535)) return set_error(XALM_ERR_INVALID, "paged append: %d query heads", heads);
@@ -886,7 +887,7 @@ int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_ba
 	Attn a;
 	if (!bytes) return set_error(XALM_ERR_INVALID, "paged attention: bytes is NULL");
 	XALM_TRY(check_cache(cache, c));
-	XALM_TRY(check_batch(batch, b));
+	XALM_TRY(check_batch(batch, c, b));
 	return plan_attn(cache, c, b, heads, n_lists, a, bytes);
 }
 
@@ -905,7 +906,7 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
                            int* out, void* stream) {
 	SelectArgs a = {};
 	XALM_TRY(check_cache(cache, a.c));
-	XALM_TRY(check_batch(batch, a.b));
+	XALM_TRY(check_batch(batch, a.c, a.b));
 	if (!a.c.means) return set_error(XALM_ERR_STATE, "paged select: the cache keeps no mean keys");
 	if (heads <= 0 || heads % a.c.G || heads > 65535) return set_error(XALM_ERR_INVALID, "paged select: %d query heads over %d", heads, a.c.G);
 	if (top <= 0 || top > MAX_LIST || first < 0 || recent < 0 || first > top || recent > top || first + recent + 1 > top)

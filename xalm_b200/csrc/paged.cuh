@@ -503,8 +503,9 @@ inline cudaError_t launch(K kernel, dim3 grid, int block, size_t smem, cudaStrea
 	return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 int launch_join(const Attn& a, int type, cudaStream_t s);
-int launch_attn_rows(const Attn& a, cudaStream_t s); // fp32 caches
-// 16-bit caches: CTAs per SM that the kernel's shared memory leaves room for
+// CTAs per SM that a kernel's shared memory leaves room for, and its launch: fp32 caches, 16-bit caches
+int rows_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists);
+int launch_attn_rows(const Attn& a, cudaStream_t s);
 int mma_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists);
 int launch_attn_mma(const Attn& a, int part, int type, cudaStream_t s);
 constexpr int TC_ROWS = 256; // rows of a unit on tcgen05

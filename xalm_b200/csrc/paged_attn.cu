@@ -5,25 +5,31 @@ namespace xalm {
 namespace paged {
 
 // =========================================================================================================================================
-// Attention by fp32 FMAs: 16 (token, head) rows of one kv head at a time, 32 keys at a time in shared memory as fp32, one running maximum and
+// Attention by fp32 FMAs: 16 (token, head) rows of one kv head at a time, 32 keys at a time in shared memory, one running maximum and
 // sum per row.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s = scale q.k; kept in log2 units: exp2((q.k - m') scale log2 e).
+// A tile's keys and values are on their way (16 bytes a copy, four threads to a key) while the tile before is worked on.  Scores: a lane to a key, four rows to a warp.
+// Sums: four neighbouring columns to a thread, CG threads side by side, the rows divided among the 128 / CG groups.  Few rows are bound by the latency of a tile's steps, many by
+// what shared memory delivers: for 16 rows of 128 entries 1024 + 640 cycles a tile against 1024 of FMAs.
 // =========================================================================================================================================
-constexpr int RM = 16, RK = 32, RT = 128;
+constexpr int RM = 16, RK = 32, RT = 128, RS = 20; // RS: floats between a key's probabilities, so that a warp's stores of four rows meet no bank twice
 
-template <int NC, bool LIST> // NC columns of V per thread
-__global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ Attn a) {
+__device__ __forceinline__ void copy16(float* dst, const float* src, bool there) { // zeros where there is nothing
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+template <int CG, bool LIST> // threads that share a value's columns
+__global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ Attn a, const int buffers) {
+	constexpr int RPT = RM * CG / RT; // rows of a thread's sums
 	extern __shared__ __align__(16) uint8_t smem[];
-	using T = float;
 	const Part& part = a.part[0];
 	const int d = a.c.d, dv = a.c.dv, kp = d + 4, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	float* sq = reinterpret_cast<float*>(smem);  // [RM][d]
-	float* sk = sq + RM * d;                      // [RK][d + 4]
-	float* sv = sk + RK * kp;                     // [RK][dv]
-	float* sp = sv + RK * dv;                     // [RM][RK]
-	float* s_corr = sp + RM * RK;                 // [RM] factor of what a row has so far, then its sum
-	int* s_lim = reinterpret_cast<int*>(s_corr + 2 * RM); // [RM] keys that a row sees
-	int* s_page = s_lim + RM;                     // [RK]
-	int* s_list = s_page + RK;                    // [S]
+	const int tile = RK * (kp + dv);                      // floats of a tile
+	float* sq = reinterpret_cast<float*>(smem);           // [RM][d]
+	float* st = sq + RM * d;                              // [buffers] of [RK][d + 4] keys and [RK][dv] values
+	float* sp = st + buffers * tile;                      // [RK][RS]
+	float* s_corr = sp + RK * RS;                         // [RM] factor of what a row has so far, then of its sum
+	int* s_lim = reinterpret_cast<int*>(s_corr + RM);     // [RM] keys that a row sees
+	int* s_list = s_lim + RM;                             // [S]
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list + ((LIST ? a.S : 0) + 1) / 2 * 2);
 	Plan plan;
 	pdl_wait();
@@ -34,6 +40,8 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
 	if (tid == 0)
 		write_head(a, part, k, more, LIST ? more && row_in_seq(k.x.q, k.x.row0) : more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, LIST ? share_of(list_total(a, part), part.grid) : plan.share);
+	const int cg = tid % CG, col = cg * 4, r0 = tid / CG * RPT;      // this thread's columns and rows
+	const int key_of = tid >> 2, P = 1 << a.c.shift;                 // this thread's key of a tile, of which it brings every fourth 16 bytes
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue; // the same for every thread
@@ -44,135 +52,161 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 			pos = x.q.len - x.q.n + x.row0 - x.q.a;
 			bool own;
 			const int n = list_pages(a, x.row0, x.g, pos >= 0 ? pos >> a.c.shift : -1, warp == 0 ? s_list : nullptr, &own);
-			listed = own ? ((n - 1) << a.c.shift) + (pos & ((1 << a.c.shift) - 1)) + 1 : n << a.c.shift;
+			listed = own ? ((n - 1) << a.c.shift) + (pos & (P - 1)) + 1 : n << a.c.shift;
 		}
 		const int shared = LIST ? 0 : plan.shs[x.s];
 		const bool prefix = !LIST && x.seg < a.b.n_groups;
 		const int rows = min(RM, x.rows - x.t * RM);
 		const int h0 = x.g * a.rep;
-		for (int i = tid; i < RM * (d / 8); i += RT) {
-			const int r = i / (d / 8), c = i % (d / 8) * 8;
-			float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+		auto keys_of = [&](int r) { return LIST ? listed : prefix ? shared : own_keys(x.q, shared, a.rep, x.t * RM + r); };
+		if (tid < RM) s_lim[tid] = tid >= rows ? 0 : keys_of(tid);
+		if (LIST) __syncthreads();
+		const int first = x.j0 * KT, last = min(x.j1 * KT, keys_of(rows - 1)); // the last row sees the most
+		auto page_at = [&](int kb) { // page of this thread's key of the tile at kb
+			if (kb + key_of >= last) return -1;
+			const int key = x.key0 + kb + key_of, pg = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
+			if (pg < 0) report(a.c, ERR_PAGE);
+			return pg;
+		};
+		auto copy = [&](int kb, int pg, float* to) {
+			const long long slot = (x.key0 + kb + key_of) & (P - 1);
+			const float* kk = reinterpret_cast<const float*>(a.c.k) + (pg < 0 ? 0 : pg * a.c.k_page + slot * a.c.k_slot + x.g * a.c.k_head);
+			const float* vv = reinterpret_cast<const float*>(a.c.v) + (pg < 0 ? 0 : pg * a.c.v_page + slot * a.c.v_slot + x.g * a.c.v_head);
+#pragma unroll 4
+			for (int c = (tid & 3) * 4; c < d; c += 16) copy16(to + key_of * kp + c, kk + c, pg >= 0);
+#pragma unroll 4
+			for (int c = (tid & 3) * 4; c < dv; c += 16) copy16(to + RK * kp + key_of * dv + c, vv + c, pg >= 0);
+			asm volatile("cp.async.commit_group;" ::: "memory");
+		};
+		int page = page_at(first);
+		copy(first, page, st);
+		page = page_at(first + RK);
+		for (int i = tid; i < RM * (d / 4); i += RT) {
+			const int r = i / (d / 4), c = i % (d / 4) * 4;
+			float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 			if (r < rows) {
 				const int w = x.t * RM + r;
-				load8(reinterpret_cast<const T*>(a.q) + (long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * d + c, v);
+				v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + (long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * d + c);
 			}
-#pragma unroll
-			for (int e = 0; e < 8; e++) sq[r * d + c + e] = v[e];
+			*reinterpret_cast<float4*>(sq + r * d + c) = v;
 		}
-		if (tid < RM) s_lim[tid] = tid >= rows ? 0 : LIST ? listed : prefix ? shared : own_keys(x.q, shared, a.rep, x.t * RM + tid);
-		__syncthreads();
-		const int first = x.j0 * KT, last = min(x.j1 * KT, s_lim[rows - 1]); // the last row sees the most
-		float m[4], l[4], acc[RM][NC];
+		float m[4], l[4], acc[RPT][4];
 #pragma unroll
 		for (int r = 0; r < 4; r++) { m[r] = -INFINITY; l[r] = 0.f; }
 #pragma unroll
-		for (int r = 0; r < RM; r++)
+		for (int r = 0; r < RPT; r++)
 #pragma unroll
-			for (int c = 0; c < NC; c++) acc[r][c] = 0.f;
+			for (int c = 0; c < 4; c++) acc[r][c] = 0.f;
 		const float c1 = a.scale * 1.4426950408889634f;
+		const bool scores = warp * 4 < rows, sums = r0 < rows && col < dv;
+		float* now = st;
 		for (int kb = first; kb < last; kb += RK) {
-			const int n_keys = min(RK, last - kb);
-			if (tid < RK) {
-				const int key = x.key0 + kb + tid;
-				int pg = -1;
-				if (tid < n_keys) {
-					pg = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
-					if (pg < 0) report(a.c, ERR_PAGE);
+			asm volatile("cp.async.wait_group 0;" ::: "memory");
+			__syncthreads(); // the tile is there, and nobody reads the one before any more
+			float* next = buffers == 1 || now != st ? st : st + tile;
+			if (buffers > 1) copy(kb + RK, page, next);
+			const int after = buffers > 1 ? page_at(kb + 2 * RK) : -1;
+			if (scores) {
+				float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+				for (int c = 0; c < d; c += 4) {
+					const float4 kk = *reinterpret_cast<const float4*>(now + lane * kp + c);
+#pragma unroll
+					for (int r = 0; r < 4; r++) {
+						const float4 qq = *reinterpret_cast<const float4*>(sq + (warp * 4 + r) * d + c);
+						s[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[r]))));
+					}
 				}
-				s_page[tid] = pg;
-			}
-			__syncthreads();
-			for (int i = tid; i < RK * (d / 8); i += RT) {
-				const int r = i / (d / 8), c = i % (d / 8) * 8, pg = s_page[r];
-				float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-				if (pg >= 0)
-					load8(reinterpret_cast<const T*>(a.c.k) + pg * a.c.k_page + ((x.key0 + kb + r) & ((1 << a.c.shift) - 1)) * a.c.k_slot + x.g * a.c.k_head + c, v);
-				reinterpret_cast<float4*>(sk + r * kp + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
-				reinterpret_cast<float4*>(sk + r * kp + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
-			}
-			for (int i = tid; i < RK * (dv / 8); i += RT) {
-				const int r = i / (dv / 8), c = i % (dv / 8) * 8, pg = s_page[r];
-				float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-				if (pg >= 0)
-					load8(reinterpret_cast<const T*>(a.c.v) + pg * a.c.v_page + ((x.key0 + kb + r) & ((1 << a.c.shift) - 1)) * a.c.v_slot + x.g * a.c.v_head + c, v);
-				reinterpret_cast<float4*>(sv + r * dv + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
-				reinterpret_cast<float4*>(sv + r * dv + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
-			}
-			__syncthreads();
-			float s[4] = {0.f, 0.f, 0.f, 0.f};
-			for (int c = 0; c < d; c += 4) { // lane = key, four rows to a warp
-				const float4 kk = *reinterpret_cast<const float4*>(sk + lane * kp + c);
+				float p[4];
 #pragma unroll
 				for (int r = 0; r < 4; r++) {
-					const float4 qq = *reinterpret_cast<const float4*>(sq + (warp * 4 + r) * d + c);
-					s[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[r]))));
+					const float sc = kb + lane < s_lim[warp * 4 + r] ? s[r] * c1 : -INFINITY;
+					const float mt = fmaxf(m[r], warp_max(sc)), base = mt == -INFINITY ? 0.f : mt, corr = exp2f(m[r] - base);
+					p[r] = exp2f(sc - base);
+					l[r] = l[r] * corr + p[r]; // of this lane's keys
+					m[r] = mt;
+					if (lane == 0) s_corr[warp * 4 + r] = corr;
 				}
-			}
-#pragma unroll
-			for (int r = 0; r < 4; r++) {
-				const float sc = kb + lane < s_lim[warp * 4 + r] ? s[r] * c1 : -INFINITY;
-				const float mt = fmaxf(m[r], warp_max(sc)), base = mt == -INFINITY ? 0.f : mt;
-				const float p = exp2f(sc - base), corr = exp2f(m[r] - base);
-				l[r] = l[r] * corr + warp_sum(p);
-				m[r] = mt;
-				sp[(warp * 4 + r) * RK + lane] = p;
-				if (lane == 0) s_corr[warp * 4 + r] = corr;
+				*reinterpret_cast<float4*>(sp + lane * RS + warp * 4) = make_float4(p[0], p[1], p[2], p[3]);
 			}
 			__syncthreads();
-			const bool all = kb + n_keys <= s_lim[0]; // every row sees every key of this tile (rows that are not there see none, and are not written)
+			if (sums) {
+				const int n_keys = min(RK, last - kb);
+				const float* vv = now + RK * kp + col;
 #pragma unroll
-			for (int c = 0; c < NC; c++) {
-				const int col = tid + c * RT;
-				if (col >= dv) break;
+				for (int r = 0; r < RPT; r++) {
+					const float f = s_corr[r0 + r];
 #pragma unroll
-				for (int r = 0; r < RM; r++) acc[r][c] *= s_corr[r];
-				if (all) {
-					for (int j = 0; j < n_keys; j++) {
-						const float v = sv[j * dv + col];
+					for (int c = 0; c < 4; c++) acc[r][c] *= f;
+				}
+				// rows that are not there see no key, and are not written
+				if (kb + n_keys <= s_lim[0]) {
+#pragma unroll 4
+					for (int j = 0; j < RK; j++) { // values behind the last key are zeros, and so are their probabilities
+						const float4 v = *reinterpret_cast<const float4*>(vv + j * dv);
 #pragma unroll
-						for (int r = 0; r < RM; r++) acc[r][c] = fmaf(sp[r * RK + j], v, acc[r][c]);
+						for (int r = 0; r < RPT; r++) {
+							const float p = sp[j * RS + r0 + r];
+							acc[r][0] = fmaf(p, v.x, acc[r][0]);
+							acc[r][1] = fmaf(p, v.y, acc[r][1]);
+							acc[r][2] = fmaf(p, v.z, acc[r][2]);
+							acc[r][3] = fmaf(p, v.w, acc[r][3]);
+						}
 					}
 				} else { // what a row does not see may be anything, an infinity or a NaN too
 					for (int j = 0; j < n_keys; j++) {
-						const float v = sv[j * dv + col];
+						const float4 v = *reinterpret_cast<const float4*>(vv + j * dv);
 #pragma unroll
-						for (int r = 0; r < RM; r++)
-							if (kb + j < s_lim[r]) acc[r][c] = fmaf(sp[r * RK + j], v, acc[r][c]);
+						for (int r = 0; r < RPT; r++)
+							if (kb + j < s_lim[r0 + r]) {
+								const float p = sp[j * RS + r0 + r];
+								acc[r][0] = fmaf(p, v.x, acc[r][0]);
+								acc[r][1] = fmaf(p, v.y, acc[r][1]);
+								acc[r][2] = fmaf(p, v.z, acc[r][2]);
+								acc[r][3] = fmaf(p, v.w, acc[r][3]);
+							}
 					}
 				}
 			}
-			__syncthreads();
+			if (buffers == 1) {
+				__syncthreads();
+				copy(kb + RK, page_at(kb + RK), next);
+			}
+			page = after;
+			now = next;
 		}
+		asm volatile("cp.async.wait_group 0;" ::: "memory");
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
 		const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
+		__syncthreads(); // the factors have been read
+		if (scores)
 #pragma unroll
-		for (int r = 0; r < 4; r++)
-			if (lane == 0) {
+			for (int r = 0; r < 4; r++) {
 				const int row = warp * 4 + r;
-				s_corr[row] = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
-				if (row < rows) {
-					if (!direct) {
-						if (slot < part.slots) part.ml[slot * RM + row] = make_float2(m[r], l[r]);
-					} else if (a.lse) {
-						const int w = x.t * RM + row;
-						a.lse[(long long) (x.row0 + w / a.rep) * a.H + h0 + w % a.rep] = l[r] > 0.f || l[r] != l[r] ? (m[r] + log2f(l[r])) * 0.6931471805599453f : -INFINITY;
+				const float sum = warp_sum(l[r]);
+				const bool any = sum > 0.f || sum != sum;
+				if (lane == 0) {
+					s_corr[row] = direct ? (any ? 1.f / sum : 0.f) : 1.f;
+					if (row < rows) {
+						if (!direct) {
+							if (slot < part.slots) part.ml[slot * RM + row] = make_float2(m[r], sum);
+						} else if (a.lse) {
+							const int w = x.t * RM + row;
+							a.lse[(long long) (x.row0 + w / a.rep) * a.H + h0 + w % a.rep] = any ? (m[r] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+						}
 					}
 				}
 			}
 		__syncthreads();
+		if (sums) {
 #pragma unroll
-		for (int c = 0; c < NC; c++) {
-			const int col = tid + c * RT;
-			if (col >= dv) break;
-#pragma unroll
-			for (int r = 0; r < RM; r++)
-				if (r < rows) {
-					if (direct) {
-						const int w = x.t * RM + r;
-						reinterpret_cast<T*>(a.out)[(long long) (x.row0 + w / a.rep) * a.out_row + (h0 + w % a.rep) * dv + col] = from_f<T>(s_corr[r] == 0.f ? 0.f : acc[r][c] * s_corr[r]);
-					} else if (slot < part.slots) part.o[(slot * RM + r) * dv + col] = acc[r][c];
-				}
+			for (int r = 0; r < RPT; r++) {
+				const int row = r0 + r, w = x.t * RM + row;
+				if (row >= rows) break;
+				const float f = s_corr[row]; // 0: a row that sees nothing, whose sums are zeros
+				float* to = direct ? reinterpret_cast<float*>(a.out) + (long long) (x.row0 + w / a.rep) * a.out_row + (h0 + w % a.rep) * dv + col : part.o + (slot * RM + row) * dv + col;
+				if (direct || slot < part.slots) *reinterpret_cast<float4*>(to) = make_float4(acc[r][0] * f, acc[r][1] * f, acc[r][2] * f, acc[r][3] * f);
+			}
 		}
 	}
 }
@@ -364,18 +398,22 @@ int launch_join(const Attn& a, int type, cudaStream_t s) {
 	return XALM_OK;
 }
 
-template <int NC, bool LIST>
+static size_t rows_smem(const Cache& c, const BatchView& b, int n_lists, int buffers) {
+	return (size_t) (RM * c.d + buffers * RK * (c.d + 4 + c.dv) + RK * RS + RM) * 4 + (RM + n_lists + 2) * 4 + 16 + (n_lists ? 0 : plan_bytes(b.B, b.n_groups));
+}
+// Two buffers where shared memory holds them, which it does not for the largest heads beside thousands of sequences; two CTAs to an SM where it holds those
+static int rows_buffers(const Cache& c, const BatchView& b, int n_lists) { return rows_smem(c, b, n_lists, 2) <= 226 * 1024 ? 2 : 1; }
+int rows_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists) { return rows_smem(c, b, n_lists, rows_buffers(c, b, n_lists)) <= 113 * 1024 ? 2 : 1; }
+template <int CG>
 static int rows_cols(const Attn& a, cudaStream_t s) {
-	const size_t smem = (size_t) (RM * a.c.d + RK * (a.c.d + 4) + RK * a.c.dv + RM * RK + 2 * RM) * 4 + (RM + RK + (LIST ? a.S : 0) + 2) * 4 + 16 +
-	                    (LIST ? 0 : plan_bytes(a.b.B, a.b.n_groups));
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_rows_kernel<NC, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-	XALM_CUDA_CHECK(launch(paged_rows_kernel<NC, LIST>, a.part[0].grid, RT, smem, s, false, a));
+	const int buffers = rows_buffers(a.c, a.b, a.S);
+	const size_t smem = rows_smem(a.c, a.b, a.S, buffers);
+	auto kernel = a.lists ? paged_rows_kernel<CG, true> : paged_rows_kernel<CG, false>;
+	XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	XALM_CUDA_CHECK(launch(kernel, a.part[0].grid, RT, smem, s, false, a, buffers));
 	return XALM_OK;
 }
-int launch_attn_rows(const Attn& a, cudaStream_t s) {
-	if (a.lists) return a.c.dv > RT ? rows_cols<2, true>(a, s) : rows_cols<1, true>(a, s);
-	return a.c.dv > RT ? rows_cols<2, false>(a, s) : rows_cols<1, false>(a, s);
-}
+int launch_attn_rows(const Attn& a, cudaStream_t s) { return a.c.dv <= 64 ? rows_cols<16>(a, s) : a.c.dv <= 128 ? rows_cols<32>(a, s) : rows_cols<64>(a, s); }
 
 } // namespace paged
 } // namespace xalm
