@@ -66,8 +66,8 @@ class Problem:
                 used[self.slots(s, torch.arange(n))] = True
         self.k[~used], self.v[~used] = fill, fill
 
-    def attend(self, lists=None, round_p=True):
-        """(out, lse, tolerance of out, tolerance of lse) in 64 bits; rows outside every sequence are NaN in `out`.
+    def attend(self, lists=None, round_p=True, only=None):
+        """(out, lse, tolerance of out, tolerance of lse) in 64 bits; rows outside every sequence, and those not in `only`, are NaN in `out`.
 
         Tolerances: scores are sums of d products in fp32, each off by at most 2^-24 of the sum of absolute products per addition, so a score is off by
         ds <= (d + 2) 2^-24 scale sum |q k|, and a probability by the factor 1 + 2 ds (its own score's and the denominator's).  The sums over n keys in fp32 add n 2^-24, exp2 and the scaling of its
@@ -76,7 +76,7 @@ class Problem:
         out = torch.full((self.rows, self.H, self.dv), math.nan, dtype=torch.float64)
         lse, tol_o, tol_l = out[..., 0].clone(), torch.zeros_like(out), torch.zeros(self.rows, self.H, dtype=torch.float64)
         half = HALF[self.type]
-        for n in range(self.rows):
+        for n in range(self.rows) if only is None else only:
             w = self.row(n)
             if w is None:
                 continue
@@ -95,7 +95,7 @@ class Problem:
                 sc = q @ k.T * self.scale
                 pr = sc.softmax(dim=1)
                 out[n, hs], lse[n, hs] = pr @ v, sc.logsumexp(dim=1)
-                ds = (self.d + 2) * F32 * (q.abs() @ k.abs().T * self.scale).max(dim=1).values
+                ds = (self.d + 2) * F32 * (q.abs() @ k.abs().T * abs(self.scale)).max(dim=1).values
                 rel = 2 * ds + 2 * len(at) * F32 + 8 * (1 + sc.abs().max(dim=1).values * 1.4427) * F32
                 spread = pr @ v.abs()
                 tol_o[n, hs] = spread * (rel + (half if round_p and self.type != "f32" else 0))[:, None] + out[n, hs].abs() * half

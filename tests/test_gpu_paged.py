@@ -78,6 +78,64 @@ def test_attend_of_any_heads(G, rep, type):
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3, 3.0])
+def test_attend_of_any_scale(scale, type):
+    """Scores' signs turned, all equal, nearly equal, and so far apart that one key has nearly everything."""
+    for groups in (None, ([0, 3], [192])):
+        p = Problem(type, [1, 9, 40], [193, 260, 300], d=64, page=64, seed=46, groups=groups)
+        p.scale = scale
+        check_attend(p)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("G,rep,d,dv,page", [(8, 4, 64, 64, 16), (8, 4, 128, 128, 64), (6, 5, 80, 72, 32), (16, 1, 128, 64, 256), (4, 16, 128, 128, 128), (2, 3, 192, 256, 64)])
+def test_long_prompts(G, rep, d, dv, page, type):
+    """Prompts of many units, whose pieces a block meets several of, with and without pages in common; some rows of every sequence are looked at."""
+    new, lens = [700, 1, 37, 300, 1, 513], [1900, 1500, 1061, 1324, 1025, 1537]
+    for groups in (None, ([0, 2, 6], [1024, 1024])):
+        p = Problem(type, new, lens, G=G, rep=rep, d=d, dv=dv, page=page, seed=47, groups=groups, pad_rows=5)
+        some = sorted({min(p.starts[s] + x, p.starts[s + 1] - 1) for s in range(len(new)) for x in (0, 1, 31, 32, 63, 64, 127, 128, 255, 256, 400, new[s] - 1)})
+        cache, batch = p.on_gpu()
+        out, lse = paged.attend(cache, batch, p.gq, p.scale, want_lse=True)
+        cache.check()
+        want, want_lse, tol, tol_lse = p.attend(only=some)
+        near(out[some], want[some], tol[some], "out")
+        near(lse[some], want_lse[some], tol_lse[some], "lse")
+
+
+def test_thousands_of_sequences_with_the_largest_heads():
+    """So many that shared memory has room for one tile of keys and values beside them only."""
+    check_attend(Problem("f32", [1] * 4000, [i % 19 + 1 for i in range(4000)], G=1, rep=1, d=256, page=16, seed=48))
+
+
+def test_calls_in_two_threads_do_not_meet():
+    """One cache and one batch, calls of different numbers of rows at the same time."""
+    import threading
+    p = Problem("bf16", [3, 5], [300, 400], G=2, d=64, page=64, seed=49, pad_rows=4)
+    cache, batch = p.on_gpu()
+    want = {n: paged.attend(cache, batch, p.gq[:n], p.scale) for n in (8, 12)}
+    wrong = []
+
+    def serve(n):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(200):
+                out = paged.attend(cache, batch, p.gq[:n], p.scale)
+                stream.synchronize()
+                if not torch.equal(out[:8], want[n][:8]):
+                    wrong.append(n)
+
+    threads = [threading.Thread(target=serve, args=(n,)) for n in (8, 12)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    cache.check()
+    assert not wrong
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 def test_groups_change_nothing_but_the_order_of_sums(type):
     """More shared tokens than the sequences have, parts of pages, overlong groups, groups of one: the annotation is cut to what holds."""
     for groups in (([0, 4], [10 ** 9]), ([0, 4], [70]), ([0, 1, 4], [64, 64]), ([0, 4], [0]), ([0, 4], [-5]), ([1, 3], [128])):

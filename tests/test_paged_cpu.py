@@ -71,6 +71,11 @@ def test_select_needs_mean_keys_and_room_for_the_scores():
     assert calls(cache(), batch(max_pages=24577, table_row=24577))["select"]() == 1
 
 
+def test_tables_of_more_tokens_than_positions_are_refused():
+    for op in calls(cache(page_size=16), batch(max_pages=(1 << 26) + 1, table_row=1 << 27)).values():
+        assert op() == 1
+
+
 def test_nothing_to_do_is_no_error_and_launches_nothing():
     for b in (batch(rows=0), batch(seqs=0, starts=0, lens=0, table=0, max_pages=0)):
         for name, call in calls(cache(), b).items():
