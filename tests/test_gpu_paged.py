@@ -103,6 +103,14 @@ def test_long_prompts(G, rep, d, dv, page, type):
         near(lse[some], want_lse[some], tol_lse[some], "lse")
 
 
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("G,rep", [(1, 1), (2, 4), (8, 2), (3, 5)])
+def test_groups_of_several_tokens_to_a_sequence(G, rep, type):
+    """Many rows that each have shared pages and pages of their own, groups of one sequence and sequences without new tokens among them."""
+    new, lens = [16, 20, 0, 9, 31, 1, 3, 17, 2, 25], [290, 276, 256, 300, 287, 70, 67, 150, 66, 600]
+    check_attend(Problem(type, new, lens, G=G, rep=rep, d=64, page=64, seed=50, groups=([0, 5, 6, 9], [256, 64, 64]), pad_rows=2, offset=1))
+
+
 def test_thousands_of_sequences_with_the_largest_heads():
     """So many that shared memory has room for one tile of keys and values beside them only."""
     check_attend(Problem("f32", [1] * 4000, [i % 19 + 1 for i in range(4000)], G=1, rep=1, d=256, page=16, seed=48))

@@ -703,8 +703,16 @@ static int sm_count(int device, int* n) {
 	return XALM_OK;
 }
 
+// Segments of up to 16 (token, head) rows fill one tile of mma.sync, more go to tcgen05's tiles of 256: with 32 rows for either, 8 prompts of 8 tokens behind 4000 take 66 us in place of 54,
+// and four groups of 8 sequences behind 8192 shared tokens 70 in place of 57 (8 kv heads, 32 rows to each)
 constexpr int SMALL_ROWS = 16;
-constexpr int LEAD = 6, LEAD_TC = 12;
+// A call of no more rows than this to a kv head has no launch of tcgen05: one group behind 8192 tokens takes 25 us in place of 35 with 24 rows, 33 in place of 38 with 64, but 44 in place of
+// 39 with 128
+constexpr int FEW_ROWS = 64;
+// What a piece costs beside its tiles, in tiles, when the work is divided.  mma.sync: 64 sequences behind 8192 shared tokens 97 us, with 2 109.  tcgen05: five prompts of 150 to 700 tokens
+// behind 2048 shared ones 147 us, with 2 176.  fp32: two prompts of 25 tokens 93 us, with 6 107.
+constexpr int LEAD = 6, LEAD_TC = 12, LEAD_F32 = 2;
+constexpr int JOIN_ROWS = 4, JOIN_BLOCKS = 8; // rows to a block of the join, and most blocks to an SM: 128 sequences of 32 heads in two groups 205 us, with 2 223; five long prompts 152, with 16 153
 
 // ---- attention: parts, workspace --------------------------------------------------------------------------------------------------------------
 static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchView& b, int heads, int n_lists, Attn& a, size_t* bytes) {
@@ -720,7 +728,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 	a.S = n_lists;
 	// Two kernels divide the segments by their rows: up to 16 fill one 16-row tile, more go to tcgen05.  The second is launched only where some segment may have more.
 	const bool f32 = cache->type == XALM_F32;
-	const bool tc = !f32 && !n_lists && tc_fits(c, b) && (b.n_groups || b.N > b.B) && (long long) b.N * a.rep > SMALL_ROWS;
+	const bool tc = !f32 && !n_lists && tc_fits(c, b) && (b.n_groups || b.N > b.B) && (long long) b.N * a.rep > FEW_ROWS;
 	a.n_parts = tc ? 2 : 1;
 	size_t at = 0;
 	auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
@@ -729,7 +737,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		const bool big = tc && i == 0;
 		p.M = big ? TC_ROWS : 16;
 		p.grid = sms * (big ? 1 : f32 ? rows_ctas_per_sm(c, b, n_lists) : mma_ctas_per_sm(c, b, n_lists));
-		p.lead = big ? LEAD_TC : LEAD;
+		p.lead = big ? LEAD_TC : f32 ? LEAD_F32 : LEAD;
 		p.least_rows = big ? SMALL_ROWS + 1 : 1;
 		p.most_rows = tc && !big ? SMALL_ROWS : 0x7fffffff;
 		const long long rows = (long long) b.N * a.rep;
@@ -748,6 +756,7 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 			p.shs = (int*) take((size_t) b.B * 4);
 		}
 	}
+	a.row_blocks = n_lists || !b.n_groups ? 0 : (int) std::min(((long long) b.N * heads + JOIN_ROWS - 1) / JOIN_ROWS, (long long) sms * JOIN_BLOCKS);
 	*bytes = at;
 	return XALM_OK;
 }

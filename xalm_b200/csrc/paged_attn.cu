@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 
 // =========================================================================================================================================
 // The join of what several CTAs have of the same rows, a warp to a row.  A lane takes a piece's maximum and sum, then the pieces' rows are added with their weights, eight
-// loads on their way at a time.  Two kinds of blocks: with groups, for a kv head of a sequence whose rows read shared pages; and for 16 rows
+// loads on their way at a time.  Two kinds of blocks: with groups, for rows that read shared pages; and for 16 rows
 // of the units that a CTA's share begins inside.  Bound by the latency of three or four loads that depend on one another.
 // =========================================================================================================================================
 constexpr int JT = 128, JR = 16;
@@ -336,32 +336,42 @@ __host__ __device__ __forceinline__ int boundary_blocks(const Part& p) { return 
 
 template <typename T, int NC>
 __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ Attn a) {
-	const int warp = threadIdx.x >> 5, n_seq = a.b.n_groups && !a.lists ? a.b.B * a.c.G : 0;
+	const int warp = threadIdx.x >> 5;
 	int id = blockIdx.x;
-	if (id < n_seq) {
-		const int s = id / a.c.G, g = id - s * a.c.G; // a sequence's rows of one kv head
+	if (id < a.row_blocks) { // a warp to a (token, head) row
 		const View v = view_of(a.c, a.b);
-		const Seq q = seq_of(v, s); // the caller's arrays are there already, the other kernels' are not
-		int lo = 0, hi = a.b.n_groups - 1; // its group
-		while (lo < hi) {
-			const int mid = (lo + hi + 1) >> 1;
-			if (a.b.bounds[mid] <= s) lo = mid;
-			else hi = mid - 1;
-		}
-		const int first = min(group_of(v, lo).x, a.b.B - 1), row0 = seq_of(v, first).a;
-		pdl_wait();
-		if (!a.part[0].shs[s]) return;
-		for (int r = warp; r < q.n * a.rep; r += JT / 32) {
+		const long long rows = (long long) a.b.N * a.H;
+		bool waited = false;
+		for (long long r = id * (JT / 32) + warp; r < rows; r += a.row_blocks * (JT / 32)) {
+			const int tok = (int) (r / a.H), h = (int) (r - (long long) tok * a.H), g = h / a.rep;
+			int s = 0, lo = 0; // its sequence and that one's group: the last that begin there or before
+			for (int hi = a.b.B - 1; s < hi;) {
+				const int mid = (s + hi + 1) >> 1;
+				if (v.starts[mid] <= tok) s = mid;
+				else hi = mid - 1;
+			}
+			for (int hi = a.b.n_groups - 1; lo < hi;) {
+				const int mid = (lo + hi + 1) >> 1;
+				if (v.bounds[mid] <= s) lo = mid;
+				else hi = mid - 1;
+			}
+			const Seq q = seq_of(v, s);
+			const int first = min(group_of(v, lo).x, a.b.B - 1), row0 = seq_of(v, first).a;
+			if (!waited) pdl_wait(); // the caller's arrays were there already, the other kernels' are not
+			waited = true;
+			const int sh = a.part[0].shs[s], of_groups = a.part[0].cum_w[a.b.n_groups] | (a.n_parts > 1 ? a.part[1].cum_w[a.b.n_groups] : 0);
+			if (!of_groups) return; // no group's pages are read once for all
+			if (!row_in_seq(q, tok) || !sh) continue;
 			JoinUnit u[2];
 			int found = 0;
-			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit(a, v, i, lo, first, (q.a - row0) * a.rep + r, g, u[0]);
+			for (int i = 0; i < a.n_parts && !found; i++) found = join_unit(a, v, i, lo, first, (tok - row0) * a.rep + h - g * a.rep, g, u[0]);
 			const int had = found;
-			for (int i = 0; i < a.n_parts && found == had; i++) found += join_unit(a, v, i, a.b.n_groups + s, s, r, g, had ? u[1] : u[0]);
-			join_row<T, NC>(a, u, found, q.a + r / a.rep, g * a.rep + r % a.rep);
+			for (int i = 0; i < a.n_parts && found == had; i++) found += join_unit(a, v, i, a.b.n_groups + s, s, (tok - q.a) * a.rep + h - g * a.rep, g, had ? u[1] : u[0]);
+			join_row<T, NC>(a, u, found, tok, h);
 		}
 		return;
 	}
-	id -= n_seq;
+	id -= a.row_blocks;
 	pdl_wait();
 	for (int i = 0; i < a.n_parts; i++) {
 		const Part& p = a.part[i];
@@ -388,9 +398,8 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ 
 }
 
 int launch_join(const Attn& a, int type, cudaStream_t s) {
-	int grid = 0;
+	int grid = a.row_blocks;
 	for (int i = 0; i < a.n_parts; i++) grid += boundary_blocks(a.part[i]);
-	if (a.b.n_groups && !a.lists) grid += a.b.B * a.c.G;
 	const bool wide = a.c.dv > 128;
 	XALM_CUDA_CHECK(type == XALM_F32   ? (wide ? launch(paged_join_kernel<float, 2>, grid, JT, 0, s, true, a) : launch(paged_join_kernel<float, 1>, grid, JT, 0, s, true, a))
 	                : type == XALM_F16 ? (wide ? launch(paged_join_kernel<__half, 2>, grid, JT, 0, s, true, a) : launch(paged_join_kernel<__half, 1>, grid, JT, 0, s, true, a))
