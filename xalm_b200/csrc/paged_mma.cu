@@ -13,7 +13,8 @@ namespace paged {
 // by TMA (a page's slots, 64 entries wide, swizzled) into a ring; four warps take 16 keys of a tile each, with maximum, sum and output of their own, so that
 // none waits for another and a stage is free again after a quarter of a tile's work: scores and sums by mma.sync m16n8k16 with the 16 rows as A, queries and sums in registers.
 // At the end of a piece the four join through shared memory.  (tcgen05 would want 64 rows or more: a step of four heads to a kv head has four.)
-// Probabilities enter the second product in the cache's type, a rounding of 2^-9 (bf16) or 2^-12 (fp16) of each, of either sign; scores, maxima and sums stay in fp32.
+// Probabilities enter the second product in two parts of the cache's type, rounded and what that left (one alone had 1.5 times the result's own rounding as its error): of up to eight rows
+// the second part are rows 8 to 15 of the same product, of more it costs a product of its own.  Scores, maxima and sums are fp32.
 // =========================================================================================================================================
 constexpr int MM = 16, CW = 4, MT = (CW + 1) * 32;
 
@@ -73,6 +74,14 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 		const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
 		return *reinterpret_cast<const uint32_t*>(&h);
 	}
+}
+// what is left of two numbers beside their rounded ones
+template <typename T>
+__device__ __forceinline__ uint32_t left16(uint32_t rounded, float lo, float hi) {
+	if constexpr (std::is_same<T, __half>::value) {
+		const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
+		return pack16<T>(lo - r.x, hi - r.y);
+	} else return pack16<T>(lo - __uint_as_float(rounded << 16), hi - __uint_as_float(rounded & 0xffff0000u));
 }
 __device__ __forceinline__ float ex2(float x) {
 	float y;
@@ -265,7 +274,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				l0 *= f0;
 				l1 *= f1;
 #pragma unroll
-				for (int i = 0; i < D / 8; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= f1; o[i][3] *= f1; }
+				for (int i = 0; i < D / 8; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= high ? f1 : f0; o[i][3] *= high ? f1 : f0; }
 				m0 = n0;
 				m1 = n1;
 				b0 = m0 == -INFINITY ? 0.f : -m0 * c1;
@@ -273,21 +282,31 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			}
 			// asked for here, known when this tile is done
 			there = j + 1 < j1 && try_wait_once(&full[st + 1 == stages ? 0 : st + 1], round ^ (st + 1 == stages));
-			uint32_t pa[4];
+			uint32_t pa[4], rest[4]; // probabilities, and what their rounding left
 #pragma unroll
 			for (int i = 0; i < 2; i++) {
 				const float x0 = ex2(fmaf(s[i][0], c1, b0)), x1 = ex2(fmaf(s[i][1], c1, b0));
 				l0 += x0 + x1;
 				pa[2 * i] = pack16<T>(x0, x1);
-				pa[2 * i + 1] = 0;
+				rest[2 * i] = left16<T>(pa[2 * i], x0, x1);
+				pa[2 * i + 1] = rest[2 * i];
 			}
-			if (high)
+			if (high) {
 #pragma unroll
 				for (int i = 0; i < 2; i++) {
 					const float x2 = ex2(fmaf(s[i][2], c1, b1)), x3 = ex2(fmaf(s[i][3], c1, b1));
 					l1 += x2 + x3;
 					pa[2 * i + 1] = pack16<T>(x2, x3);
+					rest[2 * i + 1] = left16<T>(pa[2 * i + 1], x2, x3);
 				}
+#pragma unroll
+				for (int c = 0; c < D / 16; c++) {
+					uint32_t b[4];
+					ldsm4_t(b, ((tile + v_lane) ^ ((c * 2 & 7) << 4)) + (c >> 2) * KT * 128);
+					mma16<T>(o[2 * c], rest, b[0], b[1]);
+					mma16<T>(o[2 * c + 1], rest, b[2], b[3]);
+				}
+			}
 #pragma unroll
 			for (int c = 0; c < D / 16; c++)
 			{
@@ -300,6 +319,9 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			__syncwarp();
 			if (lane == 0) mbar_arrive(&empty[st]);
 		}
+		if (!high)
+#pragma unroll
+			for (int i = 0; i < D / 8; i++) { o[i][0] += o[i][2]; o[i][1] += o[i][3]; }
 		m0 *= c1; // in units of log2 from here on
 		m1 *= c1;
 		// ---- the four warps' sums ----
