@@ -290,23 +290,27 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  *   128 or 256 slots; dim, vdim multiples of 8, at most 256.  Strides in ELEMENTS, entries of a head are neighbours: slots within heads or heads within slots, each stride a multiple
  *   of 16 bytes; pools at 16-byte boundaries.  means (pages, kv_heads, dim), dense, or NULL: the mean of a page's keys, kept for every page whose last
  *   slot was appended.  status: one int or NULL; kernels set bit 0 where a table named a page outside the pool (such a page reads as zeros and is not written) and bit 1
- *   where starts, lens and the table do not fit one another (lengths are cut to the table); nothing else reports what is only known on the device.
+ *   where starts, lens and the table do not fit one another (lengths are cut to the table; where starts or groups do not ascend, paged_attend computes nothing), bit 2 where a
+ *   kernel gave up a wait that should have taken microseconds (the call's results are not to be used); nothing else reports what is only known on the device.
  * xalm_paged_batch: rows starts[s] .. starts[s + 1] - 1 are the new tokens of sequence s, lens[s] its tokens, the new ones included: row starts[s] + i is at position
  *   lens[s] - n + i.  starts has seqs + 1 entries; rows outside [starts[0], starts[seqs]) of `rows` are left alone.  table (seqs, max_pages), rows table_row apart.
  *   Sequences group_bounds[i] .. group_bounds[i + 1] - 1 (ascending) have the same pages for their first group_shared[i] tokens: those are read once for all of
- *   them; what a call computes does not depend on it.  At most 4096 sequences and groups.
+ *   them; what a call computes does not depend on it but for the order of its sums.  At most 4096 sequences and groups, tables of at most 2^30 tokens.
  * Rows of arrays are `*_row` elements apart and begin at 16-byte boundaries; heads within a row are dense.
  *
  * paged_append: k (rows, kv_heads dim), v (rows, kv_heads vdim), q (rows, heads dim) of in_type; the first 2 rot_half entries of every head of k and q are turned by
  *   position * freq[i] (entry i with i + rot_half, or with `neighbours` 2 i with 2 i + 1; cos and sin times rot_mag); keys and values go to their pages, queries to q_out
  *   in the cache's type, rounded once.  q NULL: keys and values only.  Then the mean keys of the pages that are full now.
+ *   Two rows that a table sends to the same slot leave either's key and value there.
  * paged_attend: out[row, h] = sum_j softmax_j(scale q . k_j) v_j over the positions j up to the row's own; rows that see nothing give zeros.  lse (rows, heads): the logarithm of the
  *   softmax's denominator (-infinity where a row sees nothing), or NULL.
  * paged_select: for every row and kv head `top` pages by their place in the sequence, ascending, -1 behind them: the row's own page, the `recent` before it, the `first`
  *   of the sequence, and of the others those with the largest score = (sum of the kv head's queries) . mean key, equal scores from the lowest place on; NaN and -infinity count as the lowest
- *   finite number, +infinity as the largest.  out (rows, kv_heads, top).
+ *   finite number, +infinity as the largest.  out (rows, kv_heads, top).  first + recent + 1 <= top <= 1024, max_pages <= 24576.
  * paged_attend_selected: paged_attend over the listed pages only (rows, kv_heads, n_lists <= 1024), in any order; entries outside 0 .. the row's own page are passed
  *   over, a page counts once.
+ * Both attend in one pass: scores, maxima and sums in fp32; 16-bit caches' probabilities enter the second product as two numbers of the cache's type where a segment has up to 16
+ *   (token, head) rows to a kv head, as one of them where it has more.  The same call gives the same bits every time.
  * paged_workspace: bytes of workspace (at a 256-byte boundary) that paged_attend (n_lists 0) and paged_attend_selected need for these sizes; its contents need no preparation. */
 typedef struct xalm_paged_cache {
 	int type, device;
