@@ -429,6 +429,22 @@ def test_select_of_steps_and_prompts(pages, new):
         assert torch.equal(got[inside], want[inside])
 
 
+@pytest.mark.parametrize("new", [[3, 1, 190], [160, 0, 33]])
+@pytest.mark.parametrize("pages", [60, 512, 520])
+def test_select_of_more_rows_than_multiprocessors(pages, new):
+    """Blocks of 16 and of 8 rows."""
+    p = with_means(Problem("bf16", new, [new[0] + 5, 900, 700], d=64, page=16, G=2, seed=51, pad_rows=1))
+    width = p.table.shape[1]
+    p.table = torch.cat([p.table.clamp_min(0)] * (pages // width + 1), dim=1)[:, :pages].contiguous()
+    p.max_pages, p.lens = pages, [min(n, pages * 16) for n in (new[0] + 5, pages * 16, pages * 16 - 9)]
+    for a in (p.means, -p.means):
+        p.means = a
+        cache, batch = p.on_gpu()
+        got, want = paged.select(cache, batch, p.gq, 7).cpu(), p.select(p.means, 7, 1, 1)
+        inside = torch.tensor([p.row(n) is not None for n in range(p.rows)])
+        assert torch.equal(got[inside], want[inside])
+
+
 def test_select_of_a_long_sequence():
     """20000 pages, most of them the same few of the pool."""
     p = with_means(Problem("bf16", [1, 2], [900, 900], d=128, page=16, G=2, seed=25))

@@ -16,7 +16,8 @@ namespace paged {
 // =========================================================================================================================================
 // append: a row's position is p = len - n + i, its page table[p / P], its slot p % P.  Bound by HBM (every element in and out once), so a thread takes 16 or 32 bytes of a head
 // with those half a rotation away that they are turned with, of R rows at once: R = 4 keeps enough bytes on their way in prompts; steps of few tokens
-// have a CTA to a row.  The angle p * freq is taken in 64 bits and brought into [-pi, pi] there: in 32 bits position 100000 is 0.004 rad off.
+// have a CTA to a row.  9 prompts of 300 to 1500 tokens (209 MB) take 47 us, 4.4 TB/s; 16 rows of 32 and 8 heads 3.7, a launch and two dependent loads.  The angle
+// p * freq is taken in 64 bits and brought into [-pi, pi] there: in 32 bits position 100000 is 0.004 rad off.
 // =========================================================================================================================================
 struct AppendArgs {
 	Cache c;
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(128) paged_means_kernel(const Cache c, const B
 // =========================================================================================================================================
 // select: score_j = (sum over the kv head's queries) . mean_j, and of the pages between the first and the recent ones those with the largest scores, equal ones from the lowest
 // place on.  Which page is the last to be taken must not hang on how a sum was rounded, and sums in 64 bits cost a conversion per mean and row (279 us for 1341
-// tokens of 8 heads over 110 to 235 pages).  So scores are taken in fp32, each off by at most E = (d + rep + 4) 2^-24 sum_i (sum_r |q_ri|) max |mean|; of the want-th largest, t, the true
+// tokens of 8 heads over 110 to 235 pages, which take 56 now).  So scores are taken in fp32, each off by at most E = (d + rep + 4) 2^-24 sum_i (sum_r |q_ri|) max |mean|; of the want-th largest, t, the true
 // one is off by no more than E, so pages above t + 2 E are taken, those below t - 2 E are not, and only where those between are more than are wanted are they summed in 64 bits.
 // Steps of single tokens: a CTA to (row, kv head), 8 lanes to a page.  Longer ones: R rows of a sequence to a CTA, so that a page's mean is read and converted once for
 // all of them: 64 pages at a time in shared memory, a thread taking one page and R / 4 rows; then a warp to a row.  The want-th largest is found bit by bit from above, up to 512 keys in a warp's registers.
@@ -616,9 +617,11 @@ __global__ void __launch_bounds__(ST) paged_select_rows_kernel(const __grid_cons
 }
 
 template <typename T>
-static int select_typed(const SelectArgs& a, cudaStream_t s) {
-	// 16 rows to a CTA where their scores fit beside one another (R rows of p pages: 8 R p bytes), 8 up to twice as many pages, else and for single tokens one
-	const int R = a.b.N <= a.b.B ? 1 : a.b.max_pages <= 1024 ? 16 : a.b.max_pages <= 2048 ? 8 : 1;
+static int select_typed(const SelectArgs& a, int sms, cudaStream_t s) {
+	// A CTA to a row for single tokens, and where there are no more rows than SMs: 32 rows of 8 kv heads over 200 pages 13 us (26 with 16 rows to a CTA), over 1000 35 (64 with 8); 1400 rows
+	// of two sequences 160 (72), and 656 (386).  Else 16 rows, 8 where there are many pages (their scores are 8 bytes each: 1400 rows over 200 pages 72 and 76 us, over 1000 428 and 386) and
+	// one where shared memory does not hold more.
+	const int R = a.b.N <= a.b.B || a.b.N <= sms ? 1 : a.b.max_pages <= 512 ? 16 : a.b.max_pages <= 2048 ? 8 : 1;
 	const size_t smem = (size_t) R * a.b.max_pages * 8 + (R > 1 ? (size_t) (R * a.c.d + SP * (a.c.d + 4) + R * a.c.d / 8 + ST / 32 + a.b.max_pages) * 4 : 0);
 	const dim3 grid((unsigned) (R > 1 ? a.b.N / R + a.b.B : a.b.N), (unsigned) a.c.G);
 	void (*kernel)(SelectArgs) = R == 16 ? paged_select_rows_kernel<T, 16> : R == 8 ? paged_select_rows_kernel<T, 8> : paged_select_step_kernel<T>;
@@ -710,8 +713,8 @@ constexpr int SMALL_ROWS = 16;
 // 39 with 128
 constexpr int FEW_ROWS = 64;
 // What a piece costs beside its tiles, in tiles, when the work is divided.  mma.sync: 64 sequences behind 8192 shared tokens 97 us, with 2 109.  tcgen05: five prompts of 150 to 700 tokens
-// behind 2048 shared ones 147 us, with 2 176.  fp32: two prompts of 25 tokens 93 us, with 6 107.
-constexpr int LEAD = 6, LEAD_TC = 12, LEAD_F32 = 2;
+// behind 2048 shared ones 147 us, with 2 176.  fp32: 16 sequences of 2500 tokens 79 us, with 6 86.
+constexpr int LEAD = 6, LEAD_TC = 12, LEAD_F32 = 1;
 constexpr int JOIN_ROWS = 4, JOIN_BLOCKS = 8; // rows to a block of the join, and most blocks to an SM: 128 sequences of 32 heads in two groups 205 us, with 2 223; five long prompts 152, with 16 153
 
 // ---- attention: parts, workspace --------------------------------------------------------------------------------------------------------------
@@ -854,7 +857,8 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 	a.by_value = (unsigned) ((0x100000000ull + a.per_value - 1) / a.per_value);
 	int sms = 0;
 	XALM_TRY(sm_count(cache->device, &sms));
-	const bool many = a.b.N >= sms * 4; // four rows to a CTA once that still gives every SM one
+	// Four rows to a CTA once that still gives every SM one.  32 and 8 heads of 128, one and four rows to a CTA: 256 rows 4.5 and 5.9 us, 576 4.9 and 5.9, 1024 8.0 and 7.1, 8192 43 and 39
+	const bool many = a.b.N >= sms * 4;
 	void (*kernel)(AppendArgs) = nullptr;
 	switch (in_type * 16 + cache->type) {
 #define XALM_PAGED_APPEND(I, IT, C, CT) case IT * 16 + CT: kernel = many ? paged_append_kernel<I, C, 4> : paged_append_kernel<I, C, 1>; break;
@@ -934,10 +938,12 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
 	a.rep = heads / a.c.G;
 	a.top = top;
 	a.first = first;
+	int sms = 0;
+	XALM_TRY(sm_count(cache->device, &sms));
 	a.recent = recent;
 	a.out = out;
 	cudaStream_t s = (cudaStream_t) stream;
-	return cache->type == XALM_F32 ? select_typed<float>(a, s) : cache->type == XALM_F16 ? select_typed<__half>(a, s) : select_typed<__nv_bfloat16>(a, s);
+	return cache->type == XALM_F32 ? select_typed<float>(a, sms, s) : cache->type == XALM_F16 ? select_typed<__half>(a, sms, s) : select_typed<__nv_bfloat16>(a, sms, s);
 }
 
 } // extern "C"

@@ -169,9 +169,10 @@ struct Plan {
 	int *cum_w, *cum_u, *shs; // segments + 1, the same, sequences
 	int segs;
 	int total, share;
+	int units;           // where each is a CTA's as a whole, else 0
 	View v; // in shared memory
 };
-__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (5 * B + 3 * n_groups + 5 + 64) * 4; }
+__host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (size_t) (5 * B + 3 * n_groups + 5 + 65) * 4; }
 
 __host__ __device__ __forceinline__ int share_of(int total, int grid) { return (int) (((unsigned) total + grid - 1) / grid); }
 
@@ -217,7 +218,7 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 	p.cum_w = reinterpret_cast<int*>(smem);
 	p.cum_u = p.cum_w + p.segs + 1;
 	p.shs = p.cum_u + p.segs + 1;
-	int *starts = p.shs + B, *lens = starts + B + 1, *bounds = lens + B, *sum_w = bounds + n + 1, *sum_u = sum_w + 32;
+	int *starts = p.shs + B, *lens = starts + B + 1, *bounds = lens + B, *sum_w = bounds + n + 1, *sum_u = sum_w + 32, *longest = sum_u + 32;
 	// the arrays come in at once: what follows asks for them in turn, and every asking of memory is most of a microsecond
 	for (int i = tid; i <= B; i += NT) {
 		starts[i] = a.b.starts[i];
@@ -259,7 +260,8 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 		__syncthreads();
 	}
 	int carry_w = 0, carry_u = 0;
-	if (tid == 0) { p.cum_w[0] = 0; p.cum_u[0] = 0; }
+	if (tid == 0) { p.cum_w[0] = 0; p.cum_u[0] = 0; *longest = 0; }
+	int most = 0; // tiles of a unit
 	for (int base = 0; base < p.segs; base += NT) {
 		const int seg = base + tid;
 		int w = 0, u = 0, in_seg = 0;
@@ -272,6 +274,7 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 				if (seg < n) w = in_seg * unit_work(a, part, seg, rows, Seq(), p.shs[s], 0);
 				else if (in_seg == 1) w = unit_work(a, part, seg, rows, seq_of(p.v, s), p.shs[s], 0);
 				else wide = true;
+				if (!n) most = max(most, wide ? unit_tiles(a, part, seg, rows, seq_of(p.v, s), p.shs[s], in_seg - 1) : w - part.lead); // the last rows see the most
 			}
 		}
 		for (unsigned m = __ballot_sync(0xffffffffu, wide); m; m &= m - 1) {
@@ -301,6 +304,11 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 	}
 	p.total = carry_w;
 	p.share = share_of(p.total, part.grid);
+	if (!n) atomicMax(longest, most);
+	__syncthreads();
+	// Where each unit can have a CTA to itself, and no more tiles than an equal share counts, none is divided and nothing has to be joined.  A prompt of 1024 tokens of 8 kv heads (128 units
+	// of 16 tiles) 38 us in place of 48, 16 of 33 tokens behind 400 (128 of 7) 30 in place of 36; but 64 tokens behind 448 (8 of 8) 30 in place of 26.
+	p.units = !n && carry_u <= part.grid && *longest <= p.share ? carry_u : 0;
 	if (part.cum_w && blockIdx.x == 0) {
 		for (int i = tid; i <= p.segs; i += NT) { part.cum_w[i] = p.cum_w[i]; part.cum_u[i] = p.cum_u[i]; }
 		for (int i = tid; i < B; i += NT) part.shs[i] = p.shs[i];
@@ -343,6 +351,25 @@ __device__ __forceinline__ void walk_piece(const Part& part, Walk& k, int in) {
 }
 // false: nothing for this CTA
 __device__ __forceinline__ bool walk_begin(const Attn& a, const Part& part, const Plan& p, Walk& k) {
+	if (p.units) {
+		k.at = k.end = 0;
+		const int u = blockIdx.x;
+		if (u >= p.units) return false;
+		int lo = 0, hi = p.segs - 1; // the last segment whose units begin at or before this one
+		while (lo < hi) {
+			const int mid = (lo + hi + 1) >> 1;
+			if (p.cum_u[mid] <= u) lo = mid;
+			else hi = mid - 1;
+		}
+		k.x.seg = lo;
+		walk_segment(a, part, p, k);
+		k.x.g = (u - p.cum_u[lo]) / k.tiles;
+		k.x.t = u - p.cum_u[lo] - k.x.g * k.tiles;
+		k.x.u = u;
+		k.x.j0 = 0;
+		k.x.j1 = k.x.w = unit_tiles(a, part, lo, k.x.rows, k.x.q, p.shs[k.x.s], k.x.t);
+		return true;
+	}
 	share_begin(p.total, p.share, k);
 	if (k.at >= k.end) return false;
 	int lo = 0, hi = p.segs - 1; // the last segment that begins at or before k.at

@@ -1,34 +1,123 @@
 // paged_attn.cu — attention over the paged cache: rows of fp32 caches by fp32 FMAs, and the join of what several CTAs have of the same rows.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace xalm {
 namespace paged {
 
 // =========================================================================================================================================
-// Attention by fp32 FMAs: 16 (token, head) rows of one kv head at a time, 32 keys at a time in shared memory, one running maximum and
-// sum per row.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s = scale q.k; kept in log2 units: exp2((q.k - m') scale log2 e).
-// A tile's keys and values are on their way (16 bytes a copy, four threads to a key) while the tile before is worked on.  Scores: a lane to a key, four rows to a warp.
-// Sums: four neighbouring columns to a thread, CG threads side by side, the rows divided among the 128 / CG groups.  Few rows are bound by the latency of a tile's steps, many by
-// what shared memory delivers: for 16 rows of 128 entries 1024 + 640 cycles a tile against 1024 of FMAs.
+// Attention by fp32 FMAs: up to 16 (token, head) rows of one kv head at a time, 32 keys at a time in shared memory.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s = scale q.k;
+// kept in log2 units: exp2((q.k - m') scale log2 e).  A tile's keys and values are on their way (16 bytes a copy, four threads to a key) while the tile before is worked on.
+// A warp takes 8 of the 32 keys, with maximum, sum and output of its own, so that no warp waits for another inside a tile: scores by four lanes to a key, each every fourth 16 bytes of it;
+// sums by four or eight neighbouring columns to a lane.  At the end of a piece the four join through shared memory.  Few rows (R = 4) are bound by latency, 16 by what shared memory
+// delivers: 20 accesses to 64 FMAs of the scores, 8 to 64 of the sums.  Measured with 8 kv heads of 128: 16 sequences of 2500 tokens, four rows to a kv head, 79 us (4.2 TB/s), where a warp to
+// four rows and all keys took 151; two prompts of 300 tokens behind 300 295 us (15 TFLOP/s): 255 registers leave eight warps to an SM.
 // =========================================================================================================================================
-constexpr int RM = 16, RK = 32, RT = 128, RS = 20; // RS: floats between a key's probabilities, so that a warp's stores of four rows meet no bank twice
+constexpr int RM = 16, RK = 32, RT = 128, RW = RT / 32, WK = RK / RW; // keys of a warp
+constexpr int RS = 20; // floats between a key's probabilities of 16 rows
 
 __device__ __forceinline__ void copy16(float* dst, const float* src, bool there) { // zeros where there is nothing
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-template <int CG, bool LIST> // threads that share a value's columns
+// A warp's 8 keys of a tile for R rows.  q: [R][d]; keys: [8][kp]; values: [8][dv], this lane's columns; sp: [8][RS] of the warp; lim: keys that the rows see, `base` before these
+// COLS: 64, 128 or 256 columns of values; with 64 the lanes' halves take every other key
+template <int R, int COLS>
+__device__ __forceinline__ void rows_step(const float* q, const float* keys, const float* values, float* sp, const int* lim, int base, int n_keys, int d, int kp, int dv, int cols, float c1, int lane, float (&m)[R],
+                                          float (&l)[R], float (&acc)[R][COLS == 256 ? 8 : 4]) {
+	constexpr int C = COLS == 256 ? 2 : 1, BY = COLS == 64 ? 2 : 1;
+	const int key = lane >> 2, part = (lane & 3) * 4;
+	float s[R];
+#pragma unroll
+	for (int r = 0; r < R; r++) s[r] = 0.f;
+#pragma unroll 2
+	for (int c = part; c < d; c += 16) { // d is a multiple of 8: the last two lanes may have one step less
+		const float4 k = *reinterpret_cast<const float4*>(keys + key * kp + c);
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			const float4 x = *reinterpret_cast<const float4*>(q + r * d + c);
+			s[r] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[r]))));
+		}
+	}
+	bool grow = false;
+#pragma unroll
+	for (int r = 0; r < R; r++) {
+		s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+		s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+		s[r] = base + key < lim[r] ? s[r] * c1 : -INFINITY;
+		grow = grow || s[r] > m[r] + 8.f;
+	}
+	if (__any_sync(0xffffffffu, grow)) { // rare behind the first keys: probabilities may be up to 2^8
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			float t = s[r];
+#pragma unroll
+			for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+			t = fmaxf(m[r], t);
+			const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - t);
+			l[r] *= f;
+#pragma unroll
+			for (int c = 0; c < 4 * C; c++) acc[r][c] *= f;
+			m[r] = t;
+		}
+	}
+	float p[R];
+#pragma unroll
+	for (int r = 0; r < R; r++) {
+		p[r] = exp2f(s[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+		l[r] += p[r]; // of this lane's keys, four times each
+	}
+	__syncwarp();
+	if ((lane & 3) == 0)
+#pragma unroll
+		for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(sp + key * RS + r) = make_float4(p[r], p[r + 1], p[r + 2], p[r + 3]);
+	__syncwarp();
+	auto add = [&](int j, bool all) {
+		float4 v[C];
+#pragma unroll
+		for (int c = 0; c < C; c++) v[c] = c * 128 < cols ? *reinterpret_cast<const float4*>(values + j * dv + c * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+		for (int r = 0; r < R; r += 4) {
+			const float4 p4 = *reinterpret_cast<const float4*>(sp + j * RS + r);
+			const float x[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+			for (int e = 0; e < 4; e++)
+				if (all || base + j < lim[r + e]) {
+#pragma unroll
+					for (int c = 0; c < C; c++) {
+						acc[r + e][4 * c] = fmaf(x[e], v[c].x, acc[r + e][4 * c]);
+						acc[r + e][4 * c + 1] = fmaf(x[e], v[c].y, acc[r + e][4 * c + 1]);
+						acc[r + e][4 * c + 2] = fmaf(x[e], v[c].z, acc[r + e][4 * c + 2]);
+						acc[r + e][4 * c + 3] = fmaf(x[e], v[c].w, acc[r + e][4 * c + 3]);
+					}
+				}
+		}
+	};
+	if (cols <= 0) return; // these lanes have no columns
+	if (n_keys == WK && base + WK <= lim[0]) { // every row sees every key (rows that are not there see none, and are not written)
+#pragma unroll
+		for (int j = 0; j < WK; j += BY) add(j + (BY > 1 ? lane >> 4 : 0), true);
+	} else // what a row does not see may be anything, an infinity or a NaN too
+#pragma unroll 1
+		for (int j = BY > 1 ? lane >> 4 : 0; j < n_keys; j += BY) add(j, false);
+}
+// Floats between keys: d, and then 16 modulo 32, so that two keys' 64 bytes share no bank
+__host__ __device__ __forceinline__ int key_pitch(int d) { return d + (48 - d % 32) % 32; }
+
+template <int COLS, bool LIST>
 __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ Attn a, const int buffers) {
-	constexpr int RPT = RM * CG / RT; // rows of a thread's sums
 	extern __shared__ __align__(16) uint8_t smem[];
+	constexpr int C = COLS == 256 ? 2 : 1;
 	const Part& part = a.part[0];
-	const int d = a.c.d, dv = a.c.dv, kp = d + 4, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	const int d = a.c.d, dv = a.c.dv, kp = key_pitch(d), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	const int tile = RK * (kp + dv);                      // floats of a tile
 	float* sq = reinterpret_cast<float*>(smem);           // [RM][d]
-	float* st = sq + RM * d;                              // [buffers] of [RK][d + 4] keys and [RK][dv] values
-	float* sp = st + buffers * tile;                      // [RK][RS]
-	float* s_corr = sp + RK * RS;                         // [RM] factor of what a row has so far, then of its sum
-	int* s_lim = reinterpret_cast<int*>(s_corr + RM);     // [RM] keys that a row sees
+	float* st = sq + RM * d;                              // [buffers] of [RK][kp] keys and [RK][dv] values; then the warps' sums [RW][rows][dv]
+	float* sp = st + max(buffers * tile, RW * RM * dv);   // [RK][RS]
+	float2* s_ml = reinterpret_cast<float2*>(sp + RK * RS); // [RW][RM]
+	int* s_lim = reinterpret_cast<int*>(s_ml + RW * RM);  // [RM] keys that a row sees
 	int* s_list = s_lim + RM;                             // [S]
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list + ((LIST ? a.S : 0) + 1) / 2 * 2);
 	Plan plan;
@@ -40,8 +129,9 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 	bool more = LIST ? list_begin(a, part, k) : walk_begin(a, part, plan, k);
 	if (tid == 0)
 		write_head(a, part, k, more, LIST ? more && row_in_seq(k.x.q, k.x.row0) : more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, LIST ? share_of(list_total(a, part), part.grid) : plan.share);
-	const int cg = tid % CG, col = cg * 4, r0 = tid / CG * RPT;      // this thread's columns and rows
-	const int key_of = tid >> 2, P = 1 << a.c.shift;                 // this thread's key of a tile, of which it brings every fourth 16 bytes
+	const int col0 = (COLS == 64 ? lane & 15 : lane) * 4; // this lane's columns of values
+	const int key_of = tid >> 2, P = 1 << a.c.shift; // this thread's key of a tile, of which it brings every fourth 16 bytes
+	constexpr int NONE = -0x7fffffff;
 	for (; more; more = LIST ? list_next(a, part, k) : walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue; // the same for every thread
@@ -62,25 +152,24 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 		if (tid < RM) s_lim[tid] = tid >= rows ? 0 : keys_of(tid);
 		if (LIST) __syncthreads();
 		const int first = x.j0 * KT, last = min(x.j1 * KT, keys_of(rows - 1)); // the last row sees the most
-		auto page_at = [&](int kb) { // page of this thread's key of the tile at kb
-			if (kb + key_of >= last) return -1;
-			const int key = x.key0 + kb + key_of, pg = page_of(a.c, a.b, x.s, LIST ? s_list[key >> a.c.shift] : key >> a.c.shift);
-			if (pg < 0) report(a.c, ERR_PAGE);
-			return pg;
+		auto page_at = [&](int kb) { // what the table has for this thread's key of the tile at kb, looked at when the tile is copied
+			if (kb + key_of >= last) return NONE;
+			const int key = x.key0 + kb + key_of, at = LIST ? s_list[key >> a.c.shift] : key >> a.c.shift;
+			return a.b.table[(long long) x.s * a.b.table_row + at];
 		};
-		auto copy = [&](int kb, int pg, float* to) {
-			const long long slot = (x.key0 + kb + key_of) & (P - 1);
-			const float* kk = reinterpret_cast<const float*>(a.c.k) + (pg < 0 ? 0 : pg * a.c.k_page + slot * a.c.k_slot + x.g * a.c.k_head);
-			const float* vv = reinterpret_cast<const float*>(a.c.v) + (pg < 0 ? 0 : pg * a.c.v_page + slot * a.c.v_slot + x.g * a.c.v_head);
+		auto copy = [&](int kb, int page, float* to) {
+			const bool there = page >= 0 && page < a.c.pages;
+			if (!there && page != NONE) report(a.c, ERR_PAGE);
+			const long long pg = there ? page : 0, slot = there ? (x.key0 + kb + key_of) & (P - 1) : 0;
+			const float* kk = reinterpret_cast<const float*>(a.c.k) + pg * a.c.k_page + slot * a.c.k_slot + x.g * a.c.k_head;
+			const float* vv = reinterpret_cast<const float*>(a.c.v) + pg * a.c.v_page + slot * a.c.v_slot + x.g * a.c.v_head;
 #pragma unroll 4
-			for (int c = (tid & 3) * 4; c < d; c += 16) copy16(to + key_of * kp + c, kk + c, pg >= 0);
+			for (int c = (tid & 3) * 4; c < d; c += 16) copy16(to + key_of * kp + c, kk + c, there);
 #pragma unroll 4
-			for (int c = (tid & 3) * 4; c < dv; c += 16) copy16(to + RK * kp + key_of * dv + c, vv + c, pg >= 0);
+			for (int c = (tid & 3) * 4; c < dv; c += 16) copy16(to + RK * kp + key_of * dv + c, vv + c, there);
 			asm volatile("cp.async.commit_group;" ::: "memory");
 		};
 		int page = page_at(first);
-		copy(first, page, st);
-		page = page_at(first + RK);
 		for (int i = tid; i < RM * (d / 4); i += RT) {
 			const int r = i / (d / 4), c = i % (d / 4) * 4;
 			float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -90,122 +179,77 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 			}
 			*reinterpret_cast<float4*>(sq + r * d + c) = v;
 		}
-		float m[4], l[4], acc[RPT][4];
-#pragma unroll
-		for (int r = 0; r < 4; r++) { m[r] = -INFINITY; l[r] = 0.f; }
-#pragma unroll
-		for (int r = 0; r < RPT; r++)
-#pragma unroll
-			for (int c = 0; c < 4; c++) acc[r][c] = 0.f;
+		copy(first, page, st);
+		page = page_at(first + RK);
 		const float c1 = a.scale * 1.4426950408889634f;
-		const bool scores = warp * 4 < rows, sums = r0 < rows && col < dv;
-		float* now = st;
-		for (int kb = first; kb < last; kb += RK) {
+		auto run = [&](auto of) {
+			constexpr int R = decltype(of)::value;
+			float m[R], l[R], acc[R][4 * C];
+#pragma unroll
+			for (int r = 0; r < R; r++) {
+				m[r] = -INFINITY;
+				l[r] = 0.f;
+#pragma unroll
+				for (int c = 0; c < 4 * C; c++) acc[r][c] = 0.f;
+			}
+			float* now = st;
+			for (int kb = first; kb < last; kb += RK) {
+				asm volatile("cp.async.wait_group 0;" ::: "memory");
+				__syncthreads(); // the tile is there, and nobody reads the one before any more
+				float* next = buffers == 1 || now != st ? st : st + tile;
+				if (buffers > 1) copy(kb + RK, page, next);
+				page = page_at(kb + (buffers > 1 ? 2 : 1) * RK);
+				const int base = kb + warp * WK;
+				if (base < last)
+					rows_step<R, COLS>(sq, now + warp * WK * kp, now + RK * kp + warp * WK * dv + col0, sp + warp * WK * RS, s_lim, base, min(WK, last - base), d, kp, dv, dv - col0, c1, lane, m, l, acc);
+				if (buffers == 1) {
+					__syncthreads();
+					copy(kb + RK, page, next);
+				}
+				now = next;
+			}
 			asm volatile("cp.async.wait_group 0;" ::: "memory");
-			__syncthreads(); // the tile is there, and nobody reads the one before any more
-			float* next = buffers == 1 || now != st ? st : st + tile;
-			if (buffers > 1) copy(kb + RK, page, next);
-			const int after = buffers > 1 ? page_at(kb + 2 * RK) : -1;
-			if (scores) {
-				float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-				for (int c = 0; c < d; c += 4) {
-					const float4 kk = *reinterpret_cast<const float4*>(now + lane * kp + c);
-#pragma unroll
-					for (int r = 0; r < 4; r++) {
-						const float4 qq = *reinterpret_cast<const float4*>(sq + (warp * 4 + r) * d + c);
-						s[r] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[r]))));
-					}
-				}
-				float p[4];
-#pragma unroll
-				for (int r = 0; r < 4; r++) {
-					const float sc = kb + lane < s_lim[warp * 4 + r] ? s[r] * c1 : -INFINITY;
-					const float mt = fmaxf(m[r], warp_max(sc)), base = mt == -INFINITY ? 0.f : mt, corr = exp2f(m[r] - base);
-					p[r] = exp2f(sc - base);
-					l[r] = l[r] * corr + p[r]; // of this lane's keys
-					m[r] = mt;
-					if (lane == 0) s_corr[warp * 4 + r] = corr;
-				}
-				*reinterpret_cast<float4*>(sp + lane * RS + warp * 4) = make_float4(p[0], p[1], p[2], p[3]);
-			}
 			__syncthreads();
-			if (sums) {
-				const int n_keys = min(RK, last - kb);
-				const float* vv = now + RK * kp + col;
 #pragma unroll
-				for (int r = 0; r < RPT; r++) {
-					const float f = s_corr[r0 + r];
+			for (int r = 0; r < R; r++) {
 #pragma unroll
-					for (int c = 0; c < 4; c++) acc[r][c] *= f;
-				}
-				// rows that are not there see no key, and are not written
-				if (kb + n_keys <= s_lim[0]) {
-#pragma unroll 4
-					for (int j = 0; j < RK; j++) { // values behind the last key are zeros, and so are their probabilities
-						const float4 v = *reinterpret_cast<const float4*>(vv + j * dv);
+				for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+				if (lane == 0) s_ml[warp * RM + r] = make_float2(m[r], l[r]);
+				if (COLS == 64)
 #pragma unroll
-						for (int r = 0; r < RPT; r++) {
-							const float p = sp[j * RS + r0 + r];
-							acc[r][0] = fmaf(p, v.x, acc[r][0]);
-							acc[r][1] = fmaf(p, v.y, acc[r][1]);
-							acc[r][2] = fmaf(p, v.z, acc[r][2]);
-							acc[r][3] = fmaf(p, v.w, acc[r][3]);
-						}
-					}
-				} else { // what a row does not see may be anything, an infinity or a NaN too
-					for (int j = 0; j < n_keys; j++) {
-						const float4 v = *reinterpret_cast<const float4*>(vv + j * dv);
+					for (int c = 0; c < 4; c++) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], 16);
 #pragma unroll
-						for (int r = 0; r < RPT; r++)
-							if (kb + j < s_lim[r0 + r]) {
-								const float p = sp[j * RS + r0 + r];
-								acc[r][0] = fmaf(p, v.x, acc[r][0]);
-								acc[r][1] = fmaf(p, v.y, acc[r][1]);
-								acc[r][2] = fmaf(p, v.z, acc[r][2]);
-								acc[r][3] = fmaf(p, v.w, acc[r][3]);
-							}
-					}
-				}
+				for (int c = 0; c < C; c++)
+					if (c * 128 + col0 < dv) *reinterpret_cast<float4*>(st + (warp * R + r) * dv + c * 128 + col0) = make_float4(acc[r][4 * c], acc[r][4 * c + 1], acc[r][4 * c + 2], acc[r][4 * c + 3]);
 			}
-			if (buffers == 1) {
-				__syncthreads();
-				copy(kb + RK, page_at(kb + RK), next);
-			}
-			page = after;
-			now = next;
-		}
-		asm volatile("cp.async.wait_group 0;" ::: "memory");
+			return R;
+		};
+		const int R = rows <= 4 ? run(std::integral_constant<int, 4>()) : rows <= 8 ? run(std::integral_constant<int, 8>()) : run(std::integral_constant<int, 16>());
+		__syncthreads();
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
 		const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
-		__syncthreads(); // the factors have been read
-		if (scores)
+		for (int i = tid; i < rows * (dv / 4); i += RT) {
+			const int row = i / (dv / 4), col = i % (dv / 4) * 4, w = x.t * RM + row;
+			float mx = -INFINITY, l = 0.f;
+			float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-			for (int r = 0; r < 4; r++) {
-				const int row = warp * 4 + r;
-				const float sum = warp_sum(l[r]);
-				const bool any = sum > 0.f || sum != sum;
-				if (lane == 0) {
-					s_corr[row] = direct ? (any ? 1.f / sum : 0.f) : 1.f;
-					if (row < rows) {
-						if (!direct) {
-							if (slot < part.slots) part.ml[slot * RM + row] = make_float2(m[r], sum);
-						} else if (a.lse) {
-							const int w = x.t * RM + row;
-							a.lse[(long long) (x.row0 + w / a.rep) * a.H + h0 + w % a.rep] = any ? (m[r] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-						}
-					}
-				}
+			for (int e = 0; e < RW; e++) mx = fmaxf(mx, s_ml[e * RM + row].x);
+#pragma unroll
+			for (int e = 0; e < RW; e++) {
+				const float2 ml = s_ml[e * RM + row];
+				const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx); // times 0 a NaN stays one
+				const float4 o = *reinterpret_cast<const float4*>(st + (e * R + row) * dv + col);
+				l += ml.y * f;
+				v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
 			}
-		__syncthreads();
-		if (sums) {
-#pragma unroll
-			for (int r = 0; r < RPT; r++) {
-				const int row = r0 + r, w = x.t * RM + row;
-				if (row >= rows) break;
-				const float f = s_corr[row]; // 0: a row that sees nothing, whose sums are zeros
-				float* to = direct ? reinterpret_cast<float*>(a.out) + (long long) (x.row0 + w / a.rep) * a.out_row + (h0 + w % a.rep) * dv + col : part.o + (slot * RM + row) * dv + col;
-				if (direct || slot < part.slots) *reinterpret_cast<float4*>(to) = make_float4(acc[r][0] * f, acc[r][1] * f, acc[r][2] * f, acc[r][3] * f);
+			const bool any = l > 0.f || l != l;
+			if (direct) {
+				const float f = any ? 1.f / l : 0.f; // 0: a row that sees nothing, whose sums are zeros
+				*reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + (long long) (x.row0 + w / a.rep) * a.out_row + (h0 + w % a.rep) * dv + col) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+				if (a.lse && col == 0) a.lse[(long long) (x.row0 + w / a.rep) * a.H + h0 + w % a.rep] = any ? (mx + log2f(l)) * 0.6931471805599453f : -INFINITY;
+			} else if (slot < part.slots) {
+				*reinterpret_cast<float4*>(part.o + (slot * RM + row) * dv + col) = v;
+				if (col == 0) part.ml[slot * RM + row] = make_float2(mx, l);
 			}
 		}
 	}
@@ -408,21 +452,21 @@ int launch_join(const Attn& a, int type, cudaStream_t s) {
 }
 
 static size_t rows_smem(const Cache& c, const BatchView& b, int n_lists, int buffers) {
-	return (size_t) (RM * c.d + buffers * RK * (c.d + 4 + c.dv) + RK * RS + RM) * 4 + (RM + n_lists + 2) * 4 + 16 + (n_lists ? 0 : plan_bytes(b.B, b.n_groups));
+	return (size_t) (RM * c.d + std::max(buffers * RK * (key_pitch(c.d) + c.dv), RW * RM * c.dv) + RK * RS + 2 * RW * RM) * 4 + (RM + n_lists + 2) * 4 + 16 + (n_lists ? 0 : plan_bytes(b.B, b.n_groups));
 }
 // Two buffers where shared memory holds them, which it does not for the largest heads beside thousands of sequences; two CTAs to an SM where it holds those
 static int rows_buffers(const Cache& c, const BatchView& b, int n_lists) { return rows_smem(c, b, n_lists, 2) <= 226 * 1024 ? 2 : 1; }
 int rows_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists) { return rows_smem(c, b, n_lists, rows_buffers(c, b, n_lists)) <= 113 * 1024 ? 2 : 1; }
-template <int CG>
+template <int COLS>
 static int rows_cols(const Attn& a, cudaStream_t s) {
 	const int buffers = rows_buffers(a.c, a.b, a.S);
 	const size_t smem = rows_smem(a.c, a.b, a.S, buffers);
-	auto kernel = a.lists ? paged_rows_kernel<CG, true> : paged_rows_kernel<CG, false>;
+	auto kernel = a.lists ? paged_rows_kernel<COLS, true> : paged_rows_kernel<COLS, false>;
 	XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
 	XALM_CUDA_CHECK(launch(kernel, a.part[0].grid, RT, smem, s, false, a, buffers));
 	return XALM_OK;
 }
-int launch_attn_rows(const Attn& a, cudaStream_t s) { return a.c.dv <= 64 ? rows_cols<16>(a, s) : a.c.dv <= 128 ? rows_cols<32>(a, s) : rows_cols<64>(a, s); }
+int launch_attn_rows(const Attn& a, cudaStream_t s) { return a.c.dv <= 64 ? rows_cols<64>(a, s) : a.c.dv <= 128 ? rows_cols<128>(a, s) : rows_cols<256>(a, s); }
 
 } // namespace paged
 } // namespace xalm
