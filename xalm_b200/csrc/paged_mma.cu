@@ -10,9 +10,11 @@ namespace paged {
 // =========================================================================================================================================
 // out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j, in one pass over the pages.  A step of single tokens reads every key and value once
 // for a handful of rows: HBM bounds it, and what the kernel has to do is to keep enough bytes on their way.  A warp brings tiles of 64 keys and values
-// by TMA (a page's slots, 64 entries wide, swizzled) into a ring; four warps take 16 keys of a tile each, with maximum, sum and output of their own, so that
+// by TMA (a page's slots, 64 entries wide, swizzled) into a ring; four warps take 16 keys of a tile each (with 32 of every other tile a stage is held longer: 91 us in place of 79 for the
+// 64 sequences below behind 8192 tokens in common), with maximum, sum and output of their own, so that
 // none waits for another and a stage is free again after a quarter of a tile's work: scores and sums by mma.sync m16n8k16 with the 16 rows as A, queries and sums in registers.
 // At the end of a piece the four join through shared memory.  (tcgen05 would want 64 rows or more: a step of four heads to a kv head has four.)
+// 64 sequences of up to 1500 tokens, 8 kv heads of 128: 43 us, 4.6 TB/s of pages at random; 10700 lists of 16 pages of 64, which L2 has, 521 us, 11.3 TB/s.
 // Probabilities enter the second product in two parts of the cache's type, rounded and what that left (one alone had 1.5 times the result's own rounding as its error): of up to eight rows
 // the second part are rows 8 to 15 of the same product, of more it costs a product of its own.  Scores, maxima and sums are fp32.
 // =========================================================================================================================================

@@ -134,6 +134,13 @@ def _heads(q):
     return q.shape[1]
 
 
+def _beside(q, n, heads, dim, cache):
+    """(n, heads, dim) of the cache's type, in the quickest way: torch.empty takes 1 us longer, Tensor.new_empty half of one."""
+    if dim == cache.dim and q.dtype is cache.dtype and q.is_contiguous():
+        return torch.empty_like(q)
+    return q.new_empty((n, heads, dim), dtype=cache.dtype)
+
+
 def append(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_out=None):
     """k (rows, kv_heads, dim) and v (rows, kv_heads, vdim) into the pages of their sequences; returns the turned queries in the cache's type (None without q).  freq
     (n): the first 2 n entries of every head are turned."""
@@ -145,7 +152,7 @@ def append(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_o
         heads = _heads(q)
         qr = _rows(q, "q", n, heads, cache.dim, dt, dev)
         if q_out is None:
-            q_out = q.new_empty((n, heads, cache.dim), dtype=cache.dtype)
+            q_out = _beside(q, n, heads, cache.dim, cache)
             qor = heads * cache.dim
         else:
             qor = _rows(q_out, "q_out", n, heads, cache.dim, cache.dtype, dev)
@@ -165,7 +172,7 @@ def _attend(cache, batch, q, lists, scale, out, want_lse):
     (bp, held), stream = _start(cache, batch, n)
     qr = _rows(q, "q", n, heads, cache.dim, cache.dtype, dev)
     if out is None:
-        out = q.new_empty((n, heads, cache.vdim))  # torch.empty takes a microsecond longer
+        out = _beside(q, n, heads, cache.vdim, cache)
         outr = heads * cache.vdim
     else:
         outr = _rows(out, "out", n, heads, cache.vdim, cache.dtype, dev)
