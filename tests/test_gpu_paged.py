@@ -523,6 +523,45 @@ def test_append_of_any_head_size(d, dv, rot, neighbours, layout):
     check_append(Problem("f32", [20], [64], G=1, rep=1, d=d, dv=dv, page=64, layout=layout, seed=33), "f32", rot, neighbours, queries=False)
 
 
+def test_results_that_overlap_their_queries_are_refused():
+    p = Problem("f16", [1, 4], [30, 40], d=64, page=16, seed=53)
+    cache, batch = p.on_gpu()
+    k = torch.zeros(p.rows, p.G, 64, dtype=p.t, device="cuda")
+    rows, heads = p.rows, p.H
+    room = torch.zeros(4 * rows * heads * 64, dtype=p.t, device="cuda")
+    dense = lambda at: room[at:at + rows * heads * 64].view(rows, heads, 64)
+    wide = room[:rows * 3 * heads * 64].view(rows, 3 * heads, 64)
+    pages = torch.zeros(rows, p.G, 1, dtype=torch.int32, device="cuda")
+    freq = torch.ones(12, device="cuda")
+    one = heads * 64
+    for q, out, meets in ((dense(0), dense(8), True), (dense(8), dense(0), True), (dense(0), dense(rows * one - 8), True), (dense(0), dense(rows * one), False), (dense(rows * one), dense(0), False),
+                          (wide[:, :heads], wide[:, heads:2 * heads], False), (wide[:, heads:2 * heads], wide[:, :heads], False), (wide[:, :heads], wide[:, heads - 1:2 * heads - 1], True),
+                          (wide[:, heads:2 * heads], wide[:, 1:heads + 1], True), (dense(0), wide[:, heads:2 * heads], True), (dense(0), dense(0), True)):
+        for call in (lambda: paged.attend(cache, batch, q, 1.0, out=out), lambda: paged.attend_selected(cache, batch, q, pages, 1.0, out=out),
+                     lambda: paged.append(cache, batch, k, k, q=q, freq=freq, q_out=out)):
+            if meets:
+                with pytest.raises(capi.XalmError, match="overlaps"):
+                    call()
+            else:
+                call()
+    cache.check()
+
+
+@pytest.mark.parametrize("neighbours,rot", [(False, 32), (False, 8), (True, 5), (True, 32), (False, 0)])
+def test_append_turns_queries_in_place(neighbours, rot):
+    p = Problem("bf16", [1, 40, 700], [9, 90, 701], d=64, page=16, seed=52, pad_rows=2)
+    cache, batch = p.on_gpu()
+    k, v = (torch.randn(p.rows, p.G, 64, generator=p.gen).to(p.t).cuda() for _ in range(2))
+    freq = torch.rand(rot, generator=p.gen).cuda() if rot else None
+    want = paged.append(cache, batch, k, v, q=p.gq, freq=freq, neighbours=neighbours)
+    inside = [n for n in range(p.rows) if p.row(n) is not None]
+    wide = torch.zeros(p.rows, p.H + 3, 64, dtype=p.t, device="cuda")
+    wide[:, :p.H] = p.gq
+    q = wide[:, :p.H]
+    assert paged.append(cache, batch, k, v, q=q, freq=freq, neighbours=neighbours, q_out=q) is q
+    assert torch.equal(q[inside], want[inside]) and (wide[:, p.H:] == 0).all()
+
+
 def test_append_far_positions():
     """Position 1000000: the angle in 32 bits would be 0.03 off."""
     p = Problem("f32", [1, 2], [100, 90], d=64, page=256, seed=34)
@@ -709,3 +748,12 @@ def test_a_workspace_too_small_is_refused():
     assert L.xalm_cuda_paged_attend(*args(need.value - 1)) == 1
     assert L.xalm_cuda_paged_attend(*args(need.value)) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits,words", [(1, "names a page"), (2, "do not fit"), (4, "gave up a wait"), (5, "names a page outside the pool and a kernel gave up")])
+def test_what_kernels_report_is_raised_once(bits, words):
+    cache, _ = Problem("bf16", [1], [20], d=64, page=16, seed=54).on_gpu()
+    cache.status.fill_(bits)
+    with pytest.raises(capi.XalmError, match=words):
+        cache.check()
+    cache.check()

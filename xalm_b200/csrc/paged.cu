@@ -679,6 +679,15 @@ static int check_rows(const char* what, const void* p, long long row, int least,
 	return XALM_OK;
 }
 
+// Whether n rows of so many bytes each meet: rows that lie side by side in wider ones of the same stride do not
+static bool rows_meet(const void* p, long long p_row, long long p_bytes, const void* q, long long q_row, long long q_bytes, int n) {
+	const uintptr_t a = (uintptr_t) p, b = (uintptr_t) q;
+	if (a >= b + (n - 1) * q_row + q_bytes || b >= a + (n - 1) * p_row + p_bytes) return false;
+	if (p_row != q_row) return true;
+	const long long off = (long long) (b - a) % p_row, at = off < 0 ? off + p_row : off; // from a row of p to the next of q
+	return at < p_bytes || at + q_bytes > p_row;
+}
+
 // The calling thread's device is what it was when the call returns
 struct OnDevice {
 	int before = -1;
@@ -784,6 +793,7 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 	if (b.N == 0 || b.B == 0) return XALM_OK;
 	if (!workspace || ((uintptr_t) workspace & 255)) return set_error(XALM_ERR_INVALID, "paged attention: the workspace is NULL or not at a 256-byte boundary");
 	XALM_TRY(plan_attn(cache, c, b, heads, n_lists, a, &need));
+	if (rows_meet(q, q_row * e, (long long) heads * c.d * e, out, out_row * e, (long long) heads * c.dv * e, b.N)) return set_error(XALM_ERR_INVALID, "paged attention: out overlaps q");
 	if (workspace_bytes < need) return set_error(XALM_ERR_INVALID, "paged attention: a workspace of %zu bytes is needed, %zu given", need, workspace_bytes);
 	OnDevice on;
 	XALM_TRY(on.set(cache->device));
@@ -839,6 +849,10 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 		if (q) {
 			XALM_TRY(check_rows("q", q, q_row, heads * a.c.d, ei));
 			XALM_TRY(check_rows("q_out", q_out, q_out_row, heads * a.c.d, e));
+			// in place only where a thread has all that its results are made of
+			const bool in_place = q == q_out && q_row == q_out_row && in_type == cache->type && (neighbours || rot_half % 8 == 0);
+			if (!in_place && rows_meet(q, q_row * ei, (long long) heads * a.c.d * ei, q_out, q_out_row * e, (long long) heads * a.c.d * e, a.b.N))
+				return set_error(XALM_ERR_INVALID, "paged append: q_out overlaps q (in place: the same rows of the cache's type, and halves of a multiple of 8 pairs or neighbours)");
 		}
 	}
 	if (a.b.N == 0 || a.b.B == 0) return XALM_OK;
