@@ -191,6 +191,18 @@ def test_a_value_that_is_not_finite_stays_in_its_column_and_its_rows(type):
     assert torch.isfinite(out[:, :, rest]).all()
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rep", [1, 4, 8, 9, 16])
+@pytest.mark.parametrize("what", ["all", "shared", "lists"])
+def test_infinite_values_of_few_rows_stay_in_their_column(what, rep, type):
+    groups = ([0, 2], [64]) if what == "shared" else None
+    p = Problem(type, [1, 1, 1], [140, 150, 31], d=64, page=16, G=2, rep=rep, seed=11, groups=groups)
+    for s, at, c, x in ((0, 3, 5, math.inf), (0, 60, 6, -math.inf), (1, 149, 7, math.inf), (2, 30, 63, -math.inf), (0, 100, 9, math.nan)):
+        pg, sl = p.slots(s, at)
+        p.v[pg, sl, 1, c] = x
+    check_attend(p, lists=torch.arange(p.max_pages, dtype=torch.int32).repeat(p.rows, p.G, 1) if what == "lists" else None)
+
+
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 def test_large_and_equal_scores(type):
     p = Problem(type, [1, 8], [300, 200], d=64, page=32, seed=11, key_scale=30.0)  # one key takes all

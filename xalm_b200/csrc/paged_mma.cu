@@ -14,7 +14,7 @@ namespace paged {
 // 64 sequences below behind 8192 tokens in common), with maximum, sum and output of their own, so that
 // none waits for another and a stage is free again after a quarter of a tile's work: scores and sums by mma.sync m16n8k16 with the 16 rows as A, queries and sums in registers.
 // At the end of a piece the four join through shared memory.  (tcgen05 would want 64 rows or more: a step of four heads to a kv head has four.)
-// 64 sequences of up to 1500 tokens, 8 kv heads of 128: 43 us, 4.6 TB/s of pages at random; 10700 lists of 16 pages of 64, which L2 has, 521 us, 11.3 TB/s.
+// 64 sequences of up to 1500 tokens, 8 kv heads of 128: 43 us, 4.6 TB/s of pages at random; 10700 lists of 16 pages of 64, which L2 has, 485 us, 12.1 TB/s.
 // Probabilities enter the second product in two parts of the cache's type, rounded and what that left (one alone had 1.5 times the result's own rounding as its error): of up to eight rows
 // the second part are rows 8 to 15 of the same product, of more it costs a product of its own.  Scores, maxima and sums are fp32.
 // =========================================================================================================================================
@@ -79,11 +79,29 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 // what is left of two numbers beside their rounded ones
 template <typename T>
-__device__ __forceinline__ uint32_t left16(uint32_t rounded, float lo, float hi) {
+__device__ __forceinline__ float2 rest16(uint32_t rounded, float lo, float hi) {
 	if constexpr (std::is_same<T, __half>::value) {
 		const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
-		return pack16<T>(lo - r.x, hi - r.y);
-	} else return pack16<T>(lo - __uint_as_float(rounded << 16), hi - __uint_as_float(rounded & 0xffff0000u));
+		return make_float2(lo - r.x, hi - r.y);
+	} else return make_float2(lo - __uint_as_float(rounded << 16), hi - __uint_as_float(rounded & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t left16(uint32_t rounded, float lo, float hi) {
+	const float2 r = rest16<T>(rounded, lo, hi);
+	return pack16<T>(r.x, r.y);
+}
+// the smallest number of the type that a product does not take for 0; rounding towards 0; what that leaves, at least `least` of what is positive
+template <typename T>
+__device__ __forceinline__ constexpr float tiny16() { return std::is_same<T, __half>::value ? 5.9604645e-8f : 1.17549435e-38f; }
+template <typename T>
+__device__ __forceinline__ uint32_t cut16(float lo, float hi) {
+	if constexpr (std::is_same<T, __half>::value) return (uint32_t) __half_as_ushort(__float2half_rz(lo)) | (uint32_t) __half_as_ushort(__float2half_rz(hi)) << 16;
+	else return (uint32_t) __bfloat16_as_ushort(__float2bfloat16_rz(lo)) | (uint32_t) __bfloat16_as_ushort(__float2bfloat16_rz(hi)) << 16;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t left16(uint32_t rounded, float lo, float hi, float least) {
+	const float2 r = rest16<T>(rounded, lo, hi);
+	return pack16<T>(lo > 0.f ? fmaxf(r.x, least) : r.x, hi > 0.f ? fmaxf(r.y, least) : r.y);
 }
 __device__ __forceinline__ float ex2(float x) {
 	float y;
@@ -293,13 +311,18 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				rest[2 * i] = left16<T>(pa[2 * i], x0, x1);
 				pa[2 * i + 1] = rest[2 * i];
 			}
-			if (high) {
+			if (high) { // both parts add to the same sums: neither is negative, nor 0 beside a probability that is not, so that an infinite value gives an infinity
 #pragma unroll
-				for (int i = 0; i < 2; i++) {
-					const float x2 = ex2(fmaf(s[i][2], c1, b1)), x3 = ex2(fmaf(s[i][3], c1, b1));
-					l1 += x2 + x3;
-					pa[2 * i + 1] = pack16<T>(x2, x3);
-					rest[2 * i + 1] = left16<T>(pa[2 * i + 1], x2, x3);
+				for (int i = 0; i < 4; i++) {
+					float x[2];
+#pragma unroll
+					for (int e = 0; e < 2; e++) {
+						x[e] = ex2(fmaf(s[i >> 1][(i & 1) * 2 + e], c1, i & 1 ? b1 : b0));
+						if (i & 1) l1 += x[e];
+						x[e] = x[e] > 0.f ? fmaxf(x[e], tiny16<T>()) : x[e];
+					}
+					pa[i] = cut16<T>(x[0], x[1]);
+					rest[i] = left16<T>(pa[i], x[0], x[1], tiny16<T>());
 				}
 #pragma unroll
 				for (int c = 0; c < D / 16; c++) {
@@ -323,7 +346,9 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		}
 		if (!high)
 #pragma unroll
-			for (int i = 0; i < D / 8; i++) { o[i][0] += o[i][2]; o[i][1] += o[i][3]; }
+			for (int i = 0; i < D / 8; i++) // what an infinite value made infinite stays so: the rest may be 0 or negative
+#pragma unroll
+				for (int e = 0; e < 2; e++) o[i][e] = fabsf(o[i][e]) <= 3.4e38f ? o[i][e] + o[i][e + 2] : o[i][e];
 		m0 *= c1; // in units of log2 from here on
 		m1 *= c1;
 		// ---- the four warps' sums ----
