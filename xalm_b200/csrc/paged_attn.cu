@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(RT) paged_rows_kernel(const __grid_constant__ 
 // =========================================================================================================================================
 // The join of what several CTAs have of the same rows, a warp to a row.  A lane takes a piece's maximum and sum, then the pieces' rows are added with their weights, eight
 // loads on their way at a time.  Two kinds of blocks: with groups, for rows that read shared pages; and for 16 rows
-// of the units that a CTA's share begins inside.  Bound by the latency of three or four loads that depend on one another:
+// of the units that a CTA's share begins inside (four to a warp, which for five long prompts take 143 us of all in place of 149).  Bound by the latency of three or four loads that depend on one another:
 // 2048 rows of 128 entries in 12 us.
 // =========================================================================================================================================
 constexpr int JT = 128, JR = 16;
@@ -376,6 +376,69 @@ __device__ __forceinline__ void join_row(const Attn& a, const JoinUnit (&u)[2], 
 	if (a.lse && lane == 0) a.lse[(long long) row * a.H + h] = any ? (base + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
+// Four neighbouring rows of a unit of up to eight pieces by a warp, eight lanes to a row's maxima and sums, four rows' loads on their way together.  at: rows of the unit; w: of the segment
+template <typename T, int NC>
+__device__ __forceinline__ void join_four(const Attn& a, const JoinUnit& u, int rows, int row0, int head0, int w) {
+	const int lane = threadIdx.x & 31, mine = lane >> 3, c = lane & 7, dv = a.c.dv;
+	const Part& p = a.part[u.part];
+	auto slot_of = [&](int i) { return piece_slot(a, u.unit, u.cta + i, i == 0); };
+	float2 ml = make_float2(-INFINITY, 0.f);
+	if (mine < rows && c < u.n && slot_of(c) < p.slots) ml = p.ml[slot_of(c) * p.M + u.at + mine];
+	const bool some = ml.x != -INFINITY || ml.y != 0.f; // else nothing that the row sees
+	const unsigned there = __ballot_sync(0xffffffffu, some), nan = __ballot_sync(0xffffffffu, ml.x != ml.x);
+	float m = ml.x;
+#pragma unroll
+	for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+	const float base = nan >> (mine * 8) & 0xff ? NAN : m == -INFINITY ? 0.f : m, wgt = !some || ml.x == -INFINITY ? 0.f : exp2f(ml.x - base);
+	float l = some ? ml.y * wgt : 0.f; // a sum that is NaN stays one
+#pragma unroll
+	for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+	float4 acc[4][NC];
+#pragma unroll
+	for (int r = 0; r < 4; r++)
+#pragma unroll
+		for (int k = 0; k < NC; k++) acc[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+	for (int i = 0; i < u.n; i++) {
+		const float* o = p.o + (slot_of(i) * p.M + u.at) * dv + lane * 4;
+		float4 x[4][NC];
+#pragma unroll
+		for (int r = 0; r < 4; r++)
+#pragma unroll
+			for (int k = 0; k < NC; k++)
+				x[r][k] = (there >> (r * 8 + i) & 1) && k * 128 + lane * 4 < dv ? *reinterpret_cast<const float4*>(o + r * dv + k * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+		for (int r = 0; r < 4; r++) {
+			const float f = __shfl_sync(0xffffffffu, wgt, r * 8 + i);
+#pragma unroll
+			for (int k = 0; k < NC; k++) {
+				acc[r][k].x = fmaf(x[r][k].x, f, acc[r][k].x);
+				acc[r][k].y = fmaf(x[r][k].y, f, acc[r][k].y);
+				acc[r][k].z = fmaf(x[r][k].z, f, acc[r][k].z);
+				acc[r][k].w = fmaf(x[r][k].w, f, acc[r][k].w);
+			}
+		}
+	}
+	const bool any = l > 0.f || l != l;
+	const float inv = any ? 1.f / l : 0.f;
+	if (a.lse && c == 0 && mine < rows) a.lse[(long long) (row0 + (w + mine) / a.rep) * a.H + head0 + (w + mine) % a.rep] = any ? (base + log2f(l)) * 0.6931471805599453f : -INFINITY;
+#pragma unroll
+	for (int r = 0; r < 4; r++) {
+		const float f = __shfl_sync(0xffffffffu, inv, r * 8);
+		T* out = reinterpret_cast<T*>(a.out) + (long long) (row0 + (w + r) / a.rep) * a.out_row + (head0 + (w + r) % a.rep) * dv + lane * 4;
+#pragma unroll
+		for (int k = 0; k < NC; k++)
+			if (r < rows && k * 128 + lane * 4 < dv) {
+				const float y[4] = {acc[r][k].x * f, acc[r][k].y * f, acc[r][k].z * f, acc[r][k].w * f};
+				T v[4];
+#pragma unroll
+				for (int e = 0; e < 4; e++) v[e] = from_f<T>(f == 0.f ? 0.f : y[e]); // 0: a row that sees nothing
+				if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(out + k * 128) = *reinterpret_cast<const uint4*>(v);
+				else *reinterpret_cast<uint2*>(out + k * 128) = *reinterpret_cast<const uint2*>(v);
+			}
+	}
+}
+
 // blocks of a part's boundaries: one to 16 rows of each
 __host__ __device__ __forceinline__ int boundary_blocks(const Part& p) { return p.grid * (p.M > JR ? p.M / JR : 1); }
 
@@ -433,6 +496,12 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ 
 		u[0].unit = x.u;
 		u[0].cta = cta - 1;
 		u[0].n = (x.share - x.j0 + x.w - 1) / x.share + 1;
+		if (u[0].n <= 8) {
+			const int r = (id - cta * chunks) * JR + warp * (JR / (JT / 32)), w = x.first + r;
+			u[0].at = r;
+			if (r < x.rows) join_four<T, NC>(a, u[0], min(4, x.rows - r), x.row0, x.g * a.rep, w);
+			return;
+		}
 		for (int r = (id - cta * chunks) * JR + warp; r < min(x.rows, (id - cta * chunks) * JR + JR); r += JT / 32) {
 			const int w = x.first + r, tok = w / a.rep;
 			u[0].at = r;
