@@ -1,0 +1,95 @@
+"""The paged cache's operators where a number, a length or a caller comes to the edge of what they take, against the restatement in 64 bits (paged_ref.py, which derives the tolerances)."""
+import math
+
+import pytest
+import torch
+
+from paged_ref import Problem
+from test_gpu_paged import near
+from xalm_b200 import paged
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- probabilities far below a row's largest one ---------------------------------------------------------------------------------------------
+def sink(type, new, lens, below, rep, page=64, groups=None, wave=0.0):
+    """Key 0 of every sequence has a score `below` above all others' and a value of 0; the others' values are 1, their scores equal, or `wave` apart."""
+    p = Problem(type, new, lens, G=1, rep=rep, d=64, page=page, seed=60, groups=groups)
+    p.q.zero_()
+    p.q[:, :, 0], p.q[:, :, 1] = 4.0, 1.0
+    p.k.zero_()
+    if wave:
+        p.k[..., 1] = (torch.rand(p.k.shape[:-1], generator=p.gen) * 2 - 1).mul_(wave * 8).to(p.t)
+    p.v.fill_(1.0)
+    for s in range(len(new)):
+        at = p.slots(s, 0)
+        p.k[at], p.v[at] = 0.0, 0.0
+        p.k[at + (0, 0)] = 2.0 * below  # times 4, times the scale 1 / 8
+    return p
+
+
+def looked_at(p, n=9):
+    rows = [r for r in range(p.rows) if p.row(r) is not None]
+    return sorted(set(rows[:: max(1, len(rows) // n)] + rows[-1:]))
+
+
+def check(p, lists=None, round_p=True):
+    cache, batch = p.on_gpu()
+    some = looked_at(p)
+    args = dict(want_lse=True)
+    out, lse = paged.attend(cache, batch, p.gq, p.scale, **args) if lists is None else paged.attend_selected(cache, batch, p.gq, lists.to("cuda"), p.scale, **args)
+    cache.check()
+    want, want_lse, tol, tol_lse = p.attend(lists, round_p=round_p, only=some)
+    near(out[some], want[some], tol[some], "out")
+    near(lse[some], want_lse[some], tol_lse[some], "lse")
+
+
+# tokens and query heads to a kv head: 1, 8, 9, 16 and 256 rows
+ROWS = {1: (1, 1), 8: (1, 8), 9: (1, 9), 16: (1, 16), 256: (64, 4)}
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("n,below", [(4096, 12), (8192, 20), (32768, 14), (32768, 20)])
+@pytest.mark.parametrize("where", ["own", "shared", "lists"])
+def test_many_small_probabilities_beside_a_large_one(where, n, below, rows, type):
+    tokens, rep = ROWS[rows]
+    if where == "shared":  # the rows are those of two or more sequences
+        if rows == 9:
+            p = sink(type, [1] * 9, [n + 64 + i for i in range(9)], below, 1, groups=([0, 9], [n]))
+        elif rows == 1:
+            p = sink(type, [1, 0], [n + 64, n], below, 1, groups=([0, 2], [n]))
+        elif rows == 256:
+            p = sink(type, [1] * 16, [n + 1] * 16, below, 16, groups=([0, 16], [n]))
+        else:
+            p = sink(type, [1, 1], [n + 64, n + 7], below, rep // 2, groups=([0, 2], [n]))
+        return check(p)
+    if where == "lists" and rows == 256:
+        tokens = 3  # a unit has one token's rows there
+    p = sink(type, [tokens], [n], below, rep)
+    check(p, torch.arange(p.max_pages, dtype=torch.int32).repeat(p.rows, p.G, 1) if where == "lists" else None)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 4, 8, 9, 16])
+@pytest.mark.parametrize("where", ["own", "lists", "shared", "wide"])
+def test_probabilities_of_few_rows_keep_more_bits_than_their_type(where, rows, type):
+    """The tolerance has no rounding of the probabilities in it, and the results are near 0 beside the values that they are sums of."""
+    d = 256 if where == "wide" else 64
+    groups = ([0, 2], [192]) if where == "shared" else None
+    p = Problem(type, [1, 1], [260, 290], G=2, rep=rows, d=d, page=64, seed=61, groups=groups)
+    p.v = (p.v.float() + 3 * torch.sign(p.v.float())).to(p.t)  # results near 0 from values that are not
+    check(p, torch.arange(p.max_pages, dtype=torch.int32).repeat(p.rows, p.G, 1) if where == "lists" else None, round_p=False)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("rep", [1, 8, 9, 16])
+@pytest.mark.parametrize("below", [5, 20, 40, 60])
+def test_an_infinite_value_of_a_small_probability_gives_an_infinity(below, rep, type):
+    """Also where the probability is far below what fp16 holds beside the row's largest."""
+    for bad in (math.inf, -math.inf):
+        p = sink(type, [1], [300], below, rep)
+        p.v[p.slots(0, 200) + (0, 7)] = bad
+        cache, batch = p.on_gpu()
+        out = paged.attend(cache, batch, p.gq, p.scale)
+        assert (out[:, :, 7] == bad).all() and torch.isfinite(out[:, :, :7]).all() and torch.isfinite(out[:, :, 8:]).all()

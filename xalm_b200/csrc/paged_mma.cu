@@ -17,6 +17,8 @@ namespace paged {
 // 64 sequences of up to 1500 tokens, 8 kv heads of 128: 43 us, 4.6 TB/s of pages at random; 10700 lists of 16 pages of 64, which L2 has, 485 us, 12.1 TB/s.
 // Probabilities enter the second product in two parts of the cache's type, rounded and what that left (one alone had 1.5 times the result's own rounding as its error): of up to eight rows
 // the second part are rows 8 to 15 of the same product, of more it costs a product of its own.  Scores, maxima and sums are fp32.
+// fp16 ends at 2^-24, so its probabilities are lifted by 2^12, its second part by 2^11 more into sums of its own: what a probability loses is below 2^-47 of the row's largest one, and
+// thousands of small ones beside a large one whose value is 0 keep their sum.
 // =========================================================================================================================================
 constexpr int MM = 16, CW = 4, MT = (CW + 1) * 32;
 
@@ -85,23 +87,23 @@ __device__ __forceinline__ float2 rest16(uint32_t rounded, float lo, float hi) {
 		return make_float2(lo - r.x, hi - r.y);
 	} else return make_float2(lo - __uint_as_float(rounded << 16), hi - __uint_as_float(rounded & 0xffff0000u));
 }
+// rounding towards 0
+__device__ __forceinline__ uint32_t cut_bf16(float lo, float hi) { return (uint32_t) __bfloat16_as_ushort(__float2bfloat16_rz(lo)) | (uint32_t) __bfloat16_as_ushort(__float2bfloat16_rz(hi)) << 16; }
+constexpr float REST_LIFT = 2048.f; // of fp16: half a step of 2^15, the most a probability is, is 2^4
+// the two parts of two probabilities
 template <typename T>
-__device__ __forceinline__ uint32_t left16(uint32_t rounded, float lo, float hi) {
-	const float2 r = rest16<T>(rounded, lo, hi);
-	return pack16<T>(r.x, r.y);
-}
-// the smallest number of the type that a product does not take for 0; rounding towards 0; what that leaves, at least `least` of what is positive
-template <typename T>
-__device__ __forceinline__ constexpr float tiny16() { return std::is_same<T, __half>::value ? 5.9604645e-8f : 1.17549435e-38f; }
-template <typename T>
-__device__ __forceinline__ uint32_t cut16(float lo, float hi) {
-	if constexpr (std::is_same<T, __half>::value) return (uint32_t) __half_as_ushort(__float2half_rz(lo)) | (uint32_t) __half_as_ushort(__float2half_rz(hi)) << 16;
-	else return (uint32_t) __bfloat16_as_ushort(__float2bfloat16_rz(lo)) | (uint32_t) __bfloat16_as_ushort(__float2bfloat16_rz(hi)) << 16;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t left16(uint32_t rounded, float lo, float hi, float least) {
-	const float2 r = rest16<T>(rounded, lo, hi);
-	return pack16<T>(lo > 0.f ? fmaxf(r.x, least) : r.x, hi > 0.f ? fmaxf(r.y, least) : r.y);
+__device__ __forceinline__ void parts16(float lo, float hi, uint32_t& rounded, uint32_t& rest) {
+	if constexpr (std::is_same<T, __half>::value) {
+		// no 0, beside which an infinite value would give no infinity: what this adds to the smallest, and to masked ones, the second part takes off again
+		const __half2 h = __hmax2_nan(__floats2half2_rn(lo, hi), __halves2half2(__ushort_as_half(1), __ushort_as_half(1)));
+		rounded = *reinterpret_cast<const uint32_t*>(&h);
+		const float2 r = rest16<T>(rounded, lo, hi);
+		rest = pack16<T>(r.x * REST_LIFT, r.y * REST_LIFT);
+	} else {
+		rounded = pack16<T>(lo, hi);
+		const float2 r = rest16<T>(rounded, lo, hi);
+		rest = pack16<T>(r.x, r.y);
+	}
 }
 __device__ __forceinline__ float ex2(float x) {
 	float y;
@@ -109,7 +111,8 @@ __device__ __forceinline__ float ex2(float x) {
 	return y;
 }
 
-template <typename T, int D, bool LIST>
+// WIDE: units may have more than eight rows.  Those of a list are one token's, so that the host knows; without the code for them 10700 lists of fp16 take 481 us, with it 518.
+template <typename T, int D, bool LIST, bool WIDE>
 __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const __grid_constant__ CUtensorMap kmap,
                                                                          const __grid_constant__ CUtensorMap vmap, const int stages) {
 	using Z = Sizes<D>;
@@ -204,7 +207,9 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	// ---- the products ----
 	const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;            // a negative scale turns the queries' signs
 	const float c1 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f); // not 0: 0 times an infinity is no number
-	const float slack = 11.5f / c1;
+	constexpr bool HALF = std::is_same<T, __half>::value;
+	constexpr float LIFT = HALF ? 12.f : 0.f, LAG = HALF ? 3.f : 11.5f; // in powers of two; fp16 ends at 2^16
+	const float slack = LAG / c1;
 	// where this lane's rows of ldmatrix lie in a tile: keys (lane & 7) + 8 (lane / 16) of this warp's 16, chunk (lane / 8) & 1; values lane & 15, chunk lane / 16.  Every two chunks
 	// further on are two bits of the address turned over, every eight a block of columns.
 	const int kr = (lane & 7) + (lane >> 4) * 8, vr = lane & 15;
@@ -247,7 +252,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 #pragma unroll
 			for (int e = 0; e < 4; e++) o[i][e] = 0.f;
 		const int j1 = min(x.j1, (most + KT - 1) / KT);
-		const bool high = rows > 8;
+		const bool high = WIDE && rows > 8;
 		bool there = false; // the next tile
 		for (int j = x.j0; j < j1; j++, advance()) {
 			if (!there && !wait_for(&full[st], round, s_dead, a.c)) continue;
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 					for (int e = 0; e < 4; e++)
 						if (base + i * 8 + (lane & 3) * 2 + (e & 1) >= (e < 2 ? lim0 : lim1)) s[i][e] = -INFINITY;
 			}
-			// The maximum that probabilities are taken against may lag behind by 2^11.5, which fp16 holds: then no lane has to ask its neighbours, and sums stay as they are
+			// The maximum that probabilities are taken against may lag behind by 2^LAG: then no lane has to ask its neighbours, and sums stay as they are
 			float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
 			if (__any_sync(0xffffffffu, t0 > m0 + slack || t1 > m1 + slack)) {
 #pragma unroll
@@ -297,8 +302,8 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				for (int i = 0; i < D / 8; i++) { o[i][0] *= f0; o[i][1] *= f0; o[i][2] *= high ? f1 : f0; o[i][3] *= high ? f1 : f0; }
 				m0 = n0;
 				m1 = n1;
-				b0 = m0 == -INFINITY ? 0.f : -m0 * c1;
-				b1 = m1 == -INFINITY ? 0.f : -m1 * c1;
+				b0 = m0 == -INFINITY ? 0.f : fmaf(-m0, c1, LIFT);
+				b1 = m1 == -INFINITY ? 0.f : fmaf(-m1, c1, LIFT);
 			}
 			// asked for here, known when this tile is done
 			there = j + 1 < j1 && try_wait_once(&full[st + 1 == stages ? 0 : st + 1], round ^ (st + 1 == stages));
@@ -307,22 +312,45 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			for (int i = 0; i < 2; i++) {
 				const float x0 = ex2(fmaf(s[i][0], c1, b0)), x1 = ex2(fmaf(s[i][1], c1, b0));
 				l0 += x0 + x1;
-				pa[2 * i] = pack16<T>(x0, x1);
-				rest[2 * i] = left16<T>(pa[2 * i], x0, x1);
+				parts16<T>(x0, x1, pa[2 * i], rest[2 * i]);
 				pa[2 * i + 1] = rest[2 * i];
 			}
-			if (high) { // both parts add to the same sums: neither is negative, nor 0 beside a probability that is not, so that an infinite value gives an infinity
+			if constexpr (HALF) {
+				if (high) {
+#pragma unroll
+					for (int i = 0; i < 2; i++) {
+						const float x0 = ex2(fmaf(s[i][2], c1, b1)), x1 = ex2(fmaf(s[i][3], c1, b1));
+						l1 += x0 + x1;
+						parts16<T>(x0, x1, pa[2 * i + 1], rest[2 * i + 1]);
+					}
+#pragma unroll
+					for (int c = 0; c < D / 16; c++) {
+						uint32_t b[4];
+						float t[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+						ldsm4_t(b, ((tile + v_lane) ^ ((c * 2 & 7) << 4)) + (c >> 2) * KT * 128);
+						mma16<T>(t[0], rest, b[0], b[1]);
+						mma16<T>(t[1], rest, b[2], b[3]);
+#pragma unroll
+						for (int i = 0; i < 2; i++)
+#pragma unroll
+							for (int e = 0; e < 4; e++) // what is not finite comes from the first part's product, none of whose probabilities is 0
+								o[2 * c + i][e] = fabsf(t[i][e]) <= 3.4e38f ? fmaf(t[i][e], 1.f / REST_LIFT, o[2 * c + i][e]) : o[2 * c + i][e];
+					}
+				}
+			} else if (high) { // both parts add to the same sums: neither is negative, nor 0 beside a probability that is not, so that an infinite value gives an infinity
 #pragma unroll
 				for (int i = 0; i < 4; i++) {
+					constexpr float LEAST = 1.17549435e-38f; // the smallest number that a product does not take for 0
 					float x[2];
 #pragma unroll
 					for (int e = 0; e < 2; e++) {
 						x[e] = ex2(fmaf(s[i >> 1][(i & 1) * 2 + e], c1, i & 1 ? b1 : b0));
 						if (i & 1) l1 += x[e];
-						x[e] = x[e] > 0.f ? fmaxf(x[e], tiny16<T>()) : x[e];
+						x[e] = x[e] > 0.f ? fmaxf(x[e], LEAST) : x[e];
 					}
-					pa[i] = cut16<T>(x[0], x[1]);
-					rest[i] = left16<T>(pa[i], x[0], x[1], tiny16<T>());
+					pa[i] = cut_bf16(x[0], x[1]);
+					const float2 left = rest16<T>(pa[i], x[0], x[1]);
+					rest[i] = pack16<T>(x[0] > 0.f ? fmaxf(left.x, LEAST) : left.x, x[1] > 0.f ? fmaxf(left.y, LEAST) : left.y);
 				}
 #pragma unroll
 				for (int c = 0; c < D / 16; c++) {
@@ -348,9 +376,9 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 #pragma unroll
 			for (int i = 0; i < D / 8; i++) // what an infinite value made infinite stays so: the rest may be 0 or negative
 #pragma unroll
-				for (int e = 0; e < 2; e++) o[i][e] = fabsf(o[i][e]) <= 3.4e38f ? o[i][e] + o[i][e + 2] : o[i][e];
-		m0 *= c1; // in units of log2 from here on
-		m1 *= c1;
+				for (int e = 0; e < 2; e++) o[i][e] = fabsf(o[i][e]) <= 3.4e38f ? fmaf(o[i][e + 2], HALF ? 1.f / REST_LIFT : 1.f, o[i][e]) : o[i][e];
+		m0 = fmaf(m0, c1, -LIFT); // in units of log2 from here on
+		m1 = fmaf(m1, c1, -LIFT);
 		// ---- the four warps' sums ----
 #pragma unroll
 		for (int w = 1; w < 4; w <<= 1) {
@@ -437,20 +465,20 @@ int mma_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists) {
 	return (D == 64 ? config_of<64>(c, b, n_lists) : D == 128 ? config_of<128>(c, b, n_lists) : config_of<256>(c, b, n_lists)).per_sm;
 }
 
-template <typename T, int D, bool LIST>
+template <typename T, int D, bool LIST, bool WIDE>
 static int launch_typed(const Attn& a, int part, int type, cudaStream_t s) {
 	const MmaConfig cfg = config_of<D>(a.c, a.b, LIST ? a.S : 0);
 	if (cfg.stages < 1) return set_error(XALM_ERR_INVALID, "paged attention: no shared memory left for pages beside %d sequences", a.b.B);
 	CUtensorMap kmap, vmap;
 	XALM_TRY(pool_map(a.c, type, true, &kmap));
 	XALM_TRY(pool_map(a.c, type, false, &vmap));
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_mma_kernel<T, D, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) cfg.smem));
-	XALM_CUDA_CHECK(launch(paged_mma_kernel<T, D, LIST>, a.part[part].grid, MT, cfg.smem, s, part > 0, a, a.part[part], kmap, vmap, cfg.stages));
+	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_mma_kernel<T, D, LIST, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) cfg.smem));
+	XALM_CUDA_CHECK(launch(paged_mma_kernel<T, D, LIST, WIDE>, a.part[part].grid, MT, cfg.smem, s, part > 0, a, a.part[part], kmap, vmap, cfg.stages));
 	return XALM_OK;
 }
 template <typename T, int D>
 static int launch_lists(const Attn& a, int part, int type, cudaStream_t s) {
-	return a.lists ? launch_typed<T, D, true>(a, part, type, s) : launch_typed<T, D, false>(a, part, type, s);
+	return !a.lists ? launch_typed<T, D, false, true>(a, part, type, s) : a.rep > 8 ? launch_typed<T, D, true, true>(a, part, type, s) : launch_typed<T, D, true, false>(a, part, type, s);
 }
 template <typename T>
 static int launch_size(const Attn& a, int part, int type, cudaStream_t s) {

@@ -12,7 +12,9 @@ namespace paged {
 // turns; one load of keys and values for 256 rows asks L2 for half of what 128 rows would.  One warp that issued both halves' products was what everything waited for:
 // a product takes 30 cycles to issue and a wait that is over 150 (2800 cycles a tile).
 // P lies in tensor memory where S lay (its first 32 columns), two S buffers to a half: the scores of the next tile are under way while this one's are worked on.
-// O accumulates unscaled and is rescaled only when a row's maximum has grown by more than 2^11.5 over the one its probabilities are taken against (fp16 holds those).
+// O accumulates unscaled and is rescaled only when a row's maximum has grown by more than 2^LAG over the one its probabilities are taken against.
+// Probabilities are rounded once to the cache's type (a second part would double the second product and want columns of tensor memory that there are none of); sums l are of the unrounded
+// ones.  fp16 ends at 2^-24, so its probabilities are lifted (Lift) and the maximum lags by less: those below 2^-27 of the row's largest lose bits, those below 2^-38 count in l alone.
 // V comes with its entries as the fast dimension, which the second product reads as it is (B transposed).
 // Tensor memory: S of half h, buffer b at columns 128 h + 64 b; O of half h at 256 + 128 h: the whole 512 of an SM, so heads of more than 128 entries stay on mma.sync.
 // What runs once to a piece is kept short and in loops: code that comes from memory for the first time costs more than it takes to run.
@@ -120,6 +122,15 @@ struct TcShared {
 	uint32_t tmem;
 	int dead, flag[2], ids[32];
 	float buf[2][256];
+};
+
+template <typename T>
+struct Lift { // in powers of two; fp16 ends at 2^16
+	static constexpr float BY = 0.f, LAG = 11.5f;
+};
+template <>
+struct Lift<__half> {
+	static constexpr float BY = 13.f, LAG = 2.9f;
 };
 
 template <typename T>
@@ -304,7 +315,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				for (int i = 8; i < KT; i++) m8[i & 7] = fmaxf(m8[i & 7], __uint_as_float(s[i]));
 				float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
 				mx *= c1;
-				const bool grow = mx > m + 11.5f;
+				const bool grow = mx > m + Lift<T>::LAG;
 				if (j == 0) m = mx;
 				else if (__any_sync(0xffffffffu, grow)) { // rare: the sums so far are complete before they are rescaled
 					ok = wait_for(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c) && ok;
@@ -323,7 +334,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 					l *= f;
 					m = to;
 				}
-				const float nm = m == -INFINITY ? 0.f : -m;
+				const float nm = m == -INFINITY ? 0.f : Lift<T>::BY - m;
 				const f32x2 c2 = pack2(c1, c1), n2 = pack2(nm, nm);
 				f32x2 sum[4] = {pack2(0.f, 0.f), pack2(0.f, 0.f), pack2(0.f, 0.f), pack2(0.f, 0.f)};
 				uint32_t q[KT / 2];
@@ -354,6 +365,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // 32 rows of 128 bytes
 			const bool any = l > 0.f || l != l;
 			const float inv = direct ? (any ? 1.f / l : 0.f) : 1.f;
+			m -= Lift<T>::BY;
 			if (mine) {
 				if (!direct) {
 					if (slot < part.slots) part.ml[slot * TC_ROWS + row] = make_float2(m, l);
