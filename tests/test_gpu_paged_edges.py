@@ -6,7 +6,7 @@ import torch
 
 from paged_ref import Problem
 from test_gpu_paged import near
-from xalm_b200 import paged
+from xalm_b200 import capi, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,65 @@ def test_an_infinite_value_of_a_small_probability_gives_an_infinity(below, rep, 
         cache, batch = p.on_gpu()
         out = paged.attend(cache, batch, p.gq, p.scale)
         assert (out[:, :, 7] == bad).all() and torch.isfinite(out[:, :, :7]).all() and torch.isfinite(out[:, :, 8:]).all()
+
+
+# ---- calls from several threads ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+def test_calls_of_different_sizes_in_several_threads(type):
+    """Each thread has a batch of its own number of sequences, length of lists and width of tables, so that no two calls want the same shared memory."""
+    from concurrent.futures import ThreadPoolExecutor
+    rounds, jobs = 150, []
+    for seqs, top, width in ((3, 4, 900), (400, 40, 1500), (1500, 200, 3000), (2500, 600, 700)):
+        p = Problem(type, [1] * seqs, [i % 200 + 1 for i in range(seqs)], G=2, rep=3, d=64, page=16, seed=62)
+        p.means = p.normal(p.pages, p.G, p.d)
+        p.table = torch.cat([p.table, torch.full((seqs, width - p.max_pages), -1, dtype=torch.int32)], dim=1)
+        p.max_pages = width
+        cache, batch = p.on_gpu()
+
+        def serve(cache=cache, batch=batch, q=p.gq, top=top, scale=p.scale):
+            lists = paged.select(cache, batch, q, top)
+            return lists, paged.attend(cache, batch, q, scale), paged.attend_selected(cache, batch, q, lists, scale)
+
+        jobs.append((serve, serve(), cache))
+    torch.cuda.synchronize()
+
+    def thread(job):
+        serve, want, _ = job
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for n in range(rounds):
+                got = serve()
+                stream.synchronize()
+                assert all(torch.equal(x, y) for x, y in zip(got, want)), n
+        return rounds
+
+    with ThreadPoolExecutor(len(jobs)) as pool:
+        assert list(pool.map(thread, jobs)) == [rounds] * len(jobs)
+    for *_, cache in jobs:
+        cache.check()
+
+
+def test_no_call_takes_shared_memory_from_another():
+    """The same kernel launched from two threads with more and with less shared memory, as fast as the calls go."""
+    from concurrent.futures import ThreadPoolExecutor
+    L, jobs = capi.lib(), []
+    for width in (24000, 7000):
+        p = Problem("bf16", [1], [40], G=1, rep=1, d=64, page=16, seed=63, max_pages=width)
+        p.means = p.normal(p.pages, p.G, p.d)
+        cache, batch = p.on_gpu()
+        batch.c.rows = 1
+        jobs.append((cache, batch, p.gq, torch.empty(1, 1, 4, dtype=torch.int32, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def thread(job):
+        cache, batch, q, out, stream = job
+        args = cache.p, batch.p, q.data_ptr(), 64, 1, 4, 1, 1, out.data_ptr(), stream.cuda_stream
+        refused = sum(L.xalm_cuda_paged_select(*args) != 0 for _ in range(20000))
+        stream.synchronize()
+        return refused
+
+    with ThreadPoolExecutor(2) as pool:
+        assert list(pool.map(thread, jobs)) == [0, 0]
+    for cache, _, _, out, _ in jobs:
+        assert out.flatten().tolist() == [0, 1, 2, -1]
+        cache.check()

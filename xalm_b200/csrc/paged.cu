@@ -625,7 +625,7 @@ static int select_typed(const SelectArgs& a, int sms, cudaStream_t s) {
 	const size_t smem = (size_t) R * a.b.max_pages * 8 + (R > 1 ? (size_t) (R * a.c.d + SP * (a.c.d + 4) + R * a.c.d / 8 + ST / 32 + a.b.max_pages) * 4 : 0);
 	const dim3 grid((unsigned) (R > 1 ? a.b.N / R + a.b.B : a.b.N), (unsigned) a.c.G);
 	void (*kernel)(SelectArgs) = R == 16 ? paged_select_rows_kernel<T, 16> : R == 8 ? paged_select_rows_kernel<T, 8> : paged_select_step_kernel<T>;
-	if (smem > 48 * 1024) XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	if (smem > 48 * 1024) XALM_CUDA_CHECK(allow_smem((const void*) kernel, 2048));
 	kernel<<<grid, ST, smem, s>>>(a);
 	XALM_CUDA_CHECK(cudaGetLastError());
 	return XALM_OK;

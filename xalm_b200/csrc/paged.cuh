@@ -515,6 +515,9 @@ __device__ __forceinline__ int list_pages(const Attn& a, int row, int g, int own
 	return n;
 }
 
+// A kernel's limit of dynamic shared memory is the process's: it is set to the same number by every call, whatever the call needs, so that none lowers it between another thread's
+// setting and launch.  own: shared memory that the kernel declares
+inline cudaError_t allow_smem(const void* kernel, int own = 0) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - own); }
 // Launches; `after`: may start while the kernel before it on the stream still runs (it waits for it itself).
 template <typename K, typename... A>
 inline cudaError_t launch(K kernel, dim3 grid, int block, size_t smem, cudaStream_t s, bool after, const A&... args) {

@@ -532,7 +532,7 @@ static int rows_cols(const Attn& a, cudaStream_t s) {
 	const int buffers = rows_buffers(a.c, a.b, a.S);
 	const size_t smem = rows_smem(a.c, a.b, a.S, buffers);
 	auto kernel = a.lists ? paged_rows_kernel<COLS, true> : paged_rows_kernel<COLS, false>;
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	XALM_CUDA_CHECK(allow_smem((const void*) kernel));
 	XALM_CUDA_CHECK(launch(kernel, a.part[0].grid, RT, smem, s, false, a, buffers));
 	return XALM_OK;
 }

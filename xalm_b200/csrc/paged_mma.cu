@@ -472,7 +472,7 @@ static int launch_typed(const Attn& a, int part, int type, cudaStream_t s) {
 	CUtensorMap kmap, vmap;
 	XALM_TRY(pool_map(a.c, type, true, &kmap));
 	XALM_TRY(pool_map(a.c, type, false, &vmap));
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_mma_kernel<T, D, LIST, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) cfg.smem));
+	XALM_CUDA_CHECK(allow_smem((const void*) paged_mma_kernel<T, D, LIST, WIDE>));
 	XALM_CUDA_CHECK(launch(paged_mma_kernel<T, D, LIST, WIDE>, a.part[part].grid, MT, cfg.smem, s, part > 0, a, a.part[part], kmap, vmap, cfg.stages));
 	return XALM_OK;
 }

@@ -468,7 +468,7 @@ static int launch_typed(const Attn& a, int part, int type, cudaStream_t s) {
 		XALM_TRY(encode_map(&qmap, type, 4, const_cast<uint8_t*>(a.q), dims, strides, box));
 	}
 	const size_t smem = tc_smem(a.b);
-	XALM_CUDA_CHECK(cudaFuncSetAttribute(paged_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+	XALM_CUDA_CHECK(allow_smem((const void*) paged_tc_kernel<T>));
 	XALM_CUDA_CHECK(launch(paged_tc_kernel<T>, a.part[part].grid, TT, smem, s, false, a, a.part[part], kmap, vmap, qmap));
 	return XALM_OK;
 }
