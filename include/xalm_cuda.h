@@ -312,6 +312,8 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  *   over, a page counts once.
  * Both attend in one pass: scores, maxima and sums in fp32; 16-bit caches' probabilities enter the second product as two numbers of the cache's type where a segment has up to 16
  *   (token, head) rows to a kv head, as one of them where it has more.  The same call gives the same bits every time.
+ * paged_status: *taken (device memory) becomes the status word, which becomes 0, in one exchange behind what the stream holds: a bit that a kernel sets at the same time is in this word or
+ *   stays for the next.  What other streams hold has reported when they are done.
  * paged_workspace: bytes of workspace (at a 256-byte boundary) that paged_attend (n_lists 0) and paged_attend_selected need for these sizes; its contents need no preparation. */
 typedef struct xalm_paged_cache {
 	int type, device;
@@ -337,6 +339,7 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
                            int* out, void* cuda_stream);
 int xalm_cuda_paged_attend_selected(const xalm_paged_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, const int* lists,
                                     int n_lists, float scale, void* out, long long out_row, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream);
+int xalm_cuda_paged_status(const xalm_paged_cache* cache, int* taken, void* cuda_stream);
 int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_batch* batch, int heads, int n_lists, size_t* bytes);
 
 /* Tensor parallel plumbing (no reference analogue).  Rank 0 makes an id, the host side ships it to

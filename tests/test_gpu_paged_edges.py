@@ -155,3 +155,58 @@ def test_no_call_takes_shared_memory_from_another():
     for cache, _, _, out, _ in jobs:
         assert out.flatten().tolist() == [0, 1, 2, -1]
         cache.check()
+
+
+# ---- what kernels report -----------------------------------------------------------------------------------------------------------------------
+def test_check_waits_for_every_stream():
+    p = Problem("bf16", [1], [20], d=64, page=16, seed=64)
+    cache, batch = p.on_gpu()
+    batch.tensors[2][0, 1] = p.pages
+    rows = torch.zeros(1, p.G, 64, dtype=p.t, device="cuda")
+    paged.append(cache, batch, rows, rows)  # the kernel is in memory before it has to run late
+    with pytest.raises(capi.XalmError, match="names a page"):
+        cache.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+        paged.append(cache, batch, rows, rows)
+    with pytest.raises(capi.XalmError, match="names a page"):
+        cache.check()
+    cache.check()
+
+
+def test_no_report_is_lost_while_others_are_read():
+    """One thread keeps reading the word, another keeps reporting: every report is in what was read or still there."""
+    import threading
+    p = Problem("bf16", [1], [20], d=64, page=16, seed=65)
+    cache, batch = p.on_gpu()
+    batch.tensors[2][0, 1] = p.pages
+    rows = torch.zeros(1, p.G, 64, dtype=p.t, device="cuda")
+    done, raised = threading.Event(), []
+
+    def read():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            while not done.is_set():
+                try:
+                    cache.check()
+                except capi.XalmError:
+                    raised.append(1)
+
+    torch.cuda.synchronize()
+    reader = threading.Thread(target=read)
+    reader.start()
+    seen = 0
+    for n in range(300):
+        before = len(raised)
+        paged.append(cache, batch, rows, rows)
+        for _ in range(2000):  # a report appears in at most a check that is under way and the one after it
+            if len(raised) > before:
+                break
+            done.wait(0.001)
+        seen += len(raised) > before
+        if seen <= n:
+            break
+    done.set()
+    reader.join()
+    assert seen == 300

@@ -124,6 +124,7 @@ SYMBOLS = {
     "xalm_cuda_paged_attend": (_i, [_vp, _vp, _vp, C.c_longlong, _i, C.c_float, _vp, C.c_longlong, _vp, _vp, _sz, _vp]),
     "xalm_cuda_paged_select": (_i, [_vp, _vp, _vp, C.c_longlong, _i, _i, _i, _i, _vp, _vp]),
     "xalm_cuda_paged_attend_selected": (_i, [_vp, _vp, _vp, C.c_longlong, _i, _vp, _i, C.c_float, _vp, C.c_longlong, _vp, _vp, _sz, _vp]),
+    "xalm_cuda_paged_status": (_i, [_vp, _vp, _vp]),
     "xalm_cuda_paged_workspace": (_i, [_vp, _vp, _i, _i, C.POINTER(_sz)]),
 }
 PRECISION_BF16, PRECISION_F32 = 0, 1            # enum xalm_precision

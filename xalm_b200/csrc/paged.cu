@@ -631,6 +631,8 @@ static int select_typed(const SelectArgs& a, int sms, cudaStream_t s) {
 	return XALM_OK;
 }
 
+__global__ void paged_status_kernel(int* status, int* taken) { *taken = atomicExch(status, 0); }
+
 // ---- checks and launches -----------------------------------------------------------------------------------------------------------------------
 static int element_bytes(int type) { return type == XALM_F32 ? 4 : 2; }
 static bool is_type(int type) { return type == XALM_F32 || type == XALM_F16 || type == XALM_BF16; }
@@ -905,6 +907,17 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 		cfg.numAttrs = 1;
 		XALM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, means, a.c, a.b));
 	}
+	return XALM_OK;
+}
+
+int xalm_cuda_paged_status(const xalm_paged_cache* cache, int* taken, void* stream) {
+	Cache c;
+	XALM_TRY(check_cache(cache, c));
+	if (!taken || !c.status) return set_error(XALM_ERR_INVALID, "paged status: %s is NULL", taken ? "the cache's status word" : "taken");
+	OnDevice on;
+	XALM_TRY(on.set(cache->device));
+	paged_status_kernel<<<1, 1, 0, (cudaStream_t) stream>>>(c.status, taken);
+	XALM_CUDA_CHECK(cudaGetLastError());
 	return XALM_OK;
 }
 

@@ -71,9 +71,11 @@ class PagedCache:
         self.p = C.addressof(self.c)
 
     def check(self):
-        """Waits for the device and raises what its kernels have reported since the last check."""
-        bits = int(self.status.item())
-        self.status.zero_()
+        """Waits for the device, all its streams, and raises what its kernels have reported since the last check.  Not while a graph is captured."""
+        torch.cuda.synchronize(self.device)
+        taken = torch.empty_like(self.status)
+        capi.check(capi.lib().xalm_cuda_paged_status(self.p, taken.data_ptr(), _stream(self.index)))
+        bits = int(taken.item())
         if bits:
             _refuse("paged cache: " + " and ".join(t for b, t in ((1, "a table names a page outside the pool"), (2, "starts, lens and table do not fit"), (4, "a kernel gave up a wait for its copies or products")) if bits & b))
 
