@@ -290,7 +290,7 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  *   128 or 256 slots; dim, vdim multiples of 8, at most 256.  Strides in ELEMENTS, entries of a head are neighbours: slots within heads or heads within slots, each stride a multiple
  *   of 16 bytes; pools at 16-byte boundaries.  means (pages, kv_heads, dim), dense, or NULL: the mean of a page's keys, kept for every page whose last
  *   slot was appended.  status: one int or NULL; kernels set bit 0 where a table named a page outside the pool (such a page reads as zeros and is not written) and bit 1
- *   where starts, lens and the table do not fit one another (lengths are cut to the table; where starts or groups do not ascend, paged_attend computes nothing), bit 2 where a
+ *   where starts, lens and the table do not fit one another (lengths are cut to the table, and paged_append writes no key or value behind it; where starts or groups do not ascend, paged_attend computes nothing), bit 2 where a
  *   kernel gave up a wait that should have taken microseconds (the call's results are not to be used); nothing else reports what is only known on the device.
  * xalm_paged_batch: rows starts[s] .. starts[s + 1] - 1 are the new tokens of sequence s, lens[s] its tokens, the new ones included: row starts[s] + i is at position
  *   lens[s] - n + i.  starts has seqs + 1 entries; rows outside [starts[0], starts[seqs]) of `rows` are left alone.  table (seqs, max_pages), rows table_row apart.

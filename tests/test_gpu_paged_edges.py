@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from paged_ref import Problem
+from paged_ref import F32, HALF, Problem
 from test_gpu_paged import near
 from xalm_b200 import capi, paged
 
@@ -210,3 +210,49 @@ def test_no_report_is_lost_while_others_are_read():
     done.set()
     reader.join()
     assert seen == 300
+
+
+# ---- lengths beyond the table ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new,over", [([1, 1], [1, 0]), ([40, 3], [2, 0]), ([20, 700], [0, 650]), ([5, 2], [5, 2 ** 31 - 1 - 64])])
+def test_append_writes_nothing_behind_the_table_and_no_other_slots_instead(new, over, type):
+    """Tokens that the table has no page for are reported and left out; the others go where they belong, and every query is turned by its own position."""
+    page, cap = 16, 64
+    p = Problem(type, new, [cap, cap], d=64, page=page, seed=66)
+    p.means = p.normal(p.pages, p.G, p.d)
+    cache, batch = p.on_gpu()
+    lens = [cap + x for x in over]
+    batch.tensors[1].copy_(torch.tensor(lens, dtype=torch.int32))
+    kn, vn, qn = p.normal(p.rows, p.G, 64), p.normal(p.rows, p.G, 64), p.normal(p.rows, p.H, 64)
+    freq = torch.zeros(32)  # no turn but for the first pair's
+    freq[0] = 2.0 ** -9
+    out = paged.append(cache, batch, kn.cuda(), vn.cuda(), q=qn.cuda(), freq=freq.cuda())
+    with pytest.raises(capi.XalmError, match="do not fit"):
+        cache.check()
+    cache.check()
+    k, v, full = p.k.clone(), p.v.clone(), set()
+    angle = torch.zeros(p.rows, dtype=torch.float64)
+    for s in range(2):
+        for i in range(new[s]):
+            pos = lens[s] - new[s] + i
+            angle[p.starts[s] + i] = pos * 2.0 ** -9
+            if pos < cap:
+                at = p.slots(s, pos)
+                k[at], v[at] = kn[p.starts[s] + i], vn[p.starts[s] + i]
+                k[at + (slice(None), 0)] = math.nan  # turned: looked at below only
+                k[at + (slice(None), 32)] = math.nan
+                if pos % page == page - 1:
+                    full.add(int(p.table[s, pos // page]))
+    got, same = p.gk.cpu(), ~torch.isnan(k)
+    assert torch.equal(got[same], k[same]) and torch.equal(p.gv.cpu(), v)
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    x, y = qn[:, :, 0].double(), qn[:, :, 32].double()
+    want = torch.stack([x * c - y * s, y * c + x * s], dim=-1)
+    near(out[:, :, [0, 32]], want, want.abs() * HALF[type] + 8 * F32 * (x.abs() + y.abs())[..., None] + 2.0 ** -25)
+    means = cache.means.cpu()
+    for n in range(p.pages):
+        if n in full:
+            exact = got[n].double().mean(dim=0)
+            near(means[n], exact, exact.abs() * HALF[type] + (page + 2) * F32 * got[n].double().abs().mean(dim=0) + 2.0 ** -25)
+        else:
+            assert torch.equal(means[n], p.means[n])

@@ -66,8 +66,8 @@ __global__ void __launch_bounds__(AT) paged_append_kernel(const __grid_constant_
 			const View view = view_of(a.c, a.b);
 			const Seq q = seq_of(view, s);
 			if (row_in_seq(q, row)) {
-				pos = q.len - q.n + row - q.a;
-				if (pos >= 0) {
+				pos = max(a.b.lens[s], 0) - q.n + row - q.a; // not cut to the table: what lies behind it is turned, and written nowhere
+				if (pos >= 0 && pos < view.cap) {
 					page = page_of(a.c, a.b, s, pos >> a.c.shift);
 					if (page < 0 && (tid & 31) == 0) report(a.c, ERR_PAGE);
 				}
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(128) paged_means_kernel(const Cache c, const B
 		n = min(step, n - k * step);
 	}
 	const Seq q = seq_of(view_of(c, b), lo);
-	const int first = max(q.len - q.n, 0) >> c.shift; // page of the first new token
+	const int first = max(max(b.lens[lo], 0) - q.n, 0) >> c.shift; // page of the first new token
 	const int j = first + item - ((q.a >> c.shift) + lo);
 	if (q.n == 0 || j < first || (long long) (j + 1) << c.shift > q.len) return; // not filled
 	const int page = page_of(c, b, lo, j);
