@@ -256,3 +256,31 @@ def test_append_writes_nothing_behind_the_table_and_no_other_slots_instead(new, 
             near(means[n], exact, exact.abs() * HALF[type] + (page + 2) * F32 * got[n].double().abs().mean(dim=0) + 2.0 ** -25)
         else:
             assert torch.equal(means[n], p.means[n])
+
+
+# ---- scores at the ends of fp32 ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("new,pages", [([1, 1], 40), ([1, 1], 700), ([150, 3], 40), ([150, 3], 300)])
+def test_select_where_sums_leave_the_range_of_fp32(new, pages, type):
+    """Sums that overflow on their way to an ordinary number, and numbers whose products fp32 rounds to 0, are in the order of 64 bits."""
+    p = Problem(type, new, [new[0] + 600, new[1] + 550], G=2, rep=1, d=64, page=16, seed=67)
+    p.table = torch.cat([p.table.clamp_min(0)] * (pages // p.max_pages + 1), dim=1)[:, :pages].contiguous()
+    p.max_pages = pages
+    p.lens = [pages * 16, pages * 16 - 9]
+
+    def same(means, q, tops):
+        p.means, p.q = means.to(p.t), q.to(p.t)
+        cache, batch = p.on_gpu()
+        for top in tops:
+            assert torch.equal(paged.select(cache, batch, p.gq, top).cpu(), p.select(p.means, top, 1, 1))
+
+    rand = lambda *s: torch.randn(*s, generator=p.gen)
+    means, q = rand(p.pages, p.G, 64), torch.ones(p.rows, p.H, 64)
+    means[::7], means[3::7] = 0.0, 0.0  # scores of 0, whatever the order of the sum
+    means[::7, :, :4] = torch.tensor([2.0e38, 2.0e38, -2.0e38, -2.0e38])
+    means[3::7, :, 8:12] = torch.tensor([-2.0e38, -2.0e38, 2.0e38, 2.0e38])
+    same(means, q, (3, 20))
+    same(means, -q, (9,))
+    # 2^-75 times 2^-80, and sums just above the smallest number
+    same(rand(p.pages, p.G, 64) * 2.0 ** -75, rand(p.rows, p.H, 64) * 2.0 ** -80, (9,))
+    same(rand(p.pages, p.G, 64) * 2.0 ** -70, rand(p.rows, p.H, 64) * 2.0 ** -76, (9,))

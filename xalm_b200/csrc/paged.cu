@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(128) paged_means_kernel(const Cache c, const B
 // select: score_j = (sum over the kv head's queries) . mean_j, and of the pages between the first and the recent ones those with the largest scores, equal ones from the lowest
 // place on.  Which page is the last to be taken must not hang on how a sum was rounded, and sums in 64 bits cost a conversion per mean and row (279 us for 1341
 // tokens of 8 heads over 110 to 235 pages, which take 56 now).  So scores are taken in fp32, each off by at most E = (d + rep + 4) 2^-24 sum_i (sum_r |q_ri|) max |mean|; of the want-th largest, t, the true
-// one is off by no more than E, so pages above t + 2 E are taken, those below t - 2 E are not, and only where those between are more than are wanted are they summed in 64 bits.
+// one is off by no more than E (no E holds where fp32 may overflow: all are summed in 64 bits then), so pages above t + 2 E are taken, those below t - 2 E are not, and only where those between are more than are wanted are they summed in 64 bits.
 // Steps of single tokens: a CTA to (row, kv head), 8 lanes to a page.  Longer ones: R rows of a sequence to a CTA, so that a page's mean is read and converted once for
 // all of them: 64 pages at a time in shared memory, a thread taking one page and R / 4 rows; then a warp to a row.  The want-th largest is found bit by bit from above, up to 512 keys in a warp's registers.
 // =========================================================================================================================================
@@ -436,8 +436,10 @@ __device__ __forceinline__ unsigned grow_bound(unsigned m, const float (&v)[8]) 
 	for (int e = 0; e < 8; e++) m = max(m, (unsigned) __float_as_int(v[e]) & 0x7fffffffu);
 	return m;
 }
+// No bound where a sum may leave the range of fp32 on its way; products and sums below its normal numbers are off by half of the smallest each
 __device__ __forceinline__ float score_error(int d, int rep, float abs_q, unsigned most) {
-	return most >= 0x7f800000u ? INFINITY : 1.1f * (float) (d + rep + 4) * 5.9604645e-8f * abs_q * __int_as_float((int) most);
+	const float size = abs_q * __int_as_float((int) most);
+	return most >= 0x7f800000u || !(size < 3.0e38f) ? INFINITY : 1.1f * (float) (d + rep + 4) * 5.9604645e-8f * size + (float) (d + 4) * 1.4e-45f;
 }
 
 template <typename T>
