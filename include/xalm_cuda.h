@@ -301,8 +301,8 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  * paged_append: k (rows, kv_heads dim), v (rows, kv_heads vdim), q (rows, heads dim) of in_type; the first 2 rot_half entries of every head of k and q are turned by
  *   position * freq[i] (entry i with i + rot_half, or with `neighbours` 2 i with 2 i + 1; cos and sin times rot_mag); keys and values go to their pages, queries to q_out
  *   in the cache's type, rounded once.  q NULL: keys and values only.  Then the mean keys of the pages that are full now.
- *   q_out may be q itself where both have the cache's type and rot_half is a multiple of 8 or the pairs are neighbours; else they do not overlap, and out does not overlap q in
- *   the attending calls.  Two rows that a table sends to the same slot leave either's key and value there.
+ *   q_out may be q itself where both have the cache's type and rot_half is a multiple of 8 or the pairs are neighbours; else they do not overlap.  Rows of q, k and v may lie side by side in one array.  What a call writes
+ *   (q_out, out, lse, the workspace) lies apart from all else that it is given; of the pools, which append writes, the caller sees to that.  Two rows that a table sends to the same slot leave either's key and value there.
  * paged_attend: out[row, h] = sum_j softmax_j(scale q . k_j) v_j over the positions j up to the row's own; rows that see nothing give zeros.  lse (rows, heads): the logarithm of the
  *   softmax's denominator (-infinity where a row sees nothing), or NULL.
  * paged_select: for every row and kv head `top` pages by their place in the sequence, ascending, -1 behind them: the row's own page, the `recent` before it, the `first`

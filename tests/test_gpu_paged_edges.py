@@ -284,3 +284,54 @@ def test_select_where_sums_leave_the_range_of_fp32(new, pages, type):
     # 2^-75 times 2^-80, and sums just above the smallest number
     same(rand(p.pages, p.G, 64) * 2.0 ** -75, rand(p.rows, p.H, 64) * 2.0 ** -80, (9,))
     same(rand(p.pages, p.G, 64) * 2.0 ** -70, rand(p.rows, p.H, 64) * 2.0 ** -76, (9,))
+
+
+# ---- arrays that lie in one another ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_results_that_overlap_what_a_call_is_given_are_refused(type):
+    """Nothing is launched for them; rows side by side in one array are taken."""
+    p = Problem(type, [1, 4], [30, 40], d=64, page=16, seed=68, groups=([0, 2], [16]))
+    p.means = p.normal(p.pages, p.G, p.d)
+    cache, batch = p.on_gpu()
+    L, n, H, G, row = capi.lib(), p.rows, p.H, p.G, p.H * 64
+    new = lambda *s, dtype=p.t: torch.zeros(*s, dtype=dtype, device="cuda")
+    k, v, q, out, freq, lse, lists = new(n, G, 64), new(n, G, 64), new(n, H, 64), new(n, H, 64), new(32, dtype=torch.float32), new(n, H, dtype=torch.float32), new(n, G, 4, dtype=torch.int32)
+    work = new(1 << 27, dtype=torch.uint8)
+    bp = batch.of(n)[0]
+    at = lambda t: t.data_ptr()
+
+    def append(q_out):
+        return L.xalm_cuda_paged_append(cache.p, bp, at(k), G * 64, at(v), G * 64, at(q), row, H, cache.c.type, q_out, row, at(freq), 32, 1.0, 0, None)
+
+    def attend(out, lse, work):
+        return L.xalm_cuda_paged_attend(cache.p, bp, at(q), row, H, 0.1, out, row, lse, work, 1 << 26, None)
+
+    def selected(out, lse, work):
+        return L.xalm_cuda_paged_attend_selected(cache.p, bp, at(q), row, H, at(lists), 4, 0.1, out, row, lse, work, 1 << 26, None)
+
+    def select(out):
+        return L.xalm_cuda_paged_select(cache.p, bp, at(q), row, H, 4, 1, 1, out, None)
+
+    fixed = [p.gk, p.gv, cache.means, cache.status, *batch.tensors]
+    for x in fixed + [q]:
+        low, end = at(x) // 256 * 256, at(x) + (x.numel() - 1) * x.element_size()
+        for here in (at(x), low, end // 16 * 16):
+            calls = [attend(here, at(lse), at(work)), selected(here, at(lse), at(work)), attend(at(out), here, at(work)), selected(at(out), here, at(work)), select(here)]
+            assert calls == [1] * 5 and (x is q or append(here) == 1), (x.shape, calls)
+        assert attend(at(out), at(lse), low) == 1 and selected(at(out), at(lse), low) == 1
+    for here in (at(k), at(v) + 16, at(freq)):
+        assert append(here) == 1
+    assert selected(at(lists), at(lse), at(work)) == 1 and selected(at(out), at(lists), at(work)) == 1 and attend(at(out), at(out), at(work)) == 1
+    assert attend(at(work), at(lse), at(work)) == 1 and attend(at(out), at(work) + 4096, at(work)) == 1
+    assert b"overlaps" in L.xalm_cuda_last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(p.gk.cpu(), p.k) and torch.equal(p.gv.cpu(), p.v)
+    assert append(at(out)) == attend(at(out), at(lse), at(work)) == select(at(lists)) == selected(at(out), at(lse), at(work)) == 0
+    # one projection's rows, queries turned where they are
+    qkv = torch.randn(n, H + 2 * G, 64, generator=p.gen).to(p.t).cuda()
+    qs, ks, vs = qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:]
+    want = paged.append(cache, batch, ks.clone(), vs.clone(), q=qs.clone(), freq=freq)
+    assert torch.equal(paged.append(cache, batch, ks, vs, q=qs, freq=freq, q_out=qs), want)
+    with pytest.raises(capi.XalmError, match="overlaps k or v"):
+        paged.append(cache, batch, ks, vs, q=q, freq=freq, q_out=qkv[:, 1:H + 1])
+    cache.check()

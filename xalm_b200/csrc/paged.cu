@@ -692,6 +692,32 @@ static bool rows_meet(const void* p, long long p_row, long long p_bytes, const v
 	return at < p_bytes || at + q_bytes > p_row;
 }
 
+// What a call writes lies apart from what it reads and from what else it writes
+struct Span {
+	const char* what;
+	const void* at;
+	long long bytes;
+};
+static Span rows_span(const char* what, const void* p, long long row, long long width, int n, int bytes) { return Span{what, p, ((n - 1) * row + width) * bytes}; }
+static Span pool_span(const char* what, const Cache& c, const void* p, int dim, int e, long long page, long long slot, long long head) {
+	return Span{what, p, ((c.pages - 1) * page + ((1 << c.shift) - 1) * slot + (c.G - 1) * head + dim) * e};
+}
+template <int N>
+static int check_apart(const char* call, const Span& out, const Span (&others)[N]) {
+	const uintptr_t a = (uintptr_t) out.at;
+	for (const Span& x : others) {
+		const uintptr_t b = (uintptr_t) x.at;
+		if (a && b && out.bytes > 0 && x.bytes > 0 && a < b + x.bytes && b < a + out.bytes) return set_error(XALM_ERR_INVALID, "%s: %s overlaps %s", call, out.what, x.what);
+	}
+	return XALM_OK;
+}
+static int check_apart_from_cache(const char* call, const Span& out, const Cache& c, const BatchView& b, int e) {
+	return check_apart(call, out, {pool_span("the keys' pool", c, c.k, c.d, e, c.k_page, c.k_slot, c.k_head), pool_span("the values' pool", c, c.v, c.dv, e, c.v_page, c.v_slot, c.v_head),
+	                               Span{"the mean keys", c.means, (long long) c.pages * c.G * c.d * e}, Span{"the status word", c.status, 4}, Span{"starts", b.starts, 4ll * (b.B + 1)},
+	                               Span{"lens", b.lens, 4ll * b.B}, rows_span("the table", b.table, b.table_row, b.max_pages, b.B, 4),
+	                               Span{"group_bounds", b.bounds, 4ll * (b.n_groups + 1)}, Span{"group_shared", b.shared, 4ll * b.n_groups}});
+}
+
 // The calling thread's device is what it was when the call returns
 struct OnDevice {
 	int before = -1;
@@ -798,6 +824,14 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 	if (!workspace || ((uintptr_t) workspace & 255)) return set_error(XALM_ERR_INVALID, "paged attention: the workspace is NULL or not at a 256-byte boundary");
 	XALM_TRY(plan_attn(cache, c, b, heads, n_lists, a, &need));
 	if (rows_meet(q, q_row * e, (long long) heads * c.d * e, out, out_row * e, (long long) heads * c.dv * e, b.N)) return set_error(XALM_ERR_INVALID, "paged attention: out overlaps q");
+	{
+		const Span sq = rows_span("q", q, q_row, heads * c.d, b.N, e), so = rows_span("out", out, out_row, heads * c.dv, b.N, e), sl = {"lse", lse, 4ll * b.N * heads},
+		           sp = {"the lists", lists, 4ll * b.N * c.G * n_lists}, sw = {"the workspace", workspace, (long long) need};
+		for (const Span& x : {so, sl, sw}) XALM_TRY(check_apart_from_cache("paged attention", x, c, b, e));
+		XALM_TRY(check_apart("paged attention", sw, {sq, so, sl, sp}));
+		XALM_TRY(check_apart("paged attention", sl, {sq, so, sp}));
+		XALM_TRY(check_apart("paged attention", so, {sp}));
+	}
 	if (workspace_bytes < need) return set_error(XALM_ERR_INVALID, "paged attention: a workspace of %zu bytes is needed, %zu given", need, workspace_bytes);
 	OnDevice on;
 	XALM_TRY(on.set(cache->device));
@@ -875,6 +909,15 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 	a.by_value = (unsigned) ((0x100000000ull + a.per_value - 1) / a.per_value);
 	int sms = 0;
 	XALM_TRY(sm_count(cache->device, &sms));
+	if (q) {
+		const int ei = element_bytes(in_type), e = element_bytes(cache->type);
+		const long long width = (long long) heads * a.c.d * e;
+		const Span out = rows_span("q_out", q_out, q_out_row, heads * a.c.d, a.b.N, e);
+		XALM_TRY(check_apart_from_cache("paged append", out, a.c, a.b, e));
+		XALM_TRY(check_apart("paged append", out, {Span{"freq", freq, 4ll * rot_half}}));
+		if (rows_meet(k, k_row * ei, (long long) a.c.G * a.c.d * ei, q_out, q_out_row * e, width, a.b.N) || rows_meet(v, v_row * ei, (long long) a.c.G * a.c.dv * ei, q_out, q_out_row * e, width, a.b.N))
+			return set_error(XALM_ERR_INVALID, "paged append: q_out overlaps k or v");
+	}
 	// Four rows to a CTA once that still gives every SM one.  32 and 8 heads of 128, one and four rows to a CTA: 256 rows 4.5 and 5.9 us, 576 4.9 and 5.9, 1024 8.0 and 7.1, 8192 43 and 39
 	const bool many = a.b.N >= sms * 4;
 	void (*kernel)(AppendArgs) = nullptr;
@@ -969,6 +1012,12 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
 	a.first = first;
 	int sms = 0;
 	XALM_TRY(sm_count(cache->device, &sms));
+	{
+		const int e = element_bytes(cache->type);
+		const Span so = {"out", out, 4ll * a.b.N * a.c.G * top};
+		XALM_TRY(check_apart_from_cache("paged select", so, a.c, a.b, e));
+		XALM_TRY(check_apart("paged select", so, {rows_span("q", q, q_row, heads * a.c.d, a.b.N, e)}));
+	}
 	a.recent = recent;
 	a.out = out;
 	cudaStream_t s = (cudaStream_t) stream;
