@@ -295,7 +295,7 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  * xalm_paged_batch: rows starts[s] .. starts[s + 1] - 1 are the new tokens of sequence s, lens[s] its tokens, the new ones included: row starts[s] + i is at position
  *   lens[s] - n + i.  starts has seqs + 1 entries; rows outside [starts[0], starts[seqs]) of `rows` are left alone.  table (seqs, max_pages), rows table_row apart.
  *   Sequences group_bounds[i] .. group_bounds[i + 1] - 1 (ascending) have the same pages for their first group_shared[i] tokens: those are read once for all of
- *   them; what a call computes does not depend on it but for the order of its sums.  At most 4096 sequences and groups, tables of at most 2^30 tokens.
+ *   them that have new tokens (the others, idle places of a captured batch, need no pages); what a call computes does not depend on it but for the order of its sums.  At most 4096 sequences and groups, tables of at most 2^30 tokens.
  * Rows of arrays are `*_row` elements apart and begin at 16-byte boundaries; heads within a row are dense.
  *
  * paged_append: k (rows, kv_heads dim), v (rows, kv_heads vdim), q (rows, heads dim) of in_type; the first 2 rot_half entries of every head of k and q are turned by

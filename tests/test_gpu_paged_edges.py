@@ -335,3 +335,33 @@ def test_results_that_overlap_what_a_call_is_given_are_refused(type):
     with pytest.raises(capi.XalmError, match="overlaps k or v"):
         paged.append(cache, batch, ks, vs, q=q, freq=freq, q_out=qkv[:, 1:H + 1])
     cache.check()
+
+
+# ---- idle places of a group --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rep", [2, 20])
+@pytest.mark.parametrize("new,lens", [([0, 1, 0, 1, 1, 0], [0, 200, 0, 131, 300, 0]), ([0, 0, 3, 0, 2], [0, 0, 190, 0, 140]), ([1, 0, 0, 0, 1], [129, 0, 7, 0, 140]), ([0, 1, 0], [0, 150, 0]),
+                                      ([0, 0, 0], [0, 0, 0])])
+def test_idle_places_neither_end_the_sharing_nor_lend_their_pages(new, lens, rep, type):
+    p = Problem(type, new, lens, G=2, rep=rep, d=64, page=16, seed=69, pad_rows=1, offset=1)
+    live = [s for s in range(len(new)) if new[s]]
+    for s in live:
+        p.table[s, :8] = p.table[live[0], :8]
+    p.groups = [0, len(new)], [128]
+    cache, batch = p.on_gpu()
+    inside = [r for r in range(p.rows) if p.row(r) is not None]
+    out, lse = paged.attend(cache, batch, p.gq, p.scale, want_lse=True)
+    cache.check()
+    want, want_lse, tol, tol_lse = p.attend()
+    near(out[inside], want[inside], tol[inside], "out")
+    near(lse[inside], want_lse[inside], tol_lse[inside], "lse")
+    if len(live) < 2:
+        return
+    # What is read once is read by the first live sequence's table: where the others' name other pages, and the first's are what counts, the common part was shared
+    table = p.table.clone()
+    for s in live[1:]:
+        table[s, :8] = table[live[0], 8:9]
+    batch.tensors[2].copy_(table)
+    again, _ = paged.attend(cache, batch, p.gq, p.scale, want_lse=True)
+    cache.check()
+    assert torch.equal(again[inside], out[inside])

@@ -176,7 +176,7 @@ __host__ __device__ constexpr size_t plan_bytes(int B, int n_groups) { return (s
 
 __host__ __device__ __forceinline__ int share_of(int total, int grid) { return (int) (((unsigned) total + grid - 1) / grid); }
 
-// rows of a segment, its first row and sequence
+// rows of a segment, its first row and the sequence whose table row names the pages: a group's first with rows, since those without need not have any pages
 __device__ __forceinline__ int seg_rows(const View& v, int rep, int seg, int& row0, int& s_first) {
 	if (seg < v.n_groups) {
 		const int2 g = group_of(v, seg);
@@ -185,6 +185,14 @@ __device__ __forceinline__ int seg_rows(const View& v, int rep, int seg, int& ro
 		if (g.x == g.y) return 0;
 		row0 = seq_of(v, g.x).a;
 		const Seq l = seq_of(v, g.y - 1);
+		if (v.starts[g.x + 1] <= row0) { // the last that begins at the first row or before
+			int hi = g.y - 1;
+			while (s_first < hi) {
+				const int mid = (s_first + hi + 1) >> 1;
+				if (v.starts[mid] <= row0) s_first = mid;
+				else hi = mid - 1;
+			}
+		}
 		return max(l.a + l.n - row0, 0) * rep;
 	}
 	s_first = seg - v.n_groups;
@@ -209,8 +217,8 @@ __device__ __forceinline__ int unit_work(const Attn& a, const Part& part, int se
 	return w ? w + part.lead : 0;
 }
 
-// All threads of the CTA.  Shared keys of each group (whole pages, and no more than every row of its sequences sees; a group of one sequence, or of sequences with many rows each, has none),
-// then a running sum over the segments.
+// All threads of the CTA.  Shared keys of each group (whole pages, and no more than every row of its sequences sees; a group of one sequence, or of sequences with many rows each, has none;
+// sequences without rows do not count), then a running sum over the segments.
 template <int NT>
 __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& p) {
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.B, n = a.b.n_groups;
@@ -249,11 +257,16 @@ __device__ void make_plan(const Attn& a, const Part& part, uint8_t* smem, Plan& 
 			const int2 g = group_of(p.v, i);
 			if (g.y - g.x < 2) continue;
 			const Seq last = seq_of(p.v, g.y - 1);
-			if ((float) (last.a + last.n - seq_of(p.v, g.x).a) * a.rep > (float) (g.y - g.x) * ALONE_ROWS) continue;
+			int some = 0;
 			for (int s = g.x + lane; s < g.y; s += 32) {
 				const Seq q = seq_of(p.v, s);
-				m = min(m, max(q.len - q.n, 0));
+				if (q.n) {
+					some++;
+					m = min(m, max(q.len - q.n, 0));
+				}
 			}
+			some = __reduce_add_sync(0xffffffffu, some);
+			if (some < 2 || (float) (last.a + last.n - seq_of(p.v, g.x).a) * a.rep > (float) some * ALONE_ROWS) continue;
 			m = __reduce_min_sync(0xffffffffu, m) >> a.c.shift << a.c.shift;
 			for (int s = g.x + lane; s < g.y; s += 32) p.shs[s] = m;
 		}
