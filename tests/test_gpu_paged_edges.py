@@ -365,3 +365,57 @@ def test_idle_places_neither_end_the_sharing_nor_lend_their_pages(new, lens, rep
     again, _ = paged.attend(cache, batch, p.gq, p.scale, want_lse=True)
     cache.check()
     assert torch.equal(again[inside], out[inside])
+
+
+# ---- values that are not finite ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("below", [5, 20, 40, 60])
+@pytest.mark.parametrize("where", ["own", "shared", "divided", "long"])
+def test_infinite_values_of_many_rows_stay_in_their_columns(where, below, type):
+    """Beside probabilities far below what fp16 holds too; of both signs and a NaN in one column; seen by all rows, and by the later ones only."""
+    if where in ("shared", "long"):
+        n = 512 if where == "shared" else 32768  # a tile to a block, several
+        p = sink(type, [1] * 16, [n + 88 + i for i in range(16)], below, 16, groups=([0, 16], [n]))
+        places = [(0, 100, 7, math.inf), (0, 101, 8, math.inf), (0, 300, 8, -math.inf), (0, 5, 63, math.nan), (3, n + 88, 9, -math.inf)]
+    else:
+        n = 70 if where == "own" else 700
+        p = sink(type, [n], [n + 500], below, 4)
+        places = [(0, 100, 7, math.inf), (0, 101, 8, math.inf), (0, 520, 8, -math.inf), (0, 5, 63, math.nan), (0, 515, 9, -math.inf), (0, 560, 10, math.inf)]
+    for s, at, c, x in places:
+        p.v[p.slots(s, at) + (0, c)] = x
+    cache, batch = p.on_gpu()
+    out, lse = paged.attend(cache, batch, p.gq, p.scale, want_lse=True)
+    cache.check()
+    some = list(range(p.rows)) if where != "divided" else looked_at(p, 40) + [14, 15, 16, 18, 19, 20, 21, 59, 60, 61]
+    want, want_lse, tol, tol_lse = p.attend(only=some)
+    near(out[some], want[some], tol[some], "out")
+    near(lse[some], want_lse[some], tol_lse[some], "lse")
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("rep", [1, 4])
+def test_a_query_that_is_not_finite_makes_no_other_row_wait(rep, type):
+    """Rows of NaN are what they are: no row is done again key by key."""
+    p = Problem(type, [2000, 9], [3000, 2000], G=2, rep=rep, d=64, page=64, seed=70)
+    cache, batch = p.on_gpu()
+    bad = p.gq.clone()
+    bad[5:2005:100] = math.nan
+
+    def time(q):
+        best = math.inf
+        for _ in range(5):
+            ends = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            ends[0].record()
+            out = paged.attend(cache, batch, q, p.scale)
+            ends[1].record()
+            torch.cuda.synchronize()
+            best = min(best, ends[0].elapsed_time(ends[1]))
+        return best, out
+
+    plain, want = time(p.gq)
+    spoilt, got = time(bad)
+    assert torch.isnan(got[5:2005:100]).all()
+    fine = torch.ones(p.rows, dtype=torch.bool)
+    fine[5:2005:100] = False
+    assert torch.equal(got[fine], want[fine])
+    assert spoilt < 5 * plain, (spoilt, plain)

@@ -434,8 +434,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			bar_sync(1, CW * 32);
 		}
 		if (mixed) {
-			// A value that is not finite and that only later rows see has met probabilities of zero in the product: rows that did not come out finite
-			// are done again, key by key.
+			// A value that is not finite and that only later rows see has met probabilities of zero in the product: rows that do not see it are done again, key by key.
 			bool again = false;
 #pragma unroll
 			for (int i = 0; i < D / 8; i++)
@@ -448,8 +447,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			const bool redo = s_ml[0].x != 0.f;
 			bar_sync(1, CW * 32);
 			const Piece y = x; // in memory only here
-			if (redo)
-				for (int r = 0; r < rows; r++) slow_row<T>(a, part, y, MM, r, own_keys(x.q, x.key0, a.rep, x.t * MM + r), s_o, direct, slot, tid, 1);
+			if (redo) redo_rows<T>(a, part, y, MM, 0, rows, max(least, x.j0 * KT), min(most, x.j1 * KT), reinterpret_cast<int*>(s_ml), s_o, direct, slot, tid, 1);
 		}
 	}
 }

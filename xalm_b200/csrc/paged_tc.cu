@@ -124,6 +124,41 @@ struct TcShared {
 	float buf[2][256];
 };
 
+// fp16 rounds probabilities to 0 beside which an infinite value should give an infinity: the infinities and NaNs of column after column that a lane's row sees are put where its sums go.  A
+// whole warp, whose lanes look at 32 keys at a time; row: of the unit, lim, most: keys that the lane's row sees, and the unit's last; fix: whether the lane's row is in need of it
+__device__ __noinline__ void put_infinities(const Attn& a, const Part& part, const Piece& x, int row, int lim, int most, bool fix, bool direct, long long slot) {
+	const int lane = threadIdx.x & 31, P = 1 << a.c.shift, w = x.t * TC_ROWS + row, last = min(x.j1 * KT, most);
+	for (int c = 0; c < a.c.dv; c += 8) {
+		unsigned up = 0, down = 0; // a bit to a column; a NaN is both
+#pragma unroll 4
+		for (int kb = x.j0 * KT; kb < last; kb += 32) {
+			const int key = x.key0 + kb + lane, pg = kb + lane < last ? page_of(a.c, a.b, x.s, key >> a.c.shift) : -1;
+			uint4 u = make_uint4(0, 0, 0, 0);
+			if (pg >= 0) u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.c.v) + pg * a.c.v_page + (key & (P - 1)) * a.c.v_slot + x.g * a.c.v_head + c);
+			const uint32_t word[4] = {u.x, u.y, u.z, u.w};
+			unsigned bits = 0;
+#pragma unroll
+			for (int e = 0; e < 8; e++) {
+				const uint32_t v = word[e >> 1] >> (e & 1) * 16;
+				if ((v & 0x7c00u) == 0x7c00u) bits |= ((v & 0x3ffu ? 0x101u : v & 0x8000u ? 0x100u : 1u)) << e;
+			}
+			for (unsigned m = __ballot_sync(0xffffffffu, bits != 0); m; m &= m - 1) {
+				const int from = __ffs(m) - 1;
+				const unsigned b = __shfl_sync(0xffffffffu, bits, from);
+				if (kb + from < lim) { up |= b & 0xff; down |= b >> 8; }
+			}
+		}
+		if (fix)
+			for (unsigned m = up | down; m; m &= m - 1) {
+				const int e = __ffs(m) - 1;
+				const float v = up >> e & down >> e & 1 ? NAN : up >> e & 1 ? INFINITY : -INFINITY;
+				if (direct) reinterpret_cast<__half*>(a.out)[(long long) (x.row0 + w / a.rep) * a.out_row + (x.g * a.rep + w % a.rep) * a.c.dv + c + e] = __float2half_rn(v);
+				else if (slot < part.slots) part.o[(slot * TC_ROWS + row) * a.c.dv + c + e] = v;
+			}
+	}
+	__syncwarp();
+}
+
 template <typename T>
 struct Lift { // in powers of two; fp16 ends at 2^16
 	static constexpr float BY = 0.f, LAG = 11.5f;
@@ -415,8 +450,15 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				__syncwarp();
 			}
 			fence_before();
+			if constexpr (std::is_same<T, __half>::value) {
+				const bool fix = again && mine && l == l && tiles && ok; // not where a score is NaN: all columns are
+				if (__any_sync(0xffffffffu, fix)) {
+					const Piece y = x;
+					put_infinities(a, part, y, row, lim, p.most, fix, direct, slot);
+				}
+			}
 			if (!p.prefix && tiles && x.j1 * KT > least && least < p.most) {
-				// A value that is not finite and that only later rows see has met probabilities of zero: those rows are done again, key by key
+				// A value that is not finite and that only later rows see has met probabilities of zero: rows that do not see it are done again, key by key
 				if (wt == 0) sh.flag[h] = 0;
 				bar_sync(2 + h, 128);
 				if (again && mine && ok) sh.flag[h] = 1;
@@ -425,8 +467,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				bar_sync(2 + h, 128);
 				const Piece y = x; // in memory only here
 				if (redo)
-					for (int i = h * HALF_ROWS; i < min(p.rows, (h + 1) * HALF_ROWS); i++)
-						slow_row<T>(a, part, y, TC_ROWS, i, own_keys(x.q, x.key0, a.rep, x.t * TC_ROWS + i), sh.buf[h], direct, slot, wt, 2 + h);
+					redo_rows<T>(a, part, y, TC_ROWS, h * HALF_ROWS, min(p.rows, (h + 1) * HALF_ROWS), max(least, x.j0 * KT), min(p.most, x.j1 * KT), &sh.flag[h], sh.buf[h], direct, slot, wt, 2 + h);
 			}
 		}
 		n += tiles;

@@ -137,6 +137,27 @@ __device__ __forceinline__ void put_row(const Attn& a, const Part& part, const P
 	}
 }
 
+// Two 16-bit numbers of a word, one of them not finite
+template <typename T>
+__device__ __forceinline__ bool infinite16(uint32_t w) {
+	constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+	return (w & E) == E || (w >> 16 & E) == E;
+}
+// Of keys [from, to) of a piece's segment the last whose value is not finite in some entry, among those that this one of 128 threads looks at; -1: none
+template <typename T>
+__device__ __noinline__ int last_infinite(const Attn& a, const Piece& x, int from, int to, int tid) {
+	const int chunks = a.c.dv / 8, P = 1 << a.c.shift;
+	int last = -1;
+#pragma unroll 4
+	for (int i = tid; i < (to - from) * chunks; i += 128) {
+		const int at = from + i / chunks, key = x.key0 + at, pg = page_of(a.c, a.b, x.s, key >> a.c.shift);
+		if (pg < 0) continue;
+		const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.c.v) + pg * a.c.v_page + (key & (P - 1)) * a.c.v_slot + x.g * a.c.v_head + i % chunks * 8);
+		if (infinite16<T>(u.x) || infinite16<T>(u.y) || infinite16<T>(u.z) || infinite16<T>(u.w)) last = at;
+	}
+	return last;
+}
+
 // One row of a piece by fp32 FMAs, with only the keys that it sees: for rows that a value which is not finite has spoilt.  128 threads, which share
 // barrier `bar`; `buf`: 256 floats.
 template <typename T>
@@ -152,7 +173,14 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 			s = 0.f;
 			if (pg >= 0) {
 				const T* kk = reinterpret_cast<const T*>(a.c.k) + pg * a.c.k_page + (key & (P - 1)) * a.c.k_slot + x.g * a.c.k_head;
-				for (int i = 0; i < a.c.d; i++) s = fmaf(to_f(q[i]), to_f(kk[i]), s);
+#pragma unroll 4
+				for (int i = 0; i < a.c.d; i += 8) {
+					float u[8], w[8];
+					load8(q + i, u);
+					load8(kk + i, w);
+#pragma unroll
+					for (int e = 0; e < 8; e++) s = fmaf(u[e], w[e], s);
+				}
 			}
 			s *= a.scale * 1.4426950408889634f;
 		}
@@ -170,6 +198,7 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 		l *= f;
 		acc[0] *= f;
 		acc[1] *= f;
+#pragma unroll 8
 		for (int i = 0; i < min(128, last - kb); i++) {
 			const int key = x.key0 + kb + i, pg = page_of(a.c, a.b, x.s, key >> a.c.shift);
 			l += buf[i];
@@ -186,6 +215,23 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 	bar_sync(bar, 128);
 	for (int c = tid * 4; c < a.c.dv; c += 512) put_row<T>(a, part, x, M, row, c, *reinterpret_cast<const float4*>(buf + c), m, l, direct, slot);
 	bar_sync(bar, 128);
+}
+
+// Rows [r0, r1) of a unit of M, some of which did not come out finite: of keys [from, to), which not all of them see, the last whose value is not finite is looked for, and the rows that do not
+// see it are done again.  128 threads; mark: an int in shared memory
+template <typename T>
+__device__ __noinline__ void redo_rows(const Attn& a, const Part& part, const Piece& x, int M, int r0, int r1, int from, int to, int* mark, float* buf, bool direct, long long slot, int tid, int bar) {
+	if (tid == 0) *mark = -1;
+	bar_sync(bar, 128);
+	const int found = last_infinite<T>(a, x, from, to, tid);
+	if (found >= 0) atomicMax(mark, found);
+	bar_sync(bar, 128);
+	const int last = *(volatile int*) mark;
+	bar_sync(bar, 128);
+	for (int r = r0; r < r1; r++) {
+		const int lim = own_keys(x.q, x.key0, a.rep, x.t * M + r);
+		if (lim <= last) slow_row<T>(a, part, x, M, r, lim, buf, direct, slot, tid, bar);
+	}
 }
 
 } // namespace paged
