@@ -419,3 +419,32 @@ def test_a_query_that_is_not_finite_makes_no_other_row_wait(rep, type):
     fine[5:2005:100] = False
     assert torch.equal(got[fine], want[fine])
     assert spoilt < 5 * plain, (spoilt, plain)
+
+
+# ---- workspaces --------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("seqs,groups,most", [(128, 2, 80), (1000, 3, 400), (4000, 1, 1500)])
+def test_a_batch_of_single_tokens_needs_no_room_for_long_ones(seqs, groups, most):
+    """In MiB; 32 heads of 128 over 8, some sequences of which share pages."""
+    import ctypes as C
+    k = torch.zeros(4, 64, 8, 128, dtype=torch.bfloat16, device="cuda")
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    cache, batch = paged.PagedCache(k, k), paged.Batch(i(seqs + 1), i(seqs), i(seqs, 100), i(groups + 1), i(groups))
+    need = C.c_size_t(0)
+    capi.check(capi.lib().xalm_cuda_paged_workspace(cache.p, batch.of(seqs)[0], 32, 0, C.byref(need)))
+    assert need.value < most << 20, need.value / 2 ** 20
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("new,rep,groups", [([1] * 40, 17, ([0, 20, 40], [64, 128])), ([1] * 40, 17, ([0, 40], [64])), ([17] * 30, 1, ([0, 30], [64])), ([1, 0, 17, 2, 0, 33] * 6, 1, ([0, 18, 36], [64, 64])),
+                                            ([9] * 20, 2, ([2, 4, 6, 8, 19], [64, 64, 128, 64])), ([257, 1, 255, 256], 1, ([0, 4], [128]))])
+def test_as_many_units_as_there_is_room_for(new, rep, groups, type):
+    """Segments of just more rows than the short ones' kernel takes, each a unit of its own, in the smallest workspace."""
+    lens = [190 + n + 7 * i % 40 for i, n in enumerate(new)]
+    p = Problem(type, new, lens, G=3, rep=rep, d=64, page=64, seed=71, groups=groups)
+    cache, batch = p.on_gpu()
+    out, lse = paged.attend(cache, batch, p.gq, p.scale, want_lse=True)
+    cache.check()
+    some = looked_at(p, 60)
+    want, want_lse, tol, tol_lse = p.attend(only=some)
+    near(out[some], want[some], tol[some], "out")
+    near(lse[some], want_lse[some], tol_lse[some], "lse")

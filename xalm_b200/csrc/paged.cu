@@ -783,8 +783,11 @@ static int plan_attn(const xalm_paged_cache* cache, const Cache& c, const BatchV
 		p.least_rows = big ? SMALL_ROWS + 1 : 1;
 		p.most_rows = tc && !big ? SMALL_ROWS : 0x7fffffff;
 		const long long rows = (long long) b.N * a.rep;
-		// a segment of `rows` rows has at most rows / M + 1 tiles, a part that takes short ones only has one
-		const long long tiles = n_lists ? (long long) b.N * ((a.rep + p.M - 1) / p.M) : (tc && !big ? 0 : rows / p.M) + b.B + (b.n_groups ? (tc && !big ? 0 : rows / p.M) + b.n_groups : 0);
+		// A segment has at most its rows / M + 1 tiles, in a part that takes short ones only it has one; and there are no more segments than have room for the part's least rows, of sequences
+		// as of groups.  (128 single tokens of 32 heads of 128 over 8 in two groups: 69 MB; with a tile of 256 rows for every sequence 174.)
+		const long long whole = tc && !big ? 0 : rows / p.M, most = rows / p.least_rows;
+		const long long tiles = n_lists ? (long long) b.N * ((a.rep + p.M - 1) / p.M)
+		                                : whole + std::min((long long) b.B, most) + (b.n_groups ? whole + std::min((long long) b.n_groups, most) : 0);
 		if (tiles * c.G + p.grid > 0x7fffffff / p.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
 		const long long keys = (long long) b.max_pages << c.shift, work = n_lists ? (((long long) n_lists << c.shift) + KT - 1) / KT : keys / KT + 1;
 		if (tiles * c.G > 0x7fffffffll / (work + p.lead)) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads over up to %lld keys are too many for one call", b.N, heads, work * KT);
