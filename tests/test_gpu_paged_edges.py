@@ -448,3 +448,25 @@ def test_as_many_units_as_there_is_room_for(new, rep, groups, type):
     want, want_lse, tol, tol_lse = p.attend(only=some)
     near(out[some], want[some], tol[some], "out")
     near(lse[some], want_lse[some], tol_lse[some], "lse")
+
+
+# ---- scores of millions ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 8, 16, 256])
+def test_scores_that_fp32_holds_to_half_a_unit_give_finite_results(rows, type):
+    """Scores of some 5 million with differences that fp32 rounds: what a probability is may be off by much, but it is no infinity, and sums to one."""
+    tokens, rep = ROWS[rows]
+    n = 65536  # several tiles to a block
+    for step in (8, 16, 20):
+        p = sink(type, [tokens], [n], 0, rep)
+        p.q[:, :, 0] = 2048.0
+        p.q[:, :, 0] += (torch.arange(p.rows * p.H) % 97).view(p.rows, p.H).to(p.t) * (2.0 if type != "bf16" else 16.0)
+        p.k[..., 0], p.v = 20000.0, torch.ones_like(p.v)
+        at = torch.arange(n)
+        p.k[p.slots(0, at) + (0, 1)] = (step * (at // 128 % 2)).to(p.t)  # the larger ones come after the first that a row sees
+        cache, batch = p.on_gpu()
+        out = paged.attend(cache, batch, p.gq, p.scale)
+        assert torch.isfinite(out).all() and float((out - 1).abs().max()) < 0.5, step
+        if rows < 256:
+            out = paged.attend_selected(cache, batch, p.gq, torch.arange(p.max_pages, dtype=torch.int32).repeat(p.rows, 1, 1).cuda(), p.scale)
+            assert torch.isfinite(out).all() and float((out - 1).abs().max()) < 0.5, step

@@ -95,10 +95,11 @@ template <typename T>
 __device__ __forceinline__ void parts16(float lo, float hi, uint32_t& rounded, uint32_t& rest) {
 	if constexpr (std::is_same<T, __half>::value) {
 		// no 0, beside which an infinite value would give no infinity: what this adds to the smallest, and to masked ones, the second part takes off again
-		const __half2 h = __hmax2_nan(__floats2half2_rn(lo, hi), __halves2half2(__ushort_as_half(1), __ushort_as_half(1)));
+		const uint32_t near = probs_f16(lo, hi);
+		const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2*>(&near), __halves2half2(__ushort_as_half(1), __ushort_as_half(1)));
 		rounded = *reinterpret_cast<const uint32_t*>(&h);
 		const float2 r = rest16<T>(rounded, lo, hi);
-		rest = pack16<T>(r.x * REST_LIFT, r.y * REST_LIFT);
+		rest = probs_f16(r.x * REST_LIFT, r.y * REST_LIFT);
 	} else {
 		rounded = pack16<T>(lo, hi);
 		const float2 r = rest16<T>(rounded, lo, hi);

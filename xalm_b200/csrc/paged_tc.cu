@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 					p0 = exp2_approx(p0);
 					p1 = exp2_approx(p1);
 					sum[i & 3] = add2(sum[i & 3], pack2(p0, p1));
-					q[i] = pair16<T>(p0, p1);
+					if constexpr (std::is_same<T, __half>::value) q[i] = probs_f16(p0, p1);
+					else q[i] = pair16<T>(p0, p1);
 				}
 				{
 					float e, o;

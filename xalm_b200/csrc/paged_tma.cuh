@@ -137,6 +137,13 @@ __device__ __forceinline__ void put_row(const Attn& a, const Part& part, const P
 	}
 }
 
+// Two probabilities of fp16, no infinities: where scores are so large that fp32 holds them to half a unit, one may be above what it is meant to be at most
+__device__ __forceinline__ uint32_t probs_f16(float lo, float hi) {
+	uint32_t r;
+	asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+	return r;
+}
+
 // Two 16-bit numbers of a word, one of them not finite
 template <typename T>
 __device__ __forceinline__ bool infinite16(uint32_t w) {
