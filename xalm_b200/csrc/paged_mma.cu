@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			const bool redo = s_ml[0].x != 0.f;
 			bar_sync(1, CW * 32);
 			const Piece y = x; // in memory only here
-			if (redo) redo_rows<T>(a, part, y, MM, 0, rows, max(least, x.j0 * KT), min(most, x.j1 * KT), reinterpret_cast<int*>(s_ml), s_o, direct, slot, tid, 1);
+			if (redo) redo_rows<T, MM, MM>(a, part, y, 0, reinterpret_cast<int*>(s_ml), s_o, tid, 1);
 		}
 	}
 }

@@ -126,8 +126,10 @@ struct TcShared {
 
 // fp16 rounds probabilities to 0 beside which an infinite value should give an infinity: the infinities and NaNs of column after column that a lane's row sees are put where its sums go.  A
 // whole warp, whose lanes look at 32 keys at a time; row: of the unit, lim, most: keys that the lane's row sees, and the unit's last; fix: whether the lane's row is in need of it
-__device__ __noinline__ void put_infinities(const Attn& a, const Part& part, const Piece& x, int row, int lim, int most, bool fix, bool direct, long long slot) {
+__device__ __noinline__ void put_infinities(const Attn& a, const Part& part, const Piece& x, int row, int lim, int most, bool fix) {
 	const int lane = threadIdx.x & 31, P = 1 << a.c.shift, w = x.t * TC_ROWS + row, last = min(x.j1 * KT, most);
+	const bool direct = x.j0 == 0 && x.j1 == x.w && x.seg >= a.b.n_groups && x.key0 == 0;
+	const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
 	for (int c = 0; c < a.c.dv; c += 8) {
 		unsigned up = 0, down = 0; // a bit to a column; a NaN is both
 #pragma unroll 4
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool fix = again && mine && l == l && tiles && ok; // not where a score is NaN: all columns are
 				if (__any_sync(0xffffffffu, fix)) {
 					const Piece y = x;
-					put_infinities(a, part, y, row, lim, p.most, fix, direct, slot);
+					put_infinities(a, part, y, row, lim, p.most, fix);
 				}
 			}
 			if (!p.prefix && tiles && x.j1 * KT > least && least < p.most) {
@@ -467,8 +469,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool redo = *(volatile int*) &sh.flag[h] != 0;
 				bar_sync(2 + h, 128);
 				const Piece y = x; // in memory only here
-				if (redo)
-					redo_rows<T>(a, part, y, TC_ROWS, h * HALF_ROWS, min(p.rows, (h + 1) * HALF_ROWS), max(least, x.j0 * KT), min(p.most, x.j1 * KT), &sh.flag[h], sh.buf[h], direct, slot, wt, 2 + h);
+				if (redo) redo_rows<T, TC_ROWS, HALF_ROWS>(a, part, y, h * HALF_ROWS, &sh.flag[h], sh.buf[h], wt, 2 + h);
 			}
 		}
 		n += tiles;

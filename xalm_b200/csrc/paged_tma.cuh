@@ -224,21 +224,23 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 	bar_sync(bar, 128);
 }
 
-// Rows [r0, r1) of a unit of M, some of which did not come out finite: of keys [from, to), which not all of them see, the last whose value is not finite is looked for, and the rows that do not
-// see it are done again.  128 threads; mark: an int in shared memory
-template <typename T>
-__device__ __noinline__ void redo_rows(const Attn& a, const Part& part, const Piece& x, int M, int r0, int r1, int from, int to, int* mark, float* buf, bool direct, long long slot, int tid, int bar) {
+// ROWS rows from r0 on of an own segment's unit of M, some of which did not come out finite: of the keys that not all of the unit's rows see, the last whose value is not finite is looked for, and
+// the rows that do not see it are done again.  128 threads; mark: an int in shared memory.  (What can be told from the piece is, in here: more arguments took half a microsecond from short calls.)
+template <typename T, int M, int ROWS>
+__device__ __noinline__ void redo_rows(const Attn& a, const Part& part, const Piece& x, int r0, int* mark, float* buf, int tid, int bar) {
+	const int rows = min(M, x.rows - x.t * M);
+	const bool direct = x.j0 == 0 && x.j1 == x.w && x.key0 == 0;
+	const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
+	auto seen = [&](int r) { return own_keys(x.q, x.key0, a.rep, x.t * M + r); };
 	if (tid == 0) *mark = -1;
 	bar_sync(bar, 128);
-	const int found = last_infinite<T>(a, x, from, to, tid);
+	const int found = last_infinite<T>(a, x, max(seen(0), x.j0 * KT), min(seen(rows - 1), x.j1 * KT), tid);
 	if (found >= 0) atomicMax(mark, found);
 	bar_sync(bar, 128);
 	const int last = *(volatile int*) mark;
 	bar_sync(bar, 128);
-	for (int r = r0; r < r1; r++) {
-		const int lim = own_keys(x.q, x.key0, a.rep, x.t * M + r);
-		if (lim <= last) slow_row<T>(a, part, x, M, r, lim, buf, direct, slot, tid, bar);
-	}
+	for (int r = r0; r < min(rows, r0 + ROWS); r++)
+		if (seen(r) <= last) slow_row<T>(a, part, x, M, r, seen(r), buf, direct, slot, tid, bar);
 }
 
 } // namespace paged
