@@ -296,7 +296,7 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  *   lens[s] - n + i.  starts has seqs + 1 entries; rows outside [starts[0], starts[seqs]) of `rows` are left alone.  table (seqs, max_pages), rows table_row apart.
  *   Sequences group_bounds[i] .. group_bounds[i + 1] - 1 (ascending) have the same pages for their first group_shared[i] tokens: those are read once for all of
  *   them that have new tokens (the others, idle places of a captured batch, need no pages); what a call computes does not depend on it but for the order of its sums.  At most 4096 sequences and groups, tables of at most 2^30 tokens.
- * Rows of arrays are `*_row` elements apart and begin at 16-byte boundaries; heads within a row are dense.
+ * Rows of arrays are `*_row` elements apart and begin at 16-byte boundaries; heads within a row are dense.  Arrays of int and float begin at 4-byte boundaries.
  *
  * paged_append: k (rows, kv_heads dim), v (rows, kv_heads vdim), q (rows, heads dim) of in_type; the first 2 rot_half entries of every head of k and q are turned by
  *   position * freq[i] (entry i with i + rot_half, or with `neighbours` 2 i with 2 i + 1; cos and sin times rot_mag); keys and values go to their pages, queries to q_out

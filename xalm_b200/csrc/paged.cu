@@ -639,6 +639,7 @@ __global__ void paged_status_kernel(int* status, int* taken) { *taken = atomicEx
 static int element_bytes(int type) { return type == XALM_F32 ? 4 : 2; }
 static bool is_type(int type) { return type == XALM_F32 || type == XALM_F16 || type == XALM_BF16; }
 static bool aligned16(const void* p) { return ((uintptr_t) p & 15) == 0; }
+static bool aligned4(const void* p) { return ((uintptr_t) p & 3) == 0; }
 
 static int check_strides(const char* what, int G, int P, int pages, int dim, int bytes, long long page, long long slot, long long head) {
 	const long long most = 1ll << 40;
@@ -659,6 +660,7 @@ static int check_cache(const xalm_paged_cache* c, Cache& o) {
 	while (shift < 8 && (1 << shift) != c->page_size) shift++;
 	if ((1 << shift) != c->page_size) return set_error(XALM_ERR_INVALID, "paged cache: pages of %d slots (16, 32, 64, 128 or 256)", c->page_size);
 	if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v) || !aligned16(c->means)) return set_error(XALM_ERR_INVALID, "paged cache: pools are at 16-byte boundaries, and not NULL");
+	if (!aligned4(c->status)) return set_error(XALM_ERR_INVALID, "paged cache: the status word is not at a 4-byte boundary");
 	const int e = element_bytes(c->type);
 	XALM_TRY(check_strides("keys", c->kv_heads, c->page_size, c->pages, c->dim, e, c->k_page, c->k_slot, c->k_head));
 	XALM_TRY(check_strides("values", c->kv_heads, c->page_size, c->pages, c->vdim, e, c->v_page, c->v_slot, c->v_head));
@@ -674,6 +676,8 @@ static int check_batch(const xalm_paged_batch* b, const Cache& c, BatchView& o) 
 	if ((long long) b->max_pages << c.shift > 1ll << 30) return set_error(XALM_ERR_INVALID, "paged cache: tables of %d pages of %d tokens (at most 2^30 tokens)", b->max_pages, 1 << c.shift);
 	if (b->seqs && (!b->starts || !b->lens || (b->max_pages && !b->table))) return set_error(XALM_ERR_INVALID, "paged cache: starts/lens/table is NULL");
 	if (b->groups && (!b->group_bounds || !b->group_shared)) return set_error(XALM_ERR_INVALID, "paged cache: group_bounds/group_shared is NULL");
+	for (const int* p : {b->starts, b->lens, b->table, b->group_bounds, b->group_shared})
+		if (!aligned4(p)) return set_error(XALM_ERR_INVALID, "paged cache: starts, lens, table and groups are at 4-byte boundaries");
 	o = BatchView{b->rows, b->seqs, b->max_pages, b->groups, b->starts, b->lens, b->table, b->table_row, b->group_bounds, b->group_shared};
 	return XALM_OK;
 }
@@ -822,6 +826,7 @@ static int attend(const xalm_paged_cache* cache, const xalm_paged_batch* batch, 
 	}
 	if (heads % c.G) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
 	if (n_lists > MAX_LIST) return set_error(XALM_ERR_INVALID, "paged attention: lists of %d pages (at most %d)", n_lists, MAX_LIST);
+	if (!aligned4(lse) || !aligned4(lists)) return set_error(XALM_ERR_INVALID, "paged attention: lse and lists are at 4-byte boundaries");
 	if (!isfinite(scale)) return set_error(XALM_ERR_INVALID, "paged attention: scale is not finite");
 	if (b.N == 0 || b.B == 0) return XALM_OK;
 	if (!workspace || ((uintptr_t) workspace & 255)) return set_error(XALM_ERR_INVALID, "paged attention: the workspace is NULL or not at a 256-byte boundary");
@@ -881,6 +886,7 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 	XALM_TRY(check_cache(cache, a.c));
 	XALM_TRY(check_batch(batch, a.c, a.b));
 	if (!is_type(in_type)) return set_error(XALM_ERR_UNSUPPORTED, "paged append: rows of type %d (F32, F16 and BF16)", in_type);
+	if (!aligned4(freq)) return set_error(XALM_ERR_INVALID, "paged append: freq is not at a 4-byte boundary");
 	if (rot_half < 0 || 2 * rot_half > a.c.d || (rot_half && !freq)) return set_error(XALM_ERR_INVALID, "paged append: rotation of %d pairs in heads of %d", rot_half, a.c.d);
 	if (q && (heads <= 0 || heads > 65535)) return set_error(XALM_ERR_INVALID, "paged append: %d query heads", heads);
 	if (a.b.N) {
@@ -961,7 +967,7 @@ int xalm_cuda_paged_append(const xalm_paged_cache* cache, const xalm_paged_batch
 int xalm_cuda_paged_status(const xalm_paged_cache* cache, int* taken, void* stream) {
 	Cache c;
 	XALM_TRY(check_cache(cache, c));
-	if (!taken || !c.status) return set_error(XALM_ERR_INVALID, "paged status: %s is NULL", taken ? "the cache's status word" : "taken");
+	if (!taken || !c.status || !aligned4(taken)) return set_error(XALM_ERR_INVALID, "paged status: %s", !taken || !c.status ? "taken or the cache's status word is NULL" : "taken is not at a 4-byte boundary");
 	OnDevice on;
 	XALM_TRY(on.set(cache->device));
 	paged_status_kernel<<<1, 1, 0, (cudaStream_t) stream>>>(c.status, taken);
@@ -1002,7 +1008,7 @@ int xalm_cuda_paged_select(const xalm_paged_cache* cache, const xalm_paged_batch
 	if (a.b.max_pages > 24576) return set_error(XALM_ERR_INVALID, "paged select: sequences of %d pages (at most 24576)", a.b.max_pages);
 	if (a.b.N) {
 		XALM_TRY(check_rows("q", q, q_row, heads * a.c.d, element_bytes(cache->type)));
-		if (!out) return set_error(XALM_ERR_INVALID, "paged select: out is NULL");
+		if (!out || !aligned4(out)) return set_error(XALM_ERR_INVALID, "paged select: out is NULL or not at a 4-byte boundary");
 	}
 	if (a.b.N == 0 || a.b.B == 0) return XALM_OK;
 	OnDevice on;
