@@ -470,3 +470,21 @@ def test_scores_that_fp32_holds_to_half_a_unit_give_finite_results(rows, type):
         if rows < 256:
             out = paged.attend_selected(cache, batch, p.gq, torch.arange(p.max_pages, dtype=torch.int32).repeat(p.rows, 1, 1).cuda(), p.scale)
             assert torch.isfinite(out).all() and float((out - 1).abs().max()) < 0.5, step
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lens,bad", [([1000, 750, 1], [2000, 1500, 1000], 1600), ([1500, 20, 1], [3000, 1500, 1000], 2983), ([3, 2], [40000, 300], 39999), ([300, 300], [30000, 300], 29850)])
+def test_rows_that_take_long_end_no_wait(new, lens, bad, type):
+    """A token of NaN inside a prompt: the rows before it are done again key by key, and the warps that wait for that meanwhile do not give up."""
+    p = Problem(type, new, lens, G=8 if lens[0] < 10000 else 1, rep=4, d=128, page=64, seed=72)
+    at = p.slots(0, bad)
+    p.k[at], p.v[at] = math.nan, math.nan
+    cache, batch = p.on_gpu()
+    out = paged.attend(cache, batch, p.gq, p.scale)
+    cache.check()
+    first = bad - (lens[0] - new[0])  # row of the token
+    assert torch.isnan(out[first:new[0]]).all() and torch.isfinite(out[:first]).all() and torch.isfinite(out[new[0]:]).all()
+    p.k[at], p.v[at] = 0.0, 0.0
+    some = sorted({max(first - i, 0) for i in (1, 2, 3, 17, 33, 50, 64, 65, 130)} - {first}) + [p.rows - 1]
+    want, _, tol, _ = p.attend(only=some)
+    near(out[some], want[some], tol[some])

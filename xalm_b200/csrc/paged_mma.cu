@@ -124,14 +124,16 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 	float2* s_ml = reinterpret_cast<float2*>((uint8_t*) s_o + Z::JOIN);   // [CW][MM]
 	uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + CW * MM);         // [8]
 	uint64_t* empty = full + 8;                                           // [8]
-	int* s_dead = reinterpret_cast<int*>(empty + 8);
-	int* s_ids = s_dead + 1;                                              // [32]
+	State* state = reinterpret_cast<State*>(empty + 8);
+	int* s_sent = reinterpret_cast<int*>(state + 1);                      // tiles whose copies were sent
+	int* s_ids = s_sent + 1;                                              // [32]
 	int* s_list = reinterpret_cast<int*>((uint8_t*) full + 512);          // [S]
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_list) + ((LIST ? a.S * 4 : 0) + 15) / 16 * 16;
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	if (tid == 0) {
 		for (int i = 0; i < stages; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], CW); }
-		*s_dead = 0;
+		state->init();
+		*s_sent = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 	}
 	pdl_launch_dependents();
@@ -185,13 +187,14 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 				const int count = min(batch, j1 - j);
 				if (elect())
 					for (int i = 0, st1 = st, round1 = round; i < count; i++) {
-						if (!(ok = wait_alone(&empty[st1], round1 ^ 1, s_dead, a.c))) break;
+						if (!(ok = wait_alone<!LIST>(&empty[st1], round1 ^ 1, state, a.c))) break;
 						mbar_expect_tx(&full[st1], (uint32_t) ((dc + vc) * KT * 128));
 						const uint32_t dst = smem_u32(ring) + (uint32_t) st1 * Z::STAGE;
 						const int slot = (key0 + (j + i) * KT) & (P - 1);
 						copy_tile(dst, &kmap, a.c.d, g, slot, per, W, s_ids + i * per, a.c.pages, &full[st1]);
 						copy_tile(dst + Z::TILE, &vmap, a.c.dv, g, slot, per, W, s_ids + i * per, a.c.pages, &full[st1]);
 						if (++st1 == stages) { st1 = 0; round1 ^= 1; }
+						*s_sent = sent + i + 1;
 					}
 				ok = __all_sync(0xffffffffu, ok);
 				for (int i = 0; i < count; i++) advance();
@@ -199,8 +202,11 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			}
 			if (!ok) break;
 		}
-		if (*(volatile int*) s_dead) // gave up: copies still on their way end first
-			for (int i = max(0, sent - stages); i < sent; i++) wait_some(&full[i % stages], (i / stages) & 1);
+		if (*(volatile int*) &state->dead) { // gave up: copies still on their way end first
+			__syncwarp();
+			const int last = *(volatile int*) s_sent;
+			for (int i = max(0, last - stages); i < last; i++) wait_some(&full[i % stages], (i / stages) & 1, state);
+		}
 		pdl_wait(); // beside the kernel of many rows, whose inputs were complete before it began, but not ahead of it to the join
 		return;
 	}
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 		const bool high = WIDE && rows > 8;
 		bool there = false; // the next tile
 		for (int j = x.j0; j < j1; j++, advance()) {
-			if (!there && !wait_for(&full[st], round, s_dead, a.c)) continue;
+			if (!there && !wait_for<!LIST>(&full[st], round, state, a.c)) continue;
 			const uint32_t tile = smem_u32(ring) + (uint32_t) st * Z::STAGE;
 			const int base = j * KT + warp * 16; // this warp's 16 keys
 			const bool tail = base + 16 > most;
@@ -448,7 +454,7 @@ __global__ void __launch_bounds__(MT, D == 256 ? 1 : 2) paged_mma_kernel(const _
 			const bool redo = s_ml[0].x != 0.f;
 			bar_sync(1, CW * 32);
 			const Piece y = x; // in memory only here
-			if (redo) redo_rows<T, MM, MM>(a, part, y, 0, reinterpret_cast<int*>(s_ml), s_o, tid, 1);
+			if (redo) redo_rows<T, MM, MM>(a, part, y, 0, state, reinterpret_cast<int*>(s_ml), s_o, tid, 1);
 		}
 	}
 }

@@ -120,8 +120,9 @@ struct TcShared {
 	uint64_t full[RING], empty[RING];
 	uint64_t drained[2], q_full[2], s_full[2][2], p_full[2][2], o_full[2][2]; // by half and by the tile's parity, so that nobody is ever two phases ahead of a wait
 	uint32_t tmem;
-	int dead, flag[2], ids[32];
-	float buf[2][256];
+	State state;
+	int flag[2], ids[32], sent; // tiles whose copies were sent
+	alignas(16) float buf[2][256]; // read 16 bytes at a time
 };
 
 // fp16 rounds probabilities to 0 beside which an infinite value should give an infinity: the infinities and NaNs of column after column that a lane's row sees are put where its sums go.  A
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	uint8_t* s_v = s_k + RING * 2 * KB;
 	TcShared& sh = *reinterpret_cast<TcShared*>(s_v + RING * 2 * KB);
 	uint8_t* s_plan = reinterpret_cast<uint8_t*>(&sh + 1);
+	static_assert(sizeof(TcShared) % 16 == 0 && offsetof(TcShared, buf) % 16 == 0, "what slow_row reads");
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	if (tid == 0) {
 		for (int i = 0; i < RING; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 2); }
@@ -188,7 +190,8 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			mbar_init(&sh.q_full[h], 1);
 			for (int b = 0; b < 2; b++) { mbar_init(&sh.s_full[h][b], 1); mbar_init(&sh.p_full[h][b], 4); mbar_init(&sh.o_full[h][b], 1); }
 		}
-		sh.dead = 0;
+		sh.state.init();
+		sh.sent = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 	}
 	if (warp == 1) {
@@ -234,28 +237,27 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				if (elect())
 					for (int i = 0; i < min(batch, tiles - j); i++) {
 						const int m = n + j + i, st = m % RING, slot = (key0 + (x.j0 + j + i) * KT) & (P - 1);
-						if (!(ok = wait_alone(&sh.empty[st], ((m / RING) & 1) ^ 1, &sh.dead, a.c))) break;
+						if (!(ok = wait_alone(&sh.empty[st], ((m / RING) & 1) ^ 1, &sh.state, a.c))) break;
 						mbar_expect_tx(&sh.full[st], (uint32_t) ((dc + vc) * KB));
 						copy_tile(smem_u32(s_k) + st * 2 * KB, &kmap, a.c.d, g, slot, per, W, sh.ids + i * per, a.c.pages, &sh.full[st]);
 						copy_tile(smem_u32(s_v) + st * 2 * KB, &vmap, a.c.dv, g, slot, per, W, sh.ids + i * per, a.c.pages, &sh.full[st]);
+						sh.sent = m + 1;
 					}
 				ok = __all_sync(0xffffffffu, ok);
 			}
-			if (!ok) // gave up: copies still on their way end first
-				for (int i = max(0, n - RING); i < n + tiles; i++) wait_some(&sh.full[i % RING], (i / RING) & 1);
 		} else if (warp <= 2) { // ---- products: one thread issues them, with nothing to compute but two additions to a descriptor ----
 			if (here && tiles) {
 				__syncwarp();
 				if (elect()) { // not `lane == 0`: in a branch that the compiler cannot tell to be one thread's, it does not keep the operands of unrolled products apart
 					const uint32_t id_s = instr<T>(KT, false), id_o = instr<T>((a.c.dv + 15) / 16 * 16, true), t_s = tmem + 128 * h;
 					const uint64_t q = desc_k(smem_u32(s_q)) + h * (2 * QB >> 4), k_at = desc_k(smem_u32(s_k)), v_at = desc_mn(smem_u32(s_v), KB);
-					ok = wait_alone(&sh.q_full[h], pieces & 1, &sh.dead, a.c);
+					ok = wait_alone(&sh.q_full[h], pieces & 1, &sh.state, a.c);
 					for (int j = -1; j < tiles && ok; j++) { // the scores of tile j + 1, then the second product of tile j
 						const int m = n + j, c = done + j;
 						if (j + 1 < tiles) {
-							if (!(ok = wait_alone(&sh.full[(m + 1) % RING], ((m + 1) / RING) & 1, &sh.dead, a.c))) break;
+							if (!(ok = wait_alone(&sh.full[(m + 1) % RING], ((m + 1) / RING) & 1, &sh.state, a.c))) break;
 							// Their buffer holds the P of the product before: only products into one accumulator are sure to follow one another, so its end is waited for
-							if (j > 0 && !(ok = wait_alone(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c))) break;
+							if (j > 0 && !(ok = wait_alone(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.state, a.c))) break;
 							fence_after();
 							const uint64_t kk = k_at + ((m + 1) % RING) * (2 * KB >> 4);
 							const uint32_t d = t_s + 64 * ((c + 1) & 1);
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 							commit(&sh.s_full[h][(c + 1) & 1]);
 						}
 						if (j < 0) continue;
-						if (!(ok = wait_alone(&sh.p_full[h][c & 1], (c >> 1) & 1, &sh.dead, a.c))) break;
+						if (!(ok = wait_alone(&sh.p_full[h][c & 1], (c >> 1) & 1, &sh.state, a.c))) break;
 						fence_after();
 						const uint64_t v = v_at + (m % RING) * (2 * KB >> 4);
 						const uint32_t prob = t_s + 64 * (c & 1);
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				}
 			} else if (lane == 0) // no rows in this half: the tiles are let go one by one all the same, so that this warp does not get ahead of their barriers' phases
 				for (int j = n; j < n + tiles && ok; j++)
-					if ((ok = wait_alone(&sh.full[j % RING], (j / RING) & 1, &sh.dead, a.c))) mbar_arrive(&sh.empty[j % RING]);
+					if ((ok = wait_alone(&sh.full[j % RING], (j / RING) & 1, &sh.state, a.c))) mbar_arrive(&sh.empty[j % RING]);
 			ok = __all_sync(0xffffffffu, ok);
 		} else if (warp >= 4 && here) { // ---- softmax ----
 			const int r = quad * 32 + lane, wt = tid & 127, row = h * HALF_ROWS + r, first = x.t * TC_ROWS + h * HALF_ROWS; // row of the half, of the unit; the half's first row of the segment
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				if (HALF_ROWS % a.rep == 0) { // whole tokens: the copy engine brings them, those of other sequences behind the last too (rows that nobody asks for)
 					asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // what the piece before has laid there on its way out
 					bar_sync(2 + h, 128);
-					if (wt < 32 && elect() && !*(volatile int*) &sh.dead) {
+					if (wt < 32 && elect() && !*(volatile int*) &sh.state.dead) {
 						mbar_expect_tx(&sh.q_full[h], (uint32_t) (dc * QB));
 						for (int i = 0; i < dc; i++)
 							asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(s_q + (h * 2 + i) * QB)),
@@ -319,14 +321,14 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 			for (int j = 0; j < tiles; j++) {
 				const int c = done + j, b = c & 1, base = (x.j0 + j) * KT;
 				const uint32_t t_s = tmem + 128 * h + 64 * b + lanes;
-				ok = wait_for(&sh.s_full[h][b], (c >> 1) & 1, &sh.dead, a.c) && ok;
+				ok = wait_for(&sh.s_full[h][b], (c >> 1) & 1, &sh.state, a.c) && ok;
 				fence_after();
 				uint32_t s[KT];
 				ld32(t_s, s);
 				ld32(t_s + 32, s + 32);
 				if (base + KT > p.most) { // slots that no row sees may hold anything: as zeros they add nothing
 					const int st = (n + j) % RING;
-					ok = wait_for(&sh.full[st], ((n + j) / RING) & 1, &sh.dead, a.c) && ok;
+					ok = wait_for(&sh.full[st], ((n + j) / RING) & 1, &sh.state, a.c) && ok;
 					for (int i = wt; i < (base + KT - p.most) * vc * 8; i += 128) {
 						const int rr = p.most - base + i / (vc * 8), cc = i % (vc * 8);
 						*reinterpret_cast<uint4*>(s_v + (st * 2 + (cc >> 3)) * KB + rr * 128 + ((cc & 7) << 4)) = make_uint4(0, 0, 0, 0);
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool grow = mx > m + Lift<T>::LAG;
 				if (j == 0) m = mx;
 				else if (__any_sync(0xffffffffu, grow)) { // rare: the sums so far are complete before they are rescaled
-					ok = wait_for(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.dead, a.c) && ok;
+					ok = wait_for(&sh.o_full[h][(c - 1) & 1], ((c - 1) >> 1) & 1, &sh.state, a.c) && ok;
 					fence_after();
 					const float to = grow ? mx : m, f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - to)) : 1.f;
 #pragma unroll 1
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				if (lane == 0) mbar_arrive(&sh.p_full[h][b]);
 			}
 			// ---- the piece's sums: 32 columns at a time through this warp's rows of Q, which no product reads any more, so that what is written lies side by side ----
-			if (tiles) ok = wait_for(&sh.o_full[h][(done + tiles - 1) & 1], ((done + tiles - 1) >> 1) & 1, &sh.dead, a.c) && ok;
+			if (tiles) ok = wait_for(&sh.o_full[h][(done + tiles - 1) & 1], ((done + tiles - 1) >> 1) & 1, &sh.state, a.c) && ok;
 			fence_after();
 			bool again = false;
 			uint8_t* stage = s_q + h * 2 * QB + quad * 32 * 128; // 32 rows of 128 bytes
@@ -457,7 +459,9 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool fix = again && mine && l == l && tiles && ok; // not where a score is NaN: all columns are
 				if (__any_sync(0xffffffffu, fix)) {
 					const Piece y = x;
+					if (lane == 0) atomicAdd(&sh.state.busy, 1);
 					put_infinities(a, part, y, row, lim, p.most, fix);
+					if (lane == 0) atomicAdd(&sh.state.busy, -1);
 				}
 			}
 			if (!p.prefix && tiles && x.j1 * KT > least && least < p.most) {
@@ -469,7 +473,7 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 				const bool redo = *(volatile int*) &sh.flag[h] != 0;
 				bar_sync(2 + h, 128);
 				const Piece y = x; // in memory only here
-				if (redo) redo_rows<T, TC_ROWS, HALF_ROWS>(a, part, y, h * HALF_ROWS, &sh.flag[h], sh.buf[h], wt, 2 + h);
+				if (redo) redo_rows<T, TC_ROWS, HALF_ROWS>(a, part, y, h * HALF_ROWS, &sh.state, &sh.flag[h], sh.buf[h], wt, 2 + h);
 			}
 		}
 		n += tiles;
@@ -478,12 +482,14 @@ __global__ void __launch_bounds__(TT, 1) paged_tc_kernel(const __grid_constant__
 	}
 	fence_before();
 	__syncthreads();
-	if (*(volatile int*) &sh.dead) { // a wait gave up: what is still on its way into shared or tensor memory ends first
+	if (*(volatile int*) &sh.state.dead) { // a wait gave up: what is still on its way into shared or tensor memory ends first
+		if (warp == 0)
+			for (int i = max(0, sh.sent - RING); i < sh.sent; i++) wait_some(&sh.full[i % RING], (i / RING) & 1, &sh.state);
 		if (warp == 1 || warp == 2) {
 			if (elect()) {
 				commit(&sh.drained[h]);
-				wait_some(&sh.drained[h], 0);
-				if (pieces) wait_some(&sh.q_full[h], (pieces - 1) & 1);
+				wait_some(&sh.drained[h], 0, &sh.state);
+				if (pieces) wait_some(&sh.q_full[h], (pieces - 1) & 1, &sh.state);
 			}
 			__syncwarp();
 		}

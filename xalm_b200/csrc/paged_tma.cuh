@@ -90,32 +90,70 @@ __device__ __forceinline__ bool try_wait_once(uint64_t* bar, uint32_t parity) {
 	    : "memory");
 	return __all_sync(0xffffffffu, ok != 0);
 }
-constexpr int WAIT_TRIES = 1 << 18; // about two seconds of suspended tries: far beyond what a copy or a product takes
-__device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity) {
-	for (int i = 0; i < WAIT_TRIES; i++)
+// How the warps of a CTA stand with one another, in shared memory
+struct State {
+	int dead; // a wait has given up: nobody waits any more
+	int busy; // warps that go over rows again key by key, which ends by itself but takes as long as it takes: no wait gives up meanwhile
+	unsigned since[12]; // of each warp's wait
+	__device__ __forceinline__ void init() { dead = busy = 0; }
+};
+// A wait gives up after two seconds, far beyond what a copy or a product takes.  By the clock: a try may be over at once (2^18 of them in 50 ms) or after microseconds.  The clock is looked at
+// every 4096 tries, by a call where the loops around it are short of registers (single tokens 49.3 us in place of 49.9, a group's 64 80.5 in place of 82.3), in the loop itself in the kernel
+// of lists (476 us in place of 502), which does no rows again.
+constexpr int WAIT_TRIES = 1 << 30, LOOK = 4096;
+__device__ __forceinline__ unsigned clock_us() { // nearly
+	unsigned long long ns;
+	asm volatile("mov.u64 %0, %globaltimer;" : "=l"(ns));
+	return (unsigned) (ns >> 10);
+}
+constexpr unsigned WAIT_US = 2000000;
+static __device__ __noinline__ bool waited_long(State* st, int tries) {
+	const unsigned now = clock_us();
+	volatile unsigned* since = &st->since[threadIdx.x >> 5];
+	if (tries < LOOK || *(volatile int*) &st->busy) *since = now;
+	return now - *since > WAIT_US;
+}
+template <bool CALL>
+__device__ __forceinline__ bool gives_up(State* st, int tries, unsigned& since) {
+	if ((tries & LOOK - 1) != LOOK - 1) return false;
+	if constexpr (CALL) return waited_long(st, tries);
+	const unsigned now = clock_us();
+	if (tries < LOOK) since = now;
+	return now - since > WAIT_US;
+}
+__device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity, State* st) {
+	unsigned since = 0;
+	for (int i = 0; i < WAIT_TRIES; i++) {
 		if (try_wait(bar, parity)) return true;
+		if (gives_up<true>(st, i, since)) return false;
+	}
 	return false;
 }
 // A wait of a whole warp that ends: when it gives up, or another of the CTA has, the status word says so and nobody waits any more
-__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* dead, const Cache& c) {
+template <bool CALL = true>
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, State* st, const Cache& c) {
 	bool ok = false;
+	unsigned since = 0;
 	for (int i = 0; i < WAIT_TRIES && !(ok = try_wait(bar, parity)); i++)
-		if (*(volatile int*) dead) break;
+		if (*(volatile int*) &st->dead || gives_up<CALL>(st, i, since)) break;
 	ok = __all_sync(0xffffffffu, ok);
-	if (!ok && !*(volatile int*) dead) {
-		*(volatile int*) dead = 1;
+	if (!ok && !*(volatile int*) &st->dead) {
+		*(volatile int*) &st->dead = 1;
 		report(c, ERR_WAIT);
 	}
 	return ok;
 }
 
 // The same for one thread
-__device__ __forceinline__ bool wait_alone(uint64_t* bar, uint32_t parity, int* dead, const Cache& c) {
+template <bool CALL = true>
+__device__ __forceinline__ bool wait_alone(uint64_t* bar, uint32_t parity, State* st, const Cache& c) {
+	unsigned since = 0;
 	for (int i = 0; i < WAIT_TRIES; i++) {
 		if (try_wait(bar, parity)) return true;
-		if (*(volatile int*) dead) return false;
+		if (*(volatile int*) &st->dead) return false;
+		if (gives_up<CALL>(st, i, since)) break;
 	}
-	*(volatile int*) dead = 1;
+	*(volatile int*) &st->dead = 1;
 	report(c, ERR_WAIT);
 	return false;
 }
@@ -180,7 +218,7 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 			s = 0.f;
 			if (pg >= 0) {
 				const T* kk = reinterpret_cast<const T*>(a.c.k) + pg * a.c.k_page + (key & (P - 1)) * a.c.k_slot + x.g * a.c.k_head;
-#pragma unroll 4
+#pragma unroll 8
 				for (int i = 0; i < a.c.d; i += 8) {
 					float u[8], w[8];
 					load8(q + i, u);
@@ -205,14 +243,25 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 		l *= f;
 		acc[0] *= f;
 		acc[1] *= f;
-#pragma unroll 8
-		for (int i = 0; i < min(128, last - kb); i++) {
-			const int key = x.key0 + kb + i, pg = page_of(a.c, a.b, x.s, key >> a.c.shift);
-			l += buf[i];
-			if (pg < 0) continue;
-			const T* v = reinterpret_cast<const T*>(a.c.v) + pg * a.c.v_page + (key & (P - 1)) * a.c.v_slot + x.g * a.c.v_head;
-			for (int c = 0; c < 2; c++)
-				if (c * 128 + tid < a.c.dv) acc[c] = fmaf(buf[i], to_f(v[c * 128 + tid]), acc[c]);
+		const int n = min(128, last - kb);
+		int next = page_of(a.c, a.b, x.s, (x.key0 + kb) >> a.c.shift);
+		for (int i0 = 0; i0 < n; i0 += 16) { // the values of sixteen keys, which lie in one page, on their way at a time, and the number of the next ones' page
+			const int pg = next, key = x.key0 + kb + i0;
+			if (i0 + 16 < n) next = page_of(a.c, a.b, x.s, (key + 16) >> a.c.shift);
+			const T* at = reinterpret_cast<const T*>(a.c.v) + max(pg, 0) * a.c.v_page + (key & (P - 1)) * a.c.v_slot + x.g * a.c.v_head;
+			float p[16], v[16][2];
+#pragma unroll
+			for (int e = 0; e < 16; e++) {
+				p[e] = i0 + e < n ? buf[i0 + e] : 0.f;
+#pragma unroll
+				for (int c = 0; c < 2; c++) v[e][c] = pg >= 0 && i0 + e < n && c * 128 + tid < a.c.dv ? to_f(at[e * a.c.v_slot + c * 128 + tid]) : 0.f;
+			}
+#pragma unroll
+			for (int e = 0; e < 16; e++) {
+				l += p[e];
+				acc[0] = fmaf(p[e], v[e][0], acc[0]);
+				acc[1] = fmaf(p[e], v[e][1], acc[1]);
+			}
 		}
 		bar_sync(bar, 128);
 	}
@@ -226,13 +275,17 @@ __device__ __noinline__ void slow_row(const Attn& a, const Part& part, const Pie
 
 // ROWS rows from r0 on of an own segment's unit of M, some of which did not come out finite: of the keys that not all of the unit's rows see, the last whose value is not finite is looked for, and
 // the rows that do not see it are done again.  128 threads; mark: an int in shared memory.  (What can be told from the piece is, in here: more arguments took half a microsecond from short calls.)
+// A row takes some 30 us to 128 keys: 96 rows behind 1600 tokens 39 ms.
 template <typename T, int M, int ROWS>
-__device__ __noinline__ void redo_rows(const Attn& a, const Part& part, const Piece& x, int r0, int* mark, float* buf, int tid, int bar) {
+__device__ __noinline__ void redo_rows(const Attn& a, const Part& part, const Piece& x, int r0, State* st, int* mark, float* buf, int tid, int bar) {
 	const int rows = min(M, x.rows - x.t * M);
 	const bool direct = x.j0 == 0 && x.j1 == x.w && x.key0 == 0;
 	const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
 	auto seen = [&](int r) { return own_keys(x.q, x.key0, a.rep, x.t * M + r); };
-	if (tid == 0) *mark = -1;
+	if (tid == 0) {
+		*mark = -1;
+		atomicAdd(&st->busy, 1);
+	}
 	bar_sync(bar, 128);
 	const int found = last_infinite<T>(a, x, max(seen(0), x.j0 * KT), min(seen(rows - 1), x.j1 * KT), tid);
 	if (found >= 0) atomicMax(mark, found);
@@ -241,6 +294,7 @@ __device__ __noinline__ void redo_rows(const Attn& a, const Part& part, const Pi
 	bar_sync(bar, 128);
 	for (int r = r0; r < min(rows, r0 + ROWS); r++)
 		if (seen(r) <= last) slow_row<T>(a, part, x, M, r, seen(r), buf, direct, slot, tid, bar);
+	if (tid == 0) atomicAdd(&st->busy, -1);
 }
 
 } // namespace paged
