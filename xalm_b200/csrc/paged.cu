@@ -64,9 +64,10 @@ __global__ void __launch_bounds__(AT) paged_append_kernel(const __grid_constant_
 		if (row < a.b.N) {
 			const int s = seq_of_row(a.b, row);
 			const View view = view_of(a.c, a.b);
-			const Seq q = seq_of(view, s);
+			int whole;
+			const Seq q = seq_of(view, s, whole);
 			if (row_in_seq(q, row)) {
-				pos = max(a.b.lens[s], 0) - q.n + row - q.a; // not cut to the table: what lies behind it is turned, and written nowhere
+				pos = whole - q.n + row - q.a; // what lies behind the table is turned, and written nowhere
 				if (pos >= 0 && pos < view.cap) {
 					page = page_of(a.c, a.b, s, pos >> a.c.shift);
 					if (page < 0 && (tid & 31) == 0) report(a.c, ERR_PAGE);
@@ -166,8 +167,9 @@ __global__ void __launch_bounds__(128) paged_means_kernel(const Cache c, const B
 		lo += k * step;
 		n = min(step, n - k * step);
 	}
-	const Seq q = seq_of(view_of(c, b), lo);
-	const int first = max(max(b.lens[lo], 0) - q.n, 0) >> c.shift; // page of the first new token
+	int whole;
+	const Seq q = seq_of(view_of(c, b), lo, whole);
+	const int first = max(whole - q.n, 0) >> c.shift; // page of the first new token
 	const int j = first + item - ((q.a >> c.shift) + lo);
 	if (q.n == 0 || j < first || (long long) (j + 1) << c.shift > q.len) return; // not filled
 	const int page = page_of(c, b, lo, j);

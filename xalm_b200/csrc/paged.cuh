@@ -48,12 +48,17 @@ __device__ __forceinline__ View view_of(const Cache& c, const BatchView& b) {
 struct Seq {
 	int a, n, len;
 };
-__device__ __forceinline__ Seq seq_of(const View& v, int s) {
+__device__ __forceinline__ Seq seq_of(const View& v, int s, int& whole) { // whole: its length, not cut to the table
 	Seq q;
 	q.a = min(max(v.starts[s], 0), v.N);
 	q.n = min(max(v.starts[s + 1], q.a), v.N) - q.a;
-	q.len = min(max(v.lens[s], 0), v.cap);
+	whole = max(v.lens[s], 0);
+	q.len = min(whole, v.cap);
 	return q;
+}
+__device__ __forceinline__ Seq seq_of(const View& v, int s) {
+	int whole;
+	return seq_of(v, s, whole);
 }
 __device__ __forceinline__ bool seq_ok(const View& v, int s) {
 	const int a = v.starts[s], e = v.starts[s + 1], l = v.lens[s];
