@@ -310,8 +310,10 @@ int xalm_cuda_moe_chosen(float* x_io, float* out_pairs, int* idx, float* wgt, co
  *   finite number, +infinity as the largest.  out (rows, kv_heads, top).  first + recent + 1 <= top <= 1024, max_pages <= 24576.
  * paged_attend_selected: paged_attend over the listed pages only (rows, kv_heads, n_lists <= 1024), in any order; entries outside 0 .. the row's own page are passed
  *   over, a page counts once.
- * Both attend in one pass: scores, maxima and sums in fp32; 16-bit caches' probabilities enter the second product as two numbers of the cache's type where a segment has up to 16
- *   (token, head) rows to a kv head, as one of them where it has more.  The same call gives the same bits every time.
+ * Both attend in one pass: scores, maxima and sums in fp32.  16-bit caches' probabilities enter the second product as two numbers of the cache's type, but as one in paged_attend where more than
+ *   16 (token, head) rows to a kv head read the same keys, heads have at most 128 entries and the call has more than 64 such rows and more tokens than sequences, or groups; fp16 then loses bits
+ *   of what is below 2^-27 of a row's largest probability, and below 2^-38 counts it in the denominator alone.  The same call gives the same bits every time; a row's last bits may be others in
+ *   another batch.
  * paged_status: *taken (device memory) becomes the status word, which becomes 0, in one exchange behind what the stream holds: a bit that a kernel sets at the same time is in this word or
  *   stays for the next.  What other streams hold has reported when they are done.
  * paged_workspace: bytes of workspace (at a 256-byte boundary) that paged_attend (n_lists 0) and paged_attend_selected need for these sizes; its contents need no preparation. */

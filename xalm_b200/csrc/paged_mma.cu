@@ -14,7 +14,8 @@ namespace paged {
 // 64 sequences below behind 8192 tokens in common), with maximum, sum and output of their own, so that
 // none waits for another and a stage is free again after a quarter of a tile's work: scores and sums by mma.sync m16n8k16 with the 16 rows as A, queries and sums in registers.
 // At the end of a piece the four join through shared memory.  (tcgen05 would want 64 rows or more: a step of four heads to a kv head has four.)
-// 64 sequences of up to 1500 tokens, 8 kv heads of 128: 43 us, 4.6 TB/s of pages at random; 10700 lists of 16 pages of 64, which L2 has, 485 us, 12.1 TB/s.
+// 64 sequences of 1000 to 2000 tokens, 8 kv heads of 128: 78 us with the join, 5.0 TB/s, 128 of 4000 325 us, 6.5 TB/s, wherever the pages lie; 10700 lists of 16 pages of 64, which L2 has, 474 us,
+// 12.4 TB/s.
 // Probabilities enter the second product in two parts of the cache's type, rounded and what that left (one alone had 1.5 times the result's own rounding as its error): of up to eight rows
 // the second part are rows 8 to 15 of the same product, of more it costs a product of its own.  Scores, maxima and sums are fp32.
 // fp16 ends at 2^-24, so its probabilities are lifted by 2^12, its second part by 2^11 more into sums of its own: what a probability loses is below 2^-47 of the row's largest one, and
