@@ -344,6 +344,48 @@ int xalm_cuda_paged_attend_selected(const xalm_paged_cache* cache, const xalm_pa
 int xalm_cuda_paged_status(const xalm_paged_cache* cache, int* taken, void* cuda_stream);
 int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_batch* batch, int heads, int n_lists, size_t* bytes);
 
+/* ---- the same over a cache held in 4 bits -------------------------------------------------------------------------------------------------------
+ * Entries are stored in blocks of 32 neighbours of a head (behind its last entry, zeros): x stands as d (c - 8), d in fp16, c in 0 .. 15.  With M the block's entry of the largest magnitude
+ * (the positive one where both signs have it), d = fp16(-M / 8), at most 65504 in magnitude, and c = clamp(rint(x / d) + 8, 0, 15), halves to the even number; 8 where d is 0.  A block with
+ * an infinity or a NaN reads as NaN.  Rows of f16, bf16 and f32 alike; batches, tables, streams, rows, status bits and overlaps are as above.
+ *
+ * xalm_paged4_cache: a page has a run of bytes for each kv head, `head` bytes apart, pages `page` bytes apart (either may be the larger; multiples of 16; the pool at a 16-byte boundary).
+ *   page_size 16, 32, 64, 128 or 256 slots; dim, vdim multiples of 8, at most 256.  With K and V the blocks of a slot's key and value (2, 4 or 8: heads up to 64, 128 and 256 entries), a run is
+ *   the slots' key codes (16 K bytes each), the keys' scales (2 K), value codes (16 V) and scales (2 V): page_size 18 (K + V) bytes.  Entry 32 g + 8 t + i of a key (t < 4, i < 8) is in byte
+ *   4 K t + 4 g + i / 2 of its codes, entry 32 g + 4 u + i of a value (u < 8, i < 4) in byte 2 V u + 2 g + i / 2; even entries in the low half.
+ * paged4_append: as paged_append; keys are turned in 64 bits and rounded to fp32 before they are stored, so that what is stored is the definition's; q_out has the rows' type, apart from q.
+ * paged4_read: keys (rows, kv_heads dim) and values (rows, kv_heads vdim) at the batch's rows as the blocks stand for them, in `type`, rounded once; zeros where the table has no page for a row
+ *   (with its status bit); rows outside every sequence, and before their sequence's first token, are left alone.
+ * paged4_attend: as paged_attend; queries and results have `type`, whatever was appended.  Scores, maxima and sums in fp32; products of probability and scale enter the second product as two fp16
+ *   numbers, with a row's largest scale as unit: of a block whose scale is 2^-20 of its row's largest, 2^-18 of the result's precision is left.  fp32 queries enter the first as two.
+ * paged4_status, paged4_workspace: as above. */
+typedef struct xalm_paged4_cache {
+	int device;
+	int pages, page_size, kv_heads, dim, vdim;
+	void* pool;
+	long long page, head;
+	int* status;
+} xalm_paged4_cache;
+int xalm_cuda_paged4_append(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, const void* k, long long k_row, const void* v, long long v_row, const void* q,
+                            long long q_row, int heads, int type, void* q_out, long long q_out_row, const float* freq, int rot_half, float rot_mag, int neighbours,
+                            void* cuda_stream);
+int xalm_cuda_paged4_read(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, int type, void* k, long long k_row, void* v, long long v_row, void* cuda_stream);
+int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, int type, float scale, void* out,
+                            long long out_row, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream);
+int xalm_cuda_paged4_status(const xalm_paged4_cache* cache, int* taken, void* cuda_stream);
+int xalm_cuda_paged4_workspace(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, int type, int heads, size_t* bytes);
+
+/* verify_drafts: sequence s has rows starts[s] .. starts[s + 1] - 1 of `rows` (starts has seqs + 1 entries, ascending; at most 65535 sequences); the first is the token that it had, those behind
+ * it its drafts.  tokens (rows): what each row stands for.  target (rows, vocab): the target's probabilities of the token behind each row, draft (rows, vocab): the distributions that the drafts
+ * were drawn from, row i that of tokens[i + 1] (a sequence's last row is not read), or NULL: each draft was certain.  Both of `type`, rows *_row elements apart; they need not sum to 1, and
+ * what is negative or no number counts as zero.  accept (rows), pick (seqs): numbers from 0 to below 1.
+ * Draft i is taken where accept[i] draft[i][x] < target[i][x], x = tokens[i + 1], in exact arithmetic (a token outside the vocabulary is not); taken[s]: how many are, up to the first that is
+ * not.  out[starts[s] + i]: for i < taken[s] the draft, behind these a token drawn from max(target - draft, 0) of the row whose draft was not taken (target without the draft, where that was
+ * certain; all of target where every draft is taken, or where nothing is left): the lowest whose sum, in 64 bits, passes pick[s] times the total (for a number that is not below 1 the last that
+ * has a weight), -1 where the target has none; then -1.  Rows outside every sequence are left alone; taken is 0 for sequences without rows.  device: whose memory this is. */
+int xalm_cuda_verify_drafts(int device, int type, int seqs, int rows, int vocab, const int* starts, const int* tokens, const void* target, long long target_row, const void* draft,
+                            long long draft_row, const float* accept, const float* pick, int* out, int* taken, void* cuda_stream);
+
 /* Tensor parallel plumbing (no reference analogue).  Rank 0 makes an id, the host side ships it to
  * the other ranks (torch.distributed / MPI / a file), every rank calls comm_init before finalize. */
 #define XALM_COMM_ID_BYTES 128

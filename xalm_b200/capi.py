@@ -126,6 +126,12 @@ SYMBOLS = {
     "xalm_cuda_paged_attend_selected": (_i, [_vp, _vp, _vp, C.c_longlong, _i, _vp, _i, C.c_float, _vp, C.c_longlong, _vp, _vp, _sz, _vp]),
     "xalm_cuda_paged_status": (_i, [_vp, _vp, _vp]),
     "xalm_cuda_paged_workspace": (_i, [_vp, _vp, _i, _i, C.POINTER(_sz)]),
+    "xalm_cuda_paged4_append": (_i, [_vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong, _i, _i, _vp, C.c_longlong, _vp, _i, C.c_float, _i, _vp]),
+    "xalm_cuda_paged4_read": (_i, [_vp, _vp, _i, _vp, C.c_longlong, _vp, C.c_longlong, _vp]),
+    "xalm_cuda_paged4_attend": (_i, [_vp, _vp, _vp, C.c_longlong, _i, _i, C.c_float, _vp, C.c_longlong, _vp, _vp, _sz, _vp]),
+    "xalm_cuda_paged4_status": (_i, [_vp, _vp, _vp]),
+    "xalm_cuda_paged4_workspace": (_i, [_vp, _vp, _i, _i, C.POINTER(_sz)]),
+    "xalm_cuda_verify_drafts": (_i, [_i] * 5 + [_vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong] + [_vp] * 5),
 }
 PRECISION_BF16, PRECISION_F32 = 0, 1            # enum xalm_precision
 

@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "family.h"
+#include "paged_check.h"
 
 namespace xalm {
 namespace paged {
@@ -636,13 +637,13 @@ static int select_typed(const SelectArgs& a, int sms, cudaStream_t s) {
 }
 
 __global__ void paged_status_kernel(int* status, int* taken) { *taken = atomicExch(status, 0); }
+int launch_status(int* status, int* taken, cudaStream_t s) {
+	paged_status_kernel<<<1, 1, 0, s>>>(status, taken);
+	XALM_CUDA_CHECK(cudaGetLastError());
+	return XALM_OK;
+}
 
 // ---- checks and launches -----------------------------------------------------------------------------------------------------------------------
-static int element_bytes(int type) { return type == XALM_F32 ? 4 : 2; }
-static bool is_type(int type) { return type == XALM_F32 || type == XALM_F16 || type == XALM_BF16; }
-static bool aligned16(const void* p) { return ((uintptr_t) p & 15) == 0; }
-static bool aligned4(const void* p) { return ((uintptr_t) p & 3) == 0; }
-
 static int check_strides(const char* what, int G, int P, int pages, int dim, int bytes, long long page, long long slot, long long head) {
 	const long long most = 1ll << 40;
 	if (page <= 0 || slot <= 0 || head <= 0 || page >= most || slot >= most || head >= most || page * bytes % 16 || slot * bytes % 16 || head * bytes % 16)
@@ -670,85 +671,14 @@ static int check_cache(const xalm_paged_cache* c, Cache& o) {
 	          c->pages, shift, c->kv_heads, c->dim, c->vdim, c->status};
 	return XALM_OK;
 }
-static int check_batch(const xalm_paged_batch* b, const Cache& c, BatchView& o) {
-	if (!b) return set_error(XALM_ERR_INVALID, "paged cache: batch is NULL");
-	if (b->rows < 0 || b->seqs < 0 || b->max_pages < 0 || b->groups < 0 || b->table_row < b->max_pages)
-		return set_error(XALM_ERR_INVALID, "paged cache: %d rows, %d sequences of %d pages (rows %lld apart), %d groups", b->rows, b->seqs, b->max_pages, b->table_row, b->groups);
-	if ((long long) b->seqs + b->groups > MAX_SEGMENTS) return set_error(XALM_ERR_INVALID, "paged cache: %d sequences and %d groups are more than %d", b->seqs, b->groups, MAX_SEGMENTS);
-	if ((long long) b->max_pages << c.shift > 1ll << 30) return set_error(XALM_ERR_INVALID, "paged cache: tables of %d pages of %d tokens (at most 2^30 tokens)", b->max_pages, 1 << c.shift);
-	if (b->seqs && (!b->starts || !b->lens || (b->max_pages && !b->table))) return set_error(XALM_ERR_INVALID, "paged cache: starts/lens/table is NULL");
-	if (b->groups && (!b->group_bounds || !b->group_shared)) return set_error(XALM_ERR_INVALID, "paged cache: group_bounds/group_shared is NULL");
-	for (const int* p : {b->starts, b->lens, b->table, b->group_bounds, b->group_shared})
-		if (!aligned4(p)) return set_error(XALM_ERR_INVALID, "paged cache: starts, lens, table and groups are at 4-byte boundaries");
-	o = BatchView{b->rows, b->seqs, b->max_pages, b->groups, b->starts, b->lens, b->table, b->table_row, b->group_bounds, b->group_shared};
-	return XALM_OK;
-}
-static int check_rows(const char* what, const void* p, long long row, int least, int bytes) {
-	if (!p || !aligned16(p) || row < least || row * bytes % 16)
-		return set_error(XALM_ERR_INVALID, "paged cache: rows of %s are at 16-byte boundaries, %d entries or more apart, and not NULL", what, least);
-	return XALM_OK;
-}
-
-// Whether n rows of so many bytes each meet: rows that lie side by side in wider ones of the same stride do not
-static bool rows_meet(const void* p, long long p_row, long long p_bytes, const void* q, long long q_row, long long q_bytes, int n) {
-	const uintptr_t a = (uintptr_t) p, b = (uintptr_t) q;
-	if (a >= b + (n - 1) * q_row + q_bytes || b >= a + (n - 1) * p_row + p_bytes) return false;
-	if (p_row != q_row) return true;
-	const long long off = (long long) (b - a) % p_row, at = off < 0 ? off + p_row : off; // from a row of p to the next of q
-	return at < p_bytes || at + q_bytes > p_row;
-}
-
-// What a call writes lies apart from what it reads and from what else it writes
-struct Span {
-	const char* what;
-	const void* at;
-	long long bytes;
-};
-static Span rows_span(const char* what, const void* p, long long row, long long width, int n, int bytes) { return Span{what, p, ((n - 1) * row + width) * bytes}; }
 static Span pool_span(const char* what, const Cache& c, const void* p, int dim, int e, long long page, long long slot, long long head) {
 	return Span{what, p, ((c.pages - 1) * page + ((1 << c.shift) - 1) * slot + (c.G - 1) * head + dim) * e};
-}
-template <int N>
-static int check_apart(const char* call, const Span& out, const Span (&others)[N]) {
-	const uintptr_t a = (uintptr_t) out.at;
-	for (const Span& x : others) {
-		const uintptr_t b = (uintptr_t) x.at;
-		if (a && b && out.bytes > 0 && x.bytes > 0 && a < b + x.bytes && b < a + out.bytes) return set_error(XALM_ERR_INVALID, "%s: %s overlaps %s", call, out.what, x.what);
-	}
-	return XALM_OK;
 }
 static int check_apart_from_cache(const char* call, const Span& out, const Cache& c, const BatchView& b, int e) {
 	return check_apart(call, out, {pool_span("the keys' pool", c, c.k, c.d, e, c.k_page, c.k_slot, c.k_head), pool_span("the values' pool", c, c.v, c.dv, e, c.v_page, c.v_slot, c.v_head),
 	                               Span{"the mean keys", c.means, (long long) c.pages * c.G * c.d * e}, Span{"the status word", c.status, 4}, Span{"starts", b.starts, 4ll * (b.B + 1)},
 	                               Span{"lens", b.lens, 4ll * b.B}, rows_span("the table", b.table, b.table_row, b.max_pages, b.B, 4),
 	                               Span{"group_bounds", b.bounds, 4ll * (b.n_groups + 1)}, Span{"group_shared", b.shared, 4ll * b.n_groups}});
-}
-
-// The calling thread's device is what it was when the call returns
-struct OnDevice {
-	int before = -1;
-	int set(int device) {
-		XALM_CUDA_CHECK(cudaGetDevice(&before));
-		if (before == device) before = -1;
-		else {
-			const cudaError_t e = cudaSetDevice(device);
-			if (e != cudaSuccess) {
-				before = -1;
-				return set_error(XALM_ERR_CUDA, "cudaSetDevice(%d) failed: %s", device, cudaGetErrorString(e));
-			}
-		}
-		return XALM_OK;
-	}
-	~OnDevice() {
-		if (before >= 0) cudaSetDevice(before);
-	}
-};
-static int sm_count(int device, int* n) {
-	static int known[64]; // the same number whoever writes it
-	if (device >= 0 && device < 64 && known[device]) { *n = known[device]; return XALM_OK; }
-	XALM_CUDA_CHECK(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, device));
-	if (device >= 0 && device < 64) known[device] = *n;
-	return XALM_OK;
 }
 
 // Segments of up to 16 (token, head) rows fill one tile of mma.sync, more go to tcgen05's tiles of 256: with 32 rows for either, 8 prompts of 8 tokens behind 4000 take 66 us in place of 54,
@@ -972,9 +902,7 @@ int xalm_cuda_paged_status(const xalm_paged_cache* cache, int* taken, void* stre
 	if (!taken || !c.status || !aligned4(taken)) return set_error(XALM_ERR_INVALID, "paged status: %s", !taken || !c.status ? "taken or the cache's status word is NULL" : "taken is not at a 4-byte boundary");
 	OnDevice on;
 	XALM_TRY(on.set(cache->device));
-	paged_status_kernel<<<1, 1, 0, (cudaStream_t) stream>>>(c.status, taken);
-	XALM_CUDA_CHECK(cudaGetLastError());
-	return XALM_OK;
+	return launch_status(c.status, taken, (cudaStream_t) stream);
 }
 
 int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_batch* batch, int heads, int n_lists, size_t* bytes) {

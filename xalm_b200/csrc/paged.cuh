@@ -552,6 +552,7 @@ inline cudaError_t launch(K kernel, dim3 grid, int block, size_t smem, cudaStrea
 	return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 int launch_join(const Attn& a, int type, cudaStream_t s);
+int launch_status(int* status, int* taken, cudaStream_t s);
 // CTAs per SM that a kernel's shared memory leaves room for, and its launch: fp32 caches, 16-bit caches
 int rows_ctas_per_sm(const Cache& c, const BatchView& b, int n_lists);
 int launch_attn_rows(const Attn& a, cudaStream_t s);

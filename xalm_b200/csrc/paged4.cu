@@ -1,0 +1,426 @@
+// paged4.cu — the paged cache of 4-bit numbers: entry points (include/xalm_cuda.h, xalm_cuda_paged4_*), appending to pages, reading rows back.
+#include "paged4.cuh"
+
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged_check.h"
+
+namespace xalm {
+namespace paged {
+
+// =========================================================================================================================================
+// append: keys turned by their positions, then blocks of 32 entries: M the entry of the largest magnitude (the positive one where both signs have it), d = fp16(-M / 8), code =
+// clamp(rint(x / d) + 8, 0, 15).  What is stored does not depend on how a sum was rounded: a turned key is the fp32 number next to the turn in 64 bits, and x / d as fp32 rounds it is on the
+// same side of every n + 1/2 as the quotient itself, because d (n + 1/2) has 16 bits: where x differs from it, then by a unit of x's last place at least, and the quotient by more than half
+// a unit of its own.
+// =========================================================================================================================================
+struct Append4Args {
+	Cache c;
+	BatchView b;
+	Pool4 pool;
+	const uint8_t *k, *v, *q;
+	long long k_row, v_row, q_row, q_out_row;
+	uint8_t* q_out;
+	int H;
+	const float* freq;
+	int rot;
+	float mag;
+	int neighbours;
+};
+
+constexpr int A4T = 256;
+
+// position of a row (-1: of no sequence, or before its first token) and the page of the pool that has it (-1: none); by a whole warp
+__device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int row, bool& in_seq) {
+	int pos = -1, page = -1;
+	in_seq = false;
+	if (row < b.N) {
+		const int s = seq_of_row(b, row);
+		const View view = view_of(c, b);
+		int whole;
+		const Seq q = seq_of(view, s, whole);
+		if (row_in_seq(q, row)) {
+			in_seq = true;
+			pos = whole - q.n + row - q.a; // what lies behind the table is turned, and written nowhere
+			if (pos >= 0 && pos < view.cap) {
+				page = page_of(c, b, s, pos >> c.shift);
+				if (page < 0 && (threadIdx.x & 31) == 0) report(c, ERR_PAGE);
+			}
+		}
+	}
+	return make_int2(pos, page);
+}
+
+// Eight entries from c on of the head at p (n entries), turned
+template <typename I>
+__device__ __forceinline__ void turned8(const I* p, int c, const Append4Args& a, const double* cs, const double* sn, float (&x)[8]) {
+	load8(p + c, x);
+	if (c >= 2 * a.rot) return;
+#pragma unroll
+	for (int e = 0; e < 8; e++) {
+		const int i = c + e;
+		if (i >= 2 * a.rot) continue;
+		const bool second = a.neighbours ? i & 1 : i >= a.rot;
+		const int f = a.neighbours ? i >> 1 : second ? i - a.rot : i;
+		const double o = (double) to_f(p[a.neighbours ? i ^ 1 : second ? f : i + a.rot]), y = (double) to_f(p[i]);
+		x[e] = (float) ((second ? y * cs[f] + o * sn[f] : y * cs[f] - o * sn[f]) * (double) a.mag);
+	}
+}
+
+// What four lanes have of a block, eight entries each: scale and codes (entry i at bit 4 i)
+__device__ __forceinline__ uint32_t block4(const float (&x)[8], unsigned quad, __half& scale) {
+	float hi = x[0], lo = x[0];
+	bool odd = false;
+#pragma unroll
+	for (int e = 0; e < 8; e++) {
+		hi = fmaxf(hi, x[e]);
+		lo = fminf(lo, x[e]);
+		odd = odd || !(fabsf(x[e]) <= 3.402823466e38f);
+	}
+#pragma unroll
+	for (int o = 1; o < 4; o <<= 1) {
+		hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
+		lo = fminf(lo, __shfl_xor_sync(quad, lo, o));
+	}
+	odd = __any_sync(quad, odd);
+	scale = __float2half_rn(fminf(fmaxf((hi >= -lo ? hi : lo) * -0.125f, -65504.f), 65504.f));
+	const float d = __half2float(scale);
+	uint32_t w = 0;
+#pragma unroll
+	for (int e = 0; e < 8; e++) {
+		const int c = d == 0.f || odd ? 8 : (int) fminf(fmaxf(rintf(__fdiv_rn(x[e], d)) + 8.f, 0.f), 15.f);
+		w |= (uint32_t) c << (4 * e);
+	}
+	if (odd) scale = __ushort_as_half((unsigned short) 0x7fff); // a block with what is no finite number reads as none
+	return w;
+}
+
+template <typename I, int R>
+__global__ void __launch_bounds__(A4T) paged4_append_kernel(const __grid_constant__ Append4Args a) {
+	__shared__ double s_cos[R][128], s_sin[R][128];
+	__shared__ int s_pos[R], s_page[R];
+	const int row0 = blockIdx.x * R, tid = threadIdx.x, warp = tid >> 5, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
+	if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, A4T);
+	if (warp < R) {
+		bool in_seq;
+		const int2 p = place_of(a.c, a.b, row0 + warp, in_seq);
+		if ((tid & 31) == 0) { s_pos[warp] = in_seq ? p.x : -1; s_page[warp] = p.y; }
+	}
+	__syncthreads();
+	for (int i = tid; i < R * a.rot; i += A4T) {
+		const int r = i / a.rot, f = i - r * a.rot;
+		if (s_pos[r] < 0) continue;
+		sincos((double) s_pos[r] * (double) a.freq[f], &s_sin[r][f], &s_cos[r][f]);
+	}
+	__syncthreads();
+	const int per_q = d / 8, n_q = a.q ? a.H * per_q : 0, n_k = G * KG * 4, n_v = G * VG * 4, slot_mask = (1 << shift) - 1;
+	for (int r = 0; r < R; r++) {
+		if (s_pos[r] < 0) continue;
+		const long long row = row0 + r;
+		for (int i = tid; i < n_q; i += A4T) {
+			const int h = i / per_q, c = (i - h * per_q) * 8;
+			float x[8];
+			turned8(reinterpret_cast<const I*>(a.q) + row * a.q_row + h * d, c, a, s_cos[r], s_sin[r], x);
+			store8(reinterpret_cast<I*>(a.q_out) + row * a.q_out_row + h * d + c, x);
+		}
+		if (s_page[r] < 0) continue;
+		const int slot = s_pos[r] & slot_mask;
+		uint8_t* page = a.pool.at + s_page[r] * a.pool.page;
+		for (int i = tid; i < n_k + n_v; i += A4T) {
+			const bool value = i >= n_k;
+			const int j = value ? i - n_k : i, per = (value ? VG : KG) * 4, h = j / per, chunk = j - h * per, g = chunk >> 2, t = chunk & 3, c = chunk * 8;
+			float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+			if (value) {
+				if (c < dv) load8(reinterpret_cast<const I*>(a.v) + row * a.v_row + h * dv + c, x);
+			} else if (c < d) turned8(reinterpret_cast<const I*>(a.k) + row * a.k_row + h * d, c, a, s_cos[r], s_sin[r], x);
+			__half scale;
+			const uint32_t w = block4(x, 0xfu << (tid & 28), scale);
+			uint8_t* run = page + h * a.pool.head;
+			if (value) {
+				uint8_t* at = run + values_at(KG, shift) + slot * (VG * 16) + g * 2;
+				*reinterpret_cast<uint16_t*>(at + (2 * t) * (VG * 2)) = (uint16_t) w;
+				*reinterpret_cast<uint16_t*>(at + (2 * t + 1) * (VG * 2)) = (uint16_t) (w >> 16);
+				if (t == 0) *reinterpret_cast<__half*>(run + value_scales_at(KG, VG, shift) + slot * (VG * 2) + g * 2) = scale;
+			} else {
+				*reinterpret_cast<uint32_t*>(run + slot * (KG * 16) + t * (KG * 4) + g * 4) = w;
+				if (t == 0) *reinterpret_cast<__half*>(run + key_scales_at(KG, shift) + slot * (KG * 2) + g * 2) = scale;
+			}
+		}
+	}
+}
+
+// =========================================================================================================================================
+// read: rows of keys and values as the blocks stand for them, d (c - 8), exact in fp32 and rounded once in 16 bits.
+// =========================================================================================================================================
+struct Read4Args {
+	Cache c;
+	BatchView b;
+	Pool4 pool;
+	uint8_t *k, *v;
+	long long k_row, v_row;
+};
+template <typename T>
+__global__ void __launch_bounds__(A4T) paged4_read_kernel(const __grid_constant__ Read4Args a) {
+	__shared__ int s_pos, s_page;
+	const int row = blockIdx.x, tid = threadIdx.x, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
+	if (row == 0) check_seqs(a.c, a.b, tid, A4T);
+	if (tid < 32) {
+		bool in_seq;
+		const int2 p = place_of(a.c, a.b, row, in_seq);
+		if (tid == 0) { s_pos = in_seq ? p.x & ((1 << shift) - 1) : -1; s_page = p.y; }
+	}
+	__syncthreads();
+	if (s_pos < 0) return;
+	const int per_k = d / 8, per_v = dv / 8, n_k = G * per_k, n_all = n_k + G * per_v, slot = s_pos, page = s_page;
+	for (int i = tid; i < n_all; i += A4T) {
+		const bool value = i >= n_k;
+		const int j = value ? i - n_k : i, per = value ? per_v : per_k, h = j / per, chunk = j - h * per, g = chunk >> 2, t = chunk & 3;
+		uint32_t w = 0x88888888u;
+		__half scale = __ushort_as_half((unsigned short) 0);
+		if (page >= 0) {
+			const uint8_t* run = a.pool.at + page * a.pool.page + h * a.pool.head;
+			if (value) {
+				const uint8_t* at = run + values_at(KG, shift) + slot * (VG * 16) + g * 2;
+				w = *reinterpret_cast<const uint16_t*>(at + (2 * t) * (VG * 2)) | (uint32_t) *reinterpret_cast<const uint16_t*>(at + (2 * t + 1) * (VG * 2)) << 16;
+				scale = *reinterpret_cast<const __half*>(run + value_scales_at(KG, VG, shift) + slot * (VG * 2) + g * 2);
+			} else {
+				w = *reinterpret_cast<const uint32_t*>(run + slot * (KG * 16) + t * (KG * 4) + g * 4);
+				scale = *reinterpret_cast<const __half*>(run + key_scales_at(KG, shift) + slot * (KG * 2) + g * 2);
+			}
+		}
+		const float f = __half2float(scale);
+		float x[8];
+#pragma unroll
+		for (int e = 0; e < 8; e++) x[e] = f * (float) ((int) (w >> (4 * e) & 15) - 8);
+		store8(reinterpret_cast<T*>(value ? a.v : a.k) + row * (value ? a.v_row : a.k_row) + h * (value ? dv : d) + chunk * 8, x);
+	}
+}
+
+// ---- checks and launches -----------------------------------------------------------------------------------------------------------------------
+static int check_cache4(const xalm_paged4_cache* c, Cache& o, Pool4& p) {
+	if (!c) return set_error(XALM_ERR_INVALID, "paged cache: cache is NULL");
+	if (c->pages <= 0 || c->kv_heads <= 0 || c->dim <= 0 || c->vdim <= 0 || c->dim > 256 || c->vdim > 256 || c->dim % 8 || c->vdim % 8 || c->kv_heads > 65535)
+		return set_error(XALM_ERR_INVALID, "paged cache: %d pages, %d heads of %d and %d entries (multiples of 8, at most 256)", c->pages, c->kv_heads, c->dim, c->vdim);
+	int shift = 4;
+	while (shift < 8 && (1 << shift) != c->page_size) shift++;
+	if ((1 << shift) != c->page_size) return set_error(XALM_ERR_INVALID, "paged cache: pages of %d slots (16, 32, 64, 128 or 256)", c->page_size);
+	if (!c->pool || !aligned16(c->pool)) return set_error(XALM_ERR_INVALID, "paged cache: the pool is at a 16-byte boundary, and not NULL");
+	if (!aligned4(c->status)) return set_error(XALM_ERR_INVALID, "paged cache: the status word is not at a 4-byte boundary");
+	p = Pool4{(uint8_t*) c->pool, c->page, c->head, blocks_of(c->dim), blocks_of(c->vdim)};
+	const long long most = 1ll << 40, run = run_bytes(p.kg, p.vg, shift);
+	if (c->page <= 0 || c->head <= 0 || c->page >= most || c->head >= most || c->page % 16 || c->head % 16)
+		return set_error(XALM_ERR_INVALID, "paged cache: strides of the pool are multiples of 16 bytes, above 0");
+	const bool by_head = (c->kv_heads == 1 || c->head >= run) && (c->pages == 1 || c->page >= (c->kv_heads - 1) * c->head + run);
+	const bool by_page = (c->pages == 1 || c->page >= run) && (c->kv_heads == 1 || c->head >= (c->pages - 1) * c->page + run);
+	if (!by_head && !by_page) return set_error(XALM_ERR_INVALID, "paged cache: pages or heads of the pool overlap (a page has %lld bytes for each)", run);
+	o = Cache{p.at, nullptr, nullptr, 0, 0, 0, 0, 0, 0, c->pages, shift, c->kv_heads, c->dim, c->vdim, c->status};
+	return XALM_OK;
+}
+static int check_apart_from_cache4(const char* call, const Span& out, const Cache& c, const Pool4& p, const BatchView& b) {
+	return check_apart(call, out, {Span{"the pool", p.at, (c.pages - 1) * p.page + (c.G - 1) * p.head + run_bytes(p.kg, p.vg, c.shift)}, Span{"the status word", c.status, 4},
+	                               Span{"starts", b.starts, 4ll * (b.B + 1)}, Span{"lens", b.lens, 4ll * b.B}, rows_span("the table", b.table, b.table_row, b.max_pages, b.B, 4),
+	                               Span{"group_bounds", b.bounds, 4ll * (b.n_groups + 1)}, Span{"group_shared", b.shared, 4ll * b.n_groups}});
+}
+
+// What a piece costs beside its tiles, in tiles
+constexpr int LEAD4 = 6, LEAD4_MANY = 6, LEAD4_F32 = 6;
+constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
+
+static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, bool& many) {
+	if (heads <= 0 || heads % c.G || heads > 65535) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
+	if (!is_type(type)) return set_error(XALM_ERR_UNSUPPORTED, "paged attention: queries of type %d (F32, F16 and BF16)", type);
+	int sms = 0;
+	XALM_TRY(sm_count(device, &sms));
+	a = Attn{};
+	a.c = c;
+	a.b = b;
+	a.H = heads;
+	a.rep = heads / c.G;
+	const Shape4 few = type == XALM_F32 ? attn4_f32(p, b) : attn4_few(p, b), more = attn4_many(p, b);
+	many = type != XALM_F32 && more.rows && (b.n_groups || b.N > b.B || a.rep > few.rows) && (long long) b.N * a.rep > few.rows;
+	a.n_parts = many ? 2 : 1;
+	size_t at = 0;
+	auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+	for (int i = 0; i < a.n_parts; i++) {
+		Part& t = a.part[i];
+		const bool big = many && i == 0;
+		t.M = big ? more.rows : few.rows;
+		t.grid = sms * (big ? more.per_sm : few.per_sm);
+		t.lead = big ? LEAD4_MANY : type == XALM_F32 ? LEAD4_F32 : LEAD4;
+		t.least_rows = big ? few.rows + 1 : 1;
+		t.most_rows = many && !big ? few.rows : 0x7fffffff;
+		// as in plan_attn: a segment has at most its rows / M + 1 tiles, in a part that takes short ones only it has one
+		const long long rows = (long long) b.N * a.rep, whole = many && !big ? 0 : rows / t.M, most = rows / t.least_rows;
+		const long long tiles = whole + std::min((long long) b.B, most) + (b.n_groups ? whole + std::min((long long) b.n_groups, most) : 0);
+		if (tiles * c.G + t.grid > 0x7fffffff / t.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
+		const long long work = ((long long) b.max_pages << c.shift) / KT + 1;
+		if (tiles * c.G > 0x7fffffffll / (work + t.lead)) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads over up to %lld keys are too many for one call", b.N, heads, work * KT);
+		t.slots = !b.n_groups ? 2 * t.grid : (int) (tiles * c.G) + t.grid;
+		t.o = (float*) take((size_t) t.slots * t.M * c.dv * 4);
+		t.ml = (float2*) take((size_t) t.slots * t.M * 8);
+		t.head = (Head*) take((size_t) t.grid * sizeof(Head));
+		t.cum_w = (int*) take((size_t) (b.B + b.n_groups + 1) * 4);
+		t.cum_u = (int*) take((size_t) (b.B + b.n_groups + 1) * 4);
+		t.shs = (int*) take((size_t) b.B * 4);
+	}
+	a.row_blocks = !b.n_groups ? 0 : (int) std::min(((long long) b.N * heads + JOIN_ROWS4 - 1) / JOIN_ROWS4, (long long) sms * JOIN_BLOCKS4);
+	*bytes = at;
+	return XALM_OK;
+}
+
+} // namespace paged
+} // namespace xalm
+
+using namespace xalm;
+using namespace xalm::paged;
+
+extern "C" {
+
+int xalm_cuda_paged4_append(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, const void* k, long long k_row, const void* v, long long v_row, const void* q,
+                            long long q_row, int heads, int type, void* q_out, long long q_out_row, const float* freq, int rot_half, float rot_mag, int neighbours, void* stream) {
+	Append4Args a = {};
+	XALM_TRY(check_cache4(cache, a.c, a.pool));
+	XALM_TRY(check_batch(batch, a.c, a.b));
+	if (!is_type(type)) return set_error(XALM_ERR_UNSUPPORTED, "paged append: rows of type %d (F32, F16 and BF16)", type);
+	if (!aligned4(freq)) return set_error(XALM_ERR_INVALID, "paged append: freq is not at a 4-byte boundary");
+	if (rot_half < 0 || 2 * rot_half > a.c.d || (rot_half && !freq)) return set_error(XALM_ERR_INVALID, "paged append: rotation of %d pairs in heads of %d", rot_half, a.c.d);
+	if (q && (heads <= 0 || heads > 65535)) return set_error(XALM_ERR_INVALID, "paged append: %d query heads", heads);
+	const int e = element_bytes(type);
+	if (a.b.N) {
+		XALM_TRY(check_rows("k", k, k_row, a.c.G * a.c.d, e));
+		XALM_TRY(check_rows("v", v, v_row, a.c.G * a.c.dv, e));
+		if (q) {
+			XALM_TRY(check_rows("q", q, q_row, heads * a.c.d, e));
+			XALM_TRY(check_rows("q_out", q_out, q_out_row, heads * a.c.d, e));
+		}
+	}
+	if (a.b.N == 0 || a.b.B == 0) return XALM_OK;
+	if (q) {
+		const long long width = (long long) heads * a.c.d * e;
+		if (rows_meet(q, q_row * e, width, q_out, q_out_row * e, width, a.b.N)) return set_error(XALM_ERR_INVALID, "paged append: q_out overlaps q");
+		const Span out = rows_span("q_out", q_out, q_out_row, heads * a.c.d, a.b.N, e);
+		XALM_TRY(check_apart_from_cache4("paged append", out, a.c, a.pool, a.b));
+		XALM_TRY(check_apart("paged append", out, {Span{"freq", freq, 4ll * rot_half}}));
+		if (rows_meet(k, k_row * e, (long long) a.c.G * a.c.d * e, q_out, q_out_row * e, width, a.b.N) || rows_meet(v, v_row * e, (long long) a.c.G * a.c.dv * e, q_out, q_out_row * e, width, a.b.N))
+			return set_error(XALM_ERR_INVALID, "paged append: q_out overlaps k or v");
+	}
+	OnDevice on;
+	XALM_TRY(on.set(cache->device));
+	a.k = (const uint8_t*) k; a.v = (const uint8_t*) v; a.q = (const uint8_t*) q;
+	a.k_row = k_row; a.v_row = v_row; a.q_row = q_row; a.q_out_row = q_out_row;
+	a.q_out = (uint8_t*) q_out;
+	a.H = heads;
+	a.freq = freq; a.rot = rot_half; a.mag = rot_mag; a.neighbours = neighbours;
+	int sms = 0;
+	XALM_TRY(sm_count(cache->device, &sms));
+	const bool several = a.b.N >= sms * 4;
+	void (*kernel)(Append4Args) = type == XALM_F32   ? several ? paged4_append_kernel<float, 4> : paged4_append_kernel<float, 1>
+	                              : type == XALM_F16 ? several ? paged4_append_kernel<__half, 4> : paged4_append_kernel<__half, 1>
+	                                                 : several ? paged4_append_kernel<__nv_bfloat16, 4> : paged4_append_kernel<__nv_bfloat16, 1>;
+	kernel<<<several ? (a.b.N + 3) / 4 : a.b.N, A4T, 0, (cudaStream_t) stream>>>(a);
+	XALM_CUDA_CHECK(cudaGetLastError());
+	return XALM_OK;
+}
+
+int xalm_cuda_paged4_read(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, int type, void* k, long long k_row, void* v, long long v_row, void* stream) {
+	Read4Args a = {};
+	XALM_TRY(check_cache4(cache, a.c, a.pool));
+	XALM_TRY(check_batch(batch, a.c, a.b));
+	if (!is_type(type)) return set_error(XALM_ERR_UNSUPPORTED, "paged read: rows of type %d (F32, F16 and BF16)", type);
+	const int e = element_bytes(type);
+	if (a.b.N) {
+		XALM_TRY(check_rows("k", k, k_row, a.c.G * a.c.d, e));
+		XALM_TRY(check_rows("v", v, v_row, a.c.G * a.c.dv, e));
+	}
+	if (a.b.N == 0 || a.b.B == 0) return XALM_OK;
+	if (rows_meet(k, k_row * e, (long long) a.c.G * a.c.d * e, v, v_row * e, (long long) a.c.G * a.c.dv * e, a.b.N)) return set_error(XALM_ERR_INVALID, "paged read: k overlaps v");
+	for (const Span& x : {rows_span("k", k, k_row, a.c.G * a.c.d, a.b.N, e), rows_span("v", v, v_row, a.c.G * a.c.dv, a.b.N, e)}) XALM_TRY(check_apart_from_cache4("paged read", x, a.c, a.pool, a.b));
+	OnDevice on;
+	XALM_TRY(on.set(cache->device));
+	a.k = (uint8_t*) k; a.v = (uint8_t*) v;
+	a.k_row = k_row; a.v_row = v_row;
+	void (*kernel)(Read4Args) = type == XALM_F32 ? paged4_read_kernel<float> : type == XALM_F16 ? paged4_read_kernel<__half> : paged4_read_kernel<__nv_bfloat16>;
+	kernel<<<a.b.N, A4T, 0, (cudaStream_t) stream>>>(a);
+	XALM_CUDA_CHECK(cudaGetLastError());
+	return XALM_OK;
+}
+
+int xalm_cuda_paged4_status(const xalm_paged4_cache* cache, int* taken, void* stream) {
+	Cache c;
+	Pool4 p;
+	XALM_TRY(check_cache4(cache, c, p));
+	if (!taken || !c.status || !aligned4(taken)) return set_error(XALM_ERR_INVALID, "paged status: %s", !taken || !c.status ? "taken or the cache's status word is NULL" : "taken is not at a 4-byte boundary");
+	OnDevice on;
+	XALM_TRY(on.set(cache->device));
+	return launch_status(c.status, taken, (cudaStream_t) stream);
+}
+
+int xalm_cuda_paged4_workspace(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, int type, int heads, size_t* bytes) {
+	Cache c;
+	Pool4 p;
+	BatchView b;
+	Attn a;
+	bool many;
+	if (!bytes) return set_error(XALM_ERR_INVALID, "paged attention: bytes is NULL");
+	XALM_TRY(check_cache4(cache, c, p));
+	XALM_TRY(check_batch(batch, c, b));
+	return plan_attn4(cache->device, c, p, b, type, heads, a, bytes, many);
+}
+
+int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, int type, float scale, void* out,
+                            long long out_row, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+	Cache c;
+	Pool4 p;
+	BatchView b;
+	Attn a;
+	bool many = false;
+	size_t need = 0;
+	XALM_TRY(check_cache4(cache, c, p));
+	XALM_TRY(check_batch(batch, c, b));
+	if (!is_type(type)) return set_error(XALM_ERR_UNSUPPORTED, "paged attention: queries of type %d (F32, F16 and BF16)", type);
+	if (heads <= 0 || heads % c.G || heads > 65535) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
+	const int e = element_bytes(type);
+	if (b.N) {
+		XALM_TRY(check_rows("q", q, q_row, heads * c.d, e));
+		XALM_TRY(check_rows("out", out, out_row, heads * c.dv, e));
+	}
+	if (!aligned4(lse)) return set_error(XALM_ERR_INVALID, "paged attention: lse is not at a 4-byte boundary");
+	if (!isfinite(scale)) return set_error(XALM_ERR_INVALID, "paged attention: scale is not finite");
+	if (b.N == 0 || b.B == 0) return XALM_OK;
+	if (!workspace || ((uintptr_t) workspace & 255)) return set_error(XALM_ERR_INVALID, "paged attention: the workspace is NULL or not at a 256-byte boundary");
+	if (rows_meet(q, q_row * e, (long long) heads * c.d * e, out, out_row * e, (long long) heads * c.dv * e, b.N)) return set_error(XALM_ERR_INVALID, "paged attention: out overlaps q");
+	const Span sq = rows_span("q", q, q_row, heads * c.d, b.N, e), so = rows_span("out", out, out_row, heads * c.dv, b.N, e), sl = {"lse", lse, 4ll * b.N * heads};
+	for (const Span& x : {so, sl}) XALM_TRY(check_apart_from_cache4("paged attention", x, c, p, b));
+	XALM_TRY(check_apart("paged attention", sl, {sq, so}));
+	XALM_TRY(plan_attn4(cache->device, c, p, b, type, heads, a, &need, many));
+	const Span sw = {"the workspace", workspace, (long long) need};
+	XALM_TRY(check_apart_from_cache4("paged attention", sw, c, p, b));
+	XALM_TRY(check_apart("paged attention", sw, {sq, so, sl}));
+	if (workspace_bytes < need) return set_error(XALM_ERR_INVALID, "paged attention: a workspace of %zu bytes is needed, %zu given", need, workspace_bytes);
+	OnDevice on;
+	XALM_TRY(on.set(cache->device));
+	uint8_t* base = (uint8_t*) workspace;
+	for (int i = 0; i < a.n_parts; i++) {
+		Part& t = a.part[i];
+		t.o = (float*) (base + (size_t) t.o);
+		t.ml = (float2*) (base + (size_t) t.ml);
+		t.head = (Head*) (base + (size_t) t.head);
+		t.cum_w = (int*) (base + (size_t) t.cum_w);
+		t.cum_u = (int*) (base + (size_t) t.cum_u);
+		t.shs = (int*) (base + (size_t) t.shs);
+	}
+	a.q = (const uint8_t*) q;
+	a.q_row = q_row;
+	a.out = (uint8_t*) out;
+	a.out_row = out_row;
+	a.lse = lse;
+	a.scale = scale;
+	cudaStream_t s = (cudaStream_t) stream;
+	if (many) XALM_TRY(launch_attn4(a, p, 0, type, true, s));
+	XALM_TRY(launch_attn4(a, p, a.n_parts - 1, type, false, s));
+	return launch_join(a, type, s);
+}
+
+} // extern "C"

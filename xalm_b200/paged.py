@@ -7,6 +7,14 @@
     pages = select(cache, batch, q, top=32)               # the pages worth reading
     out = attend_selected(cache, batch, q, pages, scale)
 
+and over a cache held in 4 bits, with drafted tokens:
+
+    cache = PagedCache4(pool, page_size, dim, vdim)       # uint8 (pages, kv_heads, page4_bytes(page_size, dim, vdim))
+    q = append4(cache, batch, k_rows, v_rows, q=q_rows, freq=freq)
+    out = attend4(cache, batch, q, scale)
+    k, v = read4(cache, batch, rows)                      # the rows as they are stored
+    out, taken = verify(starts, tokens, target, accept, pick, draft=draft)
+
 Calls enqueue kernels on the current stream of the cache's device.  What the host can check is refused with XalmError; what only the device sees
 (a table that names no page of the pool, lengths beyond the table) is kept in `cache.status` and raised by cache.check().
 """
@@ -44,6 +52,15 @@ def _type(t):
     return _TYPES[t.dtype]
 
 
+def _check(cache, status):
+    torch.cuda.synchronize(cache.device)
+    taken = torch.empty_like(cache.status)
+    capi.check(status(cache.p, taken.data_ptr(), _stream(cache.index)))
+    bits = int(taken.item())
+    if bits:
+        _refuse("paged cache: " + " and ".join(t for b, t in ((1, "a table names a page outside the pool"), (2, "starts, lens and table do not fit"), (4, "a kernel gave up a wait for its copies or products")) if bits & b))
+
+
 class PagedCache:
     """Pools of keys (pages, page_size, kv_heads, dim) and values (.., vdim), both of the caller; the last dimension's entries are neighbours.  means
     (pages, kv_heads, dim), contiguous, or None."""
@@ -72,12 +89,43 @@ class PagedCache:
 
     def check(self):
         """Waits for the device, all its streams, and raises what its kernels have reported since the last check.  Not while a graph is captured."""
-        torch.cuda.synchronize(self.device)
-        taken = torch.empty_like(self.status)
-        capi.check(capi.lib().xalm_cuda_paged_status(self.p, taken.data_ptr(), _stream(self.index)))
-        bits = int(taken.item())
-        if bits:
-            _refuse("paged cache: " + " and ".join(t for b, t in ((1, "a table names a page outside the pool"), (2, "starts, lens and table do not fit"), (4, "a kernel gave up a wait for its copies or products")) if bits & b))
+        _check(self, capi.lib().xalm_cuda_paged_status)
+
+
+def _blocks(n):
+    return 2 if n <= 64 else 4 if n <= 128 else 8
+
+
+def page4_bytes(page_size, dim, vdim=None):
+    """Bytes that a page of a PagedCache4 has for each kv head."""
+    return page_size * 18 * (_blocks(dim) + _blocks(dim if vdim is None else vdim))
+
+
+class _Cache4(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("device", "pages", "page_size", "kv_heads", "dim", "vdim")] + [("pool", C.c_void_p), ("page", C.c_longlong), ("head", C.c_longlong), ("status", C.c_void_p)]
+
+
+class PagedCache4:
+    """Keys and values in blocks of 32 entries of 4 bits and a scale.  pool: uint8 (pages, kv_heads, page4_bytes(page_size, dim, vdim)) of the caller, the last dimension dense, the others any
+    multiples of 16 bytes apart."""
+
+    def __init__(self, pool, page_size, dim, vdim=None):
+        vdim = dim if vdim is None else vdim
+        if pool.dim() != 3 or pool.dtype != torch.uint8 or pool.stride(2) != 1 or pool.shape[2] != page4_bytes(page_size, dim, vdim):
+            _refuse(f"paged cache: a pool {tuple(pool.shape)} {pool.dtype} for pages of {page_size} slots, {dim} and {vdim} entries")
+        if pool.device.type != "cuda":
+            _refuse("paged cache: the pool lies on no GPU")
+        self.pool, self.device, self.index, self.page_size, self.kv_heads, self.dim, self.vdim = pool, pool.device, pool.device.index, page_size, pool.shape[1], dim, vdim
+        self.needs = {}  # bytes of workspace by the sizes of a call
+        self.status = torch.zeros(1, dtype=torch.int32, device=pool.device)
+        page, head, _ = pool.stride()
+        self.c = _Cache4(self.index, pool.shape[0], page_size, pool.shape[1], dim, vdim, pool.data_ptr(), page if pool.shape[0] > 1 else 1 << 36, head if pool.shape[1] > 1 else pool.shape[2],
+                         self.status.data_ptr())
+        self.p = C.addressof(self.c)
+
+    def check(self):
+        """As PagedCache.check."""
+        _check(self, capi.lib().xalm_cuda_paged4_status)
 
 
 class Batch:
@@ -221,3 +269,96 @@ def attend_selected(cache, batch, q, pages, scale, out=None, want_lse=False):
     if pages.dim() != 3 or pages.shape[:2] != (q.shape[0], cache.kv_heads) or pages.dtype != torch.int32 or not pages.is_contiguous() or pages.device != cache.device:
         _refuse(f"paged attention: lists {tuple(pages.shape)} {pages.dtype}")
     return _attend(cache, batch, q, pages, scale, out, want_lse)
+
+
+def _beside4(q, n, heads, dim):
+    return torch.empty_like(q) if q.shape[2] == dim and q.is_contiguous() else q.new_empty((n, heads, dim))
+
+
+def append4(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_out=None):
+    """append into a PagedCache4; the turned queries have the rows' type."""
+    n, dev, dt = k.shape[0], cache.device, k.dtype
+    (bp, held), stream = _start(cache, batch, n)
+    kr, vr = _rows(k, "k", n, cache.kv_heads, cache.dim, dt, dev), _rows(v, "v", n, cache.kv_heads, cache.vdim, dt, dev)
+    qr = qor = heads = qp = qop = fp = rot = 0
+    if q is not None:
+        heads = _heads(q)
+        qr = _rows(q, "q", n, heads, cache.dim, dt, dev)
+        if q_out is None:
+            q_out = _beside4(q, n, heads, cache.dim)
+            qor = heads * cache.dim
+        else:
+            qor = _rows(q_out, "q_out", n, heads, cache.dim, dt, dev)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        _refuse("paged append: q_out without q")
+    if freq is not None:
+        if freq.dtype is not torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev:
+            _refuse(f"paged append: freq {tuple(freq.shape)} {freq.dtype} on {freq.device}")
+        fp, rot = freq.data_ptr(), freq.shape[0]
+    capi.check(capi.lib().xalm_cuda_paged4_append(cache.p, bp, k.data_ptr(), kr, v.data_ptr(), vr, qp, qr, heads, _type(k), qop, qor, fp, rot, mag, neighbours, stream))
+    return q_out
+
+
+def read4(cache, batch, rows, dtype=torch.float32, k=None, v=None):
+    """Keys (rows, kv_heads, dim) and values (rows, kv_heads, vdim) at the batch's rows, as they are stored; rows outside every sequence are left as they were."""
+    (bp, held), stream = _start(cache, batch, rows)
+    if k is None:
+        k = torch.empty((rows, cache.kv_heads, cache.dim), dtype=dtype, device=cache.device)
+    if v is None:
+        v = torch.empty((rows, cache.kv_heads, cache.vdim), dtype=dtype, device=cache.device)
+    kr, vr = _rows(k, "k", rows, cache.kv_heads, cache.dim, dtype, cache.device), _rows(v, "v", rows, cache.kv_heads, cache.vdim, dtype, cache.device)
+    capi.check(capi.lib().xalm_cuda_paged4_read(cache.p, bp, _type(k), k.data_ptr(), kr, v.data_ptr(), vr, stream))
+    return k, v
+
+
+def attend4(cache, batch, q, scale, out=None, want_lse=False):
+    """attend over a PagedCache4; results have the queries' type."""
+    heads, n, dev, dt = _heads(q), q.shape[0], cache.device, q.dtype
+    (bp, held), stream = _start(cache, batch, n)
+    qr = _rows(q, "q", n, heads, cache.dim, dt, dev)
+    if out is None:
+        out = _beside4(q, n, heads, cache.vdim)
+        outr = heads * cache.vdim
+    else:
+        outr = _rows(out, "out", n, heads, cache.vdim, dt, dev)
+    lse = q.new_empty((n, heads), dtype=torch.float32) if want_lse else None
+    L, type = capi.lib(), _type(q)
+    sizes = n, heads, type, batch.c.seqs, batch.c.groups, batch.c.max_pages
+    need = cache.needs.get(sizes)
+    if need is None:
+        b = C.c_size_t(0)
+        capi.check(L.xalm_cuda_paged4_workspace(cache.p, bp, type, heads, C.byref(b)))
+        if len(cache.needs) > 1000:
+            cache.needs.clear()
+        need = cache.needs[sizes] = b.value
+    work = q.new_empty(need, dtype=torch.uint8)  # the current stream's, or the graph's that is being captured
+    capi.check(L.xalm_cuda_paged4_attend(cache.p, bp, q.data_ptr(), qr, heads, type, scale, out.data_ptr(), outr, None if lse is None else lse.data_ptr(), work.data_ptr(), need, stream))
+    return (out, lse) if want_lse else out
+
+
+def verify(starts, tokens, target, accept, pick, draft=None, out=None):
+    """Drafted tokens against the target's probabilities.  starts (seqs + 1) int32: sequence s has rows starts[s] .. starts[s + 1] - 1, the token that it had and its drafts, tokens (rows) int32.
+    target (rows, vocab): probabilities of the token behind each row; draft, of the same type: those that tokens[i + 1] was drawn from, in row i (None: each draft is certain).  accept (rows) and
+    pick (seqs): fp32 numbers from 0 to below 1.  Returns (rows) int32: the drafts taken and the token drawn behind them, then -1; and how many were taken (seqs)."""
+    dev = target.device
+    if target.dim() != 2 or target.stride(1) != 1 or dev.type != "cuda":
+        _refuse(f"verify: target {tuple(target.shape)} on {dev}, its rows dense and on a GPU")
+    n, V = target.shape
+    if draft is not None and (draft.shape != target.shape or draft.dtype is not target.dtype or draft.device != dev or draft.stride(1) != 1):
+        _refuse(f"verify: draft {tuple(draft.shape)} {draft.dtype} on {draft.device}")
+    if starts.dim() != 1 or starts.shape[0] < 1 or pick.shape != (starts.shape[0] - 1,) or tokens.shape != (n,) or accept.shape != (n,):
+        _refuse(f"verify: starts {tuple(starts.shape)}, tokens {tuple(tokens.shape)}, accept {tuple(accept.shape)}, pick {tuple(pick.shape)} for {n} rows")
+    if out is None:
+        out = tokens.new_empty((n,))
+    for t, dt in ((starts, torch.int32), (tokens, torch.int32), (out, torch.int32), (accept, torch.float32), (pick, torch.float32)):
+        if t.dtype is not dt or t.device != dev or not t.is_contiguous():
+            _refuse(f"verify: {t.dtype} on {t.device}, not {dt} on {dev}, dense")
+    if out.shape != (n,):
+        _refuse(f"verify: out {tuple(out.shape)}")
+    B = starts.shape[0] - 1
+    taken = starts.new_empty((B,))
+    capi.check(capi.lib().xalm_cuda_verify_drafts(dev.index, _type(target), B, n, V, starts.data_ptr(), tokens.data_ptr(), target.data_ptr(), target.stride(0) if n > 1 else V,
+                                                  0 if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0) if n > 1 else V, accept.data_ptr(), pick.data_ptr(),
+                                                  out.data_ptr(), taken.data_ptr(), _stream(dev.index)))
+    return out, taken
