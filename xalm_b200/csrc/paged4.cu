@@ -228,7 +228,7 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 constexpr int LEAD4 = 6, LEAD4_MANY = 6, LEAD4_F32 = 6;
 constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
 
-static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, bool& many) {
+static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, int (&kinds)[2]) {
 	if (heads <= 0 || heads % c.G || heads > 65535) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
 	if (!is_type(type)) return set_error(XALM_ERR_UNSUPPORTED, "paged attention: queries of type %d (F32, F16 and BF16)", type);
 	int sms = 0;
@@ -238,8 +238,13 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 	a.b = b;
 	a.H = heads;
 	a.rep = heads / c.G;
-	const Shape4 few = type == XALM_F32 ? attn4_f32(p, b) : attn4_few(p, b), more = attn4_many(p, b);
-	many = type != XALM_F32 && more.rows && (b.n_groups || b.N > b.B || a.rep > few.rows) && (long long) b.N * a.rep > few.rows;
+	// The kernel of most segments by the rows that one has on average, and where some may have more than its unit, one of more rows for those
+	const long long rows_all = (long long) b.N * a.rep, each = (rows_all + b.B - 1) / std::max(b.B, 1);
+	const int least = type == XALM_F32 ? each <= 4 ? F4 : F16 : type == XALM_F16 ? each <= 4 ? H4 : H16 : each <= 8 ? B8 : B16, most_kind = type == XALM_F16 ? H32 : B32;
+	const Shape4 few = attn4_shape(p, b, least), more = attn4_shape(p, b, most_kind);
+	const bool many = type != XALM_F32 && more.rows && (b.n_groups || b.N > b.B || a.rep > few.rows) && rows_all > few.rows;
+	kinds[0] = many ? most_kind : least;
+	kinds[1] = least;
 	a.n_parts = many ? 2 : 1;
 	size_t at = 0;
 	auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
@@ -252,7 +257,7 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 		t.least_rows = big ? few.rows + 1 : 1;
 		t.most_rows = many && !big ? few.rows : 0x7fffffff;
 		// as in plan_attn: a segment has at most its rows / M + 1 tiles, in a part that takes short ones only it has one
-		const long long rows = (long long) b.N * a.rep, whole = many && !big ? 0 : rows / t.M, most = rows / t.least_rows;
+		const long long rows = rows_all, whole = many && !big ? 0 : rows / t.M, most = rows / t.least_rows;
 		const long long tiles = whole + std::min((long long) b.B, most) + (b.n_groups ? whole + std::min((long long) b.n_groups, most) : 0);
 		if (tiles * c.G + t.grid > 0x7fffffff / t.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
 		const long long work = ((long long) b.max_pages << c.shift) / KT + 1;
@@ -362,11 +367,11 @@ int xalm_cuda_paged4_workspace(const xalm_paged4_cache* cache, const xalm_paged_
 	Pool4 p;
 	BatchView b;
 	Attn a;
-	bool many;
+	int kinds[2];
 	if (!bytes) return set_error(XALM_ERR_INVALID, "paged attention: bytes is NULL");
 	XALM_TRY(check_cache4(cache, c, p));
 	XALM_TRY(check_batch(batch, c, b));
-	return plan_attn4(cache->device, c, p, b, type, heads, a, bytes, many);
+	return plan_attn4(cache->device, c, p, b, type, heads, a, bytes, kinds);
 }
 
 int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_batch* batch, const void* q, long long q_row, int heads, int type, float scale, void* out,
@@ -375,7 +380,7 @@ int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_bat
 	Pool4 p;
 	BatchView b;
 	Attn a;
-	bool many = false;
+	int kinds[2];
 	size_t need = 0;
 	XALM_TRY(check_cache4(cache, c, p));
 	XALM_TRY(check_batch(batch, c, b));
@@ -394,7 +399,7 @@ int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_bat
 	const Span sq = rows_span("q", q, q_row, heads * c.d, b.N, e), so = rows_span("out", out, out_row, heads * c.dv, b.N, e), sl = {"lse", lse, 4ll * b.N * heads};
 	for (const Span& x : {so, sl}) XALM_TRY(check_apart_from_cache4("paged attention", x, c, p, b));
 	XALM_TRY(check_apart("paged attention", sl, {sq, so}));
-	XALM_TRY(plan_attn4(cache->device, c, p, b, type, heads, a, &need, many));
+	XALM_TRY(plan_attn4(cache->device, c, p, b, type, heads, a, &need, kinds));
 	const Span sw = {"the workspace", workspace, (long long) need};
 	XALM_TRY(check_apart_from_cache4("paged attention", sw, c, p, b));
 	XALM_TRY(check_apart("paged attention", sw, {sq, so, sl}));
@@ -418,8 +423,7 @@ int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_bat
 	a.lse = lse;
 	a.scale = scale;
 	cudaStream_t s = (cudaStream_t) stream;
-	if (many) XALM_TRY(launch_attn4(a, p, 0, type, true, s));
-	XALM_TRY(launch_attn4(a, p, a.n_parts - 1, type, false, s));
+	for (int i = 0; i < a.n_parts; i++) XALM_TRY(launch_attn4(a, p, i, type, kinds[i], s));
 	return launch_join(a, type, s);
 }
 

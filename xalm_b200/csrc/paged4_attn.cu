@@ -12,14 +12,17 @@ namespace paged {
 constexpr int FT = 128, FW = FT / 32, FK = KT / FW; // keys of a warp in every tile
 constexpr int FP = 20;                              // floats between the probabilities of a warp's rows
 
-enum { FEW, MANY, F32 };
+// Kernels by the type of the queries and the rows of a unit.  How p d enters the second product: one fp16 number (bf16 results), two in turn, or two in columns of their own (SPLIT, where a tile of
+// columns has four rows; fp32 queries enter the first product so too).
 template <int KG, int VG, int KIND>
 struct Size4 {
-	static constexpr int NT = KIND == FEW ? 2 : VG == 8 ? (KIND == F32 ? 2 : 0) : 4; // tiles of 8 columns that fit a lane's registers
-	static constexpr int M = KIND == F32 ? NT * 4 : NT * 8;                           // rows of a unit
+	static constexpr bool WIDE = KIND == F4 || KIND == F16, SPLIT = WIDE || KIND == H4, TWO = KIND == H16 || KIND == H32;
+	static constexpr int NT = KIND == B16 || KIND == H16 ? 2 : KIND == B32 || KIND == H32 ? (VG == 8 ? 0 : 4) : KIND == F16 ? (VG == 8 ? 2 : 4) : 1; // tiles of 8 columns; 0: more than registers hold
+	static constexpr int M = SPLIT ? NT * 4 : NT * 8;                                                     // rows of a unit
+	static constexpr int CTAS = NT == 1 ? (VG == 8 || KG == 8 ? 3 : 4) : NT == 2 && VG < 8 ? 3 : 2;       // to an SM, as registers allow
 	static constexpr int OP = VG * 32 + 4;                                            // floats between rows of sums
-	static constexpr int SUMS = FW * M * OP;
-	static constexpr size_t own = (size_t) (NT * KG * 2 * 64 + NT * KG * 8 + SUMS + FW * NT * 8 * FP + FW * M * 2 + NT * 8 * 2) * 4;
+	static constexpr int STAGE = (KG + VG) * 288, STAGES = 4, WARP = STAGES * STAGE > M * OP * 4 ? STAGES * STAGE : M * OP * 4; // bytes of 16 keys and values; of a warp's stages, whose place its sums take
+	static constexpr size_t own = (size_t) FW * WARP + (NT * KG * 2 * 64 + FW * NT * 8 * FP + FW * M * 2 + NT * 8 * 2) * 4;
 };
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -27,15 +30,22 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 	             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// N words from an address that is a multiple of their size (of 16 bytes at most)
+// N words of shared memory from an address that is a multiple of their size (of 16 bytes at most)
 template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&x)[N]) {
-	if constexpr (N == 1) asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(x[0]) : "l"(p));
-	else if constexpr (N == 2) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "l"(p));
-	else
+__device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&x)[N]) {
+	if constexpr (N == 1) x[0] = *reinterpret_cast<const uint32_t*>(p);
+	else if constexpr (N == 2) {
+		const uint2 y = *reinterpret_cast<const uint2*>(p);
+		x[0] = y.x; x[1] = y.y;
+	} else
 #pragma unroll
-		for (int i = 0; i < N; i += 4)
-			asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]) : "l"(p + i * 4));
+		for (int i = 0; i < N; i += 4) {
+			const uint4 y = *reinterpret_cast<const uint4*>(p + i * 4);
+			x[i] = y.x; x[i + 1] = y.y; x[i + 2] = y.z; x[i + 3] = y.w;
+		}
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool there) { // zeros where there is nothing
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short) w)); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short) (w >> 16))); }
@@ -54,22 +64,28 @@ __device__ __forceinline__ void load8_any(const uint8_t* p, long long i, int typ
 	else load8(reinterpret_cast<const __nv_bfloat16*>(p) + i, x);
 }
 
-// Codes of a word as four pairs of fp16 numbers: codes 0 and 4, 1 and 5, 2 and 6, 3 and 7.  Where they lie in the word they are numbers c 2^-20, below fp16's normal ones and exact; a product's
-// terms are lined up by their exponents, so that up to 6 of its 24 bits are lost: for fp32 results codes become c - 8.
-template <bool WIDE>
+// Codes of a word as four pairs of fp16 numbers (c - 8) 2^-10: codes 0 and 4, 1 and 5, 2 and 6, 3 and 7.  Where they lie in the word codes are numbers c 2^-24 and c 2^-20 below fp16's normal ones,
+// which one multiplication and addition bring there without a rounding.  (As they are the products would be exact too, but a product's terms are lined up by the exponents that are written:
+// results were 1.2e-5 off where these are 4e-7.)
 __device__ __forceinline__ void codes4(uint32_t w, uint32_t (&h)[4]) {
-	constexpr uint32_t M = 0x00f000f0u;
-	h[0] = (w << 4) & M;
-	h[1] = w & M;
-	h[2] = (w >> 4) & M;
-	h[3] = (w >> 8) & M;
-	if constexpr (WIDE)
+	const uint32_t w8 = w >> 8;
 #pragma unroll
-		for (int i = 0; i < 4; i++) {
-			const uint32_t x = h[i] | 0x64006400u; // 1024 + 16 c
-			const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
-			h[i] = *reinterpret_cast<const uint32_t*>(&y);
-		}
+	for (int i = 0; i < 4; i++) {
+		const uint32_t x = (i < 2 ? w : w8) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+		const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), i & 1 ? __float2half2_rn(1024.f) : __float2half2_rn(16384.f), __float2half2_rn(-0.0078125f));
+		h[i] = *reinterpret_cast<const uint32_t*>(&y);
+	}
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+// the larger magnitudes of two pairs; signs are of no use
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+	uint32_t r;
+	asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+	return r;
 }
 
 // What a lane holds of 16 keys and values as they come: of keys lane / 4 and 8 behind it a word of each block, of values 4 (lane % 4) .. + 3 four entries of each
@@ -82,89 +98,82 @@ struct Values {
 	uint32_t w[4][VG / 2], s[4 * VG / 2]; // scales: value by value
 };
 
-// A piece by one warp: its 16 keys of each tile, the unit's rows as columns of the products.
-// SPLIT: tiles of four rows, whose columns 4 .. 7 have what rounding to fp16 left of the queries (fp32) and of the probabilities
-template <int KG, int VG, int NT, bool SPLIT, bool WIDE>
-__device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const Piece& x, int vis, int least, const uint2* s_q, const float* s_init, const float* s_fac, const int* s_lim, float* sp,
-                                       float* s_o, float2* s_ml, int op, int most_rows) {
+constexpr float NONE = -3.0e38f; // the maximum before the first key
+
+// A piece by one warp: its 16 keys of each tile, the unit's rows as columns of the products
+template <typename Z, int KG, int VG>
+__device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const Piece& x, int vis, int least, const uint2* s_q, const float* s_fac, const int* s_lim, float* sp, uint8_t* stages, float2* s_ml) {
+	constexpr int NT = Z::NT, STAGES = Z::STAGES, STAGE = Z::STAGE;
+	constexpr bool SPLIT = Z::SPLIT, WIDE = Z::WIDE, TWO = Z::TWO;
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, u = lane >> 2, t = lane & 3, P = 1 << a.c.shift;
-	const int ks_at = key_scales_at(KG, a.c.shift), v_at = values_at(KG, a.c.shift), vs_at = value_scales_at(KG, VG, a.c.shift);
 	constexpr bool IN_REGS = NT == 1;
 	uint2 q[IN_REGS ? KG * 2 : 1];
-	float2 init[IN_REGS ? KG : 1];
-	if constexpr (IN_REGS) {
+	float2 fac[NT];
+	if constexpr (IN_REGS)
 #pragma unroll
 		for (int i = 0; i < KG * 2; i++) q[i] = s_q[i * 32 + lane];
-#pragma unroll
-		for (int g = 0; g < KG; g++) init[g] = *reinterpret_cast<const float2*>(s_init + g * 8 + t * 2);
-	}
-	float acc[VG * 2][NT][4], part[NT][VG], m[NT][2], l[NT][2], mu[NT], room[NT]; // part: sums of the probabilities times scales; mu: what those are multiplied with; room: the largest scale it allows
+	float acc[VG * 2][NT][4], m[NT][2], l[NT][2], mu[NT], room[NT]; // mu: what p d is multiplied with; room: the largest d that it allows
 #pragma unroll
 	for (int n = 0; n < NT; n++) {
 #pragma unroll
 		for (int i = 0; i < VG * 2; i++)
 #pragma unroll
 			for (int e = 0; e < 4; e++) acc[i][n][e] = 0.f;
-#pragma unroll
-		for (int g = 0; g < VG; g++) part[n][g] = 0.f;
-		m[n][0] = m[n][1] = -INFINITY;
+		fac[n] = *reinterpret_cast<const float2*>(s_fac + n * 8 + t * 2);
+		m[n][0] = m[n][1] = NONE;
 		l[n][0] = l[n][1] = 0.f;
 		mu[n] = 1.f;
 		room[n] = 0.f;
 	}
 	const int* table = a.b.table + (long long) x.s * a.b.table_row;
 	const uint8_t* head = pool.at + x.g * pool.head;
-	auto id_at = [&](int at) { // the page of keys `at` .. of the segment
-		if (at >= vis) return 0;
-		const int id = table[(x.key0 + at) >> a.c.shift];
-		return id;
-	};
-	Keys<KG> k;
-	Values<VG> v;
-	auto run_of = [&](int at, int id, bool& there) {
-		there = id >= 0 && id < a.c.pages;
-		return head + (there ? id : 0) * pool.page;
-	};
-	auto load_keys = [&](int at, int id) {
-		if (at >= vis) return;
-		bool there;
-		const uint8_t* run = run_of(at, id, there);
-		const int slot = (x.key0 + at) & (P - 1);
-#pragma unroll
-		for (int i = 0; i < 2; i++) {
-			const int j = slot + u + i * 8;
-			load_words<KG>(run + j * (KG * 16) + t * (KG * 4), k.w[i]);
-			load_words<KG / 2>(run + ks_at + j * (KG * 2), k.s[i]);
-		}
-		if (!there) { // reads as zeros
-			if (lane == 0) report(a.c, ERR_PAGE);
-#pragma unroll
-			for (int i = 0; i < 2; i++)
-#pragma unroll
-				for (int g = 0; g < KG / 2; g++) k.s[i][g] = 0;
-		}
-	};
-	auto load_values = [&](int at, int id) {
-		if (at >= vis) return;
-		bool there;
-		const uint8_t* run = run_of(at, id, there);
-		const int slot = (x.key0 + at) & (P - 1);
-#pragma unroll
-		for (int i = 0; i < 4; i++) load_words<VG / 2>(run + v_at + (slot + t * 4 + i) * (VG * 16) + u * (VG * 2), v.w[i]);
-		load_words<2 * VG>(run + vs_at + (slot + t * 4) * (VG * 2), v.s);
-		if (!there)
-#pragma unroll
-			for (int i = 0; i < 2 * VG; i++) v.s[i] = 0;
-	};
 	int at = x.j0 * KT + warp * FK;
 	const int end = min(x.j1 * KT, vis);
-	int id = id_at(at), id_next = id_at(at + KT);
-	if (at < end) {
-		load_keys(at, id);
-		load_values(at, id);
+	auto id_at = [&](int key) { return key < end ? table[(x.key0 + key) >> a.c.shift] : 0; }; // looked at when its page is asked for
+	// Copies, each lane's own 16 bytes at a time.  Values' 16 bytes lie in another order: those of keys 4 t + i, which four lanes t ask for at once, in different banks.
+	constexpr int VK = KG * 256, KS = VK + VG * 256, VS = KS + KG * 32; // sections of a stage
+	const uint32_t ring = smem_u32(stages);
+	auto bring = [&](int key, int id, int to) {
+		if (key < end) {
+			const bool there = (unsigned) id < (unsigned) a.c.pages;
+			if (!there && lane == 0) report(a.c, ERR_PAGE); // reads as zeros
+			const uint8_t* run = head + (there ? id : 0) * pool.page;
+			const int slot = (x.key0 + key) & (P - 1), shift = a.c.shift;
+			const uint32_t dst = ring + to * STAGE;
+			const uint8_t *kw = run + slot * (KG * 16) + lane * 16, *vw = run + values_at(KG, shift) + slot * (VG * 16) + lane * 16;
+#pragma unroll
+			for (int i = 0; i < KG / 2; i++) copy16(dst + lane * 16 + i * 512, kw + i * 512, there);
+#pragma unroll
+			for (int i = 0; i < VG / 2; i++) {
+				const int unit = lane + i * 32;
+				copy16(dst + VK + (unit ^ ((unit / VG >> 2 & 3) * 2)) * 16, vw + i * 512, there);
+			}
+			if (lane < (KG + VG) * 2)
+				copy16(dst + KS + lane * 16, lane < KG * 2 ? run + key_scales_at(KG, shift) + slot * (KG * 2) + lane * 16 : run + value_scales_at(KG, VG, shift) + slot * (VG * 2) + (lane - KG * 2) * 16, there);
+		}
+		asm volatile("cp.async.commit_group;" ::: "memory");
+	};
+	int id = id_at(at), full = 0, free = STAGES - 1; // the stage to be read, and the one to be filled
+#pragma unroll
+	for (int i = 0; i < STAGES - 1; i++) {
+		bring(at + i * KT, id, i);
+		id = id_at(at + (i + 1) * KT);
 	}
 	for (; at < end; at += KT) {
 		const bool all = at + FK <= least; // every row sees every key
+		asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+		__syncwarp(); // the stage is there, and nobody reads the one before any more
+		bring(at + (STAGES - 1) * KT, id, free);
+		id = id_at(at + STAGES * KT);
+		const uint8_t* stage = stages + full * STAGE;
+		free = full;
+		full = full == STAGES - 1 ? 0 : full + 1;
+		Keys<KG> k;
+#pragma unroll
+		for (int i = 0; i < 2; i++) {
+			read_words<KG>(stage + (u + i * 8) * (KG * 16) + t * (KG * 4), k.w[i]);
+			read_words<KG / 2>(stage + KS + (u + i * 8) * (KG * 2), k.s[i]);
+		}
 		// ---- scores: keys as rows of the product ----
 		float s[NT][4];
 #pragma unroll
@@ -174,20 +183,18 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 		for (int g = 0; g < KG; g++) {
 			uint32_t h0[4], h1[4];
-			codes4<WIDE>(k.w[0][g], h0);
-			codes4<WIDE>(k.w[1][g], h1);
+			codes4(k.w[0][g], h0);
+			codes4(k.w[1][g], h1);
 			const float d0 = g & 1 ? half_hi(k.s[0][g / 2]) : half_lo(k.s[0][g / 2]), d1 = g & 1 ? half_hi(k.s[1][g / 2]) : half_lo(k.s[1][g / 2]);
 #pragma unroll
 			for (int n = 0; n < NT; n++) {
 				uint2 qa, qb;
-				float2 from;
-				if constexpr (IN_REGS) { qa = q[g * 2]; qb = q[g * 2 + 1]; from = init[g]; }
+				if constexpr (IN_REGS) { qa = q[g * 2]; qb = q[g * 2 + 1]; }
 				else {
 					qa = s_q[((n * KG + g) * 2) * 32 + lane];
 					qb = s_q[((n * KG + g) * 2 + 1) * 32 + lane];
-					from = *reinterpret_cast<const float2*>(s_init + (n * KG + g) * 8 + t * 2);
 				}
-				float c[4] = {from.x, from.y, from.x, from.y};
+				float c[4] = {0.f, 0.f, 0.f, 0.f};
 				mma16(c, h0[0], h1[0], h0[1], h1[1], qa.x, qa.y);
 				mma16(c, h0[2], h1[2], h0[3], h1[3], qb.x, qb.y);
 				s[n][0] = fmaf(c[0], d0, s[n][0]);
@@ -196,81 +203,79 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 				s[n][3] = fmaf(c[3], d1, s[n][3]);
 			}
 		}
-		id = id_next;
-		load_keys(at + KT, id);
-		id_next = id_at(at + 2 * KT);
 		// ---- probabilities ----
+		float p[NT][4];
 		bool grow = false;
 #pragma unroll
 		for (int n = 0; n < NT; n++) {
-			if constexpr (SPLIT && WIDE) // the rest of the queries has columns of its own
+			if constexpr (WIDE) // the rest of the queries has columns of its own
 #pragma unroll
 				for (int e = 0; e < 4; e++) s[n][e] += __shfl_xor_sync(0xffffffffu, s[n][e], 2);
-			const float2 f = *reinterpret_cast<const float2*>(s_fac + n * 8 + t * 2);
 #pragma unroll
-			for (int e = 0; e < 4; e++) s[n][e] *= e & 1 ? f.y : f.x;
+			for (int e = 0; e < 4; e++) s[n][e] *= e & 1 ? fac[n].y : fac[n].x;
 			if (!all) {
 				const int2 lim = *reinterpret_cast<const int2*>(s_lim + n * 8 + t * 2);
 #pragma unroll
 				for (int e = 0; e < 4; e++)
 					if (at + u + (e >> 1) * 8 >= (e & 1 ? lim.y : lim.x)) s[n][e] = -INFINITY;
 			}
-			grow = grow || fmaxf(s[n][0], s[n][2]) - m[n][0] > 2.f || fmaxf(s[n][1], s[n][3]) - m[n][1] > 2.f; // false where both are -infinity
+#pragma unroll
+			for (int e = 0; e < 4; e++) {
+				p[n][e] = s[n][e] - m[n][e & 1]; // exact where they are near, however large
+				grow = grow || p[n][e] > 2.f;
+			}
 		}
 		if (__any_sync(0xffffffffu, grow)) { // rare behind the first keys: probabilities may be up to 4
 #pragma unroll
-			for (int n = 0; n < NT; n++) {
-				float f[2];
+			for (int n = 0; n < NT; n++)
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
 					float top = fmaxf(s[n][c], s[n][c + 2]);
 #pragma unroll
 					for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 					top = fmaxf(m[n][c], top);
-					f[c] = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - top);
+					const float f = exp2f(m[n][c] - top);
 					m[n][c] = top;
-					l[n][c] *= f[c];
+					l[n][c] *= f;
 #pragma unroll
-					for (int i = 0; i < VG * 2; i++) { acc[i][n][c] *= f[c]; acc[i][n][c + 2] *= f[c]; }
+					for (int i = 0; i < VG * 2; i++) { acc[i][n][c] *= f; acc[i][n][c + 2] *= f; }
+					p[n][c] = s[n][c] - top;
+					p[n][c + 2] = s[n][c + 2] - top;
 				}
-				const float fu = __shfl_sync(0xffffffffu, f[0], u >> 1), fv = __shfl_sync(0xffffffffu, f[1], u >> 1);
-#pragma unroll
-				for (int g = 0; g < VG; g++) part[n][g] *= u & 1 ? fv : fu;
-			}
 		}
 		__syncwarp();
 #pragma unroll
-		for (int n = 0; n < NT; n++) {
-			const float b0 = m[n][0] == -INFINITY ? 0.f : m[n][0], b1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+		for (int n = 0; n < NT; n++)
 #pragma unroll
 			for (int e = 0; e < 4; e++) {
-				const float p = exp2f(s[n][e] - (e & 1 ? b1 : b0));
-				l[n][e & 1] += p;
-				sp[(n * 8 + t * 2 + (e & 1)) * FP + u + (e >> 1) * 8] = p;
+				p[n][e] = exp2_fast(p[n][e]);
+				l[n][e & 1] += p[n][e];
+				sp[(n * 8 + t * 2 + (e & 1)) * FP + u + (e >> 1) * 8] = p[n][e];
 			}
-		}
 		__syncwarp();
 		// ---- sums: values' entries as rows of the product ----
+		Values<VG> v;
+#pragma unroll
+		for (int i = 0; i < 4; i++) read_words<VG / 2>(stage + VK + (t * (VG * 4) + ((i * VG) ^ (u * VG / 8) ^ (t * 2))) * 16 + u * (VG * 2) % 16, v.w[i]);
+		read_words<2 * VG>(stage + VS + t * (VG * 8), v.s);
+		uint32_t vs[NT][2 * VG];
+		float4 p4[NT];
 #pragma unroll
 		for (int n = 0; n < NT; n++) {
-			uint32_t vs[2 * VG];
 #pragma unroll
-			for (int i = 0; i < 2 * VG; i++) vs[i] = v.s[i];
+			for (int i = 0; i < 2 * VG; i++) vs[n][i] = v.s[i];
 			if (!all) { // what the row does not see may have any scale, a NaN too
 				const int lim = s_lim[n * 8 + u];
 #pragma unroll
 				for (int i = 0; i < 4; i++)
 					if (at + t * 4 + i >= lim)
 #pragma unroll
-						for (int w = 0; w < VG / 2; w++) vs[i * (VG / 2) + w] = 0;
+						for (int w = 0; w < VG / 2; w++) vs[n][i * (VG / 2) + w] = 0;
 			}
-			__half2 big = __float2half2_rn(0.f);
+			uint32_t big = vs[n][0];
 #pragma unroll
-			for (int i = 0; i < 2 * VG; i++) {
-				const uint32_t y = vs[i] & 0x7fff7fffu;
-				big = __hmax2(big, *reinterpret_cast<const __half2*>(&y));
-			}
-			const float top = fmaxf(__low2float(big), __high2float(big));
+			for (int i = 1; i < 2 * VG; i++) big = max_abs2(big, vs[n][i]);
+			const float top = fmaxf(fabsf(half_lo(big)), fabsf(half_hi(big)));
 			if (__any_sync(0xffffffffu, top > room[n])) {
 				float y = fmaxf(top, room[n]);
 				y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
@@ -286,38 +291,43 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 				const float f0 = __shfl_sync(0xffffffffu, f, t * 8), f1 = __shfl_sync(0xffffffffu, f, t * 8 + 4);
 #pragma unroll
 				for (int i = 0; i < VG * 2; i++) { acc[i][n][0] *= f0; acc[i][n][2] *= f0; acc[i][n][1] *= f1; acc[i][n][3] *= f1; }
-#pragma unroll
-				for (int g = 0; g < VG; g++) part[n][g] *= f;
 			}
-			float4 p = *reinterpret_cast<const float4*>(sp + (n * 8 + u) * FP + t * 4);
-			p.x *= mu[n]; p.y *= mu[n]; p.z *= mu[n]; p.w *= mu[n];
+			p4[n] = *reinterpret_cast<const float4*>(sp + (n * 8 + u) * FP + t * 4);
+			p4[n].x *= mu[n]; p4[n].y *= mu[n]; p4[n].z *= mu[n]; p4[n].w *= mu[n];
+		}
 #pragma unroll
-			for (int g = 0; g < VG; g++) {
+		for (int g = 0; g < VG; g++) {
+			const uint32_t sel = g & 1 ? 0x7632 : 0x5410;
+			uint32_t ab[4], cd[4];
+			codes4(__byte_perm(v.w[0][g / 2], v.w[1][g / 2], sel), ab);
+			codes4(__byte_perm(v.w[2][g / 2], v.w[3][g / 2], sel), cd);
+#pragma unroll
+			for (int n = 0; n < NT; n++) {
 				float y[4];
 #pragma unroll
 				for (int i = 0; i < 4; i++) {
-					const uint32_t w = vs[i * (VG / 2) + g / 2];
-					y[i] = (i == 0 ? p.x : i == 1 ? p.y : i == 2 ? p.z : p.w) * (g & 1 ? half_hi(w) : half_lo(w));
+					const uint32_t w = vs[n][i * (VG / 2) + g / 2];
+					y[i] = (i == 0 ? p4[n].x : i == 1 ? p4[n].y : i == 2 ? p4[n].z : p4[n].w) * (g & 1 ? half_hi(w) : half_lo(w));
 				}
-				if constexpr (!WIDE) part[n][g] += (y[0] + y[1]) + (y[2] + y[3]);
-				const uint32_t hi0 = pack_half(y[0], y[1]), hi1 = pack_half(y[2], y[3]);
-				const uint32_t lo0 = pack_half(y[0] - half_lo(hi0), y[1] - half_hi(hi0)), lo1 = pack_half(y[2] - half_lo(hi1), y[3] - half_hi(hi1));
-				const uint32_t sel = g & 1 ? 0x7632 : 0x5410;
-				uint32_t ab[4], cd[4];
-				codes4<WIDE>(__byte_perm(v.w[0][g / 2], v.w[1][g / 2], sel), ab);
-				codes4<WIDE>(__byte_perm(v.w[2][g / 2], v.w[3][g / 2], sel), cd);
+				uint32_t b0 = pack_half(y[0], y[1]), b1 = pack_half(y[2], y[3]), r0 = 0, r1 = 0;
+				if constexpr (SPLIT || TWO) {
+					r0 = pack_half(y[0] - half_lo(b0), y[1] - half_hi(b0));
+					r1 = pack_half(y[2] - half_lo(b1), y[3] - half_hi(b1));
+				}
+				if constexpr (SPLIT) {
+					b0 = u < 4 ? b0 : r0;
+					b1 = u < 4 ? b1 : r1;
+				}
 #pragma unroll
 				for (int i = 0; i < 2; i++) {
-					if constexpr (SPLIT) mma16(acc[g * 2 + i][n], ab[2 * i], ab[2 * i + 1], cd[2 * i], cd[2 * i + 1], u < 4 ? hi0 : lo0, u < 4 ? hi1 : lo1);
-					else {
-						mma16(acc[g * 2 + i][n], ab[2 * i], ab[2 * i + 1], cd[2 * i], cd[2 * i + 1], hi0, hi1);
-						mma16(acc[g * 2 + i][n], ab[2 * i], ab[2 * i + 1], cd[2 * i], cd[2 * i + 1], lo0, lo1);
-					}
+					mma16(acc[g * 2 + i][n], ab[2 * i], ab[2 * i + 1], cd[2 * i], cd[2 * i + 1], b0, b1);
+					if constexpr (TWO) mma16(acc[g * 2 + i][n], ab[2 * i], ab[2 * i + 1], cd[2 * i], cd[2 * i + 1], r0, r1);
 				}
 			}
 		}
-		load_values(at + KT, id);
 	}
+	asm volatile("cp.async.wait_group 0;" ::: "memory");
+	__syncwarp(); // the sums take the stages' place
 	// ---- this warp's maxima, sums and rows ----
 #pragma unroll
 	for (int n = 0; n < NT; n++) {
@@ -325,51 +335,37 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 		for (int c = 0; c < 2; c++)
 #pragma unroll
 			for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
-		const float inv = 1.f / mu[n]; // a power of two
+		const float inv = 1024.f / mu[n]; // a power of two; codes were taken as 2^-10 each
 		const float i0 = __shfl_sync(0xffffffffu, inv, t * 8), i1 = __shfl_sync(0xffffffffu, inv, t * 8 + 4);
 		const int row = SPLIT ? n * 4 + t * 2 : n * 8 + t * 2;
-		const bool mine = (!SPLIT || t < 2) && row < most_rows;
+		const bool mine = !SPLIT || t < 2;
 		if (mine && u == 0) {
-			s_ml[warp * most_rows + row] = make_float2(m[n][0], l[n][0]);
-			s_ml[warp * most_rows + row + 1] = make_float2(m[n][1], l[n][1]);
+			s_ml[warp * Z::M + row] = make_float2(m[n][0] == NONE ? -INFINITY : m[n][0], l[n][0]);
+			s_ml[warp * Z::M + row + 1] = make_float2(m[n][1] == NONE ? -INFINITY : m[n][1], l[n][1]);
 		}
 #pragma unroll
-		for (int g = 0; g < VG; g++) {
-			float z = part[n][g];
-			z += __shfl_xor_sync(0xffffffffu, z, 1);
-			z += __shfl_xor_sync(0xffffffffu, z, 2);
-			const float z0 = __shfl_sync(0xffffffffu, z, t * 8), z1 = __shfl_sync(0xffffffffu, z, t * 8 + 4);
-			float y[2][4]; // the row's entries 4 u .. 4 u + 3 of the block
+		for (int g = 0; g < VG; g++)
 #pragma unroll
-			for (int c = 0; c < 2; c++) {
-				y[c][0] = acc[g * 2][n][c];
-				y[c][1] = acc[g * 2][n][c + 2];
-				y[c][2] = acc[g * 2 + 1][n][c];
-				y[c][3] = acc[g * 2 + 1][n][c + 2];
+			for (int c = 0; c < 2; c++) { // the row's entries 4 u .. 4 u + 3 of the block
+				float y[4] = {acc[g * 2][n][c], acc[g * 2][n][c + 2], acc[g * 2 + 1][n][c], acc[g * 2 + 1][n][c + 2]};
 #pragma unroll
 				for (int e = 0; e < 4; e++) {
-					if constexpr (SPLIT) y[c][e] += __shfl_xor_sync(0xffffffffu, y[c][e], 2);
-					if constexpr (!WIDE) y[c][e] = y[c][e] * 1048576.f - 8.f * (c ? z1 : z0); // codes were taken as 2^-20 each
-					y[c][e] *= c ? i1 : i0;
+					if constexpr (SPLIT) y[e] += __shfl_xor_sync(0xffffffffu, y[e], 2);
+					y[e] *= c ? i1 : i0;
 				}
+				if (mine) *reinterpret_cast<float4*>(reinterpret_cast<float*>(stages) + (row + c) * Z::OP + g * 32 + u * 4) = make_float4(y[0], y[1], y[2], y[3]);
 			}
-			if (mine) {
-				*reinterpret_cast<float4*>(s_o + (warp * most_rows + row) * op + g * 32 + u * 4) = make_float4(y[0][0], y[0][1], y[0][2], y[0][3]);
-				*reinterpret_cast<float4*>(s_o + (warp * most_rows + row + 1) * op + g * 32 + u * 4) = make_float4(y[1][0], y[1][1], y[1][2], y[1][3]);
-			}
-		}
 	}
 }
 
 template <int KG, int VG, int KIND>
-__global__ void __launch_bounds__(FT, KIND == FEW && VG < 8 ? 3 : 2) paged4_attn_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const Pool4 pool, const int type) {
+__global__ void __launch_bounds__(FT, Size4<KG, VG, KIND>::CTAS) paged4_attn_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const Pool4 pool, const int type) {
 	using Z = Size4<KG, VG, KIND>;
-	constexpr int M = Z::M, OP = Z::OP, TILE = KIND == F32 ? 4 : 8; // rows of a tile of columns
+	constexpr int M = Z::M, OP = Z::OP;
 	extern __shared__ __align__(16) uint8_t smem[];
-	uint2* s_q = reinterpret_cast<uint2*>(smem);                       // [NT][KG][2][32]: queries as the product wants them
-	float* s_init = reinterpret_cast<float*>(s_q + Z::NT * KG * 2 * 32); // [NT][KG][8]: -8 times the sum of a block's queries
-	float* s_o = s_init + Z::NT * KG * 8;                              // [FW][M][OP]
-	float* s_p = s_o + Z::SUMS;                                        // [FW][NT * 8][FP]
+	uint8_t* s_ring = smem;                                            // [FW][WARP]
+	uint2* s_q = reinterpret_cast<uint2*>(s_ring + FW * Z::WARP);      // [NT][KG][2][32]: queries as the product wants them
+	float* s_p = reinterpret_cast<float*>(s_q + Z::NT * KG * 2 * 32);  // [FW][NT * 8][FP]
 	float2* s_ml = reinterpret_cast<float2*>(s_p + FW * Z::NT * 8 * FP); // [FW][M]
 	float* s_fac = reinterpret_cast<float*>(s_ml + FW * M);            // [NT * 8]: from a product to a score in units of log2
 	int* s_lim = reinterpret_cast<int*>(s_fac + Z::NT * 8);            // [NT * 8]: keys that the column's row sees
@@ -387,8 +383,7 @@ __global__ void __launch_bounds__(FT, KIND == FEW && VG < 8 ? 3 : 2) paged4_attn
 		const int shared = plan.shs[x.s];
 		const bool prefix = x.seg < a.b.n_groups;
 		const int rows = min(M, x.rows - x.t * M), h0 = x.g * a.rep;
-		const bool split = KIND == F32 || (KIND == FEW && rows <= 4);
-		const int per = split ? 4 : 8, tiles = (rows + per - 1) / per;
+		constexpr bool split = Z::SPLIT;
 		auto keys_of = [&](int r) { return prefix ? shared : own_keys(x.q, shared, a.rep, x.t * M + r); };
 		__syncthreads(); // the piece before is written
 		for (int n = warp; n < Z::NT; n += FW) { // queries, a tile of columns to a warp: 8 entries of each block to a lane
@@ -409,9 +404,9 @@ __global__ void __launch_bounds__(FT, KIND == FEW && VG < 8 ? 3 : 2) paged4_attn
 			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
 			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
 			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
-			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 127);
+			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
 			const float f = pow2(e);
-			if (t == 0) s_fac[n * 8 + u] = fminf(fmaxf(a.scale * 1.4426950408889634f * pow2(12 - e) * (KIND == F32 ? 1.f / 4096.f : 256.f), -3.0e38f), 3.0e38f);
+			if (t == 0) s_fac[n * 8 + u] = fminf(fmaxf(a.scale * 1.4426950408889634f * pow2(10 - e), -3.0e38f), 3.0e38f);
 #pragma unroll
 			for (int g = 0; g < KG; g++) {
 				float z[8];
@@ -419,30 +414,17 @@ __global__ void __launch_bounds__(FT, KIND == FEW && VG < 8 ? 3 : 2) paged4_attn
 				for (int i = 0; i < 8; i++) {
 					const float full = y[g][i] * f;
 					float h = __half2float(__float2half_rn(full));
-					if (KIND == F32 && u >= 4) h = full - h; // the rest
+					if (Z::WIDE && u >= 4) h = full - h; // the rest
 					z[i] = h;
 				}
-				const uint2 qa = make_uint2(pack_half(z[0], z[4]), pack_half(z[1], z[5])), qb = make_uint2(pack_half(z[2], z[6]), pack_half(z[3], z[7]));
-				s_q[((n * KG + g) * 2) * 32 + lane] = qa;
-				s_q[((n * KG + g) * 2 + 1) * 32 + lane] = qb;
-				float sum = ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
-				sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-				sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-				if (t == 0) s_init[(n * KG + g) * 8 + u] = KIND == F32 ? 0.f : sum * -7.62939453125e-6f; // 8 codes of 2^-20
+				s_q[((n * KG + g) * 2) * 32 + lane] = make_uint2(pack_half(z[0], z[4]), pack_half(z[1], z[5]));
+				s_q[((n * KG + g) * 2 + 1) * 32 + lane] = make_uint2(pack_half(z[2], z[6]), pack_half(z[3], z[7]));
 			}
 		}
 		__syncthreads();
 		const int vis = keys_of(rows - 1), least = keys_of(0); // the last row sees the most
 		float* sp = s_p + warp * Z::NT * 8 * FP;
-		if constexpr (KIND == F32) {
-			if (tiles == 1) piece4<KG, VG, 1, true, true>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
-			else if (tiles == 2) piece4<KG, VG, 2, true, true>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
-			else if constexpr (Z::NT == 4) piece4<KG, VG, 4, true, true>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
-		} else if constexpr (KIND == FEW) {
-			if (split) piece4<KG, VG, 1, true, false>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
-			else if (tiles == 1) piece4<KG, VG, 1, false, false>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
-			else piece4<KG, VG, 2, false, false>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
-		} else piece4<KG, VG, Z::NT, false, false>(a, pool, x, vis, least, s_q, s_init, s_fac, s_lim, sp, s_o, s_ml, OP, M);
+		piece4<Z, KG, VG>(a, pool, x, vis, least, s_q, s_fac, s_lim, sp, s_ring + warp * Z::WARP, s_ml);
 		__syncthreads();
 		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
 		const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
@@ -457,7 +439,7 @@ __global__ void __launch_bounds__(FT, KIND == FEW && VG < 8 ? 3 : 2) paged4_attn
 				const float2 ml = s_ml[e * M + row];
 				const bool some = ml.x != -INFINITY || ml.y != 0.f; // else nothing that the row sees; a sum that is NaN stays one
 				const float f = !some ? 0.f : ml.x == -INFINITY ? 1.f : exp2f(ml.x - mx);
-				const float4 o = *reinterpret_cast<const float4*>(s_o + (e * M + row) * OP + col);
+				const float4 o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(s_ring + e * Z::WARP) + row * OP + col);
 				l += ml.y * f;
 				v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
 			}
@@ -490,8 +472,7 @@ static Shape4 shape_of(const BatchView& b) {
 	using Z = Size4<KG, VG, KIND>;
 	if (Z::NT == 0) return Shape4{0, 0};
 	const size_t smem = Z::own + plan_bytes(b.B, b.n_groups);
-	const int most = KIND == FEW && VG < 8 ? 3 : 2;
-	return Shape4{Z::M, std::max(1, std::min(most, (int) (226 * 1024 / (smem + 1024))))};
+	return Shape4{Z::M, std::max(1, std::min(Z::CTAS, (int) (226 * 1024 / (smem + 1024))))};
 }
 template <int KIND>
 static Shape4 shape4(const Pool4& p, const BatchView& b) {
@@ -502,9 +483,10 @@ static Shape4 shape4(const Pool4& p, const BatchView& b) {
 	}
 	return Shape4{0, 0};
 }
-Shape4 attn4_few(const Pool4& p, const BatchView& b) { return shape4<FEW>(p, b); }
-Shape4 attn4_many(const Pool4& p, const BatchView& b) { return shape4<MANY>(p, b); }
-Shape4 attn4_f32(const Pool4& p, const BatchView& b) { return shape4<F32>(p, b); }
+Shape4 attn4_shape(const Pool4& p, const BatchView& b, int kind) {
+	return kind == B8 ? shape4<B8>(p, b) : kind == B16 ? shape4<B16>(p, b) : kind == B32 ? shape4<B32>(p, b) : kind == H4 ? shape4<H4>(p, b) : kind == H16 ? shape4<H16>(p, b) : kind == H32 ? shape4<H32>(p, b)
+	       : kind == F4 ? shape4<F4>(p, b) : shape4<F16>(p, b);
+}
 
 template <int KG, int VG, int KIND>
 static int launch_kind(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
@@ -515,14 +497,26 @@ static int launch_kind(const Attn& a, const Pool4& p, int part, int type, cudaSt
 	}
 	return XALM_OK;
 }
-int launch_attn4(const Attn& a, const Pool4& p, int part, int type, bool many, cudaStream_t s) {
+template <int KIND>
+static int launch_blocks(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
 	switch (p.kg * 16 + p.vg) {
-#define XALM_PAGED4(K, V) \
-	case K * 16 + V: return type == XALM_F32 ? launch_kind<K, V, F32>(a, p, part, type, s) : many ? launch_kind<K, V, MANY>(a, p, part, type, s) : launch_kind<K, V, FEW>(a, p, part, type, s);
+#define XALM_PAGED4(K, V) case K * 16 + V: return launch_kind<K, V, KIND>(a, p, part, type, s);
 		XALM_PAGED4(2, 2) XALM_PAGED4(2, 4) XALM_PAGED4(2, 8) XALM_PAGED4(4, 2) XALM_PAGED4(4, 4) XALM_PAGED4(4, 8) XALM_PAGED4(8, 2) XALM_PAGED4(8, 4) XALM_PAGED4(8, 8)
 #undef XALM_PAGED4
 	}
 	return set_error(XALM_ERR_INVALID, "paged attention: %d and %d blocks", p.kg, p.vg);
+}
+int launch_attn4(const Attn& a, const Pool4& p, int part, int type, int kind, cudaStream_t s) {
+	switch (kind) {
+		case B8: return launch_blocks<B8>(a, p, part, type, s);
+		case B16: return launch_blocks<B16>(a, p, part, type, s);
+		case B32: return launch_blocks<B32>(a, p, part, type, s);
+		case H4: return launch_blocks<H4>(a, p, part, type, s);
+		case H16: return launch_blocks<H16>(a, p, part, type, s);
+		case H32: return launch_blocks<H32>(a, p, part, type, s);
+		case F4: return launch_blocks<F4>(a, p, part, type, s);
+		default: return launch_blocks<F16>(a, p, part, type, s);
+	}
 }
 
 } // namespace paged
