@@ -2,6 +2,7 @@
 #include "paged4.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace xalm {
 namespace paged {
@@ -30,25 +31,30 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 	             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) { // added to nothing
+	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+	             : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+	             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 // N words of shared memory from an address that is a multiple of their size (of 16 bytes at most)
 template <int N>
-__device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&x)[N]) {
-	if constexpr (N == 1) x[0] = *reinterpret_cast<const uint32_t*>(p);
-	else if constexpr (N == 2) {
-		const uint2 y = *reinterpret_cast<const uint2*>(p);
-		x[0] = y.x; x[1] = y.y;
-	} else
+__device__ __forceinline__ void read_words(uint32_t p, uint32_t (&x)[N]) {
+	if constexpr (N == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[0]) : "r"(p));
+	else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(p));
+	else
 #pragma unroll
-		for (int i = 0; i < N; i += 4) {
-			const uint4 y = *reinterpret_cast<const uint4*>(p + i * 4);
-			x[i] = y.x; x[i + 1] = y.y; x[i + 2] = y.z; x[i + 3] = y.w;
-		}
+		for (int i = 0; i < N; i += 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]) : "r"(p + i * 4));
+}
+// A number that is kept in a register, not computed again wherever it is used
+__device__ __forceinline__ uint32_t kept(uint32_t x) {
+	asm volatile("" : "+r"(x));
+	return x;
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool there) { // zeros where there is nothing
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short) w)); }
-__device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short) (w >> 16))); }
+__device__ __forceinline__ float half_lo(uint32_t w) { return __low2float(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float half_hi(uint32_t w) { return __high2float(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 	uint32_t r;
 	asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -88,17 +94,18 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
 	return r;
 }
 
-// What a lane holds of 16 keys and values as they come: of keys lane / 4 and 8 behind it a word of each block, of values 4 (lane % 4) .. + 3 four entries of each
+// What a lane holds of 16 keys and values: of keys lane / 4 and 8 behind it a word of each block, of values lane % 4, and 4, 8 and 12 behind it, four entries of each
 template <int KG>
 struct Keys {
 	uint32_t w[2][KG], s[2][KG / 2];
 };
 template <int VG>
 struct Values {
-	uint32_t w[4][VG / 2], s[4 * VG / 2]; // scales: value by value
+	uint32_t w[4][VG / 2], s[4][VG / 2];
 };
 
 constexpr float NONE = -3.0e38f; // the maximum before the first key
+__device__ __forceinline__ float less(float x) { return x > 2.f ? 2.f : x; } // a NaN stays one
 
 // A piece by one warp: its 16 keys of each tile, the unit's rows as columns of the products
 template <typename Z, int KG, int VG>
@@ -126,53 +133,51 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 		room[n] = 0.f;
 	}
 	const int* table = a.b.table + (long long) x.s * a.b.table_row;
-	const uint8_t* head = pool.at + x.g * pool.head;
 	int at = x.j0 * KT + warp * FK;
 	const int end = min(x.j1 * KT, vis);
 	auto id_at = [&](int key) { return key < end ? table[(x.key0 + key) >> a.c.shift] : 0; }; // looked at when its page is asked for
-	// Copies, each lane's own 16 bytes at a time.  Values' 16 bytes lie in another order: those of keys 4 t + i, which four lanes t ask for at once, in different banks.
+	// Copies, each lane's own 16 bytes at a time.  Values' 16 bytes lie in another order: those that four lanes t ask for at once, of keys t, in different banks.
 	constexpr int VK = KG * 256, KS = VK + VG * 256, VS = KS + KG * 32; // sections of a stage
-	const uint32_t ring = smem_u32(stages);
+	auto turn = [](int key) { return VG == 8 ? (key & 3) * 32 : VG == 4 ? (key & 2) * 16 : 0; };
+	const uint32_t ring = smem_u32(stages), to_k = kept(ring + lane * 16), to_v = kept(ring + VK + ((lane * 16) ^ turn(lane / VG)));
+	const uint32_t k_lane = kept(ring + u * (KG * 16) + t * (KG * 4)), ks_lane = kept(ring + KS + u * (KG * 2)), v_lane = kept(ring + VK + t * (VG * 16) + ((u * (VG * 2)) ^ turn(t))),
+	               vs_lane = kept(ring + VS + t * (VG * 2));
+	const uint32_t p_write = kept(smem_u32(sp) + (t * 2 * FP + (u & 3) * 4 + (u >> 2)) * 4), p_read = kept(smem_u32(sp) + (u * FP + t * 4) * 4); // keys t, t + 4, .. side by side
+	const int v_at = values_at(KG, a.c.shift), s_at = lane < KG * 2 ? key_scales_at(KG, a.c.shift) : value_scales_at(KG, VG, a.c.shift) - KG * 32, s_by = lane < KG * 2 ? KG * 2 : VG * 2;
+	const uint8_t* from = pool.at + x.g * pool.head + lane * 16;
 	auto bring = [&](int key, int id, int to) {
-		if (key < end) {
-			const bool there = (unsigned) id < (unsigned) a.c.pages;
-			if (!there && lane == 0) report(a.c, ERR_PAGE); // reads as zeros
-			const uint8_t* run = head + (there ? id : 0) * pool.page;
-			const int slot = (x.key0 + key) & (P - 1), shift = a.c.shift;
-			const uint32_t dst = ring + to * STAGE;
-			const uint8_t *kw = run + slot * (KG * 16) + lane * 16, *vw = run + values_at(KG, shift) + slot * (VG * 16) + lane * 16;
+		const bool good = (unsigned) id < (unsigned) a.c.pages, there = good && key < end; // what is not there reads as zeros
+		if (!good && lane == 0) report(a.c, ERR_PAGE);
+		const uint8_t* run = from + (good ? id : 0) * pool.page;
+		const int slot = (x.key0 + key) & (P - 1);
+		const uint8_t *kw = run + slot * (KG * 16), *vw = run + (v_at + slot * (VG * 16));
 #pragma unroll
-			for (int i = 0; i < KG / 2; i++) copy16(dst + lane * 16 + i * 512, kw + i * 512, there);
+		for (int i = 0; i < KG / 2; i++) copy16(to_k + to + i * 512, kw + i * 512, there);
 #pragma unroll
-			for (int i = 0; i < VG / 2; i++) {
-				const int unit = lane + i * 32;
-				copy16(dst + VK + (unit ^ ((unit / VG >> 2 & 3) * 2)) * 16, vw + i * 512, there);
-			}
-			if (lane < (KG + VG) * 2)
-				copy16(dst + KS + lane * 16, lane < KG * 2 ? run + key_scales_at(KG, shift) + slot * (KG * 2) + lane * 16 : run + value_scales_at(KG, VG, shift) + slot * (VG * 2) + (lane - KG * 2) * 16, there);
-		}
+		for (int i = 0; i < VG / 2; i++) copy16(to_v + to + i * 512, vw + i * 512, there);
+		if ((KG + VG) * 2 == 32 || lane < (KG + VG) * 2) copy16(to_k + to + KS, run + (s_at + slot * s_by), there);
 		asm volatile("cp.async.commit_group;" ::: "memory");
 	};
-	int id = id_at(at), full = 0, free = STAGES - 1; // the stage to be read, and the one to be filled
+	int id = id_at(at), full = 0, free = (STAGES - 1) * STAGE; // the stage to be read, and the one to be filled
 #pragma unroll
 	for (int i = 0; i < STAGES - 1; i++) {
-		bring(at + i * KT, id, i);
+		bring(at + i * KT, id, i * STAGE);
 		id = id_at(at + (i + 1) * KT);
 	}
-	for (; at < end; at += KT) {
-		const bool all = at + FK <= least; // every row sees every key
+	auto step = [&](auto edge) {
+		constexpr bool EDGE = decltype(edge)::value; // some rows may not see some keys
 		asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
 		__syncwarp(); // the stage is there, and nobody reads the one before any more
 		bring(at + (STAGES - 1) * KT, id, free);
 		id = id_at(at + STAGES * KT);
-		const uint8_t* stage = stages + full * STAGE;
+		const int stage = full;
 		free = full;
-		full = full == STAGES - 1 ? 0 : full + 1;
+		full = full == (STAGES - 1) * STAGE ? 0 : full + STAGE;
 		Keys<KG> k;
 #pragma unroll
 		for (int i = 0; i < 2; i++) {
-			read_words<KG>(stage + (u + i * 8) * (KG * 16) + t * (KG * 4), k.w[i]);
-			read_words<KG / 2>(stage + KS + (u + i * 8) * (KG * 2), k.s[i]);
+			read_words<KG>(k_lane + stage + i * (KG * 128), k.w[i]);
+			read_words<KG / 2>(ks_lane + stage + i * (KG * 16), k.s[i]);
 		}
 		// ---- scores: keys as rows of the product ----
 		float s[NT][4];
@@ -194,8 +199,8 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 					qa = s_q[((n * KG + g) * 2) * 32 + lane];
 					qb = s_q[((n * KG + g) * 2 + 1) * 32 + lane];
 				}
-				float c[4] = {0.f, 0.f, 0.f, 0.f};
-				mma16(c, h0[0], h1[0], h0[1], h1[1], qa.x, qa.y);
+				float c[4];
+				mma16_new(c, h0[0], h1[0], h0[1], h1[1], qa.x, qa.y);
 				mma16(c, h0[2], h1[2], h0[3], h1[3], qb.x, qb.y);
 				s[n][0] = fmaf(c[0], d0, s[n][0]);
 				s[n][1] = fmaf(c[1], d0, s[n][1]);
@@ -212,25 +217,22 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 				for (int e = 0; e < 4; e++) s[n][e] += __shfl_xor_sync(0xffffffffu, s[n][e], 2);
 #pragma unroll
-			for (int e = 0; e < 4; e++) s[n][e] *= e & 1 ? fac[n].y : fac[n].x;
-			if (!all) {
+			for (int e = 0; e < 4; e++) p[n][e] = fmaf(s[n][e], e & 1 ? fac[n].y : fac[n].x, -m[n][e & 1]);
+			if constexpr (EDGE) {
 				const int2 lim = *reinterpret_cast<const int2*>(s_lim + n * 8 + t * 2);
 #pragma unroll
 				for (int e = 0; e < 4; e++)
-					if (at + u + (e >> 1) * 8 >= (e & 1 ? lim.y : lim.x)) s[n][e] = -INFINITY;
+					if (at + u + (e >> 1) * 8 >= (e & 1 ? lim.y : lim.x)) p[n][e] = -INFINITY;
 			}
-#pragma unroll
-			for (int e = 0; e < 4; e++) {
-				p[n][e] = s[n][e] - m[n][e & 1]; // exact where they are near, however large
-				grow = grow || p[n][e] > 2.f;
-			}
+			grow = grow || fmaxf(fmaxf(p[n][0], p[n][1]), fmaxf(p[n][2], p[n][3])) > 2.f;
 		}
 		if (__any_sync(0xffffffffu, grow)) { // rare behind the first keys: probabilities may be up to 4
 #pragma unroll
 			for (int n = 0; n < NT; n++)
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
-					float top = fmaxf(s[n][c], s[n][c + 2]);
+					const float f0 = c ? fac[n].y : fac[n].x;
+					float top = fmaxf(p[n][c] == -INFINITY ? NONE : s[n][c] * f0, p[n][c + 2] == -INFINITY ? NONE : s[n][c + 2] * f0);
 #pragma unroll
 					for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 					top = fmaxf(m[n][c], top);
@@ -239,8 +241,8 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 					l[n][c] *= f;
 #pragma unroll
 					for (int i = 0; i < VG * 2; i++) { acc[i][n][c] *= f; acc[i][n][c + 2] *= f; }
-					p[n][c] = s[n][c] - top;
-					p[n][c + 2] = s[n][c + 2] - top;
+					if (p[n][c] != -INFINITY) p[n][c] = less(fmaf(s[n][c], f0, -top)); // scores of 2^24 and more are rounded by whole numbers
+					if (p[n][c + 2] != -INFINITY) p[n][c + 2] = less(fmaf(s[n][c + 2], f0, -top));
 				}
 		}
 		__syncwarp();
@@ -250,25 +252,27 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 			for (int e = 0; e < 4; e++) {
 				p[n][e] = exp2_fast(p[n][e]);
 				l[n][e & 1] += p[n][e];
-				sp[(n * 8 + t * 2 + (e & 1)) * FP + u + (e >> 1) * 8] = p[n][e];
+				asm volatile("st.shared.f32 [%0], %1;" ::"r"(p_write + ((n * 8 + (e & 1)) * FP + (e >> 1) * 2) * 4), "f"(p[n][e]) : "memory");
 			}
 		__syncwarp();
 		// ---- sums: values' entries as rows of the product ----
 		Values<VG> v;
 #pragma unroll
-		for (int i = 0; i < 4; i++) read_words<VG / 2>(stage + VK + (t * (VG * 4) + ((i * VG) ^ (u * VG / 8) ^ (t * 2))) * 16 + u * (VG * 2) % 16, v.w[i]);
-		read_words<2 * VG>(stage + VS + t * (VG * 8), v.s);
+		for (int i = 0; i < 4; i++) {
+			read_words<VG / 2>(v_lane + stage + i * (VG * 64), v.w[i]);
+			read_words<VG / 2>(vs_lane + stage + i * (VG * 8), v.s[i]);
+		}
 		uint32_t vs[NT][2 * VG];
 		float4 p4[NT];
 #pragma unroll
 		for (int n = 0; n < NT; n++) {
 #pragma unroll
-			for (int i = 0; i < 2 * VG; i++) vs[n][i] = v.s[i];
-			if (!all) { // what the row does not see may have any scale, a NaN too
+			for (int i = 0; i < 2 * VG; i++) vs[n][i] = v.s[i / (VG / 2)][i % (VG / 2)];
+			if constexpr (EDGE) { // what the row does not see may have any scale, a NaN too
 				const int lim = s_lim[n * 8 + u];
 #pragma unroll
 				for (int i = 0; i < 4; i++)
-					if (at + t * 4 + i >= lim)
+					if (at + t + i * 4 >= lim)
 #pragma unroll
 						for (int w = 0; w < VG / 2; w++) vs[n][i * (VG / 2) + w] = 0;
 			}
@@ -292,7 +296,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 				for (int i = 0; i < VG * 2; i++) { acc[i][n][0] *= f0; acc[i][n][2] *= f0; acc[i][n][1] *= f1; acc[i][n][3] *= f1; }
 			}
-			p4[n] = *reinterpret_cast<const float4*>(sp + (n * 8 + u) * FP + t * 4);
+			asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(p4[n].x), "=f"(p4[n].y), "=f"(p4[n].z), "=f"(p4[n].w) : "r"(p_read + n * 8 * FP * 4));
 			p4[n].x *= mu[n]; p4[n].y *= mu[n]; p4[n].z *= mu[n]; p4[n].w *= mu[n];
 		}
 #pragma unroll
@@ -325,7 +329,9 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 				}
 			}
 		}
-	}
+	};
+	for (; at + FK <= least && at < end; at += KT) step(std::false_type());
+	for (; at < end; at += KT) step(std::true_type());
 	asm volatile("cp.async.wait_group 0;" ::: "memory");
 	__syncwarp(); // the sums take the stages' place
 	// ---- this warp's maxima, sums and rows ----
