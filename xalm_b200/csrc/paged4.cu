@@ -225,7 +225,8 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 }
 
 // What a piece costs beside its tiles, in tiles
-constexpr int LEAD4 = 6, LEAD4_MANY = 6, LEAD4_F32 = 6;
+constexpr int LEAD4 = 6, LEAD4_MANY = 6, LEAD4_F32 = 6, LEAD4_TILE = 4;
+constexpr int TILE_ROWS = 32; // rows of a segment that the kernel of many rows is not for
 constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
 
 static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, int (&kinds)[2]) {
@@ -238,13 +239,19 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 	a.b = b;
 	a.H = heads;
 	a.rep = heads / c.G;
-	// The kernel of most segments by the rows that one has on average, and where some may have more than its unit, one of more rows for those
+	// The kernel of most segments by the rows that one has on average, and where some may have more than TILE_ROWS, the one of many rows for those
 	const long long rows_all = (long long) b.N * a.rep, each = (rows_all + b.B - 1) / std::max(b.B, 1);
-	const int least = type == XALM_F32 ? each <= 4 ? F4 : F16 : type == XALM_F16 ? each <= 4 ? H4 : H16 : each <= 8 ? B8 : B16, most_kind = type == XALM_F16 ? H32 : B32;
-	const Shape4 few = attn4_shape(p, b, least), more = attn4_shape(p, b, most_kind);
-	const bool many = type != XALM_F32 && more.rows && (b.n_groups || b.N > b.B || a.rep > few.rows) && rows_all > few.rows;
-	kinds[0] = many ? most_kind : least;
-	kinds[1] = least;
+	const bool tile = type != XALM_F32 && tile4_shape(p).rows && (b.n_groups || b.N > b.B || a.rep > TILE_ROWS) && rows_all > TILE_ROWS;
+	const int size = each <= 4 ? 4 : each <= 8 ? 8 : each <= 16 || (tile && each > TILE_ROWS) ? 16 : 32; // rows of a unit
+	const int few16 = type == XALM_F16 ? size == 4 ? H4 : size < 32 ? H16 : H32 : size <= 8 ? B8 : size == 16 ? B16 : B32;
+	const int few_kind = type == XALM_F32 ? size == 4 ? F4 : F16 : attn4_shape(p, b, few16).rows ? few16 : type == XALM_F16 ? H16 : B16;
+	const Shape4 few = attn4_shape(p, b, few_kind);
+	const int more_kind = tile ? TILE : type == XALM_F16 ? H32 : B32;
+	const Shape4 more = tile ? tile4_shape(p) : attn4_shape(p, b, more_kind);
+	const int limit = tile ? TILE_ROWS : few.rows; // rows of a segment above which it is the second kernel's
+	const bool many = type != XALM_F32 && more.rows > few.rows && (b.n_groups || b.N > b.B || a.rep > limit) && rows_all > limit;
+	kinds[0] = many ? more_kind : few_kind;
+	kinds[1] = few_kind;
 	a.n_parts = many ? 2 : 1;
 	size_t at = 0;
 	auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
@@ -253,11 +260,11 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 		const bool big = many && i == 0;
 		t.M = big ? more.rows : few.rows;
 		t.grid = sms * (big ? more.per_sm : few.per_sm);
-		t.lead = big ? LEAD4_MANY : type == XALM_F32 ? LEAD4_F32 : LEAD4;
-		t.least_rows = big ? few.rows + 1 : 1;
-		t.most_rows = many && !big ? few.rows : 0x7fffffff;
+		t.lead = big ? tile ? LEAD4_TILE : LEAD4_MANY : type == XALM_F32 ? LEAD4_F32 : LEAD4;
+		t.least_rows = big ? limit + 1 : 1;
+		t.most_rows = many && !big ? limit : 0x7fffffff;
 		// as in plan_attn: a segment has at most its rows / M + 1 tiles, in a part that takes short ones only it has one
-		const long long rows = rows_all, whole = many && !big ? 0 : rows / t.M, most = rows / t.least_rows;
+		const long long rows = rows_all, whole = many && !big && limit <= t.M ? 0 : rows / t.M, most = rows / t.least_rows;
 		const long long tiles = whole + std::min((long long) b.B, most) + (b.n_groups ? whole + std::min((long long) b.n_groups, most) : 0);
 		if (tiles * c.G + t.grid > 0x7fffffff / t.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
 		const long long work = ((long long) b.max_pages << c.shift) / KT + 1;
@@ -423,7 +430,7 @@ int xalm_cuda_paged4_attend(const xalm_paged4_cache* cache, const xalm_paged_bat
 	a.lse = lse;
 	a.scale = scale;
 	cudaStream_t s = (cudaStream_t) stream;
-	for (int i = 0; i < a.n_parts; i++) XALM_TRY(launch_attn4(a, p, i, type, kinds[i], s));
+	for (int i = 0; i < a.n_parts; i++) XALM_TRY(kinds[i] == TILE ? launch_attn4_tile(a, p, i, type, s) : launch_attn4(a, p, i, type, kinds[i], s));
 	return launch_join(a, type, s);
 }
 

@@ -1,0 +1,425 @@
+// paged4_tile.cu — attention over paged caches of 4-bit numbers (paged4.cuh) for many rows: prompts, and groups of sequences over their shared pages.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged4.cuh"
+
+namespace xalm {
+namespace paged {
+
+// =========================================================================================================================================
+// As in paged4_attn.cu, but 128 (token, head) rows to a unit, 16 to a warp, so that what has to be done to a key's and a value's codes is done once for all of them: the CTA turns a tile of 64
+// keys into fp16 numbers d (c - 8) / 8 and its values into c - 8 in shared memory, while the tile before enters the products.  Scores by m16n8k16 with the rows as A; probabilities become A of
+// the second product where they are, times the value's scale, block by block: what a row does not see may then have any scale, a NaN too, and is left out.
+// The three roundings of fp16 that this has (d (c - 8), p, p d) are each half of what a result of fp16 is rounded by, or less, and differ from key to key.
+// =========================================================================================================================================
+constexpr int GT = 256, GW = GT / 32, GM = GW * 16; // threads, warps, rows of a unit
+constexpr int RING = 3;                             // tiles on their way or waiting as they come
+
+template <int KG, int VG>
+struct Tile4 {
+	static constexpr int RAW = KT * (KG + VG) * 18, KH = KT * KG * 64, VH = KT * VG * 64; // bytes of a tile as it comes, of its keys and values as fp16
+	static constexpr int SC = KT / 2 * VG * 4;                                             // and of its values' scales, by pairs of keys
+	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + SC) + 2 * KT * 4 + 2 * 4 + GM * 4 + 24;
+};
+
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+	             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void matrices(uint32_t at, uint32_t (&r)[4]) {
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void matrices_turned(uint32_t at, uint32_t (&r)[4]) {
+	asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void copy16_if(uint32_t dst, const uint8_t* src, bool there) { // zeros where there is nothing
+	asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+	uint32_t r;
+	asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+	return r;
+}
+__device__ __forceinline__ uint32_t bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ __half2 halves(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ float ex2(float x) {
+	float y;
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+	return y;
+}
+// a NaN stays one.  (Scores of 2^24 and more are rounded by whole numbers, and may pass the limit by some.)
+__device__ __forceinline__ float at_most(float x, float most) {
+	float y;
+	asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(most));
+	return y;
+}
+__device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
+// A word's codes, c - 8 (EIGHTH: an eighth of that), in the order 0 4 1 5 2 6 3 7: 1024 + c and 1024 + 16 c as they lie, brought there without a rounding
+template <bool EIGHTH>
+__device__ __forceinline__ void numbers(uint32_t w, __half2 (&h)[4]) {
+	const float f = EIGHTH ? 0.125f : 1.f;
+	const uint32_t w8 = w >> 8;
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+		const uint32_t x = ((i < 2 ? w : w8) & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+		h[i] = __hfma2(halves(x), __float2half2_rn(i & 1 ? f / 16.f : f), __float2half2_rn(i & 1 ? -72.f * f : -1032.f * f));
+	}
+}
+
+template <int KG, int VG>
+__global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const Pool4 pool, const int type) {
+	using Z = Tile4<KG, VG>;
+	extern __shared__ __align__(128) uint8_t smem[];
+	uint8_t* s_raw = smem;                                         // [RING][RAW]: key codes, value codes, key scales, value scales
+	uint8_t* s_k = s_raw + RING * Z::RAW;                          // [2][KT][KG * 32] fp16, 16 bytes c of key j at c ^ (j & 7)
+	uint8_t* s_v = s_k + 2 * Z::KH;                                // [2][KT][VG * 32], likewise
+	uint8_t* s_sc = s_v + 2 * Z::VH;                               // [2][KT / 2][VG] pairs of scales
+	float* s_top = reinterpret_cast<float*>(s_sc + 2 * Z::SC);     // [2][KT]: each value's largest scale
+	float* s_most = s_top + 2 * KT;                                // [2]: the tile's
+	int* s_lim = reinterpret_cast<int*>(s_most + 2);               // [GM]: keys that a row sees
+	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_lim + GM);
+	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = lane >> 2, t = lane & 3, dv = a.c.dv, P = 1 << a.c.shift, shift = a.c.shift;
+	Plan plan;
+	pdl_launch_dependents();
+	make_plan<GT>(a, part, s_plan, plan);
+	Walk k;
+	bool more = walk_begin(a, part, plan, k);
+	if (tid == 0) write_head(a, part, k, more, more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, plan.share);
+	const uint32_t raw = smem_u32(s_raw), kh = smem_u32(s_k), vh = smem_u32(s_v), sc = smem_u32(s_sc);
+	for (; more; more = walk_next(a, part, plan, k)) {
+		const Piece& x = k.x;
+		if (x.j0 == x.j1) continue; // the same for every thread
+		const int shared = plan.shs[x.s];
+		const bool prefix = x.seg < a.b.n_groups;
+		const int rows = min(GM, x.rows - x.t * GM), h0 = x.g * a.rep;
+		auto keys_of = [&](int r) { return prefix ? shared : own_keys(x.q, shared, a.rep, x.t * GM + r); };
+		__syncthreads(); // the piece before has been read
+		if (tid < GM) s_lim[tid] = tid < rows ? keys_of(tid) : 0;
+		const int vis = keys_of(rows - 1), first = x.j0 * KT, n_tiles = max(min(x.j1, (vis + KT - 1) / KT) - x.j0, 0);
+		// ---- copies: 16 bytes of codes of a key and of a value to a thread, and of scales to some ----
+		const int* table = a.b.table + (long long) x.s * a.b.table_row;
+		const uint8_t* head = pool.at + x.g * pool.head;
+		auto run_of = [&](int at, bool& there) { // of key `at` of the segment
+			const int key = min(at, vis - 1), id = table[(x.key0 + key) >> shift];
+			const bool good = (unsigned) id < (unsigned) a.c.pages;
+			if (!good) report(a.c, ERR_PAGE); // reads as zeros
+			there = good && at < vis;
+			return head + (good ? id : 0) * pool.page;
+		};
+		auto copy = [&](int i) {
+			if (i < n_tiles) {
+				const uint32_t to = raw + i % RING * Z::RAW;
+				const int at = first + i * KT;
+				bool there;
+				if (tid < KT * KG) { // 16 bytes c of key j at c ^ (j / 2 & 3) where a key has four: a quarter of a warp reads the same c of eight keys
+					const int j = tid / KG, c = tid % KG, slot = (x.key0 + at + j) & (P - 1);
+					const uint8_t* run = run_of(at + j, there);
+					copy16_if(to + j * (KG * 16) + (KG == 4 ? c ^ (j >> 1 & 3) : c) * 16, run + slot * (KG * 16) + c * 16, there);
+				}
+				if (tid < KT * VG) {
+					const int j = tid / VG, c = tid % VG, slot = (x.key0 + at + j) & (P - 1);
+					const uint8_t* run = run_of(at + j, there);
+					copy16_if(to + KT * KG * 16 + j * (VG * 16) + (VG == 4 ? c ^ (j >> 1 & 3) : c) * 16, run + values_at(KG, shift) + slot * (VG * 16) + c * 16, there);
+				}
+				constexpr int KC = KT * KG / 8, VC = KT * VG / 8; // 16 bytes of scales
+				if (tid < KC + VC) {
+					const bool value = tid >= KC;
+					const int c = value ? tid - KC : tid, per = 8 / (value ? VG : KG), j = c * per, slot = (x.key0 + at + j) & (P - 1); // 16 bytes are `per` keys', all of one page
+					const uint8_t* run = run_of(at + j, there);
+					copy16_if(to + KT * (KG + VG) * 16 + tid * 16, run + (value ? value_scales_at(KG, VG, shift) + slot * (VG * 2) : key_scales_at(KG, shift) + slot * (KG * 2)), there);
+				}
+			}
+			asm volatile("cp.async.commit_group;" ::: "memory");
+		};
+		// ---- a tile as fp16: a fourth of a key and of a value to a thread ----
+		auto convert = [&](int i) {
+			const uint8_t* from = s_raw + i % RING * Z::RAW;
+			const int b = i & 1, j = tid & (KT - 1), c = tid / KT;
+			const uint32_t to_k = kh + b * Z::KH + j * (KG * 64), to_v = vh + b * Z::VH + j * (VG * 64);
+			uint32_t w[KG], v[VG], d[KG / 2];
+			if constexpr (KG == 4) {
+				const uint4 y = *reinterpret_cast<const uint4*>(from + j * 64 + (c ^ (j >> 1 & 3)) * 16);
+				w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
+				const uint2 z = *reinterpret_cast<const uint2*>(from + KT * (KG + VG) * 16 + j * 8);
+				d[0] = z.x; d[1] = z.y;
+			} else {
+				const uint2 y = *reinterpret_cast<const uint2*>(from + j * 32 + c * 8);
+				w[0] = y.x; w[1] = y.y;
+				d[0] = *reinterpret_cast<const uint32_t*>(from + KT * (KG + VG) * 16 + j * 4);
+			}
+#pragma unroll
+			for (int g = 0; g < KG; g++) {
+				__half2 h[4];
+				numbers<true>(w[g], h);
+				const __half2 f = halves(__byte_perm(d[g / 2], 0, g & 1 ? 0x3232 : 0x1010));
+				asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to_k + (((g * 4 + c) ^ (j & 7)) * 16)), "r"(bits(__hmul2(h[0], f))), "r"(bits(__hmul2(h[1], f))), "r"(bits(__hmul2(h[2], f))),
+				             "r"(bits(__hmul2(h[3], f))) : "memory");
+			}
+			// entries 8 c .. 8 c + 7 of a value's block: 16 bits each at places 2 c and 2 c + 1
+			if constexpr (VG == 4) {
+				const uint4 y = *reinterpret_cast<const uint4*>(from + KT * KG * 16 + j * 64 + (c ^ (j >> 1 & 3)) * 16);
+				v[0] = __byte_perm(y.x, y.z, 0x5410); v[1] = __byte_perm(y.x, y.z, 0x7632);
+				v[2] = __byte_perm(y.y, y.w, 0x5410); v[3] = __byte_perm(y.y, y.w, 0x7632);
+			} else {
+				const uint2 y = *reinterpret_cast<const uint2*>(from + KT * KG * 16 + j * 32 + c * 8);
+				v[0] = __byte_perm(y.x, y.y, 0x5410); v[1] = __byte_perm(y.x, y.y, 0x7632);
+			}
+#pragma unroll
+			for (int g = 0; g < VG; g++) {
+				__half2 h[4];
+				numbers<false>(v[g], h);
+				asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to_v + (((g * 4 + c) ^ (j & 7)) * 16)), "r"(bits(h[0])), "r"(bits(h[1])), "r"(bits(h[2])), "r"(bits(h[3])) : "memory");
+			}
+			if (warp == GW - 1) { // values' scales, two keys to a lane
+				const uint8_t* s = from + KT * (KG + VG) * 16 + KT * KG * 2 + lane * (VG * 4);
+				uint32_t e[2][VG / 2];
+#pragma unroll
+				for (int y = 0; y < 2; y++)
+#pragma unroll
+					for (int z = 0; z < VG / 2; z++) e[y][z] = *reinterpret_cast<const uint32_t*>(s + y * (VG * 2) + z * 4);
+				float top[2];
+#pragma unroll
+				for (int y = 0; y < 2; y++) {
+					__half2 m = __habs2(halves(e[y][0]));
+#pragma unroll
+					for (int z = 1; z < VG / 2; z++) m = __hmax2(m, __habs2(halves(e[y][z])));
+					top[y] = fmaxf(__low2float(m), __high2float(m)); // NaN counts for nothing
+				}
+#pragma unroll
+				for (int g = 0; g < VG; g++)
+					*reinterpret_cast<uint32_t*>(s_sc + b * Z::SC + (lane * VG + g) * 4) = __byte_perm(e[0][g / 2], e[1][g / 2], g & 1 ? 0x7632 : 0x5410);
+				*reinterpret_cast<float2*>(s_top + b * KT + lane * 2) = make_float2(top[0], top[1]);
+				const float all = warp_max(fmaxf(fmaxf(top[0], top[1]), 0.f));
+				if (lane == 0) s_most[b] = all;
+			}
+		};
+		copy(0);
+		copy(1);
+		copy(2);
+		// ---- queries as A: rows lane / 4 and 8 behind it; entries in the order of the keys' ----
+		uint32_t q[KG * 2][4];
+		float fac[2], m[2], l[2], lift[2], room[2]; // m: the maximum less lift; p is 2^lift times as large, as the largest scale that the row has seen allows
+		int lim[2];
+		const int r0 = warp * 16 + u;
+#pragma unroll
+		for (int half = 0; half < 2; half++) {
+			const int r = r0 + half * 8, w = x.t * GM + r;
+			const bool there = r < rows;
+			const long long at = there ? (long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d : 0;
+			float y[KG * 4][2], top = 0.f; // entries t and t + 4 of every eight
+#pragma unroll
+			for (int c = 0; c < KG * 4; c++)
+#pragma unroll
+				for (int e = 0; e < 2; e++) {
+					const long long i = at + c * 8 + t + e * 4;
+					y[c][e] = there && c * 8 < a.c.d ? (type == XALM_F16 ? __half2float(reinterpret_cast<const __half*>(a.q)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q)[i])) : 0.f;
+					top = fmaxf(top, fabsf(y[c][e]));
+				}
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
+			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
+			const float f = two_to(e);
+			fac[half] = fminf(fmaxf(a.scale * 1.4426950408889634f * two_to(-e) * 8.f, -3.0e38f), 3.0e38f);
+#pragma unroll
+			for (int c = 0; c < KG * 4; c++) q[c / 2][half + (c & 1) * 2] = pack2(y[c][0] * f, y[c][1] * f);
+			m[half] = -3.0e38f;
+			l[half] = 0.f;
+			lift[half] = 13.f;
+			room[half] = 0.f;
+		}
+		float acc[VG * 4][4];
+#pragma unroll
+		for (int c = 0; c < VG * 4; c++)
+#pragma unroll
+			for (int e = 0; e < 4; e++) acc[c][e] = 0.f;
+		asm volatile("cp.async.wait_group 2;" ::: "memory");
+		__syncthreads();
+		lim[0] = s_lim[r0];
+		lim[1] = s_lim[r0 + 8];
+		const int least = s_lim[warp * 16], most = warp * 16 < rows ? s_lim[min(warp * 16 + 15, rows - 1)] : 0; // of this warp's rows
+		if (n_tiles) convert(0);
+		asm volatile("cp.async.wait_group 1;" ::: "memory");
+		__syncthreads();
+		auto compute = [&](int i, auto edge) {
+			constexpr bool EDGE = decltype(edge)::value;
+			const int b = i & 1, at = first + i * KT;
+			// ---- scores ----
+			float s[KT / 8][4];
+#pragma unroll
+			for (int n = 0; n < KT / 8; n++) {
+				s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+				const uint32_t row = kh + b * Z::KH + (n * 8 + (lane & 7)) * (KG * 64);
+#pragma unroll
+				for (int c = 0; c < KG; c++) {
+					uint32_t r[4];
+					matrices(row + (((c * 4 + (lane >> 3)) ^ (lane & 7)) * 16), r);
+					mma16(s[n], q[c * 2][0], q[c * 2][1], q[c * 2][2], q[c * 2][3], r[0], r[1]);
+					mma16(s[n], q[c * 2 + 1][0], q[c * 2 + 1][1], q[c * 2 + 1][2], q[c * 2 + 1][3], r[2], r[3]);
+				}
+			}
+			// ---- the largest scale that a row has seen ----
+			float top[2];
+			top[0] = top[1] = s_most[b];
+			if constexpr (EDGE) {
+				top[0] = top[1] = 0.f;
+#pragma unroll
+				for (int n = 0; n < KT / 8; n++) {
+					const float2 y = *reinterpret_cast<const float2*>(s_top + b * KT + n * 8 + t * 2);
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						if (at + n * 8 + t * 2 < lim[h]) top[h] = fmaxf(top[h], y.x);
+						if (at + n * 8 + t * 2 + 1 < lim[h]) top[h] = fmaxf(top[h], y.y);
+					}
+				}
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+					top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+				}
+			}
+			if (__any_sync(0xffffffffu, top[0] > room[0] || top[1] > room[1])) {
+#pragma unroll
+				for (int h = 0; h < 2; h++)
+					if (top[h] > room[h]) {
+						const int e = (__float_as_int(top[h]) >> 23) - 127; // 2^e <= top < 2^(e + 1): scales up to twice that have room
+						const float to = fminf(fmaxf((float) (11 - e), -4.f), 13.f), f = exp2f(to - lift[h]);
+						room[h] = two_to(min(e + 2, 127));
+						l[h] *= f;
+						m[h] += lift[h] - to;
+						lift[h] = to;
+#pragma unroll
+						for (int c = 0; c < VG * 4; c++) { acc[c][h * 2] *= f; acc[c][h * 2 + 1] *= f; }
+					}
+			}
+			// ---- probabilities ----
+			float big[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+			for (int n = 0; n < KT / 8; n++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) {
+					s[n][e] *= fac[e >> 1];
+					if (EDGE && at + n * 8 + t * 2 + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
+					big[e >> 1] = fmaxf(big[e >> 1], s[n][e]);
+				}
+			if (__any_sync(0xffffffffu, big[0] - m[0] > 2.f + lift[0] || big[1] - m[1] > 2.f + lift[1])) { // rare behind the first keys: probabilities may be up to 4
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					float y = big[h];
+					y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+					y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+					y = fmaxf(m[h], y - lift[h]);
+					const float f = exp2f(m[h] - y);
+					m[h] = y;
+					l[h] *= f;
+#pragma unroll
+					for (int c = 0; c < VG * 4; c++) { acc[c][h * 2] *= f; acc[c][h * 2 + 1] *= f; }
+				}
+			}
+			uint32_t p[KT / 8][2];
+#pragma unroll
+			for (int n = 0; n < KT / 8; n++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const float z0 = ex2(at_most(s[n][h * 2] - m[h], 2.f + lift[h])), z1 = ex2(at_most(s[n][h * 2 + 1] - m[h], 2.f + lift[h]));
+					l[h] += z0 + z1;
+					p[n][h] = pack2(z0, z1);
+				}
+			// ---- sums ----
+#pragma unroll
+			for (int kk = 0; kk < KT / 16; kk++) {
+				uint32_t lo[VG], hi[VG]; // scales of keys 2 t, 2 t + 1 and 8 behind them
+#pragma unroll
+				for (int g = 0; g < VG; g += 2) {
+					const uint2 y = *reinterpret_cast<const uint2*>(s_sc + b * Z::SC + ((kk * 8 + t) * VG + g) * 4), z = *reinterpret_cast<const uint2*>(s_sc + b * Z::SC + ((kk * 8 + 4 + t) * VG + g) * 4);
+					lo[g] = y.x; lo[g + 1] = y.y;
+					hi[g] = z.x; hi[g + 1] = z.y;
+				}
+				uint32_t seen[4];
+				if constexpr (EDGE) {
+#pragma unroll
+					for (int e = 0; e < 4; e++) { // as the product's parts: rows u, u + 8 of the first eight keys, of the second
+						const int key = at + kk * 16 + (e >> 1) * 8 + t * 2;
+						seen[e] = (key < lim[e & 1] ? 0xffffu : 0u) | (key + 1 < lim[e & 1] ? 0xffff0000u : 0u);
+					}
+				}
+				const uint32_t row = vh + b * Z::VH + (kk * 16 + (lane & 15)) * (VG * 64);
+#pragma unroll
+				for (int g = 0; g < VG; g++) {
+					uint32_t f[4] = {bits(__hmul2(halves(p[kk * 2][0]), halves(lo[g]))), bits(__hmul2(halves(p[kk * 2][1]), halves(lo[g]))), bits(__hmul2(halves(p[kk * 2 + 1][0]), halves(hi[g]))),
+					                 bits(__hmul2(halves(p[kk * 2 + 1][1]), halves(hi[g])))};
+					if constexpr (EDGE)
+#pragma unroll
+						for (int e = 0; e < 4; e++) f[e] &= seen[e];
+#pragma unroll
+					for (int c = 0; c < 4; c += 2) {
+						uint32_t r[4];
+						matrices_turned(row + (((g * 4 + c + (lane >> 4)) ^ (lane & 7)) * 16), r);
+						mma16(acc[g * 4 + c], f[0], f[1], f[2], f[3], r[0], r[1]);
+						mma16(acc[g * 4 + c + 1], f[0], f[1], f[2], f[3], r[2], r[3]);
+					}
+				}
+			}
+		};
+		for (int i = 0; i < n_tiles; i++) {
+			copy(i + RING);
+			if (i + 1 < n_tiles) convert(i + 1);
+			const int at = first + i * KT;
+			if (at + KT <= least) compute(i, std::false_type());
+			else if (at < most) compute(i, std::true_type());
+			asm volatile("cp.async.wait_group 1;" ::: "memory");
+			__syncthreads();
+		}
+		asm volatile("cp.async.wait_group 0;" ::: "memory");
+		// ---- results: two neighbouring entries to a lane, which its neighbour has one of ----
+		const bool direct = x.j0 == 0 && x.j1 == x.w && !prefix && shared == 0;
+		const long long slot = piece_slot(a, x.u, blockIdx.x, x.j0 == 0);
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			float sum = l[h];
+			sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+			sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+			const int r = r0 + h * 8, w = x.t * GM + r;
+			const bool any = sum > 0.f || sum != sum, there = r < rows;
+			const float f = direct ? any ? 1.f / sum : 0.f : 1.f;
+			const long long tok = x.row0 + w / a.rep;
+			const int hd = h0 + w % a.rep;
+			if (there && t == 0) {
+				const float top = m[h] == -3.0e38f ? -INFINITY : m[h];
+				if (!direct) {
+					if (slot < part.slots) part.ml[slot * GM + r] = make_float2(top, sum);
+				} else if (a.lse) a.lse[tok * a.H + hd] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+			}
+#pragma unroll
+			for (int c = 0; c < VG * 4; c++) {
+				const float y0 = acc[c][h * 2] * f, y1 = acc[c][h * 2 + 1] * f, other = __shfl_xor_sync(0xffffffffu, t & 1 ? y0 : y1, 1);
+				const int col = c * 8 + (t & 1 ? t + 3 : t);
+				const float2 y = t & 1 ? make_float2(other, y1) : make_float2(y0, other);
+				if (!there || c * 8 >= dv) continue;
+				if (!direct) {
+					if (slot < part.slots) *reinterpret_cast<float2*>(part.o + (slot * GM + r) * dv + col) = y;
+				} else if (type == XALM_F16) *reinterpret_cast<uint32_t*>(reinterpret_cast<__half*>(a.out) + tok * a.out_row + hd * dv + col) = pack2(y.x, y.y);
+				else *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(a.out) + tok * a.out_row + hd * dv + col) = __floats2bfloat162_rn(y.x, y.y);
+			}
+		}
+	}
+	pdl_wait(); // not ahead of the kernel before it to the join
+}
+
+template <int KG, int VG>
+static int launch_tile(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
+	const size_t smem = Tile4<KG, VG>::own + plan_bytes(a.b.B, a.b.n_groups);
+	XALM_CUDA_CHECK(allow_smem((const void*) paged4_tile_kernel<KG, VG>));
+	XALM_CUDA_CHECK(launch(paged4_tile_kernel<KG, VG>, a.part[part].grid, GT, smem, s, part > 0, a, a.part[part], p, type));
+	return XALM_OK;
+}
+Shape4 tile4_shape(const Pool4& p) { return p.kg <= 4 && p.vg <= 4 ? Shape4{GM, 1} : Shape4{0, 0}; }
+int launch_attn4_tile(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
+	if (p.kg == 4) return p.vg == 4 ? launch_tile<4, 4>(a, p, part, type, s) : launch_tile<4, 2>(a, p, part, type, s);
+	return p.vg == 4 ? launch_tile<2, 4>(a, p, part, type, s) : launch_tile<2, 2>(a, p, part, type, s);
+}
+
+} // namespace paged
+} // namespace xalm
