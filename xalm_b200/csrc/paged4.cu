@@ -28,9 +28,26 @@ struct Append4Args {
 	int rot;
 	float mag;
 	int neighbours;
+	int paired;           // halves whose chunks of eight pair up: of queries a thread takes both
+	int per_head;         // work items of a head of q
+	unsigned by_head;     // 2^32 / that, rounded up (0 for one)
 };
 
 constexpr int A4T = 256;
+
+template <typename I>
+struct Chunk8 { // eight elements as they came
+	uint4 u[sizeof(I) == 4 ? 2 : 1];
+	__device__ __forceinline__ void load(const I* p) {
+#pragma unroll
+		for (int i = 0; i < (sizeof(I) == 4 ? 2 : 1); i++) u[i] = reinterpret_cast<const uint4*>(p)[i];
+	}
+	__device__ __forceinline__ void floats(float (&x)[8]) const {
+		const I* t = reinterpret_cast<const I*>(u);
+#pragma unroll
+		for (int i = 0; i < 8; i++) x[i] = to_f(t[i]);
+	}
+};
 
 // position of a row (-1: of no sequence, or before its first token) and the page of the pool that has it (-1: none); by a whole warp
 __device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int row, bool& in_seq) {
@@ -53,19 +70,37 @@ __device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int
 	return make_int2(pos, page);
 }
 
-// Eight entries from c on of the head at p (n entries), turned
+// Eight entries of a key from c on, turned in 64 bits: x, and what they are turned with where that is eight neighbours too (PAIRED)
 template <typename I>
-__device__ __forceinline__ void turned8(const I* p, int c, const Append4Args& a, const double* cs, const double* sn, float (&x)[8]) {
-	load8(p + c, x);
+__device__ __forceinline__ void turn_key(const I* head, int c, const Append4Args& a, const double* cs, const double* sn, float (&x)[8], const float (&other)[8]) {
 	if (c >= 2 * a.rot) return;
+	if (a.paired) {
+		const bool second = c >= a.rot;
+		const int f = second ? c - a.rot : c;
 #pragma unroll
-	for (int e = 0; e < 8; e++) {
-		const int i = c + e;
-		if (i >= 2 * a.rot) continue;
-		const bool second = a.neighbours ? i & 1 : i >= a.rot;
-		const int f = a.neighbours ? i >> 1 : second ? i - a.rot : i;
-		const double o = (double) to_f(p[a.neighbours ? i ^ 1 : second ? f : i + a.rot]), y = (double) to_f(p[i]);
-		x[e] = (float) ((second ? y * cs[f] + o * sn[f] : y * cs[f] - o * sn[f]) * (double) a.mag);
+		for (int e = 0; e < 8; e++) {
+			const double y = (double) x[e] * cs[f + e], z = (double) other[e] * sn[f + e];
+			x[e] = (float) ((second ? y + z : y - z) * (double) a.mag);
+		}
+	} else if (a.neighbours) {
+#pragma unroll
+		for (int e = 0; e < 8; e += 2) {
+			const int f = (c + e) >> 1;
+			if (f < a.rot) {
+				const double y = (double) x[e], z = (double) x[e + 1];
+				x[e] = (float) ((y * cs[f] - z * sn[f]) * (double) a.mag);
+				x[e + 1] = (float) ((z * cs[f] + y * sn[f]) * (double) a.mag);
+			}
+		}
+	} else { // halves that end inside a chunk
+#pragma unroll
+		for (int e = 0; e < 8; e++) {
+			const int i = c + e;
+			if (i >= 2 * a.rot) continue;
+			const int f = i < a.rot ? i : i - a.rot;
+			const double y = (double) x[e] * cs[f], z = (double) to_f(head[i < a.rot ? i + a.rot : f]) * sn[f];
+			x[e] = (float) ((i < a.rot ? y - z : y + z) * (double) a.mag);
+		}
 	}
 }
 
@@ -100,7 +135,7 @@ __device__ __forceinline__ uint32_t block4(const float (&x)[8], unsigned quad, _
 template <typename I, int R>
 __global__ void __launch_bounds__(A4T) paged4_append_kernel(const __grid_constant__ Append4Args a) {
 	__shared__ double s_cos[R][128], s_sin[R][128];
-	__shared__ int s_pos[R], s_page[R];
+	__shared__ int s_pos[R], s_page[R]; // position (-1: of no sequence, or before its first token), page of the pool (-1: none)
 	const int row0 = blockIdx.x * R, tid = threadIdx.x, warp = tid >> 5, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
 	if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, A4T);
 	if (warp < R) {
@@ -112,32 +147,78 @@ __global__ void __launch_bounds__(A4T) paged4_append_kernel(const __grid_constan
 	for (int i = tid; i < R * a.rot; i += A4T) {
 		const int r = i / a.rot, f = i - r * a.rot;
 		if (s_pos[r] < 0) continue;
-		sincos((double) s_pos[r] * (double) a.freq[f], &s_sin[r][f], &s_cos[r][f]);
+		const double x = (double) s_pos[r] * (double) a.freq[f], turns = rint(x * 0.15915494309189535); // the product is exact, and 2 pi the sum of two doubles
+		sincos(fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x)), &s_sin[r][f], &s_cos[r][f]);
 	}
 	__syncthreads();
-	const int per_q = d / 8, n_q = a.q ? a.H * per_q : 0, n_k = G * KG * 4, n_v = G * VG * 4, slot_mask = (1 << shift) - 1;
+	bool in[R], kept[R];
+#pragma unroll
 	for (int r = 0; r < R; r++) {
-		if (s_pos[r] < 0) continue;
-		const long long row = row0 + r;
-		for (int i = tid; i < n_q; i += A4T) {
-			const int h = i / per_q, c = (i - h * per_q) * 8;
-			float x[8];
-			turned8(reinterpret_cast<const I*>(a.q) + row * a.q_row + h * d, c, a, s_cos[r], s_sin[r], x);
-			store8(reinterpret_cast<I*>(a.q_out) + row * a.q_out_row + h * d + c, x);
+		in[r] = s_pos[r] >= 0;
+		kept[r] = in[r] && s_page[r] >= 0;
+	}
+	const int n_q = a.q ? a.H * a.per_head : 0, n_k = G * KG * 4, n_v = G * VG * 4, slot_mask = (1 << shift) - 1;
+	for (int i = tid; i < n_q; i += A4T) { // queries, in fp32
+		const int h = a.per_head == 1 ? i : (int) __umulhi((unsigned) i, a.by_head), u = i - h * a.per_head;
+		const bool pair = a.paired && u * 8 < a.rot;
+		const int c = !a.paired || pair ? u * 8 : u * 8 + a.rot; // the item's first entry; behind the pairs come the chunks that are not turned
+		const I* from = reinterpret_cast<const I*>(a.q) + h * d + c;
+		Chunk8<I> x[R], y[R];
+#pragma unroll
+		for (int r = 0; r < R; r++)
+			if (in[r]) {
+				x[r].load(from + (row0 + r) * a.q_row);
+				if (pair) y[r].load(from + (row0 + r) * a.q_row + a.rot);
+			}
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			if (!in[r]) continue;
+			float lo[8], hi[8];
+			x[r].floats(lo);
+			I* to = reinterpret_cast<I*>(a.q_out) + (row0 + r) * a.q_out_row + h * d + c;
+			if (pair) {
+				y[r].floats(hi);
+#pragma unroll
+				for (int e = 0; e < 8; e++) {
+					const float cs = (float) s_cos[r][c + e] * a.mag, sn = (float) s_sin[r][c + e] * a.mag, l = lo[e];
+					lo[e] = l * cs - hi[e] * sn;
+					hi[e] = hi[e] * cs + l * sn;
+				}
+				store8(to + a.rot, hi);
+			} else if (!a.paired) turn_key(from - c + (row0 + r) * a.q_row, c, a, s_cos[r], s_sin[r], lo, lo);
+			store8(to, lo);
 		}
-		if (s_page[r] < 0) continue;
-		const int slot = s_pos[r] & slot_mask;
-		uint8_t* page = a.pool.at + s_page[r] * a.pool.page;
-		for (int i = tid; i < n_k + n_v; i += A4T) {
-			const bool value = i >= n_k;
-			const int j = value ? i - n_k : i, per = (value ? VG : KG) * 4, h = j / per, chunk = j - h * per, g = chunk >> 2, t = chunk & 3, c = chunk * 8;
-			float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-			if (value) {
-				if (c < dv) load8(reinterpret_cast<const I*>(a.v) + row * a.v_row + h * dv + c, x);
-			} else if (c < d) turned8(reinterpret_cast<const I*>(a.k) + row * a.k_row + h * d, c, a, s_cos[r], s_sin[r], x);
+	}
+	for (int i = tid; i < n_k + n_v; i += A4T) {
+		const bool value = i >= n_k;
+		const int j = value ? i - n_k : i, by = value ? VG == 2 ? 3 : VG == 4 ? 4 : 5 : KG == 2 ? 3 : KG == 4 ? 4 : 5; // chunks of eight to a head: 8, 16 or 32
+		const int h = j >> by, chunk = j - (h << by), g = chunk >> 2, t = chunk & 3, c = chunk * 8;
+		const bool there = c < (value ? dv : d), pair = there && !value && a.paired && c < 2 * a.rot;
+		const I* from = value ? reinterpret_cast<const I*>(a.v) + h * dv + c : reinterpret_cast<const I*>(a.k) + h * d + c;
+		const long long step = value ? a.v_row : a.k_row;
+		Chunk8<I> x[R], y[R];
+#pragma unroll
+		for (int r = 0; r < R; r++)
+			if (kept[r] && there) {
+				x[r].load(from + (row0 + r) * step);
+				if (pair) y[r].load(from + (row0 + r) * step + (c < a.rot ? a.rot : -a.rot));
+			}
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			if (!kept[r]) continue; // the same for the whole CTA
+			float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+			if (there) {
+				x[r].floats(z);
+				if (!value) {
+					float o[8];
+					if (pair) y[r].floats(o);
+					turn_key(from - c + (row0 + r) * step, c, a, s_cos[r], s_sin[r], z, o);
+				}
+			}
 			__half scale;
-			const uint32_t w = block4(x, 0xfu << (tid & 28), scale);
-			uint8_t* run = page + h * a.pool.head;
+			const uint32_t w = block4(z, 0xfu << (tid & 28), scale);
+			const int slot = s_pos[r] & slot_mask;
+			uint8_t* run = a.pool.at + s_page[r] * a.pool.page + h * a.pool.head;
 			if (value) {
 				uint8_t* at = run + values_at(KG, shift) + slot * (VG * 16) + g * 2;
 				*reinterpret_cast<uint16_t*>(at + (2 * t) * (VG * 2)) = (uint16_t) w;
@@ -225,8 +306,9 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 }
 
 // What a piece costs beside its tiles, in tiles
-constexpr int LEAD4 = 6, LEAD4_MANY = 6, LEAD4_F32 = 6, LEAD4_TILE = 4;
-constexpr int TILE_ROWS = 32; // rows of a segment that the kernel of many rows is not for
+constexpr int LEAD4 = 6, LEAD4_F32 = 6, LEAD4_TILE = 4;
+// Segments of more rows are the kernel's of many: 32 sequences behind 4096 tokens take 63 us (bf16) and 75 (fp16) for every 16 rows to a kv head, 245 for up to 128
+constexpr int TILE_ROWS = 56;
 constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
 
 static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, int (&kinds)[2]) {
@@ -239,18 +321,12 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 	a.b = b;
 	a.H = heads;
 	a.rep = heads / c.G;
-	// The kernel of most segments by the rows that one has on average, and where some may have more than TILE_ROWS, the one of many rows for those
+	// One kernel for segments of few rows, by the rows that one has on average, and where some may have more than TILE_ROWS, the one of many rows for those
 	const long long rows_all = (long long) b.N * a.rep, each = (rows_all + b.B - 1) / std::max(b.B, 1);
-	const bool tile = type != XALM_F32 && tile4_shape(p).rows && (b.n_groups || b.N > b.B || a.rep > TILE_ROWS) && rows_all > TILE_ROWS;
-	const int size = each <= 4 ? 4 : each <= 8 ? 8 : each <= 16 || (tile && each > TILE_ROWS) ? 16 : 32; // rows of a unit
-	const int few16 = type == XALM_F16 ? size == 4 ? H4 : size < 32 ? H16 : H32 : size <= 8 ? B8 : size == 16 ? B16 : B32;
-	const int few_kind = type == XALM_F32 ? size == 4 ? F4 : F16 : attn4_shape(p, b, few16).rows ? few16 : type == XALM_F16 ? H16 : B16;
-	const Shape4 few = attn4_shape(p, b, few_kind);
-	const int more_kind = tile ? TILE : type == XALM_F16 ? H32 : B32;
-	const Shape4 more = tile ? tile4_shape(p) : attn4_shape(p, b, more_kind);
-	const int limit = tile ? TILE_ROWS : few.rows; // rows of a segment above which it is the second kernel's
-	const bool many = type != XALM_F32 && more.rows > few.rows && (b.n_groups || b.N > b.B || a.rep > limit) && rows_all > limit;
-	kinds[0] = many ? more_kind : few_kind;
+	const int few_kind = type == XALM_F32 ? each <= 4 ? F4 : F16 : type == XALM_F16 ? each <= 4 ? H4 : H16 : each <= 8 ? B8 : B16;
+	const Shape4 few = attn4_shape(p, b, few_kind), more = tile4_shape(p);
+	const bool many = type != XALM_F32 && more.rows && (b.n_groups || b.N > b.B || a.rep > TILE_ROWS) && rows_all > TILE_ROWS;
+	kinds[0] = many ? TILE : few_kind;
 	kinds[1] = few_kind;
 	a.n_parts = many ? 2 : 1;
 	size_t at = 0;
@@ -260,11 +336,11 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 		const bool big = many && i == 0;
 		t.M = big ? more.rows : few.rows;
 		t.grid = sms * (big ? more.per_sm : few.per_sm);
-		t.lead = big ? tile ? LEAD4_TILE : LEAD4_MANY : type == XALM_F32 ? LEAD4_F32 : LEAD4;
-		t.least_rows = big ? limit + 1 : 1;
-		t.most_rows = many && !big ? limit : 0x7fffffff;
-		// as in plan_attn: a segment has at most its rows / M + 1 tiles, in a part that takes short ones only it has one
-		const long long rows = rows_all, whole = many && !big && limit <= t.M ? 0 : rows / t.M, most = rows / t.least_rows;
+		t.lead = big ? LEAD4_TILE : type == XALM_F32 ? LEAD4_F32 : LEAD4;
+		t.least_rows = big ? TILE_ROWS + 1 : 1;
+		t.most_rows = many && !big ? TILE_ROWS : 0x7fffffff;
+		// a segment has at most its rows / M + 1 tiles, and there are no more segments than have room for the part's least rows, of sequences as of groups
+		const long long rows = rows_all, whole = rows / t.M, most = rows / t.least_rows;
 		const long long tiles = whole + std::min((long long) b.B, most) + (b.n_groups ? whole + std::min((long long) b.n_groups, most) : 0);
 		if (tiles * c.G + t.grid > 0x7fffffff / t.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
 		const long long work = ((long long) b.max_pages << c.shift) / KT + 1;
@@ -325,6 +401,9 @@ int xalm_cuda_paged4_append(const xalm_paged4_cache* cache, const xalm_paged_bat
 	a.q_out = (uint8_t*) q_out;
 	a.H = heads;
 	a.freq = freq; a.rot = rot_half; a.mag = rot_mag; a.neighbours = neighbours;
+	a.paired = !neighbours && rot_half % 8 == 0;
+	a.per_head = (a.c.d - (a.paired ? rot_half : 0)) / 8;
+	a.by_head = (unsigned) ((0x100000000ull + a.per_head - 1) / a.per_head);
 	int sms = 0;
 	XALM_TRY(sm_count(cache->device, &sms));
 	const bool several = a.b.N >= sms * 4;

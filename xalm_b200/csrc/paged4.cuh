@@ -23,9 +23,9 @@ __host__ __device__ __forceinline__ int value_scales_at(int kg, int vg, int shif
 __host__ __device__ __forceinline__ int run_bytes(int kg, int vg, int shift) { return ((kg + vg) * 18) << shift; }
 
 // Kernels by the type of the queries (bf16, fp16, fp32) and the (token, head) rows of a unit
-enum Kind4 { B8, B16, B32, H4, H16, H32, F4, F16, TILE };
+enum Kind4 { B8, B16, H4, H16, F4, F16, TILE };
 struct Shape4 {
-	int rows, per_sm; // rows of a unit (0: there is none for such heads), CTAs to an SM
+	int rows, per_sm; // rows of a unit (0: none for such heads), CTAs to an SM
 };
 Shape4 attn4_shape(const Pool4& p, const BatchView& b, int kind);
 int launch_attn4(const Attn& a, const Pool4& p, int part, int type, int kind, cudaStream_t s);

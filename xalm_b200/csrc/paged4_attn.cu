@@ -17,8 +17,8 @@ constexpr int FP = 20;                              // floats between the probab
 // columns has four rows; fp32 queries enter the first product so too).
 template <int KG, int VG, int KIND>
 struct Size4 {
-	static constexpr bool WIDE = KIND == F4 || KIND == F16, SPLIT = WIDE || KIND == H4, TWO = KIND == H16 || KIND == H32;
-	static constexpr int NT = KIND == B16 || KIND == H16 ? 2 : KIND == B32 || KIND == H32 ? (VG == 8 ? 0 : 4) : KIND == F16 ? (VG == 8 ? 2 : 4) : 1; // tiles of 8 columns; 0: more than registers hold
+	static constexpr bool WIDE = KIND == F4 || KIND == F16, SPLIT = WIDE || KIND == H4, TWO = KIND == H16;
+	static constexpr int NT = KIND == B16 || KIND == H16 ? 2 : KIND == F16 ? (VG == 8 ? 2 : 4) : 1; // tiles of 8 columns
 	static constexpr int M = SPLIT ? NT * 4 : NT * 8;                                                     // rows of a unit
 	static constexpr int CTAS = NT == 1 ? (VG == 8 || KG == 8 ? 3 : 4) : NT == 2 && VG < 8 ? 3 : 2;       // to an SM, as registers allow
 	static constexpr int OP = VG * 32 + 4;                                            // floats between rows of sums
@@ -105,7 +105,9 @@ struct Values {
 };
 
 constexpr float NONE = -3.0e38f; // the maximum before the first key
-__device__ __forceinline__ float less(float x) { return x > 2.f ? 2.f : x; } // a NaN stays one
+// s f - m: in one step where that is off by less than 2^-6 from the rounded product, which m is one of; else in two, so that the largest score is 0 above itself
+constexpr float COARSE = 262144.f;
+__device__ __forceinline__ float above(float s, float f, float m, bool coarse) { return coarse ? __fsub_rn(__fmul_rn(s, f), m) : fmaf(s, f, -m); }
 
 // A piece by one warp: its 16 keys of each tile, the unit's rows as columns of the products
 template <typename Z, int KG, int VG>
@@ -158,6 +160,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 		if ((KG + VG) * 2 == 32 || lane < (KG + VG) * 2) copy16(to_k + to + KS, run + (s_at + slot * s_by), there);
 		asm volatile("cp.async.commit_group;" ::: "memory");
 	};
+	bool coarse = false;
 	int id = id_at(at), full = 0, free = (STAGES - 1) * STAGE; // the stage to be read, and the one to be filled
 #pragma unroll
 	for (int i = 0; i < STAGES - 1; i++) {
@@ -217,7 +220,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 				for (int e = 0; e < 4; e++) s[n][e] += __shfl_xor_sync(0xffffffffu, s[n][e], 2);
 #pragma unroll
-			for (int e = 0; e < 4; e++) p[n][e] = fmaf(s[n][e], e & 1 ? fac[n].y : fac[n].x, -m[n][e & 1]);
+			for (int e = 0; e < 4; e++) p[n][e] = above(s[n][e], e & 1 ? fac[n].y : fac[n].x, m[n][e & 1], coarse);
 			if constexpr (EDGE) {
 				const int2 lim = *reinterpret_cast<const int2*>(s_lim + n * 8 + t * 2);
 #pragma unroll
@@ -232,7 +235,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
 					const float f0 = c ? fac[n].y : fac[n].x;
-					float top = fmaxf(p[n][c] == -INFINITY ? NONE : s[n][c] * f0, p[n][c + 2] == -INFINITY ? NONE : s[n][c + 2] * f0);
+					float top = fmaxf(p[n][c] == -INFINITY ? NONE : __fmul_rn(s[n][c], f0), p[n][c + 2] == -INFINITY ? NONE : __fmul_rn(s[n][c + 2], f0));
 #pragma unroll
 					for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 					top = fmaxf(m[n][c], top);
@@ -241,9 +244,14 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 					l[n][c] *= f;
 #pragma unroll
 					for (int i = 0; i < VG * 2; i++) { acc[i][n][c] *= f; acc[i][n][c + 2] *= f; }
-					if (p[n][c] != -INFINITY) p[n][c] = less(fmaf(s[n][c], f0, -top)); // scores of 2^24 and more are rounded by whole numbers
-					if (p[n][c + 2] != -INFINITY) p[n][c + 2] = less(fmaf(s[n][c + 2], f0, -top));
+					coarse = coarse || (fabsf(top) > COARSE && top != NONE);
 				}
+			coarse = __any_sync(0xffffffffu, coarse);
+#pragma unroll
+			for (int n = 0; n < NT; n++)
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					if (p[n][e] != -INFINITY) p[n][e] = above(s[n][e], e & 1 ? fac[n].y : fac[n].x, m[n][e & 1], coarse);
 		}
 		__syncwarp();
 #pragma unroll
@@ -476,7 +484,6 @@ __global__ void __launch_bounds__(FT, Size4<KG, VG, KIND>::CTAS) paged4_attn_ker
 template <int KG, int VG, int KIND>
 static Shape4 shape_of(const BatchView& b) {
 	using Z = Size4<KG, VG, KIND>;
-	if (Z::NT == 0) return Shape4{0, 0};
 	const size_t smem = Z::own + plan_bytes(b.B, b.n_groups);
 	return Shape4{Z::M, std::max(1, std::min(Z::CTAS, (int) (226 * 1024 / (smem + 1024))))};
 }
@@ -490,17 +497,14 @@ static Shape4 shape4(const Pool4& p, const BatchView& b) {
 	return Shape4{0, 0};
 }
 Shape4 attn4_shape(const Pool4& p, const BatchView& b, int kind) {
-	return kind == B8 ? shape4<B8>(p, b) : kind == B16 ? shape4<B16>(p, b) : kind == B32 ? shape4<B32>(p, b) : kind == H4 ? shape4<H4>(p, b) : kind == H16 ? shape4<H16>(p, b) : kind == H32 ? shape4<H32>(p, b)
-	       : kind == F4 ? shape4<F4>(p, b) : shape4<F16>(p, b);
+	return kind == B8 ? shape4<B8>(p, b) : kind == B16 ? shape4<B16>(p, b) : kind == H4 ? shape4<H4>(p, b) : kind == H16 ? shape4<H16>(p, b) : kind == F4 ? shape4<F4>(p, b) : shape4<F16>(p, b);
 }
 
 template <int KG, int VG, int KIND>
 static int launch_kind(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
-	if constexpr (Size4<KG, VG, KIND>::NT > 0) {
-		const size_t smem = Size4<KG, VG, KIND>::own + plan_bytes(a.b.B, a.b.n_groups);
-		XALM_CUDA_CHECK(allow_smem((const void*) paged4_attn_kernel<KG, VG, KIND>));
-		XALM_CUDA_CHECK(launch(paged4_attn_kernel<KG, VG, KIND>, a.part[part].grid, FT, smem, s, part > 0, a, a.part[part], p, type));
-	}
+	const size_t smem = Size4<KG, VG, KIND>::own + plan_bytes(a.b.B, a.b.n_groups);
+	XALM_CUDA_CHECK(allow_smem((const void*) paged4_attn_kernel<KG, VG, KIND>));
+	XALM_CUDA_CHECK(launch(paged4_attn_kernel<KG, VG, KIND>, a.part[part].grid, FT, smem, s, part > 0, a, a.part[part], p, type));
 	return XALM_OK;
 }
 template <int KIND>
@@ -516,10 +520,8 @@ int launch_attn4(const Attn& a, const Pool4& p, int part, int type, int kind, cu
 	switch (kind) {
 		case B8: return launch_blocks<B8>(a, p, part, type, s);
 		case B16: return launch_blocks<B16>(a, p, part, type, s);
-		case B32: return launch_blocks<B32>(a, p, part, type, s);
 		case H4: return launch_blocks<H4>(a, p, part, type, s);
 		case H16: return launch_blocks<H16>(a, p, part, type, s);
-		case H32: return launch_blocks<H32>(a, p, part, type, s);
 		case F4: return launch_blocks<F4>(a, p, part, type, s);
 		default: return launch_blocks<F16>(a, p, part, type, s);
 	}

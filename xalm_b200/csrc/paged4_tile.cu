@@ -49,12 +49,9 @@ __device__ __forceinline__ float ex2(float x) {
 	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
 	return y;
 }
-// a NaN stays one.  (Scores of 2^24 and more are rounded by whole numbers, and may pass the limit by some.)
-__device__ __forceinline__ float at_most(float x, float most) {
-	float y;
-	asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(most));
-	return y;
-}
+// s f - m: in one step where that is off by less than 2^-6 from the rounded product, which m is one of; else in two, so that the largest score is 0 above itself
+constexpr float COARSE = 262144.f;
+__device__ __forceinline__ float above(float s, float f, float m, bool coarse) { return coarse ? __fsub_rn(__fmul_rn(s, f), m) : fmaf(s, f, -m); }
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
 // A word's codes, c - 8 (EIGHTH: an eighth of that), in the order 0 4 1 5 2 6 3 7: 1024 + c and 1024 + 16 c as they lie, brought there without a rounding
 template <bool EIGHTH>
@@ -101,35 +98,43 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 		// ---- copies: 16 bytes of codes of a key and of a value to a thread, and of scales to some ----
 		const int* table = a.b.table + (long long) x.s * a.b.table_row;
 		const uint8_t* head = pool.at + x.g * pool.head;
-		auto run_of = [&](int at, bool& there) { // of key `at` of the segment
-			const int key = min(at, vis - 1), id = table[(x.key0 + key) >> shift];
-			const bool good = (unsigned) id < (unsigned) a.c.pages;
-			if (!good) report(a.c, ERR_PAGE); // reads as zeros
-			there = good && at < vis;
-			return head + (good ? id : 0) * pool.page;
-		};
+		constexpr int KC = KT * KG / 8, VC = KT * VG / 8; // 16 bytes of scales
+		// this thread's keys of a tile: of its 16 bytes of a key's codes, of a value's, of scales (16 bytes are several keys', all of one page)
+		const int j_k = tid / KG, j_v = tid / VG, j_s = tid < KC ? tid * (8 / KG) : (tid - KC) * (8 / VG);
+		auto id_at = [&](int i, int j) { return i < n_tiles ? table[(x.key0 + min(first + i * KT + j, vis - 1)) >> shift] : 0; };
+		int id_k = id_at(0, j_k & (KT - 1)), id_v = KG == VG ? 0 : id_at(0, j_v & (KT - 1)), id_s = id_at(0, j_s & (KT - 1)); // looked at a tile ahead
 		auto copy = [&](int i) {
 			if (i < n_tiles) {
 				const uint32_t to = raw + i % RING * Z::RAW;
 				const int at = first + i * KT;
+				auto run_of = [&](int j, int id, bool& there) {
+					const bool good = (unsigned) id < (unsigned) a.c.pages;
+					if (!good) report(a.c, ERR_PAGE); // reads as zeros
+					there = good && at + j < vis;
+					return head + (good ? id : 0) * pool.page;
+				};
 				bool there;
-				if (tid < KT * KG) { // 16 bytes c of key j at c ^ (j / 2 & 3) where a key has four: a quarter of a warp reads the same c of eight keys
-					const int j = tid / KG, c = tid % KG, slot = (x.key0 + at + j) & (P - 1);
-					const uint8_t* run = run_of(at + j, there);
+				if (KG == 4 || tid < KT * KG) { // 16 bytes c of key j at c ^ (j / 2 & 3) where a key has four: a quarter of a warp reads the same c of eight keys
+					const int j = j_k, c = tid % KG, slot = (x.key0 + at + j) & (P - 1);
+					const uint8_t* run = run_of(j, id_k, there);
 					copy16_if(to + j * (KG * 16) + (KG == 4 ? c ^ (j >> 1 & 3) : c) * 16, run + slot * (KG * 16) + c * 16, there);
+					if constexpr (KG == VG) copy16_if(to + KT * KG * 16 + j * (VG * 16) + (VG == 4 ? c ^ (j >> 1 & 3) : c) * 16, run + values_at(KG, shift) + slot * (VG * 16) + c * 16, there);
 				}
-				if (tid < KT * VG) {
-					const int j = tid / VG, c = tid % VG, slot = (x.key0 + at + j) & (P - 1);
-					const uint8_t* run = run_of(at + j, there);
-					copy16_if(to + KT * KG * 16 + j * (VG * 16) + (VG == 4 ? c ^ (j >> 1 & 3) : c) * 16, run + values_at(KG, shift) + slot * (VG * 16) + c * 16, there);
-				}
-				constexpr int KC = KT * KG / 8, VC = KT * VG / 8; // 16 bytes of scales
+				if constexpr (KG != VG)
+					if (VG == 4 || tid < KT * VG) {
+						const int j = j_v, c = tid % VG, slot = (x.key0 + at + j) & (P - 1);
+						const uint8_t* run = run_of(j, id_v, there);
+						copy16_if(to + KT * KG * 16 + j * (VG * 16) + (VG == 4 ? c ^ (j >> 1 & 3) : c) * 16, run + values_at(KG, shift) + slot * (VG * 16) + c * 16, there);
+					}
 				if (tid < KC + VC) {
 					const bool value = tid >= KC;
-					const int c = value ? tid - KC : tid, per = 8 / (value ? VG : KG), j = c * per, slot = (x.key0 + at + j) & (P - 1); // 16 bytes are `per` keys', all of one page
-					const uint8_t* run = run_of(at + j, there);
+					const int j = j_s, slot = (x.key0 + at + j) & (P - 1);
+					const uint8_t* run = run_of(j, id_s, there);
 					copy16_if(to + KT * (KG + VG) * 16 + tid * 16, run + (value ? value_scales_at(KG, VG, shift) + slot * (VG * 2) : key_scales_at(KG, shift) + slot * (KG * 2)), there);
 				}
+				id_k = id_at(i + 1, j_k & (KT - 1));
+				if constexpr (KG != VG) id_v = id_at(i + 1, j_v & (KT - 1));
+				if (tid < KC + VC) id_s = id_at(i + 1, j_s & (KT - 1));
 			}
 			asm volatile("cp.async.commit_group;" ::: "memory");
 		};
@@ -200,8 +205,9 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 		copy(2);
 		// ---- queries as A: rows lane / 4 and 8 behind it; entries in the order of the keys' ----
 		uint32_t q[KG * 2][4];
-		float fac[2], m[2], l[2], lift[2], room[2]; // m: the maximum less lift; p is 2^lift times as large, as the largest scale that the row has seen allows
+		float fac[2], m[2], l[2], lift[2], room[2]; // p is 2^lift times as large, as the largest scale that the row has seen allows
 		int lim[2];
+		bool coarse = false;
 		const int r0 = warp * 16 + u;
 #pragma unroll
 		for (int half = 0; half < 2; half++) {
@@ -221,8 +227,8 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
 			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
 			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
-			const float f = two_to(e);
-			fac[half] = fminf(fmaxf(a.scale * 1.4426950408889634f * two_to(-e) * 8.f, -3.0e38f), 3.0e38f);
+			const float f = a.scale < 0.f ? -two_to(e) : two_to(e); // a negative scale turns the queries' signs
+			fac[half] = fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f * two_to(-e) * 8.f, 1e-30f), 3.0e38f); // not 0: 0 times an infinity is no number
 #pragma unroll
 			for (int c = 0; c < KG * 4; c++) q[c / 2][half + (c & 1) * 2] = pack2(y[c][0] * f, y[c][1] * f);
 			m[half] = -3.0e38f;
@@ -249,17 +255,19 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			// ---- scores ----
 			float s[KT / 8][4];
 #pragma unroll
-			for (int n = 0; n < KT / 8; n++) {
-				s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-				const uint32_t row = kh + b * Z::KH + (n * 8 + (lane & 7)) * (KG * 64);
+			for (int n = 0; n < KT / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+			for (int n = 0; n < KT / 8; n += 4) // four chains at a time
 #pragma unroll
 				for (int c = 0; c < KG; c++) {
-					uint32_t r[4];
-					matrices(row + (((c * 4 + (lane >> 3)) ^ (lane & 7)) * 16), r);
-					mma16(s[n], q[c * 2][0], q[c * 2][1], q[c * 2][2], q[c * 2][3], r[0], r[1]);
-					mma16(s[n], q[c * 2 + 1][0], q[c * 2 + 1][1], q[c * 2 + 1][2], q[c * 2 + 1][3], r[2], r[3]);
+					uint32_t r[4][4];
+#pragma unroll
+					for (int i = 0; i < 4; i++) matrices(kh + b * Z::KH + ((n + i) * 8 + (lane & 7)) * (KG * 64) + (((c * 4 + (lane >> 3)) ^ (lane & 7)) * 16), r[i]);
+#pragma unroll
+					for (int i = 0; i < 4; i++) mma16(s[n + i], q[c * 2][0], q[c * 2][1], q[c * 2][2], q[c * 2][3], r[i][0], r[i][1]);
+#pragma unroll
+					for (int i = 0; i < 4; i++) mma16(s[n + i], q[c * 2 + 1][0], q[c * 2 + 1][1], q[c * 2 + 1][2], q[c * 2 + 1][3], r[i][2], r[i][3]);
 				}
-			}
 			// ---- the largest scale that a row has seen ----
 			float top[2];
 			top[0] = top[1] = s_most[b];
@@ -288,7 +296,6 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 						const float to = fminf(fmaxf((float) (11 - e), -4.f), 13.f), f = exp2f(to - lift[h]);
 						room[h] = two_to(min(e + 2, 127));
 						l[h] *= f;
-						m[h] += lift[h] - to;
 						lift[h] = to;
 #pragma unroll
 						for (int c = 0; c < VG * 4; c++) { acc[c][h * 2] *= f; acc[c][h * 2 + 1] *= f; }
@@ -300,30 +307,37 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			for (int n = 0; n < KT / 8; n++)
 #pragma unroll
 				for (int e = 0; e < 4; e++) {
-					s[n][e] *= fac[e >> 1];
 					if (EDGE && at + n * 8 + t * 2 + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
 					big[e >> 1] = fmaxf(big[e >> 1], s[n][e]);
 				}
-			if (__any_sync(0xffffffffu, big[0] - m[0] > 2.f + lift[0] || big[1] - m[1] > 2.f + lift[1])) { // rare behind the first keys: probabilities may be up to 4
+			if (__any_sync(0xffffffffu, above(big[0], fac[0], m[0], coarse) > 2.f || above(big[1], fac[1], m[1], coarse) > 2.f)) { // rare behind the first keys: probabilities may be up to 4
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
 					float y = big[h];
 					y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
 					y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-					y = fmaxf(m[h], y - lift[h]);
+					y = fmaxf(m[h], __fmul_rn(y, fac[h]));
+					coarse = coarse || (fabsf(y) > COARSE && y != -3.0e38f);
 					const float f = exp2f(m[h] - y);
 					m[h] = y;
 					l[h] *= f;
 #pragma unroll
 					for (int c = 0; c < VG * 4; c++) { acc[c][h * 2] *= f; acc[c][h * 2 + 1] *= f; }
 				}
+				coarse = __any_sync(0xffffffffu, coarse);
 			}
+			const float ml[2] = {m[0] - lift[0], m[1] - lift[1]};
+			if (coarse)
+#pragma unroll
+				for (int n = 0; n < KT / 8; n++)
+#pragma unroll
+					for (int e = 0; e < 4; e++) s[n][e] = __fsub_rn(__fmul_rn(s[n][e], fac[e >> 1]), m[e >> 1]) + lift[e >> 1];
 			uint32_t p[KT / 8][2];
 #pragma unroll
 			for (int n = 0; n < KT / 8; n++)
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
-					const float z0 = ex2(at_most(s[n][h * 2] - m[h], 2.f + lift[h])), z1 = ex2(at_most(s[n][h * 2 + 1] - m[h], 2.f + lift[h]));
+					const float z0 = ex2(coarse ? s[n][h * 2] : fmaf(s[n][h * 2], fac[h], -ml[h])), z1 = ex2(coarse ? s[n][h * 2 + 1] : fmaf(s[n][h * 2 + 1], fac[h], -ml[h]));
 					l[h] += z0 + z1;
 					p[n][h] = pack2(z0, z1);
 				}
@@ -365,10 +379,11 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 		};
 		for (int i = 0; i < n_tiles; i++) {
 			copy(i + RING);
-			if (i + 1 < n_tiles) convert(i + 1);
 			const int at = first + i * KT;
+			if (warp < GW / 2 && i + 1 < n_tiles) convert(i + 1); // the halves in turn: one's products beside the other's conversion
 			if (at + KT <= least) compute(i, std::false_type());
 			else if (at < most) compute(i, std::true_type());
+			if (warp >= GW / 2 && i + 1 < n_tiles) convert(i + 1);
 			asm volatile("cp.async.wait_group 1;" ::: "memory");
 			__syncthreads();
 		}
@@ -383,14 +398,14 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 			const int r = r0 + h * 8, w = x.t * GM + r;
 			const bool any = sum > 0.f || sum != sum, there = r < rows;
-			const float f = direct ? any ? 1.f / sum : 0.f : 1.f;
+			const float down = ex2(-lift[h]), f = direct ? any ? 1.f / sum : 0.f : down;
 			const long long tok = x.row0 + w / a.rep;
 			const int hd = h0 + w % a.rep;
 			if (there && t == 0) {
 				const float top = m[h] == -3.0e38f ? -INFINITY : m[h];
 				if (!direct) {
-					if (slot < part.slots) part.ml[slot * GM + r] = make_float2(top, sum);
-				} else if (a.lse) a.lse[tok * a.H + hd] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+					if (slot < part.slots) part.ml[slot * GM + r] = make_float2(top, sum * down);
+				} else if (a.lse) a.lse[tok * a.H + hd] = any ? (top - lift[h] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 			}
 #pragma unroll
 			for (int c = 0; c < VG * 4; c++) {
