@@ -117,7 +117,7 @@ def magnitudes(p, low, high):
     return torch.randn(*shape, p.d, generator=g) * size(), torch.randn(*shape, p.dv, generator=g) * size()
 
 
-@pytest.mark.parametrize("rep", [4, 8, 16, 30])
+@pytest.mark.parametrize("rep", [4, 8, 16, 30, 70])
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 def test_scales_of_all_sizes(type, rep):
     """Tokens whose scales differ by up to 2^12, the largest ones anywhere: the unit of the sums grows as they come."""
@@ -186,8 +186,8 @@ def test_queries_of_any_size(type):
 
 
 @pytest.mark.parametrize("rows", [1, 3])
-@pytest.mark.parametrize("rep", [1, 8, 16])
-@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("rep", [1, 8, 16, 70])
+@pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
 def test_scores_that_fp32_holds_to_a_few_units_give_finite_results(type, rep, rows):
     """Scores around 2^26, where neighbouring fp32 numbers are more than the running maximum's slack apart."""
     p = Problem4(type, [rows], [400], G=1, rep=rep, d=64, page=16, seed=65)
@@ -199,7 +199,27 @@ def test_scores_that_fp32_holds_to_a_few_units_give_finite_results(type, rep, ro
     assert (out.abs().double().cpu().amax() <= p.v.nan_to_num().abs().max() * 1.01)
 
 
-@pytest.mark.parametrize("rep", [4, 8, 16, 40])
+@pytest.mark.parametrize("rep", [1, 8, 16, 70])
+@pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
+def test_scores_too_large_for_fp32_to_tell_apart_count_alike(type, rep):
+    """All keys the same and scores around 2^30: the mean of the values, wherever the largest scale is among them."""
+    p = Problem4(type, [1], [500], G=1, rep=rep, d=64, page=16, seed=75)
+    g = torch.Generator().manual_seed(76)
+    size = torch.exp2(torch.randint(-6, 7, (p.pages, 1, 16, 1), generator=g).float())
+    p.fill(torch.full((p.pages, 1, 16, 64), -8.0), torch.randn(p.pages, 1, 16, 64, generator=g) * size)
+    p.q[:] = -(2.0 ** 10)
+    p.scale = 2.0 ** 11
+    cache, batch = p.on_gpu()
+    out, lse = paged.attend4(cache, batch, p.gq, p.scale, want_lse=True)
+    used = p.v.nan_to_num().flatten(0, 2)[~torch.isnan(p.v).flatten(0, 2).any(dim=1)]
+    want = used.mean(dim=0)
+    # equal probabilities: sums of 500 numbers in fp32, and of products of two fp16 roundings where there are many rows; then the type's own rounding
+    tol = want.abs() * HALF[type] + used.abs().mean(dim=0) * (2.0 ** -13 if type == "f32" else 2.0 ** -10)
+    near(out.double().cpu(), want.expand(1, rep, 64), tol.expand(1, rep, 64))
+    assert torch.allclose(lse.cpu(), torch.full_like(lse.cpu(), 64 * 8 * 2.0 ** 21), rtol=2 ** -20)
+
+
+@pytest.mark.parametrize("rep", [4, 8, 16, 40, 70])
 @pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
 def test_many_small_probabilities_beside_a_large_one(type, rep):
     """8192 keys e^-14 below the first, with values that add up beside its own: they count with all the bits that the result has."""

@@ -168,7 +168,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 		id = id_at(at + (i + 1) * KT);
 	}
 	auto step = [&](auto edge) {
-		constexpr bool EDGE = decltype(edge)::value; // some rows may not see some keys
+		constexpr bool EDGE = decltype(edge)::value; // some rows may not see some keys, or scores are large
 		asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
 		__syncwarp(); // the stage is there, and nobody reads the one before any more
 		bring(at + (STAGES - 1) * KT, id, free);
@@ -220,7 +220,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 				for (int e = 0; e < 4; e++) s[n][e] += __shfl_xor_sync(0xffffffffu, s[n][e], 2);
 #pragma unroll
-			for (int e = 0; e < 4; e++) p[n][e] = above(s[n][e], e & 1 ? fac[n].y : fac[n].x, m[n][e & 1], coarse);
+			for (int e = 0; e < 4; e++) p[n][e] = above(s[n][e], e & 1 ? fac[n].y : fac[n].x, m[n][e & 1], EDGE && coarse);
 			if constexpr (EDGE) {
 				const int2 lim = *reinterpret_cast<const int2*>(s_lim + n * 8 + t * 2);
 #pragma unroll
@@ -338,7 +338,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 			}
 		}
 	};
-	for (; at + FK <= least && at < end; at += KT) step(std::false_type());
+	for (; at + FK <= least && at < end && !coarse; at += KT) step(std::false_type());
 	for (; at < end; at += KT) step(std::true_type());
 	asm volatile("cp.async.wait_group 0;" ::: "memory");
 	__syncwarp(); // the sums take the stages' place

@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 		if (n_tiles) convert(0);
 		asm volatile("cp.async.wait_group 1;" ::: "memory");
 		__syncthreads();
-		auto compute = [&](int i, auto edge) {
-			constexpr bool EDGE = decltype(edge)::value;
+		auto compute = [&](int i, auto edge) { // false: to be done again, as an edge
+			constexpr bool EDGE = decltype(edge)::value; // some rows may not see some keys, or scores are large
 			const int b = i & 1, at = first + i * KT;
 			// ---- scores ----
 			float s[KT / 8][4];
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 					if (EDGE && at + n * 8 + t * 2 + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
 					big[e >> 1] = fmaxf(big[e >> 1], s[n][e]);
 				}
-			if (__any_sync(0xffffffffu, above(big[0], fac[0], m[0], coarse) > 2.f || above(big[1], fac[1], m[1], coarse) > 2.f)) { // rare behind the first keys: probabilities may be up to 4
+			if (__any_sync(0xffffffffu, above(big[0], fac[0], m[0], EDGE && coarse) > 2.f || above(big[1], fac[1], m[1], EDGE && coarse) > 2.f)) { // rare behind the first keys: probabilities may be up to 4
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
 					float y = big[h];
@@ -325,9 +325,10 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 					for (int c = 0; c < VG * 4; c++) { acc[c][h * 2] *= f; acc[c][h * 2 + 1] *= f; }
 				}
 				coarse = __any_sync(0xffffffffu, coarse);
+				if (!EDGE && coarse) return false;
 			}
 			const float ml[2] = {m[0] - lift[0], m[1] - lift[1]};
-			if (coarse)
+			if (EDGE && coarse)
 #pragma unroll
 				for (int n = 0; n < KT / 8; n++)
 #pragma unroll
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			for (int n = 0; n < KT / 8; n++)
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
-					const float z0 = ex2(coarse ? s[n][h * 2] : fmaf(s[n][h * 2], fac[h], -ml[h])), z1 = ex2(coarse ? s[n][h * 2 + 1] : fmaf(s[n][h * 2 + 1], fac[h], -ml[h]));
+					const float z0 = ex2(EDGE && coarse ? s[n][h * 2] : fmaf(s[n][h * 2], fac[h], -ml[h])), z1 = ex2(EDGE && coarse ? s[n][h * 2 + 1] : fmaf(s[n][h * 2 + 1], fac[h], -ml[h]));
 					l[h] += z0 + z1;
 					p[n][h] = pack2(z0, z1);
 				}
@@ -376,13 +377,13 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 					}
 				}
 			}
+			return true;
 		};
 		for (int i = 0; i < n_tiles; i++) {
 			copy(i + RING);
 			const int at = first + i * KT;
 			if (warp < GW / 2 && i + 1 < n_tiles) convert(i + 1); // the halves in turn: one's products beside the other's conversion
-			if (at + KT <= least) compute(i, std::false_type());
-			else if (at < most) compute(i, std::true_type());
+			if (at < most && (coarse || at + KT > least || !compute(i, std::false_type()))) compute(i, std::true_type());
 			if (warp >= GW / 2 && i + 1 < n_tiles) convert(i + 1);
 			asm volatile("cp.async.wait_group 1;" ::: "memory");
 			__syncthreads();

@@ -21,13 +21,11 @@ struct VerifyArgs {
 	const float *accept, *pick;
 	int *out, *taken;
 };
-constexpr int VT = 512, VW = VT / 32;
-
-// four neighbouring weights from entry i on
+// four neighbouring weights from place i on, of places k .. k + V - 1 (the row lies k entries behind a boundary of four); WIDE: both rows do
 template <typename T, bool WIDE>
-__device__ __forceinline__ void weights4(const T* p, const T* q, int i, int V, int without, double (&w)[4]) {
+__device__ __forceinline__ void weights4(const T* p, const T* q, int i, int k, int V, int without, double (&w)[4]) {
 	float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
-	if (WIDE && i + 4 <= V) {
+	if (WIDE && i >= k && i + 4 <= V + k) {
 		if constexpr (sizeof(T) == 4) {
 			const float4 a = *reinterpret_cast<const float4*>(p + i);
 			x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
@@ -48,8 +46,9 @@ __device__ __forceinline__ void weights4(const T* p, const T* q, int i, int V, i
 	} else
 #pragma unroll
 		for (int e = 0; e < 4; e++) {
-			x[e] = i + e < V ? to_f(p[i + e]) : 0.f;
-			if (q) y[e] = i + e < V ? to_f(q[i + e]) : 0.f;
+			const bool there = i + e >= k && i + e < V + k;
+			x[e] = there ? to_f(p[i + e]) : 0.f;
+			if (q) y[e] = there ? to_f(q[i + e]) : 0.f;
 		}
 #pragma unroll
 	for (int e = 0; e < 4; e++) {
@@ -63,13 +62,14 @@ __device__ __forceinline__ double warp_sum64(double x) {
 	return x;
 }
 
-template <typename T, bool WIDE>
+template <typename T, int VT>
 __global__ void __launch_bounds__(VT) verify_kernel(const __grid_constant__ VerifyArgs a) {
 	namespace cg = cooperative_groups;
+	constexpr int VW = VT / 32;
 	cg::cluster_group cluster = cg::this_cluster();
 	const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), s = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	__shared__ double s_warp[VW], s_sum;
-	__shared__ int s_taken;
+	__shared__ double s_warp[VW], s_sum, s_run[VW];
+	__shared__ int s_taken, s_found;
 	const int first = min(max(a.starts[s], 0), a.N), n = min(max(a.starts[s + 1], first), a.N) - first;
 	const T *target = reinterpret_cast<const T*>(a.p), *draft = reinterpret_cast<const T*>(a.q);
 	if (warp == 0) { // how many drafts are taken: the first that is not
@@ -102,29 +102,49 @@ __global__ void __launch_bounds__(VT) verify_kernel(const __grid_constant__ Veri
 	}
 	if (n == 0) return; // the whole cluster
 	const long long row = first + taken;
-	const T* p = target + row * a.p_row;
 	const bool refused = taken < n - 1;
-	const int part = ((a.V + ranks * VW - 1) / (ranks * VW) + 127) / 128 * 128; // a warp's run
-	const long long from = ((long long) rank * VW + warp) * part;
-	const int lo = (int) min(from, (long long) a.V), hi = (int) min(from + part, (long long) a.V);
+	constexpr unsigned MASK = 4 * sizeof(T) - 1;
+	// places: from the boundary of four entries that the row begins at or behind
+	const int k = (int) (((uintptr_t) (target + row * a.p_row) & MASK) / sizeof(T)), k_draft = draft ? (int) (((uintptr_t) (draft + row * a.q_row) & MASK) / sizeof(T)) : k;
+	const T* p = target + row * a.p_row - k;
+	const int places = a.V + k, part = ((places + ranks * VW - 1) / (ranks * VW) + 127) / 128 * 128; // a warp's run
+	auto run_of = [&](int w, int& lo, int& hi) {
+		const long long from = ((long long) rank * VW + w) * part;
+		lo = (int) min(from, (long long) places);
+		hi = (int) min(from + part, (long long) places);
+	};
 	const double r = (double) a.pick[s];
 	for (int round = 0; round < 2; round++) { // the second where the draft has all that the target has: from the target's own distribution
-		const T* q = refused && draft && !round ? draft + row * a.q_row : nullptr;
-		const int without = refused && !draft && !round ? a.tokens[row + 1] : -1;
-		double sum = 0.0;
+		const T* q = refused && draft && !round ? draft + row * a.q_row - k : nullptr;
+		const int x_without = refused && !draft && !round ? a.tokens[row + 1] : -1, without = x_without >= 0 && x_without < a.V ? x_without + k : -1;
+		const bool wide = !q || k == k_draft;
+		int lo, hi;
+		run_of(warp, lo, hi);
+		double sums[4] = {0.0, 0.0, 0.0, 0.0};
+		if (wide)
 #pragma unroll 4
-		for (int i = lo + lane * 4; i < hi; i += 128) {
-			double w[4];
-			weights4<T, WIDE>(p, q, i, a.V, without, w);
-			sum += (w[0] + w[1]) + (w[2] + w[3]);
-		}
-		sum = warp_sum64(sum);
+			for (int i = lo + lane * 4; i < hi; i += 128) {
+				double w[4];
+				weights4<T, true>(p, q, i, k, a.V, without, w);
+#pragma unroll
+				for (int e = 0; e < 4; e++) sums[e] += w[e];
+			}
+		else
+#pragma unroll 2
+			for (int i = lo + lane * 4; i < hi; i += 128) {
+				double w[4];
+				weights4<T, false>(p, q, i, k, a.V, without, w);
+#pragma unroll
+				for (int e = 0; e < 4; e++) sums[e] += w[e];
+			}
+		const double sum = warp_sum64((sums[0] + sums[1]) + (sums[2] + sums[3]));
 		if (lane == 0) s_warp[warp] = sum;
 		__syncthreads();
 		if (tid == 0) {
 			double x = 0.0;
 			for (int w = 0; w < VW; w++) x += s_warp[w];
 			s_sum = x;
+			s_found = 0x7fffffff;
 		}
 		cluster.sync();
 		double before = 0.0, total = 0.0;
@@ -142,55 +162,78 @@ __global__ void __launch_bounds__(VT) verify_kernel(const __grid_constant__ Veri
 			return;
 		}
 		const double goal = fmax(r * total, 0.0);
-		// the run in which the sums pass the goal: of the CTA where they do, the first warp
+		// the run in which the sums pass the goal: of the CTA where they do, the first warp's
 		const bool none = !(total > goal); // r is no number below 1: the last token that has a weight
 		if (none ? s_sum <= 0.0 || rank != last_rank : !(before + s_sum > goal) || before > goal) return;
 		int mine = -1, last = -1;
 		double base = 0.0, x = 0.0;
 		for (int w = 0; w < VW; w++) {
 			if (s_warp[w] > 0.0) last = w;
+			if (mine < 0) base = x;
 			x += s_warp[w];
 			if (mine < 0 && before + x > goal) mine = w;
 		}
-		if (mine < 0) mine = last;
-		if (warp != mine) return;
-		for (int w = 0; w < mine; w++) base += s_warp[w];
-		int found = -1, some = -1;
-		for (int i0 = lo; i0 < hi && found < 0; i0 += 128) {
-			const int i = i0 + lane * 4;
+		if (mine < 0) {
+			mine = last;
+			base = 0.0;
+			for (int w = 0; w < last; w++) base += s_warp[w];
+		}
+		// the CTA goes over it again, four places to a thread
+		run_of(mine, lo, hi);
+		int some = -1; // the last with a weight
+		for (int i0 = lo; i0 < hi; i0 += VT * 4) {
+			const int i = i0 + tid * 4;
 			double w[4] = {0.0, 0.0, 0.0, 0.0};
-			if (i < hi) weights4<T, WIDE>(p, q, i, a.V, without, w);
+			if (i < hi) {
+				if (wide) weights4<T, true>(p, q, i, k, a.V, without, w);
+				else weights4<T, false>(p, q, i, k, a.V, without, w);
+			}
 			double run = (w[0] + w[1]) + (w[2] + w[3]), own = run;
 #pragma unroll
 			for (int o = 1; o < 32; o <<= 1) {
 				const double y = __shfl_up_sync(0xffffffffu, run, o);
 				if (lane >= o) run += y;
 			}
+			if (lane == 31) s_run[warp] = run;
+			__syncthreads();
 			double y = base + (run - own);
-			int hit = -1, any = -1;
+			for (int v = 0; v < VW; v++) {
+				if (v < warp) y += s_run[v];
+				base += s_run[v];
+			}
+			int hit = 0x7fffffff;
 #pragma unroll
 			for (int e = 0; e < 4; e++) {
 				y += w[e];
 				if (w[e] > 0.0) {
-					any = i + e;
-					if (hit < 0 && before + y > goal) hit = i + e;
+					some = i + e;
+					if (hit == 0x7fffffff && before + y > goal) hit = i + e;
 				}
 			}
-			const unsigned m = __ballot_sync(0xffffffffu, hit >= 0), h = __ballot_sync(0xffffffffu, any >= 0);
-			if (m) found = __shfl_sync(0xffffffffu, hit, __ffs(m) - 1);
-			if (h) some = __shfl_sync(0xffffffffu, any, 31 - __clz(h));
-			base += __shfl_sync(0xffffffffu, run, 31);
+			if (hit != 0x7fffffff) atomicMin(&s_found, hit);
+			__syncthreads();
+			if (s_found != 0x7fffffff) break;
 		}
-		if (lane == 0) a.out[row] = found >= 0 ? found : some;
+		if (s_found == 0x7fffffff) { // rounded otherwise here: the run's last
+			__syncthreads();
+			if (tid == 0) s_taken = -1;
+			__syncthreads();
+			atomicMax(&s_taken, some);
+			__syncthreads();
+			if (tid == 0) a.out[row] = s_taken - k;
+		} else if (tid == 0) a.out[row] = s_found - k;
 		return;
 	}
 }
 
 template <typename T>
-static int launch_verify(const VerifyArgs& a, int ranks, cudaStream_t s) {
-	const long long wide = 4 * sizeof(T) - 1;
-	const bool aligned = !(((uintptr_t) a.p | (uintptr_t) a.q) & wide) && a.p_row % 4 == 0 && (!a.q || a.q_row % 4 == 0);
-	void (*kernel)(VerifyArgs) = aligned ? verify_kernel<T, true> : verify_kernel<T, false>;
+static int launch_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
+	// CTAs to a sequence: one to every 2048 tokens, up to eight; and of eight warps, of sixteen where there are few sequences
+	int ranks = 1;
+	while (ranks < 8 && ranks * 2048 < a.V) ranks *= 2;
+	const bool large = a.B * ranks <= 2 * sms;
+	void (*kernel)(VerifyArgs) = large ? verify_kernel<T, 512> : verify_kernel<T, 256>;
+	const int VT = large ? 512 : 256;
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3((unsigned) (a.B * ranks));
 	cfg.blockDim = dim3(VT);
@@ -232,7 +275,8 @@ extern "C" int xalm_cuda_verify_drafts(int device, int type, int seqs, int rows,
 	OnDevice on;
 	XALM_TRY(on.set(device));
 	const VerifyArgs a = {type, seqs, rows, vocab, starts, tokens, (const uint8_t*) target, (const uint8_t*) draft, target_row, draft_row, accept, pick, out, taken};
-	const int ranks = 8;
+	int sms = 0;
+	XALM_TRY(sm_count(device, &sms));
 	cudaStream_t s = (cudaStream_t) stream;
-	return type == XALM_F32 ? launch_verify<float>(a, ranks, s) : type == XALM_F16 ? launch_verify<__half>(a, ranks, s) : launch_verify<__nv_bfloat16>(a, ranks, s);
+	return type == XALM_F32 ? launch_verify<float>(a, sms, s) : type == XALM_F16 ? launch_verify<__half>(a, sms, s) : launch_verify<__nv_bfloat16>(a, sms, s);
 }
