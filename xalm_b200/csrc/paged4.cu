@@ -50,7 +50,7 @@ struct Chunk8 { // eight elements as they came
 };
 
 // position of a row (-1: of no sequence, or before its first token) and the page of the pool that has it (-1: none); by a whole warp
-__device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int row, bool& in_seq) {
+__device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int row, bool& in_seq, bool paged = true) { // paged: its page too
 	int pos = -1, page = -1;
 	in_seq = false;
 	if (row < b.N) {
@@ -61,7 +61,7 @@ __device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int
 		if (row_in_seq(q, row)) {
 			in_seq = true;
 			pos = whole - q.n + row - q.a; // what lies behind the table is turned, and written nowhere
-			if (pos >= 0 && pos < view.cap) {
+			if (paged && pos >= 0 && pos < view.cap) {
 				page = page_of(c, b, s, pos >> c.shift);
 				if (page < 0 && (threadIdx.x & 31) == 0) report(c, ERR_PAGE);
 			}
@@ -70,26 +70,26 @@ __device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int
 	return make_int2(pos, page);
 }
 
-// Eight entries of a key from c on, turned in 64 bits: x, and what they are turned with where that is eight neighbours too (PAIRED)
-template <typename I>
-__device__ __forceinline__ void turn_key(const I* head, int c, const Append4Args& a, const double* cs, const double* sn, float (&x)[8], const float (&other)[8]) {
+// Eight entries of a head from c on, turned in T (keys: 64 bits, queries: 32, with mag in cos and sin); other: what they are turned with where that is eight neighbours too (PAIRED)
+template <typename I, typename T>
+__device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a, const T* cs, const T* sn, T mag, float (&x)[8], const float (&other)[8]) {
 	if (c >= 2 * a.rot) return;
 	if (a.paired) {
 		const bool second = c >= a.rot;
 		const int f = second ? c - a.rot : c;
 #pragma unroll
 		for (int e = 0; e < 8; e++) {
-			const double y = (double) x[e] * cs[f + e], z = (double) other[e] * sn[f + e];
-			x[e] = (float) ((second ? y + z : y - z) * (double) a.mag);
+			const T y = (T) x[e] * cs[f + e], z = (T) other[e] * sn[f + e];
+			x[e] = (float) ((second ? y + z : y - z) * mag);
 		}
 	} else if (a.neighbours) {
 #pragma unroll
 		for (int e = 0; e < 8; e += 2) {
 			const int f = (c + e) >> 1;
 			if (f < a.rot) {
-				const double y = (double) x[e], z = (double) x[e + 1];
-				x[e] = (float) ((y * cs[f] - z * sn[f]) * (double) a.mag);
-				x[e + 1] = (float) ((z * cs[f] + y * sn[f]) * (double) a.mag);
+				const T y = (T) x[e], z = (T) x[e + 1];
+				x[e] = (float) ((y * cs[f] - z * sn[f]) * mag);
+				x[e + 1] = (float) ((z * cs[f] + y * sn[f]) * mag);
 			}
 		}
 	} else { // halves that end inside a chunk
@@ -98,8 +98,8 @@ __device__ __forceinline__ void turn_key(const I* head, int c, const Append4Args
 			const int i = c + e;
 			if (i >= 2 * a.rot) continue;
 			const int f = i < a.rot ? i : i - a.rot;
-			const double y = (double) x[e] * cs[f], z = (double) to_f(head[i < a.rot ? i + a.rot : f]) * sn[f];
-			x[e] = (float) ((i < a.rot ? y - z : y + z) * (double) a.mag);
+			const T y = (T) x[e] * cs[f], z = (T) to_f(head[i < a.rot ? i + a.rot : f]) * sn[f];
+			x[e] = (float) ((i < a.rot ? y - z : y + z) * mag);
 		}
 	}
 }
@@ -132,32 +132,41 @@ __device__ __forceinline__ uint32_t block4(const float (&x)[8], unsigned quad, _
 	return w;
 }
 
+// blockIdx.y: 0 for keys and values, 1 for queries
 template <typename I, int R>
-__global__ void __launch_bounds__(A4T) paged4_append_kernel(const __grid_constant__ Append4Args a) {
-	__shared__ double s_cos[R][128], s_sin[R][128];
-	__shared__ int s_pos[R], s_page[R]; // position (-1: of no sequence, or before its first token), page of the pool (-1: none)
+__global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const __grid_constant__ Append4Args a) {
+	__shared__ double s_cos[R][128], s_sin[R][128]; // of queries floats
+	__shared__ int s_pos[R], s_page[R];             // position (-1: of no sequence, or before its first token), page of the pool (-1: none)
 	const int row0 = blockIdx.x * R, tid = threadIdx.x, warp = tid >> 5, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
-	if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, A4T);
+	const bool queries = blockIdx.y == 1;
+	if (blockIdx.x == 0 && !queries) check_seqs(a.c, a.b, tid, A4T);
 	if (warp < R) {
 		bool in_seq;
-		const int2 p = place_of(a.c, a.b, row0 + warp, in_seq);
+		const int2 p = place_of(a.c, a.b, row0 + warp, in_seq, !queries);
 		if ((tid & 31) == 0) { s_pos[warp] = in_seq ? p.x : -1; s_page[warp] = p.y; }
 	}
 	__syncthreads();
+	float (*q_cos)[128] = reinterpret_cast<float (*)[128]>(s_cos), (*q_sin)[128] = reinterpret_cast<float (*)[128]>(s_sin);
 	for (int i = tid; i < R * a.rot; i += A4T) {
 		const int r = i / a.rot, f = i - r * a.rot;
 		if (s_pos[r] < 0) continue;
 		const double x = (double) s_pos[r] * (double) a.freq[f], turns = rint(x * 0.15915494309189535); // the product is exact, and 2 pi the sum of two doubles
-		sincos(fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x)), &s_sin[r][f], &s_cos[r][f]);
+		const double angle = fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x));
+		if (queries) {
+			float sn, cs;
+			sincosf((float) angle, &sn, &cs);
+			q_cos[r][f] = cs * a.mag;
+			q_sin[r][f] = sn * a.mag;
+		} else sincos(angle, &s_sin[r][f], &s_cos[r][f]);
 	}
 	__syncthreads();
 	bool in[R], kept[R];
 #pragma unroll
 	for (int r = 0; r < R; r++) {
 		in[r] = s_pos[r] >= 0;
-		kept[r] = in[r] && s_page[r] >= 0;
+		kept[r] = in[r] && s_page[r] >= 0; // keys and values
 	}
-	const int n_q = a.q ? a.H * a.per_head : 0, n_k = G * KG * 4, n_v = G * VG * 4, slot_mask = (1 << shift) - 1;
+	const int n_q = queries ? a.H * a.per_head : 0, n_k = G * KG * 4, n_v = G * VG * 4, slot_mask = (1 << shift) - 1;
 	for (int i = tid; i < n_q; i += A4T) { // queries, in fp32
 		const int h = a.per_head == 1 ? i : (int) __umulhi((unsigned) i, a.by_head), u = i - h * a.per_head;
 		const bool pair = a.paired && u * 8 < a.rot;
@@ -180,15 +189,16 @@ __global__ void __launch_bounds__(A4T) paged4_append_kernel(const __grid_constan
 				y[r].floats(hi);
 #pragma unroll
 				for (int e = 0; e < 8; e++) {
-					const float cs = (float) s_cos[r][c + e] * a.mag, sn = (float) s_sin[r][c + e] * a.mag, l = lo[e];
+					const float cs = q_cos[r][c + e], sn = q_sin[r][c + e], l = lo[e];
 					lo[e] = l * cs - hi[e] * sn;
 					hi[e] = hi[e] * cs + l * sn;
 				}
 				store8(to + a.rot, hi);
-			} else if (!a.paired) turn_key(from - c + (row0 + r) * a.q_row, c, a, s_cos[r], s_sin[r], lo, lo);
+			} else if (!a.paired) turn(from - c + (row0 + r) * a.q_row, c, a, q_cos[r], q_sin[r], 1.f, lo, lo);
 			store8(to, lo);
 		}
 	}
+	if (queries) return;
 	for (int i = tid; i < n_k + n_v; i += A4T) {
 		const bool value = i >= n_k;
 		const int j = value ? i - n_k : i, by = value ? VG == 2 ? 3 : VG == 4 ? 4 : 5 : KG == 2 ? 3 : KG == 4 ? 4 : 5; // chunks of eight to a head: 8, 16 or 32
@@ -212,7 +222,7 @@ __global__ void __launch_bounds__(A4T) paged4_append_kernel(const __grid_constan
 				if (!value) {
 					float o[8];
 					if (pair) y[r].floats(o);
-					turn_key(from - c + (row0 + r) * step, c, a, s_cos[r], s_sin[r], z, o);
+					turn(from - c + (row0 + r) * step, c, a, s_cos[r], s_sin[r], (double) a.mag, z, o);
 				}
 			}
 			__half scale;
@@ -242,40 +252,44 @@ struct Read4Args {
 	uint8_t *k, *v;
 	long long k_row, v_row;
 };
-template <typename T>
+template <typename T, int R>
 __global__ void __launch_bounds__(A4T) paged4_read_kernel(const __grid_constant__ Read4Args a) {
-	__shared__ int s_pos, s_page;
-	const int row = blockIdx.x, tid = threadIdx.x, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
-	if (row == 0) check_seqs(a.c, a.b, tid, A4T);
-	if (tid < 32) {
+	__shared__ int s_slot[R], s_page[R]; // slot (-1: not to be written), page (-1: none)
+	const int row0 = blockIdx.x * R, tid = threadIdx.x, warp = tid >> 5, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
+	if (blockIdx.x == 0) check_seqs(a.c, a.b, tid, A4T);
+	if (warp < R) {
 		bool in_seq;
-		const int2 p = place_of(a.c, a.b, row, in_seq);
-		if (tid == 0) { s_pos = in_seq ? p.x & ((1 << shift) - 1) : -1; s_page = p.y; }
+		const int2 p = place_of(a.c, a.b, row0 + warp, in_seq);
+		if ((tid & 31) == 0) { s_slot[warp] = in_seq && p.x >= 0 ? p.x & ((1 << shift) - 1) : -1; s_page[warp] = p.y; }
 	}
 	__syncthreads();
-	if (s_pos < 0) return;
-	const int per_k = d / 8, per_v = dv / 8, n_k = G * per_k, n_all = n_k + G * per_v, slot = s_pos, page = s_page;
+	const int per_k = d / 8, per_v = dv / 8, n_k = G * per_k, n_all = n_k + G * per_v;
 	for (int i = tid; i < n_all; i += A4T) {
 		const bool value = i >= n_k;
-		const int j = value ? i - n_k : i, per = value ? per_v : per_k, h = j / per, chunk = j - h * per, g = chunk >> 2, t = chunk & 3;
-		uint32_t w = 0x88888888u;
-		__half scale = __ushort_as_half((unsigned short) 0);
-		if (page >= 0) {
-			const uint8_t* run = a.pool.at + page * a.pool.page + h * a.pool.head;
-			if (value) {
-				const uint8_t* at = run + values_at(KG, shift) + slot * (VG * 16) + g * 2;
-				w = *reinterpret_cast<const uint16_t*>(at + (2 * t) * (VG * 2)) | (uint32_t) *reinterpret_cast<const uint16_t*>(at + (2 * t + 1) * (VG * 2)) << 16;
-				scale = *reinterpret_cast<const __half*>(run + value_scales_at(KG, VG, shift) + slot * (VG * 2) + g * 2);
-			} else {
-				w = *reinterpret_cast<const uint32_t*>(run + slot * (KG * 16) + t * (KG * 4) + g * 4);
-				scale = *reinterpret_cast<const __half*>(run + key_scales_at(KG, shift) + slot * (KG * 2) + g * 2);
+		const int j = value ? i - n_k : i, per = value ? per_v : per_k, h = j / per, chunk = j - h * per, g = chunk >> 2, t = chunk & 3, B = value ? VG : KG;
+		const uint8_t* head = a.pool.at + h * a.pool.head + (value ? values_at(KG, shift) + 4 * t * VG + g * 2 : t * (KG * 4) + g * 4);
+		const int scales = (value ? value_scales_at(KG, VG, shift) - values_at(KG, shift) - 4 * t * VG : key_scales_at(KG, shift) - t * (KG * 4) - g * 2);
+		uint32_t w[R];
+		__half scale[R];
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			w[r] = 0x88888888u;
+			scale[r] = __ushort_as_half((unsigned short) 0);
+			if (s_slot[r] >= 0 && s_page[r] >= 0) {
+				const uint8_t *run = head + s_page[r] * a.pool.page, *at = run + s_slot[r] * (B * 16);
+				w[r] = value ? *reinterpret_cast<const uint16_t*>(at) | (uint32_t) *reinterpret_cast<const uint16_t*>(at + VG * 2) << 16 : *reinterpret_cast<const uint32_t*>(at);
+				scale[r] = *reinterpret_cast<const __half*>(run + scales + s_slot[r] * (B * 2));
 			}
 		}
-		const float f = __half2float(scale);
-		float x[8];
 #pragma unroll
-		for (int e = 0; e < 8; e++) x[e] = f * (float) ((int) (w >> (4 * e) & 15) - 8);
-		store8(reinterpret_cast<T*>(value ? a.v : a.k) + row * (value ? a.v_row : a.k_row) + h * (value ? dv : d) + chunk * 8, x);
+		for (int r = 0; r < R; r++) {
+			if (s_slot[r] < 0) continue;
+			const float f = __half2float(scale[r]);
+			float x[8];
+#pragma unroll
+			for (int e = 0; e < 8; e++) x[e] = f * (float) ((int) (w[r] >> (4 * e) & 15) - 8);
+			store8(reinterpret_cast<T*>(value ? a.v : a.k) + (row0 + r) * (value ? a.v_row : a.k_row) + h * (value ? dv : d) + chunk * 8, x);
+		}
 	}
 }
 
@@ -410,7 +424,7 @@ int xalm_cuda_paged4_append(const xalm_paged4_cache* cache, const xalm_paged_bat
 	void (*kernel)(Append4Args) = type == XALM_F32   ? several ? paged4_append_kernel<float, 4> : paged4_append_kernel<float, 1>
 	                              : type == XALM_F16 ? several ? paged4_append_kernel<__half, 4> : paged4_append_kernel<__half, 1>
 	                                                 : several ? paged4_append_kernel<__nv_bfloat16, 4> : paged4_append_kernel<__nv_bfloat16, 1>;
-	kernel<<<several ? (a.b.N + 3) / 4 : a.b.N, A4T, 0, (cudaStream_t) stream>>>(a);
+	kernel<<<dim3((unsigned) (several ? (a.b.N + 3) / 4 : a.b.N), q ? 2 : 1), A4T, 0, (cudaStream_t) stream>>>(a);
 	XALM_CUDA_CHECK(cudaGetLastError());
 	return XALM_OK;
 }
@@ -432,8 +446,13 @@ int xalm_cuda_paged4_read(const xalm_paged4_cache* cache, const xalm_paged_batch
 	XALM_TRY(on.set(cache->device));
 	a.k = (uint8_t*) k; a.v = (uint8_t*) v;
 	a.k_row = k_row; a.v_row = v_row;
-	void (*kernel)(Read4Args) = type == XALM_F32 ? paged4_read_kernel<float> : type == XALM_F16 ? paged4_read_kernel<__half> : paged4_read_kernel<__nv_bfloat16>;
-	kernel<<<a.b.N, A4T, 0, (cudaStream_t) stream>>>(a);
+	int sms = 0;
+	XALM_TRY(sm_count(cache->device, &sms));
+	const bool several = a.b.N >= sms * 4;
+	void (*kernel)(Read4Args) = type == XALM_F32   ? several ? paged4_read_kernel<float, 4> : paged4_read_kernel<float, 1>
+	                            : type == XALM_F16 ? several ? paged4_read_kernel<__half, 4> : paged4_read_kernel<__half, 1>
+	                                               : several ? paged4_read_kernel<__nv_bfloat16, 4> : paged4_read_kernel<__nv_bfloat16, 1>;
+	kernel<<<several ? (a.b.N + 3) / 4 : a.b.N, A4T, 0, (cudaStream_t) stream>>>(a);
 	XALM_CUDA_CHECK(cudaGetLastError());
 	return XALM_OK;
 }

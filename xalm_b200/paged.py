@@ -303,11 +303,15 @@ def append4(cache, batch, k, v, q=None, freq=None, mag=1.0, neighbours=False, q_
 def read4(cache, batch, rows, dtype=torch.float32, k=None, v=None):
     """Keys (rows, kv_heads, dim) and values (rows, kv_heads, vdim) at the batch's rows, as they are stored; rows outside every sequence are left as they were."""
     (bp, held), stream = _start(cache, batch, rows)
+    kr, vr = cache.kv_heads * cache.dim, cache.kv_heads * cache.vdim
     if k is None:
-        k = torch.empty((rows, cache.kv_heads, cache.dim), dtype=dtype, device=cache.device)
+        k = cache.pool.new_empty((rows, cache.kv_heads, cache.dim), dtype=dtype)
+    else:
+        kr = _rows(k, "k", rows, cache.kv_heads, cache.dim, dtype, cache.device)
     if v is None:
-        v = torch.empty((rows, cache.kv_heads, cache.vdim), dtype=dtype, device=cache.device)
-    kr, vr = _rows(k, "k", rows, cache.kv_heads, cache.dim, dtype, cache.device), _rows(v, "v", rows, cache.kv_heads, cache.vdim, dtype, cache.device)
+        v = cache.pool.new_empty((rows, cache.kv_heads, cache.vdim), dtype=dtype)
+    else:
+        vr = _rows(v, "v", rows, cache.kv_heads, cache.vdim, dtype, cache.device)
     capi.check(capi.lib().xalm_cuda_paged4_read(cache.p, bp, _type(k), k.data_ptr(), kr, v.data_ptr(), vr, stream))
     return k, v
 
@@ -341,24 +345,21 @@ def verify(starts, tokens, target, accept, pick, draft=None, out=None):
     """Drafted tokens against the target's probabilities.  starts (seqs + 1) int32: sequence s has rows starts[s] .. starts[s + 1] - 1, the token that it had and its drafts, tokens (rows) int32.
     target (rows, vocab): probabilities of the token behind each row; draft, of the same type: those that tokens[i + 1] was drawn from, in row i (None: each draft is certain).  accept (rows) and
     pick (seqs): fp32 numbers from 0 to below 1.  Returns (rows) int32: the drafts taken and the token drawn behind them, then -1; and how many were taken (seqs)."""
-    dev = target.device
-    if target.dim() != 2 or target.stride(1) != 1 or dev.type != "cuda":
-        _refuse(f"verify: target {tuple(target.shape)} on {dev}, its rows dense and on a GPU")
+    at, dt = target.get_device(), target.dtype
+    if target.dim() != 2 or at < 0 or target.stride(1) != 1:
+        _refuse(f"verify: target {tuple(target.shape)} on {target.device}, its rows dense and on a GPU")
     n, V = target.shape
-    if draft is not None and (draft.shape != target.shape or draft.dtype is not target.dtype or draft.device != dev or draft.stride(1) != 1):
-        _refuse(f"verify: draft {tuple(draft.shape)} {draft.dtype} on {draft.device}")
-    if starts.dim() != 1 or starts.shape[0] < 1 or pick.shape != (starts.shape[0] - 1,) or tokens.shape != (n,) or accept.shape != (n,):
-        _refuse(f"verify: starts {tuple(starts.shape)}, tokens {tuple(tokens.shape)}, accept {tuple(accept.shape)}, pick {tuple(pick.shape)} for {n} rows")
+    B, row, drow, dp = starts.shape[0] - 1 if starts.dim() == 1 else -1, target.stride(0) if n > 1 else V, 0, 0
+    if draft is not None:
+        if draft.shape != target.shape or draft.dtype is not dt or draft.get_device() != at or draft.stride(1) != 1:
+            _refuse(f"verify: draft {tuple(draft.shape)} {draft.dtype} on {draft.device}")
+        drow, dp = draft.stride(0) if n > 1 else V, draft.data_ptr()
     if out is None:
         out = tokens.new_empty((n,))
-    for t, dt in ((starts, torch.int32), (tokens, torch.int32), (out, torch.int32), (accept, torch.float32), (pick, torch.float32)):
-        if t.dtype is not dt or t.device != dev or not t.is_contiguous():
-            _refuse(f"verify: {t.dtype} on {t.device}, not {dt} on {dev}, dense")
-    if out.shape != (n,):
-        _refuse(f"verify: out {tuple(out.shape)}")
-    B = starts.shape[0] - 1
+    for t, size, kind in ((starts, B + 1, torch.int32), (tokens, n, torch.int32), (out, n, torch.int32), (accept, n, torch.float32), (pick, B, torch.float32)):
+        if t.dim() != 1 or t.shape[0] != size or size < 0 or t.dtype is not kind or t.get_device() != at or not t.is_contiguous():
+            _refuse(f"verify: {tuple(t.shape)} {t.dtype} on {t.device}, not ({size},) {kind} on {target.device}, dense")
     taken = starts.new_empty((B,))
-    capi.check(capi.lib().xalm_cuda_verify_drafts(dev.index, _type(target), B, n, V, starts.data_ptr(), tokens.data_ptr(), target.data_ptr(), target.stride(0) if n > 1 else V,
-                                                  0 if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0) if n > 1 else V, accept.data_ptr(), pick.data_ptr(),
-                                                  out.data_ptr(), taken.data_ptr(), _stream(dev.index)))
+    capi.check(capi.lib().xalm_cuda_verify_drafts(at, _type(target), B, n, V, starts.data_ptr(), tokens.data_ptr(), target.data_ptr(), row, dp, drow, accept.data_ptr(), pick.data_ptr(),
+                                                  out.data_ptr(), taken.data_ptr(), _stream(at)))
     return out, taken
