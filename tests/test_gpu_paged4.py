@@ -455,6 +455,19 @@ def test_append_of_any_size(in_type):
     check_append(p, in_type, x=(k, k.flip(0)), with_q=False)
 
 
+@pytest.mark.parametrize("in_type", ["f32", "bf16"])
+def test_append_where_scales_have_few_bits_or_all(in_type):
+    """Rows of sizes 2^-26 to 2^18 (scales below fp16's normal numbers are far from -M / 8), and rows whose quotients lie on borders between two codes."""
+    p = Problem4("f16", [90], [90], G=1, rep=1, d=64, page=16, seed=77)
+    g = torch.Generator().manual_seed(78)
+    k = torch.randn(90, 1, 64, generator=g) * torch.exp2(torch.arange(90) / 2 - 26)[:, None, None]
+    d = torch.exp2(torch.randint(-10, 8, (90, 1, 2), generator=g).float()) * (1 + torch.randint(0, 1024, (90, 1, 2), generator=g) / 1024)
+    half = torch.randint(-17, 16, (90, 1, 64), generator=g) / 2
+    half[..., 0], half[..., 32] = -8, -8
+    v = half.clamp_min(-8) * d.repeat_interleave(32, dim=2)
+    check_append(p, in_type, x=(k.to(TYPES[in_type]), v.to(TYPES[in_type])), with_q=False)
+
+
 def test_append_far_positions_and_many_rows():
     freq = 1e6 ** (-torch.arange(32) / 32)
     p = Problem4("f16", [2, 1], [200000, 131073], G=1, rep=1, d=64, page=256, seed=85, k=torch.zeros(1300, 1, 256, 64), v=torch.zeros(1300, 1, 256, 64), spare=1300 - 782 - 513)

@@ -77,10 +77,18 @@ __device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a,
 	if (a.paired) {
 		const bool second = c >= a.rot;
 		const int f = second ? c - a.rot : c;
+		struct alignas(16) Two {
+			T v[16 / sizeof(T)];
+		};
+		constexpr int N = 16 / sizeof(T);
 #pragma unroll
-		for (int e = 0; e < 8; e++) {
-			const T y = (T) x[e] * cs[f + e], z = (T) other[e] * sn[f + e];
-			x[e] = (float) ((second ? y + z : y - z) * mag);
+		for (int e0 = 0; e0 < 8; e0 += N) {
+			const Two co = *reinterpret_cast<const Two*>(cs + f + e0), si = *reinterpret_cast<const Two*>(sn + f + e0);
+#pragma unroll
+			for (int e = 0; e < N; e++) {
+				const T y = (T) x[e0 + e] * co.v[e], z = (T) other[e0 + e] * si.v[e];
+				x[e0 + e] = (float) ((second ? y + z : y - z) * mag);
+			}
 		}
 	} else if (a.neighbours) {
 #pragma unroll
@@ -104,38 +112,49 @@ __device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a,
 	}
 }
 
-// What four lanes have of a block, eight entries each: scale and codes (entry i at bit 4 i)
+// What four lanes have of a block, eight entries each: scale and codes (entry i at bit 4 i).  n = rint(x times the rounded 1 / d) is off from x / d by a rounding's worth; x - n d is exact in fp32, and
+// where it is less than d / 2 for all, n is the nearest; elsewhere (a border, a scale that is at its end) the quotients themselves are rounded.
 __device__ __forceinline__ uint32_t block4(const float (&x)[8], unsigned quad, __half& scale) {
-	float hi = x[0], lo = x[0];
-	bool odd = false;
+	float hi = x[0], lo = x[0], none = 0.f;
 #pragma unroll
 	for (int e = 0; e < 8; e++) {
 		hi = fmaxf(hi, x[e]);
 		lo = fminf(lo, x[e]);
-		odd = odd || !(fabsf(x[e]) <= 3.402823466e38f);
+		none = fmaf(x[e], 0.f, none); // a NaN where something is not finite
 	}
 #pragma unroll
 	for (int o = 1; o < 4; o <<= 1) {
 		hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
 		lo = fminf(lo, __shfl_xor_sync(quad, lo, o));
+		none += __shfl_xor_sync(quad, none, o);
 	}
-	odd = __any_sync(quad, odd);
 	scale = __float2half_rn(fminf(fmaxf((hi >= -lo ? hi : lo) * -0.125f, -65504.f), 65504.f));
 	const float d = __half2float(scale);
+	if (none != 0.f || d == 0.f) { // a block with what is no finite number reads as none
+		if (none != 0.f) scale = __ushort_as_half((unsigned short) 0x7fff);
+		return 0x88888888u;
+	}
+	const float inv = 1.f / d, magic = 12582912.f; // 1.5 2^23: sums with it are rounded to whole numbers
+	float most = 0.f;
 	uint32_t w = 0;
 #pragma unroll
 	for (int e = 0; e < 8; e++) {
-		const int c = d == 0.f || odd ? 8 : (int) fminf(fmaxf(rintf(__fdiv_rn(x[e], d)) + 8.f, 0.f), 15.f);
-		w |= (uint32_t) c << (4 * e);
+		const float t = fminf(fmaxf(x[e] * inv, -9.f), 9.f) + magic, n = t - magic;
+		most = fmaxf(most, fabsf(fmaf(-n, d, x[e])));
+		w |= (uint32_t) min(max(__float_as_int(t) - 0x4b400000 + 8, 0), 15) << (4 * e);
 	}
-	if (odd) scale = __ushort_as_half((unsigned short) 0x7fff); // a block with what is no finite number reads as none
+	if (!(most < fabsf(d) * 0.5f)) {
+		w = 0;
+#pragma unroll
+		for (int e = 0; e < 8; e++) w |= (uint32_t) (int) fminf(fmaxf(rintf(__fdiv_rn(x[e], d)) + 8.f, 0.f), 15.f) << (4 * e);
+	}
 	return w;
 }
 
 // blockIdx.y: 0 for keys and values, 1 for queries
 template <typename I, int R>
 __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const __grid_constant__ Append4Args a) {
-	__shared__ double s_cos[R][128], s_sin[R][128]; // of queries floats
+	__shared__ __align__(16) double s_cos[R][128], s_sin[R][128]; // of queries floats
 	__shared__ int s_pos[R], s_page[R];             // position (-1: of no sequence, or before its first token), page of the pool (-1: none)
 	const int row0 = blockIdx.x * R, tid = threadIdx.x, warp = tid >> 5, d = a.c.d, dv = a.c.dv, G = a.c.G, KG = a.pool.kg, VG = a.pool.vg, shift = a.c.shift;
 	const bool queries = blockIdx.y == 1;
@@ -187,11 +206,14 @@ __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const
 			I* to = reinterpret_cast<I*>(a.q_out) + (row0 + r) * a.q_out_row + h * d + c;
 			if (pair) {
 				y[r].floats(hi);
+				float cs[8], sn[8];
+				load8(&q_cos[r][c], cs);
+				load8(&q_sin[r][c], sn);
 #pragma unroll
 				for (int e = 0; e < 8; e++) {
-					const float cs = q_cos[r][c + e], sn = q_sin[r][c + e], l = lo[e];
-					lo[e] = l * cs - hi[e] * sn;
-					hi[e] = hi[e] * cs + l * sn;
+					const float l = lo[e];
+					lo[e] = l * cs[e] - hi[e] * sn[e];
+					hi[e] = hi[e] * cs[e] + l * sn[e];
 				}
 				store8(to + a.rot, hi);
 			} else if (!a.paired) turn(from - c + (row0 + r) * a.q_row, c, a, q_cos[r], q_sin[r], 1.f, lo, lo);
@@ -263,12 +285,13 @@ __global__ void __launch_bounds__(A4T) paged4_read_kernel(const __grid_constant_
 		if ((tid & 31) == 0) { s_slot[warp] = in_seq && p.x >= 0 ? p.x & ((1 << shift) - 1) : -1; s_page[warp] = p.y; }
 	}
 	__syncthreads();
-	const int per_k = d / 8, per_v = dv / 8, n_k = G * per_k, n_all = n_k + G * per_v;
+	constexpr int E = 16 / sizeof(T); // entries of an item: 16 bytes of the result, so that a warp's are side by side
+	const int per_k = d / E, per_v = dv / E, n_k = G * per_k, n_all = n_k + G * per_v;
 	for (int i = tid; i < n_all; i += A4T) {
 		const bool value = i >= n_k;
-		const int j = value ? i - n_k : i, per = value ? per_v : per_k, h = j / per, chunk = j - h * per, g = chunk >> 2, t = chunk & 3, B = value ? VG : KG;
-		const uint8_t* head = a.pool.at + h * a.pool.head + (value ? values_at(KG, shift) + 4 * t * VG + g * 2 : t * (KG * 4) + g * 4);
-		const int scales = (value ? value_scales_at(KG, VG, shift) - values_at(KG, shift) - 4 * t * VG : key_scales_at(KG, shift) - t * (KG * 4) - g * 2);
+		const int j = value ? i - n_k : i, per = value ? per_v : per_k, h = j / per, c = (j - h * per) * E, g = c >> 5, B = value ? VG : KG; // entries c ..
+		const int code = value ? (c & 31) / 4 * (VG * 2) + g * 2 : (c & 31) / 8 * (KG * 4) + g * 4 + (c & 7) / 2, first = value ? values_at(KG, shift) : 0;
+		const uint8_t* head = a.pool.at + h * a.pool.head;
 		uint32_t w[R];
 		__half scale[R];
 #pragma unroll
@@ -276,19 +299,20 @@ __global__ void __launch_bounds__(A4T) paged4_read_kernel(const __grid_constant_
 			w[r] = 0x88888888u;
 			scale[r] = __ushort_as_half((unsigned short) 0);
 			if (s_slot[r] >= 0 && s_page[r] >= 0) {
-				const uint8_t *run = head + s_page[r] * a.pool.page, *at = run + s_slot[r] * (B * 16);
-				w[r] = value ? *reinterpret_cast<const uint16_t*>(at) | (uint32_t) *reinterpret_cast<const uint16_t*>(at + VG * 2) << 16 : *reinterpret_cast<const uint32_t*>(at);
-				scale[r] = *reinterpret_cast<const __half*>(run + scales + s_slot[r] * (B * 2));
+				const uint8_t *run = head + s_page[r] * a.pool.page, *at = run + first + s_slot[r] * (B * 16) + code;
+				if (E == 4) w[r] = *reinterpret_cast<const uint16_t*>(at);
+				else w[r] = value ? *reinterpret_cast<const uint16_t*>(at) | (uint32_t) *reinterpret_cast<const uint16_t*>(at + VG * 2) << 16 : *reinterpret_cast<const uint32_t*>(at);
+				scale[r] = *reinterpret_cast<const __half*>(run + (value ? value_scales_at(KG, VG, shift) : key_scales_at(KG, shift)) + s_slot[r] * (B * 2) + g * 2);
 			}
 		}
 #pragma unroll
 		for (int r = 0; r < R; r++) {
 			if (s_slot[r] < 0) continue;
 			const float f = __half2float(scale[r]);
-			float x[8];
+			T x[E];
 #pragma unroll
-			for (int e = 0; e < 8; e++) x[e] = f * (float) ((int) (w[r] >> (4 * e) & 15) - 8);
-			store8(reinterpret_cast<T*>(value ? a.v : a.k) + (row0 + r) * (value ? a.v_row : a.k_row) + h * (value ? dv : d) + chunk * 8, x);
+			for (int e = 0; e < E; e++) x[e] = from_f<T>(f * (float) ((int) (w[r] >> (4 * e) & 15) - 8));
+			*reinterpret_cast<uint4*>(reinterpret_cast<T*>(value ? a.v : a.k) + (row0 + r) * (value ? a.v_row : a.k_row) + h * (value ? dv : d) + c) = *reinterpret_cast<const uint4*>(x);
 		}
 	}
 }
