@@ -344,7 +344,7 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 }
 
 // What a piece costs beside its tiles, in tiles
-constexpr int LEAD4 = 6, LEAD4_F32 = 6, LEAD4_TILE = 4;
+constexpr int LEAD4 = 6, LEAD4_F32 = 6, LEAD4_TILE = 6;
 // Segments of more rows are the kernel's of many: 32 sequences behind 4096 tokens take 63 us (bf16) and 75 (fp16) for every 16 rows to a kv head, 245 for up to 128
 constexpr int TILE_ROWS = 56;
 constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM

@@ -20,7 +20,8 @@ template <int KG, int VG>
 struct Tile4 {
 	static constexpr int RAW = KT * (KG + VG) * 18, KH = KT * KG * 64, VH = KT * VG * 64; // bytes of a tile as it comes, of its keys and values as fp16
 	static constexpr int SC = KT / 2 * VG * 4;                                             // and of its values' scales, by pairs of keys
-	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + SC) + 2 * KT * 4 + 2 * 4 + GM * 4 + 24;
+	static constexpr int QH = GM * KG * 64;                                                // of the queries
+	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + SC) + QH + 2 * KT * 4 + 2 * 4 + 2 * GM * 4 + 24;
 };
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -73,10 +74,12 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 	uint8_t* s_k = s_raw + RING * Z::RAW;                          // [2][KT][KG * 32] fp16, 16 bytes c of key j at c ^ (j & 7)
 	uint8_t* s_v = s_k + 2 * Z::KH;                                // [2][KT][VG * 32], likewise
 	uint8_t* s_sc = s_v + 2 * Z::VH;                               // [2][KT / 2][VG] pairs of scales
-	float* s_top = reinterpret_cast<float*>(s_sc + 2 * Z::SC);     // [2][KT]: each value's largest scale
+	uint8_t* s_q = s_sc + 2 * Z::SC;                               // [GM][KG * 32], as the keys
+	float* s_top = reinterpret_cast<float*>(s_q + Z::QH);          // [2][KT]: each value's largest scale
 	float* s_most = s_top + 2 * KT;                                // [2]: the tile's
 	int* s_lim = reinterpret_cast<int*>(s_most + 2);               // [GM]: keys that a row sees
-	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_lim + GM);
+	float* s_fac = reinterpret_cast<float*>(s_lim + GM);           // [GM]: from a product to a score in units of log2
+	uint8_t* s_plan = reinterpret_cast<uint8_t*>(s_fac + GM);
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = lane >> 2, t = lane & 3, dv = a.c.dv, P = 1 << a.c.shift, shift = a.c.shift;
 	Plan plan;
 	pdl_launch_dependents();
@@ -203,39 +206,42 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 		copy(0);
 		copy(1);
 		copy(2);
-		// ---- queries as A: rows lane / 4 and 8 behind it; entries in the order of the keys' ----
-		uint32_t q[KG * 2][4];
+		// ---- queries, each warp its own rows: eight entries to a lane, in the order of the keys' ----
+		constexpr int QL = KG * 4; // lanes to a row
+#pragma unroll 2
+		for (int i = 0; i < 16; i += 32 / QL) {
+			const int r = warp * 16 + i + lane / QL, c = lane % QL, w = x.t * GM + r;
+			float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, top = 0.f;
+			if (r < rows && c * 8 < a.c.d) {
+				const long long at = (long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d + c * 8;
+				if (type == XALM_F16) load8(reinterpret_cast<const __half*>(a.q) + at, y);
+				else load8(reinterpret_cast<const __nv_bfloat16*>(a.q) + at, y);
+			}
+#pragma unroll
+			for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+			for (int o = 1; o < QL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
+			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
+			const float f = a.scale < 0.f ? -two_to(e) : two_to(e); // a negative scale turns the queries' signs
+			if (c == 0) s_fac[r] = fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f * two_to(-e) * 8.f, 1e-30f), 3.0e38f); // not 0: 0 times an infinity is no number
+			*reinterpret_cast<uint4*>(s_q + r * (KG * 64) + ((c ^ (r & 7)) * 16)) =
+				make_uint4(pack2(y[0] * f, y[4] * f), pack2(y[1] * f, y[5] * f), pack2(y[2] * f, y[6] * f), pack2(y[3] * f, y[7] * f));
+		}
+		__syncwarp();
 		float fac[2], m[2], l[2], lift[2], room[2]; // p is 2^lift times as large, as the largest scale that the row has seen allows
 		int lim[2];
 		bool coarse = false;
 		const int r0 = warp * 16 + u;
 #pragma unroll
 		for (int half = 0; half < 2; half++) {
-			const int r = r0 + half * 8, w = x.t * GM + r;
-			const bool there = r < rows;
-			const long long at = there ? (long long) (x.row0 + w / a.rep) * a.q_row + (h0 + w % a.rep) * a.c.d : 0;
-			float y[KG * 4][2], top = 0.f; // entries t and t + 4 of every eight
-#pragma unroll
-			for (int c = 0; c < KG * 4; c++)
-#pragma unroll
-				for (int e = 0; e < 2; e++) {
-					const long long i = at + c * 8 + t + e * 4;
-					y[c][e] = there && c * 8 < a.c.d ? (type == XALM_F16 ? __half2float(reinterpret_cast<const __half*>(a.q)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q)[i])) : 0.f;
-					top = fmaxf(top, fabsf(y[c][e]));
-				}
-			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
-			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
-			const float f = a.scale < 0.f ? -two_to(e) : two_to(e); // a negative scale turns the queries' signs
-			fac[half] = fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f * two_to(-e) * 8.f, 1e-30f), 3.0e38f); // not 0: 0 times an infinity is no number
-#pragma unroll
-			for (int c = 0; c < KG * 4; c++) q[c / 2][half + (c & 1) * 2] = pack2(y[c][0] * f, y[c][1] * f);
+			fac[half] = s_fac[r0 + half * 8];
 			m[half] = -3.0e38f;
 			l[half] = 0.f;
 			lift[half] = 13.f;
 			room[half] = 0.f;
 		}
+		const uint32_t q_at = smem_u32(s_q) + (warp * 16 + (lane & 15)) * (KG * 64);
 		float acc[VG * 4][4];
 #pragma unroll
 		for (int c = 0; c < VG * 4; c++)
@@ -257,17 +263,21 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 #pragma unroll
 			for (int n = 0; n < KT / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-			for (int n = 0; n < KT / 8; n += 4) // four chains at a time
+			for (int c = 0; c < KG; c++) {
+				uint32_t q[2][4];
 #pragma unroll
-				for (int c = 0; c < KG; c++) {
+				for (int e = 0; e < 2; e++) matrices(q_at + (((c * 4 + e * 2 + (lane >> 4)) ^ (lane & 7)) * 16), q[e]);
+#pragma unroll
+				for (int n = 0; n < KT / 8; n += 4) { // eight chains
 					uint32_t r[4][4];
 #pragma unroll
 					for (int i = 0; i < 4; i++) matrices(kh + b * Z::KH + ((n + i) * 8 + (lane & 7)) * (KG * 64) + (((c * 4 + (lane >> 3)) ^ (lane & 7)) * 16), r[i]);
 #pragma unroll
-					for (int i = 0; i < 4; i++) mma16(s[n + i], q[c * 2][0], q[c * 2][1], q[c * 2][2], q[c * 2][3], r[i][0], r[i][1]);
+					for (int i = 0; i < 4; i++) mma16(s[n + i], q[0][0], q[0][1], q[0][2], q[0][3], r[i][0], r[i][1]);
 #pragma unroll
-					for (int i = 0; i < 4; i++) mma16(s[n + i], q[c * 2 + 1][0], q[c * 2 + 1][1], q[c * 2 + 1][2], q[c * 2 + 1][3], r[i][2], r[i][3]);
+					for (int i = 0; i < 4; i++) mma16(s[n + i], q[1][0], q[1][1], q[1][2], q[1][3], r[i][2], r[i][3]);
 				}
+			}
 			// ---- the largest scale that a row has seen ----
 			float top[2];
 			top[0] = top[1] = s_most[b];
