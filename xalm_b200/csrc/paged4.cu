@@ -15,6 +15,8 @@ namespace paged {
 // clamp(rint(x / d) + 8, 0, 15).  What is stored does not depend on how a sum was rounded: a turned key is the fp32 number next to the turn in 64 bits, and x / d as fp32 rounds it is on the
 // same side of every n + 1/2 as the quotient itself, because d (n + 1/2) has 16 bits: where x differs from it, then by a unit of x's last place at least, and the quotient by more than half
 // a unit of its own.
+// Queries are turned in fp32 by blocks of their own.  Bound by instructions (turns in 64 bits, codes) and by the lookups in front of them: nine prompts of 300 to 1500 tokens, 32 and 8 heads of 128,
+// take 61 us (173 MB, 2.8 TB/s; keys and queries by the same blocks 87, a division for each code 73), 16 rows 3.9.
 // =========================================================================================================================================
 struct Append4Args {
 	Cache c;
@@ -265,7 +267,8 @@ __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const
 }
 
 // =========================================================================================================================================
-// read: rows of keys and values as the blocks stand for them, d (c - 8), exact in fp32 and rounded once in 16 bits.
+// read: rows of keys and values as the blocks stand for them, d (c - 8), exact in fp32 and rounded once in 16 bits.  Bound by what it writes: 8475 rows of 8 heads of 128 and 128 in 15.9 us as
+// fp32 (79 MB, 5.0 TB/s; 19.6 with eight entries to a thread, whose 32 bytes lie apart from its neighbours'), 12.3 as fp16.
 // =========================================================================================================================================
 struct Read4Args {
 	Cache c;
@@ -344,7 +347,8 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 }
 
 // What a piece costs beside its tiles, in tiles
-constexpr int LEAD4 = 6, LEAD4_F32 = 6, LEAD4_TILE = 6;
+// (64 sequences behind 1000 to 8000 tokens: 94 us, with 2 98, with 14 98; five prompts 368, with 2 401, with 14 390)
+constexpr int LEAD4 = 6, LEAD4_TILE = 6;
 // Segments of more rows are the kernel's of many: 32 sequences behind 4096 tokens take 63 us (bf16) and 75 (fp16) for every 16 rows to a kv head, 245 for up to 128
 constexpr int TILE_ROWS = 56;
 constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
@@ -374,7 +378,7 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 		const bool big = many && i == 0;
 		t.M = big ? more.rows : few.rows;
 		t.grid = sms * (big ? more.per_sm : few.per_sm);
-		t.lead = big ? LEAD4_TILE : type == XALM_F32 ? LEAD4_F32 : LEAD4;
+		t.lead = big ? LEAD4_TILE : LEAD4;
 		t.least_rows = big ? TILE_ROWS + 1 : 1;
 		t.most_rows = many && !big ? TILE_ROWS : 0x7fffffff;
 		// a segment has at most its rows / M + 1 tiles, and there are no more segments than have room for the part's least rows, of sequences as of groups
@@ -444,7 +448,7 @@ int xalm_cuda_paged4_append(const xalm_paged4_cache* cache, const xalm_paged_bat
 	a.by_head = (unsigned) ((0x100000000ull + a.per_head - 1) / a.per_head);
 	int sms = 0;
 	XALM_TRY(sm_count(cache->device, &sms));
-	const bool several = a.b.N >= sms * 4;
+	const bool several = a.b.N >= sms * 4; // four rows to a block once that still gives every SM one, as in paged_append
 	void (*kernel)(Append4Args) = type == XALM_F32   ? several ? paged4_append_kernel<float, 4> : paged4_append_kernel<float, 1>
 	                              : type == XALM_F16 ? several ? paged4_append_kernel<__half, 4> : paged4_append_kernel<__half, 1>
 	                                                 : several ? paged4_append_kernel<__nv_bfloat16, 4> : paged4_append_kernel<__nv_bfloat16, 1>;
