@@ -23,15 +23,20 @@ constexpr int RING = 3;                             // tiles on their way or wai
 template <int KG, int VG>
 struct Tile4 {
 	static constexpr int RAW = KT * (KG + VG) * 18, KH = KT * KG * 64, VH = KT * VG * 64; // bytes of a tile as it comes, of its keys and values as fp16
-	static constexpr int SC = KT / 2 * VG * 4;                                             // and of its values' scales, by pairs of keys
+	static constexpr int SC = KT / 2 * VG * 4, KD = KT / 2 * KG * 8;                       // and of its values' scales, by pairs of keys; of its keys', in fp32
 	static constexpr int QH = GM * KG * 64;                                                // of the queries
-	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + SC) + QH + 2 * KT * 4 + 2 * 4 + 2 * GM * 4 + 24;
+	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + SC + KD) + QH + 2 * KT * 4 + 2 * 4 + 2 * GM * 4 + 24;
 };
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
 	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
 	             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
 	             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) { // added to nothing
+	asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+	             : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+	             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void matrices(uint32_t at, uint32_t (&r)[4]) {
 	asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -58,15 +63,13 @@ __device__ __forceinline__ float ex2(float x) {
 constexpr float COARSE = 262144.f;
 __device__ __forceinline__ float above(float s, float f, float m, bool coarse) { return coarse ? __fsub_rn(__fmul_rn(s, f), m) : fmaf(s, f, -m); }
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
-// A word's codes, c - 8 (EIGHTH: an eighth of that), in the order 0 4 1 5 2 6 3 7: 1024 + c and 1024 + 16 c as they lie, brought there without a rounding
-template <bool EIGHTH>
+// A word's codes, c - 8, in the order 0 4 1 5 2 6 3 7: 1024 + c and 1024 + 16 c as they lie, brought there without a rounding
 __device__ __forceinline__ void numbers(uint32_t w, __half2 (&h)[4]) {
-	const float f = EIGHTH ? 0.125f : 1.f;
 	const uint32_t w8 = w >> 8;
 #pragma unroll
 	for (int i = 0; i < 4; i++) {
 		const uint32_t x = ((i < 2 ? w : w8) & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
-		h[i] = __hfma2(halves(x), __float2half2_rn(i & 1 ? f / 16.f : f), __float2half2_rn(i & 1 ? -72.f * f : -1032.f * f));
+		h[i] = __hfma2(halves(x), __float2half2_rn(i & 1 ? 0.0625f : 1.f), __float2half2_rn(i & 1 ? -72.f : -1032.f));
 	}
 }
 
@@ -78,7 +81,8 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 	uint8_t* s_k = s_raw + RING * Z::RAW;                          // [2][KT][KG * 32] fp16, 16 bytes c of key j at c ^ (j & 7)
 	uint8_t* s_v = s_k + 2 * Z::KH;                                // [2][KT][VG * 32], likewise
 	uint8_t* s_sc = s_v + 2 * Z::VH;                               // [2][KT / 2][VG] pairs of scales
-	uint8_t* s_q = s_sc + 2 * Z::SC;                               // [GM][KG * 32], as the keys
+	uint8_t* s_kd = s_sc + 2 * Z::SC;                              // [2][KT / 2][KG] pairs of scales in fp32
+	uint8_t* s_q = s_kd + 2 * Z::KD;                               // [GM][KG * 32], as the keys
 	float* s_top = reinterpret_cast<float*>(s_q + Z::QH);          // [2][KT]: each value's largest scale
 	float* s_most = s_top + 2 * KT;                                // [2]: the tile's
 	int* s_lim = reinterpret_cast<int*>(s_most + 2);               // [GM]: keys that a row sees
@@ -150,25 +154,21 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			const uint8_t* from = s_raw + i % RING * Z::RAW;
 			const int b = i & 1, j = tid & (KT - 1), c = tid / KT;
 			const uint32_t to_k = kh + b * Z::KH + j * (KG * 64), to_v = vh + b * Z::VH + j * (VG * 64);
-			uint32_t w[KG], v[VG], d[KG / 2];
+			uint32_t w[KG], v[VG];
 			if constexpr (KG == 4) {
 				const uint4 y = *reinterpret_cast<const uint4*>(from + j * 64 + (c ^ (j >> 1 & 3)) * 16);
 				w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
-				const uint2 z = *reinterpret_cast<const uint2*>(from + KT * (KG + VG) * 16 + j * 8);
-				d[0] = z.x; d[1] = z.y;
 			} else {
 				const uint2 y = *reinterpret_cast<const uint2*>(from + j * 32 + c * 8);
 				w[0] = y.x; w[1] = y.y;
-				d[0] = *reinterpret_cast<const uint32_t*>(from + KT * (KG + VG) * 16 + j * 4);
 			}
-#pragma unroll
-			for (int g = 0; g < KG; g++) {
+			auto store = [&](uint32_t to, uint32_t word) {
 				__half2 h[4];
-				numbers<true>(w[g], h);
-				const __half2 f = halves(__byte_perm(d[g / 2], 0, g & 1 ? 0x3232 : 0x1010));
-				asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to_k + (((g * 4 + c) ^ (j & 7)) * 16)), "r"(bits(__hmul2(h[0], f))), "r"(bits(__hmul2(h[1], f))), "r"(bits(__hmul2(h[2], f))),
-				             "r"(bits(__hmul2(h[3], f))) : "memory");
-			}
+				numbers(word, h);
+				asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(bits(h[0])), "r"(bits(h[1])), "r"(bits(h[2])), "r"(bits(h[3])) : "memory");
+			};
+#pragma unroll
+			for (int g = 0; g < KG; g++) store(to_k + (((g * 4 + c) ^ (j & 7)) * 16), w[g]);
 			// entries 8 c .. 8 c + 7 of a value's block: 16 bits each at places 2 c and 2 c + 1
 			if constexpr (VG == 4) {
 				const uint4 y = *reinterpret_cast<const uint4*>(from + KT * KG * 16 + j * 64 + (c ^ (j >> 1 & 3)) * 16);
@@ -179,10 +179,14 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 				v[0] = __byte_perm(y.x, y.y, 0x5410); v[1] = __byte_perm(y.x, y.y, 0x7632);
 			}
 #pragma unroll
-			for (int g = 0; g < VG; g++) {
-				__half2 h[4];
-				numbers<false>(v[g], h);
-				asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to_v + (((g * 4 + c) ^ (j & 7)) * 16)), "r"(bits(h[0])), "r"(bits(h[1])), "r"(bits(h[2])), "r"(bits(h[3])) : "memory");
+			for (int g = 0; g < VG; g++) store(to_v + (((g * 4 + c) ^ (j & 7)) * 16), v[g]);
+			if (warp == GW - 2) { // keys' scales, two keys to a lane
+				const uint8_t* s = from + KT * (KG + VG) * 16 + lane * (KG * 4);
+#pragma unroll
+				for (int z = 0; z < KG / 2; z++) {
+					const float2 y0 = __half22float2(*reinterpret_cast<const __half2*>(s + z * 4)), y1 = __half22float2(*reinterpret_cast<const __half2*>(s + KG * 2 + z * 4));
+					*reinterpret_cast<float4*>(s_kd + b * Z::KD + (lane * KG + z * 2) * 8) = make_float4(y0.x, y1.x, y0.y, y1.y);
+				}
 			}
 			if (warp == GW - 1) { // values' scales, two keys to a lane
 				const uint8_t* s = from + KT * (KG + VG) * 16 + KT * KG * 2 + lane * (VG * 4);
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
 			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
 			const float f = a.scale < 0.f ? -two_to(e) : two_to(e); // a negative scale turns the queries' signs
-			if (c == 0) s_fac[r] = fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f * two_to(-e) * 8.f, 1e-30f), 3.0e38f); // not 0: 0 times an infinity is no number
+			if (c == 0) s_fac[r] = fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f * two_to(-e), 1e-30f), 3.0e38f); // not 0: 0 times an infinity is no number
 			*reinterpret_cast<uint4*>(s_q + r * (KG * 64) + ((c ^ (r & 7)) * 16)) =
 				make_uint4(pack2(y[0] * f, y[4] * f), pack2(y[1] * f, y[5] * f), pack2(y[2] * f, y[6] * f), pack2(y[3] * f, y[7] * f));
 		}
@@ -265,21 +269,26 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			// ---- scores ----
 			float s[KT / 8][4];
 #pragma unroll
-			for (int n = 0; n < KT / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
 			for (int c = 0; c < KG; c++) {
 				uint32_t q[2][4];
 #pragma unroll
 				for (int e = 0; e < 2; e++) matrices(q_at + (((c * 4 + e * 2 + (lane >> 4)) ^ (lane & 7)) * 16), q[e]);
 #pragma unroll
-				for (int n = 0; n < KT / 8; n += 4) { // eight chains
+				for (int n = 0; n < KT / 8; n += 4) { // a block of four times eight keys, then their scales
 					uint32_t r[4][4];
+					float y[4][4];
 #pragma unroll
 					for (int i = 0; i < 4; i++) matrices(kh + b * Z::KH + ((n + i) * 8 + (lane & 7)) * (KG * 64) + (((c * 4 + (lane >> 3)) ^ (lane & 7)) * 16), r[i]);
 #pragma unroll
-					for (int i = 0; i < 4; i++) mma16(s[n + i], q[0][0], q[0][1], q[0][2], q[0][3], r[i][0], r[i][1]);
+					for (int i = 0; i < 4; i++) mma16_new(y[i], q[0][0], q[0][1], q[0][2], q[0][3], r[i][0], r[i][1]);
 #pragma unroll
-					for (int i = 0; i < 4; i++) mma16(s[n + i], q[1][0], q[1][1], q[1][2], q[1][3], r[i][2], r[i][3]);
+					for (int i = 0; i < 4; i++) mma16(y[i], q[1][0], q[1][1], q[1][2], q[1][3], r[i][2], r[i][3]);
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						const float2 d = *reinterpret_cast<const float2*>(s_kd + b * Z::KD + (((n + i) * 4 + t) * KG + c) * 8);
+#pragma unroll
+						for (int e = 0; e < 4; e++) s[n + i][e] = c ? fmaf(y[i][e], e & 1 ? d.y : d.x, s[n + i][e]) : y[i][e] * (e & 1 ? d.y : d.x);
+					}
 				}
 			}
 			// ---- the largest scale that a row has seen ----
