@@ -6,7 +6,7 @@ import torch
 from paged_ref import F32, HALF, TYPES
 
 BLOCKS = lambda n: 2 if n <= 64 else 4 if n <= 128 else 8
-MANY = 56  # (token, head) rows
+MANY = 64  # (token, head) rows
 
 
 def quantise(x):
@@ -119,14 +119,12 @@ class Problem4:
     def attend(self, only=None):
         """(out, lse, tolerance of out, tolerance of lse) in 64 bits; rows outside every sequence, and those not in `only`, are NaN in `out`.
 
-        Tolerances.  A product of 16 terms and what was there lines 17 numbers up by the largest exponent and keeps 23 bits behind it: it is off by at most 17 2^-23 of the largest number as it
-        is written.  16-bit queries: codes c are written as fp16 numbers c 2^-20 of exponent -14, so the largest number is up to 2^7 max|q| where c counts units, twice for a block of 32, and a
-        score is off by ds <= scale max|q| sum_blocks |d| 2 17 2^-16, and by (dim + 16) 2^-24 scale sum |q| |d| (c + 8) for the fp32 additions.  fp32 queries: codes c - 8 are written as they are, up to
-        2^3, and the queries in two parts to 2^-22: ds <= scale max|q| sum_blocks |d| (2 2 17 2^-20 + 32 8 2^-23), and the additions.  A probability is off by the factor 1 + 2 ds (its own score's and the
-        denominator's); the sums over n keys add n 2^-24, exp2 and its argument (1 + |s| log2 e) 2^-22, all relative to sum p |v|.  The second product, in the same way: 2 17 2^-16 sum p |d| for
-        16-bit queries, 2 17 2^-20 sum p |d| for fp32, n / 16 17 2^-23 sum p |v| for what was there, and 2^-21 15 sum p |d| for p d in two parts.  bf16 queries have p d in one part: 2^-11 sum p |v|.  Where more than MANY rows of a kv head (of 16-bit
-        queries, heads of up to 128 entries) read the same keys, keys are rounded to fp16, which a score is off by 2^-11 scale sum |q k| by, and so are p and p d, each 2^-11 sum p |v|.  The result
-        is rounded once to its type."""
+        Tolerances.  A product of 16 terms and what was there lines 17 numbers up by the largest exponent and keeps 23 bits behind it: it is off by at most 17 2^-23 of the largest number in it.
+        With codes c - 8 of up to 2^3, two products to a block of 32 and queries that fp16 holds, a score is off by ds <= scale max|q| sum_blocks |d| 2 17 2^-20, and by (dim + 16) 2^-24 scale sum
+        |q| |d| 16 for the fp32 additions; fp32 queries have two parts, which twice as many products and 2^-22 of each entry add to.  A probability is off by the factor 1 + 2 ds (its own score's and the
+        denominator's); the sums over n keys add n 2^-24, exp2 and its argument (1 + |s| log2 e) 2^-22, all relative to sum p |v|.  The second product, in the same way: 2 17 2^-20 sum p |d|, n / 16
+        17 2^-23 sum p |v| for what was there, and 2^-21 15 sum p |d| for p d in two parts.  bf16 queries have p d in one part: 2^-11 sum p |v|.  Where more than MANY rows of a kv head (of 16-bit
+        queries, heads of up to 128 entries) read the same keys, p and p d are rounded to fp16, each 2^-11 sum p |v|.  The result is rounded once to its type."""
         out = torch.full((self.rows, self.H, self.dv), math.nan, dtype=torch.float64)
         lse, tol_o, tol_l = out[..., 0].clone(), torch.zeros_like(out), torch.zeros(self.rows, self.H, dtype=torch.float64)
         half, wide = HALF[self.type], self.type == "f32"
@@ -150,17 +148,16 @@ class Problem4:
                 out[n, hs], lse[n, hs] = pr @ v, sc.logsumexp(dim=1)
                 a, b = dk[pg, g, sl].double().abs(), dvs[pg, g, sl].double().abs()
                 top, size = q.abs().max(dim=1).values * abs(self.scale), a.sum(dim=1).max()
-                ds = top * size * (4 * 17 * 2.0 ** -20 + 2.0 ** -15 if wide else 2 * 17 * 2.0 ** -16)
+                ds = top * size * (4 * 17 * 2.0 ** -20 + 2.0 ** -15 if wide else 2 * 17 * 2.0 ** -20)
                 ds = ds + (self.d + 16) * F32 * (q.abs().sum(dim=1) * abs(self.scale)) * a.max() * 16
                 rough = 0.0
                 if not wide:
                     rough = 2.0 ** -11 if self.type == "bf16" else 0.0
                     if self.many(s):
-                        ds = ds + 2.0 ** -11 * (q.abs() @ k.abs().T * abs(self.scale)).max(dim=1).values
                         rough = 2 * 2.0 ** -11
                 rel = 2 * ds + rough + 2 * len(at) * F32 + 8 * (1 + sc.abs().max(dim=1).values * 1.4427) * F32
                 spread, step = pr @ v.abs(), (pr @ b).repeat_interleave(32, dim=1)[:, :self.dv]
-                tol_o[n, hs] = spread * (rel[:, None] + len(at) * 17 * 2.0 ** -27) + step * (2 * 17 * 2.0 ** -20 if wide else 2 * 17 * 2.0 ** -16) + step * 15 * 2.0 ** -21 + out[n, hs].abs() * half
+                tol_o[n, hs] = spread * (rel[:, None] + len(at) * 17 * 2.0 ** -27) + step * 2 * 17 * 2.0 ** -20 + step * 15 * 2.0 ** -21 + out[n, hs].abs() * half
                 tol_l[n, hs] = rel + 2 * F32 * lse[n, hs].abs()
         if self.type == "f16":
             tol_o += 2.0 ** -25

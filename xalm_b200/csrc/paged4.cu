@@ -347,10 +347,10 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 }
 
 // What a piece costs beside its tiles, in tiles
-// (64 sequences behind 1000 to 8000 tokens: 94 us, with 2 98, with 14 98; five prompts 368, with 2 401, with 14 390)
+// (64 sequences behind 1000 to 8000 tokens: 94 us, with 2 or 14 98; five prompts 8 % longer with 2 and 6 % with 14)
 constexpr int LEAD4 = 6, LEAD4_TILE = 6;
-// Segments of more rows are the kernel's of many: 32 sequences behind 4096 tokens take 63 us (bf16) and 75 (fp16) for every 16 rows to a kv head, 245 for up to 128
-constexpr int TILE_ROWS = 56;
+// Segments of more rows are the kernel's of many: 32 sequences behind 4096 tokens take 63 us (bf16) and 75 (fp16) for every 16 rows to a kv head, 290 for up to 128
+constexpr int TILE_ROWS = 64;
 constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
 
 static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, int (&kinds)[2]) {

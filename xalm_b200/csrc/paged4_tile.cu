@@ -8,14 +8,15 @@ namespace xalm {
 namespace paged {
 
 // =========================================================================================================================================
-// As in paged4_attn.cu, but 128 (token, head) rows to a unit, 16 to a warp, so that what has to be done to a key's and a value's codes is done once for all of them: the CTA turns a tile of 64
-// keys into fp16 numbers d (c - 8) / 8 and its values into c - 8 in shared memory, while the tile before enters the products.  Scores by m16n8k16 with the rows as A; probabilities become A of
-// the second product where they are, times the value's scale, block by block: what a row does not see may then have any scale, a NaN too, and is left out.
-// Three roundings to fp16 (d (c - 8), p, p d), each by no more than a result of fp16 is rounded by, and other ones for every key, are the price: one conversion for 128 rows.  p is 2^lift times
-// as large, so that the largest scale that its row has seen times 4 has room in p d, and small ones beside it keep their bits.
-// Bound by latency: with 255 registers to a thread an SM has eight warps, whose products keep the tensor pipe busy for 40 % of the time; one half of the warps converts the next tile before its products, the other
-// behind them.  Full units run at 275 TFLOP/s (32 sequences of 32 tokens behind 4096: 250 us), five prompts of 150 to 700 tokens behind 1000 to 3000 take 370, a prompt of 2048 194.
-// 12 warps of 168 registers, half a tile at a time: 359 and 194, but two texts in common 417 in place of 319, since units of 192 rows are filled less often.
+// As in paged4_attn.cu, but 128 (token, head) rows to a unit, 16 to a warp, so that codes are taken apart once for all of them: the CTA turns a tile of 64 keys and values into fp16 numbers
+// c - 8 in shared memory, while the tile before enters the products.  Scores by m16n8k16 with the rows as A, block by block, times the keys' scales in fp32; probabilities become A of the second
+// product where they are, times the values' scales: what a row does not see may then have any scale, a NaN too, and is left out.
+// p and p d are rounded to fp16, each by no more than a result of fp16 is, and otherwise for every key.  p is 2^lift times as large, so that the largest scale that its row has seen times 4 has
+// room in p d, and small ones beside it keep their bits.  (With d (c - 8) rounded to fp16 for the first product five prompts take 370 us in place of 433, but the logarithms of the denominators
+// are off by 1e-5.)
+// Bound by latency: with 255 registers to a thread an SM has eight warps, whose products keep the tensor pipe busy for a third of the time; one half of the warps converts the next tile before its
+// products, the other behind them.  Five prompts of 150 to 700 tokens behind 1000 to 3000 take 433 us (183 TFLOP/s), a prompt of 2048 222, 64 tokens behind 8192 in common and up to 1500 alone 91.
+// 12 warps of 168 registers, half a tile at a time, were 4 % quicker for prompts and a third slower for 128 tokens of two texts, since units of 192 rows are filled less often.
 // =========================================================================================================================================
 constexpr int GT = 256, GW = GT / 32, GM = GW * 16; // threads, warps, rows of a unit
 constexpr int RING = 3;                             // tiles on their way or waiting as they come
