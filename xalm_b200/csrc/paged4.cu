@@ -72,9 +72,9 @@ __device__ __forceinline__ int2 place_of(const Cache& c, const BatchView& b, int
 	return make_int2(pos, page);
 }
 
-// Eight entries of a head from c on, turned in T (keys: 64 bits, queries: 32, with mag in cos and sin); other: what they are turned with where that is eight neighbours too (PAIRED)
+// Eight entries of a head from c on, turned in T (keys: 64 bits, queries: 32); other: what they are turned with where that is eight neighbours too (PAIRED)
 template <typename I, typename T>
-__device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a, const T* cs, const T* sn, T mag, float (&x)[8], const float (&other)[8]) {
+__device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a, const T* cs, const T* sn, float (&x)[8], const float (&other)[8]) {
 	if (c >= 2 * a.rot) return;
 	if (a.paired) {
 		const bool second = c >= a.rot;
@@ -89,7 +89,7 @@ __device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a,
 #pragma unroll
 			for (int e = 0; e < N; e++) {
 				const T y = (T) x[e0 + e] * co.v[e], z = (T) other[e0 + e] * si.v[e];
-				x[e0 + e] = (float) ((second ? y + z : y - z) * mag);
+				x[e0 + e] = (float) (second ? y + z : y - z);
 			}
 		}
 	} else if (a.neighbours) {
@@ -98,8 +98,8 @@ __device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a,
 			const int f = (c + e) >> 1;
 			if (f < a.rot) {
 				const T y = (T) x[e], z = (T) x[e + 1];
-				x[e] = (float) ((y * cs[f] - z * sn[f]) * mag);
-				x[e + 1] = (float) ((z * cs[f] + y * sn[f]) * mag);
+				x[e] = (float) (y * cs[f] - z * sn[f]);
+				x[e + 1] = (float) (z * cs[f] + y * sn[f]);
 			}
 		}
 	} else { // halves that end inside a chunk
@@ -109,7 +109,7 @@ __device__ __forceinline__ void turn(const I* head, int c, const Append4Args& a,
 			if (i >= 2 * a.rot) continue;
 			const int f = i < a.rot ? i : i - a.rot;
 			const T y = (T) x[e] * cs[f], z = (T) to_f(head[i < a.rot ? i + a.rot : f]) * sn[f];
-			x[e] = (float) ((i < a.rot ? y - z : y + z) * mag);
+			x[e] = (float) (i < a.rot ? y - z : y + z);
 		}
 	}
 }
@@ -178,7 +178,12 @@ __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const
 			sincosf((float) angle, &sn, &cs);
 			q_cos[r][f] = cs * a.mag;
 			q_sin[r][f] = sn * a.mag;
-		} else sincos(angle, &s_sin[r][f], &s_cos[r][f]);
+		} else {
+			double sn, cs;
+			sincos(angle, &sn, &cs);
+			s_cos[r][f] = cs * (double) a.mag;
+			s_sin[r][f] = sn * (double) a.mag;
+		}
 	}
 	__syncthreads();
 	bool in[R], kept[R];
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const
 					hi[e] = hi[e] * cs[e] + l * sn[e];
 				}
 				store8(to + a.rot, hi);
-			} else if (!a.paired) turn(from - c + (row0 + r) * a.q_row, c, a, q_cos[r], q_sin[r], 1.f, lo, lo);
+			} else if (!a.paired) turn(from - c + (row0 + r) * a.q_row, c, a, q_cos[r], q_sin[r], lo, lo);
 			store8(to, lo);
 		}
 	}
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const
 				if (!value) {
 					float o[8];
 					if (pair) y[r].floats(o);
-					turn(from - c + (row0 + r) * step, c, a, s_cos[r], s_sin[r], (double) a.mag, z, o);
+					turn(from - c + (row0 + r) * step, c, a, s_cos[r], s_sin[r], z, o);
 				}
 			}
 			__half scale;
