@@ -185,6 +185,20 @@ def test_queries_of_any_size(type):
     assert bad[4, 3] and bad[4, 7] and int(bad.sum()) == 2
 
 
+@pytest.mark.parametrize("rep", [1, 8, 16, 70])
+@pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
+def test_an_infinite_query_gives_no_number_whatever_the_keys(type, rep):
+    """All keys of one sign: their scores are all the same infinity."""
+    p = Problem4(type, [2], [40], G=1, rep=rep, d=64, page=16, seed=74)
+    p.fill(-torch.rand(p.pages, 1, 16, 64, generator=p.gen) - 0.5, torch.randn(p.pages, 1, 16, 64, generator=p.gen))
+    p.q[0, 0, 7], p.q[1, rep - 1, 9] = math.inf, -math.inf
+    cache, batch = p.on_gpu()
+    out, lse = paged.attend4(cache, batch, p.gq, p.scale, want_lse=True)
+    bad = torch.zeros(2, rep, dtype=torch.bool)
+    bad[0, 0], bad[1, rep - 1] = True, True
+    assert torch.equal(torch.isnan(lse.cpu()), bad) and torch.equal(torch.isnan(out.cpu()), bad[..., None].expand(2, rep, 64))
+
+
 @pytest.mark.parametrize("rows", [1, 3])
 @pytest.mark.parametrize("rep", [1, 8, 16, 70])
 @pytest.mark.parametrize("type", ["f16", "bf16", "f32"])

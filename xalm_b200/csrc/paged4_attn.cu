@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(FT, Size4<KG, VG, KIND>::CTAS) paged4_attn_ker
 			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
 			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
 			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
-			const float f = pow2(e);
+			const float f = e0 == 128 ? NAN : pow2(e); // a row with an infinity is no number, whatever the keys' signs
 			if (t == 0) s_fac[n * 8 + u] = fminf(fmaxf(a.scale * 1.4426950408889634f * pow2(10 - e), -3.0e38f), 3.0e38f);
 #pragma unroll
 			for (int g = 0; g < KG; g++) {

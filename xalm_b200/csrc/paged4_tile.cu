@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			for (int o = 1; o < QL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 			// the row times a power of two, so that its largest entry is between 2^14 and 2^15
 			const int e0 = (__float_as_int(top) >> 23) - 127, e = e0 == 128 ? 0 : min(14 - e0, 126);
-			const float f = a.scale < 0.f ? -two_to(e) : two_to(e); // a negative scale turns the queries' signs
+			const float f = e0 == 128 ? NAN : a.scale < 0.f ? -two_to(e) : two_to(e); // a negative scale turns the queries' signs; a row with an infinity is no number, whatever the keys' signs
 			if (c == 0) s_fac[r] = fminf(fmaxf(fabsf(a.scale) * 1.4426950408889634f * two_to(-e), 1e-30f), 3.0e38f); // not 0: 0 times an infinity is no number
 			*reinterpret_cast<uint4*>(s_q + r * (KG * 64) + ((c ^ (r & 7)) * 16)) =
 				make_uint4(pack2(y[0] * f, y[4] * f), pack2(y[1] * f, y[5] * f), pack2(y[2] * f, y[6] * f), pack2(y[3] * f, y[7] * f));
