@@ -749,3 +749,13 @@ def test_serving_with_drafts(type):
             n = int(taken[s])
             kept[s] += fresh[s] + guess[s][:n]
             fresh[s] = [int(got[vstarts[s] + n])]
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("new,rep,groups", [([64] * 40, 1, None), ([65] * 40, 1, None), ([16] * 60, 4, ([0, 30, 60], [16, 16])), ([1] * 300, 7, ([0, 100, 300], [16, 32])), ([17, 3] * 30, 4, ([0, 60], [32])),
+                                            ([400] + [1] * 50, 4, None)])
+def test_as_many_units_as_there_is_room_for(new, rep, groups, type):
+    """Segments that just are, or just are not, the kernel's of many rows, in numbers that fill the workspace's places."""
+    lens = [n + 32 + (7 * i) % 40 for i, n in enumerate(new)]
+    p = Problem4(type, new, lens, G=3, rep=rep, d=64, page=16, seed=93, groups=groups)
+    check_attend(p, only=list(range(0, p.rows, max(1, p.rows // 150))) + [p.rows - 1])

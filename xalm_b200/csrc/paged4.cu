@@ -386,9 +386,11 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 		t.lead = big ? LEAD4_TILE : LEAD4;
 		t.least_rows = big ? TILE_ROWS + 1 : 1;
 		t.most_rows = many && !big ? TILE_ROWS : 0x7fffffff;
-		// a segment has at most its rows / M + 1 tiles, and there are no more segments than have room for the part's least rows, of sequences as of groups
-		const long long rows = rows_all, whole = rows / t.M, most = rows / t.least_rows;
-		const long long tiles = whole + std::min((long long) b.B, most) + (b.n_groups ? whole + std::min((long long) b.n_groups, most) : 0);
+		// a segment has at most its rows / M + 1 tiles, and there are no more segments than have room for the part's least rows, of sequences as of groups; in a part for few rows they have no more
+		// than those.  (Five prompts of 2000 tokens in all, 32 heads of 128 over 8, in a group: 83 MB for both parts, without the second bound 147.)
+		const long long rows = rows_all, most = rows / t.least_rows;
+		auto tiles_of = [&](long long n) { return std::min(rows, many && !big ? n * TILE_ROWS : rows) / t.M + std::min(n, most); };
+		const long long tiles = tiles_of(b.B) + (b.n_groups ? tiles_of(b.n_groups) : 0);
 		if (tiles * c.G + t.grid > 0x7fffffff / t.M) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads are too many for one call", b.N, heads);
 		const long long work = ((long long) b.max_pages << c.shift) / KT + 1;
 		if (tiles * c.G > 0x7fffffffll / (work + t.lead)) return set_error(XALM_ERR_INVALID, "paged attention: %d rows of %d heads over up to %lld keys are too many for one call", b.N, heads, work * KT);

@@ -70,9 +70,6 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 	return r;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); } // -126 <= e <= 127
-__device__ __forceinline__ float load_any(const uint8_t* p, long long i, int type) {
-	return type == XALM_F32 ? reinterpret_cast<const float*>(p)[i] : type == XALM_F16 ? __half2float(reinterpret_cast<const __half*>(p)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-}
 __device__ __forceinline__ void load8_any(const uint8_t* p, long long i, int type, float (&x)[8]) {
 	if (type == XALM_F32) load8(reinterpret_cast<const float*>(p) + i, x);
 	else if (type == XALM_F16) load8(reinterpret_cast<const __half*>(p) + i, x);
