@@ -1,0 +1,82 @@
+"""The 4-bit paged cache and the verification of drafts at the ends of what their numbers may be: probabilities and picks that are none, value scales far apart or near fp16's last bits, far positions."""
+import math
+
+import pytest
+import torch
+
+from paged_ref import TYPES
+from xalm_b200 import paged
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- drafts ------------------------------------------------------------------------------------------------------------------------------
+def weight(x):
+    return float(x) if float(x) > 0 else 0.0  # NaN too
+
+
+def by_definition(starts, tokens, target, accept, pick, draft=None):
+    """Tokens and how many drafts are taken; what is negative or no number is a zero before anything is done with it."""
+    V, out, taken = target.shape[1], [None] * len(tokens), []
+    for s in range(len(starts) - 1):
+        at, end = starts[s], starts[s + 1]
+        while at + 1 < end:
+            x = int(tokens[at + 1])
+            if not 0 <= x < V or not float(accept[at]) * (1.0 if draft is None else weight(draft[at, x])) < weight(target[at, x]):
+                break
+            out[at], at = x, at + 1
+        taken.append(max(at - starts[s], 0))
+        if starts[s] == end:
+            continue
+        p = [weight(w) for w in target[at].tolist()]
+        left = p
+        if at + 1 < end:
+            if draft is None:
+                left = [w if v != int(tokens[at + 1]) else 0.0 for v, w in enumerate(p)]
+            else:
+                left = [max(w - weight(d), 0.0) for w, d in zip(p, draft[at].tolist())]
+        if not any(left):
+            left = p
+        some = [v for v, w in enumerate(left) if w > 0]
+        r = float(pick[s])
+        out[at] = -1
+        if some:
+            out[at] = some[-1]
+            if r < 1:
+                goal, total = max(r, 0.0) * math.fsum(left), 0.0
+                for v in some:
+                    total += left[v]
+                    if total > goal:
+                        out[at] = v
+                        break
+        for i in range(at + 1, end):
+            out[i] = -1
+    return out, taken
+
+
+def check_verify(starts, tokens, target, accept, pick, draft=None):
+    dev = lambda x: None if x is None else x.cuda()
+    left = torch.full((tokens.shape[0],), 77, dtype=torch.int32, device="cuda")
+    out, taken = paged.verify(torch.tensor(starts, dtype=torch.int32, device="cuda"), dev(tokens), dev(target), dev(accept), dev(pick), draft=dev(draft), out=left)
+    want, want_taken = by_definition(starts, tokens, target, accept, pick, draft)
+    assert taken.tolist() == want_taken
+    assert out.tolist() == [77 if w is None else w for w in want]
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [33, 3000])
+def test_a_draft_of_no_probability_is_taken_as_one_of_zero(V, type):
+    """The drafted token's own numbers, of target and draft: a sequence of two drafts for each pair, the second an ordinary one that is always taken."""
+    odd = [-2.0, -0.0, 0.0, 0.5, 1.0, math.nan, -math.inf, -math.nan]
+    cases = [(q, p, u) for q in odd for p in odd for u in (0.0, 0.25, 0.75)] + [(math.inf, p, u) for p in odd for u in (0.25, 0.75)]
+    B, x = len(cases), 7
+    g = torch.Generator().manual_seed(11)
+    target, draft = (torch.randint(0, 8, (3 * B, V), generator=g) / 1024 for _ in range(2))  # sums are exact
+    accept = torch.full((3 * B,), 0.5)
+    tokens = torch.full((3 * B,), x, dtype=torch.int32)
+    for i, (q, p, u) in enumerate(cases):
+        draft[3 * i, x], target[3 * i, x], accept[3 * i] = q, p, u
+        draft[3 * i + 1, x], target[3 * i + 1, x] = 0.25, 0.5
+    pick = torch.rand(B, generator=g)
+    t = TYPES[type]
+    check_verify(list(range(0, 3 * B + 1, 3)), tokens, target.to(t), accept, pick, draft.to(t))

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(VT) verify_kernel(const __grid_constant__ Veri
 				const long long row = first + i;
 				const int x = a.tokens[row + 1];
 				if (x >= 0 && x < a.V) {
-					const double q = draft ? (double) to_f(draft[row * a.q_row + x]) : 1.0;
-					refused = !((double) a.accept[row] * q < (double) to_f(target[row * a.p_row + x]));
+					const float q = draft ? to_f(draft[row * a.q_row + x]) : 1.f, p = to_f(target[row * a.p_row + x]); // what is negative or no number counts as zero, as below
+					refused = !((double) a.accept[row] * (q > 0.f ? (double) q : 0.0) < (p > 0.f ? (double) p : 0.0));
 				}
 			}
 			const unsigned m = __ballot_sync(0xffffffffu, refused);
