@@ -80,3 +80,24 @@ def test_a_draft_of_no_probability_is_taken_as_one_of_zero(V, type):
     pick = torch.rand(B, generator=g)
     t = TYPES[type]
     check_verify(list(range(0, 3 * B + 1, 3)), tokens, target.to(t), accept, pick, draft.to(t))
+
+
+@pytest.mark.parametrize("known", [None, True, False])
+@pytest.mark.parametrize("type", ["f32", "f16"])
+@pytest.mark.parametrize("V", [1, 5, 1000, 40000])
+def test_a_pick_that_is_not_below_1_draws_the_last_weight(V, type, known):
+    """And one below 0 the first, as 0 does; behind refused drafts and without any."""
+    g = torch.Generator().manual_seed(V)
+    picks = [math.nan, -math.nan, 1.0, 1.0, 1.5, 2.0, 1e30, math.inf, 1 - 2.0 ** -24, 0.0, -0.0, -1.0, -math.inf]
+    B, n = len(picks), 1 if known is None else 2
+    target, draft = (torch.randn(n * B, V, generator=g).mul(3).softmax(dim=1) for _ in range(2))
+    target[:, V - V // 3:] = 0  # the last weight is not the last token, and parts of the vocabulary have none
+    target[:, :V // 4] = 0
+    tokens = torch.full((n * B,), V // 2, dtype=torch.int32)
+    accept = torch.full((n * B,), 1.0)
+    target[0::n, V // 2] = 0  # refused
+    if V == 1:
+        target[:] = 0.5
+        accept[:] = 2.0
+    t = TYPES[type]
+    check_verify(list(range(0, n * B + 1, n)), tokens, target.to(t), accept, torch.tensor(picks), draft.to(t) if known else None)

@@ -163,9 +163,9 @@ __global__ void __launch_bounds__(VT) verify_kernel(const __grid_constant__ Veri
 			if (rank == 0 && tid == 0) a.out[row] = -1;
 			return;
 		}
-		const double goal = fmax(r * total, 0.0);
+		const double goal = r < 1.0 ? r > 0.0 ? r * total : 0.0 : INFINITY;
 		// the run in which the sums pass the goal: of the CTA where they do, the first warp's
-		const bool none = !(total > goal); // r is no number below 1: the last token that has a weight
+		const bool none = !(total > goal); // r is no number below 1 (a NaN neither), or the total is infinite: the last token that has a weight
 		if (none ? s_sum <= 0.0 || rank != last_rank : !(before + s_sum > goal) || before > goal) return;
 		int mine = -1, last = -1;
 		double base = 0.0, x = 0.0;
