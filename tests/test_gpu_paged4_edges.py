@@ -1,10 +1,11 @@
 """The 4-bit paged cache and the verification of drafts at the ends of what their numbers may be: probabilities and picks that are none, value scales far apart or near fp16's last bits, far positions."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from paged_ref import TYPES
+from paged4_ref import TYPES, quantise, values
 from xalm_b200 import paged
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +102,42 @@ def test_a_pick_that_is_not_below_1_draws_the_last_weight(V, type, known):
         accept[:] = 2.0
     t = TYPES[type]
     check_verify(list(range(0, n * B + 1, n)), tokens, target.to(t), accept, torch.tensor(picks), draft.to(t) if known else None)
+
+
+# ---- appending --------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("last", [1 << 30, (1 << 29) + 77])
+def test_keys_at_the_farthest_positions_are_the_definitions(last, neighbours):
+    """Keys whose turned entries lie next to borders between two codes, at positions of 30 bits and angles to a turn for every position: the product of position and frequency has more than 53 bits."""
+    P, G, n, rot = 256, 8, 32, 1024 // 32
+    g = torch.Generator().manual_seed(12)
+    freq = (0.5 + 0.5 * torch.rand(rot, generator=g)).float()
+    pages = (last + P - 1) // P
+    pos = np.arange(last - n, last)
+    angle = pos.astype(np.longdouble)[:, None] * freq.numpy().astype(np.longdouble)  # 54 bits
+    assert np.finfo(np.longdouble).nmant >= 63
+    cs, sn = np.cos(angle)[:, None], np.sin(angle)[:, None]
+    i = np.arange(rot)
+    a, b = (2 * i, 2 * i + 1) if neighbours else (i, i + rot)
+    aim = (torch.randint(-7, 7, (n, G, 64), generator=g) + 0.5).numpy().astype(np.longdouble)
+    aim[..., 0], aim[..., 32] = -8, -8
+    k = np.zeros((n, G, 64), dtype=np.float32)
+    k[..., a], k[..., b] = aim[..., a] * cs + aim[..., b] * sn, aim[..., b] * cs - aim[..., a] * sn  # turned back
+    x, y = k[..., a].astype(np.longdouble), k[..., b].astype(np.longdouble)
+    turned = np.zeros((n, G, 64), dtype=np.float32)
+    turned[..., a], turned[..., b] = x * cs - y * sn, y * cs + x * sn
+    want = values(*quantise(torch.from_numpy(turned)), 64)
+
+    pool = torch.zeros(2, G, paged.page4_bytes(P, 64), dtype=torch.uint8, device="cuda")
+    table = torch.zeros(1, pages, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    cache = paged.PagedCache4(pool, P, 64)
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device="cuda")
+    batch = paged.Batch(i32([0, n]), i32([last]), table)
+    rows = torch.from_numpy(k).cuda()
+    q = paged.append4(cache, batch, rows, rows, q=rows, freq=freq.cuda(), neighbours=neighbours)
+    got = paged.read4(cache, batch, n)[0].double().cpu()
+    cache.check()
+    assert torch.equal(got, want), f"{int((got != want).sum())} of {got.numel()} numbers"
+    # queries: cos and sin within 2^-22, three roundings of fp32
+    assert float((q.double().cpu() - torch.from_numpy(turned).double()).abs().max()) <= 2.0 ** -21 * float(rows.abs().max())

@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(A4T, R > 1 ? 3 : 1) paged4_append_kernel(const
 	for (int i = tid; i < R * a.rot; i += A4T) {
 		const int r = i / a.rot, f = i - r * a.rot;
 		if (s_pos[r] < 0) continue;
-		const double x = (double) s_pos[r] * (double) a.freq[f], turns = rint(x * 0.15915494309189535); // the product is exact, and 2 pi the sum of two doubles
-		const double angle = fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x));
+		const double pos = (double) s_pos[r], freq = (double) a.freq[f], x = pos * freq, rest = fma(pos, freq, -x); // x + rest is the product itself: it has 54 or 55 bits from position 2^29 on
+		const double turns = rint(x * 0.15915494309189535), angle = fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, x)) + rest; // 2 pi is the sum of two doubles
 		if (queries) {
 			float sn, cs;
 			sincosf((float) angle, &sn, &cs);
