@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from paged4_ref import TYPES, quantise, values
+from paged4_ref import TYPES, Problem4, quantise, values
 from xalm_b200 import paged
 
 pytestmark = pytest.mark.gpu
@@ -102,6 +102,56 @@ def test_a_pick_that_is_not_below_1_draws_the_last_weight(V, type, known):
         accept[:] = 2.0
     t = TYPES[type]
     check_verify(list(range(0, n * B + 1, n)), tokens, target.to(t), accept, torch.tensor(picks), draft.to(t) if known else None)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------------------------
+def near(got, want, tol, what=""):
+    over = (got.double().cpu() - want).abs() - tol
+    assert float(over.max()) <= 0, f"{what}: {float(over.max())} over the tolerance at {int((over > 0).sum())} of {over.numel()}"
+
+
+def check_as_few(p):
+    """attend4 against 64 bits by the tolerances of few rows (Problem4.attend), however many there are: p d enters the second product as one fp16 number for bf16, as two for fp16 and fp32.  In units where
+    the largest scale that the row sees, D, is 2^11 at least, fp16's last place is off by 2^-25: by 2^-36 D in p d, by 8 times that in a value's part, for each key, where the largest p is 1."""
+    cache, batch = p.on_gpu()
+    out, lse = paged.attend4(cache, batch, p.gq, p.scale, want_lse=True)
+    cache.check()
+    p.many = lambda s: False
+    want, want_lse, tol, tol_lse = p.attend()
+    if p.type != "f32":
+        for n in range(p.rows):
+            s, last = p.row(n)
+            at = torch.arange(last + 1)
+            pages = p.table[s].long()[at // p.page]
+            score = torch.einsum("grd,jgd->grj", p.q[n].double().unflatten(0, (p.G, p.rep)), p.k[pages, :, at % p.page]) * p.scale
+            total = torch.exp(want_lse[n] - score.amax(dim=-1).flatten())  # the sum of p
+            scales = p.pool_scales(1)[pages, :, at % p.page].double().abs().max()
+            tol[n] += (8 * (last + 1) * 2.0 ** -36 * float(scales) / total)[:, None]
+    near(out, want, tol, "out")
+    near(lse, want_lse, tol_lse, "lse")
+
+
+MANY = [dict(new=[1], rep=70), dict(new=[20], rep=4), dict(new=[1] * 20, rep=4, groups=([0, 20], [128]))]  # more than 64 rows that read the same keys
+
+
+@pytest.mark.parametrize("power", [-8, -14, -20, -24, 12])
+@pytest.mark.parametrize("kind", range(len(MANY)))
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_many_rows_keep_small_probabilities_of_small_and_large_scales(type, kind, power):
+    """Of 64 keys 63 lie e^14 to e^19 below the first: they count with all the bits that the result has, at scales of 2^power."""
+    n = 135
+    p = Problem4(type, lens=[n] * len(MANY[kind]["new"]), G=1, d=32, page=64, seed=66, **MANY[kind])
+    k, v = torch.zeros(p.pages, 1, 64, 32), torch.zeros(p.pages, 1, 64, 32)
+    k[..., 0] = -8.0
+    v[..., 1] = -8.0 * 2.0 ** power
+    k[:, 0, 0] = 0
+    v[:, 0, 0] = 0
+    v[:, 0, 0, 0] = -8.0 * 2.0 ** power
+    p.fill(k, v)
+    p.q[:] = 0
+    p.q[..., 0] = (14 + 5 * torch.rand(p.rows, p.H, generator=p.gen)).to(p.t) / 8
+    p.scale = 1.0
+    check_as_few(p)
 
 
 # ---- appending --------------------------------------------------------------------------------------------------------------------------

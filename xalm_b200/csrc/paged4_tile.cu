@@ -24,9 +24,9 @@ constexpr int RING = 3;                             // tiles on their way or wai
 template <int KG, int VG>
 struct Tile4 {
 	static constexpr int RAW = KT * (KG + VG) * 18, KH = KT * KG * 64, VH = KT * VG * 64; // bytes of a tile as it comes, of its keys and values as fp16
-	static constexpr int SC = KT / 2 * VG * 4, KD = KT / 2 * KG * 8;                       // and of its values' scales, by pairs of keys; of its keys', in fp32
+	static constexpr int VD = KT / 2 * VG * 8, KD = KT / 2 * KG * 8;                       // and of its values' scales, by pairs of keys, and its keys', in fp32
 	static constexpr int QH = GM * KG * 64;                                                // of the queries
-	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + SC + KD) + QH + 2 * KT * 4 + 2 * 4 + 2 * GM * 4 + 24;
+	static constexpr size_t own = (size_t) RING * RAW + 2 * (KH + VH + VD + KD) + QH + 2 * KT * 4 + 2 * 4 + 2 * GM * 4 + 24;
 };
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 	uint8_t* s_raw = smem;                                         // [RING][RAW]: key codes, value codes, key scales, value scales
 	uint8_t* s_k = s_raw + RING * Z::RAW;                          // [2][KT][KG * 32] fp16, 16 bytes c of key j at c ^ (j & 7)
 	uint8_t* s_v = s_k + 2 * Z::KH;                                // [2][KT][VG * 32], likewise
-	uint8_t* s_sc = s_v + 2 * Z::VH;                               // [2][KT / 2][VG] pairs of scales
-	uint8_t* s_kd = s_sc + 2 * Z::SC;                              // [2][KT / 2][KG] pairs of scales in fp32
+	uint8_t* s_vd = s_v + 2 * Z::VH;                               // [2][KT / 2][VG] pairs of values' scales in fp32
+	uint8_t* s_kd = s_vd + 2 * Z::VD;                              // [2][KT / 2][KG] of keys'
 	uint8_t* s_q = s_kd + 2 * Z::KD;                               // [GM][KG * 32], as the keys
 	float* s_top = reinterpret_cast<float*>(s_q + Z::QH);          // [2][KT]: each value's largest scale
 	float* s_most = s_top + 2 * KT;                                // [2]: the tile's
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 	Walk k;
 	bool more = walk_begin(a, part, plan, k);
 	if (tid == 0) write_head(a, part, k, more, more && k.x.seg >= a.b.n_groups && k.x.key0 == 0, plan.share);
-	const uint32_t raw = smem_u32(s_raw), kh = smem_u32(s_k), vh = smem_u32(s_v), sc = smem_u32(s_sc);
+	const uint32_t raw = smem_u32(s_raw), kh = smem_u32(s_k), vh = smem_u32(s_v);
 	for (; more; more = walk_next(a, part, plan, k)) {
 		const Piece& x = k.x;
 		if (x.j0 == x.j1) continue; // the same for every thread
@@ -205,8 +205,10 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 					top[y] = fmaxf(__low2float(m), __high2float(m)); // NaN counts for nothing
 				}
 #pragma unroll
-				for (int g = 0; g < VG; g++)
-					*reinterpret_cast<uint32_t*>(s_sc + b * Z::SC + (lane * VG + g) * 4) = __byte_perm(e[0][g / 2], e[1][g / 2], g & 1 ? 0x7632 : 0x5410);
+				for (int z = 0; z < VG / 2; z++) {
+					const float2 y0 = __half22float2(halves(e[0][z])), y1 = __half22float2(halves(e[1][z]));
+					*reinterpret_cast<float4*>(s_vd + b * Z::VD + (lane * VG + z * 2) * 8) = make_float4(y0.x, y1.x, y0.y, y1.y);
+				}
 				*reinterpret_cast<float2*>(s_top + b * KT + lane * 2) = make_float2(top[0], top[1]);
 				const float all = warp_max(fmaxf(fmaxf(top[0], top[1]), 0.f));
 				if (lane == 0) s_most[b] = all;
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 				make_uint4(pack2(y[0] * f, y[4] * f), pack2(y[1] * f, y[5] * f), pack2(y[2] * f, y[6] * f), pack2(y[3] * f, y[7] * f));
 		}
 		__syncwarp();
-		float fac[2], m[2], l[2], lift[2], room[2]; // p is 2^lift times as large, as the largest scale that the row has seen allows
+		float fac[2], m[2], l[2], lift[2], room[2]; // p is 2^lift times as large, so that the largest scale that the row has seen is 2^11 to 2^12 in p d
 		int lim[2];
 		bool coarse = false;
 		const int r0 = warp * 16 + u;
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			fac[half] = s_fac[r0 + half * 8];
 			m[half] = -3.0e38f;
 			l[half] = 0.f;
-			lift[half] = 13.f;
+			lift[half] = 0.f;
 			room[half] = 0.f;
 		}
 		const uint32_t q_at = smem_u32(s_q) + (warp * 16 + (lane & 15)) * (KG * 64);
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 				for (int h = 0; h < 2; h++)
 					if (top[h] > room[h]) {
 						const int e = (__float_as_int(top[h]) >> 23) - 127; // 2^e <= top < 2^(e + 1): scales up to twice that have room
-						const float to = fminf(fmaxf((float) (11 - e), -4.f), 13.f), f = exp2f(to - lift[h]);
+						const float to = (float) max(11 - e, -4), f = exp2f(to - lift[h]); // -4 for the largest finite scale, 35 for the smallest
 						room[h] = two_to(min(e + 2, 127));
 						l[h] *= f;
 						lift[h] = to;
@@ -357,25 +359,17 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 				for (int n = 0; n < KT / 8; n++)
 #pragma unroll
 					for (int e = 0; e < 4; e++) s[n][e] = __fsub_rn(__fmul_rn(s[n][e], fac[e >> 1]), m[e >> 1]) + lift[e >> 1];
-			uint32_t p[KT / 8][2];
 #pragma unroll
 			for (int n = 0; n < KT / 8; n++)
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
-					const float z0 = ex2(EDGE && coarse ? s[n][h * 2] : fmaf(s[n][h * 2], fac[h], -ml[h])), z1 = ex2(EDGE && coarse ? s[n][h * 2 + 1] : fmaf(s[n][h * 2 + 1], fac[h], -ml[h]));
-					l[h] += z0 + z1;
-					p[n][h] = pack2(z0, z1);
+					s[n][h * 2] = ex2(EDGE && coarse ? s[n][h * 2] : fmaf(s[n][h * 2], fac[h], -ml[h]));
+					s[n][h * 2 + 1] = ex2(EDGE && coarse ? s[n][h * 2 + 1] : fmaf(s[n][h * 2 + 1], fac[h], -ml[h]));
+					l[h] += s[n][h * 2] + s[n][h * 2 + 1];
 				}
 			// ---- sums ----
 #pragma unroll
 			for (int kk = 0; kk < KT / 16; kk++) {
-				uint32_t lo[VG], hi[VG]; // scales of keys 2 t, 2 t + 1 and 8 behind them
-#pragma unroll
-				for (int g = 0; g < VG; g += 2) {
-					const uint2 y = *reinterpret_cast<const uint2*>(s_sc + b * Z::SC + ((kk * 8 + t) * VG + g) * 4), z = *reinterpret_cast<const uint2*>(s_sc + b * Z::SC + ((kk * 8 + 4 + t) * VG + g) * 4);
-					lo[g] = y.x; lo[g + 1] = y.y;
-					hi[g] = z.x; hi[g + 1] = z.y;
-				}
 				uint32_t seen[4];
 				if constexpr (EDGE) {
 #pragma unroll
@@ -387,8 +381,10 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 				const uint32_t row = vh + b * Z::VH + (kk * 16 + (lane & 15)) * (VG * 64);
 #pragma unroll
 				for (int g = 0; g < VG; g++) {
-					uint32_t f[4] = {bits(__hmul2(halves(p[kk * 2][0]), halves(lo[g]))), bits(__hmul2(halves(p[kk * 2][1]), halves(lo[g]))), bits(__hmul2(halves(p[kk * 2 + 1][0]), halves(hi[g]))),
-					                 bits(__hmul2(halves(p[kk * 2 + 1][1]), halves(hi[g])))};
+					// scales of keys 2 t, 2 t + 1 and 8 behind them
+					const float2 d0 = *reinterpret_cast<const float2*>(s_vd + b * Z::VD + ((kk * 8 + t) * VG + g) * 8), d1 = *reinterpret_cast<const float2*>(s_vd + b * Z::VD + ((kk * 8 + 4 + t) * VG + g) * 8);
+					const float *p0 = s[kk * 2], *p1 = s[kk * 2 + 1];
+					uint32_t f[4] = {pack2(p0[0] * d0.x, p0[1] * d0.y), pack2(p0[2] * d0.x, p0[3] * d0.y), pack2(p1[0] * d1.x, p1[1] * d1.y), pack2(p1[2] * d1.x, p1[3] * d1.y)};
 					if constexpr (EDGE)
 #pragma unroll
 						for (int e = 0; e < 4; e++) f[e] &= seen[e];
@@ -423,14 +419,14 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 			sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 			const int r = r0 + h * 8, w = x.t * GM + r;
 			const bool any = sum > 0.f || sum != sum, there = r < rows;
-			const float down = ex2(-lift[h]), f = direct ? any ? 1.f / sum : 0.f : down;
+			const float down = two_to(-(int) lift[h]), f = direct ? any ? 1.f / sum : 0.f : down;
 			const long long tok = x.row0 + w / a.rep;
 			const int hd = h0 + w % a.rep;
 			if (there && t == 0) {
 				const float top = m[h] == -3.0e38f ? -INFINITY : m[h];
 				if (!direct) {
 					if (slot < part.slots) part.ml[slot * GM + r] = make_float2(top, sum * down);
-				} else if (a.lse) a.lse[tok * a.H + hd] = any ? (top - lift[h] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+				} else if (a.lse) a.lse[tok * a.H + hd] = any ? (top + log2f(sum * down)) * 0.6931471805599453f : -INFINITY;
 			}
 #pragma unroll
 			for (int c = 0; c < VG * 4; c++) {
