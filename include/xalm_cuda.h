@@ -359,9 +359,7 @@ int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_ba
  *   (with its status bit); rows outside every sequence, and before their sequence's first token, are left alone.
  * paged4_attend: as paged_attend; queries and results have `type`, whatever was appended.  Maxima and sums in fp32, queries to 2^-39 of a row's largest entry (fp32: in two parts, 2^-22 of each);
  *   products of probability and scale enter the second product as fp16 numbers, one for bf16, two for fp16 and fp32, in units of the largest scale that the row has seen: what is below 2^-36 of its
- *   largest product is lost.  Where more than 64 (token, head) rows of a kv head read the same keys (16-bit queries, heads of at most 128 entries, and the call has more tokens than sequences, groups, or more
- *   than 64 rows to a token), probabilities are rounded to fp16 too, and what is below 2^-21 to 2^-38 of a row's largest product, the less the larger scales are, is lost.
- *   A row whose query is not finite gives no number.  What a row does not see may be anything.
+ *   largest product is lost.  A row whose query is not finite gives no number.  What a row does not see may be anything.
  * paged4_status, paged4_workspace: as above. */
 typedef struct xalm_paged4_cache {
 	int device;

@@ -154,6 +154,29 @@ def test_many_rows_keep_small_probabilities_of_small_and_large_scales(type, kind
     check_as_few(p)
 
 
+@pytest.mark.parametrize("kind", range(len(MANY)))
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_many_rows_have_the_bits_of_few(type, kind):
+    """All keys but the first of each page alike, each row with a probability of its own for them: the numbers that fp16 rounds are the same for all of them, and so are its errors."""
+    p = Problem4(type, lens=[135] * len(MANY[kind]["new"]), G=1, d=32, page=64, seed=67, **MANY[kind])
+    k, v = torch.zeros(p.pages, 1, 64, 32), torch.zeros(p.pages, 1, 64, 32)
+    k[..., 0] = -8.0
+    v[..., :] = -8.0 * (1 + torch.arange(32) // 4 / 8) * 1.2822265625  # scales of 11 bits
+    k[:, 0, 0] = 0
+    v[:, 0, 0] = 0
+    p.fill(k, v)
+    p.q[:] = 0
+    p.q[..., 0] = (2 * torch.rand(p.rows, p.H, generator=p.gen)).to(p.t) / 8
+    p.scale = 1.0
+    check_as_few(p)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_long_prompts_have_the_bits_of_few_rows(type):
+    for groups in (None, ([0, 3], [256])):
+        check_as_few(Problem4(type, [90, 1, 200], [900, 300, 456], rep=4, d=128, dv=64, page=64, seed=68, groups=groups))
+
+
 # ---- appending --------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("neighbours", [False, True])
 @pytest.mark.parametrize("last", [1 << 30, (1 << 29) + 77])

@@ -10,12 +10,13 @@ namespace paged {
 // =========================================================================================================================================
 // As in paged4_attn.cu, but 128 (token, head) rows to a unit, 16 to a warp, so that codes are taken apart once for all of them: the CTA turns a tile of 64 keys and values into fp16 numbers
 // c - 8 in shared memory, while the tile before enters the products.  Scores by m16n8k16 with the rows as A, block by block, times the keys' scales in fp32; probabilities become A of the second
-// product where they are, times the values' scales: what a row does not see may then have any scale, a NaN too, and is left out.
-// p and p d are rounded to fp16, each by no more than a result of fp16 is, and otherwise for every key.  p is 2^lift times as large, so that the largest scale that its row has seen times 4 has
-// room in p d, and small ones beside it keep their bits.  (With d (c - 8) rounded to fp16 for the first product five prompts take 370 us in place of 433, but the logarithms of the denominators
-// are off by 1e-5.)
+// product where they are, times the values' scales in fp32: what a row does not see may then have any scale, a NaN too, and is left out.
+// p d is rounded once, to one fp16 number for bf16 results, to two in turn for fp16, whose own rounding one would add to: five prompts of fp16 take 580 us with two, 456 with one, whose results have 1.31
+// times the root mean square error.  p is 2^lift times as large, so that the largest scale that its row has seen times 4 has room in p d, and small ones beside it keep their bits.  (With p rounded to
+// fp16 too and the scales multiplied as pairs, 433 us, but 1.56 times the error, and sums of small scales lost; with d (c - 8) rounded to fp16 for the first product 15 % less time, but the logarithms
+// of the denominators are off by 1e-5.)
 // Bound by latency: with 255 registers to a thread an SM has eight warps, whose products keep the tensor pipe busy for a third of the time; one half of the warps converts the next tile before its
-// products, the other behind them.  Five prompts of 150 to 700 tokens behind 1000 to 3000 take 433 us (183 TFLOP/s), a prompt of 2048 222, 64 tokens behind 8192 in common and up to 1500 alone 91.
+// products, the other behind them.  Five prompts of 150 to 700 tokens behind 1000 to 3000 take 456 us of bf16 (173 TFLOP/s), 64 tokens behind 8192 in common and up to 1500 alone 95.
 // 12 warps of 168 registers, half a tile at a time, were 4 % quicker for prompts and a third slower for 128 tokens of two texts, since units of 192 rows are filled less often.
 // =========================================================================================================================================
 constexpr int GT = 256, GW = GT / 32, GM = GW * 16; // threads, warps, rows of a unit
@@ -74,7 +75,8 @@ __device__ __forceinline__ void numbers(uint32_t w, __half2 (&h)[4]) {
 	}
 }
 
-template <int KG, int VG>
+// TWO: p d in two parts, for fp16 results
+template <int KG, int VG, bool TWO>
 __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constant__ Attn a, const __grid_constant__ Part part, const Pool4 pool, const int type) {
 	using Z = Tile4<KG, VG>;
 	extern __shared__ __align__(128) uint8_t smem[];
@@ -384,16 +386,28 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 					// scales of keys 2 t, 2 t + 1 and 8 behind them
 					const float2 d0 = *reinterpret_cast<const float2*>(s_vd + b * Z::VD + ((kk * 8 + t) * VG + g) * 8), d1 = *reinterpret_cast<const float2*>(s_vd + b * Z::VD + ((kk * 8 + 4 + t) * VG + g) * 8);
 					const float *p0 = s[kk * 2], *p1 = s[kk * 2 + 1];
-					uint32_t f[4] = {pack2(p0[0] * d0.x, p0[1] * d0.y), pack2(p0[2] * d0.x, p0[3] * d0.y), pack2(p1[0] * d1.x, p1[1] * d1.y), pack2(p1[2] * d1.x, p1[3] * d1.y)};
-					if constexpr (EDGE)
+					const float2 y[4] = {make_float2(p0[0] * d0.x, p0[1] * d0.y), make_float2(p0[2] * d0.x, p0[3] * d0.y), make_float2(p1[0] * d1.x, p1[1] * d1.y), make_float2(p1[2] * d1.x, p1[3] * d1.y)};
+					uint32_t f[4];
+					[[maybe_unused]] uint32_t rest[4];
 #pragma unroll
-						for (int e = 0; e < 4; e++) f[e] &= seen[e];
+					for (int e = 0; e < 4; e++) {
+						f[e] = pack2(y[e].x, y[e].y);
+						if constexpr (TWO) rest[e] = pack2(y[e].x - __low2float(halves(f[e])), y[e].y - __high2float(halves(f[e])));
+						if constexpr (EDGE) {
+							f[e] &= seen[e];
+							if constexpr (TWO) rest[e] &= seen[e];
+						}
+					}
 #pragma unroll
 					for (int c = 0; c < 4; c += 2) {
 						uint32_t r[4];
 						matrices_turned(row + (((g * 4 + c + (lane >> 4)) ^ (lane & 7)) * 16), r);
 						mma16(acc[g * 4 + c], f[0], f[1], f[2], f[3], r[0], r[1]);
 						mma16(acc[g * 4 + c + 1], f[0], f[1], f[2], f[3], r[2], r[3]);
+						if constexpr (TWO) {
+							mma16(acc[g * 4 + c], rest[0], rest[1], rest[2], rest[3], r[0], r[1]);
+							mma16(acc[g * 4 + c + 1], rest[0], rest[1], rest[2], rest[3], r[2], r[3]);
+						}
 					}
 				}
 			}
@@ -444,12 +458,16 @@ __global__ void __launch_bounds__(GT, 1) paged4_tile_kernel(const __grid_constan
 	pdl_wait(); // not ahead of the kernel before it to the join
 }
 
+template <int KG, int VG, bool TWO>
+static int launch_parts(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
+	const size_t smem = Tile4<KG, VG>::own + plan_bytes(a.b.B, a.b.n_groups);
+	XALM_CUDA_CHECK(allow_smem((const void*) paged4_tile_kernel<KG, VG, TWO>));
+	XALM_CUDA_CHECK(launch(paged4_tile_kernel<KG, VG, TWO>, a.part[part].grid, GT, smem, s, part > 0, a, a.part[part], p, type));
+	return XALM_OK;
+}
 template <int KG, int VG>
 static int launch_tile(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
-	const size_t smem = Tile4<KG, VG>::own + plan_bytes(a.b.B, a.b.n_groups);
-	XALM_CUDA_CHECK(allow_smem((const void*) paged4_tile_kernel<KG, VG>));
-	XALM_CUDA_CHECK(launch(paged4_tile_kernel<KG, VG>, a.part[part].grid, GT, smem, s, part > 0, a, a.part[part], p, type));
-	return XALM_OK;
+	return type == XALM_F16 ? launch_parts<KG, VG, true>(a, p, part, type, s) : launch_parts<KG, VG, false>(a, p, part, type, s);
 }
 Shape4 tile4_shape(const Pool4& p) { return p.kg <= 4 && p.vg <= 4 ? Shape4{GM, 1} : Shape4{0, 0}; }
 int launch_attn4_tile(const Attn& a, const Pool4& p, int part, int type, cudaStream_t s) {
