@@ -358,8 +358,8 @@ int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_ba
  * paged4_read: keys (rows, kv_heads dim) and values (rows, kv_heads vdim) at the batch's rows as the blocks stand for them, in `type`, rounded once; zeros where the table has no page for a row
  *   (with its status bit); rows outside every sequence, and before their sequence's first token, are left alone.
  * paged4_attend: as paged_attend; queries and results have `type`, whatever was appended.  Maxima and sums in fp32, queries to 2^-39 of a row's largest entry (fp32: in two parts, 2^-22 of each);
- *   products of probability and scale enter the second product as fp16 numbers, one for bf16, two for fp16 and fp32, in units of the largest scale that the row has seen: what is below 2^-36 of its
- *   largest product is lost.  A row whose query is not finite gives no number.  What a row does not see may be anything.
+ *   products of probability and scale enter the second product as fp16 numbers, one for bf16, two for fp16 and fp32.  Their unit follows the largest scale that the row has seen, whatever its key's
+ *   probability (what is below 2^-36 of it is lost), for fp32 the largest of the row's products (2^-35).  A row whose query is not finite gives no number.  What a row does not see may be anything.
  * paged4_status, paged4_workspace: as above. */
 typedef struct xalm_paged4_cache {
 	int device;

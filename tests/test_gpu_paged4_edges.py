@@ -177,6 +177,41 @@ def test_long_prompts_have_the_bits_of_few_rows(type):
         check_as_few(Problem4(type, [90, 1, 200], [900, 300, 456], rep=4, d=128, dv=64, page=64, seed=68, groups=groups))
 
 
+@pytest.mark.parametrize("power", [12, 18, 24, 30])
+@pytest.mark.parametrize("where", [0, 5, 150, 299])
+@pytest.mark.parametrize("rep", [1, 4, 6, 16])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+def test_a_large_scale_of_next_to_no_weight_takes_no_bits_from_fp32_rows(type, rep, where, power):
+    """A value 2^power times the others', e^-90 below their scores (the largest of the first keys, where it is the first): fp32 rows are as exact as without it, others lose what is below 2^-36 of it."""
+    p = Problem4(type, [1, 3], [300, 310], G=2, rep=rep, d=64, page=16, seed=69)
+    k, v = torch.randn(p.pages, 2, 16, 64, generator=p.gen), torch.randn(p.pages, 2, 16, 64, generator=p.gen) * 2.0 ** -14
+    p.q[..., 0] = 12.0
+    k[..., 0] = 7.5
+    for s in range(2):
+        for at in range(where + 1 if where < 6 else 0):  # those before it as far below
+            k[p.table[s, at // 16], :, at % 16, 0] = -7.5
+        k[p.table[s, where // 16], :, where % 16, 0] = -7.5
+        v[p.table[s, where // 16], :, where % 16] *= 2.0 ** power
+    p.fill(k, v)
+    p.scale = 0.5
+    check_as_few(p)
+
+
+@pytest.mark.parametrize("rep", [1, 4, 6, 16])
+def test_fp32_rows_whose_scores_grow_as_their_scales_shrink(rep):
+    """Every key some e^3 above the one before it, its value 2^-0.5 as large: the unit of the sums follows the products, down as well as up."""
+    p = Problem4("f32", [1, 3], [70, 64], G=2, rep=rep, d=64, page=16, seed=70)
+    k, v = torch.randn(p.pages, 2, 16, 64, generator=p.gen) * 0.1, torch.randn(p.pages, 2, 16, 64, generator=p.gen)
+    for s in range(2):
+        for at in range(p.lens[s]):
+            k[p.table[s, at // 16], :, at % 16, 0] = 0.15 * at - 5
+            v[p.table[s, at // 16], :, at % 16] *= 2.0 ** (12 - 0.5 * at)
+    p.fill(k, v)
+    p.q[..., 0] = 20.0
+    p.scale = 1.0
+    check_as_few(p)
+
+
 # ---- appending --------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("neighbours", [False, True])
 @pytest.mark.parametrize("last", [1 << 30, (1 << 29) + 77])

@@ -23,7 +23,9 @@ constexpr int FT = 128, FW = FT / 32, FK = KT / FW; // keys of a warp in every t
 constexpr int FP = 20;                              // floats between the probabilities of a warp's rows
 
 // Kernels by the type of the queries and the rows of a unit.  How p d enters the second product: one fp16 number (bf16 results), two in turn, or two in columns of their own (SPLIT, where a tile of
-// columns has four rows; fp32 queries enter the first product so too).
+// columns has four rows; fp32 queries enter the first product so too).  Its unit is taken from the largest scale that a row has seen, which leaves fp16 and bf16 results their bits wherever scales are
+// less than 2^24 apart; fp32 results would lose some from 2^12 on, so there it follows the products themselves, down too where the maxima grow: 64 fp32 tokens behind 1000 to 8000 take 103 us with the one, 102
+// with the other, 32 sequences of three to six 189 and 177.
 template <int KG, int VG, int KIND>
 struct Size4 {
 	static constexpr bool WIDE = KIND == F4 || KIND == F16, SPLIT = WIDE || KIND == H4, TWO = KIND == H16;
@@ -111,6 +113,7 @@ struct Values {
 };
 
 constexpr float NONE = -3.0e38f; // the maximum before the first key
+constexpr int LEAST = -100;      // products of fp32 rows below 2^LEAST make the second product's unit no smaller: they are of keys far below others whose scales are zeros
 // s f - m: in one step where that is off by less than 2^-6 from the rounded product, which m is one of; else in two, so that the largest score is 0 above itself
 constexpr float COARSE = 262144.f;
 __device__ __forceinline__ float above(float s, float f, float m, bool coarse) { return coarse ? __fsub_rn(__fmul_rn(s, f), m) : fmaf(s, f, -m); }
@@ -127,7 +130,7 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 	if constexpr (IN_REGS)
 #pragma unroll
 		for (int i = 0; i < KG * 2; i++) q[i] = s_q[i * 32 + lane];
-	float acc[VG * 2][NT][4], m[NT][2], l[NT][2], mu[NT], room[NT]; // mu: what p d is multiplied with; room: the largest d that it allows
+	float acc[VG * 2][NT][4], m[NT][2], l[NT][2], mu[NT], room[NT]; // mu: what p d is multiplied with; room: the largest d (WIDE: p d) that it allows
 #pragma unroll
 	for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -237,7 +240,8 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 		}
 		if (__any_sync(0xffffffffu, grow)) { // rare behind the first keys: probabilities may be up to 4
 #pragma unroll
-			for (int n = 0; n < NT; n++)
+			for (int n = 0; n < NT; n++) {
+				float up[2]; // what the maxima grow by, and the units with them
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
 					const float f0 = c ? fac[n].y : fac[n].x;
@@ -245,13 +249,25 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 					for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 					top = fmaxf(m[n][c], top);
-					const float f = exp2f(m[n][c] - top);
+					up[c] = top - m[n][c];
 					m[n][c] = top;
-					l[n][c] *= f;
-#pragma unroll
-					for (int i = 0; i < VG * 2; i++) { acc[i][n][c] *= f; acc[i][n][c + 2] *= f; }
+					l[n][c] *= exp2f(-up[c]);
 					coarse = coarse || (fabsf(top) > COARSE && top != NONE);
 				}
+				float g = 1.f;
+				if constexpr (WIDE) { // all products so far are as much smaller: so is what they need room for
+					const float up0 = __shfl_sync(0xffffffffu, up[0], u >> 1), up1 = __shfl_sync(0xffffffffu, up[1], u >> 1);
+					if (room[n] > 0.f) {
+						const int e = min((int) fminf(u & 1 ? up1 : up0, 100.f), (__float_as_int(room[n]) >> 23) - 127 - (LEAST + 2));
+						g = pow2(e);
+						mu[n] *= g;
+						room[n] *= pow2(-e);
+					}
+				}
+				const float f0 = exp2f(-up[0]) * (WIDE ? __shfl_sync(0xffffffffu, g, t * 8) : 1.f), f1 = exp2f(-up[1]) * (WIDE ? __shfl_sync(0xffffffffu, g, t * 8 + 4) : 1.f);
+#pragma unroll
+				for (int i = 0; i < VG * 2; i++) { acc[i][n][0] *= f0; acc[i][n][2] *= f0; acc[i][n][1] *= f1; acc[i][n][3] *= f1; }
+			}
 			coarse = __any_sync(0xffffffffu, coarse);
 #pragma unroll
 			for (int n = 0; n < NT; n++)
@@ -290,27 +306,38 @@ __device__ __forceinline__ void piece4(const Attn& a, const Pool4& pool, const P
 #pragma unroll
 						for (int w = 0; w < VG / 2; w++) vs[n][i * (VG / 2) + w] = 0;
 			}
+			asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(p4[n].x), "=f"(p4[n].y), "=f"(p4[n].z), "=f"(p4[n].w) : "r"(p_read + n * 8 * FP * 4));
 			uint32_t big = vs[n][0];
 #pragma unroll
 			for (int i = 1; i < 2 * VG; i++) big = max_abs2(big, vs[n][i]);
-			const float top = fmaxf(fabsf(half_lo(big)), fabsf(half_hi(big)));
+			float top = fmaxf(fabsf(half_lo(big)), fabsf(half_hi(big)));
+			if constexpr (WIDE) top *= fmaxf(fmaxf(p4[n].x, p4[n].y), fmaxf(p4[n].z, p4[n].w)); // no product of these keys is larger
 			if (__any_sync(0xffffffffu, top > room[n])) {
+				if constexpr (WIDE) { // the largest itself: a large scale of a key that has next to no weight takes no bits from the others
+					top = 0.f;
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						uint32_t own = vs[n][i * (VG / 2)];
+#pragma unroll
+						for (int w = 1; w < VG / 2; w++) own = max_abs2(own, vs[n][i * (VG / 2) + w]);
+						top = fmaxf(top, (i == 0 ? p4[n].x : i == 1 ? p4[n].y : i == 2 ? p4[n].z : p4[n].w) * fmaxf(fabsf(half_lo(own)), fabsf(half_hi(own))));
+					}
+				}
 				float y = fmaxf(top, room[n]);
 				y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
 				y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
 				float f = 1.f;
 				if (y > room[n]) {
-					const int e = (__float_as_int(y) >> 23) - 127; // 2^e <= y < 2^(e + 1): scales up to twice that have room
+					const int e = max((__float_as_int(y) >> 23) - 127, LEAST); // 2^e <= y < 2^(e + 1): scales up to twice that have room, and products up to eight times
 					const float to = pow2(11 - e);
 					f = to / mu[n];
 					mu[n] = to;
-					room[n] = pow2(min(e + 2, 127));
+					room[n] = pow2(min(e + (WIDE ? 4 : 2), 127));
 				}
 				const float f0 = __shfl_sync(0xffffffffu, f, t * 8), f1 = __shfl_sync(0xffffffffu, f, t * 8 + 4);
 #pragma unroll
 				for (int i = 0; i < VG * 2; i++) { acc[i][n][0] *= f0; acc[i][n][2] *= f0; acc[i][n][1] *= f1; acc[i][n][3] *= f1; }
 			}
-			asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(p4[n].x), "=f"(p4[n].y), "=f"(p4[n].z), "=f"(p4[n].w) : "r"(p_read + n * 8 * FP * 4));
 			p4[n].x *= mu[n]; p4[n].y *= mu[n]; p4[n].z *= mu[n]; p4[n].w *= mu[n];
 		}
 #pragma unroll
