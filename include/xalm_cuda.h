@@ -353,7 +353,7 @@ int xalm_cuda_paged_workspace(const xalm_paged_cache* cache, const xalm_paged_ba
  *   page_size 16, 32, 64, 128 or 256 slots; dim, vdim multiples of 8, at most 256.  With K and V the blocks of a slot's key and value (2, 4 or 8: heads up to 64, 128 and 256 entries), a run is
  *   the slots' key codes (16 K bytes each), the keys' scales (2 K), value codes (16 V) and scales (2 V): page_size 18 (K + V) bytes.  Entry 32 g + 8 t + i of a key (t < 4, i < 8) is in byte
  *   4 K t + 4 g + i / 2 of its codes, entry 32 g + 4 u + i of a value (u < 8, i < 4) in byte 2 V u + 2 g + i / 2; even entries in the low half.
- * paged4_append: as paged_append; keys are turned in 64 bits and rounded to fp32 before they are stored, so that what is stored is the definition's; q_out has the rows' type, apart from q.  Two rows
+ * paged4_append: as paged_append; keys are turned in 64 bits and rounded to fp32 before they are stored, so that what is stored is the definition's, queries in 32; q_out has the rows' type, apart from q.  Two rows
  *   that a table sends to the same slot may leave a mixture of both there.
  * paged4_read: keys (rows, kv_heads dim) and values (rows, kv_heads vdim) at the batch's rows as the blocks stand for them, in `type`, rounded once; zeros where the table has no page for a row
  *   (with its status bit); rows outside every sequence, and before their sequence's first token, are left alone.

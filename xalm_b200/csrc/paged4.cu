@@ -15,8 +15,8 @@ namespace paged {
 // clamp(rint(x / d) + 8, 0, 15).  What is stored does not depend on how a sum was rounded: a turned key is the fp32 number next to the turn in 64 bits, and x / d as fp32 rounds it is on the
 // same side of every n + 1/2 as the quotient itself, because d (n + 1/2) has 16 bits: where x differs from it, then by a unit of x's last place at least, and the quotient by more than half
 // a unit of its own.
-// Queries are turned in fp32 by blocks of their own.  Bound by instructions (turns in 64 bits, codes) and by the lookups in front of them: nine prompts of 300 to 1500 tokens, 32 and 8 heads of 128,
-// take 61 us (173 MB, 2.8 TB/s; keys and queries by the same blocks 87, a division for each code 73), 16 rows 3.9.
+// Queries are turned in fp32 by blocks of their own.  Nine prompts of 300 to 1500 tokens, 32 and 8 heads of 128, take 60 us (173 MB, 2.9 TB/s; keys and queries by the same blocks 87, a division for each
+// code 73), 16 rows 3.9.  No unit is full there (issue 55 %, ALU 38 %, DRAM 27 %): 80 registers leave three blocks to an SM, and their loads wait for the lookups in front of them.
 // =========================================================================================================================================
 struct Append4Args {
 	Cache c;
@@ -351,12 +351,13 @@ static int check_apart_from_cache4(const char* call, const Span& out, const Cach
 	                               Span{"group_bounds", b.bounds, 4ll * (b.n_groups + 1)}, Span{"group_shared", b.shared, 4ll * b.n_groups}});
 }
 
-// What a piece costs beside its tiles, in tiles
-// (64 sequences behind 1000 to 8000 tokens: 94 us, with 2 or 14 98; five prompts 8 % longer with 2 and 6 % with 14)
+// What a piece costs beside its tiles, in tiles (64 sequences behind 1000 to 8000 tokens: 94 us, with 2 97, with 14 98; 32 of three to six tokens of fp16 111, 114 and 120; five prompts 456, 474 and 486)
 constexpr int LEAD4 = 6, LEAD4_TILE = 6;
-// Segments of more rows are the kernel's of many: 32 sequences behind 4096 tokens take 63 us (bf16) and 75 (fp16) for every 16 rows to a kv head, 290 for up to 128
+// Segments of more rows are the kernel's of many.  32 sequences behind 4096 tokens, by the kernel of few rows and by this: of 48 rows to a kv head 190 and 280 us (fp16 226 and 341), of 64 243 and 289 (290 and
+// 346), of 80 293 and 342 (353 and 443), of 96 348 and 353 (418 and 451), of 128 452 and 383 (545 and 481)
 constexpr int TILE_ROWS = 64;
-constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8; // rows to a block of the join, and most blocks to an SM
+// rows to a block of the join, a warp to each, and most blocks to an SM (64 tokens behind 8192 in common: 94.6 us, with 2 101, with 4 or 16 the same; 128 in two groups 129.8, 144, 131 and 129.8)
+constexpr int JOIN_ROWS4 = 4, JOIN_BLOCKS4 = 8;
 
 static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchView& b, int type, int heads, Attn& a, size_t* bytes, int (&kinds)[2]) {
 	if (heads <= 0 || heads % c.G || heads > 65535) return set_error(XALM_ERR_INVALID, "paged attention: %d query heads over %d", heads, c.G);
@@ -368,7 +369,8 @@ static int plan_attn4(int device, const Cache& c, const Pool4& p, const BatchVie
 	a.b = b;
 	a.H = heads;
 	a.rep = heads / c.G;
-	// One kernel for segments of few rows, by the rows that one has on average, and where some may have more than TILE_ROWS, the one of many rows for those
+	// One kernel for segments of few rows, by the rows that one has on average, and where some may have more than TILE_ROWS, the one of many rows for those.  32 sequences behind 4096 tokens: of 4 rows to a kv
+	// head fp16 56.7 us by units of 4 and 79.8 by units of 16, fp32 58 and 143; of 8 rows fp16 108 and 88, fp32 104 and 147; of 8 rows bf16 60 by units of 8 and 75 by units of 16, of 12 102 and 77.
 	const long long rows_all = (long long) b.N * a.rep, each = (rows_all + b.B - 1) / std::max(b.B, 1);
 	const int few_kind = type == XALM_F32 ? each <= 4 ? F4 : F16 : type == XALM_F16 ? each <= 4 ? H4 : H16 : each <= 8 ? B8 : B16;
 	const Shape4 few = attn4_shape(p, b, few_kind), more = tile4_shape(p);

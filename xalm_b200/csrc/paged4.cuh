@@ -1,9 +1,9 @@
 // paged4.cuh — what the kernels of the paged cache of 4-bit numbers (xalm_cuda_paged4_*) share: where blocks lie in a page.
 //
 // A block is 32 neighbouring entries of a head, x = d (c - 8) with d in fp16 and codes c of 4 bits.  The kv heads of a page have a run of bytes each: the slots' key codes, the keys'
-// scales, the values' codes, the values' scales.  A slot's codes fill 64, 128 or 256 entries.  Attention brings them to the matrix units without passing through shared memory, so they lie in
-// the order in which its lanes hold them: a key's block goes to 4 lanes, 8 entries (a word) to each, a value's to 8 lanes, 4 entries to each; and what a lane has of a slot's blocks lies
-// together, so that it comes in one load.
+// scales, the values' codes, the values' scales.  A slot's codes fill 64, 128 or 256 entries.  They lie in the order in which the lanes of attention's products hold them, so that a lane reads its
+// own from the copied tile in shared memory and no exchange is needed behind that: a key's block goes to 4 lanes, 8 entries (a word) to each, a value's to 8 lanes, 4 entries to each; and what a lane has
+// of a slot's blocks lies together, 4 to 32 bytes by loads of up to 16.
 #pragma once
 #include "paged.cuh"
 

@@ -12,8 +12,8 @@ namespace paged {
 // pass r times their total.  Tokens drawn so have the target's distribution.
 // A cluster of CTAs has a sequence, each a part of the vocabulary, each warp a run of it, so that it is read once: sums in 64 bits (p - q is exact there, and a token's sum is off by less than
 // its own probability's last bits), the parts' totals by the cluster's shared memory; then the CTA in whose part the goal lies goes over that warp's run again, which is in L2.
-// Bound by latency: four loads that depend on one another before the row is known, then the row.  64 sequences over 131072 tokens, with the drafts' distributions, 19.8 us (3.4 TB/s), eight
-// over 32000 6.1; with 16 warps to a CTA everywhere, so that not all have room at once, and one warp for the second look, 30.
+// Bound by latency: four loads that depend on one another before the row is known, then the row.  64 sequences over 131072 tokens, with the drafts' distributions, 20 us (3.3 TB/s), eight
+// over 32000 6.3; with 16 warps to a CTA everywhere, so that not all have room at once, and one warp for the second look, 30.
 // =========================================================================================================================================
 struct VerifyArgs {
 	int type, B, N, V;
@@ -230,7 +230,9 @@ __global__ void __launch_bounds__(VT) verify_kernel(const __grid_constant__ Veri
 
 template <typename T>
 static int launch_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
-	// CTAs to a sequence: one to every 2048 tokens, up to eight; and of eight warps, of sixteen where there are few sequences
+	// CTAs to a sequence: one to every 2048 tokens, up to eight (eight sequences over 32000 tokens 6.2 us, with four 7.0, with two 8.2; one over 131072 8.5, 11.1 and 15.8; over 8000 tokens 256 sequences take 11.3 with
+	// four and 8.1 with two, 128 over 32000 13.4 with eight and 9.8 with four); and of eight warps, of sixteen where all of them have room at once (one over 131072 8.5, with eight 10.1; 33 over 50021 8.3 and
+	// 7.4; 64 over 131072, which have none, 16.3 with eight and 20.5 with sixteen).  Times with all rows in L2.
 	int ranks = 1;
 	while (ranks < 8 && ranks * 2048 < a.V) ranks *= 2;
 	const bool large = a.B * ranks <= 2 * sms;
