@@ -15,7 +15,7 @@ namespace paged {
 // clamp(rint(x / d) + 8, 0, 15).  What is stored does not depend on how a sum was rounded: a turned key is the fp32 number next to the turn in 64 bits, and x / d as fp32 rounds it is on the
 // same side of every n + 1/2 as the quotient itself, because d (n + 1/2) has 16 bits: where x differs from it, then by a unit of x's last place at least, and the quotient by more than half
 // a unit of its own.
-// Queries are turned in fp32 by blocks of their own.  Nine prompts of 300 to 1500 tokens, 32 and 8 heads of 128, take 60 us (173 MB, 2.9 TB/s; keys and queries by the same blocks 87, a division for each
+// Queries are turned in fp32, by blocks of their own: nothing is decided by them, 16-bit rows show none of it, and fp32 rows are off by a unit or two of their last place.  Nine prompts of 300 to 1500 tokens, 32 and 8 heads of 128, take 60 us (173 MB, 2.9 TB/s; keys and queries by the same blocks 87, a division for each
 // code 73), 16 rows 3.9.  No unit is full there (issue 55 %, ALU 38 %, DRAM 27 %): 80 registers leave three blocks to an SM, and their loads wait for the lookups in front of them.
 // =========================================================================================================================================
 struct Append4Args {
